@@ -348,6 +348,52 @@ int smoe_topk_softmax(const void* logits, int64_t slt, int64_t sle, int64_t T, i
                       float* weights_out, int64_t swt, int64_t swk, int64_t* idx_out, int64_t sit, int64_t sik,
                       int dtype, void* stream);
 
+/*
+ * A whole gated MoE layer for a few tokens, forward only, router included:
+ *   LOGITS[t,e] = sum_c X[t,c] WR[e,c]  (float32, not rounded);  experts S[t,:] = the k largest (ties: lowest id);
+ *   gates g = softmax(LOGITS[t,:])[S] (divided by their sum when `renormalize`);
+ *   OUT[t] = sum_j g[t,j] ( W2[e] glu(W1[e] X[t] + b1[e]) + b2[e] ),  e = S[t,j],  `act` as for smoe_glu_fwd.
+ * Counterpart in the reference: the router, softmax and top-k of scattermoe/utils/replace_moe.py:60-95 and
+ * GLUMLP.forward (scattermoe/mlp.py:74-95).  Sums, gates and hidden values stay in float32: OUT is the only rounding
+ * (the general path stores router logits, pre-activations, hidden and expert rows in `dtype`).
+ * Logits that are NaN or infinite: as for smoe_topk_softmax.
+ * X (T,d) strides sxm,sxk; WR (E,d) strides sre,srk; W1 (E,2F,d) strides sw1e,sw1n,sw1k; b1 (E,2F) or NULL; W2 (E,d,F)
+ * strides sw2e,sw2n,sw2k; b2 (E,d) or NULL; OUT (T,d) row stride som, columns contiguous; LOGITS (T,E) contiguous.
+ * At most SMOE_FEW_TOKENS tokens and SMOE_FEW_ROWS rows T * k, E <= 512, k <= 64: beyond that SMOE_ERR_RANGE (the caller takes
+ * the general sequence).  `workspace`: smoe_routed_glu_mlp_workspace_bytes(T, k, F) bytes, 16-byte aligned, nothing in it is
+ * read before it is written; calls that overlap in time need one each.
+ */
+#define SMOE_FEW_TOKENS 64
+#define SMOE_FEW_ROWS 512
+size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t F);
+int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR, int64_t sre, int64_t srk, const void* W1,
+                        int64_t sw1e, int64_t sw1n, int64_t sw1k, const void* b1, int64_t sb1e, int64_t sb1n,
+                        const void* W2, int64_t sw2e, int64_t sw2n, int64_t sw2k, const void* b2, int64_t sb2e,
+                        int64_t sb2n, void* OUT, int64_t som, float* LOGITS, int64_t T, int k, int64_t d, int64_t F, int E,
+                        int renormalize, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (no counterpart in the reference; rows pick their weights
+ * by id as the rows of scattermoe/parallel_experts.py:148-182 do).  Row t carries adapter ids[t]; a row whose id lies outside
+ * [0,R) carries none.
+ *   smoe_adapter_low:      U[t,j] = scales[a] sum_c X[t,c] A[a,j,c], a = ids[t]; zeros without an adapter.  float32 (T,r).
+ *   smoe_adapter_project:  Y[t,n] = sum_c X[t,c] W[n,c] (+ bias[n]) + sum_j U[t,j] B[a,n,j], rounded once.
+ *   smoe_adapter_grad:     OUT[a,j,c] = sum over the rows t of adapter a of P[t,j] M[t,c]; zeros for an adapter without rows.
+ * The backward pass is smoe_adapter_low and smoe_adapter_project on the transposed factors and smoe_adapter_grad twice.
+ * X (T,K) row stride sxm, M (T,C) row stride smm, Y (T,N) row stride sym: columns contiguous; A, B, W, OUT: any strides;
+ * scales (R) float32 or NULL (ones).  idx / off: rows ordered by adapter and inclusive offsets as smoe_route gives them
+ * (idx NULL: the rows are in order already).
+ */
+#define SMOE_ADAPTER_MAX 2047
+#define SMOE_ADAPTER_MAX_RANK 512
+int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
+                     const float* scales, float* U, int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream);
+int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
+                         const float* U, const void* B, int64_t sbr, int64_t sbn, int64_t sbj, const int64_t* ids, void* Y,
+                         int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream);
+int smoe_adapter_grad(const float* P, const void* M, int64_t smm, const int64_t* idx, const int64_t* off, void* OUT, int64_t soa,
+                      int64_t soj, int64_t soc, int64_t C, int64_t r, int64_t R, int dtype, void* stream);
+
 
 #ifdef __cplusplus
 }

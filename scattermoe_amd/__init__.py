@@ -6,6 +6,8 @@ from .parallel_experts import flatten_sort_count, flatten_and_sort, parallel_lin
 from . import parallel_experts
 from . import kernels
 from . import mlp
+from . import adapters
+from .adapters import parallel_adapters, ParallelAdapters
 
 if os.environ.get("SCATTERMOE_NO_HF_PATCH", "0") != "1":
     from . import utils
@@ -20,5 +22,8 @@ __all__ = [
     "parallel_experts",
     "kernels",
     "mlp",
+    "adapters",
+    "parallel_adapters",
+    "ParallelAdapters",
     "utils",
 ]

@@ -371,4 +371,73 @@ int smoe_topk_softmax(const void* logits, int64_t slt, int64_t sle, int64_t T, i
                              (hipStream_t)stream);
 }
 
+size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t F) {
+  if (T <= 0 || k <= 0 || F <= 0) return 0;
+  return routed_layer_workspace_bytes(T, k, F);
+}
+
+int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR, int64_t sre, int64_t srk, const void* W1,
+                        int64_t sw1e, int64_t sw1n, int64_t sw1k, const void* b1, int64_t sb1e, int64_t sb1n,
+                        const void* W2, int64_t sw2e, int64_t sw2n, int64_t sw2k, const void* b2, int64_t sb2e,
+                        int64_t sb2n, void* OUT, int64_t som, float* LOGITS, int64_t T, int k, int64_t d, int64_t F, int E,
+                        int renormalize, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  if (!dtype_ok(dtype)) { set_error("smoe_routed_glu_mlp: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (T < 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0 || k > E) { set_error("smoe_routed_glu_mlp: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (act != SMOE_ACT_SILU && act != SMOE_ACT_SILU_GATE_FIRST) { set_error("smoe_routed_glu_mlp: unknown activation %d", act); return SMOE_ERR_SHAPE; }
+  if (T > SMOE_FEW_TOKENS || T * k > SMOE_FEW_ROWS || E > 512 || k > 64 || d > 0x3fffffffLL || F > 0x3fffffffLL) {
+    set_error("smoe_routed_glu_mlp: at most %d tokens, %d (token, slot) rows, 512 experts and top-64", SMOE_FEW_TOKENS, SMOE_FEW_ROWS);
+    return SMOE_ERR_RANGE;
+  }
+  if (T == 0) return 0;
+  if (!X || !WR || !W1 || !W2 || !OUT || !LOGITS) { set_error("smoe_routed_glu_mlp: NULL pointer"); return SMOE_ERR_NULL; }
+  const size_t need = routed_layer_workspace_bytes(T, k, F);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+    set_error("smoe_routed_glu_mlp: a workspace of %zu bytes, 16-byte aligned, is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return SMOE_ERR_WORKSPACE;
+  }
+  RoutedLayerArgs a{X, sxm, sxk, WR, sre, srk, W1, sw1e, sw1n, sw1k, b1, sb1e, sb1n, W2, sw2e, sw2n, sw2k, b2, sb2e, sb2n,
+                    OUT, som, LOGITS, (int)T, k, (int)d, (int)F, E, renormalize, act};
+  return launch_routed_layer(a, workspace, dtype, (hipStream_t)stream);
+}
+
+static int adapter_checks(const char* who, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype) {
+  if (!dtype_ok(dtype)) { set_error("%s: unknown dtype %d", who, dtype); return SMOE_ERR_DTYPE; }
+  if (T < 0 || K < 0 || N < 0 || r <= 0 || R <= 0) { set_error("%s: bad sizes", who); return SMOE_ERR_SHAPE; }
+  if (T > 0x7fffffffLL || K > 0x3fffffffLL || N > 0x3fffffffLL || r > SMOE_ADAPTER_MAX_RANK || R > SMOE_ADAPTER_MAX) {
+    set_error("%s: at most 2^31 - 1 rows, 2^30 - 1 columns, rank %d and %d adapters", who, SMOE_ADAPTER_MAX_RANK, SMOE_ADAPTER_MAX);
+    return SMOE_ERR_RANGE;
+  }
+  return 0;
+}
+
+int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
+                     const float* scales, float* U, int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream) {
+  g_err[0] = 0;
+  if (int rc = adapter_checks("smoe_adapter_low", T, K, 0, r, R, dtype)) return rc;
+  if (T == 0) return 0;
+  if ((K > 0 && (!X || !A)) || !ids || !U) { set_error("smoe_adapter_low: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, U, T, (int)K, (int)r, (int)R}, dtype, (hipStream_t)stream);
+}
+
+int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
+                         const float* U, const void* B, int64_t sbr, int64_t sbn, int64_t sbj, const int64_t* ids, void* Y,
+                         int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
+  g_err[0] = 0;
+  if (int rc = adapter_checks("smoe_adapter_project", T, K, N, r, R, dtype)) return rc;
+  if (T == 0 || N == 0) return 0;
+  if ((K > 0 && (!X || !W)) || !U || !B || !ids || !Y) { set_error("smoe_adapter_project: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, B, sbr, sbn, sbj, ids, Y, sym, T, (int)K, (int)N,
+                                                   (int)r, (int)R}, dtype, (hipStream_t)stream);
+}
+
+int smoe_adapter_grad(const float* P, const void* M, int64_t smm, const int64_t* idx, const int64_t* off, void* OUT, int64_t soa,
+                      int64_t soj, int64_t soc, int64_t C, int64_t r, int64_t R, int dtype, void* stream) {
+  g_err[0] = 0;
+  if (int rc = adapter_checks("smoe_adapter_grad", 0, C, 0, r, R, dtype)) return rc;
+  if (C == 0) return 0;
+  if (!P || !M || !off || !OUT) { set_error("smoe_adapter_grad: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_adapter_grad(AdapterGradArgs{P, M, smm, idx, off, OUT, soa, soj, soc, (int)C, (int)r, (int)R}, dtype, (hipStream_t)stream);
+}
+
 }  // extern "C"

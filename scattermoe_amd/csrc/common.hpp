@@ -353,6 +353,57 @@ struct DecodeArgs {
 };
 int launch_decode_glu_mlp(const DecodeArgs& a, int dtype, hipStream_t st);
 
+// A whole gated layer for a few tokens, router included, forward only (csrc/routed_layer.hip)
+struct RoutedLayerArgs {
+  const void* X; int64_t sxm, sxk;                   // (T, d) tokens
+  const void* WR; int64_t sre, srk;                  // (E, d) router
+  const void* W1; int64_t sw1e, sw1n, sw1k;          // (E, 2F, d)
+  const void* b1; int64_t sb1e, sb1n;                // (E, 2F) or NULL
+  const void* W2; int64_t sw2e, sw2n, sw2k;          // (E, d, F)
+  const void* b2; int64_t sb2e, sb2n;                // (E, d) or NULL
+  void* OUT; int64_t som;                            // (T, d), columns contiguous
+  float* LOGITS;                                     // (T, E)
+  int T, k, d, F, E, renorm, act;
+  // in the workspace: expert and gate of row (t, j), its hidden values
+  int* experts = nullptr;
+  float* gates = nullptr;
+  float* hidden = nullptr;
+};
+size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t F);
+int launch_routed_layer(RoutedLayerArgs a, void* workspace, int dtype, hipStream_t st);
+
+// Low-rank adapters beside a shared projection (csrc/adapters.hip)
+struct AdapterLowArgs {
+  const void* X; int64_t sxm;                        // (T, K), columns contiguous
+  const void* A; int64_t sar, saj, sak;              // (R, r, K)
+  const int64_t* ids;                                // (T)
+  const float* scales;                               // (R) or NULL
+  float* U;                                          // (T, r)
+  int64_t T;
+  int K, r, R;
+};
+struct AdapterProjectArgs {
+  const void* X; int64_t sxm;                        // (T, K), columns contiguous
+  const void* W; int64_t swn, swk;                   // (N, K)
+  const void* bias; int64_t sb;                      // (N) or NULL
+  const float* U;                                    // (T, r)
+  const void* B; int64_t sbr, sbn, sbj;              // (R, N, r)
+  const int64_t* ids;                                // (T)
+  void* Y; int64_t sym;                              // (T, N), columns contiguous
+  int64_t T;
+  int K, N, r, R;
+};
+struct AdapterGradArgs {
+  const float* P;                                    // (T, r)
+  const void* M; int64_t smm;                        // (T, C), columns contiguous
+  const int64_t* idx; const int64_t* off;            // rows by adapter (NULL idx: in order), inclusive offsets (R)
+  void* OUT; int64_t soa, soj, soc;                  // (R, r, C)
+  int C, r, R;
+};
+int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st);
+int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st);
+int launch_adapter_grad(const AdapterGradArgs& a, int dtype, hipStream_t st);
+
 int launch_s2s_generic(const S2SArgs& a, int dtype, hipStream_t st);
 int launch_xty_generic(const XtYArgs& a, int dtype, hipStream_t st);
 int launch_group(const GroupArgs& a, int dtype, hipStream_t st);

@@ -307,6 +307,56 @@ class HipBackend:
                                        _C.float_code(logits.dtype), _C.stream_ptr(logits.device))
         _C.check(rc, "smoe_topk_softmax")
 
+    @staticmethod
+    def routed_glu_mlp(x, wr, w1, b1, w2, b2, out, logits, k, renormalize, act):
+        _C.require_gpu(x, "routed_glu_mlp")
+        lib = _C.load()
+        T, F, code = x.size(0), w2.size(2), _C.float_code(x.dtype)
+        sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
+        sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
+        need = lib.smoe_routed_glu_mlp_workspace_bytes(T, k, F)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        with _C.on_device(x.device):
+            rc = lib.smoe_routed_glu_mlp(
+                _C.ptr(x), x.stride(0), x.stride(1), _C.ptr(wr), wr.stride(0), wr.stride(1),
+                _C.ptr(w1), w1.stride(0), w1.stride(1), w1.stride(2), _C.ptr(b1), sb1[0], sb1[1],
+                _C.ptr(w2), w2.stride(0), w2.stride(1), w2.stride(2), _C.ptr(b2), sb2[0], sb2[1],
+                _C.ptr(out), out.stride(0), _C.ptr(logits), T, k, x.size(1), F, wr.size(0), int(bool(renormalize)), act, code,
+                _C.ptr(ws), need, _C.stream_ptr(x.device))
+        _C.check(rc, "smoe_routed_glu_mlp")
+
+    @staticmethod
+    def adapter_low(X, A, ids, scales, U):
+        _C.require_gpu(X, "adapter_low")
+        lib = _C.load()
+        with _C.on_device(X.device):
+            rc = lib.smoe_adapter_low(_C.ptr(X), X.stride(0), _C.ptr(A), A.stride(0), A.stride(1), A.stride(2), _C.ptr(ids),
+                                      _C.ptr(scales), _C.ptr(U), X.size(0), X.size(1), A.size(1), A.size(0),
+                                      _C.float_code(X.dtype), _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_adapter_low")
+
+    @staticmethod
+    def adapter_project(X, W, bias, U, B, ids, Y):
+        _C.require_gpu(X, "adapter_project")
+        lib = _C.load()
+        with _C.on_device(X.device):
+            rc = lib.smoe_adapter_project(
+                _C.ptr(X), X.stride(0), _C.ptr(W), W.stride(0), W.stride(1), _C.ptr(bias),
+                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(B), B.stride(0), B.stride(1), B.stride(2),
+                _C.ptr(ids), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0), B.size(2), B.size(0),
+                _C.float_code(X.dtype), _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_adapter_project")
+
+    @staticmethod
+    def adapter_grad(P, M, idx, off, out):
+        _C.require_gpu(M, "adapter_grad")
+        lib = _C.load()
+        with _C.on_device(M.device):
+            rc = lib.smoe_adapter_grad(_C.ptr(P), _C.ptr(M), M.stride(0), _C.ptr(idx), _C.ptr(off), _C.ptr(out),
+                                       out.stride(0), out.stride(1), out.stride(2), M.size(1), P.size(1), out.size(0),
+                                       _C.float_code(M.dtype), _C.stream_ptr(M.device))
+        _C.check(rc, "smoe_adapter_grad")
+
 
 _backend = HipBackend()
 
@@ -415,9 +465,36 @@ def _s2s_glu_bwd_op(DY: torch.Tensor, W: torch.Tensor, pre: torch.Tensor, dpre: 
         _backend.glu_bwd(pre, dh, dpre, act)
 
 
+@torch.library.custom_op("scattermoe::routed_glu_mlp", mutates_args={"out", "logits"})
+def _routed_glu_mlp_op(x: torch.Tensor, wr: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor], w2: torch.Tensor,
+                       b2: Optional[torch.Tensor], out: torch.Tensor, logits: torch.Tensor, k: int, renormalize: bool,
+                       act: int) -> None:
+    _backend.routed_glu_mlp(x, wr, w1, b1, w2, b2, out, logits, k, renormalize, act)
+
+
+@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U"})
+def _adapter_low_op(X: torch.Tensor, A: torch.Tensor, ids: torch.Tensor, scales: Optional[torch.Tensor],
+                    U: torch.Tensor) -> None:
+    _backend.adapter_low(X, A, ids, scales, U)
+
+
+@torch.library.custom_op("scattermoe::adapter_project", mutates_args={"Y"})
+def _adapter_project_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], U: torch.Tensor, B: torch.Tensor,
+                        ids: torch.Tensor, Y: torch.Tensor) -> None:
+    _backend.adapter_project(X, W, bias, U, B, ids, Y)
+
+
+@torch.library.custom_op("scattermoe::adapter_grad", mutates_args={"out"})
+def _adapter_grad_op(P: torch.Tensor, M: torch.Tensor, idx: Optional[torch.Tensor], off: torch.Tensor,
+                     out: torch.Tensor) -> None:
+    _backend.adapter_grad(P, M, idx, off, out)
+
+
 _COMPILED_OPS = {"route": _route_op, "offsets": _offsets_op, "combine": _combine_op, "gate_grad": _gate_grad_op,
                  "glu_fwd": _glu_fwd_op, "glu_bwd": _glu_bwd_op, "topk_softmax": _topk_softmax_op,
-                 "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op}
+                 "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op,
+                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_low": _adapter_low_op,
+                 "adapter_project": _adapter_project_op, "adapter_grad": _adapter_grad_op}
 
 
 def _launch(name, *args):
@@ -915,3 +992,67 @@ def decode_glu_mlp(x, expert_p, expert_idxs, w1, b1, w2, b2, act=ACT_SILU):
     if _backend.decode_glu_mlp(x, _as_i64(expert_idxs), expert_p.to(x.dtype), w1, b1, w2, b2, h, out, act):
         return out
     return None
+
+
+# ------------------------------------------------------------------------------------------------
+# a whole gated layer for a few tokens
+# ------------------------------------------------------------------------------------------------
+FEW_TOKENS, FEW_ROWS = 64, 512          # SMOE_FEW_TOKENS, SMOE_FEW_ROWS
+
+
+def few_tokens(T, k, E):
+    """Whether `routed_glu_mlp` takes T tokens of k experts out of E."""
+    return 0 < T <= FEW_TOKENS and T * k <= FEW_ROWS and E <= 512 and k <= 64
+
+
+def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=True):
+    """(out (T, d), router logits (T, E) float32) of a gated MoE layer from its tokens: router product, softmax, top-k, both
+    expert products and the gate-weighted sum, forward only (scattermoe/utils/replace_moe.py:60-95 and GLUMLP.forward,
+    mlp.py:74-95).  router_w (E, d), w1 (E, 2F, d), w2 (E, d, F) in any strides; biases (E, 2F) / (E, d) or None.  For
+    the sizes that `few_tokens` names; everything but the output stays in float32."""
+    T, d = x.shape
+    E, F = router_w.size(0), w2.size(2)
+    if not few_tokens(T, k, E):
+        raise ValueError("routed_glu_mlp: 1..%d tokens, at most %d (token, slot) rows, 512 experts and top-64" % (FEW_TOKENS, FEW_ROWS))
+    _same_dtype("routed_glu_mlp", x, router_w, w1, w2, b1, b2)
+    out = torch.empty((T, d), dtype=x.dtype, device=x.device)
+    logits = torch.empty((T, E), dtype=torch.float32, device=x.device)
+    _launch("routed_glu_mlp", x, router_w, w1, b1, w2, b2, out, logits, k, bool(renormalize), act)
+    return out, logits
+
+
+# ------------------------------------------------------------------------------------------------
+# low-rank adapters beside a shared projection
+# ------------------------------------------------------------------------------------------------
+ADAPTERS_MAX, ADAPTER_MAX_RANK = 2047, 512          # SMOE_ADAPTER_MAX, SMOE_ADAPTER_MAX_RANK
+
+
+def adapter_low(X, A, ids, scales=None):
+    """U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the rows
+    whose id lies outside [0, R)."""
+    assert A.dim() == 3 and A.size(2) == X.size(1) and ids.shape == (X.size(0),)
+    _same_dtype("adapter_low", X, A)
+    U = torch.empty((X.size(0), A.size(1)), dtype=torch.float32, device=X.device)
+    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, U)
+    return U
+
+
+def adapter_project(X, W, U, B, ids, bias=None):
+    """Y[t] = W X[t] (+ bias) + B[a] U[t], a = ids[t], for X (T, K), W (N, K), U (T, r) float32 and B (R, N, r); rows whose
+    id lies outside [0, R) get no second term."""
+    assert W.size(1) == X.size(1) and B.size(1) == W.size(0) and U.shape == (X.size(0), B.size(2)) and ids.shape == (X.size(0),)
+    _same_dtype("adapter_project", X, W, B, bias)
+    Y = torch.empty((X.size(0), W.size(0)), dtype=X.dtype, device=X.device)
+    _launch("adapter_project", _rows_contiguous(X), W, bias, U, B, ids, Y)
+    return Y
+
+
+def adapter_grad(P, M, idx, off, R, transposed=False):
+    """out[a, j, c] = sum of P[t, j] * M[t, c] over the rows t of adapter a, for P (T, r) float32 and M (T, C); the rows as
+    `route` orders them.  `transposed`: (R, C, r) instead of (R, r, C)."""
+    r, C = P.size(1), M.size(1)
+    out = torch.empty((R, C, r) if transposed else (R, r, C), dtype=M.dtype, device=M.device)
+    if P.size(0) == 0:
+        return out.zero_()
+    _launch("adapter_grad", P, _rows_contiguous(M), idx, off, out.transpose(1, 2) if transposed else out)
+    return out

@@ -160,3 +160,58 @@ class GLUMLP(_SparseMLP):
                               self.output_experts.weight.permute(0, 2, 1), self.output_experts.bias, expert_p,
                               eid, idx, off, self.top_k, ops.ACT_SILU)
         return out.view(*lead, out.size(-1))
+
+
+def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=True, gate_first=False):
+    """A gated MoE layer from its tokens: (output of x's shape, router logits (tokens, E) float32).
+
+    x (..., d); router_weight (E, d); w1 (E, 2F, d) and w2 (E, d, F) in the ParallelExperts parameter layout, biases
+    (E, 2F) / (E, d) or None, all of one type.  Every token goes to the k experts with the largest logits, weighted by its
+    softmax over all logits, divided by their sum when `renormalize`; SiLU on the second half of layer 1's columns, on the first
+    when `gate_first` (the routing of scattermoe/utils/replace_moe.py:67-71 in front of GLUMLP.forward, mlp.py:74-95).
+
+    Without autograd and for few tokens (`ops.few_tokens`) the layer is one call of the library (`ops.routed_glu_mlp`); otherwise
+    router product, `topk_softmax`, `flatten_sort_count` and the gated MLP's launches, differentiable in all float
+    arguments.  Both keep the logits in float32; the general path stores hidden and expert rows in x's type, the
+    other rounds the output only."""
+    if x.dim() < 1 or router_weight.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
+        raise ValueError("routed_glu_mlp: x (..., d), router_weight (E, d), w1 (E, 2F, d) and w2 (E, d, F)")
+    E, d = router_weight.shape
+    F = w2.size(2)
+    if x.size(-1) != d or w1.shape != (E, 2 * F, d) or w2.shape != (E, d, F) or d == 0 or F == 0:
+        raise ValueError("routed_glu_mlp: sizes of x %s, router_weight %s, w1 %s, w2 %s do not fit"
+                         % (tuple(x.shape), tuple(router_weight.shape), tuple(w1.shape), tuple(w2.shape)))
+    if (b1 is not None and b1.shape != (E, 2 * F)) or (b2 is not None and b2.shape != (E, d)):
+        raise ValueError("routed_glu_mlp: biases are (E, 2F) and (E, d)")
+    if not 0 < k <= min(E, 64) or E > 512:
+        raise ValueError("routed_glu_mlp: k must be in 1..min(num_experts, 64), and there are at most 512 experts")
+    ops._same_dtype("routed_glu_mlp", x, router_weight, w1, w2, b1, b2)
+    for t in (router_weight, w1, w2, b1, b2):
+        if t is not None and t.device != x.device:
+            raise RuntimeError("routed_glu_mlp: tensors on %s and %s" % (x.device, t.device))
+    tokens = x.reshape(-1, d)
+    T = tokens.size(0)
+    if T == 0:
+        return x.new_empty(x.shape), x.new_empty((0, E), dtype=torch.float32)
+    act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
+    if ops.few_tokens(T, k, E) and not torch.is_grad_enabled():
+        out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
+        return out.view(x.shape), logits
+    logits = nn.functional.linear(tokens.float(), router_weight.float())
+    gates, experts = ops.topk_softmax(logits, k, renormalize)
+    eid, idx, off = flatten_sort_count(experts, num_experts=E)
+    out = _GatedMLP.apply(tokens, w1.permute(0, 2, 1), b1, w2.permute(0, 2, 1), b2, gates.to(x.dtype), eid, idx, off, k, act)
+    return out.view(x.shape), logits
+
+
+class RoutedGLUMLP(GLUMLP):
+    """GLUMLP with its router: forward(x) -> (output, router logits).  State-dict keys of GLUMLP and `router.weight`."""
+
+    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, renormalize=True):
+        super().__init__(input_size, hidden_size, num_experts, top_k, bias=bias)
+        self.router = nn.Linear(input_size, num_experts, bias=False)
+        self.renormalize = renormalize
+
+    def forward(self, x: torch.Tensor):
+        return routed_glu_mlp(x, self.router.weight, self.experts.weight, self.output_experts.weight, self.top_k,
+                              b1=self.experts.bias, b2=self.output_experts.bias, renormalize=self.renormalize)
