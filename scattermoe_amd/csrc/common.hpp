@@ -368,6 +368,7 @@ struct RoutedLayerArgs {
   int* experts = nullptr;
   float* gates = nullptr;
   float* hidden = nullptr;
+  int ldh = 0;                                       // elements of a hidden row, F and padding to 16 bytes
 };
 size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t F);
 int launch_routed_layer(RoutedLayerArgs a, void* workspace, int dtype, hipStream_t st);
