@@ -360,12 +360,12 @@ int smoe_topk_softmax(const void* logits, int64_t slt, int64_t sle, int64_t T, i
  * X (T,d) strides sxm,sxk; WR (E,d) strides sre,srk; W1 (E,2F,d) strides sw1e,sw1n,sw1k; b1 (E,2F) or NULL; W2 (E,d,F)
  * strides sw2e,sw2n,sw2k; b2 (E,d) or NULL; OUT (T,d) row stride som, columns contiguous; LOGITS (T,E) contiguous.
  * At most SMOE_FEW_TOKENS tokens and SMOE_FEW_ROWS rows T * k, E <= 512, k <= 64: beyond that SMOE_ERR_RANGE (the caller takes
- * the general sequence).  `workspace`: smoe_routed_glu_mlp_workspace_bytes(T, k, F) bytes, 16-byte aligned, nothing in it is
+ * the general sequence).  `workspace`: smoe_routed_glu_mlp_workspace_bytes(T, k, d, F) bytes, 16-byte aligned, nothing in it is
  * read before it is written; calls that overlap in time need one each.
  */
 #define SMOE_FEW_TOKENS 64
 #define SMOE_FEW_ROWS 512
-size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t F);
+size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t d, int64_t F);
 int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR, int64_t sre, int64_t srk, const void* W1,
                         int64_t sw1e, int64_t sw1n, int64_t sw1k, const void* b1, int64_t sb1e, int64_t sb1n,
                         const void* W2, int64_t sw2e, int64_t sw2n, int64_t sw2k, const void* b2, int64_t sb2e,

@@ -62,7 +62,7 @@ _SIGNATURES = {
                                    _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _int, _i64, _i64,
                                    _int, _int, _int, _p]),
     "smoe_topk_softmax": (_int, [_p, _i64, _i64, _i64, _int, _int, _int, _p, _i64, _i64, _p, _i64, _i64, _int, _p]),
-    "smoe_routed_glu_mlp_workspace_bytes": (_sz, [_i64, _int, _i64]),
+    "smoe_routed_glu_mlp_workspace_bytes": (_sz, [_i64, _int, _i64, _i64]),
     "smoe_routed_glu_mlp": (_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64,
                                    _p, _i64, _i64, _p, _i64, _p, _i64, _int, _i64, _i64, _int, _int, _int, _int, _p, _sz, _p]),
     "smoe_adapter_low": (_int, [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _int, _p]),

@@ -371,9 +371,9 @@ int smoe_topk_softmax(const void* logits, int64_t slt, int64_t sle, int64_t T, i
                              (hipStream_t)stream);
 }
 
-size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t F) {
-  if (T <= 0 || k <= 0 || F <= 0) return 0;
-  return routed_layer_workspace_bytes(T, k, F);
+size_t smoe_routed_glu_mlp_workspace_bytes(int64_t T, int k, int64_t d, int64_t F) {
+  if (T <= 0 || k <= 0 || d <= 0 || F <= 0) return 0;
+  return routed_layer_workspace_bytes(T, k, d, F);
 }
 
 int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR, int64_t sre, int64_t srk, const void* W1,
@@ -391,7 +391,7 @@ int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR,
   }
   if (T == 0) return 0;
   if (!X || !WR || !W1 || !W2 || !OUT || !LOGITS) { set_error("smoe_routed_glu_mlp: NULL pointer"); return SMOE_ERR_NULL; }
-  const size_t need = routed_layer_workspace_bytes(T, k, F);
+  const size_t need = routed_layer_workspace_bytes(T, k, d, F);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
     set_error("smoe_routed_glu_mlp: a workspace of %zu bytes, 16-byte aligned, is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     return SMOE_ERR_WORKSPACE;

@@ -368,9 +368,10 @@ struct RoutedLayerArgs {
   int* experts = nullptr;
   float* gates = nullptr;
   float* hidden = nullptr;
+  float* out_rows = nullptr;                         // what row (t, j) adds to the output, (T * k, d), more than 4 tokens
   int ldh = 0;                                       // elements of a hidden row, F and padding to 16 bytes
 };
-size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t F);
+size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t d, int64_t F);
 int launch_routed_layer(RoutedLayerArgs a, void* workspace, int dtype, hipStream_t st);
 
 // Low-rank adapters beside a shared projection (csrc/adapters.hip)

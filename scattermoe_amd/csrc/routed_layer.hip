@@ -3,7 +3,7 @@
 //   S[t, :] = the k largest of l[t, :],  g[t, j] = softmax(l[t, :])[S[t, j]]  (divided by their sum when renormalised)
 //   h[t, j] = a * silu(b),  (a, b) the halves of W1[e] X[t] + b1[e],  e = S[t, j]
 //   OUT[t]  = sum_j g[t, j] (W2[e] h[t, j] + b2[e])
-// in three launches: routing (one workgroup per token), hidden rows, output.  The hidden rows, like every sum, stay in
+// in three or four launches: logits, selection (up to 4 tokens: inside the next), hidden rows, output.  The hidden rows, like every sum, stay in
 // float32; the only rounding of the layer is the output's.
 //
 // Counterpart in the reference: the router, softmax and top-k of its Hugging Face injection (scattermoe/utils/replace_moe.py:60-95)
@@ -28,67 +28,68 @@ __device__ __forceinline__ float lane_dot(const A* __restrict__ a, int64_t sa, c
   return v;
 }
 
-// ---- routing: one workgroup per token -------------------------------------------------------------------------------
-static constexpr int ROUTE_NT = 1024, ROUTE_E = 4, ROUTE_P = 2;
-// The logits of ROUTE_E experts by one wave, contiguous rows: ROUTE_P pieces of 64 x 16 bytes of each at a time
+// ---- routing --------------------------------------------------------------------------------------------------------
+// The logits of LOGIT_E experts and one token by a workgroup, whose waves take the contraction's pieces in turn.
+static constexpr int LOGIT_NW = 4, LOGIT_E = 4, LOGIT_SIDE = 2;
 template <typename T>
-__device__ __forceinline__ void route_dots(const T* __restrict__ x, const T* const (&w)[ROUTE_E], int d, float (&v)[ROUTE_E]) {
-  constexpr int PER = Few<T>::PER;
-  typedef T V __attribute__((ext_vector_type(PER)));
+__global__ __launch_bounds__(LOGIT_NW * 64) void layer_logits_kernel(RoutedLayerArgs a) {
+  __shared__ float part[LOGIT_NW][LOGIT_E];
+  const int t = blockIdx.y, e0 = blockIdx.x * LOGIT_E, wave = threadIdx.x >> 6;
+  const T* x = (const T*)a.X + t * a.sxm;
+  const T* w[LOGIT_E];
+  float v[LOGIT_E] = {};
 #pragma unroll
-  for (int j = 0; j < ROUTE_E; ++j) v[j] = 0.0f;
-  for (int k0 = lane_id() * PER; k0 < d; k0 += 64 * PER * ROUTE_P) {
-    i32x4 xv[ROUTE_P], wv[ROUTE_E][ROUTE_P];
+  for (int j = 0; j < LOGIT_E; ++j) w[j] = (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre;
+  constexpr int PER = Few<T>::PER, PIECE = 64 * PER;
+  if (a.sxk == 1 && a.srk == 1 && a.d >= PER) {
+    typedef T V __attribute__((ext_vector_type(PER)));
+    for (int k0 = threadIdx.x * PER; k0 < a.d; k0 += LOGIT_NW * PIECE * LOGIT_SIDE) {
+      i32x4 xv[LOGIT_SIDE], wv[LOGIT_E][LOGIT_SIDE];
 #pragma unroll
-    for (int p = 0; p < ROUTE_P; ++p) {
-      const int left = d - k0 - 64 * PER * p;
-      xv[p] = load_piece_of<T>(x + k0 + 64 * PER * p, left);
+      for (int p = 0; p < LOGIT_SIDE; ++p) {
+        const int k = k0 + LOGIT_NW * PIECE * p;
+        xv[p] = load_piece_of<T>(x + k, a.d - k);
 #pragma unroll
-      for (int j = 0; j < ROUTE_E; ++j) wv[j][p] = load_piece_of<T>(w[j] + k0 + 64 * PER * p, left);
+        for (int j = 0; j < LOGIT_E; ++j) wv[j][p] = load_piece_of<T>(w[j] + k, a.d - k);
+      }
+#pragma unroll
+      for (int p = 0; p < LOGIT_SIDE; ++p)
+#pragma unroll
+        for (int j = 0; j < LOGIT_E; ++j)
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            v[j] = fmaf(to_f32(__builtin_bit_cast(V, xv[p])[i]), to_f32(__builtin_bit_cast(V, wv[j][p])[i]), v[j]);
     }
+  } else {
+    for (int k = threadIdx.x; k < a.d; k += LOGIT_NW * 64)
 #pragma unroll
-    for (int p = 0; p < ROUTE_P; ++p)
-#pragma unroll
-      for (int j = 0; j < ROUTE_E; ++j)
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          v[j] = fmaf(to_f32(__builtin_bit_cast(V, xv[p])[i]), to_f32(__builtin_bit_cast(V, wv[j][p])[i]), v[j]);
+      for (int j = 0; j < LOGIT_E; ++j) v[j] = fmaf(to_f32(x[k * a.sxk]), to_f32(w[j][k * a.srk]), v[j]);
   }
 #pragma unroll
-  for (int j = 0; j < ROUTE_E; ++j) v[j] = wave_sum(v[j]);
-}
-
-template <typename T>
-__global__ __launch_bounds__(ROUTE_NT) void layer_route_kernel(RoutedLayerArgs a) {
-  __shared__ float logits[64 * ROUTER_MAX_PER_LANE];
-  const int t = blockIdx.x, wave = threadIdx.x >> 6;
-  const T* x = (const T*)a.X + t * a.sxm;
-  for (int e0 = wave * ROUTE_E; e0 < a.E; e0 += ROUTE_NT / 64 * ROUTE_E) {
-    float v[ROUTE_E];
-    if (a.sxk == 1 && a.srk == 1) {
-      const T* w[ROUTE_E];
-#pragma unroll
-      for (int j = 0; j < ROUTE_E; ++j) w[j] = (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre;
-      route_dots<T>(x, w, a.d, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < ROUTE_E; ++j)
-        v[j] = wave_sum(lane_dot(x, a.sxk, (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre, a.srk, a.d));
-    }
-#pragma unroll
-    for (int j = 0; j < ROUTE_E; ++j) {
-      if (lane_id() == 0 && e0 + j < a.E) {
-        logits[e0 + j] = v[j];
-        a.LOGITS[(int64_t)t * a.E + e0 + j] = v[j];
-      }
-    }
+  for (int j = 0; j < LOGIT_E; ++j) {
+    v[j] = wave_sum(v[j]);
+    if (lane_id() == 0) part[wave][j] = v[j];
   }
   __syncthreads();
-  if (wave != 0) return;
-  const float w = select_experts(
-      a.E, a.k, a.renorm != 0, [&](int e) { return logits[e]; }, [](float v) { return expf(v); },
-      [&](int j, int e) { a.experts[t * a.k + j] = e; });
-  if (lane_id() < a.k) a.gates[t * a.k + lane_id()] = w;
+  const int j = threadIdx.x;
+  if (j < LOGIT_E && e0 + j < a.E) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < LOGIT_NW; ++u) sum += part[u][j];
+    a.LOGITS[(int64_t)t * a.E + e0 + j] = sum;
+  }
+}
+
+// Selection of token t by one wave; `expert(j, e)` and the returned gates as select_experts
+template <class Expert>
+__device__ __forceinline__ float layer_select(const RoutedLayerArgs& a, int t, Expert expert) {
+  const float* l = a.LOGITS + (int64_t)t * a.E;
+  return select_experts(a.E, a.k, a.renorm != 0, [&](int e) { return l[e]; }, [](float v) { return expf(v); }, expert);
+}
+__global__ __launch_bounds__(64) void layer_select_kernel(RoutedLayerArgs a) {
+  const int t = blockIdx.x;
+  const float g = layer_select(a, t, [&](int j, int e) { a.experts[t * a.k + j] = e; });
+  if (lane_id() < a.k) a.gates[t * a.k + lane_id()] = g;
 }
 
 // ---- any layout: one wave per hidden value, one wave per output value ----------------------------------------------
@@ -169,78 +170,22 @@ __device__ __forceinline__ void list_rows(const int* __restrict__ experts, int L
 // Hidden values are held as two parts of the operand's type (float32: one), rows of `ldh` elements
 template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2;
 
-// Hidden rows: a workgroup of four waves has 8 NT hidden values (16 NT weight rows, each value's two next to each other) of one
-// expert's rows; the waves take the contraction's blocks in turn and are added up in LDS.
-static constexpr int HID_NW = 4, HID_NT = 2;
-template <typename T, int MT>
-__device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int f0, const int* rows, int M, float (*part)[64 * 4]) {
-  constexpr int PER = Few<T>::PER, STEP = FEW_STEP<T>, BLOCK = FEW_BLOCK<T>;
-  const int lane = lane_id(), wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const T* w[HID_NT];
-  const T* x[MT];
-#pragma unroll
-  for (int j = 0; j < HID_NT; ++j) {
-    const int f = min(f0 + 8 * j + (r >> 1), a.F - 1);
-    w[j] = (const T*)a.W1 + e * a.sw1e + (f + (r & 1 ? a.F : 0)) * a.sw1n + q * PER;
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) x[i] = (const T*)a.X + rows[min(16 * i + r, M - 1)] / a.k * a.sxm + q * PER;
-  f32x4 acc[MT][HID_NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < HID_NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int whole = a.d / BLOCK;
-  for (int b = wave; b < whole; b += HID_NW) {
-    const int k0 = b * BLOCK;
-    constexpr int SIDE = MT > 2 ? 2 : 4;
-#pragma unroll
-    for (int s0 = 0; s0 < 4; s0 += SIDE) {
-      i32x4 wv[HID_NT][SIDE], xv[MT][SIDE];
-#pragma unroll
-      for (int s = 0; s < SIDE; ++s) {
-#pragma unroll
-        for (int j = 0; j < HID_NT; ++j) wv[j][s] = load_piece<T, true>(w[j] + k0 + (s0 + s) * STEP);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) xv[i][s] = load_piece<T, false>(x[i] + k0 + (s0 + s) * STEP);
-      }
-#pragma unroll
-      for (int s = 0; s < SIDE; ++s)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < HID_NT; ++j) acc[i][j] = Few<T>::mma(wv[j][s], xv[i][s], acc[i][j]);
-    }
-  }
-  if (wave == whole % HID_NW) {
-    for (int k0 = whole * BLOCK; k0 < a.d; k0 += STEP) {
-      const int left = a.d - k0 - q * PER;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const i32x4 xv = load_piece_of<T>(x[i] + k0, left);
-#pragma unroll
-        for (int j = 0; j < HID_NT; ++j) acc[i][j] = Few<T>::mma(load_piece_of<T>(w[j] + k0, left), xv, acc[i][j]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < HID_NT; ++j) *(f32x4*)(part[(wave * MT + i) * HID_NT + j] + lane * 4) = acc[i][j];
+// Hidden rows: a workgroup of four waves has HID_ROWS weight rows (each hidden value's two next to each other) of one expert's
+// rows; the waves take the contraction's blocks in turn and are added up in LDS.
+static constexpr int HID_NW = 4, HID_ROWS = 32, MAX_GROUPS = 4, FEWEST = 4;
+static_assert(FEWEST <= HID_NW, "a wave per token");
+template <typename T, int P, int G>
+__device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int f0, const int* rows, int M, float* part) {
+  constexpr int INPUTS = G * 16 / P;
+  const T* W = (const T*)a.W1 + e * a.sw1e;
+  few_tile<T, P, G, 1, HID_NW, HID_ROWS>([&](int n) { return W + (min(f0 + (n >> 1), a.F - 1) + (n & 1 ? a.F : 0)) * a.sw1n; },
+                                         [&](int m) { return (const T*)a.X + rows[min(m, M - 1)] / a.k * a.sxm; }, 0, a.d, part);
   __syncthreads();
-  // lane (r, q) of group (i, j) held row 16 i + r, hidden values f0 + 8 j + 2 q and the next: first half, second half of each
   const T* b1 = a.b1 ? (const T*)a.b1 + e * a.sb1e : nullptr;
-  for (int p = threadIdx.x; p < MT * HID_NT * 128; p += HID_NW * 64) {
-    const int g = p >> 7, l = (p >> 1) & 63, h = p & 1;
-    const int m = 16 * (g / HID_NT) + (l & 15), f = f0 + 8 * (g % HID_NT) + 2 * (l >> 4) + h;
+  for (int p = threadIdx.x; p < HID_ROWS / 2 * INPUTS; p += HID_NW * 64) {
+    const int m = p / (HID_ROWS / 2), c = p % (HID_ROWS / 2), f = f0 + c;
     if (m >= M || f >= a.F) continue;
-    float first = 0.0f, second = 0.0f;
-#pragma unroll
-    for (int v = 0; v < HID_NW; ++v) {
-      const float* s = part[(v * MT) * HID_NT + g] + l * 4 + 2 * h;
-      first += s[0];
-      second += s[1];
-    }
+    float first = few_sum<HID_NW, HID_ROWS, INPUTS>(part, 2 * c, m), second = few_sum<HID_NW, HID_ROWS, INPUTS>(part, 2 * c + 1, m);
     T* out = (T*)a.hidden + (int64_t)rows[m] * HIDDEN_PARTS<T> * a.ldh + f;
     if (b1) {
       first += to_f32(b1[f * a.sb1n]);
@@ -252,120 +197,181 @@ __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int
   }
 }
 
-template <typename T, int MAX_MT>
+// MANY: more than 4 tokens.  Up to 4, every workgroup makes their selections for itself, a wave each, out of the logits (the
+// first one leaves them to the output's launch): a launch for that would cost more.
+template <typename T, bool MANY>
 __global__ __launch_bounds__(HID_NW * 64) void layer_hidden_kernel(RoutedLayerArgs a) {
-  __shared__ float part[HID_NW * MAX_MT * HID_NT][64 * 4];
+  __shared__ float part[FEW_PART<HID_NW, HID_ROWS, MANY ? MAX_GROUPS * 8 : 4>];
   __shared__ RowLists s;
-  list_rows<HID_NW * 64>(a.experts, a.T * a.k, a.E, s);
+  __shared__ int mine[MANY ? 1 : FEWEST * 64];
+  if constexpr (!MANY) {
+    const int t = threadIdx.x >> 6;
+    if (t < a.T) {
+      const float g = layer_select(a, t, [&](int j, int e) { mine[t * a.k + j] = e; });
+      if (blockIdx.x == 0 && blockIdx.y == 0 && lane_id() < a.k) {
+        a.gates[t * a.k + lane_id()] = g;
+        a.experts[t * a.k + lane_id()] = mine[t * a.k + lane_id()];
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (!MANY) {
+    if (a.T == 1) {                                          // (a token's experts are all different)
+      const int row = blockIdx.y;
+      hidden_tile<T, 4, 1>(a, mine[row], blockIdx.x * (HID_ROWS / 2), &row, 1, part);
+      return;
+    }
+  }
+  list_rows<HID_NW * 64>(MANY ? a.experts : mine, a.T * a.k, a.E, s);
   if ((int)blockIdx.y >= s.hits) return;
-  const int e = s.hit[blockIdx.y], f0 = blockIdx.x * 8 * HID_NT, M = s.count[e];
+  const int e = s.hit[blockIdx.y], f0 = blockIdx.x * (HID_ROWS / 2);
   const int* rows = s.rows + s.first[e];
-  if (MAX_MT == 1 || M <= 16) hidden_tile<T, 1>(a, e, f0, rows, M, part);
-  else if (M <= 32) hidden_tile<T, MAX_MT == 1 ? 1 : 2>(a, e, f0, rows, M, part);
-  else hidden_tile<T, MAX_MT>(a, e, f0, rows, M, part);
+  if constexpr (MANY) {
+    for (int M = s.count[e];;) {
+      if (M <= 8) hidden_tile<T, 2, 1>(a, e, f0, rows, M, part);
+      else if (M <= 16) hidden_tile<T, 2, 2>(a, e, f0, rows, M, part);
+      else hidden_tile<T, 2, 4>(a, e, f0, rows, min(M, 32), part);
+      if ((M -= 32) <= 0) break;
+      rows += 32;
+      __syncthreads();
+    }
+  } else {
+    hidden_tile<T, 4, 1>(a, e, f0, rows, s.count[e], part);
+  }
 }
 
-// Output: a workgroup has 16 output columns of all tokens.  The blocks of the contraction over all hit experts are dealt to
-// its waves in pieces of equal length; a wave adds what its share of an expert gives, times the gates, to sums of its
-// own per token in LDS, and the waves' sums are added up at the end in their order.
-static constexpr int OUT_NW = 16, OUT_LD = 20;
-template <typename T, int MT>
+// Output, more than 4 tokens: tiles as the hidden rows', TILE_COLS output columns of one expert's rows each, left times their gates in
+// float32; the join adds up a token's rows.  (Rows of T * k * d sums written and read are a few percent of the weights.)
+static constexpr int TILE_NW = 4, TILE_COLS = 32;
+template <typename T, int P, int G>
+__device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0, const int* rows, int M, float* part) {
+  constexpr int INPUTS = G * 16 / P, H = HIDDEN_PARTS<T>;
+  const T* W = (const T*)a.W2 + e * a.sw2e;
+  few_tile<T, P, G, H, TILE_NW, TILE_COLS>([&](int n) { return W + min(n0 + n, a.d - 1) * a.sw2n; },
+                                           [&](int m) { return (const T*)a.hidden + (int64_t)rows[min(m, M - 1)] * H * a.ldh; }, a.ldh,
+                                           a.F, part);
+  __syncthreads();
+  for (int p = threadIdx.x; p < TILE_COLS * INPUTS; p += TILE_NW * 64) {
+    const int m = p / TILE_COLS, c = p % TILE_COLS, n = n0 + c;
+    if (m >= M || n >= a.d) continue;
+    float v = few_sum<TILE_NW, TILE_COLS, INPUTS>(part, c, m);
+    if (a.b2) v += to_f32(((const T*)a.b2)[e * a.sb2e + n * a.sb2n]);
+    a.out_rows[(int64_t)rows[m] * a.d + n] = a.gates[rows[m]] * v;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(TILE_NW * 64) void layer_out_tiles_kernel(RoutedLayerArgs a) {
+  __shared__ float part[FEW_PART<TILE_NW, TILE_COLS, MAX_GROUPS * 8>];
+  __shared__ RowLists s;
+  list_rows<TILE_NW * 64>(a.experts, a.T * a.k, a.E, s);
+  if ((int)blockIdx.y >= s.hits) return;
+  const int e = s.hit[blockIdx.y], n0 = blockIdx.x * TILE_COLS;
+  const int* rows = s.rows + s.first[e];
+  for (int M = s.count[e];;) {
+    if (M <= 8) out_tile<T, 2, 1>(a, e, n0, rows, M, part);
+    else if (M <= 16) out_tile<T, 2, 2>(a, e, n0, rows, M, part);
+    else out_tile<T, 2, 4>(a, e, n0, rows, min(M, 32), part);
+    if ((M -= 32) <= 0) break;
+    rows += 32;
+    __syncthreads();
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void layer_join_kernel(RoutedLayerArgs a) {
+  const int t = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= a.d) return;
+  float v = 0.0f;
+  for (int j = 0; j < a.k; ++j) v += a.out_rows[(int64_t)(t * a.k + j) * a.d + n];
+  ((T*)a.OUT)[t * a.som + n] = from_f32<T>(v);
+}
+
+// Output, up to 4 tokens: a workgroup has OUT_COLS output columns of all tokens.  The blocks of the contraction over all hit
+// experts are dealt to its waves in pieces of equal length; a wave adds what its share of an expert gives, times the gates, to
+// sums of its own per token in LDS, and the waves' sums are added up at the end in their order.
+static constexpr int OUT_NW = 8, OUT_COLS = 16, OUT_LD = OUT_COLS + 4, OUT_BLOCK = 512;          // (bytes of a row)
+template <typename T>
 __device__ __forceinline__ void out_share(const RoutedLayerArgs& a, int e, const int* rows, int M, int n0, int b0, int b1, float* sums) {
-  constexpr int PER = Few<T>::PER, STEP = FEW_STEP<T>, BLOCK = FEW_BLOCK<T>, P = HIDDEN_PARTS<T>;
-  const int lane = lane_id(), r = lane & 15, q = lane >> 4;
-  const T* w = (const T*)a.W2 + e * a.sw2e + min(n0 + r, a.d - 1) * a.sw2n + q * PER;
-  const T* x[MT];
+  typedef FewLane<T, 4> Lane;
+  constexpr int H = HIDDEN_PARTS<T>, NT = OUT_COLS / Lane::ROWS, STEP = Lane::STEP, BLOCK = OUT_BLOCK / (int)sizeof(T), SIDE = BLOCK / STEP;
+  const Lane l;
+  const T* w[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) x[i] = (const T*)a.hidden + (int64_t)rows[min(16 * i + r, M - 1)] * P * a.ldh + q * PER;
-  f32x4 acc[MT][P];
+  for (int j = 0; j < NT; ++j) w[j] = (const T*)a.W2 + e * a.sw2e + min(n0 + j * Lane::ROWS + l.sub, a.d - 1) * a.sw2n + l.at;
+  const T* x = (const T*)a.hidden + (int64_t)rows[min(l.sub, M - 1)] * H * a.ldh + l.at;
+  f32x4 acc[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int p = 0; p < P; ++p) acc[i][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     const int k0 = b * BLOCK;
     if (k0 + BLOCK <= a.F) {
-      constexpr int SIDE = MT > 2 ? 2 : 4;
+      i32x4 wv[NT][SIDE], xv[H][SIDE];
 #pragma unroll
-      for (int s0 = 0; s0 < 4; s0 += SIDE) {
-        i32x4 wv[SIDE], xv[MT][P][SIDE];
+      for (int s = 0; s < SIDE; ++s) {
 #pragma unroll
-        for (int s = 0; s < SIDE; ++s) {
-          const int k = k0 + (s0 + s) * STEP;
-          wv[s] = load_piece<T, true>(w + k);
+        for (int j = 0; j < NT; ++j) wv[j][s] = load_piece<T, true>(w[j] + k0 + s * STEP);
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < P; ++p) xv[i][p][s] = *(const i32x4*)(x[i] + p * a.ldh + k);
-        }
-#pragma unroll
-        for (int s = 0; s < SIDE; ++s)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < P; ++p) acc[i][p] = Few<T>::mma(wv[s], xv[i][p][s], acc[i][p]);
+        for (int p = 0; p < H; ++p) xv[p][s] = *(const i32x4*)(x + p * a.ldh + k0 + s * STEP);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < SIDE; ++s)
+#pragma unroll
+        for (int p = 0; p < H; ++p)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[j] = Few<T>::mma(wv[j][s], xv[p][s], acc[j]);
     } else {
+#pragma unroll 1
       for (int k = k0; k < a.F; k += STEP) {
-        const int left = a.F - k - q * PER;
-        const i32x4 wv = load_piece_of<T>(w + k, left);
+        const int left = a.F - k - l.at;
+        i32x4 wv[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int j = 0; j < NT; ++j) wv[j] = load_piece_of<T>(w[j] + k, left);
 #pragma unroll
-          for (int p = 0; p < P; ++p) acc[i][p] = Few<T>::mma(wv, load_piece_of<T>(x[i] + p * a.ldh + k, left), acc[i][p]);
+        for (int p = 0; p < H; ++p) {
+          const i32x4 xv = load_piece_of<T>(x + p * a.ldh + k, left);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[j] = Few<T>::mma(wv[j], xv, acc[j]);
+        }
       }
     }
   }
-  // lane (r, q) holds, of row 16 i + r, columns n0 + 4 q and the next three
-  f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (a.b2 && b0 == 0) {
+  const int row = rows[min(l.sub, M - 1)];
+  const float g = a.gates[row];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (n0 + 4 * q + c < a.d) bias[c] = to_f32(((const T*)a.b2)[e * a.sb2e + (n0 + 4 * q + c) * a.sb2n]);
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = 16 * i + r;
-    if (m >= M) continue;
-    const int row = rows[m];
-    const float g = a.gates[row];
-    f32x4* to = (f32x4*)(sums + row / a.k * OUT_LD + 4 * q);
-    f32x4 v = acc[i][0];
-    if constexpr (P == 2) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = fmaf(acc[i][1][c], 1.0f / Few<T>::LOW, v[c]);
-    }
-    f32x4 old = *to;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) old[c] = fmaf(g, v[c] + bias[c], old[c]);
-    *to = old;
+  for (int j = 0; j < NT; ++j) {
+    float v[1];
+    FewSums<4>::take(acc[j], l.part, v);
+    const int n = j * Lane::ROWS + l.q;
+    if (l.part != 0 || l.sub >= M) continue;
+    if (a.b2 && b0 == 0 && n0 + n < a.d) v[0] += to_f32(((const T*)a.b2)[e * a.sb2e + (n0 + n) * a.sb2n]);
+    float* to = sums + row / a.k * OUT_LD + n;
+    *to = fmaf(g, v[0], *to);
   }
 }
 
-template <typename T, int MAX_MT>
+template <typename T>
 __global__ __launch_bounds__(OUT_NW * 64) void layer_out_kernel(RoutedLayerArgs a) {
-  __shared__ __attribute__((aligned(16))) float sums[OUT_NW][MAX_MT * 16 * OUT_LD];
+  __shared__ float sums[OUT_NW][FEWEST * OUT_LD];
   __shared__ RowLists s;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * OUT_COLS;
   for (int i = lane_id(); i < a.T * OUT_LD; i += 64) sums[wave][i] = 0.0f;
   list_rows<OUT_NW * 64>(a.experts, a.T * a.k, a.E, s);
-  const int nb = (a.F + FEW_BLOCK<T> - 1) / FEW_BLOCK<T>, total = s.hits * nb;
+  constexpr int BLOCK = OUT_BLOCK / (int)sizeof(T);
+  const int nb = (a.F + BLOCK - 1) / BLOCK, total = s.hits * nb;
   const int last = (int)((int64_t)total * (wave + 1) / OUT_NW);
   for (int u = (int)((int64_t)total * wave / OUT_NW); u < last;) {
     const int h = u / nb, b0 = u - h * nb, b1 = min(nb, b0 + last - u);
-    const int e = s.hit[h], M = s.count[e];
-    const int* rows = s.rows + s.first[e];
-    if (MAX_MT == 1 || M <= 16) out_share<T, 1>(a, e, rows, M, n0, b0, b1, sums[wave]);
-    else if (M <= 32) out_share<T, MAX_MT == 1 ? 1 : 2>(a, e, rows, M, n0, b0, b1, sums[wave]);
-    else out_share<T, MAX_MT>(a, e, rows, M, n0, b0, b1, sums[wave]);
+    const int e = s.hit[h];
+    out_share<T>(a, e, s.rows + s.first[e], s.count[e], n0, b0, b1, sums[wave]);
     u += b1 - b0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * 16; i += OUT_NW * 64) {
-    const int t = i >> 4, n = n0 + (i & 15);
+  for (int i = threadIdx.x; i < a.T * OUT_COLS; i += OUT_NW * 64) {
+    const int t = i / OUT_COLS, n = n0 + i % OUT_COLS;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < OUT_NW; ++w) v += sums[w][t * OUT_LD + (i & 15)];
+    for (int w = 0; w < OUT_NW; ++w) v += sums[w][t * OUT_LD + i % OUT_COLS];
     if (n < a.d) ((T*)a.OUT)[t * a.som + n] = from_f32<T>(v);
   }
 }
@@ -373,26 +379,38 @@ __global__ __launch_bounds__(OUT_NW * 64) void layer_out_kernel(RoutedLayerArgs 
 // The workspace: experts and gates of the T * k rows, then their hidden values, in two parts of two bytes or one of four.
 static size_t rows_bytes(int64_t L) { return (size_t)(L * 4 + 255) / 256 * 256; }
 static int64_t hidden_ld(int64_t F) { return (F + 7) / 8 * 8; }
-size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t F) {
+static int64_t hidden_bytes(int64_t L, int64_t F) { return (L * hidden_ld(F) * (int64_t)sizeof(float) + 255) / 256 * 256; }
+static bool has_out_rows(int64_t T) { return T > FEWEST; }
+size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t d, int64_t F) {
   const int64_t L = T * k;
-  return 2 * rows_bytes(L) + (size_t)L * hidden_ld(F) * sizeof(float);
+  return 2 * rows_bytes(L) + hidden_bytes(L, F) + (has_out_rows(T) ? (size_t)L * d * sizeof(float) : 0);
 }
 
-template <typename T, int MAX_MT>
+template <typename T, bool MANY>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((layer_hidden_kernel<T, MAX_MT>), dim3((a.F + 8 * HID_NT - 1) / (8 * HID_NT), std::min(a.E, a.T * a.k)),
-                     dim3(HID_NW * 64), 0, st, a);
+  const int experts = std::min(a.E, a.T * a.k);              // that can be hit
+  hipLaunchKernelGGL((layer_hidden_kernel<T, MANY>), dim3((2 * a.F + HID_ROWS - 1) / HID_ROWS, experts), dim3(HID_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_hidden_kernel")) return rc;
-  hipLaunchKernelGGL((layer_out_kernel<T, MAX_MT>), dim3((a.d + 15) / 16), dim3(OUT_NW * 64), 0, st, a);
-  return launch_status("layer_out_kernel");
+  if constexpr (!MANY) {
+    hipLaunchKernelGGL(layer_out_kernel<T>, dim3((a.d + OUT_COLS - 1) / OUT_COLS), dim3(OUT_NW * 64), 0, st, a);
+    return launch_status("layer_out_kernel");
+  } else {
+    hipLaunchKernelGGL(layer_out_tiles_kernel<T>, dim3((a.d + TILE_COLS - 1) / TILE_COLS, experts), dim3(TILE_NW * 64), 0, st, a);
+    if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
+    hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);
+    return launch_status("layer_join_kernel");
+  }
 }
 
 template <typename T>
 static int launch_t(const RoutedLayerArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(layer_route_kernel<T>, dim3(a.T), dim3(ROUTE_NT), 0, st, a);
-  if (int rc = launch_status("layer_route_kernel")) return rc;
-  if (a.sxk == 1 && a.sw1k == 1 && a.sw2k == 1)
-    return a.T <= 16 ? launch_streams<T, 1>(a, st) : launch_streams<T, 4>(a, st);
+  hipLaunchKernelGGL(layer_logits_kernel<T>, dim3((a.E + LOGIT_E - 1) / LOGIT_E, a.T), dim3(LOGIT_NW * 64), 0, st, a);
+  if (int rc = launch_status("layer_logits_kernel")) return rc;
+  const bool streams = a.sxk == 1 && a.sw1k == 1 && a.sw2k == 1 && std::min(a.d, a.F) >= Few<T>::PER;
+  if (streams && a.T <= FEWEST) return launch_streams<T, false>(a, st);
+  hipLaunchKernelGGL(layer_select_kernel, dim3(a.T), dim3(64), 0, st, a);
+  if (int rc = launch_status("layer_select_kernel")) return rc;
+  if (streams) return launch_streams<T, true>(a, st);
   hipLaunchKernelGGL(layer_hidden_any_kernel<T>, dim3((a.F + 3) / 4, a.T * a.k), dim3(256), 0, st, a);
   if (int rc = launch_status("layer_hidden_any_kernel")) return rc;
   hipLaunchKernelGGL(layer_out_any_kernel<T>, dim3((a.d + 3) / 4, a.T), dim3(256), 0, st, a);
@@ -405,6 +423,7 @@ int launch_routed_layer(RoutedLayerArgs a, void* workspace, int dtype, hipStream
   a.experts = (int*)w;
   a.gates = (float*)(w + rows_bytes(L));
   a.hidden = (float*)(w + 2 * rows_bytes(L));
+  a.out_rows = (float*)(w + 2 * rows_bytes(L) + hidden_bytes(L, a.F));
   a.ldh = (int)hidden_ld(a.F);
   switch (dtype) {
     case SMOE_F32: return launch_t<float>(a, st);

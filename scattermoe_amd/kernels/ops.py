@@ -314,7 +314,7 @@ class HipBackend:
         T, F, code = x.size(0), w2.size(2), _C.float_code(x.dtype)
         sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
         sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
-        need = lib.smoe_routed_glu_mlp_workspace_bytes(T, k, F)
+        need = lib.smoe_routed_glu_mlp_workspace_bytes(T, k, x.size(1), F)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         with _C.on_device(x.device):
             rc = lib.smoe_routed_glu_mlp(

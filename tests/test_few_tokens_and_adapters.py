@@ -198,7 +198,7 @@ def test_library_refuses_before_it_launches():
     assert layer(x=None) == -1 and layer(ws=None) == -4 and layer(ws_bytes=1000) == -4 and layer(ws=ctypes.c_void_p(264)) == -4
     assert b"workspace" in lib.smoe_last_error()
     assert layer(T=0) == 0
-    assert lib.smoe_routed_glu_mlp_workspace_bytes(0, 2, 64) == 0 and lib.smoe_routed_glu_mlp_workspace_bytes(4, 2, 64) >= 8 * 64 * 4
+    assert lib.smoe_routed_glu_mlp_workspace_bytes(0, 2, 64, 64) == 0 and lib.smoe_routed_glu_mlp_workspace_bytes(4, 2, 64, 64) >= 8 * 64 * 4
     assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 4, 64, 0, 3, 1, None) == -2
     assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 4, 64, 8, 2048, 1, None) == -5
     assert lib.smoe_adapter_low(None, 64, one, 64, 64, 1, one, None, one, 4, 64, 8, 3, 1, None) == -1
