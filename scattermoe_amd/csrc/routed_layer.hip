@@ -172,7 +172,7 @@ template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2
 
 // Hidden rows: a workgroup of four waves has HID_ROWS weight rows (each hidden value's two next to each other) of one expert's
 // rows; the waves take the contraction's blocks in turn and are added up in LDS.
-static constexpr int HID_NW = 4, HID_ROWS = 32, MAX_GROUPS = 4, FEWEST = 4;
+static constexpr int HID_NW = 4, HID_ROWS = 32, FEWEST = 4;
 static_assert(FEWEST <= HID_NW, "a wave per token");
 template <typename T, int P, int G>
 __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int f0, const int* rows, int M, float* part) {
@@ -197,11 +197,12 @@ __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int
   }
 }
 
-// MANY: more than 4 tokens.  Up to 4, every workgroup makes their selections for itself, a wave each, out of the logits (the
+// GROUPS: 0 up to 4 tokens, else groups of 8 rows that a pass over the weights takes (`row_groups`).  Up to 4, every workgroup makes their selections for itself, a wave each, out of the logits (the
 // first one leaves them to the output's launch): a launch for that would cost more.
-template <typename T, bool MANY>
-__global__ __launch_bounds__(HID_NW * 64) void layer_hidden_kernel(RoutedLayerArgs a) {
-  __shared__ float part[FEW_PART<HID_NW, HID_ROWS, MANY ? MAX_GROUPS * 8 : 4>];
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) void layer_hidden_kernel(RoutedLayerArgs a) {
+  constexpr bool MANY = GROUPS > 0;
+  __shared__ float part[FEW_PART<HID_NW, HID_ROWS, MANY ? GROUPS * 8 : 4>];
   __shared__ RowLists s;
   __shared__ int mine[MANY ? 1 : FEWEST * 64];
   if constexpr (!MANY) {
@@ -229,10 +230,10 @@ __global__ __launch_bounds__(HID_NW * 64) void layer_hidden_kernel(RoutedLayerAr
   if constexpr (MANY) {
     for (int M = s.count[e];;) {
       if (M <= 8) hidden_tile<T, 2, 1>(a, e, f0, rows, M, part);
-      else if (M <= 16) hidden_tile<T, 2, 2>(a, e, f0, rows, M, part);
-      else hidden_tile<T, 2, 4>(a, e, f0, rows, min(M, 32), part);
-      if ((M -= 32) <= 0) break;
-      rows += 32;
+      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, 2>(a, e, f0, rows, min(M, 16), part);
+      else hidden_tile<T, 2, GROUPS>(a, e, f0, rows, min(M, 8 * GROUPS), part);
+      if ((M -= 8 * GROUPS) <= 0) break;
+      rows += 8 * GROUPS;
       __syncthreads();
     }
   } else {
@@ -259,9 +260,9 @@ __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0
     a.out_rows[(int64_t)rows[m] * a.d + n] = a.gates[rows[m]] * v;
   }
 }
-template <typename T>
-__global__ __launch_bounds__(TILE_NW * 64) void layer_out_tiles_kernel(RoutedLayerArgs a) {
-  __shared__ float part[FEW_PART<TILE_NW, TILE_COLS, MAX_GROUPS * 8>];
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : 3) void layer_out_tiles_kernel(RoutedLayerArgs a) {
+  __shared__ float part[FEW_PART<TILE_NW, TILE_COLS, GROUPS * 8>];
   __shared__ RowLists s;
   list_rows<TILE_NW * 64>(a.experts, a.T * a.k, a.E, s);
   if ((int)blockIdx.y >= s.hits) return;
@@ -269,10 +270,10 @@ __global__ __launch_bounds__(TILE_NW * 64) void layer_out_tiles_kernel(RoutedLay
   const int* rows = s.rows + s.first[e];
   for (int M = s.count[e];;) {
     if (M <= 8) out_tile<T, 2, 1>(a, e, n0, rows, M, part);
-    else if (M <= 16) out_tile<T, 2, 2>(a, e, n0, rows, M, part);
-    else out_tile<T, 2, 4>(a, e, n0, rows, min(M, 32), part);
-    if ((M -= 32) <= 0) break;
-    rows += 32;
+    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, 2>(a, e, n0, rows, min(M, 16), part);
+    else out_tile<T, 2, GROUPS>(a, e, n0, rows, min(M, 8 * GROUPS), part);
+    if ((M -= 8 * GROUPS) <= 0) break;
+    rows += 8 * GROUPS;
     __syncthreads();
   }
 }
@@ -386,16 +387,16 @@ size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t d, int64_t F) {
   return 2 * rows_bytes(L) + hidden_bytes(L, F) + (has_out_rows(T) ? (size_t)L * d * sizeof(float) : 0);
 }
 
-template <typename T, bool MANY>
+template <typename T, int GROUPS>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
   const int experts = std::min(a.E, a.T * a.k);              // that can be hit
-  hipLaunchKernelGGL((layer_hidden_kernel<T, MANY>), dim3((2 * a.F + HID_ROWS - 1) / HID_ROWS, experts), dim3(HID_NW * 64), 0, st, a);
+  hipLaunchKernelGGL((layer_hidden_kernel<T, GROUPS>), dim3((2 * a.F + HID_ROWS - 1) / HID_ROWS, experts), dim3(HID_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_hidden_kernel")) return rc;
-  if constexpr (!MANY) {
+  if constexpr (GROUPS == 0) {
     hipLaunchKernelGGL(layer_out_kernel<T>, dim3((a.d + OUT_COLS - 1) / OUT_COLS), dim3(OUT_NW * 64), 0, st, a);
     return launch_status("layer_out_kernel");
   } else {
-    hipLaunchKernelGGL(layer_out_tiles_kernel<T>, dim3((a.d + TILE_COLS - 1) / TILE_COLS, experts), dim3(TILE_NW * 64), 0, st, a);
+    hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS>), dim3((a.d + TILE_COLS - 1) / TILE_COLS, experts), dim3(TILE_NW * 64), 0, st, a);
     if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
     hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);
     return launch_status("layer_join_kernel");
@@ -407,10 +408,10 @@ static int launch_t(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(layer_logits_kernel<T>, dim3((a.E + LOGIT_E - 1) / LOGIT_E, a.T), dim3(LOGIT_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_logits_kernel")) return rc;
   const bool streams = a.sxk == 1 && a.sw1k == 1 && a.sw2k == 1 && std::min(a.d, a.F) >= Few<T>::PER;
-  if (streams && a.T <= FEWEST) return launch_streams<T, false>(a, st);
+  if (streams && a.T <= FEWEST) return launch_streams<T, 0>(a, st);
   hipLaunchKernelGGL(layer_select_kernel, dim3(a.T), dim3(64), 0, st, a);
   if (int rc = launch_status("layer_select_kernel")) return rc;
-  if (streams) return launch_streams<T, true>(a, st);
+  if (streams) return a.T * a.k <= 8 * a.E ? launch_streams<T, 2>(a, st) : launch_streams<T, 4>(a, st);
   hipLaunchKernelGGL(layer_hidden_any_kernel<T>, dim3((a.F + 3) / 4, a.T * a.k), dim3(256), 0, st, a);
   if (int rc = launch_status("layer_hidden_any_kernel")) return rc;
   hipLaunchKernelGGL(layer_out_any_kernel<T>, dim3((a.d + 3) / 4, a.T), dim3(256), 0, st, a);
