@@ -17,27 +17,29 @@ class _ParallelAdapters(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, lora_a, lora_b, ids, scales):
-        u = ops.adapter_low(x, lora_a, ids, scales)
-        y = ops.adapter_project(x, weight, u, lora_b, ids, bias)
-        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scales, u)
+        order = ops.adapter_order(ids, lora_a.size(0)) if x.size(0) > ops.ADAPTER_FEW_ROWS else None
+        u, planes = ops.adapter_low(x, lora_a, ids, scales, order)
+        y = ops.adapter_project(x, weight, u, lora_b, ids, bias, planes, order)
+        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scales, u, *(order or ()))
         ctx.has_bias = bias is not None
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, lora_a, lora_b, ids, scales, u = ctx.saved_tensors
+        x, weight, lora_a, lora_b, ids, scales, u = ctx.saved_tensors[:7]
+        order = ctx.saved_tensors[7:] or None
         need_x, need_w, need_b, need_la, need_lb = ctx.needs_input_grad[:5]
         R = lora_a.size(0)
         dx = dw = db = da = dlb = None
         if not dy.is_contiguous():
             dy = dy.contiguous()
         if need_x or need_la:
-            v = ops.adapter_low(dy, lora_b.transpose(1, 2), ids, scales)
+            v, planes = ops.adapter_low(dy, lora_b.transpose(1, 2), ids, scales, order)
             if need_x:
-                dx = ops.adapter_project(dy, weight.t(), v, lora_a.transpose(1, 2), ids)
+                dx = ops.adapter_project(dy, weight.t(), v, lora_a.transpose(1, 2), ids, None, planes, order)
         if need_la or need_lb:
-            _, idx, off = ops.route(ids, R)
+            idx, off = order or ops.adapter_order(ids, R)
             if need_la:
                 da = ops.adapter_grad(v, x, idx, off, R)
             if need_lb:

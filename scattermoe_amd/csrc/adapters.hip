@@ -7,7 +7,8 @@
 //   DA[a] = sum_t V[t] X[t]^T,   DB[a] = sum_t DY[t] U[t]^T.
 //
 // The reference has no counterpart; the rows pick their weights by id as in scattermoe/parallel_experts.py:148-182.
-#include "common.hpp"
+#include "few_rows.hpp"
+#include <algorithm>
 
 namespace smoe {
 
@@ -118,20 +119,262 @@ __global__ __launch_bounds__(256) void adapter_grad_any_kernel(AdapterGradArgs a
   }
 }
 
+// ---- U, contiguous rows ------------------------------------------------------------------------------------------------
+// Few rows: DOT_ROWS values of one row by a workgroup.
+template <typename T>
+__global__ __launch_bounds__(DOT_NW * 64) void adapter_low_dots_kernel(AdapterLowArgs a) {
+  __shared__ float part[DOT_NW * DOT_ROWS];
+  const int64_t t = blockIdx.x, id = a.ids[t];
+  const int j = blockIdx.y * DOT_ROWS + threadIdx.x;
+  const bool mine = threadIdx.x < DOT_ROWS && j < a.r;
+  if ((uint64_t)id >= (uint64_t)a.R) {
+    if (mine) a.U[t * a.r + j] = 0.0f;
+    return;
+  }
+  const T* w[DOT_ROWS];
+#pragma unroll
+  for (int i = 0; i < DOT_ROWS; ++i) w[i] = (const T*)a.A + id * a.sar + std::min<int>(blockIdx.y * DOT_ROWS + i, a.r - 1) * a.saj;
+  const float v = dot_rows<T>((const T*)a.X + t * a.sxm, w, a.K, part);
+  if (mine) a.U[t * a.r + j] = v * (a.scales ? a.scales[id] : 1.0f);
+}
+
+// Many rows, ordered by adapter: 16 rows of one adapter by a workgroup, LOW_RANKS of the rank at a time.  (The rows' elements come
+// from memory once, the factor's from the caches: rows of one adapter follow one another.)
+static constexpr int LOW_NW = 8, LOW_RANKS = 16;
+template <typename T>
+__global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(AdapterLowArgs a) {
+  __shared__ float part[FEW_PART<LOW_NW, LOW_RANKS, 16>];
+  int id, row0, rows;
+  if (!find_tile<16>(a.off, a.R + 1, blockIdx.x, id, row0, rows)) return;
+  const int m_ = threadIdx.x / LOW_RANKS, n_ = threadIdx.x % LOW_RANKS;
+  for (int j0 = 0; j0 < (a.planes ? a.rp : a.r); j0 += LOW_RANKS) {
+    const bool some = id < a.R && j0 < a.r;
+    if (some)
+      few_tile<T, 2, 2, 1, LOW_NW, LOW_RANKS, false>(
+          [&](int n) { return (const T*)a.A + id * a.sar + min(j0 + n, a.r - 1) * a.saj; },
+          [&](int m) { return (const T*)a.X + a.idx[row0 + min(m, rows - 1)] * a.sxm; }, 0, a.K, part);
+    __syncthreads();
+    const int j = j0 + n_;
+    if (m_ < rows) {
+      float v = 0.0f;
+      if (some && j < a.r) v = few_sum<LOW_NW, LOW_RANKS, 16>(part, n_, m_) * (a.scales ? a.scales[id] : 1.0f);
+      const int64_t t = a.idx[row0 + m_];
+      if (j < a.r) a.U[t * a.r + j] = v;
+      if (a.planes && j < a.rp) {
+        T* p = (T*)a.planes + t * 2 * a.rp + j;
+        split<T>(v, p[0], p[a.rp]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- Y, few rows or float32: tiles of PROJ_COLS columns and 16 G / P rows, both operands from the caches or from memory ------------
+template <typename T, int P, int G, int NW, int COLS>
+__global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_kernel(AdapterProjectArgs a) {
+  constexpr int INPUTS = 16 * G / P;
+  __shared__ float part[FEW_PART<NW, COLS, INPUTS>];
+  const int n0 = blockIdx.x * COLS;
+  const int64_t t0 = (int64_t)blockIdx.y * INPUTS;
+  few_tile<T, P, G, 1, NW, COLS, false>([&](int n) { return (const T*)a.W + std::min(n0 + n, a.N - 1) * a.swn; },
+                                        [&](int m) { return (const T*)a.X + std::min<int64_t>(t0 + m, a.T - 1) * a.sxm; }, 0, a.K, part);
+  __syncthreads();
+  for (int p = threadIdx.x; p < COLS * INPUTS; p += NW * 64) {
+    const int m = p / COLS, c = p % COLS, n = n0 + c;
+    const int64_t t = t0 + m;
+    if (t >= a.T || n >= a.N) continue;
+    float v = few_sum<NW, COLS, INPUTS>(part, c, m);
+    if (a.bias) v += to_f32(((const T*)a.bias)[n * a.sb]);
+    const int64_t id = a.ids[t];
+    if ((uint64_t)id < (uint64_t)a.R) {
+      const T* b = (const T*)a.B + id * a.sbr + n * a.sbn;
+      const float* u = a.U + t * a.r;
+      int q = 0;
+      if (a.sbj == 1) {
+        constexpr int PER = Few<T>::PER;
+        typedef T V __attribute__((ext_vector_type(PER)));
+        for (; q + PER <= a.r; q += PER) {
+          const V bv = __builtin_bit_cast(V, load_piece<T, false>(b + q));
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v = fmaf(u[q + i], to_f32(bv[i]), v);
+        }
+      }
+      for (; q < a.r; ++q) v = fmaf(u[q], to_f32(b[q * a.sbj]), v);
+    }
+    ((T*)a.Y)[t * a.sym + n] = from_f32<T>(v);
+  }
+}
+
+// ---- the adapters' gradients, contiguous rows ------------------------------------------------------------------------
+// OUT[a][j][c] on float32 matrix instructions (16 x 16 x 4): P stays the float32 it is, and its rows, the contraction, need no
+// transposition, as a lane of the instruction holds one element of one row.  A lane loads 16 bytes of a row of M, and element i of
+// them is its column of product i: columns PER l + i.  A workgroup has 16 PER columns, JT x 16 of the rank and a slice of the
+// adapter's rows, which its waves take in turn, four at a time.
+static constexpr int GRAD_NW = 4;
+template <typename T, int JT>
+__global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradArgs a, int slices, float* partial) {
+  constexpr int PER = Few<T>::PER, COLS = 16 * PER;
+  typedef T V __attribute__((ext_vector_type(PER)));
+  __shared__ f32x4 part[GRAD_NW - 1][JT * PER][64];
+  const int id = blockIdx.y / slices, slice = blockIdx.y % slices, lane = lane_id(), wave = threadIdx.x >> 6;
+  const int l = lane & 15, q = lane >> 4, j0 = blockIdx.z * JT * 16;
+  const int c0 = blockIdx.x * COLS + l * PER, c = min(c0, a.C - PER);        // (the last columns: once more, by the lane before them)
+  const int64_t first = id ? a.off[id - 1] : 0, count = a.off[id] - first;
+  const int64_t lo = first + count * slice / slices, hi = first + count * (slice + 1) / slices;
+  f32x4 acc[JT][PER];
+#pragma unroll
+  for (int j = 0; j < JT; ++j)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int SIDE = 4;                                    // steps of four rows whose loads are issued side by side
+#pragma unroll 1
+  for (int64_t s = lo + wave * 4 * SIDE; s < hi; s += GRAD_NW * 4 * SIDE) {
+    V m[SIDE];
+    float p[SIDE][JT];
+#pragma unroll
+    for (int u = 0; u < SIDE; ++u) {
+      const int64_t i = s + 4 * u + q;
+      const int64_t t = i < hi ? (a.idx ? a.idx[i] : i) : -1;
+      const int64_t at = t < 0 ? (a.idx ? a.idx[lo] : lo) : t;
+      m[u] = __builtin_bit_cast(V, load_piece<T, false>((const T*)a.M + at * a.smm + c));
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        const float v = a.P[at * a.r + min(j0 + 16 * j + l, a.r - 1)];
+        p[u][j] = t < 0 ? 0.0f : v;
+      }
+      if (t < 0) m[u] = __builtin_bit_cast(V, i32x4{0, 0, 0, 0});
+    }
+#pragma unroll
+    for (int u = 0; u < SIDE; ++u)
+#pragma unroll
+      for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[u][j], to_f32(m[u][i]), acc[j][i], 0, 0, 0);
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int j = 0; j < JT; ++j)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) part[wave - 1][j * PER + i][lane] = acc[j][i];
+  }
+  __syncthreads();
+  if (wave > 0 || c0 >= a.C) return;
+  // this lane: ranks j0 + 16 j + 4 q + e, columns c + i
+#pragma unroll
+  for (int j = 0; j < JT; ++j)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      f32x4 v = acc[j][i];
+#pragma unroll
+      for (int w = 0; w < GRAD_NW - 1; ++w) v += part[w][j * PER + i][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = j0 + 16 * j + 4 * q + e;
+        if (r >= a.r) continue;
+        if (slices == 1) ((T*)a.OUT)[id * a.soa + r * a.soj + (c + i) * a.soc] = from_f32<T>(v[e]);
+        else partial[(((int64_t)slice * a.R + id) * a.r + r) * a.C + c + i] = v[e];
+      }
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_grad_join_kernel(AdapterGradArgs a, int slices, const float* partial) {
+  const int c = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, id = blockIdx.z;
+  if (c >= a.C) return;
+  float v = 0.0f;
+  for (int s = 0; s < slices; ++s) v += partial[(((int64_t)s * a.R + id) * a.r + j) * a.C + c];
+  ((T*)a.OUT)[id * a.soa + j * a.soj + c * a.soc] = from_f32<T>(v);
+}
+
+// ---- factors in another order ---------------------------------------------------------------------------------------
+// DST[a][i][0 .. ld) = SRC[a, i, 0 .. n2), zeros behind: for the products that want the contraction contiguous, whole pieces of 16 bytes
+// or rows that start at them.  With `off`, adapters without rows are left out (nobody reads them).
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs a) {
+  __shared__ T tile[64][64 + 4 / sizeof(T)];
+  const int id = blockIdx.z;
+  if (a.off && a.off[id] == (id ? a.off[id - 1] : 0)) return;
+  const int i0 = blockIdx.y * 64, k0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const T* src = (const T*)a.SRC + id * a.s0;
+  T* dst = (T*)a.DST + (int64_t)id * a.n1 * a.ld;
+  if (a.s2 == 1) {
+    for (int i = i0 + y; i < min(i0 + 64, a.n1); i += 4)
+      if (k0 + x < a.ld) dst[(int64_t)i * a.ld + k0 + x] = k0 + x < a.n2 ? src[i * a.s1 + k0 + x] : from_f32<T>(0.0f);
+    return;
+  }
+  for (int k = y; k < 64; k += 4)
+    if (i0 + x < a.n1) tile[k][x] = k0 + k < a.n2 ? src[(i0 + x) * a.s1 + (k0 + k) * a.s2] : from_f32<T>(0.0f);
+  __syncthreads();
+  for (int i = y; i < 64; i += 4)
+    if (i0 + i < a.n1 && k0 + x < a.ld) dst[(int64_t)(i0 + i) * a.ld + k0 + x] = tile[x][i];
+}
+
+// Ids of adapters as 32-bit ones of R + 1 groups: rows without an adapter are the last group
+__global__ __launch_bounds__(256) void adapter_groups_kernel(const int64_t* ids, int64_t T, int R, int* out) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t < T) out[t] = (uint64_t)ids[t] < (uint64_t)R ? (int)ids[t] : R;
+}
+
 template <typename T>
 static int low_t(const AdapterLowArgs& a, hipStream_t st) {
+  const bool pieces = a.sak == 1 && a.K >= Few<T>::PER;
+  if (pieces && a.idx != nullptr) {
+    hipLaunchKernelGGL(adapter_low_rows_kernel<T>, dim3((unsigned)max_tiles(a.T, a.R + 1, 16)), dim3(LOW_NW * 64), 0, st, a);
+    return launch_status("adapter_low_rows_kernel");
+  }
+  if (pieces) {
+    hipLaunchKernelGGL(adapter_low_dots_kernel<T>, dim3((unsigned)a.T, (a.r + DOT_ROWS - 1) / DOT_ROWS), dim3(DOT_NW * 64), 0, st, a);
+    return launch_status("adapter_low_dots_kernel");
+  }
   hipLaunchKernelGGL(adapter_low_any_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, st, a);
   return launch_status("adapter_low_any_kernel");
 }
+
+template <typename T, int P, int G, int NW, int COLS>
+static int project_rows(const AdapterProjectArgs& a, hipStream_t st) {
+  const int64_t chunks = cdiv64(a.T, 16 * G / P);
+  if (chunks > 65535) { set_error("smoe_adapter_project: too many rows for this layout"); return SMOE_ERR_RANGE; }
+  hipLaunchKernelGGL((adapter_project_rows_kernel<T, P, G, NW, COLS>), dim3((a.N + COLS - 1) / COLS, (unsigned)chunks), dim3(NW * 64), 0, st, a);
+  return launch_status("adapter_project_rows_kernel");
+}
 template <typename T>
 static int project_t(const AdapterProjectArgs& a, hipStream_t st) {
+  if (a.swk == 1 && a.K >= Few<T>::PER) {
+    if (a.T <= 4) return project_rows<T, 4, 1, 8, 16>(a, st);
+    if (a.T <= 8) return project_rows<T, 2, 1, 8, 16>(a, st);
+    if (a.T <= 16) return project_rows<T, 2, 2, 8, 16>(a, st);
+    if (a.T <= 32) return project_rows<T, 2, 4, 8, 16>(a, st);
+    return project_rows<T, 1, 4, 4, 32>(a, st);
+  }
   const int64_t rows = cdiv64(a.T, PBM);
   if (rows > 65535) { set_error("smoe_adapter_project: too many rows for this layout"); return SMOE_ERR_RANGE; }
   hipLaunchKernelGGL(adapter_project_any_kernel<T>, dim3((a.N + PBN - 1) / PBN, (unsigned)rows), dim3(PT), 0, st, a);
   return launch_status("adapter_project_any_kernel");
 }
+
+// Slices of an adapter's rows: enough workgroups for the chip, at least GRAD_MIN_ROWS rows each at even loads
+static constexpr int GRAD_WGS = 1024, GRAD_MIN_ROWS = 128, GRAD_MAX_SLICES = 32;
+static int grad_tiles(int64_t C, int dtype) { return (int)cdiv64(C, dtype == SMOE_F32 ? 64 : 128); }
+static int grad_ranks(int64_t r) { return r <= 16 ? 1 : 2; }
+static int grad_slices(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
+  const int64_t wgs = grad_tiles(C, dtype) * R * cdiv64(r, 16 * grad_ranks(r));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({GRAD_WGS / wgs, T / R / GRAD_MIN_ROWS, GRAD_MAX_SLICES, 65535 / R}));
+}
+size_t adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
+  const int slices = grad_slices(T, C, r, R, dtype);
+  return slices > 1 ? (size_t)slices * R * r * C * sizeof(float) : 0;
+}
+template <typename T, int JT>
+static int grad_ranks_t(const AdapterGradArgs& a, int slices, float* partial, hipStream_t st) {
+  hipLaunchKernelGGL((adapter_grad_kernel<T, JT>), dim3((a.C + 16 * Few<T>::PER - 1) / (16 * Few<T>::PER), a.R * slices, (a.r + 16 * JT - 1) / (16 * JT)),
+                     dim3(GRAD_NW * 64), 0, st, a, slices, partial);
+  if (int rc = launch_status("adapter_grad_kernel")) return rc;
+  if (slices == 1) return 0;
+  hipLaunchKernelGGL(adapter_grad_join_kernel<T>, dim3((a.C + 255) / 256, a.r, a.R), dim3(256), 0, st, a, slices, partial);
+  return launch_status("adapter_grad_join_kernel");
+}
 template <typename T>
-static int grad_t(const AdapterGradArgs& a, hipStream_t st) {
+static int grad_t(const AdapterGradArgs& a, int slices, float* partial, hipStream_t st) {
+  if (a.C >= Few<T>::PER) return grad_ranks(a.r) == 1 ? grad_ranks_t<T, 1>(a, slices, partial, st) : grad_ranks_t<T, 2>(a, slices, partial, st);
   hipLaunchKernelGGL(adapter_grad_any_kernel<T>, dim3((a.C + 63) / 64, a.R), dim3(256), 0, st, a);
   return launch_status("adapter_grad_any_kernel");
 }
@@ -140,10 +383,27 @@ int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st) {
   return dtype == SMOE_F32 ? low_t<float>(a, st) : dtype == SMOE_BF16 ? low_t<bf16_t>(a, st) : low_t<f16_t>(a, st);
 }
 int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st) {
+  int rc = 0;
+  if (try_adapter_tiles(a, dtype, st, rc)) return rc;
   return dtype == SMOE_F32 ? project_t<float>(a, st) : dtype == SMOE_BF16 ? project_t<bf16_t>(a, st) : project_t<f16_t>(a, st);
 }
-int launch_adapter_grad(const AdapterGradArgs& a, int dtype, hipStream_t st) {
-  return dtype == SMOE_F32 ? grad_t<float>(a, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(a, st) : grad_t<f16_t>(a, st);
+int launch_adapter_grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st) {
+  const int slices = workspace ? grad_slices(a.T, a.C, a.r, a.R, dtype) : 1;
+  float* p = (float*)workspace;
+  return dtype == SMOE_F32 ? grad_t<float>(a, slices, p, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(a, slices, p, st) : grad_t<f16_t>(a, slices, p, st);
+}
+template <typename T>
+static int pack_t(const AdapterPackArgs& a, hipStream_t st) {
+  if ((a.n1 + 63) / 64 > 65535 || a.n0 > 65535) { set_error("smoe_adapter_pack: too many rows"); return SMOE_ERR_RANGE; }
+  hipLaunchKernelGGL(adapter_pack_kernel<T>, dim3((a.ld + 63) / 64, (a.n1 + 63) / 64, a.n0), dim3(256), 0, st, a);
+  return launch_status("adapter_pack_kernel");
+}
+int launch_adapter_pack(const AdapterPackArgs& a, int dtype, hipStream_t st) {
+  return dtype == SMOE_F32 ? pack_t<float>(a, st) : dtype == SMOE_BF16 ? pack_t<bf16_t>(a, st) : pack_t<f16_t>(a, st);
+}
+int launch_adapter_groups(const int64_t* ids, int64_t T, int R, int* out, hipStream_t st) {
+  hipLaunchKernelGGL(adapter_groups_kernel, dim3((unsigned)cdiv64(T, 256)), dim3(256), 0, st, ids, T, R, out);
+  return launch_status("adapter_groups_kernel");
 }
 
 }  // namespace smoe

@@ -1,0 +1,149 @@
+// The projection beside low-rank adapters for many rows, bf16 / fp16: Y = X W^T (+ bias) + U B[a]^T in tiles of the matrix-core
+// kernels (main loops, operands and epilogues of gemm_mfma.hpp).
+//
+// The rows are taken in the order of their adapters, each adapter's padded to a whole number of 16: a fragment of 16 rows then has
+// one adapter, so its U B^T is a product of whole fragments, and what another request's adapter holds, infinities included, never meets
+// its rows.  A tile spans as many adapters as it has fragments: the shared product does not care, and no tile is cut short
+// where an adapter ends.  The accumulators start with U B^T and the main loop adds X W^T to them: one rounding.  U comes in two
+// parts of 16 bits (2^-18 of its value; one part would cost as much as the output's own rounding), operands straight from
+// global memory: for rank 16, 80 loads of 1 KB and 128 products per wave and 256 x 256 tile, against 64 slices of 128
+// products for K = 4096.
+#include "gemm_mfma.hpp"
+
+namespace smoe {
+
+struct AdapterTiles {
+  AdapterProjectArgs p;
+  Raster rast;
+};
+
+// Tile classes: 0 one wave per SIMD (long contractions of whole slices), 1 eight waves, 2 tiles of 128 x 128, two workgroups per CU
+template <int CLASS> struct AdapterTile;
+template <> struct AdapterTile<0> { typedef Tile<256, 256, 2, 2, 2, true> type; };
+template <> struct AdapterTile<1> { typedef Tile<256, 256, 2, 4> type; };
+template <> struct AdapterTile<2> { typedef Tile<128, 128, 2, 2, 2, false, 2> type; };
+
+template <typename T, int CLASS, bool W_TR>
+__global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::type::WAVES_PER_SIMD) void adapter_tiles_kernel(AdapterTiles args) {
+  typedef typename AdapterTile<CLASS>::type TL;
+  typedef DirectOp<TL::BM, TL::NT> AOp;
+  typedef typename std::conditional<W_TR, TransOp<TL::BN, TL::NT, false, false, TL::RS>, DirectOp<TL::BN, TL::NT>>::type BOp;
+  constexpr int STAGE = (TL::BM + TL::BN) * 128, FRAGS = TL::BM / 16;
+  static_assert(TL::BM * TL::BN * 2 <= TL::NS * STAGE, "staged tile must fit the operand buffers");
+  __shared__ __attribute__((aligned(16))) char lds[TL::NS * STAGE];
+  __shared__ int64_t sDst[TL::BM];
+  __shared__ int sSrc[TL::BM], sAdapter[FRAGS];
+  __shared__ __attribute__((aligned(16))) float sBias[TL::RS ? TL::BN : 4];
+  const AdapterProjectArgs& a = args.p;
+  int m_tile, n_tile, m_loc, n_loc;
+  if (!args.rast.map(blockIdx.x, m_tile, n_tile, m_loc, n_loc)) return;
+  const int n0 = n_tile * TL::BN, lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // rows of the tile's fragments; one behind the last row has adapter -1 and repeats a row that is there
+  bool any = false;
+  for (int f = wave; f < FRAGS; f += TL::NW) {
+    int id = -1, row0 = 0, rows = 0;
+    const bool has = find_tile<16>(a.off, a.R + 1, m_tile * FRAGS + f, id, row0, rows);
+    any |= has;
+    if (lane < 16) {
+      const int64_t t = has && lane < rows ? a.idx[row0 + lane] : -1;
+      sSrc[f * 16 + lane] = (int)(t >= 0 ? t : has ? a.idx[row0] : 0);
+      sDst[f * 16 + lane] = t >= 0 ? t * a.sym : -1;
+      if (lane == 0) sAdapter[f] = has && id < a.R ? id : -1;
+    }
+  }
+  if (!__syncthreads_or(any)) return;
+
+  const int wm = wave / TL::WN, wn = wave % TL::WN, lr = lane & 15, lq = lane >> 4;
+  Block acc[TL::FM][TL::FN];
+  float rs[2 * TL::FM];
+#pragma unroll
+  for (int i = 0; i < TL::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
+  for (int k0 = 0; k0 < a.rp; k0 += 32) {
+    const int k = k0 + 8 * lq;
+    const bool inside = k < a.r;                             // (r is a multiple of 8 here; U is padded with zeros to rp)
+#pragma unroll
+    for (int i = 0; i < 2 * TL::FM; ++i) {
+      const int row = wm * TL::WTM + 16 * i;
+      const int id = __builtin_amdgcn_readfirstlane(sAdapter[row >> 4]);
+      const T* u = (const T*)a.planes + (int64_t)sSrc[row + lr] * 2 * a.rp + k;
+      const i32x4 u0 = *(const i32x4*)u, u1 = *(const i32x4*)(u + a.rp);
+      const T* b = (const T*)a.B + (int64_t)max(id, 0) * a.sbr + (inside ? k : 0);
+      i32x4 bv[2 * TL::FN];
+#pragma unroll
+      for (int j = 0; j < 2 * TL::FN; ++j) {
+        bv[j] = *(const i32x4*)(b + (int64_t)min(n0 + wn * TL::WTN + 16 * j + lr, a.N - 1) * a.sbn);
+        if (!inside || id < 0) bv[j] = i32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * TL::FN; ++j) {
+        f32x4& c = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
+        c = Mfma<T>::run(bv[j], u0, c);
+        c = Mfma<T>::run(bv[j], u1, c);
+      }
+    }
+  }
+
+  AOp A;
+  A.rot = TL::RS ? 0 : (n_loc * AOp::R / Raster::SN) % AOp::R;
+  A.init((const char*)a.X, [&](int row) { return (int64_t)sSrc[row] * a.sxm * 2; });
+  BOp B;
+  B.rot = TL::RS ? 0 : (m_loc * BOp::R / Raster::SM) % BOp::R;
+  if constexpr (W_TR) B.init((const char*)a.W + (int64_t)n0 * 2, a.swk * 2, a.N - n0);
+  else B.init((const char*)a.W, [&](int row) { return (int64_t)min(n0 + row, a.N - 1) * a.swn * 2; });
+  if constexpr (TL::RS) mainloop_rs<T, TL, AOp, BOp>(A, B, a.K, lds, acc);
+  else mainloop<T, TL, AOp, BOp, false>(A, B, a.K, lds, false, acc, rs);
+
+  __syncthreads();
+  const T* bias = (const T*)a.bias;
+  if constexpr (TL::RS) {
+    stage_accumulators<T, TL>(acc, lds, [&](int tc) { return plain_bias<T>(bias, a.sb, a.N, n0 + tc); }, sBias);
+    epilogue_staged<T, TL>(acc, (T*)a.Y, sDst, n0, a.N, bias, a.sb, lds);
+  } else {
+    if (((uintptr_t)a.Y & 15) == 0 && ((a.sym | a.N) & 7) == 0) epilogue_staged<T, TL>(acc, (T*)a.Y, sDst, n0, a.N, bias, a.sb, lds);
+    else epilogue<T, TL>(acc, (T*)a.Y, sDst, n0, a.N, bias, a.sb);
+  }
+}
+
+template <typename T, int CLASS>
+static int launch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st) {
+  typedef typename AdapterTile<CLASS>::type TL;
+  const int64_t m_tiles = cdiv64(a.T + 15 * std::min<int64_t>(a.R + 1, a.T), TL::BM);
+  AdapterTiles args{a, make_raster(m_tiles, (a.N + TL::BN - 1) / TL::BN, GM_S2S)};
+  const int64_t grid = args.rast.grid();
+  if (grid > 0x7fffffffLL) { set_error("smoe_adapter_project: grid too large"); return SMOE_ERR_RANGE; }
+  if (w_tr) hipLaunchKernelGGL((adapter_tiles_kernel<T, CLASS, true>), dim3((unsigned)grid), dim3(TL::NT), 0, st, args);
+  else hipLaunchKernelGGL((adapter_tiles_kernel<T, CLASS, false>), dim3((unsigned)grid), dim3(TL::NT), 0, st, args);
+  return launch_status("adapter_tiles_kernel");
+}
+
+template <typename T>
+static int dispatch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st) {
+  const int64_t tiles = cdiv64(a.T, 256) * cdiv64(a.N, 256);
+  if (tiles < MAIN_MIN_TILES) return launch_tiles<T, 2>(a, w_tr, st);
+  const bool whole = a.K % BK == 0 && ((uintptr_t)a.Y & 15) == 0 && ((a.sym | a.N) & 7) == 0;
+  // (the descriptors of a strided operand end with its last row: rows must not overlap)
+  if (a.K >= RS_MIN_K && whole && (!w_tr || a.swk >= a.N)) return launch_tiles<T, 0>(a, w_tr, st);
+  return launch_tiles<T, 1>(a, w_tr, st);
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// Whole pieces of 16 bytes in all operands, and lane offsets of 32 bits into X and W
+bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc) {
+  if ((dtype != SMOE_BF16 && dtype != SMOE_F16) || a.planes == nullptr || a.idx == nullptr) return false;
+  if (a.K < 8 || a.K % 8 != 0 || a.sxm % 8 != 0 || !aligned16(a.X) || !aligned16(a.W)) return false;
+  if (a.r % 8 != 0 || a.sbj != 1 || a.sbn % 8 != 0 || a.sbr % 8 != 0 || !aligned16(a.B) || a.rp % 32 != 0 || !aligned16(a.planes)) return false;
+  bool w_tr;
+  if (a.swk == 1 && a.swn % 8 == 0) w_tr = false;
+  else if (a.swn == 1 && a.swk % 8 == 0 && a.N % 8 == 0) w_tr = true;
+  else return false;
+  const int64_t most = 0xffffffffLL;
+  if ((a.T - 1) * a.sxm * 2 + (int64_t)a.K * 2 > most) return false;
+  if (w_tr ? BK * a.swk * 2 + (int64_t)a.N * 2 > most : (a.N - 1) * a.swn * 2 + (int64_t)a.K * 2 > most) return false;
+  rc = dtype == SMOE_BF16 ? dispatch_tiles<bf16_t>(a, w_tr, st) : dispatch_tiles<f16_t>(a, w_tr, st);
+  return true;
+}
+
+}  // namespace smoe

@@ -411,33 +411,72 @@ static int adapter_checks(const char* who, int64_t T, int64_t K, int64_t N, int6
   return 0;
 }
 
+int smoe_adapter_groups(const int64_t* ids, int64_t T, int64_t R, int32_t* groups, void* stream) {
+  g_err[0] = 0;
+  if (int rc = adapter_checks("smoe_adapter_groups", T, 0, 0, 1, R, SMOE_F32)) return rc;
+  if (T == 0) return 0;
+  if (!ids || !groups) { set_error("smoe_adapter_groups: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_adapter_groups(ids, T, (int)R, groups, (hipStream_t)stream);
+}
+
+int smoe_adapter_pack(const void* SRC, int64_t s0, int64_t s1, int64_t s2, void* DST, int64_t n0, int64_t n1, int64_t n2,
+                      int64_t ld, const int64_t* off, int dtype, void* stream) {
+  g_err[0] = 0;
+  if (!dtype_ok(dtype)) { set_error("smoe_adapter_pack: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (n0 < 0 || n1 < 0 || n2 < 0 || ld < n2) { set_error("smoe_adapter_pack: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (n0 > 65535 || n1 > 0x3fffffLL || ld > 0x3fffffffLL) { set_error("smoe_adapter_pack: at most 65535 matrices of 2^22 - 1 rows"); return SMOE_ERR_RANGE; }
+  if (n0 == 0 || n1 == 0 || ld == 0) return 0;
+  if (!SRC || !DST) { set_error("smoe_adapter_pack: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_adapter_pack(AdapterPackArgs{SRC, s0, s1, s2, DST, (int)ld, off, (int)n0, (int)n1, (int)n2}, dtype, (hipStream_t)stream);
+}
+
 int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
-                     const float* scales, float* U, int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream) {
+                     const float* scales, const int64_t* idx, const int64_t* off, float* U, void* planes, int64_t T, int64_t K,
+                     int64_t r, int64_t R, int dtype, void* stream) {
   g_err[0] = 0;
   if (int rc = adapter_checks("smoe_adapter_low", T, K, 0, r, R, dtype)) return rc;
   if (T == 0) return 0;
   if ((K > 0 && (!X || !A)) || !ids || !U) { set_error("smoe_adapter_low: NULL pointer"); return SMOE_ERR_NULL; }
-  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, U, T, (int)K, (int)r, (int)R}, dtype, (hipStream_t)stream);
+  if (!idx != !off || (planes && (!idx || dtype == SMOE_F32 || sak != 1 || K < 8))) {
+    set_error("smoe_adapter_low: two parts need rows in order, 16-bit types and a contiguous contraction of 8 and more");
+    return SMOE_ERR_UNSUPPORTED;
+  }
+  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, idx, off, U, planes, (int)((r + 31) / 32 * 32), T, (int)K,
+                                           (int)r, (int)R}, dtype, (hipStream_t)stream);
 }
 
 int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
-                         const float* U, const void* B, int64_t sbr, int64_t sbn, int64_t sbj, const int64_t* ids, void* Y,
-                         int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
+                         const float* U, const void* planes, const void* B, int64_t sbr, int64_t sbn, int64_t sbj,
+                         const int64_t* ids, const int64_t* idx, const int64_t* off, void* Y, int64_t sym, int64_t T, int64_t K,
+                         int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
   g_err[0] = 0;
   if (int rc = adapter_checks("smoe_adapter_project", T, K, N, r, R, dtype)) return rc;
   if (T == 0 || N == 0) return 0;
   if ((K > 0 && (!X || !W)) || !U || !B || !ids || !Y) { set_error("smoe_adapter_project: NULL pointer"); return SMOE_ERR_NULL; }
-  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, B, sbr, sbn, sbj, ids, Y, sym, T, (int)K, (int)N,
-                                                   (int)r, (int)R}, dtype, (hipStream_t)stream);
+  if (!idx != !off) { set_error("smoe_adapter_project: idx and off go together"); return SMOE_ERR_NULL; }
+  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, planes, (int)((r + 31) / 32 * 32), B, sbr, sbn, sbj,
+                                                   ids, idx, off, Y, sym, T, (int)K, (int)N, (int)r, (int)R}, dtype, (hipStream_t)stream);
+}
+
+size_t smoe_adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
+  if (T <= 0 || C <= 0 || r <= 0 || R <= 0 || !dtype_ok(dtype)) return 0;
+  return adapter_grad_workspace_bytes(T, C, r, R, dtype);
 }
 
 int smoe_adapter_grad(const float* P, const void* M, int64_t smm, const int64_t* idx, const int64_t* off, void* OUT, int64_t soa,
-                      int64_t soj, int64_t soc, int64_t C, int64_t r, int64_t R, int dtype, void* stream) {
+                      int64_t soj, int64_t soc, int64_t T, int64_t C, int64_t r, int64_t R, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_grad", 0, C, 0, r, R, dtype)) return rc;
+  if (int rc = adapter_checks("smoe_adapter_grad", T, C, 0, r, R, dtype)) return rc;
   if (C == 0) return 0;
-  if (!P || !M || !off || !OUT) { set_error("smoe_adapter_grad: NULL pointer"); return SMOE_ERR_NULL; }
-  return launch_adapter_grad(AdapterGradArgs{P, M, smm, idx, off, OUT, soa, soj, soc, (int)C, (int)r, (int)R}, dtype, (hipStream_t)stream);
+  if (T == 0 || !P || !M || !off || !OUT) { set_error("smoe_adapter_grad: NULL pointer"); return SMOE_ERR_NULL; }
+  const size_t need = adapter_grad_workspace_bytes(T, C, r, R, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need)) {
+    set_error("smoe_adapter_grad: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return SMOE_ERR_WORKSPACE;
+  }
+  return launch_adapter_grad(AdapterGradArgs{P, M, smm, idx, off, OUT, soa, soj, soc, T, (int)C, (int)r, (int)R}, dtype,
+                             need ? workspace : nullptr, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -380,7 +380,9 @@ struct AdapterLowArgs {
   const void* A; int64_t sar, saj, sak;              // (R, r, K)
   const int64_t* ids;                                // (T)
   const float* scales;                               // (R) or NULL
+  const int64_t* idx; const int64_t* off;            // rows by adapter, those without one last, offsets (R + 1); or NULL
   float* U;                                          // (T, r)
+  void* planes; int rp;                              // (T, 2, rp) of the operands' type, U in two parts; or NULL
   int64_t T;
   int K, r, R;
 };
@@ -389,8 +391,10 @@ struct AdapterProjectArgs {
   const void* W; int64_t swn, swk;                   // (N, K)
   const void* bias; int64_t sb;                      // (N) or NULL
   const float* U;                                    // (T, r)
+  const void* planes; int rp;                        // as AdapterLowArgs
   const void* B; int64_t sbr, sbn, sbj;              // (R, N, r)
   const int64_t* ids;                                // (T)
+  const int64_t* idx; const int64_t* off;            // as AdapterLowArgs
   void* Y; int64_t sym;                              // (T, N), columns contiguous
   int64_t T;
   int K, N, r, R;
@@ -398,13 +402,24 @@ struct AdapterProjectArgs {
 struct AdapterGradArgs {
   const float* P;                                    // (T, r)
   const void* M; int64_t smm;                        // (T, C), columns contiguous
-  const int64_t* idx; const int64_t* off;            // rows by adapter (NULL idx: in order), inclusive offsets (R)
+  const int64_t* idx; const int64_t* off;            // rows by adapter (NULL idx: in order), inclusive offsets (R or more)
   void* OUT; int64_t soa, soj, soc;                  // (R, r, C)
+  int64_t T;
   int C, r, R;
+};
+struct AdapterPackArgs {
+  const void* SRC; int64_t s0, s1, s2;               // (n0, n1, n2)
+  void* DST; int ld;                                 // (n0, n1, ld)
+  const int64_t* off;                                // inclusive offsets (n0) or NULL
+  int n0, n1, n2;
 };
 int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st);
 int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st);
-int launch_adapter_grad(const AdapterGradArgs& a, int dtype, hipStream_t st);
+bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc);       // csrc/adapters_mfma.hip
+size_t adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype);
+int launch_adapter_grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st);
+int launch_adapter_pack(const AdapterPackArgs& a, int dtype, hipStream_t st);
+int launch_adapter_groups(const int64_t* ids, int64_t T, int R, int* out, hipStream_t st);
 
 int launch_s2s_generic(const S2SArgs& a, int dtype, hipStream_t st);
 int launch_xty_generic(const XtYArgs& a, int dtype, hipStream_t st);

@@ -62,13 +62,13 @@ template <int P>
 struct FewSums {
   static constexpr int VALUES = 4 / P;
   static __device__ __forceinline__ void take(const f32x4& acc, int part, float (&v)[VALUES]) {
-    static_assert(P == 2 || P == 4, "parts of a group of four sums");
+    static_assert(P == 1 || P == 2 || P == 4, "parts of a group of four sums");
 #pragma unroll
     for (int i = 0; i < VALUES; ++i) {
       float x = acc[i * P];
 #pragma unroll
       for (int p = 1; p < P; ++p) x = part == p ? acc[i * P + p] : x;
-      x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));                    // lane ^ 1
+      if constexpr (P > 1) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));     // lane ^ 1
       if constexpr (P == 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4e, 0xf, 0xf, true));   // lane ^ 2
       v[i] = x;
     }
@@ -115,11 +115,11 @@ static constexpr int FEW_PART = NW * WROWS * (INPUTS + 1);
 
 // Products of WROWS weight rows with G groups of 16 / P input rows over K >= PER contraction elements, by NW waves that take blocks
 // of the contraction in turn.  `weight(n)` / `input(m)`: the first element of such a row.  Inputs of H parts: `apart` elements
-// from one part of a row to the next.  Leaves the waves' sums in `part` (see few_at), without a barrier.
-template <typename T, int P, int G, int H, int NW, int WROWS, class Weight, class Input>
+// from one part of a row to the next.  ONCE: no other workgroup reads these weights.  Leaves the waves' sums in `part` (see few_at), without a barrier.
+template <typename T, int P, int G, int H, int NW, int WROWS, bool ONCE = true, class Weight, class Input>
 __device__ __forceinline__ void few_tile(Weight weight, Input input, int apart, int K, float* part) {
   typedef FewLane<T, P> Lane;
-  constexpr int NT = WROWS / Lane::ROWS, SIDE = NT * 2 <= 8 ? 8 / NT : 1, STEP = Lane::STEP, BLOCK = SIDE * STEP;
+  constexpr int NT = WROWS / Lane::ROWS, LOADS = NT + G * H, SIDE = LOADS <= 3 ? 4 : LOADS <= 6 ? 2 : 1, STEP = Lane::STEP, BLOCK = SIDE * STEP;
   constexpr int INPUTS = G * Lane::ROWS, V = FewSums<P>::VALUES;
   const Lane l;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -141,7 +141,7 @@ __device__ __forceinline__ void few_tile(Weight weight, Input input, int apart, 
 #pragma unroll
     for (int s = 0; s < SIDE; ++s) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) wv[j][s] = load_piece<T, true>(w[j] + b * BLOCK + s * STEP);
+      for (int j = 0; j < NT; ++j) wv[j][s] = load_piece<T, ONCE>(w[j] + b * BLOCK + s * STEP);
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -194,6 +194,50 @@ __device__ __forceinline__ float few_sum(const float* part, int n, int m) {
 #pragma unroll
   for (int w = 0; w < NW; ++w) v += part[few_at<WROWS, INPUTS>(w, n, m)];
   return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// The dot products of one input row with DOT_ROWS weight rows over K >= PER contiguous elements, by a workgroup of DOT_NW waves that
+// take its pieces in turn.  Thread j < DOT_ROWS returns with the j-th; `part`: DOT_NW * DOT_ROWS floats of LDS.
+static constexpr int DOT_NW = 4, DOT_ROWS = 4, DOT_SIDE = 2;
+template <typename T>
+__device__ __forceinline__ float dot_rows(const T* x, const T* const (&w)[DOT_ROWS], int K, float* part) {
+  constexpr int PER = Few<T>::PER, PIECE = 64 * PER;
+  typedef T V __attribute__((ext_vector_type(PER)));
+  float v[DOT_ROWS] = {};
+  for (int k0 = threadIdx.x * PER; k0 < K; k0 += DOT_NW * PIECE * DOT_SIDE) {
+    i32x4 xv[DOT_SIDE], wv[DOT_ROWS][DOT_SIDE];
+#pragma unroll
+    for (int p = 0; p < DOT_SIDE; ++p) {
+      const int k = k0 + DOT_NW * PIECE * p;
+      xv[p] = load_piece_of<T>(x + k, K - k);
+#pragma unroll
+      for (int j = 0; j < DOT_ROWS; ++j) wv[j][p] = load_piece_of<T>(w[j] + k, K - k);
+    }
+#pragma unroll
+    for (int p = 0; p < DOT_SIDE; ++p)
+#pragma unroll
+      for (int j = 0; j < DOT_ROWS; ++j)
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          v[j] = fmaf(to_f32(__builtin_bit_cast(V, xv[p])[i]), to_f32(__builtin_bit_cast(V, wv[j][p])[i]), v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < DOT_ROWS; ++j) {
+    v[j] = wave_sum(v[j]);
+    if (lane_id() == 0) part[(threadIdx.x >> 6) * DOT_ROWS + j] = v[j];
+  }
+  __syncthreads();
+  float sum = 0.0f;
+  if (threadIdx.x < DOT_ROWS) {
+#pragma unroll
+    for (int u = 0; u < DOT_NW; ++u) sum += part[u * DOT_ROWS + threadIdx.x];
+  }
+  return sum;
 }
 
 }  // namespace smoe

@@ -14,12 +14,6 @@
 
 namespace smoe {
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
 // This lane's share of the dot product of two strided vectors
 template <typename A, typename B>
 __device__ __forceinline__ float lane_dot(const A* __restrict__ a, int64_t sa, const B* __restrict__ b, int64_t sb, int n) {
@@ -29,54 +23,22 @@ __device__ __forceinline__ float lane_dot(const A* __restrict__ a, int64_t sa, c
 }
 
 // ---- routing --------------------------------------------------------------------------------------------------------
-// The logits of LOGIT_E experts and one token by a workgroup, whose waves take the contraction's pieces in turn.
-static constexpr int LOGIT_NW = 4, LOGIT_E = 4, LOGIT_SIDE = 2;
+// The logits of DOT_ROWS experts and one token by a workgroup
 template <typename T>
-__global__ __launch_bounds__(LOGIT_NW * 64) void layer_logits_kernel(RoutedLayerArgs a) {
-  __shared__ float part[LOGIT_NW][LOGIT_E];
-  const int t = blockIdx.y, e0 = blockIdx.x * LOGIT_E, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(DOT_NW * 64) void layer_logits_kernel(RoutedLayerArgs a) {
+  __shared__ float part[DOT_NW * DOT_ROWS];
+  const int t = blockIdx.y, e0 = blockIdx.x * DOT_ROWS;
   const T* x = (const T*)a.X + t * a.sxm;
-  const T* w[LOGIT_E];
-  float v[LOGIT_E] = {};
+  const T* w[DOT_ROWS];
 #pragma unroll
-  for (int j = 0; j < LOGIT_E; ++j) w[j] = (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre;
-  constexpr int PER = Few<T>::PER, PIECE = 64 * PER;
-  if (a.sxk == 1 && a.srk == 1 && a.d >= PER) {
-    typedef T V __attribute__((ext_vector_type(PER)));
-    for (int k0 = threadIdx.x * PER; k0 < a.d; k0 += LOGIT_NW * PIECE * LOGIT_SIDE) {
-      i32x4 xv[LOGIT_SIDE], wv[LOGIT_E][LOGIT_SIDE];
-#pragma unroll
-      for (int p = 0; p < LOGIT_SIDE; ++p) {
-        const int k = k0 + LOGIT_NW * PIECE * p;
-        xv[p] = load_piece_of<T>(x + k, a.d - k);
-#pragma unroll
-        for (int j = 0; j < LOGIT_E; ++j) wv[j][p] = load_piece_of<T>(w[j] + k, a.d - k);
-      }
-#pragma unroll
-      for (int p = 0; p < LOGIT_SIDE; ++p)
-#pragma unroll
-        for (int j = 0; j < LOGIT_E; ++j)
-#pragma unroll
-          for (int i = 0; i < PER; ++i)
-            v[j] = fmaf(to_f32(__builtin_bit_cast(V, xv[p])[i]), to_f32(__builtin_bit_cast(V, wv[j][p])[i]), v[j]);
-    }
+  for (int j = 0; j < DOT_ROWS; ++j) w[j] = (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre;
+  if (a.sxk == 1 && a.srk == 1 && a.d >= Few<T>::PER) {
+    const float v = dot_rows<T>(x, w, a.d, part);
+    if (threadIdx.x < DOT_ROWS && e0 + (int)threadIdx.x < a.E) a.LOGITS[(int64_t)t * a.E + e0 + threadIdx.x] = v;
   } else {
-    for (int k = threadIdx.x; k < a.d; k += LOGIT_NW * 64)
-#pragma unroll
-      for (int j = 0; j < LOGIT_E; ++j) v[j] = fmaf(to_f32(x[k * a.sxk]), to_f32(w[j][k * a.srk]), v[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < LOGIT_E; ++j) {
-    v[j] = wave_sum(v[j]);
-    if (lane_id() == 0) part[wave][j] = v[j];
-  }
-  __syncthreads();
-  const int j = threadIdx.x;
-  if (j < LOGIT_E && e0 + j < a.E) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < LOGIT_NW; ++u) sum += part[u][j];
-    a.LOGITS[(int64_t)t * a.E + e0 + j] = sum;
+    const int j = threadIdx.x >> 6;                          // a wave per expert
+    const float v = wave_sum(lane_dot(x, a.sxk, (const T*)a.WR + min(e0 + j, a.E - 1) * a.sre, a.srk, a.d));
+    if (lane_id() == 0 && e0 + j < a.E) a.LOGITS[(int64_t)t * a.E + e0 + j] = v;
   }
 }
 
@@ -91,6 +53,8 @@ __global__ __launch_bounds__(64) void layer_select_kernel(RoutedLayerArgs a) {
   const float g = layer_select(a, t, [&](int j, int e) { a.experts[t * a.k + j] = e; });
   if (lane_id() < a.k) a.gates[t * a.k + lane_id()] = g;
 }
+
+static_assert(DOT_NW == DOT_ROWS, "any layout: a wave per expert");
 
 // ---- any layout: one wave per hidden value, one wave per output value ----------------------------------------------
 template <typename T>
@@ -405,7 +369,7 @@ static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
 
 template <typename T>
 static int launch_t(const RoutedLayerArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(layer_logits_kernel<T>, dim3((a.E + LOGIT_E - 1) / LOGIT_E, a.T), dim3(LOGIT_NW * 64), 0, st, a);
+  hipLaunchKernelGGL(layer_logits_kernel<T>, dim3((a.E + DOT_ROWS - 1) / DOT_ROWS, a.T), dim3(DOT_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_logits_kernel")) return rc;
   const bool streams = a.sxk == 1 && a.sw1k == 1 && a.sw2k == 1 && std::min(a.d, a.F) >= Few<T>::PER;
   if (streams && a.T <= FEWEST) return launch_streams<T, 0>(a, st);

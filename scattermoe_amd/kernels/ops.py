@@ -326,35 +326,53 @@ class HipBackend:
         _C.check(rc, "smoe_routed_glu_mlp")
 
     @staticmethod
-    def adapter_low(X, A, ids, scales, U):
+    def adapter_groups(ids, R, groups):
+        _C.require_gpu(ids, "adapter_groups")
+        with _C.on_device(ids.device):
+            rc = _C.load().smoe_adapter_groups(_C.ptr(ids), ids.numel(), R, _C.ptr(groups), _C.stream_ptr(ids.device))
+        _C.check(rc, "smoe_adapter_groups")
+
+    @staticmethod
+    def adapter_pack(src, dst, off):
+        _C.require_gpu(src, "adapter_pack")
+        with _C.on_device(src.device):
+            rc = _C.load().smoe_adapter_pack(_C.ptr(src), *src.stride(), _C.ptr(dst), *src.shape, dst.size(2), _C.ptr(off),
+                                             _C.float_code(src.dtype), _C.stream_ptr(src.device))
+        _C.check(rc, "smoe_adapter_pack")
+
+    @staticmethod
+    def adapter_low(X, A, ids, scales, idx, off, U, planes):
         _C.require_gpu(X, "adapter_low")
         lib = _C.load()
         with _C.on_device(X.device):
             rc = lib.smoe_adapter_low(_C.ptr(X), X.stride(0), _C.ptr(A), A.stride(0), A.stride(1), A.stride(2), _C.ptr(ids),
-                                      _C.ptr(scales), _C.ptr(U), X.size(0), X.size(1), A.size(1), A.size(0),
-                                      _C.float_code(X.dtype), _C.stream_ptr(X.device))
+                                      _C.ptr(scales), _C.ptr(idx), _C.ptr(off), _C.ptr(U), _C.ptr(planes), X.size(0),
+                                      X.size(1), A.size(1), A.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
         _C.check(rc, "smoe_adapter_low")
 
     @staticmethod
-    def adapter_project(X, W, bias, U, B, ids, Y):
+    def adapter_project(X, W, bias, U, planes, B, ids, idx, off, Y):
         _C.require_gpu(X, "adapter_project")
         lib = _C.load()
         with _C.on_device(X.device):
             rc = lib.smoe_adapter_project(
                 _C.ptr(X), X.stride(0), _C.ptr(W), W.stride(0), W.stride(1), _C.ptr(bias),
-                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(B), B.stride(0), B.stride(1), B.stride(2),
-                _C.ptr(ids), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0), B.size(2), B.size(0),
-                _C.float_code(X.dtype), _C.stream_ptr(X.device))
+                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(planes), _C.ptr(B), B.stride(0), B.stride(1),
+                B.stride(2), _C.ptr(ids), _C.ptr(idx), _C.ptr(off), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0),
+                U.size(1), B.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
         _C.check(rc, "smoe_adapter_project")
 
     @staticmethod
     def adapter_grad(P, M, idx, off, out):
         _C.require_gpu(M, "adapter_grad")
         lib = _C.load()
+        code, T, C, r, R = _C.float_code(M.dtype), M.size(0), M.size(1), P.size(1), out.size(0)
+        need = lib.smoe_adapter_grad_workspace_bytes(T, C, r, R, code)
+        ws = torch.empty(need, dtype=torch.uint8, device=M.device) if need else None
         with _C.on_device(M.device):
             rc = lib.smoe_adapter_grad(_C.ptr(P), _C.ptr(M), M.stride(0), _C.ptr(idx), _C.ptr(off), _C.ptr(out),
-                                       out.stride(0), out.stride(1), out.stride(2), M.size(1), P.size(1), out.size(0),
-                                       _C.float_code(M.dtype), _C.stream_ptr(M.device))
+                                       out.stride(0), out.stride(1), out.stride(2), T, C, r, R, code, _C.ptr(ws), need,
+                                       _C.stream_ptr(M.device))
         _C.check(rc, "smoe_adapter_grad")
 
 
@@ -472,16 +490,28 @@ def _routed_glu_mlp_op(x: torch.Tensor, wr: torch.Tensor, w1: torch.Tensor, b1: 
     _backend.routed_glu_mlp(x, wr, w1, b1, w2, b2, out, logits, k, renormalize, act)
 
 
-@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U"})
+@torch.library.custom_op("scattermoe::adapter_groups", mutates_args={"groups"})
+def _adapter_groups_op(ids: torch.Tensor, R: int, groups: torch.Tensor) -> None:
+    _backend.adapter_groups(ids, R, groups)
+
+
+@torch.library.custom_op("scattermoe::adapter_pack", mutates_args={"dst"})
+def _adapter_pack_op(src: torch.Tensor, dst: torch.Tensor, off: Optional[torch.Tensor]) -> None:
+    _backend.adapter_pack(src, dst, off)
+
+
+@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U", "planes"})
 def _adapter_low_op(X: torch.Tensor, A: torch.Tensor, ids: torch.Tensor, scales: Optional[torch.Tensor],
-                    U: torch.Tensor) -> None:
-    _backend.adapter_low(X, A, ids, scales, U)
+                    idx: Optional[torch.Tensor], off: Optional[torch.Tensor], U: torch.Tensor,
+                    planes: Optional[torch.Tensor]) -> None:
+    _backend.adapter_low(X, A, ids, scales, idx, off, U, planes)
 
 
 @torch.library.custom_op("scattermoe::adapter_project", mutates_args={"Y"})
-def _adapter_project_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], U: torch.Tensor, B: torch.Tensor,
-                        ids: torch.Tensor, Y: torch.Tensor) -> None:
-    _backend.adapter_project(X, W, bias, U, B, ids, Y)
+def _adapter_project_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], U: torch.Tensor,
+                        planes: Optional[torch.Tensor], B: torch.Tensor, ids: torch.Tensor, idx: Optional[torch.Tensor],
+                        off: Optional[torch.Tensor], Y: torch.Tensor) -> None:
+    _backend.adapter_project(X, W, bias, U, planes, B, ids, idx, off, Y)
 
 
 @torch.library.custom_op("scattermoe::adapter_grad", mutates_args={"out"})
@@ -493,7 +523,8 @@ def _adapter_grad_op(P: torch.Tensor, M: torch.Tensor, idx: Optional[torch.Tenso
 _COMPILED_OPS = {"route": _route_op, "offsets": _offsets_op, "combine": _combine_op, "gate_grad": _gate_grad_op,
                  "glu_fwd": _glu_fwd_op, "glu_bwd": _glu_bwd_op, "topk_softmax": _topk_softmax_op,
                  "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op,
-                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_low": _adapter_low_op,
+                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_groups": _adapter_groups_op,
+                 "adapter_pack": _adapter_pack_op, "adapter_low": _adapter_low_op,
                  "adapter_project": _adapter_project_op, "adapter_grad": _adapter_grad_op}
 
 
@@ -1027,23 +1058,72 @@ def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=Tru
 ADAPTERS_MAX, ADAPTER_MAX_RANK = 2047, 512          # SMOE_ADAPTER_MAX, SMOE_ADAPTER_MAX_RANK
 
 
-def adapter_low(X, A, ids, scales=None):
-    """U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the rows
-    whose id lies outside [0, R)."""
+ADAPTER_FEW_ROWS = 64          # up to so many rows the adapters' products go row by row, without an order
+
+
+def adapter_order(ids, R):
+    """The rows by adapter, those without one last: (indices (T), inclusive offsets (R + 1)), for `adapter_low`,
+    `adapter_project` and, of whose offsets it takes the first R, `adapter_grad`."""
+    groups = torch.empty(ids.numel(), dtype=torch.int32, device=ids.device)
+    _launch("adapter_groups", ids, R, groups)
+    _, idx, off = route(groups, R + 1)
+    return idx, off
+
+
+def _adapter_pack(t, off=None, multiple=1):
+    """A copy of t (n0, n1, n2) with a contiguous last axis whose rows are a multiple of `multiple` elements (as a view of n2
+    columns), zeros behind them.  With `off`, the matrices of adapters without rows are left unwritten."""
+    n2 = t.size(2)
+    dst = torch.empty((t.size(0), t.size(1), -(-n2 // multiple) * multiple), dtype=t.dtype, device=t.device)
+    _launch("adapter_pack", t, dst, off)
+    return dst
+
+
+def _pieces(t):
+    """Whether t's rows are 16-byte pieces."""
+    return t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.size(-1) % 8 == 0 and t.data_ptr() % 16 == 0
+
+
+def adapter_low(X, A, ids, scales=None, order=None):
+    """(U, planes): U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the
+    rows whose id lies outside [0, R).  `order`: of `adapter_order`, for many rows; planes is then U in two 16-bit parts for
+    the tiles of `adapter_project`, else None."""
     assert A.dim() == 3 and A.size(2) == X.size(1) and ids.shape == (X.size(0),)
     _same_dtype("adapter_low", X, A)
-    U = torch.empty((X.size(0), A.size(1)), dtype=torch.float32, device=X.device)
-    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, U)
-    return U
+    T, K, r = X.size(0), X.size(1), A.size(1)
+    idx, off = order if order is not None else (None, None)
+    U = torch.empty((T, r), dtype=torch.float32, device=X.device)
+    planes = None
+    if order is not None and K >= 8:
+        if A.stride(2) != 1:
+            A = _adapter_pack(A, off)
+        if X.dtype != torch.float32:
+            planes = torch.empty((T, 2, -(-r // 32) * 32), dtype=X.dtype, device=X.device)
+    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, idx, off, U, planes)
+    return U, planes
 
 
-def adapter_project(X, W, U, B, ids, bias=None):
+def adapter_project(X, W, U, B, ids, bias=None, planes=None, order=None):
     """Y[t] = W X[t] (+ bias) + B[a] U[t], a = ids[t], for X (T, K), W (N, K), U (T, r) float32 and B (R, N, r); rows whose
-    id lies outside [0, R) get no second term."""
+    id lies outside [0, R) get no second term.  `planes`, `order`: of `adapter_low`, for many rows."""
     assert W.size(1) == X.size(1) and B.size(1) == W.size(0) and U.shape == (X.size(0), B.size(2)) and ids.shape == (X.size(0),)
     _same_dtype("adapter_project", X, W, B, bias)
-    Y = torch.empty((X.size(0), W.size(0)), dtype=X.dtype, device=X.device)
-    _launch("adapter_project", _rows_contiguous(X), W, bias, U, B, ids, Y)
+    T, K, N, r = X.size(0), X.size(1), W.size(0), U.size(1)
+    Y = torch.empty((T, N), dtype=X.dtype, device=X.device)
+    X = _rows_contiguous(X)
+    idx, off = order if order is not None else (None, None)
+    if planes is not None:
+        # the tiles' operands in 16-byte pieces: copies of what is not, a few percent of the product's own traffic
+        if r % 8 or not _pieces(B):
+            B = _adapter_pack(B, off, 8)
+        if not _pieces(X):
+            X = _adapter_pack(X.unsqueeze(0), None, 8)[0]
+        strided = W.stride(0) == 1 and W.stride(1) != 1
+        if not _pieces(W.t() if strided else W) or X.size(1) != K:
+            W = _adapter_pack(W.unsqueeze(0), None, 8)[0]
+    elif T > 1 and K >= 8 and W.stride(1) != 1:
+        W = _adapter_pack(W.unsqueeze(0))[0]                # row by row: a contiguous contraction
+    _launch("adapter_project", X, W, bias, U, planes, B, ids, idx, off, Y)
     return Y
 
 

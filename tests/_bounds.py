@@ -85,10 +85,10 @@ def layer(x, wr, w1, w2, k, b1=None, b2=None, renormalize=True, gate_first=False
 def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None):
     """{name: (value, bound)} of y and, with dy, of dx, da, db, dw, dbias."""
     dtype = x.dtype
-    x, w, la, lb = (t.detach().double().cpu() for t in (x, w, la, lb))
-    ids = ids.cpu().long()
+    x, w, la, lb = (t.detach().double() for t in (x, w, la, lb))
+    ids = ids.long()
     (T, K), N, (R, r) = x.shape, w.size(0), la.shape[:2]
-    s = torch.ones(R, dtype=torch.double) if scales is None else scales.detach().double().cpu()
+    s = torch.ones(R, dtype=torch.double, device=x.device) if scales is None else scales.detach().double()
     on = ((ids >= 0) & (ids < R)).double().unsqueeze(1)
     safe = ids.clamp(0, R - 1)
     A, B, sc = la[safe] * on.unsqueeze(2), lb[safe] * on.unsqueeze(2), (s[safe] * on.squeeze(1)).unsqueeze(1)
@@ -107,18 +107,18 @@ def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None):
     u, u_err = low(x, A, K)
     y, y_err = project(x, w, u, u_err, B, K)
     if bias is not None:
-        b = bias.detach().double().cpu()
+        b = bias.detach().double()
         y, y_err = y + b, y_err + U * (y.abs() + b.abs())
     found = {"y": (y, rounded(y, y_err, dtype))}
     if dy is None:
         return found
-    dy = dy.detach().double().cpu()
+    dy = dy.detach().double()
     v, v_err = low(dy, B.transpose(1, 2), N)
     dx, dx_err = project(dy, w.t(), v, v_err, A.transpose(1, 2), N)
     found["dx"] = (dx, rounded(dx, dx_err, dtype))
 
     def grad(p, p_err, m):                      # (R, r, C)
-        out, err = torch.zeros(R, r, m.size(1), dtype=torch.double), torch.zeros(R, r, m.size(1), dtype=torch.double)
+        out, err = torch.zeros(R, r, m.size(1), dtype=torch.double, device=m.device), torch.zeros(R, r, m.size(1), dtype=torch.double, device=m.device)
         for a in range(R):
             rows = (ids == a).nonzero().squeeze(1)
             out[a] = p[rows].t() @ m[rows]
@@ -135,7 +135,7 @@ def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None):
 
 
 def check(name, got, want, bound):
-    got = got.detach().double().cpu()
+    got, want, bound = got.detach().double().cpu(), want.cpu(), bound.cpu()
     assert got.shape == want.shape, "%s: shape %s, %s wanted" % (name, tuple(got.shape), tuple(want.shape))
     err = (got - want).abs()
     assert bool(torch.isfinite(got).all()), "%s: %d values are not finite" % (name, int((~torch.isfinite(got)).sum()))

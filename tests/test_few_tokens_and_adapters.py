@@ -49,21 +49,35 @@ class _Backend(OracleBackend):
         on = (ids >= 0) & (ids < factor.size(0))
         return factor[ids.clamp(0, factor.size(0) - 1)].double() * on.view(-1, 1, 1), on
 
+    @staticmethod
+    def adapter_groups(ids, R, groups):
+        groups.copy_(torch.where((ids >= 0) & (ids < R), ids, torch.full_like(ids, R)))
+
+    @staticmethod
+    def adapter_pack(src, dst, off):
+        dst.zero_()
+        dst[:, :, :src.size(2)] = src
+
     @classmethod
-    def adapter_low(cls, X, A, ids, scales, U):
+    def adapter_low(cls, X, A, ids, scales, idx, off, U, planes):
         f, _ = cls._picked(A, ids)
         s = torch.ones(A.size(0)) if scales is None else scales
         U.copy_((f @ X.double().unsqueeze(2)).squeeze(2) * s[ids.clamp(0, A.size(0) - 1)].unsqueeze(1))
+        if planes is not None:
+            planes.zero_()
+            planes[:, 0, :U.size(1)] = U.to(planes.dtype)
+            planes[:, 1, :U.size(1)] = (U - planes[:, 0, :U.size(1)].float()).to(planes.dtype)
 
     @classmethod
-    def adapter_project(cls, X, W, bias, U, B, ids, Y):
-        f, _ = cls._picked(B, ids)
-        Y.copy_(X.double() @ W.double().t() + (f @ U.double().unsqueeze(2)).squeeze(2) + (0 if bias is None else bias.double()))
+    def adapter_project(cls, X, W, bias, U, planes, B, ids, idx, off, Y):
+        f, _ = cls._picked(B[:, :, :U.size(1)], ids)
+        u = U.double() if planes is None else planes.double().sum(1)[:, :U.size(1)]
+        Y.copy_(X[:, :W.size(1)].double() @ W.double().t() + (f @ u.unsqueeze(2)).squeeze(2) + (0 if bias is None else bias.double()))
 
     @staticmethod
     def adapter_grad(P, M, idx, off, out):
         lo = 0
-        for a, hi in enumerate(off.tolist()):
+        for a, hi in enumerate(off[:out.size(0)].tolist()):
             rows = torch.arange(lo, hi) if idx is None else idx[lo:hi]
             out[a] = (P[rows].double().t() @ M[rows].double()).to(out.dtype)
             lo = hi
@@ -125,13 +139,16 @@ def test_layer_refusals():
     assert ops.few_tokens(64, 8, 128) and not ops.few_tokens(65, 1, 8) and not ops.few_tokens(64, 9, 128) and not ops.few_tokens(0, 1, 1)
 
 
-def test_adapters_values_and_gradients(backend):
+@pytest.mark.parametrize("times", [1, 10])
+def test_adapters_values_and_gradients(backend, times):
+    """Row by row, and with the rows in order."""
     torch.manual_seed(0)
     m = ParallelAdapters(3, 10, 7, 4, bias=True, scale=0.5)
     with torch.no_grad():
         for p in m.parameters():
             p.copy_(torch.randn(p.shape))
-    x, ids = torch.randn(2, 6, 10, requires_grad=True), torch.tensor([[0, 1, -1, 2, 2, 3], [1, 1, 0, 9, 2, 0]])
+    x = torch.randn(2, 6 * times, 10, requires_grad=True)
+    ids = torch.tensor([[0, 1, -1, 2, 2, 3], [1, 1, 0, 9, 2, 0]]).repeat(1, times)
     y = m(x, ids)
     flat = ids.reshape(-1)
     on = ((flat >= 0) & (flat < 3)).float()
@@ -140,11 +157,11 @@ def test_adapters_values_and_gradients(backend):
     def plain(x, w, b, la, lb):
         rows = x.reshape(-1, 10)
         low = (la[safe] @ rows.unsqueeze(2)).squeeze(2) * 0.5 * on.unsqueeze(1)
-        return (rows @ w.t() + b + (lb[safe] @ low.unsqueeze(2)).squeeze(2)).view(2, 6, 7)
+        return (rows @ w.t() + b + (lb[safe] @ low.unsqueeze(2)).squeeze(2)).view(2, 6 * times, 7)
     leaves = [x, m.weight, m.bias, m.lora_a, m.lora_b]
     want = plain(*leaves)
     torch.testing.assert_close(y, want, rtol=1e-5, atol=1e-5)
-    dy = torch.randn(2, 6, 7)
+    dy = torch.randn(2, 6 * times, 7)
     for a, b in zip(torch.autograd.grad(y, leaves, dy), torch.autograd.grad(want, leaves, dy)):
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)
 
@@ -199,11 +216,22 @@ def test_library_refuses_before_it_launches():
     assert b"workspace" in lib.smoe_last_error()
     assert layer(T=0) == 0
     assert lib.smoe_routed_glu_mlp_workspace_bytes(0, 2, 64, 64) == 0 and lib.smoe_routed_glu_mlp_workspace_bytes(4, 2, 64, 64) >= 8 * 64 * 4
-    assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 4, 64, 0, 3, 1, None) == -2
-    assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 4, 64, 8, 2048, 1, None) == -5
-    assert lib.smoe_adapter_low(None, 64, one, 64, 64, 1, one, None, one, 4, 64, 8, 3, 1, None) == -1
-    assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 0, 64, 8, 3, 1, None) == 0
-    assert lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, one, 8, 8, 1, one, one, 64, 4, 64, 64, 513, 3, 1, None) == -5
-    assert lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, one, 8, 8, 1, one, None, 64, 4, 64, 64, 8, 3, 1, None) == -1
-    assert lib.smoe_adapter_grad(one, one, 64, None, None, one, 8, 8, 1, 64, 8, 3, 1, None) == -1
-    assert lib.smoe_adapter_low(one, 64, one, 64, 64, 1, one, None, one, 0, 64, 8, 3, 1, None) == 0 and lib.smoe_last_error() == b""
+    def low(r=8, R=3, T=4, x=one, idx=None, off=None, planes=None, dtype=1, K=64):
+        return lib.smoe_adapter_low(x, 64, one, 64, 64, 1, one, None, idx, off, one, planes, T, K, r, R, dtype, None)
+    assert low(r=0) == -2 and low(R=2048) == -5 and low(r=513) == -5 and low(x=None) == -1 and low(dtype=7) == -3
+    assert low(idx=one) == -6 and low(planes=one) == -6 and low(idx=one, off=one, planes=one, dtype=0) == -6
+    assert low(idx=one, off=one, planes=one, K=7) == -6
+
+    def project(r=8, ids=one, idx=None, T=4):
+        return lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, None, one, 8, 8, 1, ids, idx, None, one, 64, T, 64, 64, r, 3, 1, None)
+    assert project(r=513) == -5 and project(ids=None) == -1 and project(idx=one) == -1 and project(T=-1) == -2
+
+    def grad(off=one, T=4, C=64, ws=None, ws_bytes=0):
+        return lib.smoe_adapter_grad(one, one, 64, None, off, one, 8, 8, 1, T, C, 8, 1, 1, ws, ws_bytes, None)
+    assert grad(off=None) == -1 and grad(T=0) == -1 and grad(T=-1) == -2
+    assert lib.smoe_adapter_grad_workspace_bytes(8192, 4096, 16, 1, 1) > 0 and lib.smoe_adapter_grad_workspace_bytes(64, 4096, 16, 1, 1) == 0
+    assert grad(T=8192, C=4096) == -4 and grad(T=8192, C=4096, ws=one, ws_bytes=64) == -4
+    assert lib.smoe_adapter_groups(None, 4, 3, one, None) == -1 and lib.smoe_adapter_groups(one, 4, 0, one, None) == -2
+    assert lib.smoe_adapter_pack(one, 64, 8, 1, one, 2, 8, 9, 8, None, 1, None) == -2
+    assert lib.smoe_adapter_pack(one, 64, 8, 1, None, 2, 8, 8, 8, None, 1, None) == -1
+    assert low(T=0) == 0 and lib.smoe_last_error() == b""

@@ -62,6 +62,14 @@ def test_values_and_gradients(T, d, n, R, r, dtype):
     _compare(i, dy)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,d,n,R,r,grouped", [(2600, 1856, 4096, 5, 8, True), (2600, 4104, 1800, 40, 24, False), (3000, 1016, 3584, 3, 40, False)])
+def test_large_tiles(T, d, n, R, r, grouped, dtype):
+    """Enough tiles of 256 x 256 for the chip: contractions of whole slices of 64 and others, forward and, transposed, backward."""
+    i, dy = _inputs(T, d, n, R, r, dtype, bias=True, grouped=grouped, seed=T + n)
+    _compare(i, dy)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [5, 64, 200])
 @pytest.mark.parametrize("which", ["none", "one", "last"])
@@ -136,7 +144,7 @@ def test_gradients_against_differences():
     _, grads = _step(i, dy)
 
     def value(s):
-        return float((_want(s)["y"][0] * dy.double().cpu()).sum())
+        return float((_want(s)["y"][0] * dy.double()).sum())
     h = 2.0 ** -10
     for name, at in (("x", (3, 5)), ("x", (69, 47)), ("weight", (7, 9)), ("lora_a", (1, 2, 30)), ("lora_b", (2, 11, 3)), ("bias", (4,))):
         pair = []
@@ -149,14 +157,18 @@ def test_gradients_against_differences():
         assert abs(float(grads[name][at]) - want) <= 1e-4 * max(1.0, abs(want)), (name, at)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [12, 300])
-def test_values_that_are_not_finite_stay_in_their_rows(T):
-    i, dy = _inputs(T, 64, 48, 4, 8, torch.float32, bare=0.0, seed=12)
+def test_values_that_are_not_finite_stay_in_their_rows(T, dtype):
+    i, dy = _inputs(T, 64, 48, 4, 8, dtype, bare=0.1, seed=12)
+    i["adapter_idxs"][:6] = torch.tensor([0, 1, 2, 3, -1, 2])
     want = parallel_adapters(**i)
     s = dict(i, x=i["x"].clone(), lora_a=i["lora_a"].clone())
     s["x"][3, 7] = float("nan")
     a = int((i["adapter_idxs"][5]))
     s["lora_a"][a, 2] = float("inf")
+    s["lora_b"] = i["lora_b"].clone()
+    s["lora_b"][a, 9] = float("nan")
     got = parallel_adapters(**s)
     keep = i["adapter_idxs"] != a
     keep[3] = False
