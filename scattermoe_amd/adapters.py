@@ -10,6 +10,16 @@ from torch import nn
 from .kernels import ops
 
 
+_ID_TYPES = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
+
+
+def _forward(x, weight, bias, lora_a, lora_b, ids, scales):
+    """(y, u, order of the rows or None)"""
+    order = ops.adapter_order(ids, lora_a.size(0)) if x.size(0) > ops.ADAPTER_FEW_ROWS else None
+    u, parts = ops.adapter_low(x, lora_a, ids, scales, order)
+    return ops.adapter_project(x, weight, u, lora_b, ids, bias, parts, order), u, order
+
+
 class _ParallelAdapters(torch.autograd.Function):
     """y = x W^T (+ bias) + u B[a]^T with u = scales[a] x A[a]^T kept in float32.  The backward pass is the same two
     products on the transposed factors, v = scales[a] dy B[a] and dx = dy W + v A[a], and the sums of v x^T and dy u^T
@@ -17,9 +27,7 @@ class _ParallelAdapters(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, lora_a, lora_b, ids, scales):
-        order = ops.adapter_order(ids, lora_a.size(0)) if x.size(0) > ops.ADAPTER_FEW_ROWS else None
-        u, planes = ops.adapter_low(x, lora_a, ids, scales, order)
-        y = ops.adapter_project(x, weight, u, lora_b, ids, bias, planes, order)
+        y, u, order = _forward(x, weight, bias, lora_a, lora_b, ids, scales)
         ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scales, u, *(order or ()))
         ctx.has_bias = bias is not None
         return y
@@ -35,9 +43,9 @@ class _ParallelAdapters(torch.autograd.Function):
         if not dy.is_contiguous():
             dy = dy.contiguous()
         if need_x or need_la:
-            v, planes = ops.adapter_low(dy, lora_b.transpose(1, 2), ids, scales, order)
+            v, parts = ops.adapter_low(dy, lora_b.transpose(1, 2), ids, scales, order)
             if need_x:
-                dx = ops.adapter_project(dy, weight.t(), v, lora_a.transpose(1, 2), ids, None, planes, order)
+                dx = ops.adapter_project(dy, weight.t(), v, lora_a.transpose(1, 2), ids, None, parts, order)
         if need_la or need_lb:
             idx, off = order or ops.adapter_order(ids, R)
             if need_la:
@@ -61,33 +69,48 @@ def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias
     same; adapter_idxs: integers of x's leading shape, and a row whose id lies outside [0, R) (-1, say) gets the shared
     projection alone; scales (R) or None (ones), a constant.  Adapters of a smaller rank are padded with zeros.  Everything but
     the output is summed and kept in float32.  Gradients go to x, weight, bias, lora_a and lora_b."""
-    if weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3 or x.dim() < 1:
+    dtype, device, shape = x.dtype, x.device, x.shape
+    tensors = (weight, lora_a, lora_b) if bias is None else (weight, lora_a, lora_b, bias)
+    if weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3 or not shape:
         raise ValueError("parallel_adapters: x (..., d), weight (n, d), lora_a (R, r, d) and lora_b (R, n, r)")
     n, d = weight.shape
-    R, r = lora_a.shape[:2]
-    if x.size(-1) != d or lora_a.size(2) != d or lora_b.shape != (R, n, r) or (bias is not None and bias.shape != (n,)):
+    R, r, _ = lora_a.shape
+    if shape[-1] != d or lora_a.size(2) != d or lora_b.shape != (R, n, r) or (bias is not None and bias.shape != (n,)):
         raise ValueError("parallel_adapters: sizes of x %s, weight %s, lora_a %s, lora_b %s%s do not fit"
-                         % (tuple(x.shape), tuple(weight.shape), tuple(lora_a.shape), tuple(lora_b.shape),
+                         % (tuple(shape), tuple(weight.shape), tuple(lora_a.shape), tuple(lora_b.shape),
                             "" if bias is None else ", bias %s" % (tuple(bias.shape),)))
     if not 0 < R <= ops.ADAPTERS_MAX or not 0 < r <= ops.ADAPTER_MAX_RANK or d == 0:
         raise ValueError("parallel_adapters: 1..%d adapters of rank 1..%d" % (ops.ADAPTERS_MAX, ops.ADAPTER_MAX_RANK))
-    if adapter_idxs.shape != x.shape[:-1]:
-        raise ValueError("parallel_adapters: adapter_idxs %s for rows %s" % (tuple(adapter_idxs.shape), tuple(x.shape[:-1])))
-    if adapter_idxs.is_floating_point() or adapter_idxs.is_complex() or adapter_idxs.dtype == torch.bool:
+    if adapter_idxs.shape != shape[:-1]:
+        raise ValueError("parallel_adapters: adapter_idxs %s for rows %s" % (tuple(adapter_idxs.shape), tuple(shape[:-1])))
+    if adapter_idxs.dtype not in _ID_TYPES:
         raise TypeError("parallel_adapters: adapter_idxs must be integers, got %s" % adapter_idxs.dtype)
-    ops._same_dtype("parallel_adapters", x, weight, lora_a, lora_b, bias)
-    for t in (weight, lora_a, lora_b, adapter_idxs, scales, bias):
-        if t is not None and t.device != x.device:
-            raise RuntimeError("parallel_adapters: tensors on %s and %s" % (x.device, t.device))
+    if adapter_idxs.device != device or (scales is not None and scales.device != device):
+        raise RuntimeError("parallel_adapters: all tensors on the device of x (%s)" % device)
+    trained = x.requires_grad
+    for t in tensors:
+        if t.dtype != dtype:
+            raise TypeError("parallel_adapters: dtype mismatch (%s vs %s)" % (dtype, t.dtype))
+        if t.device != device:
+            raise RuntimeError("parallel_adapters: all tensors on the device of x (%s)" % device)
+        trained = trained or t.requires_grad
     if scales is not None:
         if scales.shape != (R,):
             raise ValueError("parallel_adapters: scales %s for %d adapters" % (tuple(scales.shape), R))
         if scales.requires_grad:
             raise ValueError("parallel_adapters: scales are constants (no gradient goes to them)")
-        scales = scales.to(torch.float32).contiguous()
-    ids = ops._as_i64(adapter_idxs.reshape(-1)).contiguous()
-    y = _ParallelAdapters.apply(x.reshape(-1, d), weight, bias, lora_a, lora_b, ids, scales)
-    return y.view(*x.shape[:-1], n)
+        if scales.dtype != torch.float32 or not scales.is_contiguous():
+            scales = scales.to(torch.float32).contiguous()
+    ids = adapter_idxs
+    if len(shape) != 2:
+        x, ids = x.reshape(-1, d), ids.reshape(-1)
+    if ids.dtype != torch.int64 or not ids.is_contiguous():
+        ids = ids.to(torch.int64).contiguous()
+    if trained and torch.is_grad_enabled():
+        y = _ParallelAdapters.apply(x, weight, bias, lora_a, lora_b, ids, scales)
+    else:
+        y = _forward(x, weight, bias, lora_a, lora_b, ids, scales)[0]
+    return y if len(shape) == 2 else y.view(*shape[:-1], n)
 
 
 class ParallelAdapters(nn.Module):

@@ -138,34 +138,36 @@ __global__ __launch_bounds__(DOT_NW * 64) void adapter_low_dots_kernel(AdapterLo
   if (mine) a.U[t * a.r + j] = v * (a.scales ? a.scales[id] : 1.0f);
 }
 
-// Many rows, ordered by adapter: 16 rows of one adapter by a workgroup, LOW_RANKS of the rank at a time.  (The rows' elements come
+// Many rows, ordered by adapter: 16 rows of one adapter and LOW_RANKS of the rank by a workgroup.  (The rows' elements come
 // from memory once, the factor's from the caches: rows of one adapter follow one another.)
 static constexpr int LOW_NW = 8, LOW_RANKS = 16;
 template <typename T>
 __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(AdapterLowArgs a) {
   __shared__ float part[FEW_PART<LOW_NW, LOW_RANKS, 16>];
   int id, row0, rows;
-  if (!find_tile<16>(a.off, a.R + 1, blockIdx.x, id, row0, rows)) return;
+  const bool has = find_tile<16>(a.off, a.R + 1, blockIdx.x, id, row0, rows);
+  if (a.slots && blockIdx.y == 0 && threadIdx.x < 17) {
+    int* s = a.slots + (int64_t)blockIdx.x * 17;
+    if (threadIdx.x < 16) s[threadIdx.x] = has && (int)threadIdx.x < rows ? (int)a.idx[row0 + threadIdx.x] : -1;
+    else s[16] = has && id < a.R ? id : -1;
+  }
+  if (!has) return;
   const int m_ = threadIdx.x / LOW_RANKS, n_ = threadIdx.x % LOW_RANKS;
-  for (int j0 = 0; j0 < (a.planes ? a.rp : a.r); j0 += LOW_RANKS) {
-    const bool some = id < a.R && j0 < a.r;
-    if (some)
-      few_tile<T, 2, 2, 1, LOW_NW, LOW_RANKS, false>(
-          [&](int n) { return (const T*)a.A + id * a.sar + min(j0 + n, a.r - 1) * a.saj; },
-          [&](int m) { return (const T*)a.X + a.idx[row0 + min(m, rows - 1)] * a.sxm; }, 0, a.K, part);
+  const int j0 = blockIdx.y * LOW_RANKS, j = j0 + n_;
+  const bool some = id < a.R && j0 < a.r;
+  if (some) {
+    few_tile<T, 2, 2, 1, LOW_NW, LOW_RANKS, false>([&](int n) { return (const T*)a.A + id * a.sar + min(j0 + n, a.r - 1) * a.saj; },
+                                                   [&](int m) { return (const T*)a.X + a.idx[row0 + min(m, rows - 1)] * a.sxm; }, 0, a.K, part);
     __syncthreads();
-    const int j = j0 + n_;
-    if (m_ < rows) {
-      float v = 0.0f;
-      if (some && j < a.r) v = few_sum<LOW_NW, LOW_RANKS, 16>(part, n_, m_) * (a.scales ? a.scales[id] : 1.0f);
-      const int64_t t = a.idx[row0 + m_];
-      if (j < a.r) a.U[t * a.r + j] = v;
-      if (a.planes && j < a.rp) {
-        T* p = (T*)a.planes + t * 2 * a.rp + j;
-        split<T>(v, p[0], p[a.rp]);
-      }
-    }
-    __syncthreads();
+  }
+  if (m_ >= rows) return;
+  float v = 0.0f;
+  if (some && j < a.r) v = few_sum<LOW_NW, LOW_RANKS, 16>(part, n_, m_) * (a.scales ? a.scales[id] : 1.0f);
+  const int64_t t = a.idx[row0 + m_];
+  if (j < a.r) a.U[t * a.r + j] = v;
+  if (a.planes && j < a.rp) {
+    T* p = (T*)a.planes + t * 2 * a.rp + j;
+    split<T>(v, p[0], p[a.rp]);
   }
 }
 
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_k
   __shared__ float part[FEW_PART<NW, COLS, INPUTS>];
   const int n0 = blockIdx.x * COLS;
   const int64_t t0 = (int64_t)blockIdx.y * INPUTS;
-  few_tile<T, P, G, 1, NW, COLS, false>([&](int n) { return (const T*)a.W + std::min(n0 + n, a.N - 1) * a.swn; },
+  few_tile<T, P, G, 1, NW, COLS, false, P == 4 ? 4 : 0>([&](int n) { return (const T*)a.W + std::min(n0 + n, a.N - 1) * a.swn; },
                                         [&](int m) { return (const T*)a.X + std::min<int64_t>(t0 + m, a.T - 1) * a.sxm; }, 0, a.K, part);
   __syncthreads();
   for (int p = threadIdx.x; p < COLS * INPUTS; p += NW * 64) {
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_k
 // transposition, as a lane of the instruction holds one element of one row.  A lane loads 16 bytes of a row of M, and element i of
 // them is its column of product i: columns PER l + i.  A workgroup has 16 PER columns, JT x 16 of the rank and a slice of the
 // adapter's rows, which its waves take in turn, four at a time.
-static constexpr int GRAD_NW = 4;
+static constexpr int GRAD_NW = 4, GRAD_MAX_SLICES = 16;
 template <typename T, int JT>
 __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradArgs a, int slices, float* partial) {
   constexpr int PER = Few<T>::PER, COLS = 16 * PER;
@@ -227,22 +229,36 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int SIDE = 4;                                    // steps of four rows whose loads are issued side by side
+  // (the rows' indices one round ahead of their elements)
+  int64_t next[SIDE];
+  auto fetch = [&](int64_t s) {
+#pragma unroll
+    for (int u = 0; u < SIDE; ++u) {
+      const int64_t i = std::min(s + 4 * u + q, hi - 1);
+      next[u] = a.idx ? a.idx[i] : i;
+    }
+  };
+  if (lo + wave * 4 * SIDE < hi) fetch(lo + wave * 4 * SIDE);
 #pragma unroll 1
   for (int64_t s = lo + wave * 4 * SIDE; s < hi; s += GRAD_NW * 4 * SIDE) {
     V m[SIDE];
     float p[SIDE][JT];
 #pragma unroll
     for (int u = 0; u < SIDE; ++u) {
-      const int64_t i = s + 4 * u + q;
-      const int64_t t = i < hi ? (a.idx ? a.idx[i] : i) : -1;
-      const int64_t at = t < 0 ? (a.idx ? a.idx[lo] : lo) : t;
-      m[u] = __builtin_bit_cast(V, load_piece<T, false>((const T*)a.M + at * a.smm + c));
+      m[u] = __builtin_bit_cast(V, load_piece<T, false>((const T*)a.M + next[u] * a.smm + c));
 #pragma unroll
-      for (int j = 0; j < JT; ++j) {
-        const float v = a.P[at * a.r + min(j0 + 16 * j + l, a.r - 1)];
-        p[u][j] = t < 0 ? 0.0f : v;
-      }
-      if (t < 0) m[u] = __builtin_bit_cast(V, i32x4{0, 0, 0, 0});
+      for (int j = 0; j < JT; ++j) p[u][j] = a.P[next[u] * a.r + min(j0 + 16 * j + l, a.r - 1)];
+    }
+    if (s + GRAD_NW * 4 * SIDE < hi) fetch(s + GRAD_NW * 4 * SIDE);
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 4 * SIDE > hi) {
+#pragma unroll
+      for (int u = 0; u < SIDE; ++u)
+        if (s + 4 * u + q >= hi) {
+          m[u] = __builtin_bit_cast(V, i32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int j = 0; j < JT; ++j) p[u][j] = 0.0f;
+        }
     }
 #pragma unroll
     for (int u = 0; u < SIDE; ++u)
@@ -280,9 +296,14 @@ template <typename T>
 __global__ __launch_bounds__(256) void adapter_grad_join_kernel(AdapterGradArgs a, int slices, const float* partial) {
   const int c = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, id = blockIdx.z;
   if (c >= a.C) return;
-  float v = 0.0f;
-  for (int s = 0; s < slices; ++s) v += partial[(((int64_t)s * a.R + id) * a.r + j) * a.C + c];
-  ((T*)a.OUT)[id * a.soa + j * a.soj + c * a.soc] = from_f32<T>(v);
+  const float* p = partial + ((int64_t)id * a.r + j) * a.C + c;
+  const int64_t apart = (int64_t)a.R * a.r * a.C;
+  float v[GRAD_MAX_SLICES];
+#pragma unroll
+  for (int s = 0; s < GRAD_MAX_SLICES; ++s) v[s] = s < slices ? p[s * apart] : 0.0f;
+#pragma unroll
+  for (int s = 1; s < GRAD_MAX_SLICES; ++s) v[0] += v[s];
+  ((T*)a.OUT)[id * a.soa + j * a.soj + c * a.soc] = from_f32<T>(v[0]);
 }
 
 // ---- factors in another order ---------------------------------------------------------------------------------------
@@ -297,15 +318,24 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs a) {
   const T* src = (const T*)a.SRC + id * a.s0;
   T* dst = (T*)a.DST + (int64_t)id * a.n1 * a.ld;
   if (a.s2 == 1) {
-    for (int i = i0 + y; i < min(i0 + 64, a.n1); i += 4)
-      if (k0 + x < a.ld) dst[(int64_t)i * a.ld + k0 + x] = k0 + x < a.n2 ? src[i * a.s1 + k0 + x] : from_f32<T>(0.0f);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int i = i0 + y + 4 * u;
+      if (i < a.n1 && k0 + x < a.ld) dst[(int64_t)i * a.ld + k0 + x] = k0 + x < a.n2 ? src[i * a.s1 + k0 + x] : from_f32<T>(0.0f);
+    }
     return;
   }
-  for (int k = y; k < 64; k += 4)
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int k = y + 4 * u;
     if (i0 + x < a.n1) tile[k][x] = k0 + k < a.n2 ? src[(i0 + x) * a.s1 + (k0 + k) * a.s2] : from_f32<T>(0.0f);
+  }
   __syncthreads();
-  for (int i = y; i < 64; i += 4)
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int i = y + 4 * u;
     if (i0 + i < a.n1 && k0 + x < a.ld) dst[(int64_t)(i0 + i) * a.ld + k0 + x] = tile[x][i];
+  }
 }
 
 // Ids of adapters as 32-bit ones of R + 1 groups: rows without an adapter are the last group
@@ -318,7 +348,7 @@ template <typename T>
 static int low_t(const AdapterLowArgs& a, hipStream_t st) {
   const bool pieces = a.sak == 1 && a.K >= Few<T>::PER;
   if (pieces && a.idx != nullptr) {
-    hipLaunchKernelGGL(adapter_low_rows_kernel<T>, dim3((unsigned)max_tiles(a.T, a.R + 1, 16)), dim3(LOW_NW * 64), 0, st, a);
+    hipLaunchKernelGGL(adapter_low_rows_kernel<T>, dim3((unsigned)adapter_fragments(a.T, a.R), ((a.planes ? a.rp : a.r) + LOW_RANKS - 1) / LOW_RANKS), dim3(LOW_NW * 64), 0, st, a);
     return launch_status("adapter_low_rows_kernel");
   }
   if (pieces) {
@@ -339,11 +369,14 @@ static int project_rows(const AdapterProjectArgs& a, hipStream_t st) {
 template <typename T>
 static int project_t(const AdapterProjectArgs& a, hipStream_t st) {
   if (a.swk == 1 && a.K >= Few<T>::PER) {
+    // Beyond 32 rows: 16-bit types in chunks of 32 (48 rows, 2880 -> 4096 20 -> 12 us, 64 rows, 4096 -> 4096 29 -> 18, against tiles of
+    // 64 x 32: twice the workgroups count for more than half the weights' traffic from the caches); float32, whose products are what
+    // takes the time, without parts (64 rows, 2048 -> 2048 16 -> 15 us), in wider tiles from 65 rows on (1024 rows, 4096 -> 4096 695 -> 501).
     if (a.T <= 4) return project_rows<T, 4, 1, 8, 16>(a, st);
     if (a.T <= 8) return project_rows<T, 2, 1, 8, 16>(a, st);
     if (a.T <= 16) return project_rows<T, 2, 2, 8, 16>(a, st);
-    if (a.T <= 32) return project_rows<T, 2, 4, 8, 16>(a, st);
-    return project_rows<T, 1, 4, 4, 32>(a, st);
+    if (a.T <= 32 || sizeof(T) == 2) return project_rows<T, 2, 4, 8, 16>(a, st);
+    if constexpr (sizeof(T) == 4) return a.T <= 64 ? project_rows<T, 1, 2, 8, 16>(a, st) : project_rows<T, 1, 2, 8, 32>(a, st);
   }
   const int64_t rows = cdiv64(a.T, PBM);
   if (rows > 65535) { set_error("smoe_adapter_project: too many rows for this layout"); return SMOE_ERR_RANGE; }
@@ -352,7 +385,7 @@ static int project_t(const AdapterProjectArgs& a, hipStream_t st) {
 }
 
 // Slices of an adapter's rows: enough workgroups for the chip, at least GRAD_MIN_ROWS rows each at even loads
-static constexpr int GRAD_WGS = 1024, GRAD_MIN_ROWS = 128, GRAD_MAX_SLICES = 32;
+static constexpr int GRAD_WGS = 1024, GRAD_MIN_ROWS = 128;
 static int grad_tiles(int64_t C, int dtype) { return (int)cdiv64(C, dtype == SMOE_F32 ? 64 : 128); }
 static int grad_ranks(int64_t r) { return r <= 16 ? 1 : 2; }
 static int grad_slices(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {

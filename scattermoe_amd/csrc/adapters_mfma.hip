@@ -15,6 +15,7 @@ namespace smoe {
 struct AdapterTiles {
   AdapterProjectArgs p;
   Raster rast;
+  int64_t fragments;
 };
 
 // Tile classes: 0 one wave per SIMD (long contractions of whole slices), 1 eight waves, 2 tiles of 128 x 128, two workgroups per CU
@@ -39,18 +40,17 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   if (!args.rast.map(blockIdx.x, m_tile, n_tile, m_loc, n_loc)) return;
   const int n0 = n_tile * TL::BN, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // rows of the tile's fragments; one behind the last row has adapter -1 and repeats a row that is there
+  // rows of the tile's fragments; one behind the last row repeats the fragment's first, or any
+  const int64_t fragments = args.fragments, f0 = (int64_t)m_tile * FRAGS;
   bool any = false;
-  for (int f = wave; f < FRAGS; f += TL::NW) {
-    int id = -1, row0 = 0, rows = 0;
-    const bool has = find_tile<16>(a.off, a.R + 1, m_tile * FRAGS + f, id, row0, rows);
-    any |= has;
-    if (lane < 16) {
-      const int64_t t = has && lane < rows ? a.idx[row0 + lane] : -1;
-      sSrc[f * 16 + lane] = (int)(t >= 0 ? t : has ? a.idx[row0] : 0);
-      sDst[f * 16 + lane] = t >= 0 ? t * a.sym : -1;
-      if (lane == 0) sAdapter[f] = has && id < a.R ? id : -1;
-    }
+  for (int m = threadIdx.x; m < TL::BM; m += TL::NT) {
+    const int64_t f = f0 + (m >> 4);
+    const int* s = a.slots + f * 17;
+    const int t = f < fragments ? s[m & 15] : -1, first = f < fragments ? s[0] : -1;
+    any |= first >= 0;
+    sSrc[m] = t >= 0 ? t : max(first, 0);
+    sDst[m] = t >= 0 ? (int64_t)t * a.sym : -1;
+    if ((m & 15) == 0) sAdapter[m >> 4] = f < fragments ? s[16] : -1;
   }
   if (!__syncthreads_or(any)) return;
 
@@ -64,25 +64,35 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   for (int k0 = 0; k0 < a.rp; k0 += 32) {
     const int k = k0 + 8 * lq;
     const bool inside = k < a.r;                             // (r is a multiple of 8 here; U is padded with zeros to rp)
-#pragma unroll
-    for (int i = 0; i < 2 * TL::FM; ++i) {
+    // (a fragment's operands are on their way while the one before is multiplied)
+    i32x4 u[2][2], bv[2][2 * TL::FN];
+    auto load = [&](int i, int p) {
       const int row = wm * TL::WTM + 16 * i;
       const int id = __builtin_amdgcn_readfirstlane(sAdapter[row >> 4]);
-      const T* u = (const T*)a.planes + (int64_t)sSrc[row + lr] * 2 * a.rp + k;
-      const i32x4 u0 = *(const i32x4*)u, u1 = *(const i32x4*)(u + a.rp);
+      const T* x = (const T*)a.planes + (int64_t)sSrc[row + lr] * 2 * a.rp + k;
+      u[p][0] = *(const i32x4*)x;
+      u[p][1] = *(const i32x4*)(x + a.rp);
       const T* b = (const T*)a.B + (int64_t)max(id, 0) * a.sbr + (inside ? k : 0);
-      i32x4 bv[2 * TL::FN];
 #pragma unroll
-      for (int j = 0; j < 2 * TL::FN; ++j) {
-        bv[j] = *(const i32x4*)(b + (int64_t)min(n0 + wn * TL::WTN + 16 * j + lr, a.N - 1) * a.sbn);
-        if (!inside || id < 0) bv[j] = i32x4{0, 0, 0, 0};
-      }
+      for (int j = 0; j < 2 * TL::FN; ++j) bv[p][j] = *(const i32x4*)(b + (int64_t)min(n0 + wn * TL::WTN + 16 * j + lr, a.N - 1) * a.sbn);
+    };
+    load(0, 0);
 #pragma unroll
-      for (int j = 0; j < 2 * TL::FN; ++j) {
-        f32x4& c = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
-        c = Mfma<T>::run(bv[j], u0, c);
-        c = Mfma<T>::run(bv[j], u1, c);
-      }
+    for (int i = 0; i < 2 * TL::FM; ++i) {
+      if (i + 1 < 2 * TL::FM) load(i + 1, (i + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool none = !inside || sAdapter[(wm * TL::WTM >> 4) + i] < 0;
+#pragma unroll
+      for (int j = 0; j < 2 * TL::FN; ++j)
+        if (none) bv[i & 1][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2 * TL::FN; ++j) {
+          f32x4& c = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
+          c = Mfma<T>::run(bv[i & 1][j], u[i & 1][h], c);
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -107,11 +117,24 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   }
 }
 
+// Super tiles share operands best; but an XCD takes whole ones, and where one is left over it runs a round of its own: column
+// stripes then, if they make fewer rounds of `wgs` workgroups per CU (4099 rows, 24 adapters, 2880 -> 2880, nine super tiles: 139 -> 78
+// us).
+static Raster tile_order(int64_t m_tiles, int n_tiles, int wgs) {
+  const Raster supers = make_raster(m_tiles, n_tiles, GM_S2S);
+  const int64_t round = NUM_CU / 8 * wgs, super = Raster::SM * Raster::SN;
+  const int64_t by_supers = cdiv64(cdiv64(supers.supers, 8) * super, round);
+  const int64_t by_stripes = cdiv64(cdiv64(m_tiles / GM_RING * n_tiles, 8) * GM_RING + cdiv64(n_tiles, 8) * (m_tiles % GM_RING), round);
+  return by_stripes < by_supers ? make_striped(m_tiles, n_tiles, GM_RING) : supers;
+}
+
 template <typename T, int CLASS>
 static int launch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st) {
   typedef typename AdapterTile<CLASS>::type TL;
-  const int64_t m_tiles = cdiv64(a.T + 15 * std::min<int64_t>(a.R + 1, a.T), TL::BM);
-  AdapterTiles args{a, make_raster(m_tiles, (a.N + TL::BN - 1) / TL::BN, GM_S2S)};
+  const int64_t fragments = adapter_fragments(a.T, a.R);
+  const int64_t m_tiles = cdiv64(fragments, TL::BM / 16);
+  const int n_tiles = (a.N + TL::BN - 1) / TL::BN;
+  AdapterTiles args{a, tile_order(m_tiles, n_tiles, TL::WG), fragments};
   const int64_t grid = args.rast.grid();
   if (grid > 0x7fffffffLL) { set_error("smoe_adapter_project: grid too large"); return SMOE_ERR_RANGE; }
   if (w_tr) hipLaunchKernelGGL((adapter_tiles_kernel<T, CLASS, true>), dim3((unsigned)grid), dim3(TL::NT), 0, st, args);
@@ -132,7 +155,7 @@ static int dispatch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Whole pieces of 16 bytes in all operands, and lane offsets of 32 bits into X and W
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc) {
-  if ((dtype != SMOE_BF16 && dtype != SMOE_F16) || a.planes == nullptr || a.idx == nullptr) return false;
+  if ((dtype != SMOE_BF16 && dtype != SMOE_F16) || a.planes == nullptr || a.slots == nullptr) return false;
   if (a.K < 8 || a.K % 8 != 0 || a.sxm % 8 != 0 || !aligned16(a.X) || !aligned16(a.W)) return false;
   if (a.r % 8 != 0 || a.sbj != 1 || a.sbn % 8 != 0 || a.sbr % 8 != 0 || !aligned16(a.B) || a.rp % 32 != 0 || !aligned16(a.planes)) return false;
   bool w_tr;

@@ -411,12 +411,29 @@ static int adapter_checks(const char* who, int64_t T, int64_t K, int64_t N, int6
   return 0;
 }
 
-int smoe_adapter_groups(const int64_t* ids, int64_t T, int64_t R, int32_t* groups, void* stream) {
+// (T 64-bit sorted groups, T 32-bit groups, the routing's own workspace)
+static size_t order_bytes(int64_t T) { return ((size_t)T * 12 + 15) / 16 * 16; }
+size_t smoe_adapter_order_workspace_bytes(int64_t T, int64_t R) {
+  if (T <= 0 || R <= 0 || R > SMOE_ADAPTER_MAX) return 0;
+  return order_bytes(T) + route_workspace_bytes(T, (int)R + 1);
+}
+
+int smoe_adapter_order(const int64_t* ids, int64_t T, int64_t R, int64_t* idx, int64_t* off, void* workspace, size_t workspace_bytes,
+                       void* stream) {
   g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_groups", T, 0, 0, 1, R, SMOE_F32)) return rc;
-  if (T == 0) return 0;
-  if (!ids || !groups) { set_error("smoe_adapter_groups: NULL pointer"); return SMOE_ERR_NULL; }
-  return launch_adapter_groups(ids, T, (int)R, groups, (hipStream_t)stream);
+  if (int rc = adapter_checks("smoe_adapter_order", T, 0, 0, 1, R, SMOE_F32)) return rc;
+  if (!off || (T > 0 && (!ids || !idx))) { set_error("smoe_adapter_order: NULL pointer"); return SMOE_ERR_NULL; }
+  const size_t need = smoe_adapter_order_workspace_bytes(T, R);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
+    set_error("smoe_adapter_order: a workspace of %zu bytes, 16-byte aligned, is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return SMOE_ERR_WORKSPACE;
+  }
+  int64_t* eid = (int64_t*)workspace;
+  int* groups = (int*)(eid + T);
+  if (T > 0) {
+    if (int rc = launch_adapter_groups(ids, T, (int)R, groups, (hipStream_t)stream)) return rc;
+  }
+  return launch_route(groups, SMOE_I32, T, (int)R + 1, eid, idx, off, (char*)workspace + order_bytes(T), (hipStream_t)stream);
 }
 
 int smoe_adapter_pack(const void* SRC, int64_t s0, int64_t s1, int64_t s2, void* DST, int64_t n0, int64_t n1, int64_t n2,
@@ -430,32 +447,33 @@ int smoe_adapter_pack(const void* SRC, int64_t s0, int64_t s1, int64_t s2, void*
   return launch_adapter_pack(AdapterPackArgs{SRC, s0, s1, s2, DST, (int)ld, off, (int)n0, (int)n1, (int)n2}, dtype, (hipStream_t)stream);
 }
 
+size_t smoe_adapter_slots(int64_t T, int64_t R) { return T <= 0 || R <= 0 || R > SMOE_ADAPTER_MAX ? 0 : (size_t)adapter_fragments(T, R) * 17; }
+
 int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
-                     const float* scales, const int64_t* idx, const int64_t* off, float* U, void* planes, int64_t T, int64_t K,
-                     int64_t r, int64_t R, int dtype, void* stream) {
+                     const float* scales, const int64_t* idx, const int64_t* off, float* U, void* planes, int32_t* slots,
+                     int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream) {
   g_err[0] = 0;
   if (int rc = adapter_checks("smoe_adapter_low", T, K, 0, r, R, dtype)) return rc;
   if (T == 0) return 0;
   if ((K > 0 && (!X || !A)) || !ids || !U) { set_error("smoe_adapter_low: NULL pointer"); return SMOE_ERR_NULL; }
-  if (!idx != !off || (planes && (!idx || dtype == SMOE_F32 || sak != 1 || K < 8))) {
+  if (!idx != !off || !planes != !slots || (planes && (!idx || dtype == SMOE_F32 || sak != 1 || K < 8))) {
     set_error("smoe_adapter_low: two parts need rows in order, 16-bit types and a contiguous contraction of 8 and more");
     return SMOE_ERR_UNSUPPORTED;
   }
-  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, idx, off, U, planes, (int)((r + 31) / 32 * 32), T, (int)K,
+  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, idx, off, U, planes, (int)((r + 31) / 32 * 32), slots, T, (int)K,
                                            (int)r, (int)R}, dtype, (hipStream_t)stream);
 }
 
 int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
-                         const float* U, const void* planes, const void* B, int64_t sbr, int64_t sbn, int64_t sbj,
-                         const int64_t* ids, const int64_t* idx, const int64_t* off, void* Y, int64_t sym, int64_t T, int64_t K,
-                         int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
+                         const float* U, const void* planes, const int32_t* slots, const void* B, int64_t sbr, int64_t sbn, int64_t sbj,
+                         const int64_t* ids, void* Y, int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
   g_err[0] = 0;
   if (int rc = adapter_checks("smoe_adapter_project", T, K, N, r, R, dtype)) return rc;
   if (T == 0 || N == 0) return 0;
   if ((K > 0 && (!X || !W)) || !U || !B || !ids || !Y) { set_error("smoe_adapter_project: NULL pointer"); return SMOE_ERR_NULL; }
-  if (!idx != !off) { set_error("smoe_adapter_project: idx and off go together"); return SMOE_ERR_NULL; }
-  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, planes, (int)((r + 31) / 32 * 32), B, sbr, sbn, sbj,
-                                                   ids, idx, off, Y, sym, T, (int)K, (int)N, (int)r, (int)R}, dtype, (hipStream_t)stream);
+  if (!planes != !slots) { set_error("smoe_adapter_project: planes and slots go together"); return SMOE_ERR_NULL; }
+  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, planes, (int)((r + 31) / 32 * 32), slots, B, sbr, sbn, sbj,
+                                                   ids, Y, sym, T, (int)K, (int)N, (int)r, (int)R}, dtype, (hipStream_t)stream);
 }
 
 size_t smoe_adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {

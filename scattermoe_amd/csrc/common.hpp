@@ -383,6 +383,7 @@ struct AdapterLowArgs {
   const int64_t* idx; const int64_t* off;            // rows by adapter, those without one last, offsets (R + 1); or NULL
   float* U;                                          // (T, r)
   void* planes; int rp;                              // (T, 2, rp) of the operands' type, U in two parts; or NULL
+  int* slots;                                        // (fragments, 17): rows of every 16, or -1, and their adapter, or -1
   int64_t T;
   int K, r, R;
 };
@@ -391,10 +392,9 @@ struct AdapterProjectArgs {
   const void* W; int64_t swn, swk;                   // (N, K)
   const void* bias; int64_t sb;                      // (N) or NULL
   const float* U;                                    // (T, r)
-  const void* planes; int rp;                        // as AdapterLowArgs
+  const void* planes; int rp; const int* slots;      // as AdapterLowArgs
   const void* B; int64_t sbr, sbn, sbj;              // (R, N, r)
   const int64_t* ids;                                // (T)
-  const int64_t* idx; const int64_t* off;            // as AdapterLowArgs
   void* Y; int64_t sym;                              // (T, N), columns contiguous
   int64_t T;
   int K, N, r, R;
@@ -413,6 +413,8 @@ struct AdapterPackArgs {
   const int64_t* off;                                // inclusive offsets (n0) or NULL
   int n0, n1, n2;
 };
+// Fragments of 16 rows, each of one adapter, that T rows of R adapters (and of none) can make
+static inline int64_t adapter_fragments(int64_t T, int64_t R) { return max_tiles(T, (int)R + 1, 16); }
 int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st);
 int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st);
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc);       // csrc/adapters_mfma.hip

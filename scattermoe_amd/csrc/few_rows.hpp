@@ -115,11 +115,12 @@ static constexpr int FEW_PART = NW * WROWS * (INPUTS + 1);
 
 // Products of WROWS weight rows with G groups of 16 / P input rows over K >= PER contraction elements, by NW waves that take blocks
 // of the contraction in turn.  `weight(n)` / `input(m)`: the first element of such a row.  Inputs of H parts: `apart` elements
-// from one part of a row to the next.  ONCE: no other workgroup reads these weights.  Leaves the waves' sums in `part` (see few_at), without a barrier.
-template <typename T, int P, int G, int H, int NW, int WROWS, bool ONCE = true, class Weight, class Input>
+// from one part of a row to the next.  ONCE: no other workgroup reads these weights.  MORE: loads of each
+// row that are issued side by side, if not the usual number.  Leaves the waves' sums in `part` (see few_at), without a barrier.
+template <typename T, int P, int G, int H, int NW, int WROWS, bool ONCE = true, int MORE = 0, class Weight, class Input>
 __device__ __forceinline__ void few_tile(Weight weight, Input input, int apart, int K, float* part) {
   typedef FewLane<T, P> Lane;
-  constexpr int NT = WROWS / Lane::ROWS, LOADS = NT + G * H, SIDE = LOADS <= 3 ? 4 : LOADS <= 6 ? 2 : 1, STEP = Lane::STEP, BLOCK = SIDE * STEP;
+  constexpr int NT = WROWS / Lane::ROWS, LOADS = NT + G * H, SIDE = MORE ? MORE : LOADS <= 3 ? 4 : LOADS <= 6 ? 2 : 1, STEP = Lane::STEP, BLOCK = SIDE * STEP;
   constexpr int INPUTS = G * Lane::ROWS, V = FewSums<P>::VALUES;
   const Lane l;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

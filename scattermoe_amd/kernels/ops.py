@@ -7,6 +7,7 @@ parallel_experts.py:6) — with the Triton launches replaced by calls into libsc
 All device work goes through `_backend`, an object with `route / offsets / s2s / group / xty` methods.
 The only backend shipped is `HipBackend` (the C ABI); it refuses CPU tensors.
 """
+import functools
 from typing import Optional
 
 import torch
@@ -17,6 +18,22 @@ from .. import _C
 # library per launch, and gfx950 has no TF32 mode: fp32 inputs are always multiplied in full fp32.
 BLOCK_M = 128
 ALLOW_TF32 = True
+
+
+# What the library asks for, by sizes alone: asked once per size
+@functools.lru_cache(maxsize=1024)
+def _routed_layer_bytes(T, k, d, F):
+    return _C.load().smoe_routed_glu_mlp_workspace_bytes(T, k, d, F)
+
+
+@functools.lru_cache(maxsize=1024)
+def _adapter_order_bytes(T, R):
+    return _C.load().smoe_adapter_order_workspace_bytes(T, R)
+
+
+@functools.lru_cache(maxsize=1024)
+def _adapter_grad_bytes(T, C, r, R, code):
+    return _C.load().smoe_adapter_grad_workspace_bytes(T, C, r, R, code)
 
 
 class HipBackend:
@@ -314,7 +331,7 @@ class HipBackend:
         T, F, code = x.size(0), w2.size(2), _C.float_code(x.dtype)
         sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
         sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
-        need = lib.smoe_routed_glu_mlp_workspace_bytes(T, k, x.size(1), F)
+        need = _routed_layer_bytes(T, k, x.size(1), F)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         with _C.on_device(x.device):
             rc = lib.smoe_routed_glu_mlp(
@@ -326,11 +343,15 @@ class HipBackend:
         _C.check(rc, "smoe_routed_glu_mlp")
 
     @staticmethod
-    def adapter_groups(ids, R, groups):
-        _C.require_gpu(ids, "adapter_groups")
+    def adapter_order(ids, R, idx, off):
+        _C.require_gpu(ids, "adapter_order")
+        T = ids.numel()
+        need = _adapter_order_bytes(T, R)
+        ws = torch.empty(need, dtype=torch.uint8, device=ids.device)
         with _C.on_device(ids.device):
-            rc = _C.load().smoe_adapter_groups(_C.ptr(ids), ids.numel(), R, _C.ptr(groups), _C.stream_ptr(ids.device))
-        _C.check(rc, "smoe_adapter_groups")
+            rc = _C.load().smoe_adapter_order(_C.ptr(ids), T, R, _C.ptr(idx), _C.ptr(off), _C.ptr(ws), need,
+                                              _C.stream_ptr(ids.device))
+        _C.check(rc, "smoe_adapter_order")
 
     @staticmethod
     def adapter_pack(src, dst, off):
@@ -341,24 +362,24 @@ class HipBackend:
         _C.check(rc, "smoe_adapter_pack")
 
     @staticmethod
-    def adapter_low(X, A, ids, scales, idx, off, U, planes):
+    def adapter_low(X, A, ids, scales, idx, off, U, planes, slots):
         _C.require_gpu(X, "adapter_low")
         lib = _C.load()
         with _C.on_device(X.device):
             rc = lib.smoe_adapter_low(_C.ptr(X), X.stride(0), _C.ptr(A), A.stride(0), A.stride(1), A.stride(2), _C.ptr(ids),
-                                      _C.ptr(scales), _C.ptr(idx), _C.ptr(off), _C.ptr(U), _C.ptr(planes), X.size(0),
-                                      X.size(1), A.size(1), A.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
+                                      _C.ptr(scales), _C.ptr(idx), _C.ptr(off), _C.ptr(U), _C.ptr(planes), _C.ptr(slots),
+                                      X.size(0), X.size(1), A.size(1), A.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
         _C.check(rc, "smoe_adapter_low")
 
     @staticmethod
-    def adapter_project(X, W, bias, U, planes, B, ids, idx, off, Y):
+    def adapter_project(X, W, bias, U, planes, slots, B, ids, Y):
         _C.require_gpu(X, "adapter_project")
         lib = _C.load()
         with _C.on_device(X.device):
             rc = lib.smoe_adapter_project(
                 _C.ptr(X), X.stride(0), _C.ptr(W), W.stride(0), W.stride(1), _C.ptr(bias),
-                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(planes), _C.ptr(B), B.stride(0), B.stride(1),
-                B.stride(2), _C.ptr(ids), _C.ptr(idx), _C.ptr(off), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0),
+                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(planes), _C.ptr(slots), _C.ptr(B), B.stride(0), B.stride(1),
+                B.stride(2), _C.ptr(ids), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0),
                 U.size(1), B.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
         _C.check(rc, "smoe_adapter_project")
 
@@ -367,7 +388,7 @@ class HipBackend:
         _C.require_gpu(M, "adapter_grad")
         lib = _C.load()
         code, T, C, r, R = _C.float_code(M.dtype), M.size(0), M.size(1), P.size(1), out.size(0)
-        need = lib.smoe_adapter_grad_workspace_bytes(T, C, r, R, code)
+        need = _adapter_grad_bytes(T, C, r, R, code)
         ws = torch.empty(need, dtype=torch.uint8, device=M.device) if need else None
         with _C.on_device(M.device):
             rc = lib.smoe_adapter_grad(_C.ptr(P), _C.ptr(M), M.stride(0), _C.ptr(idx), _C.ptr(off), _C.ptr(out),
@@ -490,9 +511,9 @@ def _routed_glu_mlp_op(x: torch.Tensor, wr: torch.Tensor, w1: torch.Tensor, b1: 
     _backend.routed_glu_mlp(x, wr, w1, b1, w2, b2, out, logits, k, renormalize, act)
 
 
-@torch.library.custom_op("scattermoe::adapter_groups", mutates_args={"groups"})
-def _adapter_groups_op(ids: torch.Tensor, R: int, groups: torch.Tensor) -> None:
-    _backend.adapter_groups(ids, R, groups)
+@torch.library.custom_op("scattermoe::adapter_order", mutates_args={"idx", "off"})
+def _adapter_order_op(ids: torch.Tensor, R: int, idx: torch.Tensor, off: torch.Tensor) -> None:
+    _backend.adapter_order(ids, R, idx, off)
 
 
 @torch.library.custom_op("scattermoe::adapter_pack", mutates_args={"dst"})
@@ -500,18 +521,18 @@ def _adapter_pack_op(src: torch.Tensor, dst: torch.Tensor, off: Optional[torch.T
     _backend.adapter_pack(src, dst, off)
 
 
-@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U", "planes"})
+@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U", "planes", "slots"})
 def _adapter_low_op(X: torch.Tensor, A: torch.Tensor, ids: torch.Tensor, scales: Optional[torch.Tensor],
                     idx: Optional[torch.Tensor], off: Optional[torch.Tensor], U: torch.Tensor,
-                    planes: Optional[torch.Tensor]) -> None:
-    _backend.adapter_low(X, A, ids, scales, idx, off, U, planes)
+                    planes: Optional[torch.Tensor], slots: Optional[torch.Tensor]) -> None:
+    _backend.adapter_low(X, A, ids, scales, idx, off, U, planes, slots)
 
 
 @torch.library.custom_op("scattermoe::adapter_project", mutates_args={"Y"})
 def _adapter_project_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], U: torch.Tensor,
-                        planes: Optional[torch.Tensor], B: torch.Tensor, ids: torch.Tensor, idx: Optional[torch.Tensor],
-                        off: Optional[torch.Tensor], Y: torch.Tensor) -> None:
-    _backend.adapter_project(X, W, bias, U, planes, B, ids, idx, off, Y)
+                        planes: Optional[torch.Tensor], slots: Optional[torch.Tensor], B: torch.Tensor, ids: torch.Tensor,
+                        Y: torch.Tensor) -> None:
+    _backend.adapter_project(X, W, bias, U, planes, slots, B, ids, Y)
 
 
 @torch.library.custom_op("scattermoe::adapter_grad", mutates_args={"out"})
@@ -523,7 +544,7 @@ def _adapter_grad_op(P: torch.Tensor, M: torch.Tensor, idx: Optional[torch.Tenso
 _COMPILED_OPS = {"route": _route_op, "offsets": _offsets_op, "combine": _combine_op, "gate_grad": _gate_grad_op,
                  "glu_fwd": _glu_fwd_op, "glu_bwd": _glu_bwd_op, "topk_softmax": _topk_softmax_op,
                  "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op,
-                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_groups": _adapter_groups_op,
+                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_order": _adapter_order_op,
                  "adapter_pack": _adapter_pack_op, "adapter_low": _adapter_low_op,
                  "adapter_project": _adapter_project_op, "adapter_grad": _adapter_grad_op}
 
@@ -1061,12 +1082,15 @@ ADAPTERS_MAX, ADAPTER_MAX_RANK = 2047, 512          # SMOE_ADAPTER_MAX, SMOE_ADA
 ADAPTER_FEW_ROWS = 64          # up to so many rows the adapters' products go row by row, without an order
 
 
+ADAPTER_LOOK_UP = 1 << 22
+
+
 def adapter_order(ids, R):
     """The rows by adapter, those without one last: (indices (T), inclusive offsets (R + 1)), for `adapter_low`,
     `adapter_project` and, of whose offsets it takes the first R, `adapter_grad`."""
-    groups = torch.empty(ids.numel(), dtype=torch.int32, device=ids.device)
-    _launch("adapter_groups", ids, R, groups)
-    _, idx, off = route(groups, R + 1)
+    idx = torch.empty(ids.numel(), dtype=torch.int64, device=ids.device)
+    off = torch.empty(R + 1, dtype=torch.int64, device=ids.device)
+    _launch("adapter_order", ids, R, idx, off)
     return idx, off
 
 
@@ -1085,34 +1109,38 @@ def _pieces(t):
 
 
 def adapter_low(X, A, ids, scales=None, order=None):
-    """(U, planes): U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the
-    rows whose id lies outside [0, R).  `order`: of `adapter_order`, for many rows; planes is then U in two 16-bit parts for
-    the tiles of `adapter_project`, else None."""
+    """(U, parts): U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the
+    rows whose id lies outside [0, R).  `order`: of `adapter_order`, for many rows; parts is then what the tiles of
+    `adapter_project` take, U in two 16-bit parts and the rows of every 16 that share an adapter, else None."""
     assert A.dim() == 3 and A.size(2) == X.size(1) and ids.shape == (X.size(0),)
     _same_dtype("adapter_low", X, A)
     T, K, r = X.size(0), X.size(1), A.size(1)
     idx, off = order if order is not None else (None, None)
     U = torch.empty((T, r), dtype=torch.float32, device=X.device)
-    planes = None
+    planes = slots = None
     if order is not None and K >= 8:
-        if A.stride(2) != 1:
+        # (a strided factor is copied where the copy's reuse pays for its launch; single values are looked up otherwise)
+        if A.stride(2) != 1 and (X.dtype != torch.float32 or T * K * r > ADAPTER_LOOK_UP):
             A = _adapter_pack(A, off)
         if X.dtype != torch.float32:
             planes = torch.empty((T, 2, -(-r // 32) * 32), dtype=X.dtype, device=X.device)
-    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, idx, off, U, planes)
-    return U, planes
+            # (smoe_adapter_slots)
+            slots = torch.empty(17 * max(1, min(T, T // 16 + A.size(0) + 1)), dtype=torch.int32, device=X.device)
+    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, idx, off, U, planes, slots)
+    return U, (planes, slots) if planes is not None else None
 
 
-def adapter_project(X, W, U, B, ids, bias=None, planes=None, order=None):
+def adapter_project(X, W, U, B, ids, bias=None, parts=None, order=None):
     """Y[t] = W X[t] (+ bias) + B[a] U[t], a = ids[t], for X (T, K), W (N, K), U (T, r) float32 and B (R, N, r); rows whose
-    id lies outside [0, R) get no second term.  `planes`, `order`: of `adapter_low`, for many rows."""
+    id lies outside [0, R) get no second term.  `parts`, `order`: of `adapter_low`, for many rows."""
     assert W.size(1) == X.size(1) and B.size(1) == W.size(0) and U.shape == (X.size(0), B.size(2)) and ids.shape == (X.size(0),)
     _same_dtype("adapter_project", X, W, B, bias)
     T, K, N, r = X.size(0), X.size(1), W.size(0), U.size(1)
     Y = torch.empty((T, N), dtype=X.dtype, device=X.device)
     X = _rows_contiguous(X)
-    idx, off = order if order is not None else (None, None)
+    planes, slots = parts if parts is not None else (None, None)
     if planes is not None:
+        off = order[1]
         # the tiles' operands in 16-byte pieces: copies of what is not, a few percent of the product's own traffic
         if r % 8 or not _pieces(B):
             B = _adapter_pack(B, off, 8)
@@ -1123,7 +1151,7 @@ def adapter_project(X, W, U, B, ids, bias=None, planes=None, order=None):
             W = _adapter_pack(W.unsqueeze(0), None, 8)[0]
     elif T > 1 and K >= 8 and W.stride(1) != 1:
         W = _adapter_pack(W.unsqueeze(0))[0]                # row by row: a contiguous contraction
-    _launch("adapter_project", X, W, bias, U, planes, B, ids, idx, off, Y)
+    _launch("adapter_project", X, W, bias, U, planes, slots, B, ids, Y)
     return Y
 
 

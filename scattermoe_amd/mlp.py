@@ -185,17 +185,21 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
         raise ValueError("routed_glu_mlp: biases are (E, 2F) and (E, d)")
     if not 0 < k <= min(E, 64) or E > 512:
         raise ValueError("routed_glu_mlp: k must be in 1..min(num_experts, 64), and there are at most 512 experts")
-    ops._same_dtype("routed_glu_mlp", x, router_weight, w1, w2, b1, b2)
+    trained = x.requires_grad
     for t in (router_weight, w1, w2, b1, b2):
-        if t is not None and t.device != x.device:
-            raise RuntimeError("routed_glu_mlp: tensors on %s and %s" % (x.device, t.device))
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise TypeError("routed_glu_mlp: dtype mismatch (%s vs %s)" % (x.dtype, t.dtype))
+        if t.device != x.device:
+            raise RuntimeError("routed_glu_mlp: all tensors on the device of x (%s)" % x.device)
+        trained = trained or t.requires_grad
     tokens = x.reshape(-1, d)
     T = tokens.size(0)
     if T == 0:
         return x.new_empty(x.shape), x.new_empty((0, E), dtype=torch.float32)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    trained = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, router_weight, w1, w2, b1, b2))
-    if ops.few_tokens(T, k, E) and not trained:
+    if ops.few_tokens(T, k, E) and not (trained and torch.is_grad_enabled()):
         out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
         return out.view(x.shape), logits
     logits = nn.functional.linear(tokens.float(), router_weight.float())

@@ -50,8 +50,10 @@ class _Backend(OracleBackend):
         return factor[ids.clamp(0, factor.size(0) - 1)].double() * on.view(-1, 1, 1), on
 
     @staticmethod
-    def adapter_groups(ids, R, groups):
-        groups.copy_(torch.where((ids >= 0) & (ids < R), ids, torch.full_like(ids, R)))
+    def adapter_order(ids, R, idx, off):
+        groups = torch.where((ids >= 0) & (ids < R), ids, torch.full_like(ids, R))
+        idx.copy_(torch.sort(groups, stable=True).indices)
+        off.copy_(torch.bincount(groups, minlength=R + 1).cumsum(0))
 
     @staticmethod
     def adapter_pack(src, dst, off):
@@ -59,7 +61,7 @@ class _Backend(OracleBackend):
         dst[:, :, :src.size(2)] = src
 
     @classmethod
-    def adapter_low(cls, X, A, ids, scales, idx, off, U, planes):
+    def adapter_low(cls, X, A, ids, scales, idx, off, U, planes, slots):
         f, _ = cls._picked(A, ids)
         s = torch.ones(A.size(0)) if scales is None else scales
         U.copy_((f @ X.double().unsqueeze(2)).squeeze(2) * s[ids.clamp(0, A.size(0) - 1)].unsqueeze(1))
@@ -69,7 +71,7 @@ class _Backend(OracleBackend):
             planes[:, 1, :U.size(1)] = (U - planes[:, 0, :U.size(1)].float()).to(planes.dtype)
 
     @classmethod
-    def adapter_project(cls, X, W, bias, U, planes, B, ids, idx, off, Y):
+    def adapter_project(cls, X, W, bias, U, planes, slots, B, ids, Y):
         f, _ = cls._picked(B[:, :, :U.size(1)], ids)
         u = U.double() if planes is None else planes.double().sum(1)[:, :U.size(1)]
         Y.copy_(X[:, :W.size(1)].double() @ W.double().t() + (f @ u.unsqueeze(2)).squeeze(2) + (0 if bias is None else bias.double()))
@@ -217,21 +219,26 @@ def test_library_refuses_before_it_launches():
     assert layer(T=0) == 0
     assert lib.smoe_routed_glu_mlp_workspace_bytes(0, 2, 64, 64) == 0 and lib.smoe_routed_glu_mlp_workspace_bytes(4, 2, 64, 64) >= 8 * 64 * 4
     def low(r=8, R=3, T=4, x=one, idx=None, off=None, planes=None, dtype=1, K=64):
-        return lib.smoe_adapter_low(x, 64, one, 64, 64, 1, one, None, idx, off, one, planes, T, K, r, R, dtype, None)
+        return lib.smoe_adapter_low(x, 64, one, 64, 64, 1, one, None, idx, off, one, planes, planes, T, K, r, R, dtype, None)
     assert low(r=0) == -2 and low(R=2048) == -5 and low(r=513) == -5 and low(x=None) == -1 and low(dtype=7) == -3
     assert low(idx=one) == -6 and low(planes=one) == -6 and low(idx=one, off=one, planes=one, dtype=0) == -6
     assert low(idx=one, off=one, planes=one, K=7) == -6
 
-    def project(r=8, ids=one, idx=None, T=4):
-        return lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, None, one, 8, 8, 1, ids, idx, None, one, 64, T, 64, 64, r, 3, 1, None)
-    assert project(r=513) == -5 and project(ids=None) == -1 and project(idx=one) == -1 and project(T=-1) == -2
+    def project(r=8, ids=one, slots=None, T=4):
+        return lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, None, slots, one, 8, 8, 1, ids, one, 64, T, 64, 64, r, 3, 1, None)
+    assert project(r=513) == -5 and project(ids=None) == -1 and project(slots=one) == -1 and project(T=-1) == -2
+    for T, R in ((1, 1), (15, 3), (16, 1), (1777, 16), (100, 2047)):
+        assert lib.smoe_adapter_slots(T, R) == 17 * max(1, min(T, T // 16 + R + 1))
+    assert lib.smoe_adapter_slots(0, 3) == 0 and lib.smoe_adapter_slots(4, 0) == 0
 
     def grad(off=one, T=4, C=64, ws=None, ws_bytes=0):
         return lib.smoe_adapter_grad(one, one, 64, None, off, one, 8, 8, 1, T, C, 8, 1, 1, ws, ws_bytes, None)
     assert grad(off=None) == -1 and grad(T=0) == -1 and grad(T=-1) == -2
     assert lib.smoe_adapter_grad_workspace_bytes(8192, 4096, 16, 1, 1) > 0 and lib.smoe_adapter_grad_workspace_bytes(64, 4096, 16, 1, 1) == 0
     assert grad(T=8192, C=4096) == -4 and grad(T=8192, C=4096, ws=one, ws_bytes=64) == -4
-    assert lib.smoe_adapter_groups(None, 4, 3, one, None) == -1 and lib.smoe_adapter_groups(one, 4, 0, one, None) == -2
+    order = lambda ids=one, T=4, R=3, off=one, ws=one, ws_bytes=1 << 20: lib.smoe_adapter_order(ids, T, R, one, off, ws, ws_bytes, None)
+    assert order(ids=None) == -1 and order(R=0) == -2 and order(off=None) == -1 and order(ws=None) == -4 and order(ws_bytes=16) == -4
+    assert order(R=2048) == -5 and order(ws=ctypes.c_void_p(264)) == -4
     assert lib.smoe_adapter_pack(one, 64, 8, 1, one, 2, 8, 9, 8, None, 1, None) == -2
     assert lib.smoe_adapter_pack(one, 64, 8, 1, None, 2, 8, 8, 8, None, 1, None) == -1
     assert low(T=0) == 0 and lib.smoe_last_error() == b""
