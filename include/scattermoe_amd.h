@@ -374,44 +374,30 @@ int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR,
 
 /*
  * Low-rank adapters of many requests beside a shared projection (no counterpart in the reference; rows pick their weights
- * by id as the rows of scattermoe/parallel_experts.py:148-182 do).  Row t carries adapter ids[t]; a row whose id lies outside
- * [0,R) carries none.
- *   smoe_adapter_low:      U[t,j] = scales[a] sum_c X[t,c] A[a,j,c], a = ids[t]; zeros without an adapter.  float32 (T,r).
- *   smoe_adapter_project:  Y[t,n] = sum_c X[t,c] W[n,c] (+ bias[n]) + sum_j U[t,j] B[a,n,j], rounded once.
- *   smoe_adapter_grad:     OUT[a,j,c] = sum over the rows t of adapter a of P[t,j] M[t,c]; zeros for an adapter without rows.
- *   smoe_adapter_order:    idx (T) and inclusive offsets off (R + 1): the rows by adapter, those without one last, each adapter's
- *                          in their order.  workspace: smoe_adapter_order_workspace_bytes(T, R) bytes, 16-byte aligned.
- *   smoe_adapter_pack:     DST[a,i,0..ld) = SRC[a,i,0..n2) and zeros: a copy with a contiguous last axis in rows of ld elements;
- *                          with `off` (inclusive offsets of n0 groups), matrices of groups without rows are left out.
- * The backward pass is smoe_adapter_low and smoe_adapter_project on the transposed factors and smoe_adapter_grad twice.
- * X (T,K) row stride sxm, M (T,C) row stride smm, Y (T,N) row stride sym: columns contiguous; A, B, W, OUT: any strides;
- * scales (R) float32 or NULL (ones).
- * idx / off: of smoe_adapter_order (smoe_adapter_grad reads the first R offsets,
- * and idx NULL if the rows are in order already).  smoe_adapter_low takes NULL for few rows.
- * planes, slots: (T, 2, r rounded up to 32) of `dtype`, U as the sum of two 16-bit parts, and smoe_adapter_slots(T, R) integers,
- * the rows of every 16 that share an adapter; written by smoe_adapter_low and read by the matrix-core tiles of
- * smoe_adapter_project, bf16 / fp16; both NULL for few rows and float32.  The tiles take operands whose rows are
- * 16-byte pieces (X, W, B and r a multiple of 8); everything else goes row by row or by a kernel for any layout.
+ * by id as the rows of scattermoe/parallel_experts.py:148-182 do).  Row t carries adapter a = ids[t]; a row whose id lies outside
+ * [0,R) carries none, and what an adapter holds, infinities included, meets its own rows only.
+ *   smoe_adapter_forward:   U[t] = scales[a] A[a] X[t]  (float32; zeros without an adapter)
+ *                           Y[t] = W X[t] (+ bias) + B[a] U[t], rounded once
+ *   smoe_adapter_backward:  V[t] = scales[a] B[a]^T DY[t],  DX[t] = W^T DY[t] + A[a]^T V[t],
+ *                           DA[a] = sum_t V[t] X[t]^T,  DB[a] = sum_t DY[t] U[t]^T  (zeros for an adapter without rows),
+ *                           DBIAS = sum_t DY[t]; DX, DA, DB, DBIAS may be NULL (not wanted)
+ * X (T,K) row stride sxm, columns contiguous; W (N,K), bias (N) or NULL, A (R,r,K), B (R,N,r), U (T,r), Y and DY (T,N), DX, DA, DB,
+ * DBIAS like X, A, B, bias: contiguous; scales (R) float32 or NULL (ones).
+ * idx (T), off (R + 1): written by smoe_adapter_forward for more than 64 rows (NULL up to there), the rows by adapter, each
+ * adapter's in their order, those without one last, and the inclusive offsets; read by smoe_adapter_backward.
+ * workspace: smoe_adapter_workspace_bytes(..., backward, dtype) bytes, 256-byte aligned; nothing in it is read before it is
+ * written; calls that overlap in time need one each.  Sums are float32, added in an order that the sizes and the ids fix.
  */
 #define SMOE_ADAPTER_MAX 2047
 #define SMOE_ADAPTER_MAX_RANK 512
-size_t smoe_adapter_order_workspace_bytes(int64_t T, int64_t R);
-int smoe_adapter_order(const int64_t* ids, int64_t T, int64_t R, int64_t* idx, int64_t* off, void* workspace, size_t workspace_bytes,
-                       void* stream);
-int smoe_adapter_pack(const void* SRC, int64_t s0, int64_t s1, int64_t s2, void* DST, int64_t n0, int64_t n1, int64_t n2,
-                      int64_t ld, const int64_t* off, int dtype, void* stream);
-size_t smoe_adapter_slots(int64_t T, int64_t R);
-int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
-                     const float* scales, const int64_t* idx, const int64_t* off, float* U, void* planes, int32_t* slots,
-                     int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream);
-int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
-                         const float* U, const void* planes, const int32_t* slots, const void* B, int64_t sbr, int64_t sbn, int64_t sbj,
-                         const int64_t* ids, void* Y, int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream);
-/* workspace: smoe_adapter_grad_workspace_bytes(T, C, r, R, dtype) bytes (0: none) */
-size_t smoe_adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype);
-int smoe_adapter_grad(const float* P, const void* M, int64_t smm, const int64_t* idx, const int64_t* off, void* OUT, int64_t soa,
-                      int64_t soj, int64_t soc, int64_t T, int64_t C, int64_t r, int64_t R, int dtype, void* workspace,
-                      size_t workspace_bytes, void* stream);
+size_t smoe_adapter_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int backward, int dtype);
+int smoe_adapter_forward(const void* X, int64_t sxm, const void* W, const void* bias, const void* A, const void* B,
+                         const int64_t* ids, const float* scales, int64_t* idx, int64_t* off, float* U, void* Y, int64_t T,
+                         int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int smoe_adapter_backward(const void* DY, const void* X, int64_t sxm, const void* W, const void* A, const void* B, const int64_t* ids,
+                          const float* scales, const int64_t* idx, const int64_t* off, const float* U, void* DX, void* DA, void* DB,
+                          void* DBIAS, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 
 #ifdef __cplusplus

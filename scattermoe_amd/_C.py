@@ -65,15 +65,10 @@ _SIGNATURES = {
     "smoe_routed_glu_mlp_workspace_bytes": (_sz, [_i64, _int, _i64, _i64]),
     "smoe_routed_glu_mlp": (_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64,
                                    _p, _i64, _i64, _p, _i64, _p, _i64, _int, _i64, _i64, _int, _int, _int, _int, _p, _sz, _p]),
-    "smoe_adapter_order_workspace_bytes": (_sz, [_i64, _i64]),
-    "smoe_adapter_order": (_int, [_p, _i64, _i64, _p, _p, _p, _sz, _p]),
-    "smoe_adapter_pack": (_int, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _int, _p]),
-    "smoe_adapter_slots": (_sz, [_i64, _i64]),
-    "smoe_adapter_low": (_int, [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _int, _p]),
-    "smoe_adapter_project": (_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64,
-                                    _i64, _i64, _i64, _i64, _i64, _int, _p]),
-    "smoe_adapter_grad_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
-    "smoe_adapter_grad": (_int, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _sz, _p]),
+    "smoe_adapter_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _int, _int]),
+    "smoe_adapter_forward": (_int, [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _p, _sz, _p]),
+    "smoe_adapter_backward": (_int, [_p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                                     _int, _p, _sz, _p]),
 }
 
 ERR_UNSUPPORTED = -6

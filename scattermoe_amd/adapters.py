@@ -13,13 +13,6 @@ from .kernels import ops
 _ID_TYPES = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
-def _forward(x, weight, bias, lora_a, lora_b, ids, scales):
-    """(y, u, order of the rows or None)"""
-    order = ops.adapter_order(ids, lora_a.size(0)) if x.size(0) > ops.ADAPTER_FEW_ROWS else None
-    u, parts = ops.adapter_low(x, lora_a, ids, scales, order)
-    return ops.adapter_project(x, weight, u, lora_b, ids, bias, parts, order), u, order
-
-
 class _ParallelAdapters(torch.autograd.Function):
     """y = x W^T (+ bias) + u B[a]^T with u = scales[a] x A[a]^T kept in float32.  The backward pass is the same two
     products on the transposed factors, v = scales[a] dy B[a] and dx = dy W + v A[a], and the sums of v x^T and dy u^T
@@ -27,39 +20,23 @@ class _ParallelAdapters(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, lora_a, lora_b, ids, scales):
-        y, u, order = _forward(x, weight, bias, lora_a, lora_b, ids, scales)
-        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scales, u, *(order or ()))
-        ctx.has_bias = bias is not None
+        y, u, order = ops.adapter_forward(x, weight, lora_a, lora_b, ids, scales, bias)
+        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scales, u, *order)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, lora_a, lora_b, ids, scales, u = ctx.saved_tensors[:7]
-        order = ctx.saved_tensors[7:] or None
-        need_x, need_w, need_b, need_la, need_lb = ctx.needs_input_grad[:5]
-        R = lora_a.size(0)
-        dx = dw = db = da = dlb = None
-        if not dy.is_contiguous():
-            dy = dy.contiguous()
-        if need_x or need_la:
-            v, parts = ops.adapter_low(dy, lora_b.transpose(1, 2), ids, scales, order)
-            if need_x:
-                dx = ops.adapter_project(dy, weight.t(), v, lora_a.transpose(1, 2), ids, None, parts, order)
-        if need_la or need_lb:
-            idx, off = order or ops.adapter_order(ids, R)
-            if need_la:
-                da = ops.adapter_grad(v, x, idx, off, R)
-            if need_lb:
-                dlb = ops.adapter_grad(u, dy, idx, off, R, transposed=True)
-        if need_w or (need_b and ctx.has_bias):
+        x, weight, lora_a, lora_b, ids, scales, u, *order = ctx.saved_tensors
+        need_x, need_w, need_bias, need_a, need_b = ctx.needs_input_grad[:5]
+        dx = da = db = dbias = dw = None
+        if need_x or need_a or need_b or need_bias:
+            dx, da, db, dbias = ops.adapter_backward(dy, x, weight, lora_a, lora_b, ids, scales, u, order, need_x, need_a,
+                                                     need_b, need_bias)
+        if need_w:
             rows = torch.full((1,), x.size(0), dtype=torch.int64, device=x.device)
-            if need_w:
-                dw = ops.group_bwd_W(DY=dy, X=x, expert_offsets=rows, E=1)[0][0].t()
-            if need_b and ctx.has_bias:
-                ones = torch.ones((x.size(0), 1), dtype=torch.float32, device=x.device)
-                db = ops.adapter_grad(ones, dy, None, rows, 1).view(-1)
-        return dx, dw, db, da, dlb, None, None
+            dw = ops.group_bwd_W(DY=dy.contiguous(), X=x, expert_offsets=rows, E=1)[0][0].t()
+        return dx, dw, dbias, da, db, None, None
 
 
 def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias=None):
@@ -109,7 +86,7 @@ def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias
     if trained and torch.is_grad_enabled():
         y = _ParallelAdapters.apply(x, weight, bias, lora_a, lora_b, ids, scales)
     else:
-        y = _forward(x, weight, bias, lora_a, lora_b, ids, scales)[0]
+        y = ops.adapter_forward(x, weight, lora_a, lora_b, ids, scales, bias)[0]
     return y if len(shape) == 2 else y.view(*shape[:-1], n)
 
 

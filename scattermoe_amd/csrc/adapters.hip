@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void adapter_grad_any_kernel(AdapterGradArgs a
   __shared__ float part[4][GRAD_RANKS][64];
   const int id = blockIdx.y, lane = lane_id(), wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane;
-  const int64_t lo = id ? a.off[id - 1] : 0, hi = a.off[id];
+  const int64_t lo = id ? a.off[id - 1] : 0, hi = a.off ? a.off[id] : a.T;
   for (int j0 = 0; j0 < a.r; j0 += GRAD_RANKS) {
     float acc[GRAD_RANKS] = {};
     for (int64_t i = lo + wave; i < hi; i += 4) {
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void adapter_grad_any_kernel(AdapterGradArgs a
       const float m = c < a.C ? to_f32(((const T*)a.M)[t * a.smm + c]) : 0.0f;
 #pragma unroll
       for (int j = 0; j < GRAD_RANKS; ++j)
-        if (j0 + j < a.r) acc[j] = fmaf(a.P[t * a.r + j0 + j], m, acc[j]);
+        if (j0 + j < a.r) acc[j] = fmaf(a.P ? a.P[t * a.r + j0 + j] : 1.0f, m, acc[j]);
     }
 #pragma unroll
     for (int j = 0; j < GRAD_RANKS; ++j) part[wave][j][lane] = acc[j];
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
   const int id = blockIdx.y / slices, slice = blockIdx.y % slices, lane = lane_id(), wave = threadIdx.x >> 6;
   const int l = lane & 15, q = lane >> 4, j0 = blockIdx.z * JT * 16;
   const int c0 = blockIdx.x * COLS + l * PER, c = min(c0, a.C - PER);        // (the last columns: once more, by the lane before them)
-  const int64_t first = id ? a.off[id - 1] : 0, count = a.off[id] - first;
+  const int64_t first = id ? a.off[id - 1] : 0, count = (a.off ? a.off[id] : a.T) - first;
   const int64_t lo = first + count * slice / slices, hi = first + count * (slice + 1) / slices;
   f32x4 acc[JT][PER];
 #pragma unroll
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
     for (int u = 0; u < SIDE; ++u) {
       m[u] = __builtin_bit_cast(V, load_piece<T, false>((const T*)a.M + next[u] * a.smm + c));
 #pragma unroll
-      for (int j = 0; j < JT; ++j) p[u][j] = a.P[next[u] * a.r + min(j0 + 16 * j + l, a.r - 1)];
+      for (int j = 0; j < JT; ++j) p[u][j] = a.P ? a.P[next[u] * a.r + min(j0 + 16 * j + l, a.r - 1)] : 1.0f;
     }
     if (s + GRAD_NW * 4 * SIDE < hi) fetch(s + GRAD_NW * 4 * SIDE);
     __builtin_amdgcn_sched_barrier(0);
@@ -389,10 +389,11 @@ static constexpr int GRAD_WGS = 1024, GRAD_MIN_ROWS = 128;
 static int grad_tiles(int64_t C, int dtype) { return (int)cdiv64(C, dtype == SMOE_F32 ? 64 : 128); }
 static int grad_ranks(int64_t r) { return r <= 16 ? 1 : 2; }
 static int grad_slices(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
+  if (C < (dtype == SMOE_F32 ? 4 : 8)) return 1;
   const int64_t wgs = grad_tiles(C, dtype) * R * cdiv64(r, 16 * grad_ranks(r));
   return (int)std::max<int64_t>(1, std::min<int64_t>({GRAD_WGS / wgs, T / R / GRAD_MIN_ROWS, GRAD_MAX_SLICES, 65535 / R}));
 }
-size_t adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
+static size_t grad_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
   const int slices = grad_slices(T, C, r, R, dtype);
   return slices > 1 ? (size_t)slices * R * r * C * sizeof(float) : 0;
 }
@@ -412,31 +413,160 @@ static int grad_t(const AdapterGradArgs& a, int slices, float* partial, hipStrea
   return launch_status("adapter_grad_any_kernel");
 }
 
-int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st) {
+// ---- the launches of a call, over one workspace ------------------------------------------------------------------------
+static int low(const AdapterLowArgs& a, int dtype, hipStream_t st) {
   return dtype == SMOE_F32 ? low_t<float>(a, st) : dtype == SMOE_BF16 ? low_t<bf16_t>(a, st) : low_t<f16_t>(a, st);
 }
-int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st) {
+static int project(const AdapterProjectArgs& a, int dtype, hipStream_t st) {
   int rc = 0;
   if (try_adapter_tiles(a, dtype, st, rc)) return rc;
   return dtype == SMOE_F32 ? project_t<float>(a, st) : dtype == SMOE_BF16 ? project_t<bf16_t>(a, st) : project_t<f16_t>(a, st);
 }
-int launch_adapter_grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st) {
+static int grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st) {
   const int slices = workspace ? grad_slices(a.T, a.C, a.r, a.R, dtype) : 1;
   float* p = (float*)workspace;
   return dtype == SMOE_F32 ? grad_t<float>(a, slices, p, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(a, slices, p, st) : grad_t<f16_t>(a, slices, p, st);
 }
 template <typename T>
 static int pack_t(const AdapterPackArgs& a, hipStream_t st) {
-  if ((a.n1 + 63) / 64 > 65535 || a.n0 > 65535) { set_error("smoe_adapter_pack: too many rows"); return SMOE_ERR_RANGE; }
+  if ((a.n1 + 63) / 64 > 65535) { set_error("adapters: at most 2^22 columns in this layout"); return SMOE_ERR_RANGE; }
   hipLaunchKernelGGL(adapter_pack_kernel<T>, dim3((a.ld + 63) / 64, (a.n1 + 63) / 64, a.n0), dim3(256), 0, st, a);
   return launch_status("adapter_pack_kernel");
 }
-int launch_adapter_pack(const AdapterPackArgs& a, int dtype, hipStream_t st) {
+static int pack(const AdapterPackArgs& a, int dtype, hipStream_t st) {
   return dtype == SMOE_F32 ? pack_t<float>(a, st) : dtype == SMOE_BF16 ? pack_t<bf16_t>(a, st) : pack_t<f16_t>(a, st);
 }
-int launch_adapter_groups(const int64_t* ids, int64_t T, int R, int* out, hipStream_t st) {
-  hipLaunchKernelGGL(adapter_groups_kernel, dim3((unsigned)cdiv64(T, 256)), dim3(256), 0, st, ids, T, R, out);
-  return launch_status("adapter_groups_kernel");
+
+// Pieces of the workspace, each at a multiple of 256 bytes.  Without one (a dry run) it only counts, and nothing is launched.
+struct Space {
+  char* base;
+  size_t used = 0;
+  bool dry() const { return base == nullptr; }
+  template <typename T> T* take(int64_t n) {
+    T* p = dry() ? nullptr : (T*)(base + used);
+    used += ((size_t)n * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+  char* bytes(int64_t n) { return take<char>(n); }
+};
+static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+static int64_t width(int dtype) { return dtype == SMOE_F32 ? 4 : 2; }
+static int pieces(int dtype) { return dtype == SMOE_F32 ? 4 : 8; }
+
+static int order_rows(const int64_t* ids, int64_t T, int R, int64_t* idx, int64_t* off, Space& s, hipStream_t st) {
+  int64_t* eid = s.take<int64_t>(T);
+  int* groups = s.take<int>(T);
+  char* ws = s.bytes((int64_t)route_workspace_bytes(T, R + 1));
+  if (s.dry()) return 0;
+  hipLaunchKernelGGL(adapter_groups_kernel, dim3((unsigned)cdiv64(T, 256)), dim3(256), 0, st, ids, T, R, groups);
+  if (int rc = launch_status("adapter_groups_kernel")) return rc;
+  return launch_route(groups, SMOE_I32, T, R + 1, eid, idx, off, ws, st);
+}
+
+// Y = X W^T (+ bias) + U B[a]^T with U = s A[a] X, for factors in any order: the product both ways.  `off` (with the rows in order):
+// factors whose contraction is not contiguous, or not whole pieces, are copied, those of adapters that have rows.
+struct Product {
+  const void* X; int64_t sxm;
+  const void* W; int64_t swn, swk;
+  const void* bias;
+  const void* A; int64_t sar, saj, sak;
+  const void* B; int64_t sbr, sbn, sbj;
+  void* Y;                                           // NULL: U alone
+  float* U;
+  int64_t K, N;
+};
+// Up to so many multiply-adds a strided factor is looked up element by element: a copy's launch costs more
+static constexpr int64_t LOOK_UP = 1 << 22;
+static int product(const AdapterCall& c, Product p, const int64_t* idx, const int64_t* off, Space& s, hipStream_t st) {
+  const bool many = c.T > ADAPTER_FEW_ROWS, tiles = many && c.dtype != SMOE_F32 && p.K >= 8;
+  const int64_t w = width(c.dtype);
+  auto copy = [&](const void*& src, int64_t& s0, int64_t& s1, int64_t& s2, int64_t n0, int64_t n1, int64_t n2, int64_t ld) {
+    char* dst = s.bytes(n0 * n1 * ld * w);
+    const AdapterPackArgs a{src, s0, s1, s2, dst, (int)ld, n0 == 1 ? nullptr : off, (int)n0, (int)n1, (int)n2};
+    src = dst;
+    s0 = n1 * ld, s1 = ld, s2 = 1;
+    return s.dry() ? 0 : pack(a, c.dtype, st);
+  };
+  if (p.sak != 1 && p.K >= pieces(c.dtype) && (tiles || c.T * p.K * c.r > LOOK_UP))
+    if (int rc = copy(p.A, p.sar, p.saj, p.sak, c.R, c.r, p.K, p.K)) return rc;
+  const int rp = (c.r + 31) / 32 * 32;
+  char* planes = tiles ? s.bytes(c.T * 2 * rp * w) : nullptr;
+  int* slots = tiles ? s.take<int>(adapter_fragments(c.T, c.R) * 17) : nullptr;
+  if (!s.dry()) {
+    const AdapterLowArgs a{p.X, p.sxm, p.A, p.sar, p.saj, p.sak, c.ids, c.scales, many ? idx : nullptr, many ? off : nullptr, p.U, planes, rp, slots,
+                           c.T, (int)p.K, c.r, c.R};
+    if (int rc = low(a, c.dtype, st)) return rc;
+  }
+  if (p.Y == nullptr) return 0;
+  int64_t zero = 0, one = 1;
+  if (tiles) {
+    const int64_t k8 = up8(p.K);
+    if (p.sbj != 1 || c.r % 8)
+      if (int rc = copy(p.B, p.sbr, p.sbn, p.sbj, c.R, p.N, c.r, up8(c.r))) return rc;
+    const bool w_tr = p.swn == 1 && p.swk != 1;
+    if (p.K % 8 || (w_tr && p.N % 8))
+      if (int rc = copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, k8)) return rc;
+    if (p.K % 8) {
+      if (int rc = copy(p.X, zero, p.sxm, one, 1, c.T, p.K, k8)) return rc;
+      p.K = k8;
+    }
+  } else if (p.swk != 1 && p.K >= pieces(c.dtype)) {
+    if (int rc = copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, p.K)) return rc;
+  }
+  if (s.dry()) return 0;
+  const AdapterProjectArgs a{p.X, p.sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
+                             c.T, (int)p.K, (int)p.N, c.r, c.R};
+  return project(a, c.dtype, st);
+}
+
+static int forward(const AdapterCall& c, Space& s, hipStream_t st) {
+  if (c.T > ADAPTER_FEW_ROWS)
+    if (int rc = order_rows(c.ids, c.T, c.R, c.idx, c.off, s, st)) return rc;
+  // (a dry run asks for all that the call may want)
+  return product(c, Product{c.X, c.sxm, c.W, c.K, 1, c.bias, c.A, c.r * c.K, c.K, 1, c.B, c.N * c.r, c.r, 1, s.dry() ? &s : c.Y, c.U, c.K, c.N},
+                 c.idx, c.off, s, st);
+}
+
+static int backward(const AdapterCall& c, Space& s, hipStream_t st) {
+  const bool dry = s.dry(), any = dry || c.DA || c.DB;
+  const int64_t *idx = c.idx, *off = c.off;
+  if (c.T <= ADAPTER_FEW_ROWS && any) {
+    int64_t* own = s.take<int64_t>(c.T + c.R + 1);
+    if (int rc = order_rows(c.ids, c.T, c.R, own, own + c.T, s, st)) return rc;
+    idx = own, off = own + c.T;
+  }
+  if (dry || c.DX || c.DA) {
+    float* V = s.take<float>(c.T * c.r);
+    const Product p{c.DY, c.N, c.W, 1, c.K, nullptr, c.B, c.N * c.r, 1, c.r, c.A, c.r * c.K, 1, c.K, dry ? &s : c.DX, V, c.N, c.K};
+    if (int rc = product(c, p, idx, off, s, st)) return rc;
+    void* ws = s.bytes((int64_t)grad_bytes(c.T, c.K, c.r, c.R, c.dtype));
+    if (c.DA && !dry) {
+      const AdapterGradArgs g{V, c.X, c.sxm, idx, off, c.DA, c.r * c.K, c.K, 1, c.T, (int)c.K, c.r, c.R};
+      if (int rc = grad(g, c.dtype, ws, st)) return rc;
+    }
+  }
+  void* ws = s.bytes((int64_t)grad_bytes(c.T, c.N, c.r, c.R, c.dtype));
+  if (c.DB && !dry) {
+    const AdapterGradArgs g{c.U, c.DY, c.N, idx, off, c.DB, c.N * c.r, 1, c.r, c.T, (int)c.N, c.r, c.R};
+    if (int rc = grad(g, c.dtype, ws, st)) return rc;
+  }
+  ws = s.bytes((int64_t)grad_bytes(c.T, c.N, 1, 1, c.dtype));
+  if (c.DBIAS && !dry) return grad(AdapterGradArgs{nullptr, c.DY, c.N, nullptr, nullptr, c.DBIAS, 0, 0, 1, c.T, (int)c.N, 1, 1}, c.dtype, ws, st);
+  return 0;
+}
+
+size_t adapter_workspace_bytes(const AdapterCall& call, bool back) {
+  AdapterCall c{};                                           // (its sizes alone)
+  c.T = call.T, c.K = call.K, c.N = call.N, c.r = call.r, c.R = call.R, c.dtype = call.dtype;
+  Space s{nullptr};
+  if (back) backward(c, s, nullptr);
+  else forward(c, s, nullptr);
+  return s.used;
+}
+int launch_adapter_call(const AdapterCall& c, bool back, void* workspace, hipStream_t st) {
+  static char none;
+  Space s{workspace ? (char*)workspace : &none};
+  return back ? backward(c, s, st) : forward(c, s, st);
 }
 
 }  // namespace smoe

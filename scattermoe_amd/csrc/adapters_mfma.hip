@@ -63,7 +63,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
     for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
   for (int k0 = 0; k0 < a.rp; k0 += 32) {
     const int k = k0 + 8 * lq;
-    const bool inside = k < a.r;                             // (r is a multiple of 8 here; U is padded with zeros to rp)
+    const bool inside = k < a.r;                             // (rows of B end with a whole piece, those of U with a whole step, in zeros)
     // (a fragment's operands are on their way while the one before is multiplied)
     i32x4 u[2][2], bv[2][2 * TL::FN];
     auto load = [&](int i, int p) {
@@ -153,11 +153,11 @@ static int dispatch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-// Whole pieces of 16 bytes in all operands, and lane offsets of 32 bits into X and W
+// Whole pieces of 16 bytes in all operands (rows of B padded with zeros to them), and lane offsets of 32 bits into X and W
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc) {
   if ((dtype != SMOE_BF16 && dtype != SMOE_F16) || a.planes == nullptr || a.slots == nullptr) return false;
   if (a.K < 8 || a.K % 8 != 0 || a.sxm % 8 != 0 || !aligned16(a.X) || !aligned16(a.W)) return false;
-  if (a.r % 8 != 0 || a.sbj != 1 || a.sbn % 8 != 0 || a.sbr % 8 != 0 || !aligned16(a.B) || a.rp % 32 != 0 || !aligned16(a.planes)) return false;
+  if (a.sbn < (a.r + 7) / 8 * 8 || a.sbj != 1 || a.sbn % 8 != 0 || a.sbr % 8 != 0 || !aligned16(a.B) || a.rp % 32 != 0 || !aligned16(a.planes)) return false;
   bool w_tr;
   if (a.swk == 1 && a.swn % 8 == 0) w_tr = false;
   else if (a.swn == 1 && a.swk % 8 == 0 && a.N % 8 == 0) w_tr = true;

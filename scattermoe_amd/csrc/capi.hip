@@ -411,90 +411,46 @@ static int adapter_checks(const char* who, int64_t T, int64_t K, int64_t N, int6
   return 0;
 }
 
-// (T 64-bit sorted groups, T 32-bit groups, the routing's own workspace)
-static size_t order_bytes(int64_t T) { return ((size_t)T * 12 + 15) / 16 * 16; }
-size_t smoe_adapter_order_workspace_bytes(int64_t T, int64_t R) {
-  if (T <= 0 || R <= 0 || R > SMOE_ADAPTER_MAX) return 0;
-  return order_bytes(T) + route_workspace_bytes(T, (int)R + 1);
+size_t smoe_adapter_workspace_bytes(int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int backward, int dtype) {
+  if (T <= 0 || K <= 0 || adapter_checks("smoe_adapter_workspace_bytes", T, K, N, r, R, dtype)) return 0;
+  AdapterCall c{};
+  c.T = T, c.K = K, c.N = N, c.r = (int)r, c.R = (int)R, c.dtype = dtype;
+  return adapter_workspace_bytes(c, backward != 0);
 }
 
-int smoe_adapter_order(const int64_t* ids, int64_t T, int64_t R, int64_t* idx, int64_t* off, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_order", T, 0, 0, 1, R, SMOE_F32)) return rc;
-  if (!off || (T > 0 && (!ids || !idx))) { set_error("smoe_adapter_order: NULL pointer"); return SMOE_ERR_NULL; }
-  const size_t need = smoe_adapter_order_workspace_bytes(T, R);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
-    set_error("smoe_adapter_order: a workspace of %zu bytes, 16-byte aligned, is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+static int adapter_call(const char* who, const AdapterCall& c, bool back, void* workspace, size_t workspace_bytes, void* stream) {
+  if (c.T > ADAPTER_FEW_ROWS && (!c.idx || !c.off)) { set_error("%s: idx and off are needed for more than %d rows", who, ADAPTER_FEW_ROWS); return SMOE_ERR_NULL; }
+  const size_t need = adapter_workspace_bytes(c, back);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) {
+    set_error("%s: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
     return SMOE_ERR_WORKSPACE;
   }
-  int64_t* eid = (int64_t*)workspace;
-  int* groups = (int*)(eid + T);
-  if (T > 0) {
-    if (int rc = launch_adapter_groups(ids, T, (int)R, groups, (hipStream_t)stream)) return rc;
-  }
-  return launch_route(groups, SMOE_I32, T, (int)R + 1, eid, idx, off, (char*)workspace + order_bytes(T), (hipStream_t)stream);
+  return launch_adapter_call(c, back, workspace, (hipStream_t)stream);
 }
 
-int smoe_adapter_pack(const void* SRC, int64_t s0, int64_t s1, int64_t s2, void* DST, int64_t n0, int64_t n1, int64_t n2,
-                      int64_t ld, const int64_t* off, int dtype, void* stream) {
+int smoe_adapter_forward(const void* X, int64_t sxm, const void* W, const void* bias, const void* A, const void* B,
+                         const int64_t* ids, const float* scales, int64_t* idx, int64_t* off, float* U, void* Y, int64_t T,
+                         int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = 0;
-  if (!dtype_ok(dtype)) { set_error("smoe_adapter_pack: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
-  if (n0 < 0 || n1 < 0 || n2 < 0 || ld < n2) { set_error("smoe_adapter_pack: bad sizes"); return SMOE_ERR_SHAPE; }
-  if (n0 > 65535 || n1 > 0x3fffffLL || ld > 0x3fffffffLL) { set_error("smoe_adapter_pack: at most 65535 matrices of 2^22 - 1 rows"); return SMOE_ERR_RANGE; }
-  if (n0 == 0 || n1 == 0 || ld == 0) return 0;
-  if (!SRC || !DST) { set_error("smoe_adapter_pack: NULL pointer"); return SMOE_ERR_NULL; }
-  return launch_adapter_pack(AdapterPackArgs{SRC, s0, s1, s2, DST, (int)ld, off, (int)n0, (int)n1, (int)n2}, dtype, (hipStream_t)stream);
-}
-
-size_t smoe_adapter_slots(int64_t T, int64_t R) { return T <= 0 || R <= 0 || R > SMOE_ADAPTER_MAX ? 0 : (size_t)adapter_fragments(T, R) * 17; }
-
-int smoe_adapter_low(const void* X, int64_t sxm, const void* A, int64_t sar, int64_t saj, int64_t sak, const int64_t* ids,
-                     const float* scales, const int64_t* idx, const int64_t* off, float* U, void* planes, int32_t* slots,
-                     int64_t T, int64_t K, int64_t r, int64_t R, int dtype, void* stream) {
-  g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_low", T, K, 0, r, R, dtype)) return rc;
-  if (T == 0) return 0;
-  if ((K > 0 && (!X || !A)) || !ids || !U) { set_error("smoe_adapter_low: NULL pointer"); return SMOE_ERR_NULL; }
-  if (!idx != !off || !planes != !slots || (planes && (!idx || dtype == SMOE_F32 || sak != 1 || K < 8))) {
-    set_error("smoe_adapter_low: two parts need rows in order, 16-bit types and a contiguous contraction of 8 and more");
-    return SMOE_ERR_UNSUPPORTED;
-  }
-  return launch_adapter_low(AdapterLowArgs{X, sxm, A, sar, saj, sak, ids, scales, idx, off, U, planes, (int)((r + 31) / 32 * 32), slots, T, (int)K,
-                                           (int)r, (int)R}, dtype, (hipStream_t)stream);
-}
-
-int smoe_adapter_project(const void* X, int64_t sxm, const void* W, int64_t swn, int64_t swk, const void* bias, int64_t sb,
-                         const float* U, const void* planes, const int32_t* slots, const void* B, int64_t sbr, int64_t sbn, int64_t sbj,
-                         const int64_t* ids, void* Y, int64_t sym, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* stream) {
-  g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_project", T, K, N, r, R, dtype)) return rc;
+  if (int rc = adapter_checks("smoe_adapter_forward", T, K, N, r, R, dtype)) return rc;
+  if (K == 0) { set_error("smoe_adapter_forward: bad sizes"); return SMOE_ERR_SHAPE; }
   if (T == 0 || N == 0) return 0;
-  if ((K > 0 && (!X || !W)) || !U || !B || !ids || !Y) { set_error("smoe_adapter_project: NULL pointer"); return SMOE_ERR_NULL; }
-  if (!planes != !slots) { set_error("smoe_adapter_project: planes and slots go together"); return SMOE_ERR_NULL; }
-  return launch_adapter_project(AdapterProjectArgs{X, sxm, W, swn, swk, bias, sb, U, planes, (int)((r + 31) / 32 * 32), slots, B, sbr, sbn, sbj,
-                                                   ids, Y, sym, T, (int)K, (int)N, (int)r, (int)R}, dtype, (hipStream_t)stream);
+  if (!X || !W || !A || !B || !ids || !U || !Y) { set_error("smoe_adapter_forward: NULL pointer"); return SMOE_ERR_NULL; }
+  AdapterCall c{X, sxm, W, bias, A, B, ids, scales, idx, off, U, Y, nullptr, nullptr, nullptr, nullptr, nullptr, T, K, N, (int)r, (int)R, dtype};
+  return adapter_call("smoe_adapter_forward", c, false, workspace, workspace_bytes, stream);
 }
 
-size_t smoe_adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
-  if (T <= 0 || C <= 0 || r <= 0 || R <= 0 || !dtype_ok(dtype)) return 0;
-  return adapter_grad_workspace_bytes(T, C, r, R, dtype);
-}
-
-int smoe_adapter_grad(const float* P, const void* M, int64_t smm, const int64_t* idx, const int64_t* off, void* OUT, int64_t soa,
-                      int64_t soj, int64_t soc, int64_t T, int64_t C, int64_t r, int64_t R, int dtype, void* workspace,
-                      size_t workspace_bytes, void* stream) {
+int smoe_adapter_backward(const void* DY, const void* X, int64_t sxm, const void* W, const void* A, const void* B, const int64_t* ids,
+                          const float* scales, const int64_t* idx, const int64_t* off, const float* U, void* DX, void* DA, void* DB,
+                          void* DBIAS, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   g_err[0] = 0;
-  if (int rc = adapter_checks("smoe_adapter_grad", T, C, 0, r, R, dtype)) return rc;
-  if (C == 0) return 0;
-  if (T == 0 || !P || !M || !off || !OUT) { set_error("smoe_adapter_grad: NULL pointer"); return SMOE_ERR_NULL; }
-  const size_t need = adapter_grad_workspace_bytes(T, C, r, R, dtype);
-  if (need > 0 && (!workspace || workspace_bytes < need)) {
-    set_error("smoe_adapter_grad: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
-    return SMOE_ERR_WORKSPACE;
-  }
-  return launch_adapter_grad(AdapterGradArgs{P, M, smm, idx, off, OUT, soa, soj, soc, T, (int)C, (int)r, (int)R}, dtype,
-                             need ? workspace : nullptr, (hipStream_t)stream);
+  if (int rc = adapter_checks("smoe_adapter_backward", T, K, N, r, R, dtype)) return rc;
+  if (T == 0 || K == 0 || N == 0) { set_error("smoe_adapter_backward: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (!DY || !X || !W || !A || !B || !ids || !U) { set_error("smoe_adapter_backward: NULL pointer"); return SMOE_ERR_NULL; }
+  AdapterCall c{X, sxm, W, nullptr, A, B, ids, scales, (int64_t*)idx, (int64_t*)off, (float*)U, nullptr, DY, DX, DA, DB, DBIAS, T, K, N,
+                (int)r, (int)R, dtype};
+  return adapter_call("smoe_adapter_backward", c, true, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

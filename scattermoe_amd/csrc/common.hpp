@@ -400,9 +400,9 @@ struct AdapterProjectArgs {
   int K, N, r, R;
 };
 struct AdapterGradArgs {
-  const float* P;                                    // (T, r)
+  const float* P;                                    // (T, r) or NULL (ones)
   const void* M; int64_t smm;                        // (T, C), columns contiguous
-  const int64_t* idx; const int64_t* off;            // rows by adapter (NULL idx: in order), inclusive offsets (R or more)
+  const int64_t* idx; const int64_t* off;            // rows by adapter (NULL idx: in order), inclusive offsets (NULL: one, all rows)
   void* OUT; int64_t soa, soj, soc;                  // (R, r, C)
   int64_t T;
   int C, r, R;
@@ -415,13 +415,24 @@ struct AdapterPackArgs {
 };
 // Fragments of 16 rows, each of one adapter, that T rows of R adapters (and of none) can make
 static inline int64_t adapter_fragments(int64_t T, int64_t R) { return max_tiles(T, (int)R + 1, 16); }
-int launch_adapter_low(const AdapterLowArgs& a, int dtype, hipStream_t st);
-int launch_adapter_project(const AdapterProjectArgs& a, int dtype, hipStream_t st);
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc);       // csrc/adapters_mfma.hip
-size_t adapter_grad_workspace_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype);
-int launch_adapter_grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st);
-int launch_adapter_pack(const AdapterPackArgs& a, int dtype, hipStream_t st);
-int launch_adapter_groups(const int64_t* ids, int64_t T, int R, int* out, hipStream_t st);
+// A call, forward or backward: contiguous tensors, but for the row stride of X
+static constexpr int ADAPTER_FEW_ROWS = 64;          // up to so many rows the products go row by row, without an order
+struct AdapterCall {
+  const void* X; int64_t sxm;                        // (T, K)
+  const void* W;                                     // (N, K)
+  const void* bias;                                  // (N) or NULL
+  const void* A; const void* B;                      // (R, r, K), (R, N, r)
+  const int64_t* ids; const float* scales;           // (T), (R) or NULL
+  int64_t* idx; int64_t* off;                        // rows by adapter, those without one last, offsets (R + 1): more than few rows
+  float* U;                                          // (T, r)
+  void* Y;                                           // forward: (T, N)
+  const void* DY; void* DX; void* DA; void* DB; void* DBIAS;       // backward: gradients, NULL if not wanted
+  int64_t T, K, N;
+  int r, R, dtype;
+};
+size_t adapter_workspace_bytes(const AdapterCall& c, bool back);
+int launch_adapter_call(const AdapterCall& c, bool back, void* workspace, hipStream_t st);
 
 int launch_s2s_generic(const S2SArgs& a, int dtype, hipStream_t st);
 int launch_xty_generic(const XtYArgs& a, int dtype, hipStream_t st);

@@ -27,13 +27,22 @@ def _routed_layer_bytes(T, k, d, F):
 
 
 @functools.lru_cache(maxsize=1024)
-def _adapter_order_bytes(T, R):
-    return _C.load().smoe_adapter_order_workspace_bytes(T, R)
+def _adapter_bytes(T, K, N, r, R, backward, code):
+    return _C.load().smoe_adapter_workspace_bytes(T, K, N, r, R, backward, code)
 
 
-@functools.lru_cache(maxsize=1024)
-def _adapter_grad_bytes(T, C, r, R, code):
-    return _C.load().smoe_adapter_grad_workspace_bytes(T, C, r, R, code)
+def _whole(t):
+    """t, contiguous and at a multiple of 16 bytes."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _whole_rows(x):
+    """x (T, K) with contiguous columns and rows that start where 16-byte pieces can."""
+    if x.stride(1) == 1 and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return _whole(x)
 
 
 class HipBackend:
@@ -343,58 +352,36 @@ class HipBackend:
         _C.check(rc, "smoe_routed_glu_mlp")
 
     @staticmethod
-    def adapter_order(ids, R, idx, off):
-        _C.require_gpu(ids, "adapter_order")
-        T = ids.numel()
-        need = _adapter_order_bytes(T, R)
-        ws = torch.empty(need, dtype=torch.uint8, device=ids.device)
-        with _C.on_device(ids.device):
-            rc = _C.load().smoe_adapter_order(_C.ptr(ids), T, R, _C.ptr(idx), _C.ptr(off), _C.ptr(ws), need,
-                                              _C.stream_ptr(ids.device))
-        _C.check(rc, "smoe_adapter_order")
-
-    @staticmethod
-    def adapter_pack(src, dst, off):
-        _C.require_gpu(src, "adapter_pack")
-        with _C.on_device(src.device):
-            rc = _C.load().smoe_adapter_pack(_C.ptr(src), *src.stride(), _C.ptr(dst), *src.shape, dst.size(2), _C.ptr(off),
-                                             _C.float_code(src.dtype), _C.stream_ptr(src.device))
-        _C.check(rc, "smoe_adapter_pack")
-
-    @staticmethod
-    def adapter_low(X, A, ids, scales, idx, off, U, planes, slots):
-        _C.require_gpu(X, "adapter_low")
-        lib = _C.load()
+    def adapter_forward(X, W, bias, A, B, ids, scales, idx, off, U, Y):
+        _C.require_gpu(X, "adapter_forward")
+        X, W, A, B = _whole_rows(X), _whole(W), _whole(A), _whole(B)
+        bias = None if bias is None else _whole(bias)
+        T, K = X.shape
+        R, N, r = B.shape
+        code = _C.float_code(X.dtype)
+        need = _adapter_bytes(T, K, N, r, R, 0, code)
+        ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
         with _C.on_device(X.device):
-            rc = lib.smoe_adapter_low(_C.ptr(X), X.stride(0), _C.ptr(A), A.stride(0), A.stride(1), A.stride(2), _C.ptr(ids),
-                                      _C.ptr(scales), _C.ptr(idx), _C.ptr(off), _C.ptr(U), _C.ptr(planes), _C.ptr(slots),
-                                      X.size(0), X.size(1), A.size(1), A.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
-        _C.check(rc, "smoe_adapter_low")
+            rc = _C.load().smoe_adapter_forward(
+                _C.ptr(X), X.stride(0), _C.ptr(W), _C.ptr(bias), _C.ptr(A), _C.ptr(B), _C.ptr(ids), _C.ptr(scales), _C.ptr(idx),
+                _C.ptr(off), _C.ptr(U), _C.ptr(Y), T, K, N, r, R, code, _C.ptr(ws), need, _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_adapter_forward")
 
     @staticmethod
-    def adapter_project(X, W, bias, U, planes, slots, B, ids, Y):
-        _C.require_gpu(X, "adapter_project")
-        lib = _C.load()
+    def adapter_backward(DY, X, W, A, B, ids, scales, idx, off, U, DX, DA, DB, DBIAS):
+        _C.require_gpu(X, "adapter_backward")
+        DY, X, W, A, B = _whole(DY), _whole_rows(X), _whole(W), _whole(A), _whole(B)
+        T, K = X.shape
+        R, N, r = B.shape
+        code = _C.float_code(X.dtype)
+        need = _adapter_bytes(T, K, N, r, R, 1, code)
+        ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
         with _C.on_device(X.device):
-            rc = lib.smoe_adapter_project(
-                _C.ptr(X), X.stride(0), _C.ptr(W), W.stride(0), W.stride(1), _C.ptr(bias),
-                bias.stride(0) if bias is not None else 0, _C.ptr(U), _C.ptr(planes), _C.ptr(slots), _C.ptr(B), B.stride(0), B.stride(1),
-                B.stride(2), _C.ptr(ids), _C.ptr(Y), Y.stride(0), X.size(0), X.size(1), W.size(0),
-                U.size(1), B.size(0), _C.float_code(X.dtype), _C.stream_ptr(X.device))
-        _C.check(rc, "smoe_adapter_project")
-
-    @staticmethod
-    def adapter_grad(P, M, idx, off, out):
-        _C.require_gpu(M, "adapter_grad")
-        lib = _C.load()
-        code, T, C, r, R = _C.float_code(M.dtype), M.size(0), M.size(1), P.size(1), out.size(0)
-        need = _adapter_grad_bytes(T, C, r, R, code)
-        ws = torch.empty(need, dtype=torch.uint8, device=M.device) if need else None
-        with _C.on_device(M.device):
-            rc = lib.smoe_adapter_grad(_C.ptr(P), _C.ptr(M), M.stride(0), _C.ptr(idx), _C.ptr(off), _C.ptr(out),
-                                       out.stride(0), out.stride(1), out.stride(2), T, C, r, R, code, _C.ptr(ws), need,
-                                       _C.stream_ptr(M.device))
-        _C.check(rc, "smoe_adapter_grad")
+            rc = _C.load().smoe_adapter_backward(
+                _C.ptr(DY), _C.ptr(X), X.stride(0), _C.ptr(W), _C.ptr(A), _C.ptr(B), _C.ptr(ids), _C.ptr(scales), _C.ptr(idx),
+                _C.ptr(off), _C.ptr(U), _C.ptr(DX), _C.ptr(DA), _C.ptr(DB), _C.ptr(DBIAS), T, K, N, r, R, code, _C.ptr(ws), need,
+                _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_adapter_backward")
 
 
 _backend = HipBackend()
@@ -511,42 +498,26 @@ def _routed_glu_mlp_op(x: torch.Tensor, wr: torch.Tensor, w1: torch.Tensor, b1: 
     _backend.routed_glu_mlp(x, wr, w1, b1, w2, b2, out, logits, k, renormalize, act)
 
 
-@torch.library.custom_op("scattermoe::adapter_order", mutates_args={"idx", "off"})
-def _adapter_order_op(ids: torch.Tensor, R: int, idx: torch.Tensor, off: torch.Tensor) -> None:
-    _backend.adapter_order(ids, R, idx, off)
+@torch.library.custom_op("scattermoe::adapter_forward", mutates_args={"idx", "off", "U", "Y"})
+def _adapter_forward_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], A: torch.Tensor, B: torch.Tensor,
+                        ids: torch.Tensor, scales: Optional[torch.Tensor], idx: Optional[torch.Tensor],
+                        off: Optional[torch.Tensor], U: torch.Tensor, Y: torch.Tensor) -> None:
+    _backend.adapter_forward(X, W, bias, A, B, ids, scales, idx, off, U, Y)
 
 
-@torch.library.custom_op("scattermoe::adapter_pack", mutates_args={"dst"})
-def _adapter_pack_op(src: torch.Tensor, dst: torch.Tensor, off: Optional[torch.Tensor]) -> None:
-    _backend.adapter_pack(src, dst, off)
-
-
-@torch.library.custom_op("scattermoe::adapter_low", mutates_args={"U", "planes", "slots"})
-def _adapter_low_op(X: torch.Tensor, A: torch.Tensor, ids: torch.Tensor, scales: Optional[torch.Tensor],
-                    idx: Optional[torch.Tensor], off: Optional[torch.Tensor], U: torch.Tensor,
-                    planes: Optional[torch.Tensor], slots: Optional[torch.Tensor]) -> None:
-    _backend.adapter_low(X, A, ids, scales, idx, off, U, planes, slots)
-
-
-@torch.library.custom_op("scattermoe::adapter_project", mutates_args={"Y"})
-def _adapter_project_op(X: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor], U: torch.Tensor,
-                        planes: Optional[torch.Tensor], slots: Optional[torch.Tensor], B: torch.Tensor, ids: torch.Tensor,
-                        Y: torch.Tensor) -> None:
-    _backend.adapter_project(X, W, bias, U, planes, slots, B, ids, Y)
-
-
-@torch.library.custom_op("scattermoe::adapter_grad", mutates_args={"out"})
-def _adapter_grad_op(P: torch.Tensor, M: torch.Tensor, idx: Optional[torch.Tensor], off: torch.Tensor,
-                     out: torch.Tensor) -> None:
-    _backend.adapter_grad(P, M, idx, off, out)
+@torch.library.custom_op("scattermoe::adapter_backward", mutates_args={"DX", "DA", "DB", "DBIAS"})
+def _adapter_backward_op(DY: torch.Tensor, X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
+                         scales: Optional[torch.Tensor], idx: Optional[torch.Tensor], off: Optional[torch.Tensor],
+                         U: torch.Tensor, DX: Optional[torch.Tensor], DA: Optional[torch.Tensor], DB: Optional[torch.Tensor],
+                         DBIAS: Optional[torch.Tensor]) -> None:
+    _backend.adapter_backward(DY, X, W, A, B, ids, scales, idx, off, U, DX, DA, DB, DBIAS)
 
 
 _COMPILED_OPS = {"route": _route_op, "offsets": _offsets_op, "combine": _combine_op, "gate_grad": _gate_grad_op,
                  "glu_fwd": _glu_fwd_op, "glu_bwd": _glu_bwd_op, "topk_softmax": _topk_softmax_op,
                  "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op,
-                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_order": _adapter_order_op,
-                 "adapter_pack": _adapter_pack_op, "adapter_low": _adapter_low_op,
-                 "adapter_project": _adapter_project_op, "adapter_grad": _adapter_grad_op}
+                 "routed_glu_mlp": _routed_glu_mlp_op, "adapter_forward": _adapter_forward_op,
+                 "adapter_backward": _adapter_backward_op}
 
 
 def _launch(name, *args):
@@ -1079,88 +1050,37 @@ def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=Tru
 ADAPTERS_MAX, ADAPTER_MAX_RANK = 2047, 512          # SMOE_ADAPTER_MAX, SMOE_ADAPTER_MAX_RANK
 
 
-ADAPTER_FEW_ROWS = 64          # up to so many rows the adapters' products go row by row, without an order
+ADAPTER_FEW_ROWS = 64          # up to so many rows the adapters' products go row by row, without an order of the rows
 
 
-ADAPTER_LOOK_UP = 1 << 22
+def adapter_forward(x, weight, lora_a, lora_b, ids, scales=None, bias=None):
+    """(y, u, order): u[t] = scales[a] * lora_a[a] @ x[t] (T, r) float32, y[t] = weight @ x[t] (+ bias) + lora_b[a] @ u[t],
+    a = ids[t] (int64), for x (T, d), weight (n, d), lora_a (R, r, d), lora_b (R, n, r); rows whose id lies outside [0, R)
+    get no second term.  `order`: what `adapter_backward` takes."""
+    T, n = x.size(0), weight.size(0)
+    R, r = lora_a.size(0), lora_a.size(1)
+    y = torch.empty((T, n), dtype=x.dtype, device=x.device)
+    u = torch.empty((T, r), dtype=torch.float32, device=x.device)
+    idx = off = None
+    if T > ADAPTER_FEW_ROWS:
+        idx = torch.empty(T, dtype=torch.int64, device=x.device)
+        off = torch.empty(R + 1, dtype=torch.int64, device=x.device)
+    if T and n:
+        _launch("adapter_forward", x, weight, bias, lora_a, lora_b, ids, scales, idx, off, u, y)
+    return y, u, (idx, off)
 
 
-def adapter_order(ids, R):
-    """The rows by adapter, those without one last: (indices (T), inclusive offsets (R + 1)), for `adapter_low`,
-    `adapter_project` and, of whose offsets it takes the first R, `adapter_grad`."""
-    idx = torch.empty(ids.numel(), dtype=torch.int64, device=ids.device)
-    off = torch.empty(R + 1, dtype=torch.int64, device=ids.device)
-    _launch("adapter_order", ids, R, idx, off)
-    return idx, off
-
-
-def _adapter_pack(t, off=None, multiple=1):
-    """A copy of t (n0, n1, n2) with a contiguous last axis whose rows are a multiple of `multiple` elements (as a view of n2
-    columns), zeros behind them.  With `off`, the matrices of adapters without rows are left unwritten."""
-    n2 = t.size(2)
-    dst = torch.empty((t.size(0), t.size(1), -(-n2 // multiple) * multiple), dtype=t.dtype, device=t.device)
-    _launch("adapter_pack", t, dst, off)
-    return dst
-
-
-def _pieces(t):
-    """Whether t's rows are 16-byte pieces."""
-    return t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.size(-1) % 8 == 0 and t.data_ptr() % 16 == 0
-
-
-def adapter_low(X, A, ids, scales=None, order=None):
-    """(U, parts): U[t, j] = scales[a] * <X[t], A[a, j]>, a = ids[t], for X (T, K) and A (R, r, K): (T, r) float32, zeros in the
-    rows whose id lies outside [0, R).  `order`: of `adapter_order`, for many rows; parts is then what the tiles of
-    `adapter_project` take, U in two 16-bit parts and the rows of every 16 that share an adapter, else None."""
-    assert A.dim() == 3 and A.size(2) == X.size(1) and ids.shape == (X.size(0),)
-    _same_dtype("adapter_low", X, A)
-    T, K, r = X.size(0), X.size(1), A.size(1)
-    idx, off = order if order is not None else (None, None)
-    U = torch.empty((T, r), dtype=torch.float32, device=X.device)
-    planes = slots = None
-    if order is not None and K >= 8:
-        # (a strided factor is copied where the copy's reuse pays for its launch; single values are looked up otherwise)
-        if A.stride(2) != 1 and (X.dtype != torch.float32 or T * K * r > ADAPTER_LOOK_UP):
-            A = _adapter_pack(A, off)
-        if X.dtype != torch.float32:
-            planes = torch.empty((T, 2, -(-r // 32) * 32), dtype=X.dtype, device=X.device)
-            # (smoe_adapter_slots)
-            slots = torch.empty(17 * max(1, min(T, T // 16 + A.size(0) + 1)), dtype=torch.int32, device=X.device)
-    _launch("adapter_low", _rows_contiguous(X), A, ids, scales, idx, off, U, planes, slots)
-    return U, (planes, slots) if planes is not None else None
-
-
-def adapter_project(X, W, U, B, ids, bias=None, parts=None, order=None):
-    """Y[t] = W X[t] (+ bias) + B[a] U[t], a = ids[t], for X (T, K), W (N, K), U (T, r) float32 and B (R, N, r); rows whose
-    id lies outside [0, R) get no second term.  `parts`, `order`: of `adapter_low`, for many rows."""
-    assert W.size(1) == X.size(1) and B.size(1) == W.size(0) and U.shape == (X.size(0), B.size(2)) and ids.shape == (X.size(0),)
-    _same_dtype("adapter_project", X, W, B, bias)
-    T, K, N, r = X.size(0), X.size(1), W.size(0), U.size(1)
-    Y = torch.empty((T, N), dtype=X.dtype, device=X.device)
-    X = _rows_contiguous(X)
-    planes, slots = parts if parts is not None else (None, None)
-    if planes is not None:
-        off = order[1]
-        # the tiles' operands in 16-byte pieces: copies of what is not, a few percent of the product's own traffic
-        if r % 8 or not _pieces(B):
-            B = _adapter_pack(B, off, 8)
-        if not _pieces(X):
-            X = _adapter_pack(X.unsqueeze(0), None, 8)[0]
-        strided = W.stride(0) == 1 and W.stride(1) != 1
-        if not _pieces(W.t() if strided else W) or X.size(1) != K:
-            W = _adapter_pack(W.unsqueeze(0), None, 8)[0]
-    elif T > 1 and K >= 8 and W.stride(1) != 1:
-        W = _adapter_pack(W.unsqueeze(0))[0]                # row by row: a contiguous contraction
-    _launch("adapter_project", X, W, bias, U, planes, slots, B, ids, Y)
-    return Y
-
-
-def adapter_grad(P, M, idx, off, R, transposed=False):
-    """out[a, j, c] = sum of P[t, j] * M[t, c] over the rows t of adapter a, for P (T, r) float32 and M (T, C); the rows as
-    `route` orders them.  `transposed`: (R, C, r) instead of (R, r, C)."""
-    r, C = P.size(1), M.size(1)
-    out = torch.empty((R, C, r) if transposed else (R, r, C), dtype=M.dtype, device=M.device)
-    if P.size(0) == 0:
-        return out.zero_()
-    _launch("adapter_grad", P, _rows_contiguous(M), idx, off, out.transpose(1, 2) if transposed else out)
-    return out
+def adapter_backward(dy, x, weight, lora_a, lora_b, ids, scales, u, order, need_x=True, need_a=True, need_b=True,
+                     need_bias=False):
+    """Gradients (dx, d lora_a, d lora_b, d bias) of `adapter_forward`, None for those that are not wanted."""
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    da = torch.empty(lora_a.shape, dtype=x.dtype, device=x.device) if need_a else None
+    db = torch.empty(lora_b.shape, dtype=x.dtype, device=x.device) if need_b else None
+    dbias = torch.empty(weight.size(0), dtype=x.dtype, device=x.device) if need_bias else None
+    if x.size(0) and weight.size(0):
+        _launch("adapter_backward", dy, x, weight, lora_a, lora_b, ids, scales, *order, u, dx, da, db, dbias)
+    else:
+        for t in (dx, da, db, dbias):
+            if t is not None:
+                t.zero_()
+    return dx, da, db, dbias

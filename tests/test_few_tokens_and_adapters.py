@@ -47,42 +47,37 @@ class _Backend(OracleBackend):
     @staticmethod
     def _picked(factor, ids):
         on = (ids >= 0) & (ids < factor.size(0))
-        return factor[ids.clamp(0, factor.size(0) - 1)].double() * on.view(-1, 1, 1), on
-
-    @staticmethod
-    def adapter_order(ids, R, idx, off):
-        groups = torch.where((ids >= 0) & (ids < R), ids, torch.full_like(ids, R))
-        idx.copy_(torch.sort(groups, stable=True).indices)
-        off.copy_(torch.bincount(groups, minlength=R + 1).cumsum(0))
-
-    @staticmethod
-    def adapter_pack(src, dst, off):
-        dst.zero_()
-        dst[:, :, :src.size(2)] = src
+        return factor[ids.clamp(0, factor.size(0) - 1)].double() * on.view(-1, 1, 1)
 
     @classmethod
-    def adapter_low(cls, X, A, ids, scales, idx, off, U, planes, slots):
-        f, _ = cls._picked(A, ids)
+    def _product(cls, X, W, A, B, ids, scales):
         s = torch.ones(A.size(0)) if scales is None else scales
-        U.copy_((f @ X.double().unsqueeze(2)).squeeze(2) * s[ids.clamp(0, A.size(0) - 1)].unsqueeze(1))
-        if planes is not None:
-            planes.zero_()
-            planes[:, 0, :U.size(1)] = U.to(planes.dtype)
-            planes[:, 1, :U.size(1)] = (U - planes[:, 0, :U.size(1)].float()).to(planes.dtype)
+        u = (cls._picked(A, ids) @ X.double().unsqueeze(2)).squeeze(2) * s[ids.clamp(0, A.size(0) - 1)].unsqueeze(1)
+        return u, X.double() @ W.double().t() + (cls._picked(B, ids) @ u.unsqueeze(2)).squeeze(2)
 
     @classmethod
-    def adapter_project(cls, X, W, bias, U, planes, slots, B, ids, Y):
-        f, _ = cls._picked(B[:, :, :U.size(1)], ids)
-        u = U.double() if planes is None else planes.double().sum(1)[:, :U.size(1)]
-        Y.copy_(X[:, :W.size(1)].double() @ W.double().t() + (f @ u.unsqueeze(2)).squeeze(2) + (0 if bias is None else bias.double()))
+    def adapter_forward(cls, X, W, bias, A, B, ids, scales, idx, off, U, Y):
+        u, y = cls._product(X, W, A, B, ids, scales)
+        U.copy_(u)
+        Y.copy_(y if bias is None else y + bias.double())
+        if idx is not None:
+            groups = torch.where((ids >= 0) & (ids < A.size(0)), ids, torch.full_like(ids, A.size(0)))
+            idx.copy_(torch.sort(groups, stable=True).indices)
+            off.copy_(torch.bincount(groups, minlength=A.size(0) + 1).cumsum(0))
 
-    @staticmethod
-    def adapter_grad(P, M, idx, off, out):
-        lo = 0
-        for a, hi in enumerate(off[:out.size(0)].tolist()):
-            rows = torch.arange(lo, hi) if idx is None else idx[lo:hi]
-            out[a] = (P[rows].double().t() @ M[rows].double()).to(out.dtype)
-            lo = hi
+    @classmethod
+    def adapter_backward(cls, DY, X, W, A, B, ids, scales, idx, off, U, DX, DA, DB, DBIAS):
+        v, dx = cls._product(DY, W.t(), B.transpose(1, 2), A.transpose(1, 2), ids, scales)
+        if DX is not None:
+            DX.copy_(dx)
+        for a in range(A.size(0)):
+            rows = ids == a
+            if DA is not None:
+                DA[a] = (v[rows].t() @ X[rows].double()).to(DA.dtype)
+            if DB is not None:
+                DB[a] = (DY[rows].double().t() @ U[rows].double()).to(DB.dtype)
+        if DBIAS is not None:
+            DBIAS.copy_(DY.double().sum(0))
 
 
 @pytest.fixture
@@ -218,27 +213,18 @@ def test_library_refuses_before_it_launches():
     assert b"workspace" in lib.smoe_last_error()
     assert layer(T=0) == 0
     assert lib.smoe_routed_glu_mlp_workspace_bytes(0, 2, 64, 64) == 0 and lib.smoe_routed_glu_mlp_workspace_bytes(4, 2, 64, 64) >= 8 * 64 * 4
-    def low(r=8, R=3, T=4, x=one, idx=None, off=None, planes=None, dtype=1, K=64):
-        return lib.smoe_adapter_low(x, 64, one, 64, 64, 1, one, None, idx, off, one, planes, planes, T, K, r, R, dtype, None)
-    assert low(r=0) == -2 and low(R=2048) == -5 and low(r=513) == -5 and low(x=None) == -1 and low(dtype=7) == -3
-    assert low(idx=one) == -6 and low(planes=one) == -6 and low(idx=one, off=one, planes=one, dtype=0) == -6
-    assert low(idx=one, off=one, planes=one, K=7) == -6
+    bytes_ = lib.smoe_adapter_workspace_bytes
+    assert bytes_(0, 64, 64, 8, 3, 0, 1) == 0 and bytes_(4, 64, 64, 0, 3, 0, 1) == 0 and bytes_(4, 64, 64, 8, 2048, 0, 1) == 0
 
-    def project(r=8, ids=one, slots=None, T=4):
-        return lib.smoe_adapter_project(one, 64, one, 64, 1, None, 0, one, None, slots, one, 8, 8, 1, ids, one, 64, T, 64, 64, r, 3, 1, None)
-    assert project(r=513) == -5 and project(ids=None) == -1 and project(slots=one) == -1 and project(T=-1) == -2
-    for T, R in ((1, 1), (15, 3), (16, 1), (1777, 16), (100, 2047)):
-        assert lib.smoe_adapter_slots(T, R) == 17 * max(1, min(T, T // 16 + R + 1))
-    assert lib.smoe_adapter_slots(0, 3) == 0 and lib.smoe_adapter_slots(4, 0) == 0
+    def forward(T=100, K=64, N=64, r=8, R=3, x=one, idx=one, dtype=1, ws=one, ws_bytes=1 << 30):
+        return lib.smoe_adapter_forward(x, K, one, None, one, one, one, None, idx, one, one, one, T, K, N, r, R, dtype, ws, ws_bytes, None)
+    assert forward(r=0) == -2 and forward(R=0) == -2 and forward(K=0) == -2 and forward(T=-1) == -2 and forward(dtype=7) == -3
+    assert forward(R=2048) == -5 and forward(r=513) == -5 and forward(T=1 << 31) == -5 and forward(x=None) == -1
+    assert forward(idx=None) == -1 and forward(ws=None) == -4 and forward(ws_bytes=1000) == -4 and forward(ws=ctypes.c_void_p(264)) == -4
 
-    def grad(off=one, T=4, C=64, ws=None, ws_bytes=0):
-        return lib.smoe_adapter_grad(one, one, 64, None, off, one, 8, 8, 1, T, C, 8, 1, 1, ws, ws_bytes, None)
-    assert grad(off=None) == -1 and grad(T=0) == -1 and grad(T=-1) == -2
-    assert lib.smoe_adapter_grad_workspace_bytes(8192, 4096, 16, 1, 1) > 0 and lib.smoe_adapter_grad_workspace_bytes(64, 4096, 16, 1, 1) == 0
-    assert grad(T=8192, C=4096) == -4 and grad(T=8192, C=4096, ws=one, ws_bytes=64) == -4
-    order = lambda ids=one, T=4, R=3, off=one, ws=one, ws_bytes=1 << 20: lib.smoe_adapter_order(ids, T, R, one, off, ws, ws_bytes, None)
-    assert order(ids=None) == -1 and order(R=0) == -2 and order(off=None) == -1 and order(ws=None) == -4 and order(ws_bytes=16) == -4
-    assert order(R=2048) == -5 and order(ws=ctypes.c_void_p(264)) == -4
-    assert lib.smoe_adapter_pack(one, 64, 8, 1, one, 2, 8, 9, 8, None, 1, None) == -2
-    assert lib.smoe_adapter_pack(one, 64, 8, 1, None, 2, 8, 8, 8, None, 1, None) == -1
-    assert low(T=0) == 0 and lib.smoe_last_error() == b""
+    def backward(T=100, K=64, N=64, dy=one, idx=one, ws=one, ws_bytes=1 << 30):
+        return lib.smoe_adapter_backward(dy, one, K, one, one, one, one, None, idx, one, one, one, one, one, one, T, K, N, 8, 3, 1, ws,
+                                         ws_bytes, None)
+    assert backward(T=0) == -2 and backward(N=0) == -2 and backward(dy=None) == -1 and backward(idx=None) == -1
+    assert backward(ws=None) == -4 and backward(ws_bytes=1000) == -4 and backward(T=4, ws=None) == -4
+    assert forward(T=0) == 0 and lib.smoe_last_error() == b""
