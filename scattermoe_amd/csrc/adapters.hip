@@ -477,8 +477,13 @@ struct Product {
 };
 // Up to so many multiply-adds a strided factor is looked up element by element: a copy's launch costs more
 static constexpr int64_t LOOK_UP = 1 << 22;
+// Rows from which 16-bit products go in tiles, fewer where there is more to do: the rows' own kernel reads the weights once per 32
+// rows, but has a workgroup per 16 columns (us of a call, row by row / tiles: 80 rows, 4096 -> 4096 33 / 42; 128 rows 40 / 42; 256
+// rows 63 / 43; 100 rows, 2048 -> 2048 18 / 28; 300 rows, 512 -> 512 13 / 17; 777 rows, 2880 -> 2880 93 / 42)
+static constexpr int64_t TILES_MIN_ROWS = 320, TILES_MIN_WORK = 2000000000;
 static int product(const AdapterCall& c, Product p, const int64_t* idx, const int64_t* off, Space& s, hipStream_t st) {
-  const bool many = c.T > ADAPTER_FEW_ROWS, tiles = many && c.dtype != SMOE_F32 && p.K >= 8;
+  const bool many = c.T > ADAPTER_FEW_ROWS;
+  const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && c.T * p.N * p.K > TILES_MIN_WORK));
   const int64_t w = width(c.dtype);
   auto copy = [&](const void*& src, int64_t& s0, int64_t& s1, int64_t& s2, int64_t n0, int64_t n1, int64_t n2, int64_t ld) {
     char* dst = s.bytes(n0 * n1 * ld * w);

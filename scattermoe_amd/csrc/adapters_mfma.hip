@@ -15,13 +15,15 @@ namespace smoe {
 struct AdapterTiles {
   AdapterProjectArgs p;
   Raster rast;
-  int64_t fragments;
+  int64_t fragments, first;                          // all, the launch's first
 };
 
-// Tile classes: 0 one wave per SIMD (long contractions of whole slices), 1 eight waves, 2 tiles of 128 x 128, two workgroups per CU
+// Tile classes: 0 one wave per SIMD (long contractions of whole slices), 1 eight waves, 2 tiles of 128 x 128 and 3 of 64 x 128, two
+// workgroups per CU
 template <int CLASS> struct AdapterTile;
 template <> struct AdapterTile<0> { typedef Tile<256, 256, 2, 2, 2, true> type; };
 template <> struct AdapterTile<1> { typedef Tile<256, 256, 2, 4> type; };
+template <> struct AdapterTile<3> { typedef Tile<64, 128, 2, 2, 3, false, 2> type; };
 template <> struct AdapterTile<2> { typedef Tile<128, 128, 2, 2, 2, false, 2> type; };
 
 template <typename T, int CLASS, bool W_TR>
@@ -41,7 +43,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   const int n0 = n_tile * TL::BN, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // rows of the tile's fragments; one behind the last row repeats the fragment's first, or any
-  const int64_t fragments = args.fragments, f0 = (int64_t)m_tile * FRAGS;
+  const int64_t fragments = args.fragments, f0 = args.first + (int64_t)m_tile * FRAGS;
   bool any = false;
   for (int m = threadIdx.x; m < TL::BM; m += TL::NT) {
     const int64_t f = f0 + (m >> 4);
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   if constexpr (W_TR) B.init((const char*)a.W + (int64_t)n0 * 2, a.swk * 2, a.N - n0);
   else B.init((const char*)a.W, [&](int row) { return (int64_t)min(n0 + row, a.N - 1) * a.swn * 2; });
   if constexpr (TL::RS) mainloop_rs<T, TL, AOp, BOp>(A, B, a.K, lds, acc);
+  else if constexpr (TL::NS > 2) mainloop_ring<T, TL, AOp, BOp>(A, B, a.K, lds, acc);
   else mainloop<T, TL, AOp, BOp, false>(A, B, a.K, lds, false, acc, rs);
 
   __syncthreads();
@@ -128,28 +131,43 @@ static Raster tile_order(int64_t m_tiles, int n_tiles, int wgs) {
   return by_stripes < by_supers ? make_striped(m_tiles, n_tiles, GM_RING) : supers;
 }
 
+// Fragments [first, last) in tiles of a class
 template <typename T, int CLASS>
-static int launch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st) {
+static int launch_tiles(const AdapterProjectArgs& a, bool w_tr, int64_t first, int64_t last, hipStream_t st) {
   typedef typename AdapterTile<CLASS>::type TL;
-  const int64_t fragments = adapter_fragments(a.T, a.R);
-  const int64_t m_tiles = cdiv64(fragments, TL::BM / 16);
+  const int64_t m_tiles = cdiv64(last - first, TL::BM / 16);
   const int n_tiles = (a.N + TL::BN - 1) / TL::BN;
-  AdapterTiles args{a, tile_order(m_tiles, n_tiles, TL::WG), fragments};
+  AdapterTiles args{a, tile_order(m_tiles, n_tiles, TL::WG), last, first};
   const int64_t grid = args.rast.grid();
-  if (grid > 0x7fffffffLL) { set_error("smoe_adapter_project: grid too large"); return SMOE_ERR_RANGE; }
+  if (grid > 0x7fffffffLL) { set_error("adapters: grid too large"); return SMOE_ERR_RANGE; }
   if (w_tr) hipLaunchKernelGGL((adapter_tiles_kernel<T, CLASS, true>), dim3((unsigned)grid), dim3(TL::NT), 0, st, args);
   else hipLaunchKernelGGL((adapter_tiles_kernel<T, CLASS, false>), dim3((unsigned)grid), dim3(TL::NT), 0, st, args);
   return launch_status("adapter_tiles_kernel");
 }
 
+// Below two thirds of a round of 256 x 256 tiles: smaller ones, 64 x 128 while 128 x 128 ones would leave CUs without a tile.  us of
+// a whole call, 128 x 128 / 64 x 128, T rows K -> N: 256, 4096 -> 4096 56 / 43; 512, 4096 -> 4096 58 / 52; 777, 2880 -> 2880 47 / 42;
+// 1000, 4096 -> 1024 58 / 45; 1024, 4096 -> 4096 69 / 83; 1777, 2048 -> 4096 49 / 64 (256 x 128 tiles 56).
+static constexpr int SMALL_MIN_TILES = 200;
+template <typename T>
+static int launch_small(const AdapterProjectArgs& a, bool w_tr, int64_t first, int64_t last, hipStream_t st) {
+  return cdiv64(last - first, 8) * cdiv64(a.N, 128) < SMALL_MIN_TILES ? launch_tiles<T, 3>(a, w_tr, first, last, st)
+                                                                      : launch_tiles<T, 2>(a, w_tr, first, last, st);
+}
+
 template <typename T>
 static int dispatch_tiles(const AdapterProjectArgs& a, bool w_tr, hipStream_t st) {
-  const int64_t tiles = cdiv64(a.T, 256) * cdiv64(a.N, 256);
-  if (tiles < MAIN_MIN_TILES) return launch_tiles<T, 2>(a, w_tr, st);
-  const bool whole = a.K % BK == 0 && ((uintptr_t)a.Y & 15) == 0 && ((a.sym | a.N) & 7) == 0;
+  const int64_t fragments = adapter_fragments(a.T, a.R), rows = cdiv64(fragments, 16), columns = cdiv64(a.N, 256), tiles = rows * columns;
+  if (cdiv64(a.T, 256) * columns < MAIN_MIN_TILES) return launch_small<T>(a, w_tr, 0, fragments, st);
+  // Whole rounds of 256 x 256 tiles; what is left, up to half a round, would take as long as a round (4096 rows and eight adapters'
+  // padding, 4096 -> 4096, a call: 204 -> 158 us): tile rows of a launch of their own, in smaller tiles.
+  const int64_t whole = tiles / NUM_CU * NUM_CU;
+  const int64_t main = whole > 0 && tiles - whole <= NUM_CU / 2 ? std::min(fragments, whole / columns * 16) : fragments;
+  const bool slices = a.K % BK == 0 && ((uintptr_t)a.Y & 15) == 0 && ((a.sym | a.N) & 7) == 0;
   // (the descriptors of a strided operand end with its last row: rows must not overlap)
-  if (a.K >= RS_MIN_K && whole && (!w_tr || a.swk >= a.N)) return launch_tiles<T, 0>(a, w_tr, st);
-  return launch_tiles<T, 1>(a, w_tr, st);
+  const int rc = a.K >= RS_MIN_K && slices && (!w_tr || a.swk >= a.N) ? launch_tiles<T, 0>(a, w_tr, 0, main, st)
+                                                                      : launch_tiles<T, 1>(a, w_tr, 0, main, st);
+  return rc || main == fragments ? rc : launch_small<T>(a, w_tr, main, fragments, st);
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

@@ -63,9 +63,11 @@ def test_values_and_gradients(T, d, n, R, r, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("T,d,n,R,r,grouped", [(2600, 1856, 4096, 5, 8, True), (2600, 4104, 1800, 40, 24, False), (3000, 1016, 3584, 3, 40, False)])
+@pytest.mark.parametrize("T,d,n,R,r,grouped", [(2600, 1856, 4096, 5, 8, True), (2600, 4104, 1800, 40, 24, False), (3000, 1016, 3584, 3, 40, False),
+                                                (4096, 1792, 4096, 9, 8, False), (700, 2048, 1800, 20, 12, False), (330, 264, 1000, 6, 33, True)])
 def test_large_tiles(T, d, n, R, r, grouped, dtype):
-    """Enough tiles of 256 x 256 for the chip: contractions of whole slices of 64 and others, forward and, transposed, backward."""
+    """Tiles of every class: contractions of whole slices of 64 and others, forward and, transposed, backward; more than a round of
+    256 x 256 tiles by less than half, in two launches."""
     i, dy = _inputs(T, d, n, R, r, dtype, bias=True, grouped=grouped, seed=T + n)
     _compare(i, dy)
 
