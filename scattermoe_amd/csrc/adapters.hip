@@ -217,7 +217,7 @@ template <typename T, int JT>
 __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradArgs a, int slices, float* partial) {
   constexpr int PER = Few<T>::PER, COLS = 16 * PER;
   typedef T V __attribute__((ext_vector_type(PER)));
-  __shared__ f32x4 part[GRAD_NW - 1][JT * PER][64];
+  __shared__ __attribute__((aligned(16))) float part[GRAD_NW][16][COLS];
   const int id = blockIdx.y / slices, slice = blockIdx.y % slices, lane = lane_id(), wave = threadIdx.x >> 6;
   const int l = lane & 15, q = lane >> 4, j0 = blockIdx.z * JT * 16;
   const int c0 = blockIdx.x * COLS + l * PER, c = min(c0, a.C - PER);        // (the last columns: once more, by the lane before them)
@@ -267,30 +267,40 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
 #pragma unroll
         for (int i = 0; i < PER; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[u][j], to_f32(m[u][i]), acc[j][i], 0, 0, 0);
   }
-  if (wave > 0) {
+  // a lane holds ranks j0 + 16 j + 4 q + e of columns c + i: the waves' sums in LDS as rows of columns, then a piece of a row per thread
+  const int row = threadIdx.x >> 4, piece = threadIdx.x & 15;
+  const int from = blockIdx.x * COLS + piece * PER, to = min(from, a.C - PER);
+  static_assert(GRAD_NW * 64 == 256, "a piece per thread");
 #pragma unroll
-    for (int j = 0; j < JT; ++j)
+  for (int j = 0; j < JT; ++j) {
+    if (j > 0) __syncthreads();
 #pragma unroll
-      for (int i = 0; i < PER; ++i) part[wave - 1][j * PER + i][lane] = acc[j][i];
-  }
-  __syncthreads();
-  if (wave > 0 || c0 >= a.C) return;
-  // this lane: ranks j0 + 16 j + 4 q + e, columns c + i
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-  for (int j = 0; j < JT; ++j)
+      for (int i = 0; i < PER; i += 4)
+        *(f32x4*)(part[wave][4 * q + e] + l * PER + i) = f32x4{acc[j][i][e], acc[j][i + 1][e], acc[j][i + 2][e], acc[j][i + 3][e]};
+    __syncthreads();
+    const int r = j0 + 16 * j + row;
+    if (r >= a.r || from >= a.C) continue;
+    float v[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      f32x4 v = acc[j][i];
+    for (int i = 0; i < PER; i += 4) {
+      f32x4 s = *(const f32x4*)(part[0][row] + piece * PER + i);
 #pragma unroll
-      for (int w = 0; w < GRAD_NW - 1; ++w) v += part[w][j * PER + i][lane];
+      for (int w = 1; w < GRAD_NW; ++w) s += *(const f32x4*)(part[w][row] + piece * PER + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = j0 + 16 * j + 4 * q + e;
-        if (r >= a.r) continue;
-        if (slices == 1) ((T*)a.OUT)[id * a.soa + r * a.soj + (c + i) * a.soc] = from_f32<T>(v[e]);
-        else partial[(((int64_t)slice * a.R + id) * a.r + r) * a.C + c + i] = v[e];
-      }
+      for (int k = 0; k < 4; ++k) v[i + k] = s[k];
     }
+    if (slices > 1) {
+      float* p = partial + (((int64_t)slice * a.R + id) * a.r + r) * a.C + to;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) p[i] = v[i];
+    } else {
+      T* out = (T*)a.OUT + id * a.soa + r * a.soj + to * a.soc;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) out[i * a.soc] = from_f32<T>(v[i]);
+    }
+  }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_grad_join_kernel(AdapterGradArgs a, int slices, const float* partial) {
@@ -309,12 +319,18 @@ __global__ __launch_bounds__(256) void adapter_grad_join_kernel(AdapterGradArgs 
 // ---- factors in another order ---------------------------------------------------------------------------------------
 // DST[a][i][0 .. ld) = SRC[a, i, 0 .. n2), zeros behind: for the products that want the contraction contiguous, whole pieces of 16 bytes
 // or rows that start at them.  With `off`, adapters without rows are left out (nobody reads them).
+// Two copies in one launch: every launch costs about as much as the copy.
+struct AdapterPacks { AdapterPackArgs of[2]; };
 template <typename T>
-__global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs a) {
+__global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPacks packs) {
   __shared__ T tile[64][64 + 4 / sizeof(T)];
-  const int id = blockIdx.z;
+  const int first = packs.of[0].tiles();
+  const AdapterPackArgs& a = packs.of[(int)blockIdx.x < first ? 0 : 1];
+  int at = (int)blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+  const int across = (a.ld + 63) / 64, down = (a.n1 + 63) / 64, id = at / (across * down);
+  at -= id * across * down;
   if (a.off && a.off[id] == (id ? a.off[id - 1] : 0)) return;
-  const int i0 = blockIdx.y * 64, k0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int i0 = at / across * 64, k0 = at % across * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
   const T* src = (const T*)a.SRC + id * a.s0;
   T* dst = (T*)a.DST + (int64_t)id * a.n1 * a.ld;
   if (a.s2 == 1) {
@@ -427,14 +443,16 @@ static int grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_
   float* p = (float*)workspace;
   return dtype == SMOE_F32 ? grad_t<float>(a, slices, p, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(a, slices, p, st) : grad_t<f16_t>(a, slices, p, st);
 }
-template <typename T>
-static int pack_t(const AdapterPackArgs& a, hipStream_t st) {
-  if ((a.n1 + 63) / 64 > 65535) { set_error("adapters: at most 2^22 columns in this layout"); return SMOE_ERR_RANGE; }
-  hipLaunchKernelGGL(adapter_pack_kernel<T>, dim3((a.ld + 63) / 64, (a.n1 + 63) / 64, a.n0), dim3(256), 0, st, a);
+static int pack(const AdapterPackArgs& a, const AdapterPackArgs& b, int dtype, hipStream_t st) {
+  const int64_t tiles = a.all_tiles() + b.all_tiles();
+  if (tiles > 0x7fffffffLL) { set_error("adapters: factors too large to copy"); return SMOE_ERR_RANGE; }
+  if (tiles == 0) return 0;
+  const dim3 grid((unsigned)tiles), block(256);
+  const AdapterPacks p{{a, b}};
+  if (dtype == SMOE_F32) hipLaunchKernelGGL(adapter_pack_kernel<float>, grid, block, 0, st, p);
+  else if (dtype == SMOE_BF16) hipLaunchKernelGGL(adapter_pack_kernel<bf16_t>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(adapter_pack_kernel<f16_t>, grid, block, 0, st, p);
   return launch_status("adapter_pack_kernel");
-}
-static int pack(const AdapterPackArgs& a, int dtype, hipStream_t st) {
-  return dtype == SMOE_F32 ? pack_t<float>(a, st) : dtype == SMOE_BF16 ? pack_t<bf16_t>(a, st) : pack_t<f16_t>(a, st);
 }
 
 // Pieces of the workspace, each at a multiple of 256 bytes.  Without one (a dry run) it only counts, and nothing is launched.
@@ -485,15 +503,30 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   const bool many = c.T > ADAPTER_FEW_ROWS;
   const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && c.T * p.N * p.K > TILES_MIN_WORK));
   const int64_t w = width(c.dtype);
+  // The copies, at most the factors' and those of the shared product, in pairs
+  AdapterPackArgs copies[4] = {};
+  int n = 0;
   auto copy = [&](const void*& src, int64_t& s0, int64_t& s1, int64_t& s2, int64_t n0, int64_t n1, int64_t n2, int64_t ld) {
     char* dst = s.bytes(n0 * n1 * ld * w);
-    const AdapterPackArgs a{src, s0, s1, s2, dst, (int)ld, n0 == 1 ? nullptr : off, (int)n0, (int)n1, (int)n2};
+    copies[n++] = AdapterPackArgs{src, s0, s1, s2, dst, (int)ld, n0 == 1 ? nullptr : off, (int)n0, (int)n1, (int)n2};
     src = dst;
     s0 = n1 * ld, s1 = ld, s2 = 1;
-    return s.dry() ? 0 : pack(a, c.dtype, st);
   };
-  if (p.sak != 1 && p.K >= pieces(c.dtype) && (tiles || c.T * p.K * c.r > LOOK_UP))
-    if (int rc = copy(p.A, p.sar, p.saj, p.sak, c.R, c.r, p.K, p.K)) return rc;
+  int64_t zero = 0, one = 1;
+  if (p.sak != 1 && p.K >= pieces(c.dtype) && (tiles || c.T * p.K * c.r > LOOK_UP)) copy(p.A, p.sar, p.saj, p.sak, c.R, c.r, p.K, p.K);
+  const void* X = p.X;
+  int64_t sxm = p.sxm, K = p.K;
+  if (p.Y != nullptr && tiles) {
+    K = up8(p.K);
+    if (p.sbj != 1 || c.r % 8) copy(p.B, p.sbr, p.sbn, p.sbj, c.R, p.N, c.r, up8(c.r));
+    const bool w_tr = p.swn == 1 && p.swk != 1;
+    if (p.K % 8 || (w_tr && p.N % 8)) copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, K);
+    if (p.K % 8) copy(X, zero, sxm, one, 1, c.T, p.K, K);
+  } else if (p.Y != nullptr && p.swk != 1 && p.K >= pieces(c.dtype)) {
+    copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, p.K);
+  }
+  for (int i = 0; i < n && !s.dry(); i += 2)
+    if (int rc = pack(copies[i], copies[i + 1], c.dtype, st)) return rc;
   const int rp = (c.r + 31) / 32 * 32;
   char* planes = tiles ? s.bytes(c.T * 2 * rp * w) : nullptr;
   int* slots = tiles ? s.take<int>(adapter_fragments(c.T, c.R) * 17) : nullptr;
@@ -503,24 +536,9 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
     if (int rc = low(a, c.dtype, st)) return rc;
   }
   if (p.Y == nullptr) return 0;
-  int64_t zero = 0, one = 1;
-  if (tiles) {
-    const int64_t k8 = up8(p.K);
-    if (p.sbj != 1 || c.r % 8)
-      if (int rc = copy(p.B, p.sbr, p.sbn, p.sbj, c.R, p.N, c.r, up8(c.r))) return rc;
-    const bool w_tr = p.swn == 1 && p.swk != 1;
-    if (p.K % 8 || (w_tr && p.N % 8))
-      if (int rc = copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, k8)) return rc;
-    if (p.K % 8) {
-      if (int rc = copy(p.X, zero, p.sxm, one, 1, c.T, p.K, k8)) return rc;
-      p.K = k8;
-    }
-  } else if (p.swk != 1 && p.K >= pieces(c.dtype)) {
-    if (int rc = copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, p.K)) return rc;
-  }
   if (s.dry()) return 0;
-  const AdapterProjectArgs a{p.X, p.sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
-                             c.T, (int)p.K, (int)p.N, c.r, c.R};
+  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
+                             c.T, (int)K, (int)p.N, c.r, c.R};
   return project(a, c.dtype, st);
 }
 

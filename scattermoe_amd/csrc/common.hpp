@@ -412,6 +412,8 @@ struct AdapterPackArgs {
   void* DST; int ld;                                 // (n0, n1, ld)
   const int64_t* off;                                // inclusive offsets (n0) or NULL
   int n0, n1, n2;
+  __host__ __device__ int64_t all_tiles() const { return (int64_t)n0 * ((n1 + 63) / 64) * ((ld + 63) / 64); }      // of 64 x 64
+  __host__ __device__ int tiles() const { return (int)all_tiles(); }
 };
 // Fragments of 16 rows, each of one adapter, that T rows of R adapters (and of none) can make
 static inline int64_t adapter_fragments(int64_t T, int64_t R) { return max_tiles(T, (int)R + 1, 16); }
