@@ -142,7 +142,7 @@ template <typename T, int P, int G>
 __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int f0, const int* rows, int M, float* part) {
   constexpr int INPUTS = G * 16 / P;
   const T* W = (const T*)a.W1 + e * a.sw1e;
-  few_tile<T, P, G, 1, HID_NW, HID_ROWS>([&](int n) { return W + (min(f0 + (n >> 1), a.F - 1) + (n & 1 ? a.F : 0)) * a.sw1n; },
+  few_tile<T, P, G, 1, HID_NW, HID_ROWS, true, G == 4 ? 2 : 0>([&](int n) { return W + (min(f0 + (n >> 1), a.F - 1) + (n & 1 ? a.F : 0)) * a.sw1n; },
                                          [&](int m) { return (const T*)a.X + rows[min(m, M - 1)] / a.k * a.sxm; }, 0, a.d, part);
   __syncthreads();
   const T* b1 = a.b1 ? (const T*)a.b1 + e * a.sb1e : nullptr;
@@ -161,8 +161,9 @@ __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int
   }
 }
 
-// GROUPS: 0 up to 4 tokens, else groups of 8 rows that a pass over the weights takes (`row_groups`).  Up to 4, every workgroup makes their selections for itself, a wave each, out of the logits (the
-// first one leaves them to the output's launch): a launch for that would cost more.
+// GROUPS: 0 for up to 4 tokens, else the groups of 8 rows that a pass over an expert's weights takes (row_groups).  Up to 4 tokens
+// every workgroup makes their selections for itself, a wave each, out of the logits (the first one leaves them to the
+// output's launch): a launch for that would cost more.
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) void layer_hidden_kernel(RoutedLayerArgs a) {
   constexpr bool MANY = GROUPS > 0;
@@ -193,8 +194,8 @@ __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) 
   const int* rows = s.rows + s.first[e];
   if constexpr (MANY) {
     for (int M = s.count[e];;) {
-      if (M <= 8) hidden_tile<T, 2, 1>(a, e, f0, rows, M, part);
-      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, 2>(a, e, f0, rows, min(M, 16), part);
+      if (GROUPS == 1 || M <= 8) hidden_tile<T, 2, 1>(a, e, f0, rows, min(M, 8), part);
+      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, GROUPS == 1 ? 1 : 2>(a, e, f0, rows, min(M, 16), part);
       else hidden_tile<T, 2, GROUPS>(a, e, f0, rows, min(M, 8 * GROUPS), part);
       if ((M -= 8 * GROUPS) <= 0) break;
       rows += 8 * GROUPS;
@@ -212,7 +213,7 @@ template <typename T, int P, int G>
 __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0, const int* rows, int M, float* part) {
   constexpr int INPUTS = G * 16 / P, H = HIDDEN_PARTS<T>;
   const T* W = (const T*)a.W2 + e * a.sw2e;
-  few_tile<T, P, G, H, TILE_NW, TILE_COLS>([&](int n) { return W + min(n0 + n, a.d - 1) * a.sw2n; },
+  few_tile<T, P, G, H, TILE_NW, TILE_COLS, true, G == 4 ? 2 : 0>([&](int n) { return W + min(n0 + n, a.d - 1) * a.sw2n; },
                                            [&](int m) { return (const T*)a.hidden + (int64_t)rows[min(m, M - 1)] * H * a.ldh; }, a.ldh,
                                            a.F, part);
   __syncthreads();
@@ -225,7 +226,7 @@ __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0
   }
 }
 template <typename T, int GROUPS>
-__global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : 3) void layer_out_tiles_kernel(RoutedLayerArgs a) {
+__global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) void layer_out_tiles_kernel(RoutedLayerArgs a) {
   __shared__ float part[FEW_PART<TILE_NW, TILE_COLS, GROUPS * 8>];
   __shared__ RowLists s;
   list_rows<TILE_NW * 64>(a.experts, a.T * a.k, a.E, s);
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : 3) void layer_out_ti
   const int e = s.hit[blockIdx.y], n0 = blockIdx.x * TILE_COLS;
   const int* rows = s.rows + s.first[e];
   for (int M = s.count[e];;) {
-    if (M <= 8) out_tile<T, 2, 1>(a, e, n0, rows, M, part);
-    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, 2>(a, e, n0, rows, min(M, 16), part);
+    if (GROUPS == 1 || M <= 8) out_tile<T, 2, 1>(a, e, n0, rows, min(M, 8), part);
+    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, GROUPS == 1 ? 1 : 2>(a, e, n0, rows, min(M, 16), part);
     else out_tile<T, 2, GROUPS>(a, e, n0, rows, min(M, 8 * GROUPS), part);
     if ((M -= 8 * GROUPS) <= 0) break;
     rows += 8 * GROUPS;
@@ -375,7 +376,13 @@ static int launch_t(const RoutedLayerArgs& a, hipStream_t st) {
   if (streams && a.T <= FEWEST) return launch_streams<T, 0>(a, st);
   hipLaunchKernelGGL(layer_select_kernel, dim3(a.T), dim3(64), 0, st, a);
   if (int rc = launch_status("layer_select_kernel")) return rc;
-  if (streams) return a.T * a.k <= 8 * a.E ? launch_streams<T, 2>(a, st) : launch_streams<T, 4>(a, st);
+  if (streams) {
+    // Groups per pass by the rows that an expert gets on average; experts with more take several passes.  Fewer groups leave registers
+    // for more waves: us of the output's launch, 64 tokens over 128 experts, 1 / 2 / 4 groups 75 / 82 / 92, 17 over 32 74 / 74 / 81.
+    const int rows = a.T * a.k;
+    if (rows <= 4 * a.E) return launch_streams<T, 1>(a, st);
+    return rows <= 8 * a.E ? launch_streams<T, 2>(a, st) : launch_streams<T, 4>(a, st);
+  }
   hipLaunchKernelGGL(layer_hidden_any_kernel<T>, dim3((a.F + 3) / 4, a.T * a.k), dim3(256), 0, st, a);
   if (int rc = launch_status("layer_hidden_any_kernel")) return rc;
   hipLaunchKernelGGL(layer_out_any_kernel<T>, dim3((a.d + 3) / 4, a.T), dim3(256), 0, st, a);

@@ -1028,6 +1028,13 @@ def few_tokens(T, k, E):
     return 0 < T <= FEW_TOKENS and T * k <= FEW_ROWS and E <= 512 and k <= 64
 
 
+def few_tokens_pay(T, k, E, d, F, dtype):
+    """Whether it is also the faster way.  Beyond eight rows per expert a 16-bit stream over many weights is faster in the general
+    path's tiles, which share the rows among more columns (8 experts, 4096 -> 14336, us: 32 tokens 456 against 450, 64 tokens 520
+    against 460; 32 experts of 2880, 64 tokens 273 against 276; 16 experts, 1024 -> 512, 64 tokens 25 against 39)."""
+    return few_tokens(T, k, E) and (dtype == torch.float32 or T * k <= 8 * E or E * d * F < 1 << 27)
+
+
 def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=True):
     """(out (T, d), router logits (T, E) float32) of a gated MoE layer from its tokens: router product, softmax, top-k, both
     expert products and the gate-weighted sum, forward only (scattermoe/utils/replace_moe.py:60-95 and GLUMLP.forward,

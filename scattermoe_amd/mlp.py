@@ -170,7 +170,7 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
     softmax over all logits, divided by their sum when `renormalize`; SiLU on the second half of layer 1's columns, on the first
     when `gate_first` (the routing of scattermoe/utils/replace_moe.py:67-71 in front of GLUMLP.forward, mlp.py:74-95).
 
-    Where nothing asks for a gradient and for few tokens (`ops.few_tokens`) the layer is one call of the library (`ops.routed_glu_mlp`); otherwise
+    Where nothing asks for a gradient and for few tokens (`ops.few_tokens_pay`) the layer is one call of the library (`ops.routed_glu_mlp`); otherwise
     router product, `topk_softmax`, `flatten_sort_count` and the gated MLP's launches, differentiable in all float
     arguments.  Both keep the logits in float32; the general path stores hidden and expert rows in x's type, the
     other rounds the output only."""
@@ -199,7 +199,7 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
     if T == 0:
         return x.new_empty(x.shape), x.new_empty((0, E), dtype=torch.float32)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    if ops.few_tokens(T, k, E) and not (trained and torch.is_grad_enabled()):
+    if ops.few_tokens_pay(T, k, E, d, F, x.dtype) and not (trained and torch.is_grad_enabled()):
         out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
         return out.view(x.shape), logits
     logits = nn.functional.linear(tokens.float(), router_weight.float())
