@@ -38,8 +38,8 @@ template <typename T>
 __global__ __launch_bounds__(PT) void adapter_project_any_kernel(AdapterProjectArgs a) {
   __shared__ float sA[PBK][PBM + 4];
   __shared__ float sB[PBK][PBN + 4];
-  const int64_t t0 = (int64_t)blockIdx.y * PBM;
-  const int n0 = blockIdx.x * PBN, tid = threadIdx.x;
+  const int across = (a.N + PBN - 1) / PBN, n0 = (int)(blockIdx.x % across) * PBN, tid = threadIdx.x;
+  const int64_t t0 = (int64_t)(blockIdx.x / across) * PBM;
   const int ty = tid / 16, tx = tid % 16;
   const T* X = (const T*)a.X;
   const T* W = (const T*)a.W;
@@ -176,8 +176,8 @@ template <typename T, int P, int G, int NW, int COLS>
 __global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_kernel(AdapterProjectArgs a) {
   constexpr int INPUTS = 16 * G / P;
   __shared__ float part[FEW_PART<NW, COLS, INPUTS>];
-  const int n0 = blockIdx.x * COLS;
-  const int64_t t0 = (int64_t)blockIdx.y * INPUTS;
+  const int across = (a.N + COLS - 1) / COLS, n0 = (int)(blockIdx.x % across) * COLS;
+  const int64_t t0 = (int64_t)(blockIdx.x / across) * INPUTS;
   few_tile<T, P, G, 1, NW, COLS, false, P == 4 ? 4 : 0>([&](int n) { return (const T*)a.W + std::min(n0 + n, a.N - 1) * a.swn; },
                                         [&](int m) { return (const T*)a.X + std::min<int64_t>(t0 + m, a.T - 1) * a.sxm; }, 0, a.K, part);
   __syncthreads();
@@ -212,15 +212,36 @@ __global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_k
 // transposition, as a lane of the instruction holds one element of one row.  A lane loads 16 bytes of a row of M, and element i of
 // them is its column of product i: columns PER l + i.  A workgroup has 16 PER columns, JT x 16 of the rank and a slice of the
 // adapter's rows, which its waves take in turn, four at a time.
+// The gradients of both factors in one launch: the one's workgroups fill what the other's leave idle.
 static constexpr int GRAD_NW = 4, GRAD_MAX_SLICES = 16;
+struct GradLaunch {
+  AdapterGradArgs a;
+  int slices, columns, ranks;                        // of the rows; tiles of columns, of ranks
+  float* partial;                                    // the slices' sums, (slices, R, r, C)
+  __host__ __device__ int64_t all_blocks() const { return (int64_t)columns * ranks * a.R * slices; }
+  __host__ __device__ int64_t all_joins() const { return slices > 1 ? (int64_t)((a.C + 255) / 256) * a.r * a.R : 0; }
+  __host__ __device__ int blocks() const { return (int)all_blocks(); }
+  __host__ __device__ int joins() const { return (int)all_joins(); }
+};
+struct GradPair { GradLaunch of[2]; };
 template <typename T, int JT>
-__global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradArgs a, int slices, float* partial) {
+__global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(GradPair pair) {
+  const bool second = (int)blockIdx.x >= pair.of[0].blocks();
+  const GradLaunch& g = pair.of[second];
+  const AdapterGradArgs& a = g.a;
+  const int slices = g.slices;
+  float* partial = g.partial;
+  int at = blockIdx.x - (second ? pair.of[0].blocks() : 0);
+  const int column = at % g.columns;
+  at /= g.columns;
+  const int rank = at % g.ranks;
+  at /= g.ranks;
   constexpr int PER = Few<T>::PER, COLS = 16 * PER;
   typedef T V __attribute__((ext_vector_type(PER)));
   __shared__ __attribute__((aligned(16))) float part[GRAD_NW][16][COLS];
-  const int id = blockIdx.y / slices, slice = blockIdx.y % slices, lane = lane_id(), wave = threadIdx.x >> 6;
-  const int l = lane & 15, q = lane >> 4, j0 = blockIdx.z * JT * 16;
-  const int c0 = blockIdx.x * COLS + l * PER, c = min(c0, a.C - PER);        // (the last columns: once more, by the lane before them)
+  const int id = at / slices, slice = at % slices, lane = lane_id(), wave = threadIdx.x >> 6;
+  const int l = lane & 15, q = lane >> 4, j0 = rank * JT * 16;
+  const int c0 = column * COLS + l * PER, c = min(c0, a.C - PER);        // (the last columns: once more, by the lane before them)
   const int64_t first = id ? a.off[id - 1] : 0, count = (a.off ? a.off[id] : a.T) - first;
   const int64_t lo = first + count * slice / slices, hi = first + count * (slice + 1) / slices;
   f32x4 acc[JT][PER];
@@ -269,7 +290,7 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
   }
   // a lane holds ranks j0 + 16 j + 4 q + e of columns c + i: the waves' sums in LDS as rows of columns, then a piece of a row per thread
   const int row = threadIdx.x >> 4, piece = threadIdx.x & 15;
-  const int from = blockIdx.x * COLS + piece * PER, to = min(from, a.C - PER);
+  const int from = column * COLS + piece * PER, to = min(from, a.C - PER);
   static_assert(GRAD_NW * 64 == 256, "a piece per thread");
 #pragma unroll
   for (int j = 0; j < JT; ++j) {
@@ -303,8 +324,14 @@ __global__ __launch_bounds__(GRAD_NW * 64) void adapter_grad_kernel(AdapterGradA
   }
 }
 template <typename T>
-__global__ __launch_bounds__(256) void adapter_grad_join_kernel(AdapterGradArgs a, int slices, const float* partial) {
-  const int c = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, id = blockIdx.z;
+__global__ __launch_bounds__(256) void adapter_grad_join_kernel(GradPair pair) {
+  const bool second = (int)blockIdx.x >= pair.of[0].joins();
+  const GradLaunch& g = pair.of[second];
+  const AdapterGradArgs& a = g.a;
+  const int slices = g.slices, across = (a.C + 255) / 256;
+  const float* partial = g.partial;
+  const int at = blockIdx.x - (second ? pair.of[0].joins() : 0);
+  const int c = at % across * 256 + threadIdx.x, j = at / across % a.r, id = at / across / a.r;
   if (c >= a.C) return;
   const float* p = partial + ((int64_t)id * a.r + j) * a.C + c;
   const int64_t apart = (int64_t)a.R * a.r * a.C;
@@ -377,9 +404,9 @@ static int low_t(const AdapterLowArgs& a, hipStream_t st) {
 
 template <typename T, int P, int G, int NW, int COLS>
 static int project_rows(const AdapterProjectArgs& a, hipStream_t st) {
-  const int64_t chunks = cdiv64(a.T, 16 * G / P);
-  if (chunks > 65535) { set_error("smoe_adapter_project: too many rows for this layout"); return SMOE_ERR_RANGE; }
-  hipLaunchKernelGGL((adapter_project_rows_kernel<T, P, G, NW, COLS>), dim3((a.N + COLS - 1) / COLS, (unsigned)chunks), dim3(NW * 64), 0, st, a);
+  const int64_t grid = cdiv64(a.T, 16 * G / P) * cdiv64(a.N, COLS);
+  if (grid > 0x7fffffffLL) { set_error("adapters: too many rows and columns for one launch"); return SMOE_ERR_RANGE; }
+  hipLaunchKernelGGL((adapter_project_rows_kernel<T, P, G, NW, COLS>), dim3((unsigned)grid), dim3(NW * 64), 0, st, a);
   return launch_status("adapter_project_rows_kernel");
 }
 template <typename T>
@@ -394,37 +421,41 @@ static int project_t(const AdapterProjectArgs& a, hipStream_t st) {
     if (a.T <= 32 || sizeof(T) == 2) return project_rows<T, 2, 4, 8, 16>(a, st);
     if constexpr (sizeof(T) == 4) return a.T <= 64 ? project_rows<T, 1, 2, 8, 16>(a, st) : project_rows<T, 1, 2, 8, 32>(a, st);
   }
-  const int64_t rows = cdiv64(a.T, PBM);
-  if (rows > 65535) { set_error("smoe_adapter_project: too many rows for this layout"); return SMOE_ERR_RANGE; }
-  hipLaunchKernelGGL(adapter_project_any_kernel<T>, dim3((a.N + PBN - 1) / PBN, (unsigned)rows), dim3(PT), 0, st, a);
+  const int64_t grid = cdiv64(a.T, PBM) * cdiv64(a.N, PBN);
+  if (grid > 0x7fffffffLL) { set_error("adapters: too many rows and columns for one launch"); return SMOE_ERR_RANGE; }
+  hipLaunchKernelGGL(adapter_project_any_kernel<T>, dim3((unsigned)grid), dim3(PT), 0, st, a);
   return launch_status("adapter_project_any_kernel");
 }
 
+static int pieces(int dtype) { return dtype == SMOE_F32 ? 4 : 8; }           // elements of 16 bytes
 // Slices of an adapter's rows: enough workgroups for the chip, at least GRAD_MIN_ROWS rows each at even loads
 static constexpr int GRAD_WGS = 1024, GRAD_MIN_ROWS = 128;
 static int grad_tiles(int64_t C, int dtype) { return (int)cdiv64(C, dtype == SMOE_F32 ? 64 : 128); }
 static int grad_ranks(int64_t r) { return r <= 16 ? 1 : 2; }
 static int grad_slices(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
-  if (C < (dtype == SMOE_F32 ? 4 : 8)) return 1;
+  if (C < pieces(dtype)) return 1;
   const int64_t wgs = grad_tiles(C, dtype) * R * cdiv64(r, 16 * grad_ranks(r));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({GRAD_WGS / wgs, T / R / GRAD_MIN_ROWS, GRAD_MAX_SLICES, 65535 / R}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({GRAD_WGS / wgs, T / R / GRAD_MIN_ROWS, GRAD_MAX_SLICES}));
 }
 static size_t grad_bytes(int64_t T, int64_t C, int64_t r, int64_t R, int dtype) {
   const int slices = grad_slices(T, C, r, R, dtype);
   return slices > 1 ? (size_t)slices * R * r * C * sizeof(float) : 0;
 }
-template <typename T, int JT>
-static int grad_ranks_t(const AdapterGradArgs& a, int slices, float* partial, hipStream_t st) {
-  hipLaunchKernelGGL((adapter_grad_kernel<T, JT>), dim3((a.C + 16 * Few<T>::PER - 1) / (16 * Few<T>::PER), a.R * slices, (a.r + 16 * JT - 1) / (16 * JT)),
-                     dim3(GRAD_NW * 64), 0, st, a, slices, partial);
-  if (int rc = launch_status("adapter_grad_kernel")) return rc;
-  if (slices == 1) return 0;
-  hipLaunchKernelGGL(adapter_grad_join_kernel<T>, dim3((a.C + 255) / 256, a.r, a.R), dim3(256), 0, st, a, slices, partial);
+template <typename T>
+static int grad_t(const GradPair& p, int r, hipStream_t st) {
+  const int64_t blocks = p.of[0].all_blocks() + p.of[1].all_blocks(), joins = p.of[0].all_joins() + p.of[1].all_joins();
+  if (blocks > 0x7fffffffLL || joins > 0x7fffffffLL) { set_error("adapters: too many adapters and columns for one launch"); return SMOE_ERR_RANGE; }
+  if (blocks > 0) {
+    if (grad_ranks(r) == 1) hipLaunchKernelGGL((adapter_grad_kernel<T, 1>), dim3((unsigned)blocks), dim3(GRAD_NW * 64), 0, st, p);
+    else hipLaunchKernelGGL((adapter_grad_kernel<T, 2>), dim3((unsigned)blocks), dim3(GRAD_NW * 64), 0, st, p);
+    if (int rc = launch_status("adapter_grad_kernel")) return rc;
+  }
+  if (joins == 0) return 0;
+  hipLaunchKernelGGL(adapter_grad_join_kernel<T>, dim3((unsigned)joins), dim3(256), 0, st, p);
   return launch_status("adapter_grad_join_kernel");
 }
 template <typename T>
-static int grad_t(const AdapterGradArgs& a, int slices, float* partial, hipStream_t st) {
-  if (a.C >= Few<T>::PER) return grad_ranks(a.r) == 1 ? grad_ranks_t<T, 1>(a, slices, partial, st) : grad_ranks_t<T, 2>(a, slices, partial, st);
+static int grad_any_t(const AdapterGradArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(adapter_grad_any_kernel<T>, dim3((a.C + 63) / 64, a.R), dim3(256), 0, st, a);
   return launch_status("adapter_grad_any_kernel");
 }
@@ -438,10 +469,21 @@ static int project(const AdapterProjectArgs& a, int dtype, hipStream_t st) {
   if (try_adapter_tiles(a, dtype, st, rc)) return rc;
   return dtype == SMOE_F32 ? project_t<float>(a, st) : dtype == SMOE_BF16 ? project_t<bf16_t>(a, st) : project_t<f16_t>(a, st);
 }
-static int grad(const AdapterGradArgs& a, int dtype, void* workspace, hipStream_t st) {
-  const int slices = workspace ? grad_slices(a.T, a.C, a.r, a.R, dtype) : 1;
-  float* p = (float*)workspace;
-  return dtype == SMOE_F32 ? grad_t<float>(a, slices, p, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(a, slices, p, st) : grad_t<f16_t>(a, slices, p, st);
+// Gradients that go into the launch together; one narrower than a piece goes by itself
+static int grads(const AdapterGradArgs* of, void* const* workspace, int n, int dtype, hipStream_t st) {
+  GradPair pair = {};
+  int rank = 1;
+  for (int i = 0; i < n; ++i) {
+    const AdapterGradArgs& a = of[i];
+    if (a.C < pieces(dtype)) {
+      const int rc = dtype == SMOE_F32 ? grad_any_t<float>(a, st) : dtype == SMOE_BF16 ? grad_any_t<bf16_t>(a, st) : grad_any_t<f16_t>(a, st);
+      if (rc) return rc;
+      continue;
+    }
+    rank = a.r;
+    pair.of[i] = GradLaunch{a, grad_slices(a.T, a.C, a.r, a.R, dtype), grad_tiles(a.C, dtype), (int)cdiv64(a.r, 16 * grad_ranks(a.r)), (float*)workspace[i]};
+  }
+  return dtype == SMOE_F32 ? grad_t<float>(pair, rank, st) : dtype == SMOE_BF16 ? grad_t<bf16_t>(pair, rank, st) : grad_t<f16_t>(pair, rank, st);
 }
 static int pack(const AdapterPackArgs& a, const AdapterPackArgs& b, int dtype, hipStream_t st) {
   const int64_t tiles = a.all_tiles() + b.all_tiles();
@@ -469,7 +511,6 @@ struct Space {
 };
 static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 static int64_t width(int dtype) { return dtype == SMOE_F32 ? 4 : 2; }
-static int pieces(int dtype) { return dtype == SMOE_F32 ? 4 : 8; }
 
 static int order_rows(const int64_t* ids, int64_t T, int R, int64_t* idx, int64_t* off, Space& s, hipStream_t st) {
   int64_t* eid = s.take<int64_t>(T);
@@ -558,23 +599,29 @@ static int backward(const AdapterCall& c, Space& s, hipStream_t st) {
     if (int rc = order_rows(c.ids, c.T, c.R, own, own + c.T, s, st)) return rc;
     idx = own, off = own + c.T;
   }
+  AdapterGradArgs of[2];
+  void* ws[2];
+  int n = 0;
   if (dry || c.DX || c.DA) {
     float* V = s.take<float>(c.T * c.r);
     const Product p{c.DY, c.N, c.W, 1, c.K, nullptr, c.B, c.N * c.r, 1, c.r, c.A, c.r * c.K, 1, c.K, dry ? &s : c.DX, V, c.N, c.K};
     if (int rc = product(c, p, idx, off, s, st)) return rc;
-    void* ws = s.bytes((int64_t)grad_bytes(c.T, c.K, c.r, c.R, c.dtype));
-    if (c.DA && !dry) {
-      const AdapterGradArgs g{V, c.X, c.sxm, idx, off, c.DA, c.r * c.K, c.K, 1, c.T, (int)c.K, c.r, c.R};
-      if (int rc = grad(g, c.dtype, ws, st)) return rc;
+    if (dry || c.DA) {
+      ws[n] = s.bytes((int64_t)grad_bytes(c.T, c.K, c.r, c.R, c.dtype));
+      of[n++] = AdapterGradArgs{V, c.X, c.sxm, idx, off, c.DA, c.r * c.K, c.K, 1, c.T, (int)c.K, c.r, c.R};
     }
   }
-  void* ws = s.bytes((int64_t)grad_bytes(c.T, c.N, c.r, c.R, c.dtype));
-  if (c.DB && !dry) {
-    const AdapterGradArgs g{c.U, c.DY, c.N, idx, off, c.DB, c.N * c.r, 1, c.r, c.T, (int)c.N, c.r, c.R};
-    if (int rc = grad(g, c.dtype, ws, st)) return rc;
+  if (dry || c.DB) {
+    ws[n] = s.bytes((int64_t)grad_bytes(c.T, c.N, c.r, c.R, c.dtype));
+    of[n++] = AdapterGradArgs{c.U, c.DY, c.N, idx, off, c.DB, c.N * c.r, 1, c.r, c.T, (int)c.N, c.r, c.R};
   }
-  ws = s.bytes((int64_t)grad_bytes(c.T, c.N, 1, 1, c.dtype));
-  if (c.DBIAS && !dry) return grad(AdapterGradArgs{nullptr, c.DY, c.N, nullptr, nullptr, c.DBIAS, 0, 0, 1, c.T, (int)c.N, 1, 1}, c.dtype, ws, st);
+  if (n > 0 && !dry)
+    if (int rc = grads(of, ws, n, c.dtype, st)) return rc;
+  if (dry || c.DBIAS) {
+    ws[0] = s.bytes((int64_t)grad_bytes(c.T, c.N, 1, 1, c.dtype));
+    of[0] = AdapterGradArgs{nullptr, c.DY, c.N, nullptr, nullptr, c.DBIAS, 0, 0, 1, c.T, (int)c.N, 1, 1};
+    if (!dry) return grads(of, ws, 1, c.dtype, st);
+  }
   return 0;
 }
 

@@ -385,7 +385,7 @@ int smoe_routed_glu_mlp(const void* X, int64_t sxm, int64_t sxk, const void* WR,
   if (!dtype_ok(dtype)) { set_error("smoe_routed_glu_mlp: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
   if (T < 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0 || k > E) { set_error("smoe_routed_glu_mlp: bad sizes"); return SMOE_ERR_SHAPE; }
   if (act != SMOE_ACT_SILU && act != SMOE_ACT_SILU_GATE_FIRST) { set_error("smoe_routed_glu_mlp: unknown activation %d", act); return SMOE_ERR_SHAPE; }
-  if (T > SMOE_FEW_TOKENS || T * k > SMOE_FEW_ROWS || E > 512 || k > 64 || d > 0x3fffffffLL || F > 0x3fffffffLL) {
+  if (T > SMOE_FEW_TOKENS || T * k > SMOE_FEW_ROWS || E > 512 || k > 64 || d > 0x1fffffffLL || F > 0x1fffffffLL) {
     set_error("smoe_routed_glu_mlp: at most %d tokens, %d (token, slot) rows, 512 experts and top-64", SMOE_FEW_TOKENS, SMOE_FEW_ROWS);
     return SMOE_ERR_RANGE;
   }

@@ -208,7 +208,7 @@ def test_library_refuses_before_it_launches():
         return lib.smoe_routed_glu_mlp(x, d, 1, one, d, 1, one, 2 * F * d, d, 1, None, 0, 0, one, F * d, F, 1, None, 0, 0, one, d, one,
                                        T, k, d, F, E, 1, act, dtype, ws, ws_bytes, None)
     assert layer(dtype=5) == -3 and layer(k=0) == -2 and layer(k=9) == -2 and layer(F=0) == -2 and layer(act=3) == -2
-    assert layer(T=65) == -5 and layer(T=64, k=9, E=16) == -5 and layer(E=513) == -5
+    assert layer(T=ops.FEW_TOKENS + 1) == -5 and layer(F=1 << 29) == -5 and layer(T=64, k=9, E=16) == -5 and layer(E=513) == -5
     assert layer(x=None) == -1 and layer(ws=None) == -4 and layer(ws_bytes=1000) == -4 and layer(ws=ctypes.c_void_p(264)) == -4
     assert b"workspace" in lib.smoe_last_error()
     assert layer(T=0) == 0
@@ -226,5 +226,6 @@ def test_library_refuses_before_it_launches():
         return lib.smoe_adapter_backward(dy, one, K, one, one, one, one, None, idx, one, one, one, one, one, one, T, K, N, 8, 3, 1, ws,
                                          ws_bytes, None)
     assert backward(T=0) == -2 and backward(N=0) == -2 and backward(dy=None) == -1 and backward(idx=None) == -1
+    assert backward(T=ops.ADAPTER_FEW_ROWS, idx=None, ws=None) == -4 and backward(T=ops.ADAPTER_FEW_ROWS + 1, idx=None, ws=None) == -1
     assert backward(ws=None) == -4 and backward(ws_bytes=1000) == -4 and backward(T=4, ws=None) == -4
     assert forward(T=0) == 0 and lib.smoe_last_error() == b""
