@@ -8,7 +8,7 @@ from scattermoe_amd import flatten_sort_count, parallel_linear, ParallelExperts,
 
 __all__ = list(_impl.__all__)
 
-for _name in ("parallel_experts", "kernels", "kernels.ops", "kernels.single", "mlp", "utils", "utils.replace_moe"):
+for _name in ("parallel_experts", "kernels", "kernels.ops", "kernels.single", "mlp", "adapters", "utils", "utils.replace_moe"):
     try:
         sys.modules[__name__ + "." + _name] = importlib.import_module("scattermoe_amd." + _name)
     except Exception:      # utils.* needs transformers' model classes only when they exist

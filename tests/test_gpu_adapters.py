@@ -123,6 +123,40 @@ def test_id_types_and_leading_dimensions(itype):
     assert got.shape == (2, 3, 4, 48) and torch.equal(got.view(24, 48), want)
 
 
+def test_without_scales_and_ids_of_one_byte():
+    i, dy = _inputs(70, 64, 48, 5, 8, torch.bfloat16, seed=15)
+    i["scales"] = None
+    i["adapter_idxs"] = torch.where(i["adapter_idxs"] < 0, torch.full_like(i["adapter_idxs"], 255), i["adapter_idxs"]).to(torch.uint8)
+    _compare(i, dy)
+
+
+@pytest.mark.parametrize("T", [40, 300, 1000])
+def test_as_many_adapters_as_there_may_be(T):
+    """2047 adapters, most of them without rows, in a table of more elements than 32 bits count: what holds nothing is not read."""
+    R, r, d, n = 2047, 8, 64, 32
+    i, dy = _inputs(T, d, n, 4, r, torch.bfloat16, seed=16)
+    used = torch.tensor([0, 1023, 1024, 2046], device=DEV)
+    want = _want(i, dy)
+    ids = i["adapter_idxs"]
+    inside = (ids >= 0) & (ids < 4)
+    s = dict(i, adapter_idxs=torch.where(inside, used[ids.clamp(0, 3)], torch.full_like(ids, R)))
+    wide = torch.full((R, r, 1 << 18), float("nan"), dtype=torch.bfloat16, device=DEV)       # 4.3e9 elements, d of each row used
+    s["lora_a"] = wide[:, :, :d]
+    s["lora_a"][used] = i["lora_a"]
+    s["lora_b"] = torch.full((R, n, r), float("nan"), dtype=torch.bfloat16, device=DEV)
+    s["lora_b"][used] = i["lora_b"]
+    s["scales"] = torch.ones(R, device=DEV)
+    s["scales"][used] = i["scales"]
+    y, grads = _step(s, dy, ["x", "lora_a", "lora_b"])
+    _bounds.check("y", y, *want["y"])
+    _bounds.check("dx", grads["x"], *want["dx"])
+    for key, name in (("da", "lora_a"), ("db", "lora_b")):
+        _bounds.check(key, grads[name][used], *want[key])
+        rest = torch.ones(R, dtype=torch.bool, device=DEV)
+        rest[used] = False
+        assert not bool(grads[name][rest].any())
+
+
 def test_no_rows():
     i, _ = _inputs(4, 64, 48, 5, 8, torch.bfloat16)
     s = dict(i, x=i["x"][:0].requires_grad_(), adapter_idxs=i["adapter_idxs"][:0], lora_a=i["lora_a"].clone().requires_grad_(),
@@ -208,6 +242,50 @@ def test_captured_steps_and_eager_work_between():
             want = parallel_adapters(**i)
             torch.cuda.synchronize()
             assert torch.equal(y, want), (T, r)
+
+
+@pytest.mark.parametrize("T", [20, 150, 700])
+def test_captured_gradients(T):
+    """The backward call by itself, captured and replayed with eager work between the replays."""
+    from scattermoe_amd.kernels import ops
+    i, dy = _inputs(T, 96, 64, 5, 8, torch.bfloat16, seed=17)
+    args = (i["x"], i["weight"], i["lora_a"], i["lora_b"], i["adapter_idxs"], i["scales"])
+
+    def both():
+        y, u, order = ops.adapter_forward(*args)
+        return (y,) + ops.adapter_backward(dy, *args, u, order, need_bias=True)
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for r in range(3):
+        g = torch.Generator().manual_seed(r)
+        i["x"].copy_(torch.randn(T, 96, generator=g))
+        dy.copy_(torch.randn(T, 64, generator=g))
+        i["adapter_idxs"].copy_(torch.randint(-1, 6, (T,), generator=g))
+        graph.replay()
+        want = both()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), r
+
+
+def test_two_calls_at_once():
+    """On two streams, over the same weights, while neither waits for the other."""
+    i, dy = _inputs(500, 256, 192, 6, 16, torch.bfloat16, seed=18)
+    j = dict(i, x=torch.randn_like(i["x"]))
+    want = [_step(s, dy) for s in (i, j)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+        got = []
+        for st, s in zip(streams, (i, j)):
+            with torch.cuda.stream(st):
+                got.append(_step(s, dy))
+        torch.cuda.synchronize()
+        for (y, grads), (y2, grads2) in zip(got, want):
+            assert torch.equal(y, y2) and all(torch.equal(grads[n], grads2[n]) for n in grads2)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

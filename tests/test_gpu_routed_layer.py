@@ -223,6 +223,43 @@ def value64(x, wr, i, dy):
     return float((total * dy.double().cpu()).sum())
 
 
+def test_weights_of_more_elements_than_32_bits_count():
+    """512 experts in 10.5 GB: the chosen ones lie far apart, and nothing else is read."""
+    E, F, d, k = 512, 1664, 2048, 2
+    chosen = [1, 300, 510, 511]
+    i = _inputs(6, d, 64, E, torch.bfloat16, seed=31)
+    g = torch.Generator(DEV).manual_seed(0)
+    w1 = torch.full((E, 2 * F, d), float("nan"), dtype=torch.bfloat16, device=DEV)
+    w2 = torch.full((E, d, F), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wr = torch.zeros(E, d, dtype=torch.bfloat16, device=DEV)
+    wr[:, 0] = -4.0
+    i["x"][:, 0] = 1.0
+    for e in chosen:
+        w1[e] = torch.randn(2 * F, d, generator=g, device=DEV) * d ** -0.5
+        w2[e] = torch.randn(d, F, generator=g, device=DEV) * F ** -0.5
+        wr[e] = (torch.randn(d, generator=g, device=DEV) * d ** -0.5).bfloat16()
+    for T in (1, 6):
+        s = dict(i, x=i["x"][:T], wr=wr, w1=w1, w2=w2)
+        out, logits = _call(s, k)
+        small = dict(s, wr=wr[chosen], w1=w1[chosen], w2=w2[chosen])
+        # (the other experts' share of the softmax drops out of the renormalised gates)
+        _compare(small, k, (out, logits[:, chosen]))
+
+
+def test_two_calls_at_once():
+    i, j = _inputs(30, 256, 192, 16, torch.bfloat16, seed=32), _inputs(3, 256, 192, 16, torch.bfloat16, seed=33)
+    want = [_call(s, 2) for s in (i, j)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for st, s in zip(streams, (i, j)):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(_call(s, 2))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+
+
 def test_refusals():
     i = _inputs(4, 64, 32, 8, torch.bfloat16)
     with torch.no_grad():
