@@ -135,20 +135,19 @@ __device__ __forceinline__ void few_tile(Weight weight, Input input, int apart, 
   for (int i = 0; i < G; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int whole = K / BLOCK;
-#pragma unroll 1
-  for (int b = wave; b < whole; b += NW) {
+  // a block's products: all its loads ahead of the first wait
+  auto block = [&](int k0, auto load) {
     i32x4 wv[NT][SIDE], xv[G][H][SIDE];
 #pragma unroll
     for (int s = 0; s < SIDE; ++s) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) wv[j][s] = load_piece<T, ONCE>(w[j] + b * BLOCK + s * STEP);
+      for (int j = 0; j < NT; ++j) wv[j][s] = load(w[j], k0 + s * STEP, std::integral_constant<bool, ONCE>());
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
-        for (int p = 0; p < H; ++p) xv[i][p][s] = load_piece<T, false>(x[i] + p * apart + b * BLOCK + s * STEP);
+        for (int p = 0; p < H; ++p) xv[i][p][s] = load(x[i] + p * apart, k0 + s * STEP, std::false_type());
     }
-    __builtin_amdgcn_sched_barrier(0);                       // (all loads ahead of the first wait)
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s = 0; s < SIDE; ++s)
 #pragma unroll
@@ -157,24 +156,12 @@ __device__ __forceinline__ void few_tile(Weight weight, Input input, int apart, 
         for (int p = 0; p < H; ++p)
 #pragma unroll
           for (int j = 0; j < NT; ++j) acc[i][j] = Few<T>::mma(wv[j][s], xv[i][p][s], acc[i][j]);
-  }
-  if (wave == whole % NW) {
+  };
+  const int whole = K / BLOCK;
 #pragma unroll 1
-    for (int k0 = whole * BLOCK; k0 < K; k0 += STEP) {
-      const int left = K - k0 - l.at;
-      i32x4 wv[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) wv[j] = load_piece_of<T>(w[j] + k0, left);
-#pragma unroll
-      for (int i = 0; i < G; ++i)
-#pragma unroll
-        for (int p = 0; p < H; ++p) {
-          const i32x4 xv = load_piece_of<T>(x[i] + p * apart + k0, left);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = Few<T>::mma(wv[j], xv, acc[i][j]);
-        }
-    }
-  }
+  for (int b = wave; b < whole; b += NW) block(b * BLOCK, [&](const T* p, int k, auto once) { return load_piece<T, decltype(once)::value>(p + k); });
+  if (whole * BLOCK < K && wave == whole % NW)
+    block(whole * BLOCK, [&](const T* p, int k, auto) { return load_piece_of<T>(p + k, K - k - l.at); });
 #pragma unroll
   for (int i = 0; i < G; ++i)
 #pragma unroll

@@ -134,22 +134,22 @@ __device__ __forceinline__ void list_rows(const int* __restrict__ experts, int L
 // Hidden values are held as two parts of the operand's type (float32: one), rows of `ldh` elements
 template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2;
 
-// Hidden rows: a workgroup of four waves has HID_ROWS weight rows (each hidden value's two next to each other) of one expert's
+// Hidden rows: a workgroup of four waves has ROWS weight rows (each hidden value's two next to each other) of one expert's
 // rows; the waves take the contraction's blocks in turn and are added up in LDS.
-static constexpr int HID_NW = 4, HID_ROWS = 32, FEWEST = 4;
+static constexpr int HID_NW = 4, FEWEST = 4;
 static_assert(FEWEST <= HID_NW, "a wave per token");
-template <typename T, int P, int G>
+template <typename T, int P, int G, int ROWS>
 __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int f0, const int* rows, int M, float* part) {
   constexpr int INPUTS = G * 16 / P;
   const T* W = (const T*)a.W1 + e * a.sw1e;
-  few_tile<T, P, G, 1, HID_NW, HID_ROWS, true, G == 4 ? 2 : 0>([&](int n) { return W + (min(f0 + (n >> 1), a.F - 1) + (n & 1 ? a.F : 0)) * a.sw1n; },
+  few_tile<T, P, G, 1, HID_NW, ROWS, true, P == 4 && ROWS == 16 ? 4 : G == 4 ? 2 : 0>([&](int n) { return W + (min(f0 + (n >> 1), a.F - 1) + (n & 1 ? a.F : 0)) * a.sw1n; },
                                          [&](int m) { return (const T*)a.X + rows[min(m, M - 1)] / a.k * a.sxm; }, 0, a.d, part);
   __syncthreads();
   const T* b1 = a.b1 ? (const T*)a.b1 + e * a.sb1e : nullptr;
-  for (int p = threadIdx.x; p < HID_ROWS / 2 * INPUTS; p += HID_NW * 64) {
-    const int m = p / (HID_ROWS / 2), c = p % (HID_ROWS / 2), f = f0 + c;
+  for (int p = threadIdx.x; p < ROWS / 2 * INPUTS; p += HID_NW * 64) {
+    const int m = p / (ROWS / 2), c = p % (ROWS / 2), f = f0 + c;
     if (m >= M || f >= a.F) continue;
-    float first = few_sum<HID_NW, HID_ROWS, INPUTS>(part, 2 * c, m), second = few_sum<HID_NW, HID_ROWS, INPUTS>(part, 2 * c + 1, m);
+    float first = few_sum<HID_NW, ROWS, INPUTS>(part, 2 * c, m), second = few_sum<HID_NW, ROWS, INPUTS>(part, 2 * c + 1, m);
     T* out = (T*)a.hidden + (int64_t)rows[m] * HIDDEN_PARTS<T> * a.ldh + f;
     if (b1) {
       first += to_f32(b1[f * a.sb1n]);
@@ -164,10 +164,10 @@ __device__ __forceinline__ void hidden_tile(const RoutedLayerArgs& a, int e, int
 // GROUPS: 0 for up to 4 tokens, else the groups of 8 rows that a pass over an expert's weights takes (row_groups).  Up to 4 tokens
 // every workgroup makes their selections for itself, a wave each, out of the logits (the first one leaves them to the
 // output's launch): a launch for that would cost more.
-template <typename T, int GROUPS>
+template <typename T, int GROUPS, int ROWS>
 __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) void layer_hidden_kernel(RoutedLayerArgs a) {
   constexpr bool MANY = GROUPS > 0;
-  __shared__ float part[FEW_PART<HID_NW, HID_ROWS, MANY ? GROUPS * 8 : 4>];
+  __shared__ float part[FEW_PART<HID_NW, ROWS, MANY ? GROUPS * 8 : 4>];
   __shared__ RowLists s;
   __shared__ int mine[MANY ? 1 : FEWEST * 64];
   if constexpr (!MANY) {
@@ -184,25 +184,25 @@ __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) 
   if constexpr (!MANY) {
     if (a.T == 1) {                                          // (a token's experts are all different)
       const int row = blockIdx.y;
-      hidden_tile<T, 4, 1>(a, mine[row], blockIdx.x * (HID_ROWS / 2), &row, 1, part);
+      hidden_tile<T, 4, 1, ROWS>(a, mine[row], blockIdx.x * (ROWS / 2), &row, 1, part);
       return;
     }
   }
   list_rows<HID_NW * 64>(MANY ? a.experts : mine, a.T * a.k, a.E, s);
   if ((int)blockIdx.y >= s.hits) return;
-  const int e = s.hit[blockIdx.y], f0 = blockIdx.x * (HID_ROWS / 2);
+  const int e = s.hit[blockIdx.y], f0 = blockIdx.x * (ROWS / 2);
   const int* rows = s.rows + s.first[e];
   if constexpr (MANY) {
     for (int M = s.count[e];;) {
-      if (GROUPS == 1 || M <= 8) hidden_tile<T, 2, 1>(a, e, f0, rows, min(M, 8), part);
-      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, GROUPS == 1 ? 1 : 2>(a, e, f0, rows, min(M, 16), part);
-      else hidden_tile<T, 2, GROUPS>(a, e, f0, rows, min(M, 8 * GROUPS), part);
+      if (GROUPS == 1 || M <= 8) hidden_tile<T, 2, 1, ROWS>(a, e, f0, rows, min(M, 8), part);
+      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, GROUPS == 1 ? 1 : 2, ROWS>(a, e, f0, rows, min(M, 16), part);
+      else hidden_tile<T, 2, GROUPS, ROWS>(a, e, f0, rows, min(M, 8 * GROUPS), part);
       if ((M -= 8 * GROUPS) <= 0) break;
       rows += 8 * GROUPS;
       __syncthreads();
     }
   } else {
-    hidden_tile<T, 4, 1>(a, e, f0, rows, s.count[e], part);
+    hidden_tile<T, 4, 1, ROWS>(a, e, f0, rows, s.count[e], part);
   }
 }
 
@@ -251,14 +251,16 @@ __global__ __launch_bounds__(256) void layer_join_kernel(RoutedLayerArgs a) {
   ((T*)a.OUT)[t * a.som + n] = from_f32<T>(v);
 }
 
-// Output, up to 4 tokens: a workgroup has OUT_COLS output columns of all tokens.  The blocks of the contraction over all hit
+// Output, up to 4 tokens: a workgroup has COLS output columns of all tokens.  The blocks of the contraction over all hit
 // experts are dealt to its waves in pieces of equal length; a wave adds what its share of an expert gives, times the gates, to
 // sums of its own per token in LDS, and the waves' sums are added up at the end in their order.
-static constexpr int OUT_NW = 8, OUT_COLS = 16, OUT_LD = OUT_COLS + 4, OUT_BLOCK = 512;          // (bytes of a row)
-template <typename T>
+static constexpr int OUT_NW = 8;
+template <int COLS> static constexpr int OUT_LD = COLS + 4;
+template <typename T, int COLS> static constexpr int OUT_BLOCK = 8192 / COLS / (int)sizeof(T);          // eight loads of a wave
+template <typename T, int COLS>
 __device__ __forceinline__ void out_share(const RoutedLayerArgs& a, int e, const int* rows, int M, int n0, int b0, int b1, float* sums) {
   typedef FewLane<T, 4> Lane;
-  constexpr int H = HIDDEN_PARTS<T>, NT = OUT_COLS / Lane::ROWS, STEP = Lane::STEP, BLOCK = OUT_BLOCK / (int)sizeof(T), SIDE = BLOCK / STEP;
+  constexpr int H = HIDDEN_PARTS<T>, NT = COLS / Lane::ROWS, STEP = Lane::STEP, BLOCK = OUT_BLOCK<T, COLS>, SIDE = BLOCK / STEP;
   const Lane l;
   const T* w[NT];
 #pragma unroll
@@ -267,41 +269,27 @@ __device__ __forceinline__ void out_share(const RoutedLayerArgs& a, int e, const
   f32x4 acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
-    const int k0 = b * BLOCK;
-    if (k0 + BLOCK <= a.F) {
-      i32x4 wv[NT][SIDE], xv[H][SIDE];
+  auto block = [&](int k0, auto load) {
+    i32x4 wv[NT][SIDE], xv[H][SIDE];
 #pragma unroll
-      for (int s = 0; s < SIDE; ++s) {
+    for (int s = 0; s < SIDE; ++s) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) wv[j][s] = load_piece<T, true>(w[j] + k0 + s * STEP);
+      for (int j = 0; j < NT; ++j) wv[j][s] = load(w[j], k0 + s * STEP, std::true_type());
 #pragma unroll
-        for (int p = 0; p < H; ++p) xv[p][s] = *(const i32x4*)(x + p * a.ldh + k0 + s * STEP);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < SIDE; ++s)
-#pragma unroll
-        for (int p = 0; p < H; ++p)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[j] = Few<T>::mma(wv[j][s], xv[p][s], acc[j]);
-    } else {
-#pragma unroll 1
-      for (int k = k0; k < a.F; k += STEP) {
-        const int left = a.F - k - l.at;
-        i32x4 wv[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) wv[j] = load_piece_of<T>(w[j] + k, left);
-#pragma unroll
-        for (int p = 0; p < H; ++p) {
-          const i32x4 xv = load_piece_of<T>(x + p * a.ldh + k, left);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[j] = Few<T>::mma(wv[j], xv, acc[j]);
-        }
-      }
+      for (int p = 0; p < H; ++p) xv[p][s] = load(x + p * a.ldh, k0 + s * STEP, std::false_type());
     }
-  }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < SIDE; ++s)
+#pragma unroll
+      for (int p = 0; p < H; ++p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = Few<T>::mma(wv[j][s], xv[p][s], acc[j]);
+  };
+  const int whole = min(b1, a.F / BLOCK);
+#pragma unroll 1
+  for (int b = b0; b < whole; ++b) block(b * BLOCK, [&](const T* p, int k, auto once) { return load_piece<T, decltype(once)::value>(p + k); });
+  if (whole < b1) block(whole * BLOCK, [&](const T* p, int k, auto) { return load_piece_of<T>(p + k, a.F - k - l.at); });
   const int row = rows[min(l.sub, M - 1)];
   const float g = a.gates[row];
 #pragma unroll
@@ -311,33 +299,43 @@ __device__ __forceinline__ void out_share(const RoutedLayerArgs& a, int e, const
     const int n = j * Lane::ROWS + l.q;
     if (l.part != 0 || l.sub >= M) continue;
     if (a.b2 && b0 == 0 && n0 + n < a.d) v[0] += to_f32(((const T*)a.b2)[e * a.sb2e + (n0 + n) * a.sb2n]);
-    float* to = sums + row / a.k * OUT_LD + n;
+    float* to = sums + row / a.k * OUT_LD<COLS> + n;
     *to = fmaf(g, v[0], *to);
   }
 }
 
-template <typename T>
+template <typename T, int COLS>
 __global__ __launch_bounds__(OUT_NW * 64) void layer_out_kernel(RoutedLayerArgs a) {
-  __shared__ float sums[OUT_NW][FEWEST * OUT_LD];
+  __shared__ float sums[OUT_NW][FEWEST * OUT_LD<COLS>];
   __shared__ RowLists s;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * OUT_COLS;
-  for (int i = lane_id(); i < a.T * OUT_LD; i += 64) sums[wave][i] = 0.0f;
-  list_rows<OUT_NW * 64>(a.experts, a.T * a.k, a.E, s);
-  constexpr int BLOCK = OUT_BLOCK / (int)sizeof(T);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * COLS;
+  for (int i = lane_id(); i < a.T * OUT_LD<COLS>; i += 64) sums[wave][i] = 0.0f;
+  if (a.T == 1) {                                            // (a token's experts are all different)
+    const int i = threadIdx.x;
+    if (i < a.k) {
+      const int e = a.experts[i];
+      s.hit[i] = e, s.rows[i] = i, s.first[e] = i, s.count[e] = 1;
+    }
+    if (i == 0) s.hits = a.k;
+    __syncthreads();
+  } else {
+    list_rows<OUT_NW * 64>(a.experts, a.T * a.k, a.E, s);
+  }
+  constexpr int BLOCK = OUT_BLOCK<T, COLS>;
   const int nb = (a.F + BLOCK - 1) / BLOCK, total = s.hits * nb;
   const int last = (int)((int64_t)total * (wave + 1) / OUT_NW);
   for (int u = (int)((int64_t)total * wave / OUT_NW); u < last;) {
     const int h = u / nb, b0 = u - h * nb, b1 = min(nb, b0 + last - u);
     const int e = s.hit[h];
-    out_share<T>(a, e, s.rows + s.first[e], s.count[e], n0, b0, b1, sums[wave]);
+    out_share<T, COLS>(a, e, s.rows + s.first[e], s.count[e], n0, b0, b1, sums[wave]);
     u += b1 - b0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * OUT_COLS; i += OUT_NW * 64) {
-    const int t = i / OUT_COLS, n = n0 + i % OUT_COLS;
+  for (int i = threadIdx.x; i < a.T * COLS; i += OUT_NW * 64) {
+    const int t = i / COLS, n = n0 + i % COLS;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < OUT_NW; ++w) v += sums[w][t * OUT_LD + i % OUT_COLS];
+    for (int w = 0; w < OUT_NW; ++w) v += sums[w][t * OUT_LD<COLS> + i % COLS];
     if (n < a.d) ((T*)a.OUT)[t * a.som + n] = from_f32<T>(v);
   }
 }
@@ -352,20 +350,33 @@ size_t routed_layer_workspace_bytes(int64_t T, int k, int64_t d, int64_t F) {
   return 2 * rows_bytes(L) + hidden_bytes(L, F) + (has_out_rows(T) ? (size_t)L * d * sizeof(float) : 0);
 }
 
+static int hit_experts(const RoutedLayerArgs& a) { return std::min(a.E, a.T * a.k); }          // at most
+template <typename T, int GROUPS, int ROWS>
+static int launch_hidden(const RoutedLayerArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((layer_hidden_kernel<T, GROUPS, ROWS>), dim3((2 * a.F + ROWS - 1) / ROWS, hit_experts(a)), dim3(HID_NW * 64), 0, st, a);
+  return launch_status("layer_hidden_kernel");
+}
+template <typename T, int COLS>
+static int launch_out(const RoutedLayerArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((layer_out_kernel<T, COLS>), dim3((a.d + COLS - 1) / COLS), dim3(OUT_NW * 64), 0, st, a);
+  return launch_status("layer_out_kernel");
+}
+// Up to 4 tokens.  Half as much per workgroup where there would be few of them (1 token, 8 of 128 experts, 2048 / 768, us: hidden rows
+// rows 15.6 -> 14.1, output 9.1 -> 7.0).
+static constexpr int FEWEST_WGS = 1024;
+template <typename T>
+static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
+  const int64_t tiles = (int64_t)(2 * a.F + 31) / 32 * hit_experts(a);
+  if (int rc = tiles < FEWEST_WGS ? launch_hidden<T, 0, 16>(a, st) : launch_hidden<T, 0, 32>(a, st)) return rc;
+  return a.d / 16 < 256 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
+}
 template <typename T, int GROUPS>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
-  const int experts = std::min(a.E, a.T * a.k);              // that can be hit
-  hipLaunchKernelGGL((layer_hidden_kernel<T, GROUPS>), dim3((2 * a.F + HID_ROWS - 1) / HID_ROWS, experts), dim3(HID_NW * 64), 0, st, a);
-  if (int rc = launch_status("layer_hidden_kernel")) return rc;
-  if constexpr (GROUPS == 0) {
-    hipLaunchKernelGGL(layer_out_kernel<T>, dim3((a.d + OUT_COLS - 1) / OUT_COLS), dim3(OUT_NW * 64), 0, st, a);
-    return launch_status("layer_out_kernel");
-  } else {
-    hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS>), dim3((a.d + TILE_COLS - 1) / TILE_COLS, experts), dim3(TILE_NW * 64), 0, st, a);
-    if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
-    hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);
-    return launch_status("layer_join_kernel");
-  }
+  if (int rc = launch_hidden<T, GROUPS, 32>(a, st)) return rc;
+  hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS>), dim3((a.d + TILE_COLS - 1) / TILE_COLS, hit_experts(a)), dim3(TILE_NW * 64), 0, st, a);
+  if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
+  hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);
+  return launch_status("layer_join_kernel");
 }
 
 template <typename T>
@@ -373,7 +384,7 @@ static int launch_t(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(layer_logits_kernel<T>, dim3((a.E + DOT_ROWS - 1) / DOT_ROWS, a.T), dim3(DOT_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_logits_kernel")) return rc;
   const bool streams = a.sxk == 1 && a.sw1k == 1 && a.sw2k == 1 && std::min(a.d, a.F) >= Few<T>::PER;
-  if (streams && a.T <= FEWEST) return launch_streams<T, 0>(a, st);
+  if (streams && a.T <= FEWEST) return launch_fewest<T>(a, st);
   hipLaunchKernelGGL(layer_select_kernel, dim3(a.T), dim3(64), 0, st, a);
   if (int rc = launch_status("layer_select_kernel")) return rc;
   if (streams) {
