@@ -361,14 +361,15 @@ static int launch_out(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((layer_out_kernel<T, COLS>), dim3((a.d + COLS - 1) / COLS), dim3(OUT_NW * 64), 0, st, a);
   return launch_status("layer_out_kernel");
 }
-// Up to 4 tokens.  Half as much per workgroup where there would be few of them (1 token, 8 of 128 experts, 2048 / 768, us: hidden rows
-// rows 15.6 -> 14.1, output 9.1 -> 7.0).
-static constexpr int FEWEST_WGS = 1024;
+// Up to 4 tokens.  Half as much per workgroup where there would be few of them, us, whole against half: 1 token, 8 of 128 experts,
+// 2048 / 768 (384 workgroups): hidden 15.6 against 14.1, output 9.1 against 7.0; 1 token, 4 of 32 experts, 2880 / 2880 (720
+// workgroups): hidden 24.8 against 28.0, output (180 of 16 columns) 14.2 against 15.8.
+static constexpr int FEWEST_WGS = 512;
 template <typename T>
 static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
   const int64_t tiles = (int64_t)(2 * a.F + 31) / 32 * hit_experts(a);
   if (int rc = tiles < FEWEST_WGS ? launch_hidden<T, 0, 16>(a, st) : launch_hidden<T, 0, 32>(a, st)) return rc;
-  return a.d / 16 < 256 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
+  return a.d / 16 < 160 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
 }
 template <typename T, int GROUPS>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
