@@ -534,8 +534,6 @@ struct Product {
   float* U;
   int64_t K, N;
 };
-// Up to so many multiply-adds a strided factor is looked up element by element: a copy's launch costs more
-static constexpr int64_t LOOK_UP = 1 << 22;
 // Rows from which 16-bit products go in tiles, fewer where there is more to do: the rows' own kernel reads the weights once per 32
 // rows, but has a workgroup per 16 columns (us of a call, row by row / tiles: 80 rows, 4096 -> 4096 33 / 42; 128 rows 40 / 42; 256
 // rows 63 / 43; 100 rows, 2048 -> 2048 18 / 28; 300 rows, 512 -> 512 13 / 17; 777 rows, 2880 -> 2880 93 / 42)
@@ -554,7 +552,9 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
     s0 = n1 * ld, s1 = ld, s2 = 1;
   };
   int64_t zero = 0, one = 1;
-  if (p.sak != 1 && p.K >= pieces(c.dtype) && (tiles || c.T * p.K * c.r > LOOK_UP)) copy(p.A, p.sar, p.saj, p.sak, c.R, c.r, p.K, p.K);
+  // (also where the rows are few; us of a backward call, bf16, elements looked up where they lie / copied first: 1 row 4096 -> 4096,
+  // rank 16 87 / 50; 64 rows 1024 -> 1024 31 / 24; 16 rows 2048 -> 2048, rank 64 159 / 85)
+  if (p.sak != 1 && p.K >= pieces(c.dtype)) copy(p.A, p.sar, p.saj, p.sak, c.R, c.r, p.K, p.K);
   const void* X = p.X;
   int64_t sxm = p.sxm, K = p.K;
   if (p.Y != nullptr && tiles) {
