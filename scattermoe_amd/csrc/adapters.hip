@@ -538,9 +538,14 @@ struct Product {
 // rows, but has a workgroup per 16 columns (us of a call, row by row / tiles: 80 rows, 4096 -> 4096 33 / 42; 128 rows 40 / 42; 256
 // rows 63 / 43; 100 rows, 2048 -> 2048 18 / 28; 300 rows, 512 -> 512 13 / 17; 777 rows, 2880 -> 2880 93 / 42)
 static constexpr int64_t TILES_MIN_ROWS = 320, TILES_MIN_WORK = 2000000000;
+// ... and a shared weight whose contraction is strided (dx) would be copied for the rows' kernel: tiles earlier, where the copy is
+// long and there are tiles enough (us of a backward call, row by row / tiles: 65 rows, 4096 -> 4096 65 / 51; 120, 2880 -> 2880 69 / 55;
+// 300, 2048 -> 2048 47 / 37; 128, 768 -> 8192 101 / 40; but 300, 512 -> 512 19 / 22; 65, 8192 -> 768 63 / 85)
+static constexpr int64_t COPY_MIN = 1 << 22, COPY_MIN_TILES = 32;
 static int product(const AdapterCall& c, Product p, const int64_t* idx, const int64_t* off, Space& s, hipStream_t st) {
   const bool many = c.T > ADAPTER_FEW_ROWS;
-  const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && c.T * p.N * p.K > TILES_MIN_WORK));
+  const bool long_copy = p.swk != 1 && p.N * p.K >= COPY_MIN && cdiv64(c.T, 64) * cdiv64(p.N, 128) >= COPY_MIN_TILES;
+  const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && (long_copy || c.T * p.N * p.K > TILES_MIN_WORK)));
   const int64_t w = width(c.dtype);
   // The copies, at most the factors' and those of the shared product, in pairs
   AdapterPackArgs copies[4] = {};

@@ -72,6 +72,14 @@ def test_large_tiles(T, d, n, R, r, grouped, dtype):
     _compare(i, dy)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,d,n,R,r", [(65, 4096, 1024, 6, 16), (130, 2056, 2048, 9, 5), (319, 2048, 2050, 200, 40)])
+def test_few_rows_beside_a_large_weight(T, d, n, R, r, dtype):
+    """The gradient of the input in tiles, the output row by row or in tiles too."""
+    i, dy = _inputs(T, d, n, R, r, dtype, bias=False, grouped=False, seed=T + d)
+    _compare(i, dy)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [5, 64, 200])
 @pytest.mark.parametrize("which", ["none", "one", "last"])
