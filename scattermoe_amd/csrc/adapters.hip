@@ -381,12 +381,6 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPacks packs) {
   }
 }
 
-// Ids of adapters as 32-bit ones of R + 1 groups: rows without an adapter are the last group
-__global__ __launch_bounds__(256) void adapter_groups_kernel(const int64_t* ids, int64_t T, int R, int* out) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t < T) out[t] = (uint64_t)ids[t] < (uint64_t)R ? (int)ids[t] : R;
-}
-
 template <typename T>
 static int low_t(const AdapterLowArgs& a, hipStream_t st) {
   const bool pieces = a.sak == 1 && a.K >= Few<T>::PER;
@@ -514,12 +508,9 @@ static int64_t width(int dtype) { return dtype == SMOE_F32 ? 4 : 2; }
 
 static int order_rows(const int64_t* ids, int64_t T, int R, int64_t* idx, int64_t* off, Space& s, hipStream_t st) {
   int64_t* eid = s.take<int64_t>(T);
-  int* groups = s.take<int>(T);
   char* ws = s.bytes((int64_t)route_workspace_bytes(T, R + 1));
   if (s.dry()) return 0;
-  hipLaunchKernelGGL(adapter_groups_kernel, dim3((unsigned)cdiv64(T, 256)), dim3(256), 0, st, ids, T, R, groups);
-  if (int rc = launch_status("adapter_groups_kernel")) return rc;
-  return launch_route(groups, SMOE_I32, T, R + 1, eid, idx, off, ws, st);
+  return launch_route_adapters(ids, T, R, eid, idx, off, ws, st);
 }
 
 // Y = X W^T (+ bias) + U B[a]^T with U = s A[a] X, for factors in any order: the product both ways.  `off` (with the rows in order):

@@ -467,6 +467,8 @@ int launch_topk_softmax(const void* logits, int64_t slt, int64_t sle, float* w, 
                         hipStream_t st);
 int launch_route(const void* expert_idxs, int idx_dtype, int64_t L, int E, int64_t* eid_out,
                  int64_t* idx_out, int64_t* off_out, void* ws, hipStream_t st);
+int launch_route_adapters(const int64_t* ids, int64_t L, int R, int64_t* eid_out, int64_t* idx_out, int64_t* off_out, void* workspace,
+                          hipStream_t st);
 size_t route_workspace_bytes(int64_t L, int E);
 int launch_route_static(const void* expert_idxs, int idx_dtype, int64_t L, int E, int64_t* eid_out,
                         int64_t* idx_out, int64_t* off_out, hipStream_t st);

@@ -25,6 +25,12 @@ static constexpr int kRouteFusedMaxE = 512;    // ... for at most this many expe
 // An id is compared at its full width: the low half of a 64-bit id that is no expert may look like one.
 template <typename I>
 __device__ __forceinline__ bool is_expert(I id, int E) { return (uint64_t)(int64_t)id < (uint64_t)E; }
+// The expert that an id names, -1 for none
+template <typename I>
+__device__ __forceinline__ int expert_of(I id, int E) { return is_expert(id, E) ? (int)id : -1; }
+// Ids of adapters: whatever is none of the first E - 1 is of the last group (launch_route_adapters)
+struct AdapterId { int64_t id; };
+__device__ __forceinline__ int expert_of(AdapterId a, int E) { return is_expert(a.id, E - 1) ? (int)a.id : E - 1; }
 
 // Lanes of the wave that hold the same key as this lane (keys < 2^nbits), inactive lanes excluded.
 __device__ __forceinline__ unsigned long long match_any(int key, int nbits, bool active) {
@@ -57,12 +63,12 @@ __device__ __forceinline__ void wave_rank(const I* __restrict__ ids, int64_t seg
 #pragma unroll
   for (int u = 0; u < IT; ++u) {
     const int64_t p = seg_lo + u * 64 + lane;
-    id[u] = p < seg_hi ? ids[p] : (I)0;
+    id[u] = p < seg_hi ? ids[p] : I{};
   }
 #pragma unroll
   for (int u = 0; u < IT; ++u) {
-    const bool ok = seg_lo + u * 64 + lane < seg_hi && is_expert(id[u], E);
-    key[u] = ok ? (int)id[u] : -1;
+    key[u] = seg_lo + u * 64 + lane < seg_hi ? expert_of(id[u], E) : -1;
+    const bool ok = key[u] >= 0;
     loc[u] = 0;
     if (seg_lo + u * 64 < seg_hi) {
       const unsigned long long same = match_any(ok ? key[u] : 0, nbits, ok);
@@ -171,8 +177,8 @@ __global__ __launch_bounds__(THREADS) void route_hist_kernel(
   const int64_t lo = (int64_t)blockIdx.x * kRouteChunk;
   const int64_t hi = min(lo + kRouteChunk, L);
   for (int64_t p = lo + tid; p < hi; p += THREADS) {
-    const I id = ids[p];
-    if (is_expert(id, E)) atomicAdd(&lds[(int)id], 1);
+    const int e = expert_of(ids[p], E);
+    if (e >= 0) atomicAdd(&lds[e], 1);
   }
   __syncthreads();
   for (int i = tid; i < E; i += THREADS) counts[(int64_t)blockIdx.x * E + i] = lds[i];
@@ -392,6 +398,16 @@ int launch_route(const void* ids, int idx_dtype, int64_t L, int E, int64_t* eid_
     case SMOE_U8: return launch_route_t((const uint8_t*)ids, L, E, eid_out, idx_out, off_out, ws, st);
     default: set_error("smoe_route: unknown index dtype %d", idx_dtype); return SMOE_ERR_DTYPE;
   }
+}
+
+// Rows in the order of their adapters: R + 1 groups, those without an adapter the last
+int launch_route_adapters(const int64_t* ids, int64_t L, int R, int64_t* eid_out, int64_t* idx_out, int64_t* off_out, void* ws,
+                          hipStream_t st) {
+  if (R >= kRouteMaxE) {
+    set_error("adapters: R=%d exceeds the supported maximum %d", R, kRouteMaxE - 1);
+    return SMOE_ERR_RANGE;
+  }
+  return launch_route_t((const AdapterId*)ids, L, R + 1, eid_out, idx_out, off_out, ws, st);
 }
 
 // off[e] = number of rows with id <= e, from an ascending id vector.  Boundary n (between rows n-1
