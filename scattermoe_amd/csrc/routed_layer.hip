@@ -3,8 +3,13 @@
 //   S[t, :] = the k largest of l[t, :],  g[t, j] = softmax(l[t, :])[S[t, j]]  (divided by their sum when renormalised)
 //   h[t, j] = a * silu(b),  (a, b) the halves of W1[e] X[t] + b1[e],  e = S[t, j]
 //   OUT[t]  = sum_j g[t, j] (W2[e] h[t, j] + b2[e])
-// in three or four launches: logits, selection (up to 4 tokens: inside the next), hidden rows, output.  The hidden rows, like every sum, stay in
-// float32; the only rounding of the layer is the output's.
+// in three launches up to 4 tokens (logits; hidden rows, selection inside; output) and five beyond (logits, selection, hidden rows,
+// output rows, their sum).  Every sum stays in float32, the hidden rows in two parts of the operand's type (few_rows.hpp, split): the
+// only rounding of the layer is the output's.  A hidden value beyond float16's range is infinite, as in the general path.
+//
+// What bounds it: the weights of the experts that were hit, read once; a kernel that only reads reaches 6.3 to 6.75 TB/s here.
+// us, all launches (weights at TB/s): 1 token, 8 of 128 experts, 2048 / 768 24.2 (3.1; launches that depend on each other);
+// 1 token, 2 of 8, 4096 / 14336 118 (6.0); 17 tokens, 4 of 32, 2880 / 2880 222 (6.4); 64 tokens, 8 of 128, 2048 / 768 220 (5.4).
 //
 // Counterpart in the reference: the router, softmax and top-k of its Hugging Face injection (scattermoe/utils/replace_moe.py:60-95)
 // and GLUMLP.forward (scattermoe/mlp.py:74-95) behind them.
@@ -23,7 +28,8 @@ __device__ __forceinline__ float lane_dot(const A* __restrict__ a, int64_t sa, c
 }
 
 // ---- routing --------------------------------------------------------------------------------------------------------
-// The logits of DOT_ROWS experts and one token by a workgroup
+// The logits of DOT_ROWS experts and one token by a workgroup.  Bound by latency: 1 token, 128 experts of 2048 4.1 us, 64 tokens 7.8 us
+// (33 MB read from the caches).
 template <typename T>
 __global__ __launch_bounds__(DOT_NW * 64) void layer_logits_kernel(RoutedLayerArgs a) {
   __shared__ float part[DOT_NW * DOT_ROWS];
@@ -42,7 +48,7 @@ __global__ __launch_bounds__(DOT_NW * 64) void layer_logits_kernel(RoutedLayerAr
   }
 }
 
-// Selection of token t by one wave; `expert(j, e)` and the returned gates as select_experts
+// Selection of token t by one wave (64 tokens, 8 of 128 experts 5.5 us, k rounds of a maximum across the wave); `expert(j, e)` and the returned gates as select_experts
 template <class Expert>
 __device__ __forceinline__ float layer_select(const RoutedLayerArgs& a, int t, Expert expert) {
   const float* l = a.LOGITS + (int64_t)t * a.E;
@@ -135,7 +141,9 @@ __device__ __forceinline__ void list_rows(const int* __restrict__ experts, int L
 template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2;
 
 // Hidden rows: a workgroup of four waves has ROWS weight rows (each hidden value's two next to each other) of one expert's
-// rows; the waves take the contraction's blocks in turn and are added up in LDS.
+// rows; the waves take the contraction's blocks in turn and are added up in LDS.  Two weight rows of each hidden value meet in one
+// workgroup, so its halves need no trip through memory.  us (weights at TB/s): 1 token, 2048 -> 2 x 768, 8 experts 14.0 (3.6); 1 token,
+// 4096 -> 2 x 14336, 2 experts 75.9 (6.2); 17 tokens, 2880 -> 2 x 2880, 29 experts 139 (6.9); 64 tokens, 126 experts 132 (6.0).
 static constexpr int HID_NW = 4, FEWEST = 4;
 static_assert(FEWEST <= HID_NW, "a wave per token");
 template <typename T, int P, int G, int ROWS>
@@ -207,7 +215,9 @@ __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) 
 }
 
 // Output, more than 4 tokens: tiles as the hidden rows', TILE_COLS output columns of one expert's rows each, left times their gates in
-// float32; the join adds up a token's rows.  (Rows of T * k * d sums written and read are a few percent of the weights.)
+// float32; the join adds up a token's rows in the order of their slots, so that no atomics decide it.  (Rows of T * k * d sums written
+// and read are a few percent of the weights.)  us (weights at TB/s): 17 tokens, 2880 -> 2880, 29 experts 73.2 (6.6); 64 tokens,
+// 768 -> 2048, 126 experts 76.0 (5.2: one or two blocks of the contraction per wave) and 4.9 for the join.
 static constexpr int TILE_NW = 4, TILE_COLS = 32;
 template <typename T, int P, int G>
 __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0, const int* rows, int M, float* part) {
@@ -253,7 +263,8 @@ __global__ __launch_bounds__(256) void layer_join_kernel(RoutedLayerArgs a) {
 
 // Output, up to 4 tokens: a workgroup has COLS output columns of all tokens.  The blocks of the contraction over all hit
 // experts are dealt to its waves in pieces of equal length; a wave adds what its share of an expert gives, times the gates, to
-// sums of its own per token in LDS, and the waves' sums are added up at the end in their order.
+// sums of its own per token in LDS, and the waves' sums are added up at the end in their order.  us (weights at TB/s): 1 token,
+// 768 -> 2048, 8 experts 7.3 (3.4); 14336 -> 4096, 2 experts 37.8 (6.2).
 static constexpr int OUT_NW = 8;
 template <int COLS> static constexpr int OUT_LD = COLS + 4;
 template <typename T, int COLS> static constexpr int OUT_BLOCK = 8192 / COLS / (int)sizeof(T);          // eight loads of a wave
