@@ -220,6 +220,37 @@ def test_values_that_are_not_finite_stay_in_their_rows(T, dtype):
     assert bool(torch.isnan(got[3]).all()) and not bool(torch.isfinite(got[5]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,d,n,grouped", [(700, 1024, 1024, False), (700, 1024, 1024, True), (3000, 1792, 4096, True), (3000, 256, 4096, False)])
+def test_values_that_are_not_finite_stay_in_their_rows_of_tiles(T, d, n, grouped, dtype):
+    """Tiles of every class; the adapter beside, before and behind others and rows without one, in runs of its own or alone."""
+    i, dy = _inputs(T, d, n, 5, 8, dtype, bare=0.2, grouped=grouped, seed=21)
+    y, grads = _step(i, dy)
+    ids = i["adapter_idxs"]
+    for a in (0, 2, 4):
+        s = dict(i, lora_a=i["lora_a"].clone(), lora_b=i["lora_b"].clone())
+        s["lora_a"][a, 2] = float("inf")
+        s["lora_b"][a, 9] = float("nan")
+        got, g = _step(s, dy)
+        keep, others = ids != a, [j for j in range(5) if j != a]
+        assert torch.equal(got[keep], y[keep]) and bool(torch.isnan(got[~keep, 9]).all())
+        assert torch.equal(g["x"][keep], grads["x"][keep])
+        for name in ("lora_a", "lora_b"):
+            assert torch.equal(g[name][others], grads[name][others])
+
+
+@pytest.mark.parametrize("T", [5, 100, 700])
+def test_broadcast_rows_and_a_broadcast_gradient(T):
+    """One row for all, and the gradient of a sum: strides of zero either way."""
+    i, _ = _inputs(T, 256, 192, 4, 8, torch.bfloat16, bias=True, seed=22)
+    i["x"] = i["x"][:1].expand(T, 256)
+    dy = torch.ones(1, 1, dtype=torch.bfloat16, device=DEV).expand(T, 192)
+    y, grads = _step(i, dy)
+    want, grads_want = _step(dict(i, x=i["x"].contiguous()), dy.contiguous())
+    assert torch.equal(y, want) and all(torch.equal(grads[n], grads_want[n]) for n in grads)
+    _bounds.check("y", y, *_want(i)["y"])
+
+
 @pytest.mark.parametrize("T", [9, 200])
 def test_same_bits_every_time_and_on_another_stream(T):
     i, dy = _inputs(T, 128, 96, 6, 16, torch.bfloat16, seed=13)
