@@ -382,9 +382,19 @@ static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
   if (int rc = tiles < FEWEST_WGS ? launch_hidden<T, 0, 16>(a, st) : launch_hidden<T, 0, 32>(a, st)) return rc;
   return a.d / 16 < 160 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
 }
+// More than 4 tokens: 16 weight rows per workgroup, so that a wave has more of each on its way, for float32, and for 16 bits
+// where few rows of an expert meet long weight rows.  us of a layer, 32 / 16: float32, 8 tokens, 4 of 32 experts, 2880 / 720 121 / 96,
+// 8 of 128, 2048 / 768 186 / 165; bf16, 8 tokens, 4 of 32, 2880 / 2880 180 / 165, 12 tokens 217 / 195; 16 tokens, 2 of 16, 4096 / 1024
+// 76 / 63; 8 tokens, 8 of 128, 2048 / 768 94 / 98; and where it does not hold, 64 tokens, 8 of 128, 2048 / 768 224 / 233; 16 tokens, 4
+// of 60, 1536 / 1536 95 / 100.
 template <typename T, int GROUPS>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
-  if (int rc = launch_hidden<T, GROUPS, 32>(a, st)) return rc;
+  if constexpr (GROUPS == 1) {
+    const bool narrow = sizeof(T) == 4 || (a.d >= 2048 && a.T * a.k <= 2 * a.E);
+    if (int rc = narrow ? launch_hidden<T, 1, 16>(a, st) : launch_hidden<T, 1, 32>(a, st)) return rc;
+  } else {
+    if (int rc = launch_hidden<T, GROUPS, 32>(a, st)) return rc;
+  }
   hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS>), dim3((a.d + TILE_COLS - 1) / TILE_COLS, hit_experts(a)), dim3(TILE_NW * 64), 0, st, a);
   if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
   hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);

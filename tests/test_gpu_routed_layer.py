@@ -44,6 +44,14 @@ def test_layer(T, d, F, E, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,d,F,E,k", [(5, 2048, 72, 32, 4), (16, 2500, 40, 20, 2), (9, 2051, 33, 64, 3), (3, 2880, 1440, 16, 4), (11, 2056, 264, 6, 1)])
+def test_long_weight_rows(T, d, F, E, k, dtype):
+    """Workgroups of fewer or more weight rows, widths that no block of the contraction divides."""
+    i = _inputs(T, d, F, E, dtype, bias=T % 2 == 1, seed=T + d)
+    _compare(i, k, _call(i, k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("renormalize,gate_first", [(False, False), (True, True), (False, True)])
 def test_conventions(renormalize, gate_first, dtype):
     i = _inputs(6, 96, 72, 10, dtype, bias=True, seed=3)
