@@ -24,9 +24,9 @@ def _call(i, k, **kw):
         return routed_glu_mlp(i["x"], i["wr"], i["w1"], i["w2"], k, b1=i["b1"], b2=i["b2"], **kw)
 
 
-def _compare(i, k, got, **kw):
+def _compare(i, k, got, least=0.9, **kw):
     out, bound, logits, logits_bound, clear = _bounds.layer(i["x"], i["wr"], i["w1"], i["w2"], k, i["b1"], i["b2"], **kw)
-    assert int(clear.sum()) >= 0.9 * len(clear)
+    assert int(clear.sum()) >= least * len(clear)
     _bounds.check("logits", got[1], logits, logits_bound)
     _bounds.check("out", got[0].cpu().reshape(out.shape)[clear], out[clear], bound[clear])
 
@@ -48,7 +48,9 @@ def test_layer(T, d, F, E, k, dtype):
 def test_long_weight_rows(T, d, F, E, k, dtype):
     """Workgroups of fewer or more weight rows, widths that no block of the contraction divides."""
     i = _inputs(T, d, F, E, dtype, bias=T % 2 == 1, seed=T + d)
-    _compare(i, k, _call(i, k))
+    # (of so few tokens one or two whose k-th and next logits lie within twice the logits' own bound of each other - sums of
+    # 2051 products and 64 experts to choose from - are more than a tenth; which of them is taken is then no error)
+    _compare(i, k, _call(i, k), least=0.7)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
