@@ -218,8 +218,8 @@ __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) 
 // float32; the join adds up a token's rows in the order of their slots, so that no atomics decide it.  (Rows of T * k * d sums written
 // and read are a few percent of the weights.)  us (weights at TB/s): 17 tokens, 2880 -> 2880, 29 experts 73.2 (6.6); 64 tokens,
 // 768 -> 2048, 126 experts 76.0 (5.2: one or two blocks of the contraction per wave) and 4.9 for the join.
-static constexpr int TILE_NW = 4, TILE_COLS = 32;
-template <typename T, int P, int G>
+static constexpr int TILE_NW = 4;
+template <typename T, int P, int G, int TILE_COLS>
 __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0, const int* rows, int M, float* part) {
   constexpr int INPUTS = G * 16 / P, H = HIDDEN_PARTS<T>;
   const T* W = (const T*)a.W2 + e * a.sw2e;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void out_tile(const RoutedLayerArgs& a, int e, int n0
     a.out_rows[(int64_t)rows[m] * a.d + n] = a.gates[rows[m]] * v;
   }
 }
-template <typename T, int GROUPS>
+template <typename T, int GROUPS, int TILE_COLS>
 __global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) void layer_out_tiles_kernel(RoutedLayerArgs a) {
   __shared__ float part[FEW_PART<TILE_NW, TILE_COLS, GROUPS * 8>];
   __shared__ RowLists s;
@@ -244,9 +244,9 @@ __global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4)
   const int e = s.hit[blockIdx.y], n0 = blockIdx.x * TILE_COLS;
   const int* rows = s.rows + s.first[e];
   for (int M = s.count[e];;) {
-    if (GROUPS == 1 || M <= 8) out_tile<T, 2, 1>(a, e, n0, rows, min(M, 8), part);
-    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, GROUPS == 1 ? 1 : 2>(a, e, n0, rows, min(M, 16), part);
-    else out_tile<T, 2, GROUPS>(a, e, n0, rows, min(M, 8 * GROUPS), part);
+    if (GROUPS == 1 || M <= 8) out_tile<T, 2, 1, TILE_COLS>(a, e, n0, rows, min(M, 8), part);
+    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, GROUPS == 1 ? 1 : 2, TILE_COLS>(a, e, n0, rows, min(M, 16), part);
+    else out_tile<T, 2, GROUPS, TILE_COLS>(a, e, n0, rows, min(M, 8 * GROUPS), part);
     if ((M -= 8 * GROUPS) <= 0) break;
     rows += 8 * GROUPS;
     __syncthreads();
@@ -367,6 +367,11 @@ static int launch_hidden(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((layer_hidden_kernel<T, GROUPS, ROWS>), dim3((2 * a.F + ROWS - 1) / ROWS, hit_experts(a)), dim3(HID_NW * 64), 0, st, a);
   return launch_status("layer_hidden_kernel");
 }
+template <typename T, int GROUPS, int COLS>
+static int launch_out_tiles(const RoutedLayerArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS, COLS>), dim3((a.d + COLS - 1) / COLS, hit_experts(a)), dim3(TILE_NW * 64), 0, st, a);
+  return launch_status("layer_out_tiles_kernel");
+}
 template <typename T, int COLS>
 static int launch_out(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((layer_out_kernel<T, COLS>), dim3((a.d + COLS - 1) / COLS), dim3(OUT_NW * 64), 0, st, a);
@@ -382,21 +387,26 @@ static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
   if (int rc = tiles < FEWEST_WGS ? launch_hidden<T, 0, 16>(a, st) : launch_hidden<T, 0, 32>(a, st)) return rc;
   return a.d / 16 < 160 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
 }
-// More than 4 tokens: 16 weight rows per workgroup, so that a wave has more of each on its way, for float32, and for 16 bits
-// where few rows of an expert meet long weight rows.  us of a layer, 32 / 16: float32, 8 tokens, 4 of 32 experts, 2880 / 720 121 / 96,
-// 8 of 128, 2048 / 768 186 / 165; bf16, 8 tokens, 4 of 32, 2880 / 2880 180 / 165, 12 tokens 217 / 195; 16 tokens, 2 of 16, 4096 / 1024
-// 76 / 63; 8 tokens, 8 of 128, 2048 / 768 94 / 98; and where it does not hold, 64 tokens, 8 of 128, 2048 / 768 224 / 233; 16 tokens, 4
-// of 60, 1536 / 1536 95 / 100.
+// More than 4 tokens, eight rows of an expert per pass: 16 weight rows per workgroup instead of 32, so that a wave has more of each on
+// its way, where weight rows are long and, 16 bits, few rows of an expert meet them.  us of a layer, 32 / 16 for both products: bf16, 2 of
+// 16 experts, 1024 / 4096, 5 tokens 53 / 50, 16 tokens 74 / 70; 4 of 32, 2880 / 2880, 5 tokens 129 / 126; for the hidden rows 4 of 32,
+// 2048 / 1024, 16 tokens 68 / 65; float32, 4 of 32, 2880 / 2880, 12 tokens 420 / 399; 2 of 16, 4096 / 1024, 16 tokens 149 / 142.
+// Where it does not hold: bf16, 8 of 128, 2048 / 768, 64 tokens 227 / 245; 4 of 64, 512 / 3584, 20 tokens 100 / 123; float32, 8 of
+// 128, 2048 / 768 (the output) 404 / 423.
+static constexpr int LONG_ROW = 3500;                        // bytes
+template <typename T>
+static bool few_per_workgroup(const RoutedLayerArgs& a, int length) {
+  return (int64_t)length * (int64_t)sizeof(T) >= LONG_ROW && (sizeof(T) == 4 || a.T * a.k <= 2 * a.E);
+}
 template <typename T, int GROUPS>
 static int launch_streams(const RoutedLayerArgs& a, hipStream_t st) {
   if constexpr (GROUPS == 1) {
-    const bool narrow = sizeof(T) == 4 || (a.d >= 2048 && a.T * a.k <= 2 * a.E);
-    if (int rc = narrow ? launch_hidden<T, 1, 16>(a, st) : launch_hidden<T, 1, 32>(a, st)) return rc;
+    if (int rc = few_per_workgroup<T>(a, a.d) ? launch_hidden<T, 1, 16>(a, st) : launch_hidden<T, 1, 32>(a, st)) return rc;
+    if (int rc = few_per_workgroup<T>(a, a.F) ? launch_out_tiles<T, 1, 16>(a, st) : launch_out_tiles<T, 1, 32>(a, st)) return rc;
   } else {
     if (int rc = launch_hidden<T, GROUPS, 32>(a, st)) return rc;
+    if (int rc = launch_out_tiles<T, GROUPS, 32>(a, st)) return rc;
   }
-  hipLaunchKernelGGL((layer_out_tiles_kernel<T, GROUPS>), dim3((a.d + TILE_COLS - 1) / TILE_COLS, hit_experts(a)), dim3(TILE_NW * 64), 0, st, a);
-  if (int rc = launch_status("layer_out_tiles_kernel")) return rc;
   hipLaunchKernelGGL(layer_join_kernel<T>, dim3((a.d + 255) / 256, a.T), dim3(256), 0, st, a);
   return launch_status("layer_join_kernel");
 }
