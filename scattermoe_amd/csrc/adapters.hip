@@ -143,6 +143,7 @@ __global__ __launch_bounds__(DOT_NW * 64) void adapter_low_dots_kernel(AdapterLo
 // from memory once, the factor's from the caches: rows of one adapter follow one another.)  8192 rows of 4096, rank 16 17.3 us: 67 MB
 // of rows at 3.9 TB/s; 1777 rows of 2048, rank 64 9.3 us, four workgroups reading a row.
 static constexpr int LOW_NW = 8, LOW_RANKS = 16;
+static_assert(LOW_RANKS == 16, "exponents of the planes: one for the 16 ranks of a workgroup");
 template <typename T>
 __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(AdapterLowArgs a) {
   __shared__ float part[FEW_PART<LOW_NW, LOW_RANKS, 16>];
@@ -153,8 +154,14 @@ __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(Adapte
     if (threadIdx.x < 16) s[threadIdx.x] = has && (int)threadIdx.x < rows ? (int)a.idx[row0 + threadIdx.x] : -1;
     else s[16] = has && id < a.R ? id : -1;
   }
-  if (!has) return;
   const int m_ = threadIdx.x / LOW_RANKS, n_ = threadIdx.x % LOW_RANKS;
+  // where this row of the fragment has its power of two
+  int* exponent = nullptr;
+  if constexpr (std::is_same<T, f16_t>::value) {
+    if (a.planes && n_ == 0 && m_ < 16) exponent = a.exponents + ((int64_t)blockIdx.x * 16 + m_) * (a.rp / LOW_RANKS) + blockIdx.y;
+    if (exponent && (!has || m_ >= rows)) *exponent = PLANES_NONE;
+  }
+  if (!has) return;
   const int j0 = blockIdx.y * LOW_RANKS, j = j0 + n_;
   const bool some = id < a.R && j0 < a.r;
   if (some) {
@@ -168,8 +175,19 @@ __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(Adapte
   const int64_t t = a.idx[row0 + m_];
   if (j < a.r) a.U[t * a.r + j] = v;
   if (a.planes && j < a.rp) {
+    float w = v;
+    if constexpr (std::is_same<T, f16_t>::value) {
+      // (the 16 lanes of a row; beside a value that is not finite the finite ones are nothing)
+      float most = v == v ? fabsf(v) : INFINITY;
+#pragma unroll
+      for (int o = LOW_RANKS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+      const int log = most > 0.0f ? ilogbf(most) : PLANES_NONE + PLANES_TOP;
+      const int e = log >= PLANES_LEAST && log <= PLANES_TOP ? 0 : min(max(log - PLANES_TOP, PLANES_NONE), PLANES_MOST);
+      w = ldexpf(v, -e);
+      if (exponent) *exponent = e;
+    }
     T* p = (T*)a.planes + t * 2 * a.rp + j;
-    split<T>(v, p[0], p[a.rp]);
+    split<T>(w, p[0], p[a.rp]);
   }
 }
 
@@ -576,14 +594,15 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   const int rp = (c.r + 31) / 32 * 32;
   char* planes = tiles ? s.bytes(c.T * 2 * rp * w) : nullptr;
   int* slots = tiles ? s.take<int>(adapter_fragments(c.T, c.R) * 17) : nullptr;
+  int* exponents = tiles && c.dtype == SMOE_F16 ? s.take<int>(adapter_fragments(c.T, c.R) * rp) : nullptr;
   if (!s.dry()) {
-    const AdapterLowArgs a{p.X, p.sxm, p.A, p.sar, p.saj, p.sak, c.ids, c.scales, many ? idx : nullptr, many ? off : nullptr, p.U, planes, rp, slots,
+    const AdapterLowArgs a{p.X, p.sxm, p.A, p.sar, p.saj, p.sak, c.ids, c.scales, many ? idx : nullptr, many ? off : nullptr, p.U, planes, rp, slots, exponents,
                            c.T, (int)p.K, c.r, c.R};
     if (int rc = low(a, c.dtype, st)) return rc;
   }
   if (p.Y == nullptr) return 0;
   if (s.dry()) return 0;
-  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
+  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, exponents, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
                              c.T, (int)K, (int)p.N, c.r, c.R};
   return project(a, c.dtype, st);
 }

@@ -5,7 +5,8 @@
 // one adapter, so its U B^T is a product of whole fragments, and what another request's adapter holds, infinities included, never meets
 // its rows.  A tile spans as many adapters as it has fragments: the shared product does not care, and no tile is cut short
 // where an adapter ends.  The accumulators start with U B^T and the main loop adds X W^T to them: one rounding.  U comes in two
-// parts of 16 bits (2^-18 of its value; one part would cost as much as the output's own rounding), operands straight from
+// parts of 16 bits (2^-18 of its value; one part would cost as much as the output's own rounding; float16 parts times a power of
+// two of their row where float16 would not hold them, PLANES_TOP, 81 us of a product instead of 80), operands straight from
 // global memory: for rank 16, 80 loads of 1 KB and 128 products per wave and 256 x 256 tile, against 64 slices of 128
 // products for K = 4096.
 //
@@ -32,6 +33,14 @@ template <> struct AdapterTile<1> { typedef Tile<256, 256, 2, 4> type; };
 template <> struct AdapterTile<3> { typedef Tile<64, 128, 2, 2, 3, false, 2> type; };
 template <> struct AdapterTile<2> { typedef Tile<128, 128, 2, 2, 2, false, 2> type; };
 
+// Eight values of a float16 plane from their block's power of two to the row's, 2^down <= 1 of it (what that leaves below float16 is
+// at most 2^-22 of the row's largest)
+template <typename T>
+__device__ __forceinline__ i32x4 planes_times(i32x4 u, int down) {
+  typedef T v8 __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(i32x4, __builtin_bit_cast(v8, u) * (T)ldexpf(1.0f, down));
+}
+
 template <typename T, int CLASS, bool W_TR>
 __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::type::WAVES_PER_SIMD) void adapter_tiles_kernel(AdapterTiles args) {
   typedef typename AdapterTile<CLASS>::type TL;
@@ -41,7 +50,8 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   static_assert(TL::BM * TL::BN * 2 <= TL::NS * STAGE, "staged tile must fit the operand buffers");
   __shared__ __attribute__((aligned(16))) char lds[TL::NS * STAGE];
   __shared__ int64_t sDst[TL::BM];
-  __shared__ int sSrc[TL::BM], sAdapter[FRAGS];
+  constexpr bool SCALED = std::is_same<T, f16_t>::value;      // planes of powers of two (PLANES_TOP)
+  __shared__ int sSrc[TL::BM], sAdapter[FRAGS], sExponent[SCALED ? TL::BM : 1];
   __shared__ __attribute__((aligned(16))) float sBias[TL::RS ? TL::BN : 4];
   const AdapterProjectArgs& a = args.p;
   int m_tile, n_tile, m_loc, n_loc;
@@ -59,6 +69,12 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
     sSrc[m] = t >= 0 ? t : max(first, 0);
     sDst[m] = t >= 0 ? (int64_t)t * a.sym : -1;
     if ((m & 15) == 0) sAdapter[m >> 4] = f < fragments ? s[16] : -1;
+    if constexpr (SCALED) {                                  // the row's: the largest of its blocks'
+      int e = PLANES_NONE;
+      const int* of = a.exponents + (f * 16 + (m & 15)) * (a.rp / 16);
+      for (int b = 0; b < a.rp / 16 && f < fragments; ++b) e = max(e, of[b]);
+      sExponent[m] = e == PLANES_NONE ? 0 : e;
+    }
   }
   if (!__syncthreads_or(any)) return;
 
@@ -79,12 +95,17 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
       return i > 0 && __builtin_amdgcn_readfirstlane(sAdapter[f]) == __builtin_amdgcn_readfirstlane(sAdapter[max(f - 1, 0)]);
     };
     i32x4 u[2][2], bv[2][2 * TL::FN];
+    int down[2];
     auto load = [&](int i, int p) {
       const int row = wm * TL::WTM + 16 * i;
       const int id = __builtin_amdgcn_readfirstlane(sAdapter[row >> 4]);
-      const T* x = (const T*)a.planes + (int64_t)sSrc[row + lr] * 2 * a.rp + k;
+      int src = sSrc[row + lr];
+      if constexpr (SCALED && TL::RS) asm volatile("" : "+v"(src));      // (addresses of all fragments, kept, would be spilled)
+      const T* x = (const T*)a.planes + (int64_t)src * 2 * a.rp + k;
       u[p][0] = *(const i32x4*)x;
       u[p][1] = *(const i32x4*)(x + a.rp);
+      if constexpr (SCALED)
+        down[p] = a.exponents[(min(f0 + (row >> 4), fragments - 1) * 16 + lr) * (a.rp / 16) + (k >> 4)] - sExponent[row + lr];
       if (same(i)) return;
       const T* b = (const T*)a.B + (int64_t)max(id, 0) * a.sbr + (inside ? k : 0);
 #pragma unroll
@@ -103,6 +124,10 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j)
         if (none) bv[i & 1][j] = i32x4{0, 0, 0, 0};
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) u[i & 1][h] = planes_times<T>(u[i & 1][h], down[i & 1]);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -111,6 +136,23 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
           c = Mfma<T>::run(bv[i & 1][j], u[i & 1][h], c);
         }
       __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if constexpr (SCALED) {                                    // (a lane's accumulators of a fragment are of one row)
+#pragma unroll
+    for (int i = 0; i < 2 * TL::FM; ++i) {
+      const int e = sExponent[wm * TL::WTM + 16 * i + lr];
+      if (!__any(e != 0)) continue;
+      const float back = ldexpf(1.0f, e);
+#pragma unroll
+      for (int j = 0; j < 2 * TL::FN; ++j) {
+        f32x4& c = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
+        if constexpr (TL::RS) asm volatile("" : "+a"(c));
+        c *= back;
+        // (back to the matrix unit's own registers at once: all of them together would not fit the vector unit's)
+        if constexpr (TL::RS) asm volatile("" : "+a"(c));
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 

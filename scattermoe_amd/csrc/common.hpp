@@ -384,15 +384,20 @@ struct AdapterLowArgs {
   float* U;                                          // (T, r)
   void* planes; int rp;                              // (T, 2, rp) of the operands' type, U in two parts; or NULL
   int* slots;                                        // (fragments, 17): rows of every 16, or -1, and their adapter, or -1
+  int* exponents;                                    // float16 planes: (fragments, 16, rp / 16), see PLANES_TOP; or NULL
   int64_t T;
   int K, r, R;
 };
+// float16 planes hold U times 2^-e, e for a row's every 16 ranks: U is a float32 value and may lie beyond what float16 holds, either
+// way.  e = 0 where the largest of them lies in [2^-3, 2^15), which it mostly does, else what puts it in [2^14, 2^15).  PLANES_NONE: no
+// value but zero; PLANES_MOST: float32's largest, or a value that is not finite.
+static constexpr int PLANES_LEAST = -3, PLANES_TOP = 14, PLANES_NONE = -100, PLANES_MOST = 127 - PLANES_TOP;
 struct AdapterProjectArgs {
   const void* X; int64_t sxm;                        // (T, K), columns contiguous
   const void* W; int64_t swn, swk;                   // (N, K)
   const void* bias; int64_t sb;                      // (N) or NULL
   const float* U;                                    // (T, r)
-  const void* planes; int rp; const int* slots;      // as AdapterLowArgs
+  const void* planes; int rp; const int* slots; const int* exponents;      // as AdapterLowArgs
   const void* B; int64_t sbr, sbn, sbj;              // (R, N, r)
   const int64_t* ids;                                // (T)
   void* Y; int64_t sym;                              // (T, N), columns contiguous
