@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void layer_out_any_kernel(RoutedLayerArgs a) {
 // ---- contiguous rows: streams over the weights of the experts that were hit ----------------------------------------
 // The rows (token, slot) by expert, put together by every workgroup for itself (at most 512 ids; a launch for it would cost
 // more than the workgroups wait).  The order of an expert's rows among themselves is whatever the LDS atomics make it: a row's
-// values do not depend on its place.
+// values do not depend on its place, since all passes over an expert's rows have one form.
 struct RowLists {
   int count[512], first[513], rows[SMOE_FEW_ROWS], hit[512], hits;
 };
@@ -201,9 +201,11 @@ __global__ __launch_bounds__(HID_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4) 
   const int e = s.hit[blockIdx.y], f0 = blockIdx.x * (ROWS / 2);
   const int* rows = s.rows + s.first[e];
   if constexpr (MANY) {
-    for (int M = s.count[e];;) {
-      if (GROUPS == 1 || M <= 8) hidden_tile<T, 2, 1, ROWS>(a, e, f0, rows, min(M, 8), part);
-      else if (GROUPS == 2 || M <= 16) hidden_tile<T, 2, GROUPS == 1 ? 1 : 2, ROWS>(a, e, f0, rows, min(M, 16), part);
+    // (the form goes by all of the expert's rows, not by those that are left: forms sum in orders of their own)
+    const int count = s.count[e];
+    for (int M = count;;) {
+      if (GROUPS == 1 || count <= 8) hidden_tile<T, 2, 1, ROWS>(a, e, f0, rows, min(M, 8), part);
+      else if (GROUPS == 2 || count <= 16) hidden_tile<T, 2, GROUPS == 1 ? 1 : 2, ROWS>(a, e, f0, rows, min(M, 16), part);
       else hidden_tile<T, 2, GROUPS, ROWS>(a, e, f0, rows, min(M, 8 * GROUPS), part);
       if ((M -= 8 * GROUPS) <= 0) break;
       rows += 8 * GROUPS;
@@ -243,9 +245,10 @@ __global__ __launch_bounds__(TILE_NW * 64, GROUPS > 2 ? 2 : GROUPS == 2 ? 3 : 4)
   if ((int)blockIdx.y >= s.hits) return;
   const int e = s.hit[blockIdx.y], n0 = blockIdx.x * TILE_COLS;
   const int* rows = s.rows + s.first[e];
-  for (int M = s.count[e];;) {
-    if (GROUPS == 1 || M <= 8) out_tile<T, 2, 1, TILE_COLS>(a, e, n0, rows, min(M, 8), part);
-    else if (GROUPS == 2 || M <= 16) out_tile<T, 2, GROUPS == 1 ? 1 : 2, TILE_COLS>(a, e, n0, rows, min(M, 16), part);
+  const int count = s.count[e];
+  for (int M = count;;) {
+    if (GROUPS == 1 || count <= 8) out_tile<T, 2, 1, TILE_COLS>(a, e, n0, rows, min(M, 8), part);
+    else if (GROUPS == 2 || count <= 16) out_tile<T, 2, GROUPS == 1 ? 1 : 2, TILE_COLS>(a, e, n0, rows, min(M, 16), part);
     else out_tile<T, 2, GROUPS, TILE_COLS>(a, e, n0, rows, min(M, 8 * GROUPS), part);
     if ((M -= 8 * GROUPS) <= 0) break;
     rows += 8 * GROUPS;
