@@ -93,3 +93,13 @@ def test_module_with_loss_scaling():
     want = _bounds.adapters(x.detach(), m.weight, m.lora_a, m.lora_b, ids, m.scales, None, dy)["dx"]
     assert float((dy.double() @ m.lora_b[0].double()).abs().max()) > 65504
     _bounds.check("dx", dx, *want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_more_columns_in_a_tile_row_than_a_round(dtype):
+    """A projection to a vocabulary: the tiles of one row are more than the CUs."""
+    i, dy = _inputs(200, 160, 65800, 3, 8, dtype, seed=5)
+    y, grads = _step(i, dy, ["x"])
+    want = _want(i, dy)
+    _bounds.check("y", y, *want["y"])
+    _bounds.check("dx", grads["x"], *want["dx"])
