@@ -45,7 +45,7 @@ def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias
     x (..., d), weight (n, d), bias (n) or None, lora_a (R, r, d), lora_b (R, n, r): float32, bfloat16 or float16, all the
     same; adapter_idxs: integers of x's leading shape, and a row whose id lies outside [0, R) (-1, say) gets the shared
     projection alone; scales (R) or None (ones), a constant.  Adapters of a smaller rank are padded with zeros.  Everything but
-    the output is summed and kept in float32.  Gradients go to x, weight, bias, lora_a and lora_b."""
+    the output is summed and kept in float32.  Gradients go to x, weight, bias, lora_a and lora_b; forward-mode derivatives are refused."""
     dtype, device, shape = x.dtype, x.device, x.shape
     tensors = (weight, lora_a, lora_b) if bias is None else (weight, lora_a, lora_b, bias)
     if weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3 or not shape:
@@ -83,7 +83,7 @@ def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias
         x, ids = x.reshape(-1, d), ids.reshape(-1)
     if ids.dtype != torch.int64 or not ids.is_contiguous():
         ids = ids.to(torch.int64).contiguous()
-    if trained and torch.is_grad_enabled():
+    if (trained and torch.is_grad_enabled()) or ops.has_tangents(x, scales, *tensors):
         y = _ParallelAdapters.apply(x, weight, bias, lora_a, lora_b, ids, scales)
     else:
         y = ops.adapter_forward(x, weight, lora_a, lora_b, ids, scales, bias)[0]

@@ -11,6 +11,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _C
 
@@ -525,6 +526,12 @@ def _launch(name, *args):
     if torch.compiler.is_compiling():
         return _COMPILED_OPS[name](*args)
     return getattr(_backend, name)(*args)
+
+
+def has_tangents(*tensors):
+    """Whether forward-mode derivatives are asked of any of them (None: no tensor).  The library knows nothing of them: a call that
+    hands tensors to it goes through its autograd function then, which refuses."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _same_dtype(what, ref, *others):

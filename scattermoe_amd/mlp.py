@@ -150,7 +150,8 @@ class GLUMLP(_SparseMLP):
             return super().forward(x, expert_p, expert_idxs)
         lead = x.shape[:-1]
         tokens = x.view(-1, x.size(-1))
-        if expert_idxs.numel() <= ops.DECODE_MAX_ROWS and not torch.is_grad_enabled() and expert_idxs.dim() == 2:
+        if (expert_idxs.numel() <= ops.DECODE_MAX_ROWS and not torch.is_grad_enabled() and expert_idxs.dim() == 2
+                and not ops.has_tangents(tokens, expert_p, *self.parameters())):
             out = ops.decode_glu_mlp(tokens, expert_p, expert_idxs, self.experts.weight, self.experts.bias,
                                      self.output_experts.weight, self.output_experts.bias, ops.ACT_SILU)
             if out is not None:
@@ -172,7 +173,7 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
 
     Where nothing asks for a gradient and for few tokens (`ops.few_tokens_pay`) the layer is one call of the library (`ops.routed_glu_mlp`); otherwise
     router product, `topk_softmax`, `flatten_sort_count` and the gated MLP's launches, differentiable in all float
-    arguments.  Both keep the logits in float32; the general path stores hidden and expert rows in x's type, the
+    arguments (forward-mode derivatives are refused).  Both keep the logits in float32; the general path stores hidden and expert rows in x's type, the
     other rounds the output only."""
     if x.dim() < 1 or router_weight.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
         raise ValueError("routed_glu_mlp: x (..., d), router_weight (E, d), w1 (E, 2F, d) and w2 (E, d, F)")
@@ -199,7 +200,8 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
     if T == 0:
         return x.new_empty(x.shape), x.new_empty((0, E), dtype=torch.float32)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    if ops.few_tokens_pay(T, k, E, d, F, x.dtype) and not (trained and torch.is_grad_enabled()):
+    if (ops.few_tokens_pay(T, k, E, d, F, x.dtype) and not (trained and torch.is_grad_enabled())
+            and not ops.has_tangents(x, router_weight, w1, w2, b1, b2)):
         out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
         return out.view(x.shape), logits
     logits = nn.functional.linear(tokens.float(), router_weight.float())
