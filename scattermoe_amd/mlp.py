@@ -204,7 +204,8 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
             and not ops.has_tangents(x, router_weight, w1, w2, b1, b2)):
         out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
         return out.view(x.shape), logits
-    logits = nn.functional.linear(tokens.float(), router_weight.float())
+    with torch.autocast(x.device.type, enabled=False):               # (it would take this product, and no other here, to 16 bits)
+        logits = nn.functional.linear(tokens.float(), router_weight.float())
     gates, experts = ops.topk_softmax(logits, k, renormalize)
     eid, idx, off = flatten_sort_count(experts, num_experts=E)
     out = _GatedMLP.apply(tokens, w1.permute(0, 2, 1), b1, w2.permute(0, 2, 1), b2, gates.to(x.dtype), eid, idx, off, k, act)
