@@ -354,8 +354,9 @@ int smoe_topk_softmax(const void* logits, int64_t slt, int64_t sle, int64_t T, i
  *   gates g = softmax(LOGITS[t,:])[S] (divided by their sum when `renormalize`);
  *   OUT[t] = sum_j g[t,j] ( W2[e] glu(W1[e] X[t] + b1[e]) + b2[e] ),  e = S[t,j],  `act` as for smoe_glu_fwd.
  * Counterpart in the reference: the router, softmax and top-k of scattermoe/utils/replace_moe.py:60-95 and
- * GLUMLP.forward (scattermoe/mlp.py:74-95).  Sums, gates and hidden values stay in float32: OUT is the only rounding
- * (the general path stores pre-activations, hidden and expert rows in `dtype`).
+ * GLUMLP.forward (scattermoe/mlp.py:74-95).  Sums and gates stay in float32 and OUT is rounded once (the
+ * general path stores pre-activations, hidden and expert rows in `dtype`).  Hidden values are the sum of two `dtype` values: off by
+ * 2^-18 of them (bfloat16), 2^-24 or 2^-25 in all (float16; infinite where float16 is), by nothing (float32).
  * Logits that are NaN or infinite: as for smoe_topk_softmax.
  * X (T,d) strides sxm,sxk; WR (E,d) strides sre,srk; W1 (E,2F,d) strides sw1e,sw1n,sw1k; b1 (E,2F) or NULL; W2 (E,d,F)
  * strides sw2e,sw2n,sw2k; b2 (E,d) or NULL; OUT (T,d) row stride som, columns contiguous; LOGITS (T,E) contiguous.

@@ -4,8 +4,9 @@
 //   h[t, j] = a * silu(b),  (a, b) the halves of W1[e] X[t] + b1[e],  e = S[t, j]
 //   OUT[t]  = sum_j g[t, j] (W2[e] h[t, j] + b2[e])
 // in three launches up to 4 tokens (logits; hidden rows, selection inside; output) and five beyond (logits, selection, hidden rows,
-// output rows, their sum).  Every sum stays in float32, the hidden rows in two parts of the operand's type (few_rows.hpp, split): the
-// only rounding of the layer is the output's.  A hidden value beyond float16's range is infinite, as in the general path.
+// output rows, their sum).  Every sum and gate stays in float32; hidden values are the sum of two of the operand's type (few_rows.hpp,
+// split): bfloat16 2^-18 of the value off, float16 2^-24 or 2^-25 in all, infinite where float16 is, as in the general path.  So
+// whatever the weights' layout: what a token gets does not depend on it.
 //
 // What bounds it: the weights of the experts that were hit, read once; a kernel that only reads reaches 6.3 to 6.75 TB/s here.
 // us, all launches (weights at TB/s): 1 token, 8 of 128 experts, 2048 / 768 24.2 (3.1; launches that depend on each other);
@@ -62,6 +63,9 @@ __global__ __launch_bounds__(64) void layer_select_kernel(RoutedLayerArgs a) {
 
 static_assert(DOT_NW == DOT_ROWS, "any layout: a wave per expert");
 
+// Hidden values are held as two parts of the operand's type (float32: one)
+template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2;
+
 // ---- any layout: one wave per hidden value, one wave per output value ----------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void layer_hidden_any_kernel(RoutedLayerArgs a) {
@@ -77,7 +81,15 @@ __global__ __launch_bounds__(256) void layer_hidden_any_kernel(RoutedLayerArgs a
     first += to_f32(b[f * a.sb1n]);
     second += to_f32(b[(f + a.F) * a.sb1n]);
   }
-  if (lane_id() == 0) a.hidden[(int64_t)row * a.F + f] = (a.act & 1) ? glu_h(a.act, first, second) : glu_h(a.act, second, first);
+  if (lane_id() == 0) {
+    float v = (a.act & 1) ? glu_h(a.act, first, second) : glu_h(a.act, second, first);
+    if constexpr (HIDDEN_PARTS<T> == 2) {
+      T part, rest;
+      split<T>(v, part, rest);
+      v = to_f32(part) + to_f32(rest);
+    }
+    a.hidden[(int64_t)row * a.F + f] = v;
+  }
 }
 
 template <typename T>
@@ -137,10 +149,7 @@ __device__ __forceinline__ void list_rows(const int* __restrict__ experts, int L
   __syncthreads();
 }
 
-// Hidden values are held as two parts of the operand's type (float32: one), rows of `ldh` elements
-template <typename T> static constexpr int HIDDEN_PARTS = sizeof(T) == 4 ? 1 : 2;
-
-// Hidden rows: a workgroup of four waves has ROWS weight rows (each hidden value's two next to each other) of one expert's
+// Hidden rows, `ldh` elements of every part: a workgroup of four waves has ROWS weight rows (each hidden value's two next to each other) of one expert's
 // rows; the waves take the contraction's blocks in turn and are added up in LDS.  Two weight rows of each hidden value meet in one
 // workgroup, so its halves need no trip through memory.  us (weights at TB/s): 1 token, 2048 -> 2 x 768, 8 experts 14.0 (3.6); 1 token,
 // 4096 -> 2 x 14336, 2 experts 75.9 (6.2); 17 tokens, 2880 -> 2 x 2880, 29 experts 139 (6.9); 64 tokens, 126 experts 132 (6.0).

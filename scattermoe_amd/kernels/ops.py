@@ -1046,7 +1046,8 @@ def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=Tru
     """(out (T, d), router logits (T, E) float32) of a gated MoE layer from its tokens: router product, softmax, top-k, both
     expert products and the gate-weighted sum, forward only (scattermoe/utils/replace_moe.py:60-95 and GLUMLP.forward,
     mlp.py:74-95).  router_w (E, d), w1 (E, 2F, d), w2 (E, d, F) in any strides; biases (E, 2F) / (E, d) or None.  For
-    the sizes that `few_tokens` names; everything but the output stays in float32."""
+    the sizes that `few_tokens` names; sums, logits and gates stay in float32, hidden values in two parts of x's type (2^-18 of them,
+    float16 2^-24 or 2^-25 in all, and infinite where float16 is), and the output is rounded once."""
     T, d = x.shape
     E, F = router_w.size(0), w2.size(2)
     if not few_tokens(T, k, E):

@@ -173,8 +173,8 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
 
     Where nothing asks for a gradient and for few tokens (`ops.few_tokens_pay`) the layer is one call of the library (`ops.routed_glu_mlp`); otherwise
     router product, `topk_softmax`, `flatten_sort_count` and the gated MLP's launches, differentiable in all float
-    arguments (forward-mode derivatives are refused).  Both keep the logits in float32; the general path stores hidden and expert rows in x's type, the
-    other rounds the output only."""
+    arguments (forward-mode derivatives are refused).  Both keep the logits in float32; the general path stores gates, hidden and expert rows in x's type, the
+    other hidden values in two parts of it (float16: infinite above 65504 in both) and rounds the output."""
     if x.dim() < 1 or router_weight.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
         raise ValueError("routed_glu_mlp: x (..., d), router_weight (E, d), w1 (E, 2F, d) and w2 (E, d, F)")
     E, d = router_weight.shape

@@ -3,6 +3,9 @@ expert's rows take several passes, of which the last is not full."""
 import pytest
 import torch
 
+import _bounds
+from scattermoe_amd.kernels import ops
+from scattermoe_amd.mlp import routed_glu_mlp
 from test_gpu_routed_layer import DEV, DTYPES, _call, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -24,3 +27,41 @@ def test_order_of_the_tokens(T, E, k, dtype):
         assert torch.equal(got[0], want[0][order]), "%d values differ" % int((got[0] != want[0][order]).sum())
     again = _call(i, k)
     assert torch.equal(again[0], want[0])
+
+
+def _layouts(i):
+    """The same weights in both layouts, and without the weights' streams."""
+    turned = {n: i[n].transpose(1, 2).contiguous().transpose(1, 2) for n in ("w1", "w2")}
+    return [i, dict(i, w2=turned["w2"]), dict(i, w1=turned["w1"]), dict(i, **turned)]
+
+
+@pytest.mark.parametrize("T", [3, 9])
+def test_hidden_values_beyond_float16(T):
+    """float16 hidden values above 65504 are infinite, whatever the weights' layout and as where they are stored: the rows that have one
+    are not finite, and the others are what they are without them."""
+    i = _inputs(T, 64, 96, 4, torch.float16, seed=T)
+    large = dict(i, x=i["x"].clone(), w1=(i["w1"].float() * 16).half())
+    large["x"][1] = (i["x"][1].float() * 24).half()
+    _, _, _, _, clear = _bounds.layer(large["x"], large["wr"], large["w1"], large["w2"], 2)
+    assert bool(clear.all())
+    others = [t for t in range(T) if t != 1]
+    for s in _layouts(large):
+        got = ops.routed_glu_mlp(s["x"], s["wr"], s["w1"], None, s["w2"], None, 2)
+        assert not bool(torch.isfinite(got[0][1]).any())
+        out, bound, _, _, _ = _bounds.layer(s["x"], s["wr"], s["w1"], s["w2"], 2)
+        _bounds.check("others", got[0][others], out[others], bound[others])
+    general = routed_glu_mlp(large["x"].clone().requires_grad_(), large["wr"], large["w1"], large["w2"], 2)[0]
+    assert not bool(torch.isfinite(general[1]).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [3, 9, 40])
+def test_small_hidden_values(T, dtype):
+    """Hidden values of about 2^-20, a part of the smallest step of float16 away from their sum: every layout within the same bound."""
+    i = _inputs(T, 64, 96, 4, dtype, seed=T + 1)
+    s = dict(i, w1=(i["w1"].float() * 2.0 ** -9).to(dtype), w2=(i["w2"].float() * 2.0 ** 10).to(dtype))
+    out, bound, _, _, clear = _bounds.layer(s["x"], s["wr"], s["w1"], s["w2"], 2)
+    assert bool(clear.all())
+    for of in _layouts(s):
+        got = ops.routed_glu_mlp(of["x"], of["wr"], of["w1"], None, of["w2"], None, 2)
+        _bounds.check("out", got[0], out, bound)
