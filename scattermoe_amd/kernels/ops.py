@@ -1035,11 +1035,19 @@ def few_tokens(T, k, E):
     return 0 < T <= FEW_TOKENS and T * k <= FEW_ROWS and E <= 512 and k <= 64
 
 
-def few_tokens_pay(T, k, E, d, F, dtype):
+STRIDED_WORK = 1 << 23
+
+
+def few_tokens_pay(T, k, E, d, F, dtype, streams=True):
     """Whether it is also the faster way.  Beyond eight rows per expert a 16-bit stream over many weights is faster in the general
     path's tiles, which share the rows among more columns (8 experts, 4096 -> 14336, us: 32 tokens 456 against 450, 64 tokens 520
-    against 460; 32 experts of 2880, 64 tokens 273 against 276; 16 experts, 1024 -> 512, 64 tokens 25 against 39)."""
-    return few_tokens(T, k, E) and (dtype == torch.float32 or T * k <= 8 * E or E * d * F < 1 << 27)
+    against 460; 32 experts of 2880, 64 tokens 273 against 276; 16 experts, 1024 -> 512, 64 tokens 25 against 39); a float32 one
+    is not (64 tokens: 8 experts, 4096 -> 14336 1550 against 2460, 32 of 2880 551 against 1900).  `streams`: whether the weights'
+    contraction is contiguous.  The kernels for others have a wave per value and read a line of memory per element (bf16, 32
+    experts of 2880, 1 / 64 tokens 384 / 46600 against 121 / 283; 16 experts, 256 -> 512, 16 / 64 tokens, 4.2 / 17 million
+    products per half 50 / 161 against 119 / 125, of which the host takes 80); the general path's tiles take either axis."""
+    return (few_tokens(T, k, E) and (dtype == torch.float32 or T * k <= 8 * E or E * d * F < 1 << 27)
+            and (streams or T * k * d * F <= STRIDED_WORK))
 
 
 def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=True):
@@ -1053,6 +1061,8 @@ def routed_glu_mlp(x, router_w, w1, b1, w2, b2, k, act=ACT_SILU, renormalize=Tru
     if not few_tokens(T, k, E):
         raise ValueError("routed_glu_mlp: 1..%d tokens, at most %d (token, slot) rows, 512 experts and top-64" % (FEW_TOKENS, FEW_ROWS))
     _same_dtype("routed_glu_mlp", x, router_w, w1, w2, b1, b2)
+    if x.stride(1) != 1:
+        x = x.contiguous()                               # (the weights' streams want it, and it is a few rows)
     out = torch.empty((T, d), dtype=x.dtype, device=x.device)
     logits = torch.empty((T, E), dtype=torch.float32, device=x.device)
     _launch("routed_glu_mlp", x, router_w, w1, b1, w2, b2, out, logits, k, bool(renormalize), act)

@@ -65,3 +65,20 @@ def test_small_hidden_values(T, dtype):
     for of in _layouts(s):
         got = ops.routed_glu_mlp(of["x"], of["wr"], of["w1"], None, of["w2"], None, 2)
         _bounds.check("out", got[0], out, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [2, 30])
+def test_larger_weights_of_a_strided_contraction(T, dtype):
+    """The general path, within the bound of its own roundings, and columns of the tokens that lie apart."""
+    i = _inputs(T, 512, 520, 8, dtype, bias=True, seed=T + 2)
+    args = (i["x"], i["wr"], i["w1"], i["w2"], 4, i["b1"], i["b2"])
+    out, bound, logits, logits_bound, clear = _bounds.layer(*args, stored=True)
+    assert int(clear.sum()) >= 0.9 * T
+    for s in _layouts(i)[1:]:
+        got = _call(s, 4)
+        _bounds.check("logits", got[1], logits, logits_bound)
+        _bounds.check("out", got[0].cpu()[clear], out[clear], bound[clear])
+    want = _call(i, 4)
+    got = _call(dict(i, x=i["x"].t().contiguous().t()), 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
