@@ -92,7 +92,8 @@ def parallel_adapters(x, weight, lora_a, lora_b, adapter_idxs, scales=None, bias
 
 class ParallelAdapters(nn.Module):
     """A linear map (weight (out, in), optional bias) shared by all rows, with R low-rank adapters beside it:
-    lora_a (R, rank, in), drawn like a weight, lora_b (R, out, rank), zeros, and their factors `scales` (R)."""
+    lora_a (R, rank, in), drawn like a weight, lora_b (R, out, rank), zeros, and their factors `scales` (R), which are float32
+    whatever type the module is taken to."""
 
     def __init__(self, num_adapters, input_size, output_size, rank, bias=False, scale=1.0) -> None:
         super().__init__()
@@ -104,8 +105,15 @@ class ParallelAdapters(nn.Module):
         self.bias = nn.Parameter(torch.empty(output_size)) if bias else None
         self.lora_a = nn.Parameter(torch.empty(num_adapters, rank, input_size))
         self.lora_b = nn.Parameter(torch.empty(num_adapters, output_size, rank))
-        self.register_buffer("scales", torch.full((num_adapters,), float(scale)))
+        self.register_buffer("scales", torch.full((num_adapters,), float(scale), dtype=torch.float32))
         self.reset_parameters()
+
+    def _apply(self, fn, recurse=True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:                       # (eight bits of them would be left in bfloat16)
+            self.scales = scales.to(device=self.scales.device, dtype=torch.float32)
+        return self
 
     def reset_parameters(self) -> None:
         nn.init.normal_(self.weight, std=0.02)
