@@ -191,10 +191,10 @@ __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(Adapte
   }
 }
 
-// ---- Y, few rows or float32: tiles of COLS columns and 16 G / P rows, both operands from the caches or from memory ------------
+// ---- Y, few rows or little work: tiles of COLS columns and 16 G / P rows, both operands from the caches or from memory ------------
 // Few rows are a stream over the weights: 1 row, 4096 -> 4096 8.0 us (4.2 TB/s; the launch's ends are a third of it), 48 rows,
-// 2880 -> 4096 13.3 us (the weights come once from memory and once more from the caches).  float32 is bound by its matrix
-// instruction and by the operands' way from the caches: 203 rows, 1003 -> 1517 21.2 us (0.62 GFLOP).
+// 2880 -> 4096 13.3 us (the weights come once from memory and once more from the caches).  float32 is bound by the operands' way from
+// the caches (66 TFLOP/s): 203 rows, 1003 -> 1517 21.2 us (0.62 GFLOP); beyond a measured line its products go in adapters_f32.hip's tiles.
 template <typename T, int P, int G, int NW, int COLS>
 __global__ __launch_bounds__(NW * 64, G > 4 ? 2 : 4) void adapter_project_rows_kernel(AdapterProjectArgs a) {
   constexpr int INPUTS = 16 * G / P;
@@ -564,6 +564,7 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   const bool many = c.T > ADAPTER_FEW_ROWS;
   const bool long_copy = p.swk != 1 && p.N * p.K >= COPY_MIN && cdiv64(c.T, 64) * cdiv64(p.N, 128) >= COPY_MIN_TILES;
   const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && (long_copy || c.T * p.N * p.K > TILES_MIN_WORK)));
+  const bool tiles_f32 = c.dtype == SMOE_F32 && adapter_takes_tiles_f32(c.T, p.K, p.N, p.swk != 1);
   const int64_t w = width(c.dtype);
   // The copies, at most the factors' and those of the shared product, in pairs
   AdapterPackArgs copies[4] = {};
@@ -586,7 +587,7 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
     const bool w_tr = p.swn == 1 && p.swk != 1;
     if (p.K % 8 || (w_tr && p.N % 8)) copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, K);
     if (p.K % 8) copy(X, zero, sxm, one, 1, c.T, p.K, K);
-  } else if (p.Y != nullptr && p.swk != 1 && p.K >= pieces(c.dtype)) {
+  } else if (p.Y != nullptr && !tiles_f32 && p.swk != 1 && p.K >= pieces(c.dtype)) {
     copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, p.K);
   }
   for (int i = 0; i < n && !s.dry(); i += 2)
@@ -602,9 +603,9 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   }
   if (p.Y == nullptr) return 0;
   if (s.dry()) return 0;
-  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, exponents, p.B, p.sbr, p.sbn, p.sbj, c.ids, p.Y, p.N,
+  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, exponents, p.B, p.sbr, p.sbn, p.sbj, c.ids, many ? idx : nullptr, p.Y, p.N,
                              c.T, (int)K, (int)p.N, c.r, c.R};
-  return project(a, c.dtype, st);
+  return tiles_f32 ? launch_adapter_tiles_f32(a, st) : project(a, c.dtype, st);
 }
 
 static int forward(const AdapterCall& c, Space& s, hipStream_t st) {

@@ -399,7 +399,7 @@ struct AdapterProjectArgs {
   const float* U;                                    // (T, r)
   const void* planes; int rp; const int* slots; const int* exponents;      // as AdapterLowArgs
   const void* B; int64_t sbr, sbn, sbj;              // (R, N, r)
-  const int64_t* ids;                                // (T)
+  const int64_t* ids; const int64_t* idx;            // (T); rows by adapter, or NULL
   void* Y; int64_t sym;                              // (T, N), columns contiguous
   int64_t T;
   int K, N, r, R;
@@ -423,6 +423,8 @@ struct AdapterPackArgs {
 // Fragments of 16 rows, each of one adapter, that T rows of R adapters (and of none) can make
 static inline int64_t adapter_fragments(int64_t T, int64_t R) { return max_tiles(T, (int)R + 1, 16); }
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc);       // csrc/adapters_mfma.hip
+bool adapter_takes_tiles_f32(int64_t T, int64_t K, int64_t N, bool strided);                   // csrc/adapters_f32.hip
+int launch_adapter_tiles_f32(const AdapterProjectArgs& a, hipStream_t st);
 // A call, forward or backward: contiguous tensors, but for the row stride of X
 static constexpr int ADAPTER_FEW_ROWS = 64;          // up to so many rows the products go row by row, without an order
 struct AdapterCall {

@@ -90,3 +90,20 @@ def test_one_row_of_tiles_beyond_a_round(launches):
     assert which[0] == 0 and which[1] >= 594
     (which,) = _tiles(launches(100, 1024, 65800, 16, 8))
     assert which[0] == 1 and which[1] >= 258
+
+
+def _f32(found):
+    """The side of the float32 tiles of a call, 0 for the rows' kernel, and whether a weight or factor is copied."""
+    side = [int(re.search(r"SIDE = (\d+)", who).group(1)) for who, kernel, _, _ in found if "adapter_tiles_f32_kernel" in kernel]
+    return (side or [0])[0], any("pack" in kernel for _, kernel, _, _ in found)
+
+
+@pytest.mark.parametrize("T,K,N,want,want_back", [
+    (64, 4096, 4096, 0, 0), (65, 4096, 4096, 0, 0), (128, 1024, 1024, 0, 0), (128, 4096, 4096, 0, 64), (256, 4096, 4096, 64, 64),
+    (512, 2048, 2048, 64, 64), (1024, 512, 512, 0, 0), (203, 1003, 1517, 0, 0), (1024, 1003, 1517, 64, 64), (1024, 2048, 2048, 64, 64),
+    (1024, 4096, 4096, 128, 128), (1300, 4096, 4096, 64, 64), (4096, 4096, 4096, 128, 128), (2048, 1536, 2000, 128, 64)])
+def test_float32_tiles(launches, T, K, N, want, want_back):
+    """The rows' kernel read all weights per 32 rows (1024 rows, 4096 -> 4096 513 us where an elementary product takes 281)."""
+    assert _f32(launches(T, K, N, 16, 8, 0)) == (want, False)
+    side, copied = _f32(launches(T, K, N, 16, 8, 0, True))
+    assert side == want_back and copied
