@@ -528,10 +528,15 @@ def _launch(name, *args):
     return getattr(_backend, name)(*args)
 
 
+def in_dual_level():
+    """Whether tensors may carry tangents here (forward-mode derivatives)."""
+    return forward_ad._current_level >= 0
+
+
 def has_tangents(*tensors):
     """Whether forward-mode derivatives are asked of any of them (None: no tensor).  The library knows nothing of them: a call that
     hands tensors to it goes through its autograd function then, which refuses."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return in_dual_level() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _same_dtype(what, ref, *others):

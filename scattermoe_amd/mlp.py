@@ -151,7 +151,7 @@ class GLUMLP(_SparseMLP):
         lead = x.shape[:-1]
         tokens = x.view(-1, x.size(-1))
         if (expert_idxs.numel() <= ops.DECODE_MAX_ROWS and not torch.is_grad_enabled() and expert_idxs.dim() == 2
-                and not ops.has_tangents(tokens, expert_p, *self.parameters())):
+                and not ops.in_dual_level()):
             out = ops.decode_glu_mlp(tokens, expert_p, expert_idxs, self.experts.weight, self.experts.bias,
                                      self.output_experts.weight, self.output_experts.bias, ops.ACT_SILU)
             if out is not None:
