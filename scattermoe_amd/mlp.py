@@ -197,11 +197,12 @@ def routed_glu_mlp(x, router_weight, w1, w2, k, b1=None, b2=None, renormalize=Tr
         trained = trained or t.requires_grad
     tokens = x.reshape(-1, d)
     T = tokens.size(0)
-    if T == 0:
+    trained = trained and torch.is_grad_enabled()
+    if T == 0 and not trained:
         return x.new_empty(x.shape), x.new_empty((0, E), dtype=torch.float32)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
     streams = w1.stride(2) == 1 and w2.stride(2) == 1
-    if (ops.few_tokens_pay(T, k, E, d, F, x.dtype, streams) and not (trained and torch.is_grad_enabled())
+    if (ops.few_tokens_pay(T, k, E, d, F, x.dtype, streams) and not trained
             and not ops.has_tangents(x, router_weight, w1, w2, b1, b2)):
         out, logits = ops.routed_glu_mlp(tokens, router_weight, w1, b1, w2, b2, k, act, renormalize)
         return out.view(x.shape), logits

@@ -5,7 +5,7 @@ import torch
 
 import _bounds
 from scattermoe_amd.kernels import ops
-from scattermoe_amd.mlp import routed_glu_mlp
+from scattermoe_amd.mlp import RoutedGLUMLP, routed_glu_mlp
 from test_gpu_routed_layer import DEV, DTYPES, _call, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +82,19 @@ def test_larger_weights_of_a_strided_contraction(T, dtype):
     want = _call(i, 4)
     got = _call(dict(i, x=i["x"].t().contiguous().t()), 4)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_training_step_without_tokens(dtype):
+    """... as on a rank that got none: the outputs are part of the graph, and every gradient is zeros."""
+    m = RoutedGLUMLP(64, 96, 8, 2, bias=True).to(DEV).to(dtype)
+    x = torch.randn(0, 3, 64, device=DEV).to(dtype).requires_grad_()
+    out, logits = m(x)
+    assert out.shape == x.shape and logits.shape == (0, 8) and out.requires_grad and logits.requires_grad
+    (out.float().sum() + logits.sum()).backward()
+    assert x.grad.shape == x.shape
+    for name, p in m.named_parameters():
+        assert p.grad is not None and p.grad.shape == p.shape and not bool(p.grad.any()), name
+    with torch.no_grad():
+        out, logits = m(x)
+    assert out.shape == x.shape and logits.shape == (0, 8) and logits.dtype == torch.float32

@@ -19,6 +19,17 @@ class _Library(_Backend):
                 return call(*args)
         return plain if callable(call) else call
 
+    # (the double's views have no shape without rows)
+    @staticmethod
+    def combine(Y, gates, out, k):
+        if out.numel():
+            _Backend.combine(Y, gates, out, k)
+
+    @staticmethod
+    def gate_grad(Y, d_out, d_gates, k):
+        if d_out.numel():
+            _Backend.gate_grad(Y, d_out, d_gates, k)
+
 
 @pytest.fixture
 def backend(monkeypatch):
@@ -78,3 +89,12 @@ def test_columns_of_the_tokens_are_contiguous_in_the_library(backend, monkeypatc
         rows = m(torch.cat([x, x], 1)[:, :16])
     assert [t.stride() for t in calls] == [(16, 1), (16, 1), (32, 1)]
     assert all(torch.equal(a, b) for other in (got, rows) for a, b in zip(other, want))
+
+
+def test_a_training_step_without_tokens(backend):
+    m, x = _layer(), torch.randn(0, 16, requires_grad=True)
+    out, logits = m(x)
+    assert out.requires_grad and logits.requires_grad and out.shape == (0, 16) and logits.shape == (0, 6)
+    (out.sum() + logits.sum()).backward()
+    assert x.grad.shape == (0, 16)
+    assert all(p.grad is not None and not bool(p.grad.any()) for p in m.parameters())
