@@ -82,8 +82,9 @@ def layer(x, wr, w1, w2, k, b1=None, b2=None, renormalize=True, gate_first=False
     return out, rounded(out, err, dtype), logits, logits_err, clear
 
 
-def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None):
-    """{name: (value, bound)} of y and, with dy, of dx, da, db, dw, dbias."""
+def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None, held_in_gradients=True):
+    """{name: (value, bound)} of y and, with dy, of dx, da, db, dw, dbias.  `held_in_gradients`: whether the low-rank values may have been
+    held in two parts for the factors' gradients, as they may for y and dx."""
     dtype = x.dtype
     x, w, la, lb = (t.detach().double() for t in (x, w, la, lb))
     ids = ids.long()
@@ -122,7 +123,8 @@ def adapters(x, w, la, lb, ids, scales=None, bias=None, dy=None):
         for a in range(R):
             rows = (ids == a).nonzero().squeeze(1)
             out[a] = p[rows].t() @ m[rows]
-            err[a] = held(p[rows], p_err[rows], dtype).t() @ m[rows].abs() + (2 * len(rows) + 8) * U * (p[rows].abs().t() @ m[rows].abs())
+            p_held = held(p[rows], p_err[rows], dtype) if held_in_gradients else p_err[rows]
+            err[a] = p_held.t() @ m[rows].abs() + (2 * len(rows) + 8) * U * (p[rows].abs().t() @ m[rows].abs())
         return out, rounded(out, err, dtype)
 
     found["da"] = grad(v, v_err, x)
