@@ -191,6 +191,26 @@ __global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_rows_kernel(Adapte
   }
 }
 
+// ... float32, where such workgroups would be few: 16 / P rows and ranks each, so that a CU fetches less.  us, 16 x 16 / 8 x 8 / 4 x 4, rows of
+// 4096: 320 rows, rank 8 13.0 / 6.5 / 4.6, eight adapters of rank 16 13.8 / 7.2 / 8.5; 1024 rows, rank 8 13.2 / 6.7 / 7.6, eight adapters of rank 16 14.6
+// / 14.0 / 15.6; 2048 rows 16.1 / 17.6 / 26.0; 1024 rows, 64 adapters of rank 32 16.4 / 24.6 / 41.8, one of rank 64 28.0 / 22.5 / 40.6.
+static constexpr int64_t LOW_PARTS4 = 4096, LOW_PARTS2 = 16384;          // rows times rank
+template <int P>
+__global__ __launch_bounds__(LOW_NW * 64, 4) void adapter_low_parts_kernel(AdapterLowArgs a) {
+  constexpr int SIDE = 16 / P;
+  __shared__ float part[FEW_PART<LOW_NW, SIDE, SIDE>];
+  int id, row0, rows;
+  if (!find_tile<SIDE>(a.off, a.R + 1, blockIdx.x, id, row0, rows)) return;
+  const int m = threadIdx.x / SIDE, n = threadIdx.x % SIDE, j0 = blockIdx.y * SIDE, j = j0 + n;
+  if (id < a.R) {
+    few_tile<float, P, 1, 1, LOW_NW, SIDE, false>([&](int n) { return (const float*)a.A + id * a.sar + min(j0 + n, a.r - 1) * a.saj; },
+                                                  [&](int m) { return (const float*)a.X + a.idx[row0 + min(m, rows - 1)] * a.sxm; }, 0, a.K, part);
+    __syncthreads();
+  }
+  if (m >= rows || j >= a.r) return;
+  a.U[a.idx[row0 + m] * a.r + j] = id < a.R ? few_sum<LOW_NW, SIDE, SIDE>(part, n, m) * (a.scales ? a.scales[id] : 1.0f) : 0.0f;
+}
+
 // ---- Y, few rows or little work: tiles of COLS columns and 16 G / P rows, both operands from the caches or from memory ------------
 // Few rows are a stream over the weights: 1 row, 4096 -> 4096 8.0 us (4.2 TB/s; the launch's ends are a third of it), 48 rows,
 // 2880 -> 4096 13.3 us (the weights come once from memory and once more from the caches).  float32 is bound by the operands' way from
@@ -412,6 +432,13 @@ template <typename T>
 static int low_t(const AdapterLowArgs& a, hipStream_t st) {
   const bool pieces = a.sak == 1 && a.K >= Few<T>::PER;
   if (pieces && a.idx != nullptr) {
+    if constexpr (sizeof(T) == 4) {
+      const int P = a.T * a.r <= LOW_PARTS4 ? 4 : a.T * a.r <= LOW_PARTS2 ? 2 : 1;
+      const dim3 grid((unsigned)max_tiles(a.T, a.R + 1, 16 / P), (unsigned)cdiv64(a.r, 16 / P)), block(LOW_NW * 64);
+      if (P == 4) hipLaunchKernelGGL(adapter_low_parts_kernel<4>, grid, block, 0, st, a);
+      else if (P == 2) hipLaunchKernelGGL(adapter_low_parts_kernel<2>, grid, block, 0, st, a);
+      if (P > 1) return launch_status("adapter_low_parts_kernel");
+    }
     hipLaunchKernelGGL(adapter_low_rows_kernel<T>, dim3((unsigned)adapter_fragments(a.T, a.R), ((a.planes ? a.rp : a.r) + LOW_RANKS - 1) / LOW_RANKS), dim3(LOW_NW * 64), 0, st, a);
     return launch_status("adapter_low_rows_kernel");
   }
@@ -564,7 +591,7 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   const bool many = c.T > ADAPTER_FEW_ROWS;
   const bool long_copy = p.swk != 1 && p.N * p.K >= COPY_MIN && cdiv64(c.T, 64) * cdiv64(p.N, 128) >= COPY_MIN_TILES;
   const bool tiles = c.dtype != SMOE_F32 && p.K >= 8 && (c.T > TILES_MIN_ROWS || (many && (long_copy || c.T * p.N * p.K > TILES_MIN_WORK)));
-  const bool tiles_f32 = c.dtype == SMOE_F32 && adapter_takes_tiles_f32(c.T, p.K, p.N, p.swk != 1);
+  const AdapterF32 f32 = c.dtype == SMOE_F32 ? adapter_f32_class(c.T, p.K, p.N, p.swk != 1) : ADAPTER_F32_ROWS;
   const int64_t w = width(c.dtype);
   // The copies, at most the factors' and those of the shared product, in pairs
   AdapterPackArgs copies[4] = {};
@@ -587,7 +614,7 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
     const bool w_tr = p.swn == 1 && p.swk != 1;
     if (p.K % 8 || (w_tr && p.N % 8)) copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, K);
     if (p.K % 8) copy(X, zero, sxm, one, 1, c.T, p.K, K);
-  } else if (p.Y != nullptr && !tiles_f32 && p.swk != 1 && p.K >= pieces(c.dtype)) {
+  } else if (p.Y != nullptr && f32 == ADAPTER_F32_ROWS && p.swk != 1 && p.K >= pieces(c.dtype)) {
     copy(p.W, zero, p.swn, p.swk, 1, p.N, p.K, p.K);
   }
   for (int i = 0; i < n && !s.dry(); i += 2)
@@ -595,6 +622,7 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   const int rp = (c.r + 31) / 32 * 32;
   char* planes = tiles ? s.bytes(c.T * 2 * rp * w) : nullptr;
   int* slots = tiles ? s.take<int>(adapter_fragments(c.T, c.R) * 17) : nullptr;
+  float* parts = f32 == ADAPTER_F32_RUNS ? s.take<float>(adapter_f32_parts()) : nullptr;
   int* exponents = tiles && c.dtype == SMOE_F16 ? s.take<int>(adapter_fragments(c.T, c.R) * rp) : nullptr;
   if (!s.dry()) {
     const AdapterLowArgs a{p.X, p.sxm, p.A, p.sar, p.saj, p.sak, c.ids, c.scales, many ? idx : nullptr, many ? off : nullptr, p.U, planes, rp, slots, exponents,
@@ -603,9 +631,9 @@ static int product(const AdapterCall& c, Product p, const int64_t* idx, const in
   }
   if (p.Y == nullptr) return 0;
   if (s.dry()) return 0;
-  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, exponents, p.B, p.sbr, p.sbn, p.sbj, c.ids, many ? idx : nullptr, p.Y, p.N,
-                             c.T, (int)K, (int)p.N, c.r, c.R};
-  return tiles_f32 ? launch_adapter_tiles_f32(a, st) : project(a, c.dtype, st);
+  const AdapterProjectArgs a{X, sxm, p.W, p.swn, p.swk, p.bias, 1, p.U, planes, rp, slots, exponents, p.B, p.sbr, p.sbn, p.sbj, c.ids,
+                             many ? idx : nullptr, p.Y, p.N, c.T, (int)K, (int)p.N, c.r, c.R};
+  return f32 != ADAPTER_F32_ROWS ? launch_adapter_f32(a, f32, parts, st) : project(a, c.dtype, st);
 }
 
 static int forward(const AdapterCall& c, Space& s, hipStream_t st) {

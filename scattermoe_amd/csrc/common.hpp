@@ -423,8 +423,11 @@ struct AdapterPackArgs {
 // Fragments of 16 rows, each of one adapter, that T rows of R adapters (and of none) can make
 static inline int64_t adapter_fragments(int64_t T, int64_t R) { return max_tiles(T, (int)R + 1, 16); }
 bool try_adapter_tiles(const AdapterProjectArgs& a, int dtype, hipStream_t st, int& rc);       // csrc/adapters_mfma.hip
-bool adapter_takes_tiles_f32(int64_t T, int64_t K, int64_t N, bool strided);                   // csrc/adapters_f32.hip
-int launch_adapter_tiles_f32(const AdapterProjectArgs& a, hipStream_t st);
+// How a float32 product of many rows goes (csrc/adapters_f32.hip): row by row, in whole tiles, in tiles whose slices are dealt out
+enum AdapterF32 { ADAPTER_F32_ROWS, ADAPTER_F32_128, ADAPTER_F32_64, ADAPTER_F32_RUNS };
+AdapterF32 adapter_f32_class(int64_t T, int64_t K, int64_t N, bool strided);
+int64_t adapter_f32_parts();                         // floats that the last one leaves
+int launch_adapter_f32(const AdapterProjectArgs& a, AdapterF32 how, float* parts, hipStream_t st);
 // A call, forward or backward: contiguous tensors, but for the row stride of X
 static constexpr int ADAPTER_FEW_ROWS = 64;          // up to so many rows the products go row by row, without an order
 struct AdapterCall {

@@ -8,7 +8,7 @@ import subprocess
 
 import pytest
 
-from scattermoe_amd import _build
+from scattermoe_amd import _C, _build
 
 pytestmark = pytest.mark.skipif(shutil.which("hipcc") is None and not os.path.exists("/opt/rocm/bin/hipcc"), reason="needs hipcc")
 
@@ -93,17 +93,31 @@ def test_one_row_of_tiles_beyond_a_round(launches):
 
 
 def _f32(found):
-    """The side of the float32 tiles of a call, 0 for the rows' kernel, and whether a weight or factor is copied."""
-    side = [int(re.search(r"SIDE = (\d+)", who).group(1)) for who, kernel, _, _ in found if "adapter_tiles_f32_kernel" in kernel]
-    return (side or [0])[0], any("pack" in kernel for _, kernel, _, _ in found)
+    """How a float32 product goes, and whether a weight or factor is copied."""
+    names = [who + kernel for who, kernel, _, _ in found]
+    if any("adapter_runs_f32_kernel" in n for n in names):
+        assert "adapter_runs_join_f32_kernel" in names[-1]
+        how = "runs"
+    else:
+        how = ([int(re.search(r"SIDE = (\d+)", n).group(1)) for n in names if "adapter_tiles_f32_kernel" in n] or ["rows"])[0]
+    return how, any("pack" in n for n in names)
 
 
 @pytest.mark.parametrize("T,K,N,want,want_back", [
-    (64, 4096, 4096, 0, 0), (65, 4096, 4096, 0, 0), (128, 1024, 1024, 0, 0), (128, 4096, 4096, 0, 64), (256, 4096, 4096, 64, 64),
-    (512, 2048, 2048, 64, 64), (1024, 512, 512, 0, 0), (203, 1003, 1517, 0, 0), (1024, 1003, 1517, 64, 64), (1024, 2048, 2048, 64, 64),
-    (1024, 4096, 4096, 128, 128), (1300, 4096, 4096, 64, 64), (4096, 4096, 4096, 128, 128), (2048, 1536, 2000, 128, 64)])
-def test_float32_tiles(launches, T, K, N, want, want_back):
-    """The rows' kernel read all weights per 32 rows (1024 rows, 4096 -> 4096 513 us where an elementary product takes 281)."""
+    (64, 4096, 4096, "rows", "rows"), (65, 4096, 4096, "runs", "runs"), (128, 1024, 1024, "rows", "rows"), (128, 2048, 2048, "rows", "runs"),
+    (256, 4096, 4096, 64, 64), (320, 4096, 4096, "runs", "runs"), (512, 2048, 2048, 64, 64), (1024, 512, 512, "rows", "rows"),
+    (203, 1003, 1517, "rows", "rows"), (1024, 1472, 2064, "runs", "runs"), (1024, 4096, 4096, 128, 128), (4096, 4096, 4096, 128, 128),
+    (2048, 1536, 2000, 128, 64), (300, 4, 4, "rows", 64)])
+def test_float32_products(launches, T, K, N, want, want_back):
+    """The rows' kernel reads all weights per 32 rows (1024 rows, 4096 -> 4096 509 us where an elementary product takes 281), and a few tiles more than
+    whole rounds of them took a round more."""
     assert _f32(launches(T, K, N, 16, 8, 0)) == (want, False)
-    side, copied = _f32(launches(T, K, N, 16, 8, 0, True))
-    assert side == want_back and copied
+    how, copied = _f32(launches(T, K, N, 16, 8, 0, True))
+    assert how == want_back and copied
+
+
+def test_float32_runs_have_their_parts_in_the_workspace(launches):
+    """512 runs of slices of 64 x 64 tiles leave at most two parts each."""
+    lib = _C.load()
+    size = lambda T, back: lib.smoe_adapter_workspace_bytes(T, 4096, 4096, 16, 8, back, 0)
+    assert min(size(320, 0) - size(1024, 0), size(320, 1) - size(1024, 1)) > 0 and min(size(320, 0), size(320, 1)) >= 2 * 512 * 64 * 64 * 4

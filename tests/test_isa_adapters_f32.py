@@ -17,8 +17,8 @@ def test_memory_instructions_stand_between_products(tmp_path):
     subprocess.run([_build._hipcc()] + _build.HIPCC_FLAGS + ["--cuda-device-only", "-S", "-o", str(out), os.path.join(_build.CSRC, "adapters_f32.hip")],
                    check=True, stderr=subprocess.DEVNULL)
     text = out.read_text()
-    kernels = re.findall(r"^(_ZN4smoe24adapter_tiles_f32_kernel\w+):(.*?)^\.Lfunc_end", text, re.S | re.M)
-    assert len(kernels) == 4
+    kernels = re.findall(r"^(_ZN4smoe\d+adapter_(?:tiles|runs)_f32_kernel\w+):(.*?)^\.Lfunc_end", text, re.S | re.M)
+    assert len(kernels) == 6
     for name, body in kernels:
         assert "scratch_" not in body, name
         loops = [b for b in re.split(r"^\.LBB\w+:", body, flags=re.M) if b.count("v_mfma") >= 16 and "s_barrier" in b]
