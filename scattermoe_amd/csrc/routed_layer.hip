@@ -8,7 +8,8 @@
 // split): bfloat16 2^-18 of the value off, float16 2^-24 or 2^-25 in all, infinite where float16 is, as in the general path.  So
 // whatever the weights' layout: what a token gets does not depend on it.
 //
-// What bounds it: the weights of the experts that were hit, read once; a kernel that only reads reaches 6.3 to 6.75 TB/s here.
+// What bounds it: the weights of the experts that were hit, read from memory once (counted: 471 + 236 MB for 1 token, 2 of 8 experts,
+// 4096 / 14336, 942 + 477 for 17 tokens, 4 of 32, 2880 / 2880); a kernel that only reads reaches 6.3 to 6.75 TB/s here.
 // us, all launches (weights at TB/s): 1 token, 8 of 128 experts, 2048 / 768 24.2 (3.1; launches that depend on each other);
 // 1 token, 2 of 8, 4096 / 14336 118 (6.0); 17 tokens, 4 of 32, 2880 / 2880 222 (6.4); 64 tokens, 8 of 128, 2048 / 768 220 (5.4).
 //
@@ -152,7 +153,7 @@ __device__ __forceinline__ void list_rows(const int* __restrict__ experts, int L
 // Hidden rows, `ldh` elements of every part: a workgroup of four waves has ROWS weight rows (each hidden value's two next to each other) of one expert's
 // rows; the waves take the contraction's blocks in turn and are added up in LDS.  Two weight rows of each hidden value meet in one
 // workgroup, so its halves need no trip through memory.  us (weights at TB/s): 1 token, 2048 -> 2 x 768, 8 experts 14.0 (3.6); 1 token,
-// 4096 -> 2 x 14336, 2 experts 75.9 (6.2); 17 tokens, 2880 -> 2 x 2880, 29 experts 139 (6.9); 64 tokens, 126 experts 132 (6.0).
+// 4096 -> 2 x 14336, 2 experts 75.9 (6.2); 17 tokens, 2880 -> 2 x 2880, 29 experts 139 (6.8); 64 tokens, 126 experts 132 (6.1).
 static constexpr int HID_NW = 4, FEWEST = 4;
 static_assert(FEWEST <= HID_NW, "a wave per token");
 template <typename T, int P, int G, int ROWS>
@@ -389,9 +390,11 @@ static int launch_out(const RoutedLayerArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((layer_out_kernel<T, COLS>), dim3((a.d + COLS - 1) / COLS), dim3(OUT_NW * 64), 0, st, a);
   return launch_status("layer_out_kernel");
 }
-// Up to 4 tokens.  Half as much per workgroup where there would be few of them, us, whole against half: 1 token, 8 of 128 experts,
-// 2048 / 768 (384 workgroups): hidden 15.6 against 14.1, output 9.1 against 7.0; 1 token, 4 of 32 experts, 2880 / 2880 (720
-// workgroups): hidden 24.8 against 28.0, output (180 of 16 columns) 14.2 against 15.8.
+// Up to 4 tokens.  Half as much per workgroup where there would be few of them.  us, whole / half, 1 token: hidden, by workgroups of whole
+// ones: 128 10.6 / 8.3 (float32, 1024 / 1024), 256 11.0 / 10.6 (2048 / 1024), 384 14.9 / 14.0 (2048 / 768), 448 19.2 / 20.8 (3584 / 1792), 512 16.4 /
+// 17.2 (2560 / 2048) and 16.7 / 15.0 (2048 / 2048), 528 19.2 / 20.0 (2048 / 1408), 720 23.8 / 27.1 (2880 / 2880), 1792 75.5 / 71.7 (4096 /
+// 14336); output, by workgroups of 16 columns: 64 6.2 / 4.7, 128 8.6 / 7.0, 10.2 / 8.1 and 11.0 / 8.4, 160 10.7 / 11.8, 10.2 / 11.6 and, float32, 7.8 /
+// 7.5, 180 15.1 / 16.2, 224 10.9 / 11.0, 256 36.8 / 37.6 and 8.2 / 7.4.
 static constexpr int FEWEST_WGS = 512;
 template <typename T>
 static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
@@ -400,11 +403,14 @@ static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
   return a.d / 16 < 160 ? launch_out<T, 8>(a, st) : launch_out<T, 16>(a, st);
 }
 // More than 4 tokens, eight rows of an expert per pass: 16 weight rows per workgroup instead of 32, so that a wave has more of each on
-// its way, where weight rows are long and, 16 bits, few rows of an expert meet them.  us of a layer, 32 / 16 for both products: bf16, 2 of
-// 16 experts, 1024 / 4096, 5 tokens 53 / 50, 16 tokens 74 / 70; 4 of 32, 2880 / 2880, 5 tokens 129 / 126; for the hidden rows 4 of 32,
-// 2048 / 1024, 16 tokens 68 / 65; float32, 4 of 32, 2880 / 2880, 12 tokens 420 / 399; 2 of 16, 4096 / 1024, 16 tokens 149 / 142.
-// Where it does not hold: bf16, 8 of 128, 2048 / 768, 64 tokens 227 / 245; 4 of 64, 512 / 3584, 20 tokens 100 / 123; float32, 8 of
-// 128, 2048 / 768 (the output) 404 / 423.
+// its way, where weight rows are long and, 16 bits, few rows of an expert meet them; for each product by its own rows.  us, 32 / 16,
+// bytes of a weight row in brackets.  bf16, hidden: 2 of 16 experts, 1024 / 4096, 5 tokens (2048) 27.0 / 30.2; 4 of 64, 512 / 3584, 20 tokens (1024)
+// 61.7 / 80.8; 4 of 64, 1792 / 1792, 20 tokens (3584) 90.3 / 89.0; 4 of 32, 2048 / 1024, 16 tokens (4096) 42.8 / 38.0; 2880 / 2880, 16 tokens (5760)
+// 131.2 / 130.1; 4 of 64, 3584 / 512, 20 tokens (7168) 56.2 / 53.6; output: 2048 / 1024 (2048) 21.1 / 21.3; 512 / 3584 (7168) 32.9 / 31.4; 1024 / 4096 (8192)
+// 23.5 / 17.2; many rows of an expert: 8 of 128, 2048 / 768, 64 tokens, hidden (4096) 133.9 / 136.1.  Beyond the line and slower: 2 of 8, 4096 /
+// 14336, 5 tokens 205 / 213 (8192) and 108 / 119 (28672).  float32, hidden: 4 of 64, 512 / 3584 (2048) 107.9 / 122.9; 3 of 13, 1003 / 1411, 5 tokens
+// (4012) 29.9 / 28.1; 8 of 128, 2048 / 768, 64 tokens (8192) 252.0 / 246.9; 2 of 16, 4096 / 1024, 16 tokens (16384) 92.2 / 76.8; output: 2048 / 768
+// (3072) 132.2 / 147.9; 1003 / 1411 (5644) 21.1 / 17.0; 2880 / 2880, 12 tokens (11520) 138.3 / 130.1; slower: 4096 / 1024 (4096) 42.0 / 50.5.
 static constexpr int LONG_ROW = 3500;                        // bytes
 template <typename T>
 static bool few_per_workgroup(const RoutedLayerArgs& a, int length) {
