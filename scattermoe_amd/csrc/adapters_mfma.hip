@@ -60,7 +60,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // rows of the tile's fragments; one behind the last row repeats the fragment's first, or any
   const int64_t fragments = args.fragments, f0 = args.first + (int64_t)m_tile * FRAGS;
-  bool any = false;
+  bool any = false, scaled = false;                          // some row of the tile, some plane not as it is
   for (int m = threadIdx.x; m < TL::BM; m += TL::NT) {
     const int64_t f = f0 + (m >> 4);
     const int* s = a.slots + f * 17;
@@ -72,11 +72,16 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
     if constexpr (SCALED) {                                  // the row's: the largest of its blocks'
       int e = PLANES_NONE;
       const int* of = a.exponents + (f * 16 + (m & 15)) * (a.rp / 16);
-      for (int b = 0; b < a.rp / 16 && f < fragments; ++b) e = max(e, of[b]);
+      for (int b = 0; b < a.rp / 16 && f < fragments; ++b) {
+        const int block = of[b];
+        e = max(e, block);
+        scaled |= block != 0 && block != PLANES_NONE;
+      }
       sExponent[m] = e == PLANES_NONE ? 0 : e;
     }
   }
   if (!__syncthreads_or(any)) return;
+  if constexpr (SCALED) scaled = __syncthreads_or(scaled);
 
   const int wm = wave / TL::WN, wn = wave % TL::WN, lr = lane & 15, lq = lane >> 4;
   Block acc[TL::FM][TL::FN];
@@ -104,7 +109,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
       const T* x = (const T*)a.planes + (int64_t)src * 2 * a.rp + k;
       u[p][0] = *(const i32x4*)x;
       u[p][1] = *(const i32x4*)(x + a.rp);
-      if constexpr (SCALED)
+      if (SCALED && scaled)
         down[p] = a.exponents[(min(f0 + (row >> 4), fragments - 1) * 16 + lr) * (a.rp / 16) + (k >> 4)] - sExponent[row + lr];
       if (same(i)) return;
       const T* b = (const T*)a.B + (int64_t)max(id, 0) * a.sbr + (inside ? k : 0);
@@ -124,7 +129,7 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j)
         if (none) bv[i & 1][j] = i32x4{0, 0, 0, 0};
-      if constexpr (SCALED) {
+      if (SCALED && scaled) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) u[i & 1][h] = planes_times<T>(u[i & 1][h], down[i & 1]);
       }
@@ -138,12 +143,10 @@ __global__ __launch_bounds__(AdapterTile<CLASS>::type::NT, AdapterTile<CLASS>::t
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if constexpr (SCALED) {                                    // (a lane's accumulators of a fragment are of one row)
+  if (SCALED && scaled) {                                    // (a lane's accumulators of a fragment are of one row)
 #pragma unroll
     for (int i = 0; i < 2 * TL::FM; ++i) {
-      const int e = sExponent[wm * TL::WTM + 16 * i + lr];
-      if (!__any(e != 0)) continue;
-      const float back = ldexpf(1.0f, e);
+      const float back = ldexpf(1.0f, sExponent[wm * TL::WTM + 16 * i + lr]);
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
         f32x4& c = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
