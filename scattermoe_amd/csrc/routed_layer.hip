@@ -410,7 +410,7 @@ static int launch_fewest(const RoutedLayerArgs& a, hipStream_t st) {
 // 23.5 / 17.2; many rows of an expert: 8 of 128, 2048 / 768, 64 tokens, hidden (4096) 133.9 / 136.1.  Beyond the line and slower: 2 of 8, 4096 /
 // 14336, 5 tokens 205 / 213 (8192) and 108 / 119 (28672).  float32, hidden: 4 of 64, 512 / 3584 (2048) 107.9 / 122.9; 3 of 13, 1003 / 1411, 5 tokens
 // (4012) 29.9 / 28.1; 8 of 128, 2048 / 768, 64 tokens (8192) 252.0 / 246.9; 2 of 16, 4096 / 1024, 16 tokens (16384) 92.2 / 76.8; output: 2048 / 768
-// (3072) 132.2 / 147.9; 1003 / 1411 (5644) 21.1 / 17.0; 2880 / 2880, 12 tokens (11520) 138.3 / 130.1; slower: 4096 / 1024 (4096) 42.0 / 50.5.
+// 132.2 / 147.9 (shorter than the line); 1003 / 1411 (5644) 21.1 / 17.0; 2880 / 2880, 12 tokens (11520) 138.3 / 130.1; slower: 4096 / 1024 (4096) 42.0 / 50.5.
 static constexpr int LONG_ROW = 3500;                        // bytes
 template <typename T>
 static bool few_per_workgroup(const RoutedLayerArgs& a, int length) {
