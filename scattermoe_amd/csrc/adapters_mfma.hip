@@ -34,11 +34,12 @@ template <> struct AdapterTile<3> { typedef Tile<64, 128, 2, 2, 3, false, 2> typ
 template <> struct AdapterTile<2> { typedef Tile<128, 128, 2, 2, 2, false, 2> type; };
 
 // Eight values of a float16 plane from their block's power of two to the row's, 2^down <= 1 of it (what that leaves below float16 is
-// at most 2^-22 of the row's largest)
+// at most 2^-22 of the row's largest).  In two halves: the values begin at 2^15, so that 2^down itself may lie below float16's smallest.
 template <typename T>
 __device__ __forceinline__ i32x4 planes_times(i32x4 u, int down) {
   typedef T v8 __attribute__((ext_vector_type(8)));
-  return __builtin_bit_cast(i32x4, __builtin_bit_cast(v8, u) * (T)ldexpf(1.0f, down));
+  const int all = max(down, -48), half = all / 2;
+  return __builtin_bit_cast(i32x4, __builtin_bit_cast(v8, u) * (T)ldexpf(1.0f, half) * (T)ldexpf(1.0f, all - half));
 }
 
 template <typename T, int CLASS, bool W_TR>

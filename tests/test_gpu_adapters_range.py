@@ -61,6 +61,20 @@ def test_one_large_rank_among_small_ones(T):
         _bounds.check("y", y, *_want(s)["y"])
 
 
+@pytest.mark.parametrize("T", [400, 3000])
+@pytest.mark.parametrize("log", range(-34, 1, 2))
+def test_small_ranks_beside_ordinary_ones(log, T):
+    """A block of 16 ranks far below the row's largest: what is left of it counts as long as float16 can hold it beside the others."""
+    i, dy = _inputs(T, 128 if T == 400 else 1856, 192, 4, 40, torch.float16, seed=T - log)
+    for block in (slice(0, 16), slice(16, 32), slice(32, 40)):
+        s = dict(i, lora_a=i["lora_a"].clone(), lora_b=i["lora_b"].clone())
+        up = min(8, -log)                                # (a small value in front of a large factor)
+        s["lora_a"][:, block] = (s["lora_a"][:, block].float() * 2.0 ** log).half()
+        s["lora_b"][:, :, block] = (s["lora_b"][:, :, block].float() * 2.0 ** up).half()
+        y, _ = _step(s, dy, ["x"])
+        _bounds.check("y", y, *_want(s)["y"])
+
+
 @pytest.mark.parametrize("T", [65, 400, 3000])
 def test_an_infinite_low_value(T):
     """... makes the outputs infinite that it adds to, and those of its row alone."""
