@@ -400,6 +400,84 @@ int smoe_adapter_backward(const void* DY, const void* X, int64_t sxm, const void
                           void* DBIAS, int64_t T, int64_t K, int64_t N, int64_t r, int64_t R, int dtype, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/*
+ * Experts whose weights are held in 8 bits, and 8-bit copies of what a training step keeps (no counterpart in the reference, whose
+ * kernels take float32, bfloat16 and float16).  8 bits are e4m3 (four significant bits, largest 448, no infinities) times
+ * a scale for each block of 128.
+ *
+ * Rows of K values in 8 bits: smoe_row_8bit_bytes(K) = K rounded up to 16 bytes, filled with zeros, 16-byte aligned; a scale for every 128
+ * columns, a power of two >= 2^-126 held as its exponent + 127 in 8 bits: the smallest by which the block's largest magnitude divided
+ * is at most 448.  Rounded to nearest, ties to even.  NaN and infinities become NaN; a block that holds an infinity keeps nothing of
+ * its other values.  The scales' rows are smoe_row_8bit_scales(K) bytes apart: ceil(K / 128), rounded up to 4.
+ */
+int64_t smoe_row_8bit_bytes(int64_t K);
+int64_t smoe_row_8bit_scales(int64_t K);
+
+/* X (rows, K) row stride sxm, columns contiguous -> Q, S as above. */
+int smoe_quantize_rows(const void* X, int64_t sxm, int64_t rows, int64_t K, void* Q, void* S, int dtype, void* stream);
+
+/*
+ * W (E, N, K), strides swe, swn, columns contiguous -> Q (E, N, K rounded up to 16) and, unless NULL, QT (E, K, N rounded up to 16), both
+ * contiguous and filled with zeros, S (E, ceil(N / 128), ceil(K / 128)): a scale as above for every 128 x 128 values.
+ */
+int smoe_quantize_weights(const void* W, int64_t swe, int64_t swn, int E, int64_t N, int64_t K, void* Q, void* QT, void* S, int dtype,
+                          void* stream);
+
+/* Y (E, N, K) contiguous = Q times its scales, one for every block_rows (1 or 128) x 128 values, 8 bits (as above) or float32. */
+int smoe_dequantize_8bit(const void* Q, int64_t sqe, int64_t sqn, const void* S, int64_t sse, int64_t ssn, int64_t ssk, int scales_float32,
+                         int block_rows, int E, int64_t N, int64_t K, void* Y, int dtype, void* stream);
+
+/*
+ * Gated unit that keeps its input in 8 bits.  pre (rows, 2F) row stride spm -> h (rows, F) contiguous, rounded from pre itself, and
+ * P8 (rows, 2, F rounded up to 16), PS (rows, 2, ceil(F / 128)): the first and the second half of pre, each with blocks of its own.
+ * Backward: dpre (rows, 2F) contiguous from P8, PS and dh (rows, F) row stride sdh; h, unless NULL, is the unit's value of what P8 stands for.
+ */
+int smoe_glu_8bit_fwd(const void* pre, int64_t spm, void* h, void* P8, void* PS, int64_t rows, int64_t F, int act, int dtype, void* stream);
+int smoe_glu_8bit_bwd(const void* P8, const void* PS, const void* dh, int64_t sdh, void* dpre, void* h, int64_t rows, int64_t F, int act,
+                      int dtype, void* stream);
+
+/*
+ * A weight in 8 bits: q (E, N, K), contraction contiguous and filled with zeros to a multiple of 16, rows at multiples of 16
+ * bytes; s: a scale for every 128 x 128 values, 8 bits (a power of two) or float32 (any).  Strides in elements.  A transposed
+ * weight has the scales, and the scales' strides, of the weight that it is the transpose of.
+ */
+typedef struct {
+  const void* q;
+  int64_t q_expert, q_row;
+  const void* s;
+  int64_t s_expert, s_row, s_col;
+  int s_float32;
+} smoe_weight_8bit;
+
+/*
+ * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, summed in float32 and rounded once to `dtype`; rows as for
+ * smoe_scatter2scatter.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
+ * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, fan_out, x_grouped,
+ * coeff != NULL) bytes, 256-byte aligned; nothing in it is read before it is written; calls that overlap in time need one each.
+ */
+size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int fan_out, int x_grouped, int scaled);
+int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_weight_8bit* W, int transposed, const void* b, int64_t sbe,
+                     int64_t sbn, void* Y, int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E,
+                     int fan_out, int x_grouped, int y_grouped, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A gated layer on such weights (GLUMLP.forward, scattermoe/mlp.py:74-95):
+ *   pre = Q(X) W1[e]^T + b1[e];  y = Q(glu(pre)) W2[e]^T + b2[e];  OUT[t] = sum_j gates[t,j] y
+ * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) by slot (y, rounded), OUT (T,d)
+ * contiguous; P8, PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL.
+ * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with
+ * the scales of the weights; DROWS (T k, d): what every slot adds to DX (T,d).  Workspaces as above.
+ */
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E);
+int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const smoe_weight_8bit* W1, const void* b1, int64_t sb1e, int64_t sb1n,
+                      const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT, void* P8, void* PS,
+                      const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E);
+int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, const smoe_weight_8bit* W1T, const smoe_weight_8bit* W2T,
+                          const void* P8, const void* PS, void* DROWS, void* DX, const int64_t* idx, const int64_t* off, int64_t T, int k,
+                          int64_t d, int64_t F, int E, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 
 #ifdef __cplusplus
 }

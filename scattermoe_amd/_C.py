@@ -22,6 +22,16 @@ _INDEX_CODES = {torch.int64: I64, torch.int32: I32, torch.int16: I16, torch.uint
 
 _p, _i64, _int, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
+
+
+class Weight8bit(ctypes.Structure):
+    """smoe_weight_8bit"""
+    _fields_ = [("q", _p), ("q_expert", _i64), ("q_row", _i64), ("s", _p), ("s_expert", _i64), ("s_row", _i64), ("s_col", _i64),
+                ("s_float32", _int)]
+
+
+_w8 = ctypes.POINTER(Weight8bit)
+
 _SIGNATURES = {
     "smoe_version": (_int, []),
     "smoe_last_error": (ctypes.c_char_p, []),
@@ -69,6 +79,21 @@ _SIGNATURES = {
     "smoe_adapter_forward": (_int, [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _p, _sz, _p]),
     "smoe_adapter_backward": (_int, [_p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                      _int, _p, _sz, _p]),
+    "smoe_row_8bit_bytes": (_i64, [_i64]),
+    "smoe_row_8bit_scales": (_i64, [_i64]),
+    "smoe_quantize_rows": (_int, [_p, _i64, _i64, _i64, _p, _p, _int, _p]),
+    "smoe_quantize_weights": (_int, [_p, _i64, _i64, _int, _i64, _i64, _p, _p, _p, _int, _p]),
+    "smoe_dequantize_8bit": (_int, [_p, _i64, _i64, _p, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _p, _int, _p]),
+    "smoe_glu_8bit_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _int, _int, _p]),
+    "smoe_glu_8bit_bwd": (_int, [_p, _p, _p, _i64, _p, _p, _i64, _i64, _int, _int, _p]),
+    "smoe_linear_8bit_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int]),
+    "smoe_linear_8bit": (_int, [_p, _i64, _p, _w8, _int, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _int, _int, _int, _int, _int,
+                                _p, _sz, _p]),
+    "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int]),
+    "smoe_glu_mlp_8bit": (_int, [_p, _i64, _p, _w8, _p, _i64, _i64, _w8, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64,
+                                 _int, _int, _int, _p, _sz, _p]),
+    "smoe_glu_mlp_8bit_bwd_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int]),
+    "smoe_glu_mlp_8bit_bwd": (_int, [_p, _i64, _p, _w8, _w8, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64, _int, _int, _int, _p, _sz, _p]),
 }
 
 ERR_UNSUPPORTED = -6

@@ -8,6 +8,8 @@ from . import kernels
 from . import mlp
 from . import adapters
 from .adapters import parallel_adapters, ParallelAdapters
+from . import eight_bit
+from .eight_bit import parallel_linear_8bit, GLUMLP8bit
 
 if os.environ.get("SCATTERMOE_NO_HF_PATCH", "0") != "1":
     from . import utils
@@ -25,5 +27,8 @@ __all__ = [
     "adapters",
     "parallel_adapters",
     "ParallelAdapters",
+    "eight_bit",
+    "parallel_linear_8bit",
+    "GLUMLP8bit",
     "utils",
 ]

@@ -1,0 +1,257 @@
+// extern "C" entry points of the products on 8-bit operands and of the passes around them: argument checks, the workspace's layout,
+// the launches of a call.  Nothing here allocates; every launch goes to the caller's stream.
+#include "eight_bit.hpp"
+
+namespace smoe {
+
+static bool float_type(int d) { return d == SMOE_F32 || d == SMOE_BF16 || d == SMOE_F16; }
+static bool act_ok(int a) { return a == SMOE_ACT_SILU || a == SMOE_ACT_SILU_GATE_FIRST; }
+static constexpr int64_t MOST = 0x3fffffff;                        // columns
+
+// pieces of a workspace, each at a multiple of 256 bytes
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <typename T = uint8_t>
+  T* take(int64_t bytes) {
+    T* p = base ? (T*)(base + used) : nullptr;
+    used += ((size_t)bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+// Rows of 8-bit activations of a product of L rows: the tokens once, or a copy for each row where they are scaled one by one or where
+// the token matrix passes the 32-bit offsets that a gathered operand has
+static bool gathers(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
+  return !x_grouped && !scaled && L / fan * padded_row(K) < (1LL << 32);
+}
+struct Rows8Bit { uint8_t* q; uint8_t* s; int64_t rows; };
+static Rows8Bit take_rows(Carver& c, int64_t rows, int64_t K) {
+  Rows8Bit r{nullptr, nullptr, rows};
+  r.q = c.take(rows * padded_row(K));
+  r.s = c.take(rows * scale_row(K));
+  return r;
+}
+static int quantize(const Rows8Bit& r, const void* X, int64_t sxm, const int64_t* idx, int fan, const void* coeff, int64_t K, int dtype,
+                    hipStream_t st) {
+  QuantRowsArgs a{X, sxm, idx, fan, coeff, r.rows, K, r.q, r.s};
+  return launch_quantize_rows(a, dtype, st);
+}
+
+static int weight_checks(const char* who, const smoe_weight_8bit* w, int64_t N, int64_t K) {
+  if (!w || !w->q || !w->s) { set_error("%s: NULL weight", who); return SMOE_ERR_NULL; }
+  if (((uintptr_t)w->q | w->q_expert | w->q_row) & 15) { set_error("%s: weights' rows start at multiples of 16 bytes", who); return SMOE_ERR_SHAPE; }
+  if (w->q_row < padded_row(K) && N > 1) { set_error("%s: weights' rows of %lld bytes are needed", who, (long long)padded_row(K)); return SMOE_ERR_SHAPE; }
+  if (N * w->q_row >= (1LL << 40)) { set_error("%s: weights too large", who); return SMOE_ERR_RANGE; }
+  return 0;
+}
+static Product8Args product(const Rows8Bit& x, const smoe_weight_8bit* w, bool transposed, const void* b, int64_t sbe, int64_t sbn, void* Y,
+                            int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E, int fan,
+                            int x_grouped, int y_grouped) {
+  Product8Args a{};
+  a.X = x.q, a.XS = x.s, a.x_rows = x.rows;
+  a.W = (const uint8_t*)w->q, a.swe = w->q_expert, a.swn = w->q_row;
+  a.WS = w->s, a.sse = w->s_expert, a.ssn = transposed ? w->s_col : w->s_row, a.ssk = transposed ? w->s_row : w->s_col;
+  a.ws_f32 = w->s_float32;
+  a.b = b, a.sbe = sbe, a.sbn = sbn;
+  a.Y = Y, a.sym = sym;
+  a.idx = idx, a.off = off;
+  a.L = (int)L, a.K = (int)padded_row(K), a.N = (int)N, a.E = E, a.fan = fan, a.x_grouped = x_grouped, a.y_grouped = y_grouped;
+  return a;
+}
+
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" {
+
+int64_t smoe_row_8bit_bytes(int64_t K) { return padded_row(K); }
+int64_t smoe_row_8bit_scales(int64_t K) { return scale_row(K); }
+
+int smoe_quantize_rows(const void* X, int64_t sxm, int64_t rows, int64_t K, void* Q, void* S, int dtype, void* stream) {
+  set_error("%s", "");
+  if (!float_type(dtype)) { set_error("smoe_quantize_rows: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (rows < 0 || K < 0) { set_error("smoe_quantize_rows: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (K > MOST) { set_error("smoe_quantize_rows: size beyond int32"); return SMOE_ERR_RANGE; }
+  if (rows == 0 || K == 0) return 0;
+  if (!X || !Q || !S) { set_error("smoe_quantize_rows: NULL pointer"); return SMOE_ERR_NULL; }
+  if ((uintptr_t)Q & 15) { set_error("smoe_quantize_rows: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
+  QuantRowsArgs a{X, sxm, nullptr, 1, nullptr, rows, K, (uint8_t*)Q, (uint8_t*)S};
+  return launch_quantize_rows(a, dtype, (hipStream_t)stream);
+}
+
+int smoe_quantize_weights(const void* W, int64_t swe, int64_t swn, int E, int64_t N, int64_t K, void* Q, void* QT, void* S, int dtype,
+                          void* stream) {
+  set_error("%s", "");
+  if (!float_type(dtype)) { set_error("smoe_quantize_weights: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (E < 0 || N < 0 || K < 0) { set_error("smoe_quantize_weights: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (K > MOST || N > MOST) { set_error("smoe_quantize_weights: size beyond int32"); return SMOE_ERR_RANGE; }
+  if (E == 0 || N == 0 || K == 0) return 0;
+  if (!W || !Q || !S) { set_error("smoe_quantize_weights: NULL pointer"); return SMOE_ERR_NULL; }
+  if (((uintptr_t)Q | (uintptr_t)QT) & 15) { set_error("smoe_quantize_weights: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
+  QuantWeightsArgs a{W, swe, swn, E, N, K, (uint8_t*)Q, (uint8_t*)QT, (uint8_t*)S};
+  return launch_quantize_weights(a, dtype, (hipStream_t)stream);
+}
+
+int smoe_dequantize_8bit(const void* Q, int64_t sqe, int64_t sqn, const void* S, int64_t sse, int64_t ssn, int64_t ssk, int scales_float32,
+                         int block_rows, int E, int64_t N, int64_t K, void* Y, int dtype, void* stream) {
+  set_error("%s", "");
+  if (!float_type(dtype)) { set_error("smoe_dequantize_8bit: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (E < 0 || N < 0 || K < 0 || (block_rows != 1 && block_rows != QB)) { set_error("smoe_dequantize_8bit: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (K > MOST) { set_error("smoe_dequantize_8bit: size beyond int32"); return SMOE_ERR_RANGE; }
+  if (E == 0 || N == 0 || K == 0) return 0;
+  if (!Q || !S || !Y) { set_error("smoe_dequantize_8bit: NULL pointer"); return SMOE_ERR_NULL; }
+  DequantArgs a{(const uint8_t*)Q, sqe, sqn, S, sse, ssn, ssk, scales_float32, block_rows, E, N, K, Y};
+  return launch_dequantize(a, dtype, (hipStream_t)stream);
+}
+
+static int unit_checks(const char* who, int64_t rows, int64_t F, int act, int dtype) {
+  if (!float_type(dtype)) { set_error("%s: unknown dtype %d", who, dtype); return SMOE_ERR_DTYPE; }
+  if (rows < 0 || F < 0) { set_error("%s: bad sizes", who); return SMOE_ERR_SHAPE; }
+  if (!act_ok(act)) { set_error("%s: unknown activation %d", who, act); return SMOE_ERR_SHAPE; }
+  if (F > MOST) { set_error("%s: size beyond int32", who); return SMOE_ERR_RANGE; }
+  return 0;
+}
+
+int smoe_glu_8bit_fwd(const void* pre, int64_t spm, void* h, void* P8, void* PS, int64_t rows, int64_t F, int act, int dtype, void* stream) {
+  set_error("%s", "");
+  if (int rc = unit_checks("smoe_glu_8bit_fwd", rows, F, act, dtype)) return rc;
+  if (rows == 0 || F == 0) return 0;
+  if (!pre || !h || !P8 || !PS) { set_error("smoe_glu_8bit_fwd: NULL pointer"); return SMOE_ERR_NULL; }
+  if ((uintptr_t)P8 & 15) { set_error("smoe_glu_8bit_fwd: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
+  UnitArgs a{pre, spm, h, nullptr, nullptr, (uint8_t*)P8, (uint8_t*)PS, rows, F, act};
+  return launch_unit_fwd(a, dtype, (hipStream_t)stream);
+}
+
+int smoe_glu_8bit_bwd(const void* P8, const void* PS, const void* dh, int64_t sdh, void* dpre, void* h, int64_t rows, int64_t F, int act,
+                      int dtype, void* stream) {
+  set_error("%s", "");
+  if (int rc = unit_checks("smoe_glu_8bit_bwd", rows, F, act, dtype)) return rc;
+  if (rows == 0 || F == 0) return 0;
+  if (!P8 || !PS || !dh || !dpre) { set_error("smoe_glu_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
+  if ((uintptr_t)P8 & 15) { set_error("smoe_glu_8bit_bwd: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
+  UnitBackArgs a{(const uint8_t*)P8, (const uint8_t*)PS, dh, sdh, dpre, nullptr, nullptr, h, rows, F, act};
+  return launch_unit_bwd(a, dtype, (hipStream_t)stream);
+}
+
+static int product_checks(const char* who, int64_t L, int64_t K, int64_t N, int E, int fan, int dtype) {
+  if (!float_type(dtype)) { set_error("%s: unknown dtype %d", who, dtype); return SMOE_ERR_DTYPE; }
+  if (L < 0 || K <= 0 || N < 0 || E <= 0 || fan <= 0 || L % fan != 0) { set_error("%s: bad sizes", who); return SMOE_ERR_SHAPE; }
+  if (L > 0x7fffffffLL || K > MOST || N > MOST) { set_error("%s: size beyond int32", who); return SMOE_ERR_RANGE; }
+  return 0;
+}
+static int workspace_check(const char* who, size_t need, const void* workspace, size_t bytes) {
+  if (workspace && bytes >= need && ((uintptr_t)workspace & 255) == 0) return 0;
+  set_error("%s: a workspace of %zu bytes, 256-byte aligned, is needed, %zu given", who, need, workspace ? bytes : (size_t)0);
+  return SMOE_ERR_WORKSPACE;
+}
+
+size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int fan_out, int x_grouped, int scaled) {
+  if (L <= 0 || K <= 0 || fan_out <= 0) return 0;
+  Carver c{nullptr};
+  take_rows(c, gathers(L, K, fan_out, x_grouped, scaled != 0) ? L / fan_out : L, K);
+  return c.used;
+}
+
+int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_weight_8bit* W, int transposed, const void* b, int64_t sbe,
+                     int64_t sbn, void* Y, int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E,
+                     int fan_out, int x_grouped, int y_grouped, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("%s", "");
+  if (int rc = product_checks("smoe_linear_8bit", L, K, N, E, fan_out, dtype)) return rc;
+  if (L == 0 || N == 0) return 0;
+  if (!X || !Y || !idx || !off) { set_error("smoe_linear_8bit: NULL pointer"); return SMOE_ERR_NULL; }
+  if (coeff && x_grouped) { set_error("smoe_linear_8bit: rows that are scaled come by token"); return SMOE_ERR_SHAPE; }
+  if (int rc = weight_checks("smoe_linear_8bit", W, N, K)) return rc;
+  if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, fan_out, x_grouped, coeff != nullptr), workspace, workspace_bytes)) return rc;
+  Carver c{(char*)workspace};
+  const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
+  const Rows8Bit x = take_rows(c, by_token ? L / fan_out : L, K);
+  const bool copies = !x_grouped && !by_token;
+  if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
+  return launch_product_8bit(product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan_out, !by_token, y_grouped), dtype, dtype,
+                             (hipStream_t)stream);
+}
+
+// the pieces of a gated layer's workspace
+struct LayerPieces { Rows8Bit x, h; float* pre; };
+static LayerPieces layer_pieces(Carver& c, int64_t L, int k, int64_t d, int64_t F) {
+  LayerPieces p{};
+  p.x = take_rows(c, gathers(L, d, k, 0, false) ? L / k : L, d);
+  p.h = take_rows(c, L, F);
+  p.pre = c.take<float>(L * 2 * F * 4);
+  return p;
+}
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E) {
+  if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
+  Carver c{nullptr};
+  layer_pieces(c, T * k, k, d, F);
+  return c.used;
+}
+
+int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const smoe_weight_8bit* W1, const void* b1, int64_t sb1e, int64_t sb1n,
+                      const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT, void* P8, void* PS,
+                      const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("%s", "");
+  hipStream_t st = (hipStream_t)stream;
+  if (k <= 0 || F <= 0) { set_error("smoe_glu_mlp_8bit: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (int rc = product_checks("smoe_glu_mlp_8bit", T * k, d, F, E, k, dtype)) return rc;
+  if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit: unknown activation %d", act); return SMOE_ERR_SHAPE; }
+  if (T == 0) return 0;
+  if (!X || !gates || !Y || !OUT || !idx || !off || (P8 && !PS)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W1, 2 * F, d)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W2, d, F)) return rc;
+  if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E), workspace, workspace_bytes)) return rc;
+  const int64_t L = T * k;
+  Carver c{(char*)workspace};
+  const LayerPieces p = layer_pieces(c, L, k, d, F);
+  const bool by_token = p.x.rows != L || k == 1;
+  if (int rc = quantize(p.x, X, sxm, by_token ? nullptr : idx, k, nullptr, d, dtype, st)) return rc;
+  if (int rc = launch_product_8bit(product(p.x, W1, false, b1, sb1e, sb1n, p.pre, 2 * F, idx, off, L, d, 2 * F, E, k, !by_token, 1), dtype, SMOE_F32, st)) return rc;
+  UnitArgs u{p.pre, 2 * F, nullptr, p.h.q, p.h.s, (uint8_t*)P8, (uint8_t*)PS, L, F, act};
+  if (int rc = launch_unit_fwd(u, SMOE_F32, st)) return rc;
+  if (int rc = launch_product_8bit(product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
+  return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
+}
+
+struct BackPieces { Rows8Bit dy, dp; float* dh; };
+static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F) {
+  BackPieces p{};
+  p.dy = take_rows(c, L, d);
+  p.dp = take_rows(c, L, 2 * F);
+  p.dh = c.take<float>(L * F * 4);
+  return p;
+}
+size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E) {
+  if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
+  Carver c{nullptr};
+  back_pieces(c, T * k, d, F);
+  return c.used;
+}
+
+int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, const smoe_weight_8bit* W1T, const smoe_weight_8bit* W2T,
+                          const void* P8, const void* PS, void* DROWS, void* DX, const int64_t* idx, const int64_t* off, int64_t T, int k,
+                          int64_t d, int64_t F, int E, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("%s", "");
+  hipStream_t st = (hipStream_t)stream;
+  if (k <= 0 || F <= 0) { set_error("smoe_glu_mlp_8bit_bwd: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (int rc = product_checks("smoe_glu_mlp_8bit_bwd", T * k, 2 * F, d, E, k, dtype)) return rc;
+  if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit_bwd: unknown activation %d", act); return SMOE_ERR_SHAPE; }
+  if (T == 0 || d == 0) return 0;
+  if (!DOUT || !gates || !P8 || !PS || !DROWS || !DX || !idx || !off) { set_error("smoe_glu_mlp_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T, d, 2 * F)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T, F, d)) return rc;
+  if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E), workspace, workspace_bytes)) return rc;
+  const int64_t L = T * k;
+  Carver c{(char*)workspace};
+  const BackPieces p = back_pieces(c, L, d, F);
+  if (int rc = quantize(p.dy, DOUT, sdm, idx, k, gates, d, dtype, st)) return rc;
+  if (int rc = launch_product_8bit(product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, 1, 1), dtype, SMOE_F32, st)) return rc;
+  UnitBackArgs u{(const uint8_t*)P8, (const uint8_t*)PS, p.dh, F, nullptr, p.dp.q, p.dp.s, nullptr, L, F, act};
+  if (int rc = launch_unit_bwd(u, SMOE_F32, st)) return rc;
+  if (int rc = launch_product_8bit(product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
+  return launch_combine(DROWS, d, nullptr, 0, 0, DX, d, T, k, (int)d, dtype, st);
+}
+
+}  // extern "C"

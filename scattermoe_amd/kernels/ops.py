@@ -46,6 +46,12 @@ def _whole_rows(x):
     return _whole(x)
 
 
+def _weight_8bit(q, s):
+    """smoe_weight_8bit of a weight (E, N, K) and its scales."""
+    return _C.Weight8bit(q.data_ptr(), q.stride(0), q.stride(1), s.data_ptr(), s.stride(0), s.stride(1), s.stride(2),
+                         int(s.dtype == torch.float32))
+
+
 class HipBackend:
     """Launches the gfx950 kernels on the current torch stream of the tensors' device."""
 
@@ -384,6 +390,89 @@ class HipBackend:
                 _C.stream_ptr(X.device))
         _C.check(rc, "smoe_adapter_backward")
 
+    @staticmethod
+    def quantize_rows(X, Q, S):
+        _C.require_gpu(X, "quantize_blocks")
+        with _C.on_device(X.device):
+            rc = _C.load().smoe_quantize_rows(_C.ptr(X), X.stride(0), X.size(0), X.size(1), _C.ptr(Q), _C.ptr(S), _C.float_code(X.dtype),
+                                              _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_quantize_rows")
+
+    @staticmethod
+    def quantize_weights(W, Q, QT, S):
+        _C.require_gpu(W, "quantize_blocks")
+        with _C.on_device(W.device):
+            rc = _C.load().smoe_quantize_weights(_C.ptr(W), W.stride(0), W.stride(1), W.size(0), W.size(1), W.size(2), _C.ptr(Q), _C.ptr(QT),
+                                                 _C.ptr(S), _C.float_code(W.dtype), _C.stream_ptr(W.device))
+        _C.check(rc, "smoe_quantize_weights")
+
+    @staticmethod
+    def dequantize(Q, S, block_rows, Y):
+        _C.require_gpu(Q, "dequantize_blocks")
+        with _C.on_device(Q.device):
+            rc = _C.load().smoe_dequantize_8bit(_C.ptr(Q), Q.stride(0), Q.stride(1), _C.ptr(S), S.stride(0), S.stride(1), S.stride(2),
+                                                int(S.dtype == torch.float32), block_rows, Y.size(0), Y.size(1), Y.size(2), _C.ptr(Y),
+                                                _C.float_code(Y.dtype), _C.stream_ptr(Q.device))
+        _C.check(rc, "smoe_dequantize_8bit")
+
+    @staticmethod
+    def glu_8bit_fwd(pre, h, P8, PS, act):
+        _C.require_gpu(pre, "glu_8bit_fwd")
+        with _C.on_device(pre.device):
+            rc = _C.load().smoe_glu_8bit_fwd(_C.ptr(pre), pre.stride(0), _C.ptr(h), _C.ptr(P8), _C.ptr(PS), pre.size(0), pre.size(1) // 2,
+                                             act, _C.float_code(pre.dtype), _C.stream_ptr(pre.device))
+        _C.check(rc, "smoe_glu_8bit_fwd")
+
+    @staticmethod
+    def glu_8bit_bwd(P8, PS, dh, dpre, h, act):
+        _C.require_gpu(dh, "glu_8bit_bwd")
+        with _C.on_device(dh.device):
+            rc = _C.load().smoe_glu_8bit_bwd(_C.ptr(P8), _C.ptr(PS), _C.ptr(dh), dh.stride(0), _C.ptr(dpre), _C.ptr(h), dh.size(0), dh.size(1),
+                                             act, _C.float_code(dh.dtype), _C.stream_ptr(dh.device))
+        _C.check(rc, "smoe_glu_8bit_bwd")
+
+    @staticmethod
+    def linear_8bit(X, coeff, W, S, transposed, b, Y, idx, off, k, x_grouped, y_grouped):
+        _C.require_gpu(X, "linear_8bit")
+        lib = _C.load()
+        L, K = idx.numel(), X.size(1)
+        sb = (b.stride(0), b.stride(1)) if b is not None else (0, 0)
+        need = lib.smoe_linear_8bit_workspace_bytes(L, K, k, int(x_grouped), int(coeff is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=X.device)
+        with _C.on_device(X.device):
+            rc = lib.smoe_linear_8bit(_C.ptr(X), X.stride(0), _C.ptr(coeff), _weight_8bit(W, S), int(transposed), _C.ptr(b), *sb, _C.ptr(Y),
+                                      Y.stride(0), _C.ptr(idx), _C.ptr(off), L, K, Y.size(1), W.size(0), k, int(x_grouped), int(y_grouped),
+                                      _C.float_code(X.dtype), _C.ptr(ws), need, _C.stream_ptr(X.device))
+        _C.check(rc, "smoe_linear_8bit")
+
+    @staticmethod
+    def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act):
+        _C.require_gpu(x, "glu_mlp_8bit")
+        lib = _C.load()
+        T, k, d, F, E = x.size(0), gates.size(1), x.size(1), w1.size(1) // 2, w1.size(0)
+        sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
+        sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
+        need = lib.smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        with _C.on_device(x.device):
+            rc = lib.smoe_glu_mlp_8bit(_C.ptr(x), x.stride(0), _C.ptr(gates), _weight_8bit(w1, s1), _C.ptr(b1), *sb1, _weight_8bit(w2, s2),
+                                       _C.ptr(b2), *sb2, _C.ptr(rows), _C.ptr(out), _C.ptr(P8), _C.ptr(PS), _C.ptr(idx), _C.ptr(off), T, k, d,
+                                       F, E, act, _C.float_code(x.dtype), _C.ptr(ws), need, _C.stream_ptr(x.device))
+        _C.check(rc, "smoe_glu_mlp_8bit")
+
+    @staticmethod
+    def glu_mlp_8bit_bwd(d_out, gates, w1t, s1, w2t, s2, P8, PS, drows, dx, idx, off, act):
+        _C.require_gpu(d_out, "glu_mlp_8bit backward")
+        lib = _C.load()
+        T, k, d, F, E = d_out.size(0), gates.size(1), d_out.size(1), w2t.size(1), w1t.size(0)
+        need = lib.smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=d_out.device)
+        with _C.on_device(d_out.device):
+            rc = lib.smoe_glu_mlp_8bit_bwd(_C.ptr(d_out), d_out.stride(0), _C.ptr(gates), _weight_8bit(w1t, s1), _weight_8bit(w2t, s2),
+                                           _C.ptr(P8), _C.ptr(PS), _C.ptr(drows), _C.ptr(dx), _C.ptr(idx), _C.ptr(off), T, k, d, F, E, act,
+                                           _C.float_code(d_out.dtype), _C.ptr(ws), need, _C.stream_ptr(d_out.device))
+        _C.check(rc, "smoe_glu_mlp_8bit_bwd")
+
 
 _backend = HipBackend()
 
@@ -514,11 +603,61 @@ def _adapter_backward_op(DY: torch.Tensor, X: torch.Tensor, W: torch.Tensor, A: 
     _backend.adapter_backward(DY, X, W, A, B, ids, scales, idx, off, U, DX, DA, DB, DBIAS)
 
 
+@torch.library.custom_op("scattermoe::quantize_rows", mutates_args={"Q", "S"})
+def _quantize_rows_op(X: torch.Tensor, Q: torch.Tensor, S: torch.Tensor) -> None:
+    _backend.quantize_rows(X, Q, S)
+
+
+@torch.library.custom_op("scattermoe::quantize_weights", mutates_args={"Q", "QT", "S"})
+def _quantize_weights_op(W: torch.Tensor, Q: torch.Tensor, QT: Optional[torch.Tensor], S: torch.Tensor) -> None:
+    _backend.quantize_weights(W, Q, QT, S)
+
+
+@torch.library.custom_op("scattermoe::dequantize", mutates_args={"Y"})
+def _dequantize_op(Q: torch.Tensor, S: torch.Tensor, block_rows: int, Y: torch.Tensor) -> None:
+    _backend.dequantize(Q, S, block_rows, Y)
+
+
+@torch.library.custom_op("scattermoe::glu_8bit_fwd", mutates_args={"h", "P8", "PS"})
+def _glu_8bit_fwd_op(pre: torch.Tensor, h: torch.Tensor, P8: torch.Tensor, PS: torch.Tensor, act: int) -> None:
+    _backend.glu_8bit_fwd(pre, h, P8, PS, act)
+
+
+@torch.library.custom_op("scattermoe::glu_8bit_bwd", mutates_args={"dpre", "h"})
+def _glu_8bit_bwd_op(P8: torch.Tensor, PS: torch.Tensor, dh: torch.Tensor, dpre: torch.Tensor, h: Optional[torch.Tensor],
+                     act: int) -> None:
+    _backend.glu_8bit_bwd(P8, PS, dh, dpre, h, act)
+
+
+@torch.library.custom_op("scattermoe::linear_8bit", mutates_args={"Y"})
+def _linear_8bit_op(X: torch.Tensor, coeff: Optional[torch.Tensor], W: torch.Tensor, S: torch.Tensor, transposed: bool,
+                    b: Optional[torch.Tensor], Y: torch.Tensor, idx: torch.Tensor, off: torch.Tensor, k: int, x_grouped: bool,
+                    y_grouped: bool) -> None:
+    _backend.linear_8bit(X, coeff, W, S, transposed, b, Y, idx, off, k, x_grouped, y_grouped)
+
+
+@torch.library.custom_op("scattermoe::glu_mlp_8bit", mutates_args={"rows", "out", "P8", "PS"})
+def _glu_mlp_8bit_op(x: torch.Tensor, gates: torch.Tensor, w1: torch.Tensor, s1: torch.Tensor, b1: Optional[torch.Tensor],
+                     w2: torch.Tensor, s2: torch.Tensor, b2: Optional[torch.Tensor], rows: torch.Tensor, out: torch.Tensor,
+                     P8: Optional[torch.Tensor], PS: Optional[torch.Tensor], idx: torch.Tensor, off: torch.Tensor, act: int) -> None:
+    _backend.glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act)
+
+
+@torch.library.custom_op("scattermoe::glu_mlp_8bit_bwd", mutates_args={"drows", "dx"})
+def _glu_mlp_8bit_bwd_op(d_out: torch.Tensor, gates: torch.Tensor, w1t: torch.Tensor, s1: torch.Tensor, w2t: torch.Tensor,
+                         s2: torch.Tensor, P8: torch.Tensor, PS: torch.Tensor, drows: torch.Tensor, dx: torch.Tensor,
+                         idx: torch.Tensor, off: torch.Tensor, act: int) -> None:
+    _backend.glu_mlp_8bit_bwd(d_out, gates, w1t, s1, w2t, s2, P8, PS, drows, dx, idx, off, act)
+
+
 _COMPILED_OPS = {"route": _route_op, "offsets": _offsets_op, "combine": _combine_op, "gate_grad": _gate_grad_op,
                  "glu_fwd": _glu_fwd_op, "glu_bwd": _glu_bwd_op, "topk_softmax": _topk_softmax_op,
                  "oss_glu_fwd": _oss_glu_fwd_op, "oss_glu_bwd": _oss_glu_bwd_op,
                  "routed_glu_mlp": _routed_glu_mlp_op, "adapter_forward": _adapter_forward_op,
-                 "adapter_backward": _adapter_backward_op}
+                 "adapter_backward": _adapter_backward_op,
+                 "quantize_rows": _quantize_rows_op, "quantize_weights": _quantize_weights_op, "dequantize": _dequantize_op,
+                 "glu_8bit_fwd": _glu_8bit_fwd_op, "glu_8bit_bwd": _glu_8bit_bwd_op, "linear_8bit": _linear_8bit_op,
+                 "glu_mlp_8bit": _glu_mlp_8bit_op, "glu_mlp_8bit_bwd": _glu_mlp_8bit_bwd_op}
 
 
 def _launch(name, *args):
@@ -1114,3 +1253,107 @@ def adapter_backward(dy, x, weight, lora_a, lora_b, ids, scales, u, order, need_
             if t is not None:
                 t.zero_()
     return dx, da, db, dbias
+
+
+# ------------------------------------------------------------------------------------------------
+# 8 bits: e4m3 with a scale for each block of 128 (a power of two, held as its exponent + 127)
+# ------------------------------------------------------------------------------------------------
+BLOCK_8BIT = 128
+TYPE_8BIT, SCALE_8BIT = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def row_8bit(K):
+    """Bytes of a row of K values in 8 bits: rows start where 16-byte pieces can."""
+    return (K + 15) // 16 * 16
+
+
+def blocks_8bit(K):
+    return (K + BLOCK_8BIT - 1) // BLOCK_8BIT
+
+
+def quantize_rows(x):
+    """(q (rows, K rounded up to 16) e4m3, scales (rows, blocks) e8m0) of x (rows, K)."""
+    rows, K = x.shape
+    x = _rows_contiguous(x)
+    q = torch.empty((rows, row_8bit(K)), dtype=TYPE_8BIT, device=x.device)
+    s = torch.empty((rows, (blocks_8bit(K) + 3) // 4 * 4), dtype=SCALE_8BIT, device=x.device)
+    if rows and K:
+        _launch("quantize_rows", x, q, s)
+    return q, s[:, :blocks_8bit(K)]
+
+
+def quantize_weights(w, transposed=False):
+    """(q (E, N, K rounded up to 16) e4m3, scales (E, N blocks, K blocks) e8m0, q of the transpose (E, K, N rounded up to 16) or None)."""
+    E, N, K = w.shape
+    w = _rows_contiguous(w)
+    q = torch.empty((E, N, row_8bit(K)), dtype=TYPE_8BIT, device=w.device)
+    qt = torch.empty((E, K, row_8bit(N)), dtype=TYPE_8BIT, device=w.device) if transposed else None
+    s = torch.empty((E, blocks_8bit(N), blocks_8bit(K)), dtype=SCALE_8BIT, device=w.device)
+    if w.numel():
+        _launch("quantize_weights", w, q, qt, s)
+    return q, s, qt
+
+
+def dequantize(q, s, block_rows, K, dtype):
+    """The values (E, N, K) that q (E, N, K or more) and its scales, one for block_rows x 128 of them, stand for."""
+    q = _rows_contiguous(q)
+    y = torch.empty((q.size(0), q.size(1), K), dtype=dtype, device=q.device)
+    if y.numel():
+        _launch("dequantize", q, s, block_rows, y)
+    return y
+
+
+def glu_8bit_fwd(pre, act=ACT_SILU):
+    """(h, p8, ps): the gated unit of pre (rows, 2F), and the halves of pre in 8 bits (rows, 2, F rounded up to 16) with their scales."""
+    assert pre.dim() == 2 and pre.size(1) % 2 == 0
+    pre = _rows_contiguous(pre)
+    rows, F = pre.size(0), pre.size(1) // 2
+    h = torch.empty((rows, F), dtype=pre.dtype, device=pre.device)
+    p8 = torch.empty((rows, 2, row_8bit(F)), dtype=TYPE_8BIT, device=pre.device)
+    ps = torch.empty((rows, 2, blocks_8bit(F)), dtype=SCALE_8BIT, device=pre.device)
+    if h.numel():
+        _launch("glu_8bit_fwd", pre, h, p8, ps, act)
+    return h, p8, ps
+
+
+def glu_8bit_bwd(p8, ps, dh, act=ACT_SILU, need_h=False):
+    """(d(pre), h): the gradient of what `glu_8bit_fwd` kept, and (`need_h`) the unit's value of it."""
+    dh = _rows_contiguous(dh)
+    rows, F = dh.shape
+    dpre = torch.empty((rows, 2 * F), dtype=dh.dtype, device=dh.device)
+    h = torch.empty((rows, F), dtype=dh.dtype, device=dh.device) if need_h else None
+    if dh.numel():
+        _launch("glu_8bit_bwd", p8, ps, dh, dpre, h, act)
+    return dpre, h
+
+
+def linear_8bit(x, w, s, idx, off, k, b=None, coeff=None, transposed=False, x_grouped=False, y_grouped=False):
+    """scatter2scatter with x (rows of it taken to 8 bits, times coeff[slot] before that) and w (E, N, K) e4m3: (L, N) rows."""
+    x = _rows_contiguous(x)
+    y = torch.empty((idx.numel(), w.size(1)), dtype=x.dtype, device=x.device)
+    if y.numel():
+        _launch("linear_8bit", x, coeff, w, s, transposed, b, y, idx, off, k, x_grouped, y_grouped)
+    return y
+
+
+def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, idx, off, act=ACT_SILU, keep=False):
+    """(out (T, d), rows (T k, d) by slot, p8, ps): a gated layer on weights in 8 bits; `keep`: the halves of its pre-activation."""
+    x = _rows_contiguous(x)
+    T, d, L, F = x.size(0), x.size(1), idx.numel(), w1.size(1) // 2
+    out = torch.empty((T, d), dtype=x.dtype, device=x.device)
+    rows = torch.empty((L, d), dtype=x.dtype, device=x.device)
+    p8 = torch.empty((L, 2, row_8bit(F)), dtype=TYPE_8BIT, device=x.device) if keep else None
+    ps = torch.empty((L, 2, blocks_8bit(F)), dtype=SCALE_8BIT, device=x.device) if keep else None
+    if out.numel():
+        _launch("glu_mlp_8bit", x, gates.contiguous(), w1, s1, b1, w2, s2, b2, rows, out, p8, ps, idx, off, act)
+    return out, rows, p8, ps
+
+
+def glu_mlp_8bit_bwd(d_out, gates, w1t, s1, w2t, s2, p8, ps, idx, off, act=ACT_SILU):
+    """The gradient of the layer's tokens, from the transposed weights."""
+    d_out = _rows_contiguous(d_out)
+    dx = torch.empty(d_out.shape, dtype=d_out.dtype, device=d_out.device)
+    drows = torch.empty((idx.numel(), d_out.size(1)), dtype=d_out.dtype, device=d_out.device)
+    if dx.numel():
+        _launch("glu_mlp_8bit_bwd", d_out, gates.contiguous(), w1t, s1, w2t, s2, p8, ps, drows, dx, idx, off, act)
+    return dx
