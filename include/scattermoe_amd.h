@@ -437,13 +437,13 @@ int smoe_glu_8bit_bwd(const void* P8, const void* PS, const void* dh, int64_t sd
                       int dtype, void* stream);
 
 /*
- * A weight in 8 bits: q (E, N, K), contraction contiguous and filled with zeros to a multiple of 16, rows at multiples of 16
- * bytes; s: a scale for every 128 x 128 values, 8 bits (a power of two) or float32 (any).  Strides in elements.  A transposed
+ * A weight in 8 bits: q (E, N, K rounded up to 16), filled with zeros, an expert's values contiguous from a multiple of 16
+ * bytes on; s: a scale for every 128 x 128 values, 8 bits (a power of two) or float32 (any).  Strides in elements.  A transposed
  * weight has the scales, and the scales' strides, of the weight that it is the transpose of.
  */
 typedef struct {
   const void* q;
-  int64_t q_expert, q_row;
+  int64_t q_expert;
   const void* s;
   int64_t s_expert, s_row, s_col;
   int s_float32;
@@ -464,15 +464,18 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
  * A gated layer on such weights (GLUMLP.forward, scattermoe/mlp.py:74-95):
  *   pre = Q(X) W1[e]^T + b1[e];  y = Q(glu(pre)) W2[e]^T + b2[e];  OUT[t] = sum_j gates[t,j] y
  * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) by slot (y, rounded), OUT (T,d)
- * contiguous; P8, PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL.
+ * contiguous; P8, PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
+ * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
+ * alone, and ids outside [0,E) drop their row.
  * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with
  * the scales of the weights; DROWS (T k, d): what every slot adds to DX (T,d).  Workspaces as above.
  */
-size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E);
-int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const smoe_weight_8bit* W1, const void* b1, int64_t sb1e, int64_t sb1n,
-                      const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT, void* P8, void* PS,
-                      const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act, int dtype,
-                      void* workspace, size_t workspace_bytes, void* stream);
+#define SMOE_8BIT_FEW_ROWS 64
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep);
+int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64_t* experts, const smoe_weight_8bit* W1, const void* b1,
+                      int64_t sb1e, int64_t sb1n, const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT,
+                      void* P8, void* PS, const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act,
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream);
 size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E);
 int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, const smoe_weight_8bit* W1T, const smoe_weight_8bit* W2T,
                           const void* P8, const void* PS, void* DROWS, void* DX, const int64_t* idx, const int64_t* off, int64_t T, int k,

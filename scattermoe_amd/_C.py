@@ -26,7 +26,7 @@ _p, _i64, _int, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctype
 
 class Weight8bit(ctypes.Structure):
     """smoe_weight_8bit"""
-    _fields_ = [("q", _p), ("q_expert", _i64), ("q_row", _i64), ("s", _p), ("s_expert", _i64), ("s_row", _i64), ("s_col", _i64),
+    _fields_ = [("q", _p), ("q_expert", _i64), ("s", _p), ("s_expert", _i64), ("s_row", _i64), ("s_col", _i64),
                 ("s_float32", _int)]
 
 
@@ -89,8 +89,8 @@ _SIGNATURES = {
     "smoe_linear_8bit_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int]),
     "smoe_linear_8bit": (_int, [_p, _i64, _p, _w8, _int, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _int, _int, _int, _int, _int,
                                 _p, _sz, _p]),
-    "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int]),
-    "smoe_glu_mlp_8bit": (_int, [_p, _i64, _p, _w8, _p, _i64, _i64, _w8, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64,
+    "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int, _int, _int]),
+    "smoe_glu_mlp_8bit": (_int, [_p, _i64, _p, _p, _w8, _p, _i64, _i64, _w8, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64,
                                  _int, _int, _int, _p, _sz, _p]),
     "smoe_glu_mlp_8bit_bwd_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int]),
     "smoe_glu_mlp_8bit_bwd": (_int, [_p, _i64, _p, _w8, _w8, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64, _int, _int, _int, _p, _sz, _p]),

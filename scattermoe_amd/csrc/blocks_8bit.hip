@@ -94,22 +94,23 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantRowsArgs a, int
   if (!u.there) return;
   int64_t src = u.row;
   float f = 1.0f;
+  bool have = true;                                                // (a row that the routing dropped has no source)
   if (a.idx) {
     const int64_t i = a.idx[u.row];
-    src = i / a.fan;
-    if (a.coeff) f = to_f32(((const T*)a.coeff)[i]);
+    have = i >= 0 && i < a.slots;
+    src = have ? i / a.fan : 0;
+    if (a.coeff && have) f = to_f32(((const T*)a.coeff)[i]);
   }
   float v[8];
-  load8<T, VEC>((const T*)a.X + src * a.sxm, u.c, a.K, v);
+  load8<T, VEC>((const T*)a.X + src * a.sxm, have ? u.c : a.K, a.K, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= f;
-  const int64_t Kp = padded_row(a.K);
-  store_block(a.Q + u.row * Kp, a.S + u.row * scale_row(a.K) + u.block, u.c, Kp, v);
+  store_block(a.Q + u.row * a.ld, a.S + u.row * scale_row(a.K) + u.block, u.c, a.ld, v);
 }
 
 template <typename T>
 static int quantize_rows(QuantRowsArgs a, hipStream_t st) {
-  const int64_t blocks = scale_blocks(a.K), Kp = padded_row(a.K), Sr = scale_row(a.K);
+  const int64_t blocks = scale_blocks(a.K), Sr = scale_row(a.K);
   const bool vec = ((uintptr_t)a.X & 15) == 0 && a.sxm * (int64_t)sizeof(T) % 16 == 0 && a.K % 8 == 0;
   int64_t left = a.rows;
   while (left > 0) {
@@ -120,7 +121,7 @@ static int quantize_rows(QuantRowsArgs a, hipStream_t st) {
     left -= a.rows;
     if (a.idx) a.idx += a.rows;
     else a.X = (const T*)a.X + a.rows * a.sxm;
-    a.Q += a.rows * Kp;
+    a.Q += a.rows * a.ld;
     a.S += a.rows * Sr;
   }
   return launch_status("quantize_rows");
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(256) void unit_fwd_kernel(UnitArgs a, int blocks) {
   load8<TI, VEC>(pre + (a.act & 1 ? 0 : F), u.c, F, gat);
 #pragma unroll
   for (int i = 0; i < 8; ++i) h[i] = glu_h(a.act, gat[i], lin[i]);
-  if constexpr (QUANT) store_block(a.H8 + u.row * Fp, a.HS + u.row * scale_row(F) + u.block, u.c, Fp, h);
+  if constexpr (QUANT) store_block(a.H8 + u.row * block_row(F), a.HS + u.row * scale_row(F) + u.block, u.c, block_row(F), h);
   else store8<TI, VEC>((TI*)a.h + u.row * F, u.c, F, h);
   if (a.P8) {
     store_block(a.P8 + u.row * 2 * Fp, a.PS + u.row * 2 * blocks + u.block, u.c, Fp, lin);
@@ -268,7 +269,7 @@ static int unit_fwd(UnitArgs a, hipStream_t st) {
     left -= a.rows;
     a.pre = (const TI*)a.pre + a.rows * a.spm;
     if (a.h) a.h = (TI*)a.h + a.rows * a.F;
-    if (a.H8) a.H8 += a.rows * Fp, a.HS += a.rows * scale_row(a.F);
+    if (a.H8) a.H8 += a.rows * block_row(a.F), a.HS += a.rows * scale_row(a.F);
     if (a.P8) a.P8 += a.rows * 2 * Fp, a.PS += a.rows * 2 * blocks;
   }
   return launch_status("unit_fwd");
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(256) void unit_bwd_kernel(UnitBackArgs a, int block
 __global__ __launch_bounds__(256) void unit_bwd_8bit_kernel(UnitBackArgs a, int blocks) {
   const Unit u(a.rows, blocks);
   if (!u.there) return;
-  const int64_t F = a.F, Fp = padded_row(F), D = 2 * F, Dp = padded_row(D);
+  const int64_t F = a.F, Fp = padded_row(F), D = 2 * F, Dp = block_row(D);
   const int hb = (int)scale_blocks(F);
   const uint8_t* p8 = a.P8 + u.row * 2 * Fp;
   const uint8_t* ps = a.PS + u.row * 2 * hb;
@@ -363,7 +364,7 @@ static int unit_bwd(UnitBackArgs a, hipStream_t st) {
     left -= a.rows;
     a.P8 += a.rows * 2 * Fp, a.PS += a.rows * 2 * hb;
     a.dh = (const T*)a.dh + a.rows * a.sdh;
-    if (quant) a.D8 += a.rows * padded_row(2 * F), a.DS += a.rows * scale_row(2 * F);
+    if (quant) a.D8 += a.rows * block_row(2 * F), a.DS += a.rows * scale_row(2 * F);
     else a.dpre = (T*)a.dpre + a.rows * 2 * F;
     if (a.h) a.h = (T*)a.h + a.rows * F;
   }

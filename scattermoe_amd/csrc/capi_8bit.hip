@@ -23,34 +23,32 @@ struct Carver {
 // Rows of 8-bit activations of a product of L rows: the tokens once, or a copy for each row where they are scaled one by one or where
 // the token matrix passes the 32-bit offsets that a gathered operand has
 static bool gathers(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
-  return !x_grouped && !scaled && L / fan * padded_row(K) < (1LL << 32);
+  return !x_grouped && !scaled && L / fan * block_row(K) < (1LL << 32);
 }
 struct Rows8Bit { uint8_t* q; uint8_t* s; int64_t rows; };
 static Rows8Bit take_rows(Carver& c, int64_t rows, int64_t K) {
   Rows8Bit r{nullptr, nullptr, rows};
-  r.q = c.take(rows * padded_row(K));
+  r.q = c.take(rows * block_row(K) + QB);                          // (a product reads a slice further, and does not look at it)
   r.s = c.take(rows * scale_row(K));
   return r;
 }
 static int quantize(const Rows8Bit& r, const void* X, int64_t sxm, const int64_t* idx, int fan, const void* coeff, int64_t K, int dtype,
                     hipStream_t st) {
-  QuantRowsArgs a{X, sxm, idx, fan, coeff, r.rows, K, r.q, r.s};
+  QuantRowsArgs a{X, sxm, idx, fan, coeff, r.rows, K, r.q, r.s, r.rows, block_row(K)};
   return launch_quantize_rows(a, dtype, st);
 }
 
-static int weight_checks(const char* who, const smoe_weight_8bit* w, int64_t N, int64_t K) {
+static int weight_checks(const char* who, const smoe_weight_8bit* w) {
   if (!w || !w->q || !w->s) { set_error("%s: NULL weight", who); return SMOE_ERR_NULL; }
-  if (((uintptr_t)w->q | w->q_expert | w->q_row) & 15) { set_error("%s: weights' rows start at multiples of 16 bytes", who); return SMOE_ERR_SHAPE; }
-  if (w->q_row < padded_row(K) && N > 1) { set_error("%s: weights' rows of %lld bytes are needed", who, (long long)padded_row(K)); return SMOE_ERR_SHAPE; }
-  if (N * w->q_row >= (1LL << 40)) { set_error("%s: weights too large", who); return SMOE_ERR_RANGE; }
+  if (((uintptr_t)w->q | w->q_expert) & 15) { set_error("%s: an expert's weights start at multiples of 16 bytes", who); return SMOE_ERR_SHAPE; }
   return 0;
 }
 static Product8Args product(const Rows8Bit& x, const smoe_weight_8bit* w, bool transposed, const void* b, int64_t sbe, int64_t sbn, void* Y,
                             int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E, int fan,
                             int x_grouped, int y_grouped) {
   Product8Args a{};
-  a.X = x.q, a.XS = x.s, a.x_rows = x.rows;
-  a.W = (const uint8_t*)w->q, a.swe = w->q_expert, a.swn = w->q_row;
+  a.X = x.q, a.XS = x.s;
+  a.W = (const uint8_t*)w->q, a.swe = w->q_expert, a.swn = padded_row(K);
   a.WS = w->s, a.sse = w->s_expert, a.ssn = transposed ? w->s_col : w->s_row, a.ssk = transposed ? w->s_row : w->s_col;
   a.ws_f32 = w->s_float32;
   a.b = b, a.sbe = sbe, a.sbn = sbn;
@@ -59,6 +57,20 @@ static Product8Args product(const Rows8Bit& x, const smoe_weight_8bit* w, bool t
   a.L = (int)L, a.K = (int)padded_row(K), a.N = (int)N, a.E = E, a.fan = fan, a.x_grouped = x_grouped, a.y_grouped = y_grouped;
   return a;
 }
+
+static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64_t sbn, void* Y, int64_t sym, int out_dtype, const int64_t* ids,
+                    const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E, int fan, int x_grouped, int y_grouped, int act) {
+  Few8Args a{};
+  a.W = (const uint8_t*)w->q, a.swe = w->q_expert;
+  a.WS = w->s, a.sse = w->s_expert, a.ssn = w->s_row, a.ssk = w->s_col, a.ws_f32 = w->s_float32;
+  a.b = b, a.sbe = sbe, a.sbn = sbn;
+  a.Y = Y, a.sym = sym, a.out_dtype = out_dtype;
+  a.ids = ids, a.idx = idx, a.off = off;
+  a.L = (int)L, a.K = (int)K, a.N = (int)N, a.E = E, a.fan = fan, a.x_grouped = x_grouped, a.y_grouped = y_grouped, a.act = act;
+  return a;
+}
+// Streams over the weights instead of tiles
+static bool few_rows_pay(int64_t L, int E) { return L <= 16 * (int64_t)E; }
 
 }  // namespace smoe
 
@@ -77,7 +89,7 @@ int smoe_quantize_rows(const void* X, int64_t sxm, int64_t rows, int64_t K, void
   if (rows == 0 || K == 0) return 0;
   if (!X || !Q || !S) { set_error("smoe_quantize_rows: NULL pointer"); return SMOE_ERR_NULL; }
   if ((uintptr_t)Q & 15) { set_error("smoe_quantize_rows: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
-  QuantRowsArgs a{X, sxm, nullptr, 1, nullptr, rows, K, (uint8_t*)Q, (uint8_t*)S};
+  QuantRowsArgs a{X, sxm, nullptr, 1, nullptr, rows, K, (uint8_t*)Q, (uint8_t*)S, rows, padded_row(K)};
   return launch_quantize_rows(a, dtype, (hipStream_t)stream);
 }
 
@@ -162,55 +174,103 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   if (L == 0 || N == 0) return 0;
   if (!X || !Y || !idx || !off) { set_error("smoe_linear_8bit: NULL pointer"); return SMOE_ERR_NULL; }
   if (coeff && x_grouped) { set_error("smoe_linear_8bit: rows that are scaled come by token"); return SMOE_ERR_SHAPE; }
-  if (int rc = weight_checks("smoe_linear_8bit", W, N, K)) return rc;
+  if (int rc = weight_checks("smoe_linear_8bit", W)) return rc;
   if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, fan_out, x_grouped, coeff != nullptr), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
   const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
   const Rows8Bit x = take_rows(c, by_token ? L / fan_out : L, K);
   const bool copies = !x_grouped && !by_token;
   if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
+  if (few_rows_pay(L, E)) {
+    Few8Args a = few(W, b, sbe, sbn, Y, sym, dtype, nullptr, idx, off, L, K, N, E, fan_out, !by_token, y_grouped, 0);
+    if (transposed) a.ssn = W->s_col, a.ssk = W->s_row;
+    a.X = x.q, a.sxm = block_row(K), a.XS = x.s;
+    return launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, (hipStream_t)stream);
+  }
   return launch_product_8bit(product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan_out, !by_token, y_grouped), dtype, dtype,
                              (hipStream_t)stream);
 }
 
+// How a layer goes.  Without an order of its rows: by their ids, two streams over the weights of the experts that they name.  Few rows per
+// expert: streams over the weights, rows by expert.  Else tiles, with the unit behind the first product where it rides.
+enum LayerWay { LAYER_BY_IDS, LAYER_FEW, LAYER_TILES, LAYER_TILES_UNIT };
+static LayerWay layer_way(int64_t L, int64_t d, int64_t F, int E, bool ordered, bool keep) {
+  if (!ordered) return LAYER_BY_IDS;
+  if (!keep && few_rows_pay(L, E)) return LAYER_FEW;
+  return unit_rides(d, F) ? LAYER_TILES_UNIT : LAYER_TILES;
+}
 // the pieces of a gated layer's workspace
-struct LayerPieces { Rows8Bit x, h; float* pre; };
-static LayerPieces layer_pieces(Carver& c, int64_t L, int k, int64_t d, int64_t F) {
+struct LayerPieces { Rows8Bit x, h; float* pre; float* hidden; float* rows; };
+static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64_t d, int64_t F) {
   LayerPieces p{};
+  if (way == LAYER_BY_IDS) {
+    p.hidden = c.take<float>(L * F * 4);
+    p.rows = c.take<float>(L * d * 4);
+    return p;
+  }
   p.x = take_rows(c, gathers(L, d, k, 0, false) ? L / k : L, d);
   p.h = take_rows(c, L, F);
-  p.pre = c.take<float>(L * 2 * F * 4);
+  if (way == LAYER_FEW) p.hidden = c.take<float>(L * F * 4);
+  if (way == LAYER_TILES) p.pre = c.take<float>(L * 2 * F * 4);
   return p;
 }
-size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E) {
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep) {
   if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
   Carver c{nullptr};
-  layer_pieces(c, T * k, k, d, F);
+  layer_pieces(c, layer_way(T * k, d, F, E, ordered != 0, keep != 0), T * k, k, d, F);
   return c.used;
 }
 
-int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const smoe_weight_8bit* W1, const void* b1, int64_t sb1e, int64_t sb1n,
-                      const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT, void* P8, void* PS,
-                      const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act, int dtype,
-                      void* workspace, size_t workspace_bytes, void* stream) {
+int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64_t* experts, const smoe_weight_8bit* W1, const void* b1,
+                      int64_t sb1e, int64_t sb1n, const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT,
+                      void* P8, void* PS, const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act,
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   set_error("%s", "");
   hipStream_t st = (hipStream_t)stream;
   if (k <= 0 || F <= 0) { set_error("smoe_glu_mlp_8bit: bad sizes"); return SMOE_ERR_SHAPE; }
   if (int rc = product_checks("smoe_glu_mlp_8bit", T * k, d, F, E, k, dtype)) return rc;
   if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit: unknown activation %d", act); return SMOE_ERR_SHAPE; }
   if (T == 0) return 0;
-  if (!X || !gates || !Y || !OUT || !idx || !off || (P8 && !PS)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
-  if (int rc = weight_checks("smoe_glu_mlp_8bit", W1, 2 * F, d)) return rc;
-  if (int rc = weight_checks("smoe_glu_mlp_8bit", W2, d, F)) return rc;
-  if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
+  const bool ordered = idx != nullptr;
+  const LayerWay way = layer_way(L, d, F, E, ordered, P8 != nullptr);
+  if (!ordered && (L > SMOE_8BIT_FEW_ROWS || P8)) { set_error("smoe_glu_mlp_8bit: an order is needed for more than %d rows, and to keep P8", SMOE_8BIT_FEW_ROWS); return SMOE_ERR_NULL; }
+  if (!X || !gates || !OUT || (P8 && !PS) || (ordered ? !Y || !off : !experts)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W1)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W2)) return rc;
+  if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, P8 != nullptr), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
-  const LayerPieces p = layer_pieces(c, L, k, d, F);
+  const LayerPieces p = layer_pieces(c, way, L, k, d, F);
+  if (way == LAYER_BY_IDS) {
+    Few8Args a = few(W1, b1, sb1e, sb1n, p.hidden, F, SMOE_F32, experts, nullptr, nullptr, L, d, 2 * F, E, k, 0, 1, act);
+    a.X = X, a.sxm = sxm, a.x_vec = ((uintptr_t)X & 15) == 0 && sxm * (dtype == SMOE_F32 ? 4 : 2) % 16 == 0;
+    if (int rc = launch_few_rows_8bit(a, dtype, dtype, EPI_UNIT, st)) return rc;
+    a = few(W2, b2, sb2e, sb2n, p.rows, d, SMOE_F32, experts, nullptr, nullptr, L, F, d, E, 1, 1, 1, act);
+    a.X = p.hidden, a.sxm = F, a.x_vec = F % 4 == 0;
+    if (int rc = launch_few_rows_8bit(a, SMOE_F32, dtype, EPI_ROWS, st)) return rc;
+    return launch_few_combine(p.rows, gates, experts, OUT, (int)T, k, (int)d, E, dtype, st);
+  }
   const bool by_token = p.x.rows != L || k == 1;
   if (int rc = quantize(p.x, X, sxm, by_token ? nullptr : idx, k, nullptr, d, dtype, st)) return rc;
-  if (int rc = launch_product_8bit(product(p.x, W1, false, b1, sb1e, sb1n, p.pre, 2 * F, idx, off, L, d, 2 * F, E, k, !by_token, 1), dtype, SMOE_F32, st)) return rc;
-  UnitArgs u{p.pre, 2 * F, nullptr, p.h.q, p.h.s, (uint8_t*)P8, (uint8_t*)PS, L, F, act};
-  if (int rc = launch_unit_fwd(u, SMOE_F32, st)) return rc;
+  if (way == LAYER_FEW) {
+    Few8Args a = few(W1, b1, sb1e, sb1n, p.hidden, F, SMOE_F32, nullptr, idx, off, L, d, 2 * F, E, k, !by_token, 1, act);
+    a.X = p.x.q, a.sxm = block_row(d), a.XS = p.x.s;
+    if (int rc = launch_few_rows_8bit(a, -1, dtype, EPI_UNIT, st)) return rc;
+    if (int rc = quantize(p.h, p.hidden, F, nullptr, 1, nullptr, F, SMOE_F32, st)) return rc;
+    a = few(W2, b2, sb2e, sb2n, Y, d, dtype, nullptr, idx, off, L, F, d, E, 1, 1, 0, act);
+    a.X = p.h.q, a.sxm = block_row(F), a.XS = p.h.s;
+    if (int rc = launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, st)) return rc;
+    return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
+  }
+  Product8Args a = product(p.x, W1, false, b1, sb1e, sb1n, p.pre, 2 * F, idx, off, L, d, 2 * F, E, k, !by_token, 1);
+  if (way == LAYER_TILES_UNIT) {
+    a.H8 = p.h.q, a.HS = p.h.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
+    if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st, EPI_UNIT)) return rc;
+  } else {
+    if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st)) return rc;
+    UnitArgs u{p.pre, 2 * F, nullptr, p.h.q, p.h.s, (uint8_t*)P8, (uint8_t*)PS, L, F, act};
+    if (int rc = launch_unit_fwd(u, SMOE_F32, st)) return rc;
+  }
   if (int rc = launch_product_8bit(product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
   return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
 }
@@ -220,7 +280,7 @@ static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F) {
   BackPieces p{};
   p.dy = take_rows(c, L, d);
   p.dp = take_rows(c, L, 2 * F);
-  p.dh = c.take<float>(L * F * 4);
+  p.dh = unit_grad_rides(F) ? nullptr : c.take<float>(L * F * 4);
   return p;
 }
 size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E) {
@@ -240,16 +300,22 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit_bwd: unknown activation %d", act); return SMOE_ERR_SHAPE; }
   if (T == 0 || d == 0) return 0;
   if (!DOUT || !gates || !P8 || !PS || !DROWS || !DX || !idx || !off) { set_error("smoe_glu_mlp_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
-  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T, d, 2 * F)) return rc;
-  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T, F, d)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T)) return rc;
   if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
   Carver c{(char*)workspace};
   const BackPieces p = back_pieces(c, L, d, F);
   if (int rc = quantize(p.dy, DOUT, sdm, idx, k, gates, d, dtype, st)) return rc;
-  if (int rc = launch_product_8bit(product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, 1, 1), dtype, SMOE_F32, st)) return rc;
-  UnitBackArgs u{(const uint8_t*)P8, (const uint8_t*)PS, p.dh, F, nullptr, p.dp.q, p.dp.s, nullptr, L, F, act};
-  if (int rc = launch_unit_bwd(u, SMOE_F32, st)) return rc;
+  Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, 1, 1);
+  if (!p.dh) {
+    a.H8 = p.dp.q, a.HS = p.dp.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
+    if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st, EPI_UNIT_GRAD)) return rc;
+  } else {
+    if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st)) return rc;
+    UnitBackArgs u{(const uint8_t*)P8, (const uint8_t*)PS, p.dh, F, nullptr, p.dp.q, p.dp.s, nullptr, L, F, act};
+    if (int rc = launch_unit_bwd(u, SMOE_F32, st)) return rc;
+  }
   if (int rc = launch_product_8bit(product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
   return launch_combine(DROWS, d, nullptr, 0, 0, DX, d, T, k, (int)d, dtype, st);
 }

@@ -5,8 +5,8 @@
 // the matrix instruction applies it by itself (it takes a power of two, held as its exponent + 127 in 8 bits, per operand row).  A
 // scale that is no power of two would use at most one more binade of e4m3's subnormals.  NaN and infinities become NaN; a block
 // that holds an infinity keeps nothing of its other values.
-// Rows are Kp = K rounded up to 16 bytes long, filled with zeros, so that they start where 16-byte pieces can; their scales are
-// rows of KB = ceil(K / 128) bytes, KB rounded up to 4 apart.
+// Rows are Kp = K rounded up to 16 bytes long, filled with zeros, so that they start where 16-byte pieces can; those that a product
+// reads from a workspace are rounded up to whole blocks.  Their scales are rows of KB = ceil(K / 128) bytes, KB rounded up to 4 apart.
 #pragma once
 #include "common.hpp"
 
@@ -19,6 +19,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 static constexpr int QB = 128;                                     // columns (and, of weights, rows) that share a scale
 
 __host__ __device__ static inline int64_t padded_row(int64_t k) { return (k + 15) / 16 * 16; }
+__host__ __device__ static inline int64_t block_row(int64_t k) { return (k + QB - 1) / QB * QB; }
 __host__ __device__ static inline int64_t scale_blocks(int64_t k) { return (k + QB - 1) / QB; }
 __host__ __device__ static inline int64_t scale_row(int64_t k) { return (scale_blocks(k) + 3) / 4 * 4; }
 
@@ -83,6 +84,8 @@ struct QuantRowsArgs {
   const void* coeff;                                               // times coeff[idx[n]]; NULL: 1
   int64_t rows, K;
   uint8_t* Q; uint8_t* S;
+  int64_t slots;                                                   // with idx: entries outside [0, slots) make a row of zeros
+  int64_t ld;                                                      // bytes of a row of Q, a multiple of 16, zeros behind the last value
 };
 int launch_quantize_rows(const QuantRowsArgs& a, int dtype, hipStream_t st);
 
@@ -106,7 +109,7 @@ int launch_dequantize(const DequantArgs& a, int dtype, hipStream_t st);
 // of pre in 8 bits, each with blocks of its own (NULL: not wanted)
 struct UnitArgs {
   const void* pre; int64_t spm;
-  void* h; uint8_t* H8; uint8_t* HS;
+  void* h; uint8_t* H8; uint8_t* HS;                               // rows of H8 are whole blocks long
   uint8_t* P8; uint8_t* PS;
   int64_t rows, F;
   int act;
@@ -116,7 +119,7 @@ int launch_unit_fwd(const UnitArgs& a, int dtype, hipStream_t st);
 struct UnitBackArgs {
   const uint8_t* P8; const uint8_t* PS;
   const void* dh; int64_t sdh;
-  void* dpre; uint8_t* D8; uint8_t* DS;
+  void* dpre; uint8_t* D8; uint8_t* DS;                            // rows of D8 are whole blocks long
   void* h;                                                         // the unit's value of the halves in 8 bits, too (NULL: not wanted)
   int64_t rows, F;
   int act;
@@ -125,18 +128,44 @@ int launch_unit_bwd(const UnitBackArgs& a, int dtype, hipStream_t st);
 
 // Y[dst(n)] = X[src(n)] W[e(n)]^T (+ b[e(n)]) over rows sorted by expert, X and W in 8 bits
 struct Product8Args {
-  const uint8_t* X; const uint8_t* XS; int64_t x_rows;            // (x_rows, Kp), scales as above
+  const uint8_t* X; const uint8_t* XS;                            // rows of whole blocks, 128 bytes more behind the last; scales as above
   const uint8_t* W; int64_t swe, swn;                             // (E, N, K), contraction contiguous, K a multiple of 16
   const void* WS; int64_t sse, ssn, ssk; int ws_f32;              // a scale per 128 x 128: 8 bits or float32
   const void* b; int64_t sbe, sbn;
   void* Y; int64_t sym;                                           // `out_dtype`
   const int64_t* idx; const int64_t* off;
   int L, K, N, E, fan, x_grouped, y_grouped;
-  // gated unit on the product's columns (lin | gate, F = N / 2) instead of Y: (H8, HS), and (P8, PS) where wanted
+  // instead of Y, of a product whose rows come out by expert:
+  //   the gated unit on its columns (two halves of F = N / 2): H8, HS, and the halves themselves, P8, PS, where wanted
+  //   the gated unit's gradient, the product being dh (F = N), from P8, PS: H8, HS, blocks along all 2F columns
   uint8_t* H8 = nullptr; uint8_t* HS = nullptr; uint8_t* P8 = nullptr; uint8_t* PS = nullptr;
   int act = 0;
 };
+// whether a product can be followed by the unit, or by its gradient, within its tiles
+bool unit_rides(int64_t d, int64_t F);
+bool unit_grad_rides(int64_t F);
+enum Epilogue8 { EPI_ROWS, EPI_UNIT, EPI_UNIT_GRAD };
 // row_dtype: of the rows that were taken to 8 bits and of the bias
-int launch_product_8bit(const Product8Args& a, int row_dtype, int out_dtype, hipStream_t st);
+int launch_product_8bit(const Product8Args& a, int row_dtype, int out_dtype, hipStream_t st, int epilogue = EPI_ROWS);
+
+// The same for a few rows per expert (csrc/few_rows_8bit.hip)
+struct Few8Args {
+  const void* X; int64_t sxm;                                     // float rows, columns contiguous, or rows in 8 bits (whole blocks) with XS
+  const uint8_t* XS; int x_vec;                                   // x_vec: float rows start at multiples of 16 bytes
+  const uint8_t* W; int64_t swe;                                  // (E, N, K rounded up to 16)
+  const void* WS; int64_t sse, ssn, ssk; int ws_f32;
+  const void* b; int64_t sbe, sbn;
+  void* Y; int64_t sym; int out_dtype;                            // EPI_UNIT: the unit's values, float32
+  const int64_t* ids;                                             // (L) expert of every slot, L <= 64: rows are slots; or NULL:
+  const int64_t* idx; const int64_t* off;                         // rows sorted by expert
+  int L, K, N, E, fan, x_grouped, y_grouped, act;
+};
+int launch_few_rows_8bit(const Few8Args& a, int x_dtype, int dtype, int epilogue, hipStream_t st);      // x_dtype -1: 8 bits
+int launch_few_combine(const float* rows, const void* gates, const int64_t* ids, void* out, int T, int k, int d, int E, int dtype, hipStream_t st);
+__device__ __forceinline__ float bias_value(const void* b, int64_t at, int dtype) {
+  if (dtype == SMOE_BF16) return to_f32(((const bf16_t*)b)[at]);
+  if (dtype == SMOE_F16) return to_f32(((const f16_t*)b)[at]);
+  return ((const float*)b)[at];
+}
 
 }  // namespace smoe

@@ -80,7 +80,7 @@ def _weight(what, name, q, s, device, E, N, K, t=None):
             raise RuntimeError("%s: all tensors on the device of the rows (%s)" % (what, device))
 
     def rows(u):
-        return u if u is None or (u.stride(2) == 1 and (u.stride(0) | u.stride(1) | u.data_ptr()) % 16 == 0) else u.clone(memory_format=torch.contiguous_format)
+        return u if u is None or (u.is_contiguous() and u.data_ptr() % 16 == 0) else u.clone(memory_format=torch.contiguous_format)
 
     return rows(q), s, rows(t)
 
@@ -174,7 +174,7 @@ class _GluMLP8bit(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gates, w1, s1, w1t, b1, w2, s2, w2t, b2, idx, off, act):
         need_x, need_g = ctx.needs_input_grad[:2]
-        out, rows, p8, ps = ops.glu_mlp_8bit(x, gates.to(x.dtype), w1, s1, b1, w2, s2, b2, idx, off, act, keep=need_x)
+        out, rows, p8, ps = ops.glu_mlp_8bit(x, gates.to(x.dtype), w1, s1, b1, w2, s2, b2, order=(idx, off), act=act, keep=need_x)
         ctx.save_for_backward(gates, rows if need_g else None, w1t, s1, w2t, s2, p8, ps, idx, off)
         ctx.act = act
         return out
@@ -216,9 +216,17 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
         raise RuntimeError("%s: all tensors on the device of the rows (%s)" % (what, x.device))
     if x.requires_grad and torch.is_grad_enabled() and (w1_t is None or w2_t is None):
         raise ValueError("%s: the gradient of x needs w1_t and w2_t, the transposed weights" % what)
-    _, idx, off = flatten_sort_count(expert_idxs, num_experts=E)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    out = _GluMLP8bit.apply(x.reshape(T, d), expert_p, w1, s1, w1_t, b1, w2, s2, w2_t, b2, idx, off, act)
+    tokens = x.reshape(T, d)
+    trained = ((x.requires_grad or expert_p.requires_grad) and torch.is_grad_enabled()) or ops.has_tangents(x, expert_p, b1, b2)
+    if not trained and T * k <= ops.FEW_ROWS_8BIT:
+        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=ops._as_i64(expert_idxs).contiguous(), act=act)[0]
+        return out.view(x.shape)
+    _, idx, off = flatten_sort_count(expert_idxs, num_experts=E)
+    if trained:
+        out = _GluMLP8bit.apply(tokens, expert_p, w1, s1, w1_t, b1, w2, s2, w2_t, b2, idx, off, act)
+    else:
+        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, order=(idx, off), act=act)[0]
     return out.view(x.shape)
 
 

@@ -28,6 +28,11 @@ def _routed_layer_bytes(T, k, d, F):
 
 
 @functools.lru_cache(maxsize=1024)
+def _layer_8bit_bytes(T, k, d, F, E, ordered, keep):
+    return _C.load().smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, keep)
+
+
+@functools.lru_cache(maxsize=1024)
 def _adapter_bytes(T, K, N, r, R, backward, code):
     return _C.load().smoe_adapter_workspace_bytes(T, K, N, r, R, backward, code)
 
@@ -48,7 +53,7 @@ def _whole_rows(x):
 
 def _weight_8bit(q, s):
     """smoe_weight_8bit of a weight (E, N, K) and its scales."""
-    return _C.Weight8bit(q.data_ptr(), q.stride(0), q.stride(1), s.data_ptr(), s.stride(0), s.stride(1), s.stride(2),
+    return _C.Weight8bit(q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), s.stride(1), s.stride(2),
                          int(s.dtype == torch.float32))
 
 
@@ -446,16 +451,16 @@ class HipBackend:
         _C.check(rc, "smoe_linear_8bit")
 
     @staticmethod
-    def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act):
+    def glu_mlp_8bit(x, gates, experts, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act):
         _C.require_gpu(x, "glu_mlp_8bit")
         lib = _C.load()
         T, k, d, F, E = x.size(0), gates.size(1), x.size(1), w1.size(1) // 2, w1.size(0)
         sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
         sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
-        need = lib.smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E)
+        need = _layer_8bit_bytes(T, k, d, F, E, int(idx is not None), int(P8 is not None))
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         with _C.on_device(x.device):
-            rc = lib.smoe_glu_mlp_8bit(_C.ptr(x), x.stride(0), _C.ptr(gates), _weight_8bit(w1, s1), _C.ptr(b1), *sb1, _weight_8bit(w2, s2),
+            rc = lib.smoe_glu_mlp_8bit(_C.ptr(x), x.stride(0), _C.ptr(gates), _C.ptr(experts), _weight_8bit(w1, s1), _C.ptr(b1), *sb1, _weight_8bit(w2, s2),
                                        _C.ptr(b2), *sb2, _C.ptr(rows), _C.ptr(out), _C.ptr(P8), _C.ptr(PS), _C.ptr(idx), _C.ptr(off), T, k, d,
                                        F, E, act, _C.float_code(x.dtype), _C.ptr(ws), need, _C.stream_ptr(x.device))
         _C.check(rc, "smoe_glu_mlp_8bit")
@@ -637,10 +642,11 @@ def _linear_8bit_op(X: torch.Tensor, coeff: Optional[torch.Tensor], W: torch.Ten
 
 
 @torch.library.custom_op("scattermoe::glu_mlp_8bit", mutates_args={"rows", "out", "P8", "PS"})
-def _glu_mlp_8bit_op(x: torch.Tensor, gates: torch.Tensor, w1: torch.Tensor, s1: torch.Tensor, b1: Optional[torch.Tensor],
-                     w2: torch.Tensor, s2: torch.Tensor, b2: Optional[torch.Tensor], rows: torch.Tensor, out: torch.Tensor,
-                     P8: Optional[torch.Tensor], PS: Optional[torch.Tensor], idx: torch.Tensor, off: torch.Tensor, act: int) -> None:
-    _backend.glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act)
+def _glu_mlp_8bit_op(x: torch.Tensor, gates: torch.Tensor, experts: Optional[torch.Tensor], w1: torch.Tensor, s1: torch.Tensor,
+                     b1: Optional[torch.Tensor], w2: torch.Tensor, s2: torch.Tensor, b2: Optional[torch.Tensor],
+                     rows: Optional[torch.Tensor], out: torch.Tensor, P8: Optional[torch.Tensor], PS: Optional[torch.Tensor],
+                     idx: Optional[torch.Tensor], off: Optional[torch.Tensor], act: int) -> None:
+    _backend.glu_mlp_8bit(x, gates, experts, w1, s1, b1, w2, s2, b2, rows, out, P8, PS, idx, off, act)
 
 
 @torch.library.custom_op("scattermoe::glu_mlp_8bit_bwd", mutates_args={"drows", "dx"})
@@ -1336,16 +1342,24 @@ def linear_8bit(x, w, s, idx, off, k, b=None, coeff=None, transposed=False, x_gr
     return y
 
 
-def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, idx, off, act=ACT_SILU, keep=False):
-    """(out (T, d), rows (T k, d) by slot, p8, ps): a gated layer on weights in 8 bits; `keep`: the halves of its pre-activation."""
+FEW_ROWS_8BIT = 64          # SMOE_8BIT_FEW_ROWS: a layer's forward goes by the ids, without an order of its rows
+
+
+def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, experts=None, order=None, act=ACT_SILU, keep=False):
+    """(out (T, d), rows (T k, d) by slot or None, p8, ps): a gated layer on weights in 8 bits, from the experts (T, k) int64 for at most
+    FEW_ROWS_8BIT rows, or from their order (idx, off); `keep`: the halves of its pre-activation."""
     x = _rows_contiguous(x)
-    T, d, L, F = x.size(0), x.size(1), idx.numel(), w1.size(1) // 2
+    T, d, L, F = x.size(0), x.size(1), gates.numel(), w1.size(1) // 2
     out = torch.empty((T, d), dtype=x.dtype, device=x.device)
-    rows = torch.empty((L, d), dtype=x.dtype, device=x.device)
-    p8 = torch.empty((L, 2, row_8bit(F)), dtype=TYPE_8BIT, device=x.device) if keep else None
-    ps = torch.empty((L, 2, blocks_8bit(F)), dtype=SCALE_8BIT, device=x.device) if keep else None
-    if out.numel():
-        _launch("glu_mlp_8bit", x, gates.contiguous(), w1, s1, b1, w2, s2, b2, rows, out, p8, ps, idx, off, act)
+    rows = p8 = ps = idx = off = None
+    if order is not None:
+        idx, off = order
+        rows = torch.empty((L, d), dtype=x.dtype, device=x.device)
+    if keep:
+        p8 = torch.empty((L, 2, row_8bit(F)), dtype=TYPE_8BIT, device=x.device)
+        ps = torch.empty((L, 2, blocks_8bit(F)), dtype=SCALE_8BIT, device=x.device)
+    if T:
+        _launch("glu_mlp_8bit", x, gates.contiguous(), experts, w1, s1, b1, w2, s2, b2, rows, out, p8, ps, idx, off, act)
     return out, rows, p8, ps
 
 
