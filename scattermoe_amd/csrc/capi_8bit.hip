@@ -70,7 +70,7 @@ static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64
   return a;
 }
 // Streams over the weights instead of tiles
-static bool few_rows_pay(int64_t L, int E) { return L <= 16 * (int64_t)E; }
+static bool few_rows_pay(int64_t L, int E) { return L <= 8 * (int64_t)E; }
 
 }  // namespace smoe
 

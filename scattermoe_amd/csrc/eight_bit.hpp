@@ -54,15 +54,32 @@ __device__ __forceinline__ float max16(float v) {
 }
 
 // 32 values of e4m3 as bfloat16, which holds every one of them: eight of each of four matrix instructions' operands
-typedef __bf16 bf16x2_8b __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_8b __attribute__((ext_vector_type(8)));
+typedef int i32x4_8b __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void to_bf16x32(i32x8 q, bf16x8_8b (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bf16x2_8b lo = __builtin_bit_cast(bf16x2_8b, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], 1.0f, false));
-    const bf16x2_8b hi = __builtin_bit_cast(bf16x2_8b, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], 1.0f, true));
-    v[i >> 1][(i & 1) * 4 + 0] = lo[0], v[i >> 1][(i & 1) * 4 + 1] = lo[1];
-    v[i >> 1][(i & 1) * 4 + 2] = hi[0], v[i >> 1][(i & 1) * 4 + 3] = hi[1];
+  for (int u = 0; u < 4; ++u) {
+    i32x4_8b r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * u + i], 1.0f, false));
+      r[2 * i + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * u + i], 1.0f, true));
+    }
+    v[u] = __builtin_bit_cast(bf16x8_8b, r);
+  }
+}
+
+// 16 values times their scale, a power of two, which bfloat16 holds as well (values under 2^-126 may lose bits)
+__device__ __forceinline__ void to_bf16x16(i32x4_8b q, float scale, bf16x8_8b (&v)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    i32x4_8b r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * u + i], scale, false));
+      r[2 * i + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * u + i], scale, true));
+    }
+    v[u] = __builtin_bit_cast(bf16x8_8b, r);
   }
 }
 

@@ -1,11 +1,13 @@
 // scatter2scatter on 8-bit weights for a few rows per expert: a stream over the weights.
 //
-// A workgroup has CF groups of 16 output columns and up to 16 MF rows of one expert; its eight waves share the contraction, each a run of
-// slices of 128, and add their sums up through LDS, in the order of the waves.  A wave's fragments go from memory to registers, two
-// slices of them on their way (16 KB per wave at CF = 4), since nobody else reads them.  Products are of bfloat16, which holds e4m3 exactly,
-// with both scales on every slice's sums (Scaling8): the matrix cores have time for it, a slice's 2 KB of weights take about 900 cycles
-// to come from memory and 64 MF + 64 to multiply.
-// Rows come as they are (float32, bfloat16, float16) and are taken to 8 bits on the way, a block's largest of four lanes, or from
+// Products are of bfloat16, which holds e4m3 times a power of two exactly (Scaling8): the matrix cores have time for it.  Scales of
+// float32 multiply every slice's sums.
+// 16 weight rows in an instruction would take 64 bytes each per load, half a line.  Instead its 16 rows are 8 rows in two parts of a
+// slice of 128: a load takes whole lines of 8 weight rows, rows and weights alike, and of the 16 x 16 sums those count whose parts
+// agree (few_rows.hpp).  A workgroup has GROUPS groups of 8 columns and 8 MF rows of one expert; its waves share the
+// contraction, each a run of slices, two of them on their way from memory to registers, and add their sums up through LDS, in
+// the order of the waves.
+// Rows come as they are (float32, bfloat16, float16) and are taken to 8 bits on the way, a block's largest of eight lanes, or from
 // a workspace where there are so many that each column group would do it again.
 #include "eight_bit.hpp"
 
@@ -13,34 +15,22 @@ namespace smoe {
 
 typedef int w_i32x4 __attribute__((ext_vector_type(4)));
 typedef float w_f32x4 __attribute__((ext_vector_type(4)));
-static constexpr int FEW_NW = 8, FEW_NT = FEW_NW * 64;
+static constexpr int FEW_NW = 4, FEW_NT = FEW_NW * 64, GROUPS = 8;
 
-// What lane l has of a row's slice: its 16 values from 16 (l / 16) on, and the 16 that are 64 further
-template <typename T>
-__device__ __forceinline__ void load_values(const T* __restrict__ row, int k0, int K, bool vec, float (&v)[32]) {
-  const int g = (lane_id() >> 4) << 4;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = k0 + h * 64 + g;
-    if (vec && c + 16 <= K) {
-      constexpr int PER = 16 / (int)sizeof(T);
-      T t[16];
-#pragma unroll
-      for (int p = 0; p < 16 / PER; ++p) __builtin_memcpy(t + p * PER, (const char*)__builtin_assume_aligned((const char*)(row + c) + p * 16, 16), 16);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[h * 16 + i] = to_f32(t[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[h * 16 + i] = c + i < K ? to_f32(row[c + i]) : 0.0f;
-    }
-  }
+// `bytes` of memory from one address for the wave on, with 32-bit offsets; behind them is nothing (zeros).  Plain pointers would have two
+// registers per offset.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t from_here(const void* p, int64_t bytes) {
+  const uint64_t v = (uint64_t)p;
+  const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+  const int range = __builtin_amdgcn_readfirstlane(bytes < 0xffffffffLL ? (int)(unsigned)bytes : -1);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, range, 0x00020000);
 }
 
-template <typename TX, int MF, int CF, int EPI>
+template <typename TX, int MF, int EPI, bool SF>
 __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, int dtype, int per) {
   constexpr bool FROM_8BIT = sizeof(TX) == 1;
-  constexpr int ROWS = 16 * MF;
-  __shared__ __attribute__((aligned(16))) w_f32x4 sums[FEW_NW][MF * CF][64];
+  constexpr int ROWS = 8 * MF;
+  __shared__ __attribute__((aligned(16))) w_f32x4 sums[FEW_NW][MF * GROUPS][64];
   __shared__ int s_src[64], s_dst[64];
   const int t = threadIdx.x, l = lane_id(), wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // ---- whose rows
@@ -75,138 +65,179 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
   __syncthreads();
   // ---- this wave's weight rows and scales
   const int F = a.N / 2;
-  constexpr int HALF = EPI == EPI_UNIT ? CF / 2 : CF;              // groups of neighbouring columns
-  const int n0 = blockIdx.x * (HALF * 16);
-  const int64_t Kp = padded_row(a.K);
-  const char* W = (const char*)a.W + e * a.swe;
-  const char* wrow[CF];
-  const char* wscale[CF];
-  const int WSB = a.ws_f32 ? 4 : 1;
+  constexpr int HALF = EPI == EPI_UNIT ? GROUPS / 2 : GROUPS;      // groups of neighbouring columns
+  const int n0 = blockIdx.x * (HALF * 8);
+  const int Kp = (int)padded_row(a.K);
+  constexpr int WSB = SF ? 4 : 1;                                  // bytes of a scale (a type of its own: a branch at each of their loads
+                                                                   // would order the loads around it)
+  // 32-bit offsets from the first row of either half (the launcher checks)
+  e = __builtin_amdgcn_readfirstlane(e);
+  const char* We = (const char*)a.W + e * a.swe;
+  const int64_t n1 = n0 + (EPI == EPI_UNIT ? F : 0);
+  const __amdgpu_buffer_rsrc_t W[2] = {from_here(We + (int64_t)n0 * Kp, (a.N - n0) * (int64_t)Kp), from_here(We + n1 * Kp, (a.N - n1) * Kp)};
+  const __amdgpu_buffer_rsrc_t WS = from_here((const char*)a.WS + e * a.sse * WSB, 0xffffffffLL);
+  const int sub = (l & 15) >> 1, at = (l & 1) * 64 + (l >> 4) * 16;  // row of a group, and this lane's 16 values of a slice
+  unsigned woff[HALF], soff[GROUPS];
 #pragma unroll
-  for (int j = 0; j < CF; ++j) {
-    int n = min(n0 + (j % HALF) * 16 + (l & 15), (EPI == EPI_UNIT ? F : a.N) - 1);
-    if (EPI == EPI_UNIT && j >= HALF) n += F;
-    wrow[j] = W + n * Kp;
-    wscale[j] = (const char*)a.WS + (e * a.sse + n / QB * a.ssn) * WSB;
+  for (int j = 0; j < GROUPS; ++j) {
+    const int n = min(n0 + (j % HALF) * 8 + sub, (EPI == EPI_UNIT ? F : a.N) - 1);
+    if (j < HALF) woff[j] = (unsigned)(n - n0) * (unsigned)Kp + at;
+    soff[j] = (unsigned)((n + (j >= HALF ? F : 0)) / QB * a.ssn) * WSB;
   }
   const int nk = (int)scale_blocks(a.K), first = wave * per, last = min(first + per, nk);
-  const int g16 = (l >> 4) << 4;
-  // a slice's fragment: 16 bytes and those 64 further; pieces behind the row's end are the row's first, and zeros
-  auto load_cols = [&](int kt, int j, i32x8& f) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = kt * QB + h * 64 + g16;
-      const bool there = c < Kp;
-      const w_i32x4 v = __builtin_nontemporal_load((const w_i32x4*)(wrow[j] + (there ? c : 0)));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[h * 4 + i] = there ? v[i] : 0;
-    }
-  };
   auto scale_at = [&](int kt, int j) {
-    const char* p = wscale[j] + kt * a.ssk * WSB;
-    return a.ws_f32 ? *(const float*)p : scale_of(*(const uint8_t*)p);
+    const int o = (int)(kt * a.ssk) * WSB;
+    if constexpr (SF) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(WS, (int)soff[j], o, 0));
+    else return scale_of((int)__builtin_amdgcn_raw_buffer_load_b8(WS, (int)soff[j], o, 0));
   };
   for (int base = 0; base < rows; base += ROWS) {                  // (by ids, an expert may have more rows than ROWS)
     const int here = min(ROWS, rows - base);
-    w_f32x4 acc[MF][CF];
+    w_f32x4 acc[MF][GROUPS];
 #pragma unroll
     for (int i = 0; i < MF; ++i)
 #pragma unroll
-      for (int j = 0; j < CF; ++j) acc[i][j] = w_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < GROUPS; ++j) acc[i][j] = w_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const TX* xrow[MF];
     const uint8_t* xs[MF];
-    bool have[MF];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-      const int m = i * 16 + (l & 15);
-      have[i] = m < here;
-      const int64_t src = s_src[base + (have[i] ? m : 0)];
-      xrow[i] = (const TX*)a.X + src * a.sxm;
+      const int m = i * 8 + sub;
+      const int64_t src = s_src[base + (m < here ? m : 0)];          // (what a lane without a row multiplies is not looked at)
+      xrow[i] = (const TX*)a.X + src * a.sxm + at;
       xs[i] = FROM_8BIT ? a.XS + src * scale_row(a.K) : nullptr;
     }
-    const bool vec = a.x_vec != 0;
-    i32x8 w[2][CF];
-    float ws[2][CF];
-    auto fetch = [&](int kt, int p) {
+    // rows of a slice: 8 bits and their scale (the dword of four slices), or values on their way to that
+    constexpr int XV = FROM_8BIT ? 4 : 4 * (int)sizeof(TX);
+    typedef int XRegs __attribute__((ext_vector_type(XV)));
+    w_i32x4 w[2][GROUPS];
+    float ws[2][GROUPS];
+    XRegs xv[2][MF];
+    int xb[2][MF];
+    // slices that go two at a time: all of rows in 8 bits, which are whole slices long, whole ones of aligned float rows
+    const int whole = FROM_8BIT ? max(first, last) : a.x_vec ? max(first, min(last, a.K / QB)) : first;
+    auto fetch = [&](int slice, int p) {
+      const int kt = min(slice, whole - 1);
 #pragma unroll
-      for (int j = 0; j < CF; ++j) load_cols(kt, j, w[p][j]);
+      for (int j = 0; j < GROUPS; ++j) {
+        w[p][j] = __builtin_bit_cast(w_i32x4, __builtin_amdgcn_raw_buffer_load_b128(W[j / HALF], (int)woff[j % HALF], kt * QB, 0));
+      }
 #pragma unroll
-      for (int j = 0; j < CF; ++j) ws[p][j] = scale_at(kt, j);
-    };
-    auto multiply = [&](int kt, int p) {
-      bf16x8_8b x[MF][4];
-      float fx[MF];
+      for (int j = 0; j < GROUPS; ++j) {
+        ws[p][j] = scale_at(kt, j);
+      }
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        i32x8 q = {0, 0, 0, 0, 0, 0, 0, 0};
-        fx[i] = 0.0f;
-        if constexpr (FROM_8BIT) {
-          // (the workspace's rows are whole slices long)
-          if (have[i]) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const w_i32x4 v = *(const w_i32x4*)(xrow[i] + kt * QB + h * 64 + g16);
+        for (int u = 0; u < XV / 4; ++u) {
+          const w_i32x4 v = *(const w_i32x4*)((const char*)(xrow[i] + kt * QB) + u * 16);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) q[h * 4 + c] = v[c];
-            }
-            fx[i] = scale_of(xs[i][kt]);
-          }
-        } else {
-          float v[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = 0.0f;
-          if (have[i]) load_values<TX>(xrow[i], kt * QB, a.K, vec, v);
-          float top = 0.0f;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) top = fmaxf(top, fabsf(v[c]));
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const int byte = scale_byte(top);
-          const float inv = inverse_scale(byte);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) q[c] = to_e4m3x4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3], inv);
-          fx[i] = scale_of(byte);
+          for (int c = 0; c < 4; ++c) xv[p][i][u * 4 + c] = v[c];
         }
-        to_bf16x32(q, x[i]);
+        if constexpr (FROM_8BIT) xb[p][i] = *(const int*)(xs[i] + (kt & ~3));
       }
+    };
+    auto fetch_some = [&](int kt) {                                // a slice that ends before its 128th value, or of other rows
 #pragma unroll
-      for (int j = 0; j < CF; ++j) {
-        bf16x8_8b wv[4];
-        to_bf16x32(w[p][j], wv);
+      for (int j = 0; j < GROUPS; ++j) {
+        w[0][j] = __builtin_bit_cast(w_i32x4, __builtin_amdgcn_raw_buffer_load_b128(W[j / HALF], (int)woff[j % HALF], kt * QB, 0));
+        ws[0][j] = scale_at(kt, j);
+      }
+      if constexpr (!FROM_8BIT) {
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
-          w_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+          TX v[16];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][u], wv[u], s, 0, 0, 0);
-          // (rows down the lanes' four values, columns across them: a column's scale is the lane's own)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(s[c] * ws[p][j], __shfl(fx[i], 4 * (l >> 4) + c), acc[i][j][c]);
+          for (int c = 0; c < 16; ++c) v[c] = kt * QB + at + c < a.K ? xrow[i][kt * QB + c] : from_f32<TX>(0.0f);
+          __builtin_memcpy(&xv[0][i], v, sizeof(v));
         }
       }
     };
-    if (first < last) fetch(first, 0);
-    for (int kt = first; kt < last; kt += 2) {
-      if (kt + 1 < last) fetch(kt + 1, 1);
-      multiply(kt, 0);
-      if (kt + 2 < last) fetch(kt + 2, 0);
-      if (kt + 1 < last) multiply(kt + 1, 1);
+    auto multiply = [&](int slice, int p, int end) {
+      bf16x8_8b x[MF][2];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        w_i32x4 q;
+        int byte;
+        if constexpr (FROM_8BIT) {
+          q = xv[p][i];
+          byte = (xb[p][i] >> (8 * (min(slice, last - 1) & 3))) & 255;
+        } else {
+          TX v[16];
+          __builtin_memcpy(v, &xv[p][i], sizeof(v));
+          float top = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) top = fmaxf(top, fabsf(to_f32(v[c])));
+          top = fmaxf(top, __shfl_xor(top, 1));
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          byte = scale_byte(top);
+          const float inv = inverse_scale(byte);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) q[c] = to_e4m3x4(to_f32(v[4 * c]), to_f32(v[4 * c + 1]), to_f32(v[4 * c + 2]), to_f32(v[4 * c + 3]), inv);
+        }
+        to_bf16x16(q, scale_of(byte), x[i]);
+      }
+      // (behind a row's end is the next one's, which may be no number; behind the last slice, that one again)
+      const bool there = slice < end && slice * QB + at < Kp;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        bf16x8_8b wv[2];
+        w_i32x4 q = w[p][j];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) q[c] = there ? q[c] : 0;
+        to_bf16x16(q, SF ? 1.0f : ws[p][j], wv);
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+          w_f32x4 s = SF ? w_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][j];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][u], wv[u], s, 0, 0, 0);
+          // (columns across the lanes: a column's scale is the lane's own)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[i][j][c] = SF ? fmaf(s[c], ws[p][j], acc[i][j][c]) : s[c];
+        }
+        if (j & 1) __builtin_amdgcn_sched_barrier(0);              // (all groups' conversions at once take too many registers)
+      }
+    };
+    // (pairs of slices; one behind the last is the last again, its weights zeros: no branches, whose joins cost registers)
+    if (first < whole) {
+      fetch(first, 0);
+      fetch(first + 1, 1);
+#pragma nounroll
+      for (int kt = first; kt < whole; kt += 2) {
+        multiply(kt, 0, whole);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(kt + 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(kt + 1, 1, whole);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(kt + 3, 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    for (int kt = whole; kt < last; ++kt) {
+      fetch_some(kt);
+      multiply(kt, 0, last);
     }
 #pragma unroll
     for (int i = 0; i < MF; ++i)
 #pragma unroll
-      for (int j = 0; j < CF; ++j) sums[wave][i * CF + j][l] = acc[i][j];
+      for (int j = 0; j < GROUPS; ++j) sums[wave][i * GROUPS + j][l] = acc[i][j];
     __syncthreads();
-    // ---- the waves' sums, one value per thread and step: row 16 i + 4 (lane / 16) + c, column 16 j + lane % 16
-    constexpr int VALUES = ROWS * HALF * 16;
+    // ---- the waves' sums, one value per thread and step: row r of a fragment in part p is instruction row 2 r + p, columns alike
+    constexpr int VALUES = ROWS * HALF * 8;
     for (int v = t; v < VALUES; v += FEW_NT) {
-      const int m = v / (HALF * 16), n = v % (HALF * 16), i = m >> 4, j = n >> 4;
-      const int lane = ((m >> 2) & 3) * 16 + (n & 15), c = m & 3;
+      const int m = v / (HALF * 8), n = v % (HALF * 8), i = m >> 3, j = n >> 3;
       const int col = n0 + n;
       if (m >= here || col >= (EPI == EPI_UNIT ? F : a.N)) continue;
       auto total = [&](int jj) {
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < FEW_NW; ++k) s += ((const float*)&sums[k][i * CF + jj][lane])[c];
+        for (int k = 0; k < FEW_NW; ++k)
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const int row = 2 * (m & 7) + part;
+            s += ((const float*)&sums[k][i * GROUPS + jj][(row >> 2) * 16 + 2 * (n & 7) + part])[row & 3];
+          }
         return s;
       };
       auto biased = [&](float s, int at) { return a.b ? s + bias_value(a.b, e * a.sbe + at * a.sbn, dtype) : s; };
@@ -247,25 +278,26 @@ int launch_few_combine(const float* rows, const void* gates, const int64_t* ids,
   return launch_status("few_combine");
 }
 
-template <typename TX, int MF, int CF, int EPI>
+template <typename TX, int MF, int EPI>
 static int launch_few(const Few8Args& a, int dtype, hipStream_t st) {
-  const int cols = EPI == EPI_UNIT ? a.N / 2 : a.N, group = (EPI == EPI_UNIT ? CF / 2 : CF) * 16;
-  const int64_t segments = a.ids ? (a.L < a.E ? a.L : a.E) : max_tiles(a.L, a.E, 16 * MF);
+  const int cols = EPI == EPI_UNIT ? a.N / 2 : a.N, group = (EPI == EPI_UNIT ? GROUPS / 2 : GROUPS) * 8;
+  const int64_t segments = a.ids ? (a.L < a.E ? a.L : a.E) : max_tiles(a.L, a.E, 8 * MF);
   const int per = (int)((scale_blocks(a.K) + FEW_NW - 1) / FEW_NW);
   if (segments > 65535) { set_error("few_rows_8bit: too many rows"); return SMOE_ERR_RANGE; }
-  few_rows_8bit_kernel<TX, MF, CF, EPI><<<dim3((cols + group - 1) / group, (unsigned)segments), FEW_NT, 0, st>>>(a, dtype, per);
+  const dim3 grid((cols + group - 1) / group, (unsigned)segments);
+  if (a.ws_f32) few_rows_8bit_kernel<TX, MF, EPI, true><<<grid, FEW_NT, 0, st>>>(a, dtype, per);
+  else few_rows_8bit_kernel<TX, MF, EPI, false><<<grid, FEW_NT, 0, st>>>(a, dtype, per);
   return launch_status("few_rows_8bit");
 }
 template <typename TX, int MF>
 static int launch_few(const Few8Args& a, int dtype, int epilogue, hipStream_t st) {
-  if (epilogue == EPI_UNIT) return launch_few<TX, MF, 4, EPI_UNIT>(a, dtype, st);
-  return launch_few<TX, MF, 4, EPI_ROWS>(a, dtype, st);
+  return epilogue == EPI_UNIT ? launch_few<TX, MF, EPI_UNIT>(a, dtype, st) : launch_few<TX, MF, EPI_ROWS>(a, dtype, st);
 }
 int launch_few_rows_8bit(const Few8Args& a, int x_dtype, int dtype, int epilogue, hipStream_t st) {
   if (x_dtype == SMOE_BF16) return launch_few<bf16_t, 1>(a, dtype, epilogue, st);
   if (x_dtype == SMOE_F16) return launch_few<f16_t, 1>(a, dtype, epilogue, st);
   if (x_dtype == SMOE_F32) return launch_few<float, 1>(a, dtype, epilogue, st);
-  return launch_few<uint8_t, 1>(a, dtype, epilogue, st);
+  return a.L <= 4 * (int64_t)a.E ? launch_few<uint8_t, 1>(a, dtype, epilogue, st) : launch_few<uint8_t, 2>(a, dtype, epilogue, st);
 }
 
 }  // namespace smoe

@@ -76,14 +76,15 @@ struct Cols8 {
 // The rows in 8 bits are whole slices long here (zeros behind the last value); sx: this thread's (t < 128) dwords of its row's scales;
 // s_scale: [2][128] dwords of LDS, four slices each.  What is loaded ahead behind the last slice is not looked at.
 template <int SC>
-__device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, char* lds,
-                                              unsigned* s_scale, Block (&acc)[Tile8::FM][Tile8::FN]) {
+__device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, int rows_in,
+                                              char* lds, unsigned* s_scale, Block (&acc)[Tile8::FM][Tile8::FN]) {
   typedef Tile8 TL;
   typedef typename WeightScales<SC>::V V;
   constexpr int COLS = 2 * TL::FN, LOADS = Rows8::R + Cols8::R, PER_STEP = LOADS / 3;
   static_assert(LOADS % 3 == 0, "the loads of the next slice go with three quarters of a slice's products");
   const int l = lane_id(), t = threadIdx.x, wave = t >> 6;
   const int nk = (K + 127) / 128;
+  const int steps = __builtin_amdgcn_readfirstlane((rows_in + 31) / 32);   // blocks of 32 rows that there are: an expert's last tile is lower
   const unsigned lds_u = lds_address(lds);
   unsigned fetched = 0;
   V ws[2];
@@ -141,6 +142,7 @@ __device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, co
         else A.issue_one(na, (kt + 1) * 64, q - Cols8::R);
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (s > 0 && s >= steps) continue;
       if (s + 1 < TL::FM) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) rows(s + 1, i);
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
   for (int i = 0; i < TL::FM; ++i)
 #pragma unroll
     for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
-  mainloop_8bit<SC>(A, B, W, sx, a.K, lds, s_scale, acc);
+  mainloop_8bit<SC>(A, B, W, sx, a.K, rows, lds, s_scale, acc);
   __syncthreads();
   const int wave = t >> 6, l = lane_id();
   if (EPI != EPI_UNIT_GRAD && a.b) {
