@@ -452,10 +452,10 @@ typedef struct {
 /*
  * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, summed in float32 and rounded once to `dtype`; rows as for
  * smoe_scatter2scatter.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
- * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, fan_out, x_grouped,
- * coeff != NULL) bytes, 256-byte aligned; nothing in it is read before it is written; calls that overlap in time need one each.
+ * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out,
+ * x_grouped, coeff != NULL, dtype) bytes, 256-byte aligned; nothing in it is read before it is written; calls that overlap in time need one each.
  */
-size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int fan_out, int x_grouped, int scaled);
+size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, int fan_out, int x_grouped, int scaled, int dtype);
 int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_weight_8bit* W, int transposed, const void* b, int64_t sbe,
                      int64_t sbn, void* Y, int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E,
                      int fan_out, int x_grouped, int y_grouped, int dtype, void* workspace, size_t workspace_bytes, void* stream);
@@ -471,12 +471,12 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
  * the scales of the weights; DROWS (T k, d): what every slot adds to DX (T,d).  Workspaces as above.
  */
 #define SMOE_8BIT_FEW_ROWS 64
-size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep);
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep, int dtype);
 int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64_t* experts, const smoe_weight_8bit* W1, const void* b1,
                       int64_t sb1e, int64_t sb1n, const smoe_weight_8bit* W2, const void* b2, int64_t sb2e, int64_t sb2n, void* Y, void* OUT,
                       void* P8, void* PS, const int64_t* idx, const int64_t* off, int64_t T, int k, int64_t d, int64_t F, int E, int act,
                       int dtype, void* workspace, size_t workspace_bytes, void* stream);
-size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E);
+size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int dtype);
 int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, const smoe_weight_8bit* W1T, const smoe_weight_8bit* W2T,
                           const void* P8, const void* PS, void* DROWS, void* DX, const int64_t* idx, const int64_t* off, int64_t T, int k,
                           int64_t d, int64_t F, int E, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);

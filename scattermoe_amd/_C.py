@@ -86,13 +86,13 @@ _SIGNATURES = {
     "smoe_dequantize_8bit": (_int, [_p, _i64, _i64, _p, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _p, _int, _p]),
     "smoe_glu_8bit_fwd": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _int, _int, _p]),
     "smoe_glu_8bit_bwd": (_int, [_p, _p, _p, _i64, _p, _p, _i64, _i64, _int, _int, _p]),
-    "smoe_linear_8bit_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int]),
+    "smoe_linear_8bit_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int, _int, _int, _int]),
     "smoe_linear_8bit": (_int, [_p, _i64, _p, _w8, _int, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _int, _int, _int, _int, _int,
                                 _p, _sz, _p]),
-    "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int, _int, _int]),
+    "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int, _int, _int, _int]),
     "smoe_glu_mlp_8bit": (_int, [_p, _i64, _p, _p, _w8, _p, _i64, _i64, _w8, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64,
                                  _int, _int, _int, _p, _sz, _p]),
-    "smoe_glu_mlp_8bit_bwd_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int]),
+    "smoe_glu_mlp_8bit_bwd_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int, _int]),
     "smoe_glu_mlp_8bit_bwd": (_int, [_p, _i64, _p, _w8, _w8, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64, _int, _int, _int, _p, _sz, _p]),
 }
 

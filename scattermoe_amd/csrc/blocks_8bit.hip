@@ -54,8 +54,8 @@ __device__ __forceinline__ float top8(const float (&v)[8]) {
 // the lane's eight values of a block in 8 bits (rows end at Kp, a multiple of 16), and its scale
 __device__ __forceinline__ void store_block(uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t c, int64_t Kp, const float (&v)[8]) {
   const int byte = scale_byte(top8(v));
-  const float inv = inverse_scale(byte);
-  if (c < Kp) *(i32x2*)(q + c) = i32x2{to_e4m3x4(v[0], v[1], v[2], v[3], inv), to_e4m3x4(v[4], v[5], v[6], v[7], inv)};
+  const float scale = scale_of(byte);
+  if (c < Kp) *(i32x2*)(q + c) = i32x2{to_e4m3x4(v[0], v[1], v[2], v[3], scale), to_e4m3x4(v[4], v[5], v[6], v[7], scale)};
   if ((threadIdx.x & 15) == 0) *s = (uint8_t)byte;
 }
 __device__ __forceinline__ void load_block(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s, int64_t c, int64_t Kp, float (&v)[8]) {
@@ -63,8 +63,8 @@ __device__ __forceinline__ void load_block(const uint8_t* __restrict__ q, const 
   if (c < Kp) {
     const i32x2 p = *(const i32x2*)(q + c);
     const float f = scale_of(*s);
-    from_e4m3x4(p[0], f, lo);
-    from_e4m3x4(p[1], f, hi);
+    from_e4m3x4_exact(p[0], f, lo);
+    from_e4m3x4_exact(p[1], f, hi);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
@@ -158,13 +158,13 @@ __global__ __launch_bounds__(256) void quantize_weights_kernel(QuantWeightsArgs 
   if ((t & 63) == 0) tops[t >> 6] = top;
   __syncthreads();
   const int byte = scale_byte(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-  const float inv = inverse_scale(byte);
+  const float scale = scale_of(byte);
   if (t == 0) a.S[b] = (uint8_t)byte;
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const int r = p * 16 + (t >> 4);
     const int64_t n = (int64_t)nblk * QB + r;
-    const i32x2 q = {to_e4m3x4(v[p][0], v[p][1], v[p][2], v[p][3], inv), to_e4m3x4(v[p][4], v[p][5], v[p][6], v[p][7], inv)};
+    const i32x2 q = {to_e4m3x4(v[p][0], v[p][1], v[p][2], v[p][3], scale), to_e4m3x4(v[p][4], v[p][5], v[p][6], v[p][7], scale)};
     if (n < a.N && c < Kp) *(i32x2*)(a.Q + ((int64_t)e * a.N + n) * Kp + c) = q;
     if (a.QT) {
 #pragma unroll

@@ -25,6 +25,7 @@ struct Carver {
 static bool gathers(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
   return !x_grouped && !scaled && L / fan * block_row(K) < (1LL << 32);
 }
+static float* take_partial(Carver& c, int64_t floats) { return floats ? c.take<float>(floats * 4) : nullptr; }
 struct Rows8Bit { uint8_t* q; uint8_t* s; int64_t rows; };
 static Rows8Bit take_rows(Carver& c, int64_t rows, int64_t K) {
   Rows8Bit r{nullptr, nullptr, rows};
@@ -159,10 +160,11 @@ static int workspace_check(const char* who, size_t need, const void* workspace, 
   return SMOE_ERR_WORKSPACE;
 }
 
-size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int fan_out, int x_grouped, int scaled) {
-  if (L <= 0 || K <= 0 || fan_out <= 0) return 0;
+size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, int fan_out, int x_grouped, int scaled, int dtype) {
+  if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
   take_rows(c, gathers(L, K, fan_out, x_grouped, scaled != 0) ? L / fan_out : L, K);
+  if (!few_rows_pay(L, E)) c.take(product_8bit_floats(L, K, N, E, dtype) * 4);
   return c.used;
 }
 
@@ -175,7 +177,7 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   if (!X || !Y || !idx || !off) { set_error("smoe_linear_8bit: NULL pointer"); return SMOE_ERR_NULL; }
   if (coeff && x_grouped) { set_error("smoe_linear_8bit: rows that are scaled come by token"); return SMOE_ERR_SHAPE; }
   if (int rc = weight_checks("smoe_linear_8bit", W)) return rc;
-  if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, fan_out, x_grouped, coeff != nullptr), workspace, workspace_bytes)) return rc;
+  if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out, x_grouped, coeff != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
   const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
   const Rows8Bit x = take_rows(c, by_token ? L / fan_out : L, K);
@@ -187,8 +189,9 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
     a.X = x.q, a.sxm = block_row(K), a.XS = x.s;
     return launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, (hipStream_t)stream);
   }
-  return launch_product_8bit(product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan_out, !by_token, y_grouped), dtype, dtype,
-                             (hipStream_t)stream);
+  Product8Args a = product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan_out, !by_token, y_grouped);
+  a.partial = take_partial(c, product_8bit_floats(L, K, N, E, dtype));
+  return launch_product_8bit(a, dtype, dtype, (hipStream_t)stream);
 }
 
 // How a layer goes.  Without an order of its rows: by their ids, two streams over the weights of the experts that they name.  Few rows per
@@ -200,8 +203,8 @@ static LayerWay layer_way(int64_t L, int64_t d, int64_t F, int E, bool ordered, 
   return unit_rides(d, F) ? LAYER_TILES_UNIT : LAYER_TILES;
 }
 // the pieces of a gated layer's workspace
-struct LayerPieces { Rows8Bit x, h; float* pre; float* hidden; float* rows; };
-static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64_t d, int64_t F) {
+struct LayerPieces { Rows8Bit x, h; float* pre; float* hidden; float* rows; float* partial1; float* partial2; };
+static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64_t d, int64_t F, int E, int dtype) {
   LayerPieces p{};
   if (way == LAYER_BY_IDS) {
     p.hidden = c.take<float>(L * F * 4);
@@ -212,12 +215,17 @@ static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64
   p.h = take_rows(c, L, F);
   if (way == LAYER_FEW) p.hidden = c.take<float>(L * F * 4);
   if (way == LAYER_TILES) p.pre = c.take<float>(L * 2 * F * 4);
+  if (way != LAYER_FEW) {                                          // (one after the other: the same piece for both products)
+    const int64_t one = product_8bit_floats(L, d, 2 * F, E, dtype), two = product_8bit_floats(L, F, d, E, dtype);
+    float* both = take_partial(c, one > two ? one : two);
+    p.partial1 = one ? both : nullptr, p.partial2 = two ? both : nullptr;
+  }
   return p;
 }
-size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep) {
+size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep, int dtype) {
   if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
   Carver c{nullptr};
-  layer_pieces(c, layer_way(T * k, d, F, E, ordered != 0, keep != 0), T * k, k, d, F);
+  layer_pieces(c, layer_way(T * k, d, F, E, ordered != 0, keep != 0), T * k, k, d, F, E, dtype);
   return c.used;
 }
 
@@ -238,9 +246,9 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   if (!X || !gates || !OUT || (P8 && !PS) || (ordered ? !Y || !off : !experts)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
   if (int rc = weight_checks("smoe_glu_mlp_8bit", W1)) return rc;
   if (int rc = weight_checks("smoe_glu_mlp_8bit", W2)) return rc;
-  if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, P8 != nullptr), workspace, workspace_bytes)) return rc;
+  if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, P8 != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
-  const LayerPieces p = layer_pieces(c, way, L, k, d, F);
+  const LayerPieces p = layer_pieces(c, way, L, k, d, F, E, dtype);
   if (way == LAYER_BY_IDS) {
     Few8Args a = few(W1, b1, sb1e, sb1n, p.hidden, F, SMOE_F32, experts, nullptr, nullptr, L, d, 2 * F, E, k, 0, 1, act);
     a.X = X, a.sxm = sxm, a.x_vec = ((uintptr_t)X & 15) == 0 && sxm * (dtype == SMOE_F32 ? 4 : 2) % 16 == 0;
@@ -263,6 +271,7 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
     return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
   }
   Product8Args a = product(p.x, W1, false, b1, sb1e, sb1n, p.pre, 2 * F, idx, off, L, d, 2 * F, E, k, !by_token, 1);
+  a.partial = p.partial1;
   if (way == LAYER_TILES_UNIT) {
     a.H8 = p.h.q, a.HS = p.h.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
     if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st, EPI_UNIT)) return rc;
@@ -271,22 +280,27 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
     UnitArgs u{p.pre, 2 * F, nullptr, p.h.q, p.h.s, (uint8_t*)P8, (uint8_t*)PS, L, F, act};
     if (int rc = launch_unit_fwd(u, SMOE_F32, st)) return rc;
   }
-  if (int rc = launch_product_8bit(product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
+  a = product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0);
+  a.partial = p.partial2;
+  if (int rc = launch_product_8bit(a, dtype, dtype, st)) return rc;
   return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
 }
 
-struct BackPieces { Rows8Bit dy, dp; float* dh; };
-static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F) {
+struct BackPieces { Rows8Bit dy, dp; float* dh; float* partial1; float* partial2; };
+static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F, int E, int dtype) {
   BackPieces p{};
   p.dy = take_rows(c, L, d);
   p.dp = take_rows(c, L, 2 * F);
   p.dh = unit_grad_rides(F) ? nullptr : c.take<float>(L * F * 4);
+  const int64_t one = product_8bit_floats(L, d, F, E, dtype), two = product_8bit_floats(L, 2 * F, d, E, dtype);
+  float* both = take_partial(c, one > two ? one : two);
+  p.partial1 = one ? both : nullptr, p.partial2 = two ? both : nullptr;
   return p;
 }
-size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E) {
+size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int dtype) {
   if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
   Carver c{nullptr};
-  back_pieces(c, T * k, d, F);
+  back_pieces(c, T * k, d, F, E, dtype);
   return c.used;
 }
 
@@ -302,12 +316,13 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   if (!DOUT || !gates || !P8 || !PS || !DROWS || !DX || !idx || !off) { set_error("smoe_glu_mlp_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
   if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T)) return rc;
   if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T)) return rc;
-  if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E), workspace, workspace_bytes)) return rc;
+  if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E, dtype), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
   Carver c{(char*)workspace};
-  const BackPieces p = back_pieces(c, L, d, F);
+  const BackPieces p = back_pieces(c, L, d, F, E, dtype);
   if (int rc = quantize(p.dy, DOUT, sdm, idx, k, gates, d, dtype, st)) return rc;
   Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, 1, 1);
+  a.partial = p.partial1;
   if (!p.dh) {
     a.H8 = p.dp.q, a.HS = p.dp.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
     if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st, EPI_UNIT_GRAD)) return rc;
@@ -316,7 +331,9 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
     UnitBackArgs u{(const uint8_t*)P8, (const uint8_t*)PS, p.dh, F, nullptr, p.dp.q, p.dp.s, nullptr, L, F, act};
     if (int rc = launch_unit_bwd(u, SMOE_F32, st)) return rc;
   }
-  if (int rc = launch_product_8bit(product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0), dtype, dtype, st)) return rc;
+  a = product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0);
+  a.partial = p.partial2;
+  if (int rc = launch_product_8bit(a, dtype, dtype, st)) return rc;
   return launch_combine(DROWS, d, nullptr, 0, 0, DX, d, T, k, (int)d, dtype, st);
 }
 

@@ -29,13 +29,18 @@ __device__ __forceinline__ int scale_byte(float top) {
   return max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
 }
 __device__ __forceinline__ float scale_of(int byte) { return __builtin_bit_cast(float, byte << 23); }
-__device__ __forceinline__ float inverse_scale(int byte) { return __builtin_bit_cast(float, (254 - byte) << 23); }
 
-// four values divided by their scale, to the nearest of e4m3 (ties to even); the conversion takes what is above 448 to NaN, and
-// nothing finite is
-__device__ __forceinline__ int to_e4m3x4(float a, float b, float c, float d, float inv) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-  return __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, r, true);
+// four values divided by their scale, a power of two, to the nearest of e4m3 (ties to even); the conversion takes what is above
+// 448 to NaN, and nothing finite is
+__device__ __forceinline__ int to_e4m3x4(float a, float b, float c, float d, float scale) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, a, b, scale, false);
+  return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true));
+}
+// times a scale that is a power of two
+__device__ __forceinline__ void from_e4m3x4_exact(int q, float s, float (&v)[4]) {
+  const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, s, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, s, true);
+  v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
 }
 __device__ __forceinline__ void from_e4m3x4(int q, float s, float (&v)[4]) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
@@ -157,7 +162,10 @@ struct Product8Args {
   //   the gated unit's gradient, the product being dh (F = N), from P8, PS: H8, HS, blocks along all 2F columns
   uint8_t* H8 = nullptr; uint8_t* HS = nullptr; uint8_t* P8 = nullptr; uint8_t* PS = nullptr;
   int act = 0;
+  float* partial = nullptr;                                        // product_8bit_floats() of them, or NULL
 };
+// floats with which a product can cut the contraction of the tiles of its last round (0: it would not)
+int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, int row_dtype);
 // whether a product can be followed by the unit, or by its gradient, within its tiles
 bool unit_rides(int64_t d, int64_t F);
 bool unit_grad_rides(int64_t F);

@@ -171,9 +171,9 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
           top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32));
           byte = scale_byte(top);
-          const float inv = inverse_scale(byte);
+          const float scale = scale_of(byte);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) q[c] = to_e4m3x4(to_f32(v[4 * c]), to_f32(v[4 * c + 1]), to_f32(v[4 * c + 2]), to_f32(v[4 * c + 3]), inv);
+          for (int c = 0; c < 4; ++c) q[c] = to_e4m3x4(to_f32(v[4 * c]), to_f32(v[4 * c + 1]), to_f32(v[4 * c + 2]), to_f32(v[4 * c + 3]), scale);
         }
         to_bf16x16(q, scale_of(byte), x[i]);
       }

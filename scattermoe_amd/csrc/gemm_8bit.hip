@@ -15,7 +15,7 @@
 
 namespace smoe {
 
-typedef Tile<128, 256, 1, 4, 2, false, 2, true> Tile8;
+typedef Tile<128, 256, 1, 4, 2, false, 3, true> Tile8;               // (3: epilogues derive nothing from the thread's index ahead of the loop)
 typedef DirectOp<Tile8::BM, Tile8::NT> Rows8;
 typedef DirectOp<Tile8::BN, Tile8::NT> Stage8;
 static constexpr int LDS8_B = 2 * Rows8::LDS_BYTES, LDS8 = LDS8_B + Stage8::LDS_BYTES;
@@ -76,15 +76,14 @@ struct Cols8 {
 // The rows in 8 bits are whole slices long here (zeros behind the last value); sx: this thread's (t < 128) dwords of its row's scales;
 // s_scale: [2][128] dwords of LDS, four slices each.  What is loaded ahead behind the last slice is not looked at.
 template <int SC>
-__device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, int rows_in,
-                                              char* lds, unsigned* s_scale, Block (&acc)[Tile8::FM][Tile8::FN]) {
+__device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, char* lds,
+                                              unsigned* s_scale, Block (&acc)[Tile8::FM][Tile8::FN]) {
   typedef Tile8 TL;
   typedef typename WeightScales<SC>::V V;
   constexpr int COLS = 2 * TL::FN, LOADS = Rows8::R + Cols8::R, PER_STEP = LOADS / 3;
   static_assert(LOADS % 3 == 0, "the loads of the next slice go with three quarters of a slice's products");
   const int l = lane_id(), t = threadIdx.x, wave = t >> 6;
   const int nk = (K + 127) / 128;
-  const int steps = __builtin_amdgcn_readfirstlane((rows_in + 31) / 32);   // blocks of 32 rows that there are: an expert's last tile is lower
   const unsigned lds_u = lds_address(lds);
   unsigned fetched = 0;
   V ws[2];
@@ -142,7 +141,6 @@ __device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, co
         else A.issue_one(na, (kt + 1) * 64, q - Cols8::R);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (s > 0 && s >= steps) continue;
       if (s + 1 < TL::FM) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) rows(s + 1, i);
@@ -195,9 +193,10 @@ struct ByteTile {
   // ROWS rows to `out`, `ld` bytes apart, `rows` and `cols` (a multiple of 16) of them there
   template <int ROWS>
   static __device__ __forceinline__ void store(const char* lds, uint8_t* out, int64_t ld, int rows, int cols) {
+    const int t = late_thread<Tile8>();
 #pragma unroll
     for (int p = 0; p < ROWS * (WIDTH / 16) / Tile8::NT; ++p) {
-      const int piece = p * Tile8::NT + (int)threadIdx.x, r = piece / (WIDTH / 16), c = piece % (WIDTH / 16) * 16;
+      const int piece = p * Tile8::NT + t, r = piece / (WIDTH / 16), c = piece % (WIDTH / 16) * 16;
       const i32x4 v = *(const i32x4*)(lds + r * ROW + c);
       if (r < rows && c < cols) *(i32x4*)(out + r * ld + c) = v;
     }
@@ -205,103 +204,118 @@ struct ByteTile {
 };
 
 // The gated unit behind a product.  A tile holds 128 columns of the hidden rows, one block: a wave 32 of each half (accumulators [.][0],
-// [.][1]), so that a lane has both halves of its values, and a row's largest magnitude is that of four lanes and four waves.  Against
-// the product's float32 rows written, read and taken to 8 bits by a pass (4099 tokens, 4096 / 14336): see the launcher.
-__device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int row0, int rows, int n_tile, char* lds) {
+// [.][1]: the linear half and the gate's, by which rows of the weights the wave takes), so that a lane has both halves of its
+// values, and a row's largest magnitude is that of four lanes and four waves.  It is bound by its own arithmetic: with a choice of the
+// gate's half and of columns that are not there for each value, and the scale multiplied in before a conversion without one,
+// 4150 instructions instead of 2660, 1054 instead of 1015 us (4099 tokens, 8 experts, 4096 / 14336; 8192 tokens to 8 of 128
+// experts, 2048 / 768, with the checkpoint: 319, 303).  As a pass over the product's float32 rows: 1065 + 191 us (229 + 90).
+__device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int row0, int rows, int n_tile,
+                                              const float* s_bias, char* lds) {
   typedef Tile8 TL;
   typedef ByteTile<QB> Bytes;
-  const int t = threadIdx.x, wave = t >> 6, l = lane_id(), F = a.N / 2;
-  const bool mine = n_tile * QB + wave * 32 < F;                   // (F is a multiple of 32)
-  float* top = (float*)(lds + TL::BM * Bytes::ROW);               // [wave][row]
-  const int fb = (int)scale_blocks(F);
-  // one value per accumulator of half h (2: the unit's) to 8 bits, its rows to `out`
-  auto write = [&](auto value, uint8_t* out, int64_t ld, int cols, uint8_t* scales, int64_t sld) {
-    __syncthreads();
+  constexpr int PARTS = 2, ROWS = TL::BM / PARTS, FR = ROWS / 16, SIDE = ROWS * Bytes::ROW;
+  const int t = late_thread<TL>(), wave = t >> 6, l = t & 63, F = a.N / 2, fb = (int)scale_blocks(F);
+  const bool mine = n_tile * QB + wave * 32 < F;          // (F is a multiple of 32)
+  const int64_t ld = scale_blocks(F) * QB;                         // (hidden rows are whole slices long, zeros behind the last value)
+  const int swapped = a.act & 1;                                   // the gate's half is the first one
+  float* top = (float*)(lds + 3 * SIDE);                           // [the unit, its halves][wave][row]
 #pragma unroll
-    for (int i = 0; i < 2 * TL::FM; ++i) {
-      float m = 0.0f;
+  for (int part = 0; part < PARTS; ++part) {
+    float unit[FR][2][4];
+    if (part) __syncthreads();
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+    for (int i = 0; i < FR; ++i) {
+      const int ai = (part * FR + i) >> 1, aq = 2 * ((part * FR + i) & 1);
+      float m[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) m = fmaxf(m, fabsf(value(i, g, c)));
-      m = row_max(mine ? m : 0.0f);
-      if (l < 16) top[wave * TL::BM + i * 16 + l] = m;
-    }
-    __syncthreads();
+      for (int g = 0; g < 2; ++g) {
+        const float* b = s_bias + wave * TL::WTN + 16 * g + 4 * (l >> 4);
+        f32x4 &lin = acc[ai][0].q[aq + g], &gate = acc[ai][1].q[aq + g];
+        lin += *(const f32x4*)b, gate += *(const f32x4*)(b + 32);
 #pragma unroll
-    for (int i = 0; i < 2 * TL::FM; ++i) {
-      const int r = i * 16 + (l & 15);
-      const int byte = scale_byte(fmaxf(fmaxf(top[r], top[TL::BM + r]), fmaxf(top[2 * TL::BM + r], top[3 * TL::BM + r])));
-      const float inv = inverse_scale(byte);
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        Bytes::put(lds, r, wave * 32 + 16 * g + 4 * (l >> 4), to_e4m3x4(value(i, g, 0), value(i, g, 1), value(i, g, 2), value(i, g, 3), inv));
-      if (wave == 0 && l < 16 && r < rows) scales[r * sld] = (uint8_t)byte;
-    }
-    __syncthreads();
-    Bytes::template store<TL::BM>(lds, out, ld, rows, cols);
-  };
-  auto half = [&](int h) { return [&acc, h](int i, int g, int c) { return acc[i >> 1][h].q[2 * (i & 1) + g][c]; }; };
-  if (a.P8) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      write(half(h), a.P8 + ((int64_t)row0 * 2 + h) * F + n_tile * QB, 2 * F, min(QB, F - n_tile * QB), a.PS + ((int64_t)row0 * 2 + h) * fb + n_tile, 2 * fb);
-  }
-  const bool gate_first = (a.act & 1) != 0;
-#pragma unroll
-  for (int i = 0; i < 2 * TL::FM; ++i)
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float one = acc[i >> 1][0].q[2 * (i & 1) + g][c], two = acc[i >> 1][1].q[2 * (i & 1) + g][c];
-        acc[i >> 1][0].q[2 * (i & 1) + g][c] = gate_first ? glu_h(a.act, one, two) : glu_h(a.act, two, one);
+        for (int c = 0; c < 4; ++c) {
+          unit[i][g][c] = glu_h(a.act, gate[c], lin[c]);
+          m[0] = fmaxf(m[0], fabsf(unit[i][g][c])), m[1] = fmaxf(m[1], fabsf(lin[c])), m[2] = fmaxf(m[2], fabsf(gate[c]));
+        }
       }
-  // (hidden rows are whole slices long, zeros behind the last value)
-  const int64_t ld = scale_blocks(F) * QB;
-  if (!mine) {
 #pragma unroll
-    for (int i = 0; i < TL::FM; ++i) acc[i][0].clear();
+      for (int s = 0; s < 3; ++s) {
+        m[s] = row_max(mine ? m[s] : 0.0f);
+        if (l < 16) top[(s * 4 + wave) * ROWS + i * 16 + l] = m[s];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FR; ++i) {
+      const int ai = (part * FR + i) >> 1, aq = 2 * ((part * FR + i) & 1), r = i * 16 + (l & 15);
+      const int64_t row = row0 + part * ROWS + r;
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        if (s && !a.P8) break;
+        const float* most = top + s * 4 * ROWS + r;
+        const int byte = scale_byte(fmaxf(fmaxf(most[0], most[ROWS]), fmaxf(most[2 * ROWS], most[3 * ROWS])));
+        const float scale = scale_of(byte);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 &lin = acc[ai][0].q[aq + g], &gate = acc[ai][1].q[aq + g];
+          const int q = s == 0   ? to_e4m3x4(unit[i][g][0], unit[i][g][1], unit[i][g][2], unit[i][g][3], scale)
+                        : s == 1 ? to_e4m3x4(lin[0], lin[1], lin[2], lin[3], scale)
+                                 : to_e4m3x4(gate[0], gate[1], gate[2], gate[3], scale);
+          Bytes::put(lds + s * SIDE, r, wave * 32 + 16 * g + 4 * (l >> 4), mine ? q : 0);
+        }
+        if (wave == 0 && l < 16 && part * ROWS + r < rows) {
+          uint8_t* out = s == 0 ? a.HS + row * scale_row(F) : a.PS + (2 * row + ((s - 1) ^ swapped)) * fb;
+          out[n_tile] = (uint8_t)byte;
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t first = row0 + part * ROWS;
+    Bytes::template store<ROWS>(lds, a.H8 + first * ld + n_tile * QB, ld, rows - part * ROWS, QB);
+    if (a.P8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        Bytes::template store<ROWS>(lds + (1 + h) * SIDE, a.P8 + (first * 2 + (h ^ swapped)) * F + n_tile * QB, 2 * F, rows - part * ROWS, min(QB, F - n_tile * QB));
+    }
   }
-  write(half(0), a.H8 + (int64_t)row0 * ld + n_tile * QB, ld, QB, a.HS + (int64_t)row0 * scale_row(F) + n_tile, scale_row(F));
 }
 
 // The gated unit's gradient behind a product that is dh.  F is a multiple of 128, so that the blocks of both halves of d(pre) lie in a tile: 256
-// columns of dh, two blocks of each half.  32 rows at a time: their gradients of the first half take dh's registers, those of the second 32 more.
+// columns of dh, two blocks of each half.  32 rows at a time: the linear half's gradients take dh's registers, the gate's 32 more.
+// 8192 tokens to 8 of 128 experts, 2048 / 768: 222 us, as a pass over the product's float32 rows 229 + 112.
 __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int row0, int rows, int n0, char* lds) {
   typedef Tile8 TL;
   typedef ByteTile<TL::BN> Bytes;
   constexpr int PARTS = 4, ROWS = TL::BM / PARTS, FR = ROWS / 16;
-  const int t = threadIdx.x, wave = t >> 6, l = lane_id(), F = a.N;
+  const int t = late_thread<TL>(), wave = t >> 6, l = t & 63, F = a.N;
   float* top = (float*)(lds + 2 * ROWS * Bytes::ROW);             // [half][wave][row]
-  const bool gate_first = (a.act & 1) != 0;
+  const int swapped = a.act & 1, lin_at = swapped * F, gate_at = F - lin_at;            // the gate's half is the first one
   const bool mine = n0 + wave * TL::WTN < F;
   const int n = mine ? n0 + wave * TL::WTN : 0, fb = F / QB;
   const int64_t Ds = scale_row(2 * F);
 #pragma unroll
   for (int part = 0; part < PARTS; ++part) {
-    float second[FR][2 * TL::FN][4];
+    float dgate[FR][2 * TL::FN][4];
     if (part) __syncthreads();
 #pragma unroll
     for (int i = 0; i < FR; ++i) {
       const int r = part * ROWS + i * 16 + (l & 15), row = row0 + min(r, rows - 1);
       const uint8_t* p8 = a.P8 + (int64_t)row * 2 * F + n;
       const uint8_t* ps = a.PS + (int64_t)row * 2 * fb + n / QB;
-      const float s1 = scale_of(ps[0]), s2 = scale_of(ps[fb]);
+      const float s1 = scale_of(ps[swapped * fb]), s2 = scale_of(ps[(1 - swapped) * fb]);
       float m1 = 0.0f, m2 = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
-        float one[4], two[4];
-        from_e4m3x4(*(const int*)(p8 + j * 16 + 4 * (l >> 4)), s1, one);
-        from_e4m3x4(*(const int*)(p8 + F + j * 16 + 4 * (l >> 4)), s2, two);
+        float lin[4], gate[4];
+        from_e4m3x4_exact(*(const int*)(p8 + lin_at + j * 16 + 4 * (l >> 4)), s1, lin);
+        from_e4m3x4_exact(*(const int*)(p8 + gate_at + j * 16 + 4 * (l >> 4)), s2, gate);
         f32x4& d = acc[(part * FR + i) >> 1][j >> 1].q[2 * ((part * FR + i) & 1) + (j & 1)];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float dl, dg;
-          glu_grad(a.act, d[c], gate_first ? one[c] : two[c], gate_first ? two[c] : one[c], dl, dg);
-          d[c] = gate_first ? dg : dl;
-          second[i][j][c] = gate_first ? dl : dg;
-          m1 = fmaxf(m1, fabsf(d[c])), m2 = fmaxf(m2, fabsf(second[i][j][c]));
+          float dl;
+          glu_grad(a.act, d[c], gate[c], lin[c], dl, dgate[i][j][c]);
+          d[c] = dl;
+          m1 = fmaxf(m1, fabsf(d[c])), m2 = fmaxf(m2, fabsf(dgate[i][j][c]));
         }
       }
       m1 = row_max(m1), m2 = row_max(m2);
@@ -313,41 +327,215 @@ __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8
       const int r = i * 16 + (l & 15), pair = wave & 2;            // the two waves that share this one's blocks
       const int b1 = scale_byte(fmaxf(top[pair * ROWS + r], top[(pair + 1) * ROWS + r]));
       const int b2 = scale_byte(fmaxf(top[(4 + pair) * ROWS + r], top[(5 + pair) * ROWS + r]));
-      const float inv1 = inverse_scale(b1), inv2 = inverse_scale(b2);
+      const float f1 = scale_of(b1), f2 = scale_of(b2);
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
         const f32x4& d = acc[(part * FR + i) >> 1][j >> 1].q[2 * ((part * FR + i) & 1) + (j & 1)];
         const int col = wave * TL::WTN + j * 16 + 4 * (l >> 4);
-        Bytes::put(lds, r, col, to_e4m3x4(d[0], d[1], d[2], d[3], inv1));
-        Bytes::put(lds + ROWS * Bytes::ROW, r, col, to_e4m3x4(second[i][j][0], second[i][j][1], second[i][j][2], second[i][j][3], inv2));
+        Bytes::put(lds, r, col, to_e4m3x4(d[0], d[1], d[2], d[3], f1));
+        Bytes::put(lds + ROWS * Bytes::ROW, r, col, to_e4m3x4(dgate[i][j][0], dgate[i][j][1], dgate[i][j][2], dgate[i][j][3], f2));
       }
       if ((wave & 1) == 0 && l < 16 && part * ROWS + r < rows && mine) {
         uint8_t* s = a.HS + (int64_t)(row0 + part * ROWS + r) * Ds + n / QB;
-        s[0] = (uint8_t)b1, s[fb] = (uint8_t)b2;
+        s[swapped * fb] = (uint8_t)b1, s[(1 - swapped) * fb] = (uint8_t)b2;
       }
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      Bytes::template store<ROWS>(lds + h * ROWS * Bytes::ROW, a.H8 + (int64_t)(row0 + part * ROWS) * 2 * F + h * F + n0, 2 * F, rows - part * ROWS,
+      Bytes::template store<ROWS>(lds + h * ROWS * Bytes::ROW, a.H8 + (int64_t)(row0 + part * ROWS) * 2 * F + (h ? gate_at : lin_at) + n0, 2 * F, rows - part * ROWS,
                                   min(TL::BN, F - n0));      // (whole slices: 2 F is a multiple of them)
+  }
+}
+
+// ---- who takes what --------------------------------------------------------------------------------------
+// Tiles in one line: expert by expert, inside an expert bands of eight tile rows, inside a band column by column.  A round is what the card
+// runs side by side, two workgroups per CU; XCD x (a workgroup's index modulo 8) takes the x-th eighth of a round, 64 neighbours in
+// line, which share eight row panels and eight column panels in its L2.  A product of few rounds that ends in a round of at
+// most half the card's tiles cuts their contraction into parts, one workgroup each, which leave their sums in `partial`;
+// product_8bit_join_kernel adds the parts up in their order.  8 experts x 1025 rows on average, 14336 -> 4096, 2.3 rounds: 554 us,
+// in parts 461 + 16 for the sums.  At 4096 values to contract the parts save less than the sums cost (12 tile rows x 16 columns: 78 us, in parts 78 + 15).
+// Bands of 4 and 16 tile rows: 1.00 and 1.01 times the time.
+static constexpr int BAND8 = 8, PARTS8 = 8, PART_SLICES = 16, SPLIT_SLICES = 64, SPLIT_ROUNDS = 8;
+static constexpr int64_t TILE8_FLOATS = Tile8::BM * Tile8::BN;
+template <int SC> static constexpr int round_tiles = SC == SCALES_EXACT ? 256 : 512;
+struct Share8 {
+  int e, row0, rows, row, column;
+  int part, parts, slice0, slices;      // the contraction's part, of `parts`; its slices
+  int slot;                             // of this part's sums
+};
+// Share number b of a product (JOIN: tile number b of those whose contraction is cut).  The same answer in every wave.
+template <int ROUND, bool JOIN>
+__device__ __forceinline__ bool find_share(const Product8Args& a, int b, int n_tiles, Share8& s) {
+  constexpr int BM = Tile8::BM;
+  const int nk = (a.K + QB - 1) / QB;
+  const int total = count_tile_rows<BM>(a.off, a.E) * n_tiles;
+  int rest = 0;
+  s.part = 0, s.parts = 1, s.slice0 = 0, s.slices = nk, s.slot = 0;
+  if (a.partial) {
+    rest = total % ROUND;
+    int parts = rest ? min(min(ROUND / rest, PARTS8), nk / PART_SLICES) : 1;
+    if (parts < 2) {
+      rest = 0;
+    } else {
+      s.slices = ((nk + parts - 1) / parts + 3) & ~3;               // (four slices' scales are one dword)
+      s.parts = (nk + s.slices - 1) / s.slices;
+    }
+  }
+  const int whole = total - rest;                                  // tiles that are multiplied in one piece
+  int l;
+  if (JOIN) {
+    if (b >= rest) return false;
+    l = whole + b;
+    s.slot = b * s.parts;
+  } else {
+    const int first = b / ROUND * ROUND;                           // of this workgroup's round
+    const int x = b & 7, j = (b - first) >> 3;
+    if (first < whole) {
+      const int there = min(ROUND, whole - first), len = (there + 7) >> 3;
+      if (j >= len || x * len + j >= there) return false;
+      l = first + x * len + j;
+      s.parts = 1, s.slices = nk;
+    } else {
+      const int start = (whole + ROUND - 1) / ROUND * ROUND, there = rest * s.parts, len = (there + 7) >> 3;
+      if (first != start || j >= len || x * len + j >= there) return false;
+      const int u = x * len + j;
+      s.part = u / rest;
+      const int tile = u - s.part * rest;
+      l = whole + tile;
+      s.slot = tile * s.parts + s.part;
+      s.slice0 = s.part * s.slices;
+      s.slices = min(s.slices, nk - s.slice0);
+    }
+  }
+  int before = 0;                                                  // tile rows of the experts before this group of 64
+  for (int e0 = 0; e0 < a.E; e0 += 64) {
+    int lo, hi;
+    load_expert_rows(a.off, a.E, e0, lo, hi);
+    const int nt = (hi - lo + BM - 1) / BM, incl = wave_scan(nt), cum = before + incl;
+    const unsigned long long hit = __ballot((int64_t)cum * n_tiles > l);
+    if (hit) {
+      const int src = __ffsll((long long)hit) - 1;
+      const int lo_s = __builtin_amdgcn_readlane(lo, src), hi_s = __builtin_amdgcn_readlane(hi, src);
+      const int rows_e = __builtin_amdgcn_readlane(nt, src);
+      int in = l - (__builtin_amdgcn_readlane(cum, src) - rows_e) * n_tiles;
+      const int bands = max(1, (rows_e + BAND8 / 2 - 1) / BAND8), step = (rows_e + bands - 1) / bands;      // 1 to 12 tile rows each
+      const int band = in / (step * n_tiles), high = min(step, rows_e - band * step);
+      in -= band * (step * n_tiles);
+      const int column = in / high, row = band * step + in - column * high;
+      s.e = __builtin_amdgcn_readfirstlane(e0 + src);
+      s.column = __builtin_amdgcn_readfirstlane(column);
+      s.row = __builtin_amdgcn_readfirstlane(row);
+      s.row0 = lo_s + s.row * BM;
+      s.rows = min(BM, hi_s - s.row0);
+      s.part = __builtin_amdgcn_readfirstlane(s.part), s.parts = __builtin_amdgcn_readfirstlane(s.parts);
+      s.slice0 = __builtin_amdgcn_readfirstlane(s.slice0), s.slices = __builtin_amdgcn_readfirstlane(s.slices);
+      s.slot = __builtin_amdgcn_readfirstlane(s.slot);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+// A tile's sums, rounded, through LDS to its rows: 16-byte pieces, a wave whole 128-byte lines, or value by value where rows do not
+// start at multiples of 16 bytes.  Float32 goes in two halves of 128 columns, the 64 KB of a 16-bit tile.
+template <typename TO>
+__device__ __forceinline__ void store_rows(const Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int n0, const int64_t* s_dst,
+                                           const float* s_bias, char* lds) {
+  typedef Tile8 TL;
+  typedef TO T4 __attribute__((ext_vector_type(4)));
+  constexpr int PER = 16 / (int)sizeof(TO), HALVES = (int)sizeof(TO) / 2, COLS = TL::BN / HALVES, CPR = COLS / PER;      // 32 pieces a row
+  const int t = late_thread<TL>(), wave = t >> 6, l = t & 63;
+  TO* Y = (TO*)a.Y;
+  const bool whole = ((uintptr_t)Y & 15) == 0 && ((a.sym | a.N) & (PER - 1)) == 0;
+  auto place = [](int row, int col) { return row * (COLS * (int)sizeof(TO)) + (((col / PER) ^ (row & (CPR - 1))) << 4) + (col % PER) * (int)sizeof(TO); };
+#pragma unroll
+  for (int half = 0; half < HALVES; ++half) {
+    if (half) __syncthreads();
+    if (HALVES == 1 || (wave >> 1) == half) {
+#pragma unroll
+      for (int j = 0; j < 2 * TL::FN; ++j) {
+        const int tc = wave * TL::WTN + j * 16 + 4 * (l >> 4);
+        const f32x4 b = *(const f32x4*)(s_bias + tc);
+#pragma unroll
+        for (int i = 0; i < 2 * TL::FM; ++i) {
+          const f32x4& q = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
+          T4 v;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = from_f32<TO>(q[c] + b[c]);
+          *(T4*)(lds + place(i * 16 + (l & 15), tc % COLS)) = v;
+        }
+      }
+    }
+    __syncthreads();
+    constexpr int PIECES = TL::BM * CPR / TL::NT, GRP = 8;
+#pragma unroll
+    for (int g0 = 0; g0 < PIECES; g0 += GRP) {
+      i32x4 v[GRP];
+      int64_t d[GRP];
+#pragma unroll
+      for (int g = 0; g < GRP; ++g) {
+        const int p = (g0 + g) * TL::NT + t, r = p / CPR;
+        d[g] = s_dst[r];
+        v[g] = *(const i32x4*)(lds + place(r, p % CPR * PER));
+      }
+#pragma unroll
+      for (int g = 0; g < GRP; ++g) {
+        const int n = n0 + half * COLS + ((g0 + g) * TL::NT + t) % CPR * PER;
+        if (d[g] < 0 || n >= a.N) continue;
+        if (whole) {
+          stream_store(v[g], (i32x4*)(Y + d[g] + n));
+        } else {
+          TO e[PER];
+          __builtin_memcpy(e, &v[g], 16);
+#pragma unroll
+          for (int c = 0; c < PER; ++c)
+            if (n + c < a.N) Y[d[g] + n + c] = e[c];
+        }
+      }
+    }
+  }
+}
+
+// What follows a tile's sums: the bias, and the rows or the unit or its gradient
+template <typename TO, int EPI>
+__device__ __forceinline__ void finish(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int bias_dtype, int e, int row0, int rows, int n_tile,
+                                       const int64_t* s_dst, float* s_bias, char* lds) {
+  typedef Tile8 TL;
+  const int t = late_thread<TL>(), F = a.N / 2, n0 = n_tile * (EPI == EPI_UNIT ? QB : TL::BN);
+  if constexpr (EPI == EPI_UNIT_GRAD) {
+    epilogue_unit_grad(acc, a, row0, rows, n0, lds);
+  } else {
+    // the tile's 256 columns' biases through LDS, zeros without one
+    int n = n0 + t;
+    bool there = n < a.N;
+    if constexpr (EPI == EPI_UNIT) {
+      n = n0 + (t >> 6) * 32 + (t & 31);
+      there = n < F;
+      n += (t & 32 ? 1 - (a.act & 1) : a.act & 1) * F;
+    }
+    s_bias[t] = a.b && there ? bias_value(a.b, e * a.sbe + n * a.sbn, bias_dtype) : 0.0f;
+    __syncthreads();
+    if constexpr (EPI == EPI_UNIT) epilogue_unit(acc, a, row0, rows, n_tile, s_bias, lds);
+    else store_rows<TO>(acc, a, n0, s_dst, s_bias, lds);
   }
 }
 
 // (float32 rows: the operands as bfloat16 take the registers of a second workgroup)
 template <typename TO, int SC, int EPI>
-__global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product_8bit_kernel(Product8Args a, int bias_dtype, Raster rast) {
+__global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product_8bit_kernel(Product8Args a, int bias_dtype, int n_tiles) {
   typedef Tile8 TL;
   __shared__ __attribute__((aligned(16))) char lds[LDS8];
   __shared__ unsigned s_scale[2 * TL::BM];
   __shared__ int64_t s_dst[EPI == EPI_ROWS ? TL::BM : 1];
+  __shared__ __attribute__((aligned(16))) float s_bias[TL::BN];
   __shared__ int s_src[TL::BM];
-  int m_tile, n_tile, m_loc, n_loc, e, row0, rows;
-  if (!rast.map<2 * Raster::SN>(blockIdx.x, m_tile, n_tile, m_loc, n_loc)) return;
-  if (!find_tile<TL::BM>(a.off, a.E, m_tile, e, row0, rows)) return;
+  Share8 share;
+  if (!find_share<round_tiles<SC>, false>(a, blockIdx.x, n_tiles, share)) return;
+  const int e = share.e, row0 = share.row0, rows = share.rows, n_tile = share.column, k0 = share.slice0;
   const int t = threadIdx.x, F = a.N / 2;
-  // first output column of the tile, and of this wave's two halves of 32
-  const int n0 = n_tile * (EPI == EPI_UNIT ? QB : TL::BN);
+  const int n0 = n_tile * (EPI == EPI_UNIT ? QB : TL::BN);         // first output column of the tile (of either half)
   const uint8_t* sx = nullptr;
   if (t < TL::BM) {
     const int row = row0 + (t < rows ? t : rows - 1);                  // rows behind the last one repeat it
@@ -356,34 +544,35 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
     const int src = a.x_grouped ? row : (int)((unsigned)slot / (unsigned)a.fan);
     s_src[t] = src;
     if constexpr (EPI == EPI_ROWS) s_dst[t] = t < rows ? (int64_t)(a.y_grouped ? row : slot) * a.sym : -1;
-    sx = a.XS + src * scale_row(a.K);
+    sx = a.XS + src * scale_row(a.K) + k0;
   }
   __syncthreads();
   Rows8 A;
-  A.rot = (n_loc * Rows8::R / (2 * Raster::SN)) % Rows8::R;
+  A.rot = (n_tile % BAND8 * Rows8::R / BAND8) % Rows8::R;
   const int src0 = a.x_grouped ? row0 : 0;
   const int64_t ld = (a.K + QB - 1) / QB * QB;                         // the rows are whole slices long
-  A.init((const char*)a.X + src0 * ld, [&](int row) { return (int64_t)(s_src[row] - src0) * ld; });
+  A.init((const char*)a.X + src0 * ld + k0 * QB, [&](int row) { return (int64_t)(s_src[row] - src0) * ld; });
   Cols8 B;
-  const int turn = (m_loc * Cols8::R / Raster::SM) % Cols8::R;
+  const int turn = (share.row % BAND8 * Cols8::R / BAND8) % Cols8::R;
   const int64_t swn = a.swn;
   const int wave_u = (int)wave_uniform_id();
   int nb[2];
   if constexpr (EPI == EPI_UNIT) {
-    // tile column -> weight row: wave, first 32 of its 64 from the first half of the rows, the others from the second
-    B.init((const char*)a.W + e * a.swe, (int64_t)a.N * swn, turn,
-           [&](int tc) { return (int64_t)(min(n0 + (tc >> 6) * 32 + (tc & 31), F - 1) + (tc & 32 ? F : 0)) * swn; });
+    // tile column -> weight row: first 32 of a wave's 64 from the linear half of the rows, the others from the gate's
+    const int lin_at = (a.act & 1) * F, gate_at = F - lin_at;
+    B.init((const char*)a.W + e * a.swe + k0 * QB, (int64_t)a.N * swn - k0 * QB, turn,
+           [&](int tc) { return (int64_t)(min(n0 + (tc >> 6) * 32 + (tc & 31), F - 1) + (tc & 32 ? gate_at : lin_at)) * swn; });
     const int hc = min(n0 + wave_u * 32, F - 1);
-    nb[0] = hc / QB, nb[1] = (F + hc) / QB;
+    nb[0] = (lin_at + hc) / QB, nb[1] = (gate_at + hc) / QB;
   } else {
     const int last = a.N - 1 - n0;
-    B.init((const char*)a.W + e * a.swe + n0 * swn, (a.N - n0) * swn, turn, [&](int row) { return (int64_t)min(row, last) * swn; });
+    B.init((const char*)a.W + e * a.swe + n0 * swn + k0 * QB, (a.N - n0) * swn - k0 * QB, turn, [&](int row) { return (int64_t)min(row, last) * swn; });
     nb[0] = nb[1] = min(n0 + wave_u * TL::WTN, a.N - 1) / QB;
   }
   WeightScales<SC> W;
   const int WSB = SC == SCALES_BYTES ? 1 : SC == SCALES_FLOAT || a.ws_f32 ? 4 : 1;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) W.at[h] = (const char*)a.WS + (e * a.sse + nb[h] * a.ssn) * WSB;
+  for (int h = 0; h < 2; ++h) W.at[h] = (const char*)a.WS + (e * a.sse + nb[h] * a.ssn + k0 * a.ssk) * WSB;
   W.step = a.ssk * WSB;
   W.f32 = a.ws_f32 != 0;
   Block acc[TL::FM][TL::FN];
@@ -391,78 +580,80 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
   for (int i = 0; i < TL::FM; ++i)
 #pragma unroll
     for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
-  mainloop_8bit<SC>(A, B, W, sx, a.K, rows, lds, s_scale, acc);
+  mainloop_8bit<SC>(A, B, W, sx, min(a.K - k0 * QB, share.slices * QB), lds, s_scale, acc);
+  if (share.parts > 1) {
+    // this part's sums as they lie in the registers (scalar offsets: addresses in registers would have to be held beside them)
+    const __amdgpu_buffer_rsrc_t P =
+        __builtin_amdgcn_make_buffer_rsrc((void*)make_uniform((const char*)(a.partial + share.slot * TILE8_FLOATS)), 0, TILE8_FLOATS * 4, 0x00020000);
+    typedef unsigned u32x4_8b __attribute__((ext_vector_type(4)));
+    const int at = late_thread<TL>() * 16;
+#pragma unroll
+    for (int i = 0; i < TL::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::FN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_8b, acc[i][j].q[g]), P, at, ((i * TL::FN + j) * 4 + g) * TL::NT * 16, 0);
+    return;
+  }
   __syncthreads();
-  const int wave = t >> 6, l = lane_id();
-  if (EPI != EPI_UNIT_GRAD && a.b) {
-#pragma unroll
-    for (int j = 0; j < 2 * TL::FN; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        int n = n0 + wave * TL::WTN + j * 16 + 4 * (l >> 4) + c;
-        bool there = n < a.N;
-        if constexpr (EPI == EPI_UNIT) {
-          n = n0 + wave * 32 + (j & 1) * 16 + 4 * (l >> 4) + c;
-          there = n < F;
-          n += j >= 2 ? F : 0;
-        }
-        const float b = there ? bias_value(a.b, e * a.sbe + n * a.sbn, bias_dtype) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2 * TL::FM; ++i) acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)][c] += b;
-      }
-  }
-  if constexpr (EPI == EPI_UNIT) {
-    epilogue_unit(acc, a, row0, rows, n_tile, lds);
-    return;
-  } else if constexpr (EPI == EPI_UNIT_GRAD) {
-    epilogue_unit_grad(acc, a, row0, rows, n0, lds);
-    return;
-  } else {
-  TO* Y = (TO*)a.Y;
-  if constexpr (sizeof(TO) == 2) {
-    if (((uintptr_t)Y & 15) == 0 && ((a.sym | a.N) & 7) == 0) epilogue_staged<TO, TL>(acc, Y, s_dst, n0, a.N, nullptr, 0, lds);
-    else epilogue<TO, TL>(acc, Y, s_dst, n0, a.N, nullptr, 0);
-  } else {
-    // 16 rows of 64 bytes per wave and store: whole sectors as they lie in the registers
-    const bool whole = ((uintptr_t)Y & 15) == 0 && ((a.sym | a.N) & 3) == 0;
-    auto walk = [&](auto put) {
-#pragma unroll
-      for (int i = 0; i < 2 * TL::FM; ++i) {
-        const int64_t d = s_dst[i * 16 + (l & 15)];
-        if (d >= 0) {
-#pragma unroll
-          for (int j = 0; j < 2 * TL::FN; ++j) put(d, n0 + wave * TL::WTN + j * 16 + 4 * (l >> 4), acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    if (whole) {
-      walk([&](int64_t d, int n, const f32x4& v) {
-        if (n < a.N) *(f32x4*)(Y + d + n) = v;
-      });
-    } else {
-      walk([&](int64_t d, int n, const f32x4& v) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (n + c < a.N) Y[d + n + c] = v[c];
-      });
-    }
-  }
-  }
+  finish<TO, EPI>(acc, a, bias_dtype, e, row0, rows, n_tile, s_dst, s_bias, lds);
 }
 
+// The tiles whose contraction was cut: the parts' sums in their order, and what follows a product
+template <typename TO, int SC, int EPI>
+__global__ __launch_bounds__(Tile8::NT, 2) void product_8bit_join_kernel(Product8Args a, int bias_dtype, int n_tiles) {
+  typedef Tile8 TL;
+  __shared__ __attribute__((aligned(16))) char lds[LDS8];
+  __shared__ int64_t s_dst[EPI == EPI_ROWS ? TL::BM : 1];
+  __shared__ __attribute__((aligned(16))) float s_bias[TL::BN];
+  Share8 share;
+  if (!find_share<round_tiles<SC>, true>(a, blockIdx.x, n_tiles, share)) return;
+  const int t = threadIdx.x;
+  if (EPI == EPI_ROWS && t < TL::BM)
+    s_dst[t] = t < share.rows ? (a.y_grouped ? (int64_t)(share.row0 + t) : a.idx[share.row0 + t]) * a.sym : -1;
+  Block acc[TL::FM][TL::FN];
+#pragma unroll
+  for (int i = 0; i < TL::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
+  for (int p = 0; p < share.parts; ++p) {
+    const f32x4* P = (const f32x4*)(a.partial + (share.slot + p) * TILE8_FLOATS) + t;
+#pragma unroll
+    for (int i = 0; i < TL::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::FN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) acc[i][j].q[g] += P[((i * TL::FN + j) * 4 + g) * TL::NT];
+  }
+  __syncthreads();
+  finish<TO, EPI>(acc, a, bias_dtype, share.e, share.row0, share.rows, share.column, s_dst, s_bias, lds);
+}
+
+template <typename TO, int SC, int EPI>
+static int launch_product(const Product8Args& a, int bias_dtype, int n_tiles, hipStream_t st) {
+  constexpr int ROUND = round_tiles<SC>;
+  // every share of the most tiles that the rows can make, and a round of parts
+  const int64_t tiles = max_tiles(a.L, a.E, Tile8::BM) * n_tiles;
+  const int64_t grid = (tiles + ROUND - 1) / ROUND * ROUND + (a.partial ? ROUND : 0);
+  if (grid > 0x7fffff00LL) { set_error("product_8bit: grid too large"); return SMOE_ERR_RANGE; }
+  product_8bit_kernel<TO, SC, EPI><<<(unsigned)grid, Tile8::NT, 0, st>>>(a, bias_dtype, n_tiles);
+  if (a.partial) product_8bit_join_kernel<TO, SC, EPI><<<ROUND / 2, Tile8::NT, 0, st>>>(a, bias_dtype, n_tiles);
+  return launch_status("product_8bit");
+}
 template <typename TO, bool EXACT, int EPI>
 static int launch_product(const Product8Args& a, int bias_dtype, hipStream_t st) {
-  const int64_t m_tiles = max_tiles(a.L, a.E, Tile8::BM);
   const int n_tiles = EPI == EPI_UNIT ? (a.N / 2 + QB - 1) / QB : (a.N + Tile8::BN - 1) / Tile8::BN;
-  const Raster r = a.L < (int64_t)STRIPE_BELOW * a.E ? make_striped(m_tiles, n_tiles, GM_RING)
-                                                     : make_raster(m_tiles, n_tiles, GM_S2S, 2 * Raster::SN);
-  if (r.grid() > 0x7fffffffLL) { set_error("product_8bit: grid too large"); return SMOE_ERR_RANGE; }
-  const unsigned grid = (unsigned)r.grid();
-  if constexpr (EXACT) product_8bit_kernel<TO, SCALES_EXACT, EPI><<<grid, Tile8::NT, 0, st>>>(a, bias_dtype, r);
-  else if (a.ws_f32) product_8bit_kernel<TO, SCALES_FLOAT, EPI><<<grid, Tile8::NT, 0, st>>>(a, bias_dtype, r);
-  else product_8bit_kernel<TO, SCALES_BYTES, EPI><<<grid, Tile8::NT, 0, st>>>(a, bias_dtype, r);
-  return launch_status("product_8bit");
+  if constexpr (EXACT) return launch_product<TO, SCALES_EXACT, EPI>(a, bias_dtype, n_tiles, st);
+  else return a.ws_f32 ? launch_product<TO, SCALES_FLOAT, EPI>(a, bias_dtype, n_tiles, st) : launch_product<TO, SCALES_BYTES, EPI>(a, bias_dtype, n_tiles, st);
+}
+
+int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, int row_dtype) {
+  const int64_t round = row_dtype == SMOE_F32 ? round_tiles<SCALES_EXACT> : round_tiles<SCALES_BYTES>;
+  const int64_t tiles = max_tiles(L, E, Tile8::BM) * ((columns + Tile8::BN - 1) / Tile8::BN);
+  if ((K + QB - 1) / QB < SPLIT_SLICES || tiles > SPLIT_ROUNDS * round) return 0;
+  const int64_t slots = tiles * PARTS8 < round ? tiles * PARTS8 : round;
+  return slots * TILE8_FLOATS;
 }
 
 // The unit's blocks are 128 hidden columns, and a wave's 32 of either half have one scale of the weights; its weight rows are

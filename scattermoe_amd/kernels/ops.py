@@ -28,8 +28,8 @@ def _routed_layer_bytes(T, k, d, F):
 
 
 @functools.lru_cache(maxsize=1024)
-def _layer_8bit_bytes(T, k, d, F, E, ordered, keep):
-    return _C.load().smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, keep)
+def _layer_8bit_bytes(T, k, d, F, E, ordered, keep, code):
+    return _C.load().smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, keep, code)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -442,7 +442,7 @@ class HipBackend:
         lib = _C.load()
         L, K = idx.numel(), X.size(1)
         sb = (b.stride(0), b.stride(1)) if b is not None else (0, 0)
-        need = lib.smoe_linear_8bit_workspace_bytes(L, K, k, int(x_grouped), int(coeff is not None))
+        need = lib.smoe_linear_8bit_workspace_bytes(L, K, Y.size(1), W.size(0), k, int(x_grouped), int(coeff is not None), _C.float_code(X.dtype))
         ws = torch.empty(need, dtype=torch.uint8, device=X.device)
         with _C.on_device(X.device):
             rc = lib.smoe_linear_8bit(_C.ptr(X), X.stride(0), _C.ptr(coeff), _weight_8bit(W, S), int(transposed), _C.ptr(b), *sb, _C.ptr(Y),
@@ -457,7 +457,7 @@ class HipBackend:
         T, k, d, F, E = x.size(0), gates.size(1), x.size(1), w1.size(1) // 2, w1.size(0)
         sb1 = (b1.stride(0), b1.stride(1)) if b1 is not None else (0, 0)
         sb2 = (b2.stride(0), b2.stride(1)) if b2 is not None else (0, 0)
-        need = _layer_8bit_bytes(T, k, d, F, E, int(idx is not None), int(P8 is not None))
+        need = _layer_8bit_bytes(T, k, d, F, E, int(idx is not None), int(P8 is not None), _C.float_code(x.dtype))
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         with _C.on_device(x.device):
             rc = lib.smoe_glu_mlp_8bit(_C.ptr(x), x.stride(0), _C.ptr(gates), _C.ptr(experts), _weight_8bit(w1, s1), _C.ptr(b1), *sb1, _weight_8bit(w2, s2),
@@ -470,7 +470,7 @@ class HipBackend:
         _C.require_gpu(d_out, "glu_mlp_8bit backward")
         lib = _C.load()
         T, k, d, F, E = d_out.size(0), gates.size(1), d_out.size(1), w2t.size(1), w1t.size(0)
-        need = lib.smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E)
+        need = lib.smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E, _C.float_code(d_out.dtype))
         ws = torch.empty(need, dtype=torch.uint8, device=d_out.device)
         with _C.on_device(d_out.device):
             rc = lib.smoe_glu_mlp_8bit_bwd(_C.ptr(d_out), d_out.stride(0), _C.ptr(gates), _weight_8bit(w1t, s1), _weight_8bit(w2t, s2),

@@ -134,8 +134,8 @@ def test_c_entry_points_name_bad_calls():
     assert linear(x=zero) == -1 and linear(L=7) == -2 and linear(k=0) == -2 and linear(dtype=9) == -3
     assert linear(weight=bad) == -2 and b"16 bytes" in lib.smoe_last_error()
     assert linear(weight=none) == -1 and linear(coeff=one, grouped=1) == -2
-    need = lib.smoe_linear_8bit_workspace_bytes(8, 64, 2, 0, 0)
-    assert need == 1024 and lib.smoe_linear_8bit_workspace_bytes(8, 64, 2, 0, 1) == 1536
+    need = lib.smoe_linear_8bit_workspace_bytes(8, 64, 64, 2, 2, 0, 0, _C.BF16)
+    assert need == 1024 and lib.smoe_linear_8bit_workspace_bytes(8, 64, 64, 2, 2, 0, 1, _C.BF16) == 1536
     assert linear(size=need - 1) == -4 and linear(ws=zero) == -4 and linear(ws=ctypes.c_void_p(264)) == -4
     assert linear(L=1 << 32) == -5 and linear(L=0) == 0
 
@@ -143,10 +143,10 @@ def test_c_entry_points_name_bad_calls():
         return lib.smoe_glu_mlp_8bit(one, 64, one, one, w, zero, 0, 0, w, zero, 0, 0, one, one, p8, ps, idx, one, T, k, 64, 64, 2, act, _C.BF16, ws, size, None)
 
     assert layer(k=0) == -2 and layer(act=9) == -2 and layer(p8=one) == -1 and layer(idx=zero, T=33) == -1 and layer(T=1 << 32) == -5 and layer(T=0) == 0
-    assert layer(size=lib.smoe_glu_mlp_8bit_workspace_bytes(4, 2, 64, 64, 2, 1, 0) - 1) == -4
+    assert layer(size=lib.smoe_glu_mlp_8bit_workspace_bytes(4, 2, 64, 64, 2, 1, 0, _C.BF16) - 1) == -4
 
     def back(T=4, k=2, ws=one, size=1 << 24, p8=one):
         return lib.smoe_glu_mlp_8bit_bwd(one, 64, one, w, w, p8, one, one, one, one, one, T, k, 64, 32, 2, 0, _C.BF16, ws, size, None)
 
     assert back(k=0) == -2 and back(p8=zero) == -1 and back(T=0) == 0
-    assert back(size=lib.smoe_glu_mlp_8bit_bwd_workspace_bytes(4, 2, 64, 32, 2) - 1) == -4
+    assert back(size=lib.smoe_glu_mlp_8bit_bwd_workspace_bytes(4, 2, 64, 32, 2, _C.BF16) - 1) == -4
