@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a, unsigned
   if (u >= rows * pieces) return;
   const int64_t row = u / pieces, c = (u - row * pieces) * 16, e = row / a.N, n = row - e * a.N;
   const int64_t at = e * a.sse + n / a.tall * a.ssn + c / QB * a.ssk;
-  const float s = a.s_f32 ? ((const float*)a.S)[at] : scale_of(((const uint8_t*)a.S)[at]);
+  const float s = a.s_f32 ? ((const float*)a.S)[at] : weight_scale(((const uint8_t*)a.S)[at]);
   const uint8_t* q = a.Q + e * a.sqe + n * a.sqn + c;
   T* y = (T*)a.Y + row * a.K;
   if (c + 16 <= a.K && ((uintptr_t)q & 15) == 0) {

@@ -7,6 +7,7 @@ namespace smoe {
 static bool float_type(int d) { return d == SMOE_F32 || d == SMOE_BF16 || d == SMOE_F16; }
 static bool act_ok(int a) { return a == SMOE_ACT_SILU || a == SMOE_ACT_SILU_GATE_FIRST; }
 static constexpr int64_t MOST = 0x3fffffff;                        // columns
+static constexpr int64_t WIDEST = 1 << 21;                         // of a product: the rows of a tile are 32-bit offsets from its first
 
 // pieces of a workspace, each at a multiple of 256 bytes
 struct Carver {
@@ -39,9 +40,14 @@ static int quantize(const Rows8Bit& r, const void* X, int64_t sxm, const int64_t
   return launch_quantize_rows(a, dtype, st);
 }
 
-static int weight_checks(const char* who, const smoe_weight_8bit* w) {
+static int weight_checks(const char* who, const smoe_weight_8bit* w, int64_t rows, int64_t cols) {
   if (!w || !w->q || !w->s) { set_error("%s: NULL weight", who); return SMOE_ERR_NULL; }
   if (((uintptr_t)w->q | w->q_expert) & 15) { set_error("%s: an expert's weights start at multiples of 16 bytes", who); return SMOE_ERR_SHAPE; }
+  // (an expert's scales are 32-bit offsets from its first)
+  if (w->s_row < 0 || w->s_col < 0 || scale_blocks(rows) * w->s_row + scale_blocks(cols) * w->s_col > (1LL << 28)) {
+    set_error("%s: an expert's scales lie too far apart", who);
+    return SMOE_ERR_RANGE;
+  }
   return 0;
 }
 static Product8Args product(const Rows8Bit& x, const smoe_weight_8bit* w, bool transposed, const void* b, int64_t sbe, int64_t sbn, void* Y,
@@ -71,7 +77,7 @@ static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64
   return a;
 }
 // Streams over the weights instead of tiles
-static bool few_rows_pay(int64_t L, int E) { return L <= 8 * (int64_t)E; }
+static bool few_rows_pay(int64_t L, int E) { return L <= 8 * (int64_t)E && L <= 32768; }   // (a segment per expert or 8 rows: a grid's second side)
 
 }  // namespace smoe
 
@@ -151,7 +157,7 @@ int smoe_glu_8bit_bwd(const void* P8, const void* PS, const void* dh, int64_t sd
 static int product_checks(const char* who, int64_t L, int64_t K, int64_t N, int E, int fan, int dtype) {
   if (!float_type(dtype)) { set_error("%s: unknown dtype %d", who, dtype); return SMOE_ERR_DTYPE; }
   if (L < 0 || K <= 0 || N < 0 || E <= 0 || fan <= 0 || L % fan != 0) { set_error("%s: bad sizes", who); return SMOE_ERR_SHAPE; }
-  if (L > 0x7fffffffLL || K > MOST || N > MOST) { set_error("%s: size beyond int32", who); return SMOE_ERR_RANGE; }
+  if (L > 0x7fffffffLL || K > WIDEST || N > WIDEST) { set_error("%s: size beyond int32", who); return SMOE_ERR_RANGE; }
   return 0;
 }
 static int workspace_check(const char* who, size_t need, const void* workspace, size_t bytes) {
@@ -176,7 +182,7 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   if (L == 0 || N == 0) return 0;
   if (!X || !Y || !idx || !off) { set_error("smoe_linear_8bit: NULL pointer"); return SMOE_ERR_NULL; }
   if (coeff && x_grouped) { set_error("smoe_linear_8bit: rows that are scaled come by token"); return SMOE_ERR_SHAPE; }
-  if (int rc = weight_checks("smoe_linear_8bit", W)) return rc;
+  if (int rc = weight_checks("smoe_linear_8bit", W, transposed ? K : N, transposed ? N : K)) return rc;
   if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out, x_grouped, coeff != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
   const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
@@ -244,8 +250,8 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   const LayerWay way = layer_way(L, d, F, E, ordered, P8 != nullptr);
   if (!ordered && (L > SMOE_8BIT_FEW_ROWS || P8)) { set_error("smoe_glu_mlp_8bit: an order is needed for more than %d rows, and to keep P8", SMOE_8BIT_FEW_ROWS); return SMOE_ERR_NULL; }
   if (!X || !gates || !OUT || (P8 && !PS) || (ordered ? !Y || !off : !experts)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
-  if (int rc = weight_checks("smoe_glu_mlp_8bit", W1)) return rc;
-  if (int rc = weight_checks("smoe_glu_mlp_8bit", W2)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W1, 2 * F, d)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit", W2, d, F)) return rc;
   if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, P8 != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
   const LayerPieces p = layer_pieces(c, way, L, k, d, F, E, dtype);
@@ -310,12 +316,12 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   set_error("%s", "");
   hipStream_t st = (hipStream_t)stream;
   if (k <= 0 || F <= 0) { set_error("smoe_glu_mlp_8bit_bwd: bad sizes"); return SMOE_ERR_SHAPE; }
-  if (int rc = product_checks("smoe_glu_mlp_8bit_bwd", T * k, 2 * F, d, E, k, dtype)) return rc;
+  if (int rc = product_checks("smoe_glu_mlp_8bit_bwd", T * k, F, d, E, k, dtype)) return rc;
   if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit_bwd: unknown activation %d", act); return SMOE_ERR_SHAPE; }
   if (T == 0 || d == 0) return 0;
   if (!DOUT || !gates || !P8 || !PS || !DROWS || !DX || !idx || !off) { set_error("smoe_glu_mlp_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
-  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T)) return rc;
-  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T, 2 * F, d)) return rc;
+  if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T, d, F)) return rc;
   if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E, dtype), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
   Carver c{(char*)workspace};

@@ -29,6 +29,10 @@ __device__ __forceinline__ int scale_byte(float top) {
   return max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
 }
 __device__ __forceinline__ float scale_of(int byte) { return __builtin_bit_cast(float, byte << 23); }
+// of any byte of a weight's scale, its lowest (2^-127) and the one that is no number among them
+__device__ __forceinline__ float weight_scale(int byte) {
+  return __builtin_bit_cast(float, byte == 0 ? 0x400000 : byte == 255 ? 0x7fc00000 : byte << 23);
+}
 
 // four values divided by their scale, a power of two, to the nearest of e4m3 (ties to even); the conversion takes what is above
 // 448 to NaN, and nothing finite is

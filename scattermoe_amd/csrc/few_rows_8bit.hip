@@ -88,7 +88,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
   auto scale_at = [&](int kt, int j) {
     const int o = (int)(kt * a.ssk) * WSB;
     if constexpr (SF) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(WS, (int)soff[j], o, 0));
-    else return scale_of((int)__builtin_amdgcn_raw_buffer_load_b8(WS, (int)soff[j], o, 0));
+    else return weight_scale((int)__builtin_amdgcn_raw_buffer_load_b8(WS, (int)soff[j], o, 0));
   };
   for (int base = 0; base < rows; base += ROWS) {                  // (by ids, an expert may have more rows than ROWS)
     const int here = min(ROWS, rows - base);

@@ -44,7 +44,7 @@ struct WeightScales {
       const char* p = at[h] + kt * step;
       if constexpr (SC == SCALES_BYTES) v[h] = *(const uint8_t*)p;
       else if constexpr (SC == SCALES_FLOAT) v[h] = *(const float*)p;
-      else v[h] = f32 ? *(const float*)p : scale_of(*(const uint8_t*)p);
+      else v[h] = f32 ? *(const float*)p : weight_scale(*(const uint8_t*)p);
     }
   }
 };

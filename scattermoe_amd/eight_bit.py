@@ -78,11 +78,9 @@ def _weight(what, name, q, s, device, E, N, K, t=None):
     for u in (q, s, t):
         if u is not None and u.device != device:
             raise RuntimeError("%s: all tensors on the device of the rows (%s)" % (what, device))
-
-    def rows(u):
-        return u if u is None or (u.is_contiguous() and u.data_ptr() % 16 == 0) else u.clone(memory_format=torch.contiguous_format)
-
-    return rows(q), s, rows(t)
+    if s.size(1) * s.stride(1) + s.size(2) * s.stride(2) > 1 << 28:
+        s = s.contiguous()
+    return q.contiguous(), s, None if t is None else t.contiguous()
 
 
 def _rows_and_bias(what, x, b, name, shape):

@@ -32,26 +32,36 @@ class _GatedMLP(torch.autograd.Function):
 
     w1 (E, d, 2F) and w2 (E, F, d) are the (E, in, out) views the kernels take, in either memory layout: the
     permuted ParallelExperts parameters, or weights stored that way (gpt-oss); their gradients come back in the
-    layout of the weight they belong to.  `act`: ops.ACT_SILU / ACT_SILU_GATE_FIRST / ACT_GPT_OSS (+ alpha, limit)."""
+    layout of the weight they belong to.  `act`: ops.ACT_SILU / ACT_SILU_GATE_FIRST / ACT_GPT_OSS (+ alpha, limit).
+
+    `checkpoint_8bit` (SiLU): between the passes the pre-activation is held in 8 bits and the hidden rows not at all; the
+    backward pass takes the unit's gradient, and the hidden rows for w2's, from those bits."""
 
     @staticmethod
-    def forward(ctx, x, w1, b1, w2, b2, gates, eid, idx, off, k, act, alpha=1.702, limit=7.0):
+    def forward(ctx, x, w1, b1, w2, b2, gates, eid, idx, off, k, act, alpha=1.702, limit=7.0, checkpoint_8bit=False):
         T = x.size(0)
         need_grad = any(ctx.needs_input_grad[:6])
-        pre, h = ops.scatter2scatter_glu(x, w1, eid, idx, k, b=b1, act=act, expert_offsets=off,
-                                         need_pre=need_grad, alpha=alpha, limit=limit)
+        p8 = ps = None
+        if checkpoint_8bit and need_grad:
+            pre = ops.scatter2scatter(x, w1, eid, idx, k, b=b1, y_grouped=True, expert_offsets=off)
+            h, p8, ps = ops.glu_8bit_fwd(pre, act)
+        else:
+            pre, h = ops.scatter2scatter_glu(x, w1, eid, idx, k, b=b1, act=act, expert_offsets=off,
+                                             need_pre=need_grad, alpha=alpha, limit=limit)
         expanded = ops.scatter2scatter(h, w2, eid, idx, 1, b=b2, x_grouped=True, y_grouped=False,
                                        expert_offsets=off)
         kept = expanded.view(T, k, expanded.size(-1))
         out = ops.combine(kept, gates)
         if need_grad:
-            ctx.save_for_backward(x, w1, b1, w2, b2, gates, eid, idx, off, pre, h, kept)
+            if p8 is not None:
+                pre = h = None
+            ctx.save_for_backward(x, w1, b1, w2, b2, gates, eid, idx, off, pre, h, kept, p8, ps)
         ctx.k, ctx.act, ctx.alpha, ctx.limit = k, act, alpha, limit
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        x, w1, b1, w2, b2, gates, eid, idx, off, pre, h, kept = ctx.saved_tensors
+        x, w1, b1, w2, b2, gates, eid, idx, off, pre, h, kept, p8, ps = ctx.saved_tensors
         k, act = ctx.k, ctx.act
         need_x, need_w1, need_b1, need_w2, need_b2, need_g = ctx.needs_input_grad[:6]
         need_b1 = need_b1 and b1 is not None
@@ -68,14 +78,22 @@ class _GatedMLP(torch.autograd.Function):
             d_gates = None
             dy = ops.group(grad_out, idx, coeff=gates.reshape(-1).to(grad_out.dtype), fan_out=k, permutation=True,
                            out=kept.view(-1, kept.size(-1)))
+        dpre = None
+        need_pre = need_x or need_w1 or need_b1
+        if p8 is not None and need_pre:
+            dh = ops.scatter2scatter(dy, w2.permute(0, 2, 1), eid, idx, 1, x_grouped=True, y_grouped=True, expert_offsets=off)
+            dpre, h = ops.glu_8bit_bwd(p8, ps, dh, act, need_h=need_w2 or need_b2)
+        elif p8 is not None and (need_w2 or need_b2):
+            h = ops.glu_fwd(ops.dequantize(p8, ps, 1, w2.size(1), dy.dtype).flatten(1), act)
         d_w2 = d_b2 = None
         if need_w2 or need_b2:
             d_w2, d_b2 = ops.group_bwd_W(DY=dy, X=h, expert_offsets=off, E=E, has_bias=b2 is not None, like=w2)
             d_w2 = d_w2 if need_w2 else None
         d_x = d_w1 = d_b1 = None
-        if need_x or need_w1 or need_b1:
-            dpre = ops.scatter2scatter_glu_bwd(dy, w2.permute(0, 2, 1), pre, eid, idx, act=act, expert_offsets=off,
-                                               alpha=ctx.alpha, limit=ctx.limit)
+        if need_pre:
+            if dpre is None:
+                dpre = ops.scatter2scatter_glu_bwd(dy, w2.permute(0, 2, 1), pre, eid, idx, act=act, expert_offsets=off,
+                                                   alpha=ctx.alpha, limit=ctx.limit)
             if need_w1 or need_b1:
                 # rows of x by idx: looked up inside the launch, or copied ahead of it where that is faster
                 d_w1, d_b1 = ops.group_bwd_W(DY=dpre, X=x, expert_offsets=off, E=E, has_bias=b1 is not None, like=w1,
@@ -86,7 +104,7 @@ class _GatedMLP(torch.autograd.Function):
                                             expert_offsets=off)
                 d_x = ops.slot_sum(d_exp, x.size(0), k)
         return d_x, d_w1, (d_b1 if need_b1 else None), d_w2, (d_b2 if need_b2 else None), d_gates, \
-            None, None, None, None, None, None, None
+            None, None, None, None, None, None, None, None
 
 
 class _SparseMLP(nn.Module):
@@ -132,12 +150,20 @@ class MLP(_SparseMLP):
 
 class GLUMLP(_SparseMLP):
     """Gated variant: layer 1 produces 2*hidden columns; the FIRST half is the linear branch and the
-    SECOND half goes through the activation (reference mlp.py:81-87)."""
+    SECOND half goes through the activation (reference mlp.py:81-87).
+
+    `checkpoint_8bit` (SiLU only): a training step keeps layer 1's rows in 8 bits, a scale for every 128 columns of each half, and not
+    the hidden rows: 2 bytes per hidden value instead of 6 of a 16-bit type.  The output is the same; gradients of x, the first
+    layer and the second layer's weights carry the 8 bits' error (up to 2^-4 of a linear or gate value)."""
 
     _hidden_mult = 2
+    checkpoint_8bit = False
 
-    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=nn.SiLU()):
+    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=nn.SiLU(), checkpoint_8bit=False):
+        if checkpoint_8bit and type(activation) is not nn.SiLU:
+            raise ValueError("GLUMLP: checkpoint_8bit goes with SiLU")
         super().__init__(input_size, hidden_size, num_experts, top_k, bias, activation)
+        self.checkpoint_8bit = checkpoint_8bit
 
     def _hidden(self, pre):
         if type(self.activation) is nn.SiLU and pre.dim() == 2:
@@ -159,7 +185,7 @@ class GLUMLP(_SparseMLP):
         eid, idx, off = flatten_sort_count(expert_idxs, num_experts=self.num_experts)
         out = _GatedMLP.apply(tokens, self.experts.weight.permute(0, 2, 1), self.experts.bias,
                               self.output_experts.weight.permute(0, 2, 1), self.output_experts.bias, expert_p,
-                              eid, idx, off, self.top_k, ops.ACT_SILU)
+                              eid, idx, off, self.top_k, ops.ACT_SILU, 1.702, 7.0, self.checkpoint_8bit)
         return out.view(*lead, out.size(-1))
 
 

@@ -113,6 +113,7 @@ PRODUCTS = [
     # T, k, E, K, N, ids
     (1, 1, 1, 16, 1, "any"), (1, 2, 3, 64, 40, "any"), (5, 3, 13, 203, 117, "any"), (37, 2, 5, 300, 203, "gap"), (64, 4, 8, 128, 256, "any"),
     (130, 1, 2, 129, 257, "any"), (150, 2, 4, 520, 300, "one"), (90, 2, 6, 1000, 72, "same"), (0, 2, 3, 64, 32, "any"), (300, 2, 3, 272, 513, "any"),
+    (50, 2, 16, 144, 200, "any"), (24, 4, 12, 208, 72, "same"),                                  # 4 to 8 rows per expert
     (50, 1, 2, 8400, 260, "any"), (30, 2, 3, 72, 8320, "gap"), (70, 1, 4, 9000, 17, "one"),      # long contractions of few tiles
 ]
 
@@ -241,6 +242,7 @@ LAYERS = [
     (1, 1, 1, 32, 16, "any", False, False), (1, 2, 4, 128, 96, "any", True, False), (3, 4, 6, 203, 117, "any", False, True),
     (8, 2, 3, 256, 128, "same", True, False), (33, 2, 5, 130, 203, "gap", True, True), (70, 2, 4, 256, 160, "one", False, False),
     (140, 3, 4, 160, 256, "any", True, False), (0, 2, 3, 64, 32, "any", False, False),
+    (30, 2, 3, 144, 80, "one", True, False), (25, 2, 8, 200, 72, "any", True, True),
     (40, 1, 2, 8208, 128, "any", True, True), (20, 2, 1, 96, 8200, "same", False, False),
 ]
 

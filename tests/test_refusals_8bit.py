@@ -109,6 +109,12 @@ def test_module_keeps_its_weights_whatever_type_it_is_taken_to():
     assert not list(m.parameters())
 
 
+def test_gated_layer_with_its_checkpoint_is_a_silu_one():
+    with pytest.raises(ValueError, match="SiLU"):
+        GLUMLP(8, 8, 2, 1, activation=torch.nn.GELU(), checkpoint_8bit=True)
+    assert GLUMLP(8, 8, 2, 1, checkpoint_8bit=True).checkpoint_8bit and not GLUMLP(8, 8, 2, 1).checkpoint_8bit
+
+
 def test_c_entry_points_name_bad_calls():
     lib = _C.load()
     one, zero = ctypes.c_void_p(256), None
@@ -138,6 +144,9 @@ def test_c_entry_points_name_bad_calls():
     assert need == 1024 and lib.smoe_linear_8bit_workspace_bytes(8, 64, 64, 2, 2, 0, 1, _C.BF16) == 1536
     assert linear(size=need - 1) == -4 and linear(ws=zero) == -4 and linear(ws=ctypes.c_void_p(264)) == -4
     assert linear(L=1 << 32) == -5 and linear(L=0) == 0
+    assert linear(weight=_C.Weight8bit(256, 4096, 256, 1, 1 << 28, 1, 0)) == -5 and linear(weight=_C.Weight8bit(256, 4096, 256, 1, 1, -1, 0)) == -5
+    for K, N in (((1 << 21) + 1, 64), (64, (1 << 21) + 1)):
+        assert lib.smoe_linear_8bit(one, K, zero, w, 0, zero, 0, 0, one, N, one, one, 8, K, N, 2, 2, 0, 0, _C.BF16, one, 1 << 40, None) == -5
 
     def layer(T=4, k=2, p8=zero, ps=zero, ws=one, size=1 << 24, act=0, idx=one):
         return lib.smoe_glu_mlp_8bit(one, 64, one, one, w, zero, 0, 0, w, zero, 0, 0, one, one, p8, ps, idx, one, T, k, 64, 64, 2, act, _C.BF16, ws, size, None)
