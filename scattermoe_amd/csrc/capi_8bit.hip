@@ -21,10 +21,10 @@ struct Carver {
   }
 };
 
-// Rows of 8-bit activations of a product of L rows: the tokens once, or a copy for each row where they are scaled one by one or where
-// the token matrix passes the 32-bit offsets that a gathered operand has
+// Rows of 8-bit activations of a product of L rows that come by token: the tokens once, or once per slot where those are scaled, and the product looks
+// them up; a copy for each row, in the rows' order, where they pass the 32-bit offsets of a look-up
 static bool gathers(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
-  return !x_grouped && !scaled && L / fan * block_row(K) < (1LL << 32);
+  return !x_grouped && (scaled ? L : L / fan) * block_row(K) < (1LL << 32);
 }
 static float* take_partial(Carver& c, int64_t floats) { return floats ? c.take<float>(floats * 4) : nullptr; }
 struct Rows8Bit { uint8_t* q; uint8_t* s; int64_t rows; };
@@ -36,7 +36,7 @@ static Rows8Bit take_rows(Carver& c, int64_t rows, int64_t K) {
 }
 static int quantize(const Rows8Bit& r, const void* X, int64_t sxm, const int64_t* idx, int fan, const void* coeff, int64_t K, int dtype,
                     hipStream_t st) {
-  QuantRowsArgs a{X, sxm, idx, fan, coeff, r.rows, K, r.q, r.s, r.rows, block_row(K)};
+  QuantRowsArgs a{X, sxm, idx, fan, coeff, coeff && !idx ? r.rows / fan : r.rows, K, r.q, r.s, r.rows, block_row(K)};
   return launch_quantize_rows(a, dtype, st);
 }
 
@@ -169,7 +169,7 @@ static int workspace_check(const char* who, size_t need, const void* workspace, 
 size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, int fan_out, int x_grouped, int scaled, int dtype) {
   if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
-  take_rows(c, gathers(L, K, fan_out, x_grouped, scaled != 0) ? L / fan_out : L, K);
+  take_rows(c, !scaled && gathers(L, K, fan_out, x_grouped, false) ? L / fan_out : L, K);
   if (!few_rows_pay(L, E)) c.take(product_8bit_floats(L, K, N, E, dtype) * 4);
   return c.used;
 }
@@ -186,16 +186,17 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out, x_grouped, coeff != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
   const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
-  const Rows8Bit x = take_rows(c, by_token ? L / fan_out : L, K);
+  const Rows8Bit x = take_rows(c, by_token && !coeff ? L / fan_out : L, K);
+  const int fan = coeff ? 1 : fan_out;                             // rows of x per row of the product's left side
   const bool copies = !x_grouped && !by_token;
   if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
   if (few_rows_pay(L, E)) {
-    Few8Args a = few(W, b, sbe, sbn, Y, sym, dtype, nullptr, idx, off, L, K, N, E, fan_out, !by_token, y_grouped, 0);
+    Few8Args a = few(W, b, sbe, sbn, Y, sym, dtype, nullptr, idx, off, L, K, N, E, fan, !by_token, y_grouped, 0);
     if (transposed) a.ssn = W->s_col, a.ssk = W->s_row;
     a.X = x.q, a.sxm = block_row(K), a.XS = x.s;
     return launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, (hipStream_t)stream);
   }
-  Product8Args a = product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan_out, !by_token, y_grouped);
+  Product8Args a = product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan, !by_token, y_grouped);
   a.partial = take_partial(c, product_8bit_floats(L, K, N, E, dtype));
   return launch_product_8bit(a, dtype, dtype, (hipStream_t)stream);
 }
@@ -250,6 +251,7 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   const LayerWay way = layer_way(L, d, F, E, ordered, P8 != nullptr);
   if (!ordered && (L > SMOE_8BIT_FEW_ROWS || P8)) { set_error("smoe_glu_mlp_8bit: an order is needed for more than %d rows, and to keep P8", SMOE_8BIT_FEW_ROWS); return SMOE_ERR_NULL; }
   if (!X || !gates || !OUT || (P8 && !PS) || (ordered ? !Y || !off : !experts)) { set_error("smoe_glu_mlp_8bit: NULL pointer"); return SMOE_ERR_NULL; }
+  if ((uintptr_t)P8 & 15) { set_error("smoe_glu_mlp_8bit: P8 starts at a multiple of 16 bytes"); return SMOE_ERR_SHAPE; }
   if (int rc = weight_checks("smoe_glu_mlp_8bit", W1, 2 * F, d)) return rc;
   if (int rc = weight_checks("smoe_glu_mlp_8bit", W2, d, F)) return rc;
   if (int rc = workspace_check("smoe_glu_mlp_8bit", smoe_glu_mlp_8bit_workspace_bytes(T, k, d, F, E, ordered, P8 != nullptr, dtype), workspace, workspace_bytes)) return rc;
@@ -320,14 +322,16 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   if (!act_ok(act)) { set_error("smoe_glu_mlp_8bit_bwd: unknown activation %d", act); return SMOE_ERR_SHAPE; }
   if (T == 0 || d == 0) return 0;
   if (!DOUT || !gates || !P8 || !PS || !DROWS || !DX || !idx || !off) { set_error("smoe_glu_mlp_8bit_bwd: NULL pointer"); return SMOE_ERR_NULL; }
+  if ((uintptr_t)P8 & 15) { set_error("smoe_glu_mlp_8bit_bwd: P8 starts at a multiple of 16 bytes"); return SMOE_ERR_SHAPE; }
   if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W1T, 2 * F, d)) return rc;
   if (int rc = weight_checks("smoe_glu_mlp_8bit_bwd", W2T, d, F)) return rc;
   if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E, dtype), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
   Carver c{(char*)workspace};
   const BackPieces p = back_pieces(c, L, d, F, E, dtype);
-  if (int rc = quantize(p.dy, DOUT, sdm, idx, k, gates, d, dtype, st)) return rc;
-  Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, 1, 1);
+  const bool by_slot = gathers(L, d, k, 0, true);
+  if (int rc = quantize(p.dy, DOUT, sdm, by_slot ? nullptr : idx, k, gates, d, dtype, st)) return rc;
+  Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, !by_slot, 1);
   a.partial = p.partial1;
   if (!p.dh) {
     a.H8 = p.dp.q, a.HS = p.dp.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;

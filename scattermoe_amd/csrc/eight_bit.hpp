@@ -106,9 +106,9 @@ enum Scaling8 {
 // ---- arguments ---------------------------------------------------------------------------------------
 struct QuantRowsArgs {
   const void* X; int64_t sxm;                                      // columns contiguous
-  const int64_t* idx; int fan;                                     // row n is source row idx[n] / fan; NULL: row n
-  const void* coeff;                                               // times coeff[idx[n]]; NULL: 1
-  int64_t rows, K;
+  const int64_t* idx; int fan;                                     // row n is source row idx[n] / fan; NULL: n, of n / fan with coeff
+  const void* coeff;                                               // times coeff[idx[n]], coeff[n]; NULL: 1
+  int64_t rows, K;                                                 // (rows: of the source where there is coeff, and no idx)
   uint8_t* Q; uint8_t* S;
   int64_t slots;                                                   // with idx: entries outside [0, slots) make a row of zeros
   int64_t ld;                                                      // bytes of a row of Q, a multiple of 16, zeros behind the last value

@@ -189,7 +189,8 @@ __device__ __forceinline__ float row_max(float v) {
 template <int WIDTH>
 struct ByteTile {
   static constexpr int ROW = WIDTH + 16;
-  static __device__ __forceinline__ void put(char* lds, int row, int col, int q) { *(int*)(lds + row * ROW + col) = q; }
+  template <typename V>
+  static __device__ __forceinline__ void put(char* lds, int row, int col, V q) { *(V*)(lds + row * ROW + col) = q; }
   // ROWS rows to `out`, `ld` bytes apart, `rows` and `cols` (a multiple of 16) of them there
   template <int ROWS>
   static __device__ __forceinline__ void store(const char* lds, uint8_t* out, int64_t ld, int rows, int cols) {
@@ -229,7 +230,7 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
       float m[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const float* b = s_bias + wave * TL::WTN + 16 * g + 4 * (l >> 4);
+        const float* b = s_bias + wave * TL::WTN + 8 * (l >> 4) + 4 * g;
         f32x4 &lin = acc[ai][0].q[aq + g], &gate = acc[ai][1].q[aq + g];
         lin += *(const f32x4*)b, gate += *(const f32x4*)(b + 32);
 #pragma unroll
@@ -255,14 +256,16 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
         const float* most = top + s * 4 * ROWS + r;
         const int byte = scale_byte(fmaxf(fmaxf(most[0], most[ROWS]), fmaxf(most[2 * ROWS], most[3 * ROWS])));
         const float scale = scale_of(byte);
+        i32x2 both;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const f32x4 &lin = acc[ai][0].q[aq + g], &gate = acc[ai][1].q[aq + g];
           const int q = s == 0   ? to_e4m3x4(unit[i][g][0], unit[i][g][1], unit[i][g][2], unit[i][g][3], scale)
                         : s == 1 ? to_e4m3x4(lin[0], lin[1], lin[2], lin[3], scale)
                                  : to_e4m3x4(gate[0], gate[1], gate[2], gate[3], scale);
-          Bytes::put(lds + s * SIDE, r, wave * 32 + 16 * g + 4 * (l >> 4), mine ? q : 0);
+          both[g] = mine ? q : 0;
         }
+        Bytes::put(lds + s * SIDE, r, wave * 32 + 8 * (l >> 4), both);
         if (wave == 0 && l < 16 && part * ROWS + r < rows) {
           uint8_t* out = s == 0 ? a.HS + row * scale_row(F) : a.PS + (2 * row + ((s - 1) ^ swapped)) * fb;
           out[n_tile] = (uint8_t)byte;
@@ -304,11 +307,12 @@ __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8
       const uint8_t* ps = a.PS + (int64_t)row * 2 * fb + n / QB;
       const float s1 = scale_of(ps[swapped * fb]), s2 = scale_of(ps[(1 - swapped) * fb]);
       float m1 = 0.0f, m2 = 0.0f;
+      const i32x4 lin8 = *(const i32x4*)(p8 + lin_at + 16 * (l >> 4)), gate8 = *(const i32x4*)(p8 + gate_at + 16 * (l >> 4));
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
         float lin[4], gate[4];
-        from_e4m3x4_exact(*(const int*)(p8 + lin_at + j * 16 + 4 * (l >> 4)), s1, lin);
-        from_e4m3x4_exact(*(const int*)(p8 + gate_at + j * 16 + 4 * (l >> 4)), s2, gate);
+        from_e4m3x4_exact(lin8[j], s1, lin);
+        from_e4m3x4_exact(gate8[j], s2, gate);
         f32x4& d = acc[(part * FR + i) >> 1][j >> 1].q[2 * ((part * FR + i) & 1) + (j & 1)];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -328,13 +332,15 @@ __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8
       const int b1 = scale_byte(fmaxf(top[pair * ROWS + r], top[(pair + 1) * ROWS + r]));
       const int b2 = scale_byte(fmaxf(top[(4 + pair) * ROWS + r], top[(5 + pair) * ROWS + r]));
       const float f1 = scale_of(b1), f2 = scale_of(b2);
+      i32x4 dl8, dg8;
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
         const f32x4& d = acc[(part * FR + i) >> 1][j >> 1].q[2 * ((part * FR + i) & 1) + (j & 1)];
-        const int col = wave * TL::WTN + j * 16 + 4 * (l >> 4);
-        Bytes::put(lds, r, col, to_e4m3x4(d[0], d[1], d[2], d[3], f1));
-        Bytes::put(lds + ROWS * Bytes::ROW, r, col, to_e4m3x4(dgate[i][j][0], dgate[i][j][1], dgate[i][j][2], dgate[i][j][3], f2));
+        dl8[j] = to_e4m3x4(d[0], d[1], d[2], d[3], f1);
+        dg8[j] = to_e4m3x4(dgate[i][j][0], dgate[i][j][1], dgate[i][j][2], dgate[i][j][3], f2);
       }
+      Bytes::put(lds, r, wave * TL::WTN + 16 * (l >> 4), dl8);
+      Bytes::put(lds + ROWS * Bytes::ROW, r, wave * TL::WTN + 16 * (l >> 4), dg8);
       if ((wave & 1) == 0 && l < 16 && part * ROWS + r < rows && mine) {
         uint8_t* s = a.HS + (int64_t)(row0 + part * ROWS + r) * Ds + n / QB;
         s[swapped * fb] = (uint8_t)b1, s[(1 - swapped) * fb] = (uint8_t)b2;
@@ -444,7 +450,6 @@ template <typename TO>
 __device__ __forceinline__ void store_rows(const Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int n0, const int64_t* s_dst,
                                            const float* s_bias, char* lds) {
   typedef Tile8 TL;
-  typedef TO T4 __attribute__((ext_vector_type(4)));
   constexpr int PER = 16 / (int)sizeof(TO), HALVES = (int)sizeof(TO) / 2, COLS = TL::BN / HALVES, CPR = COLS / PER;      // 32 pieces a row
   const int t = late_thread<TL>(), wave = t >> 6, l = t & 63;
   TO* Y = (TO*)a.Y;
@@ -455,16 +460,17 @@ __device__ __forceinline__ void store_rows(const Block (&acc)[Tile8::FM][Tile8::
     if (half) __syncthreads();
     if (HALVES == 1 || (wave >> 1) == half) {
 #pragma unroll
-      for (int j = 0; j < 2 * TL::FN; ++j) {
-        const int tc = wave * TL::WTN + j * 16 + 4 * (l >> 4);
-        const f32x4 b = *(const f32x4*)(s_bias + tc);
+      for (int j = 0; j < 2 * TL::FN; j += PER / 4) {
+        const int tc = wave * TL::WTN + 16 * (l >> 4) + 4 * j;
 #pragma unroll
         for (int i = 0; i < 2 * TL::FM; ++i) {
-          const f32x4& q = acc[i >> 1][j >> 1].q[2 * (i & 1) + (j & 1)];
-          T4 v;
+          TO v[PER];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = from_f32<TO>(q[c] + b[c]);
-          *(T4*)(lds + place(i * 16 + (l & 15), tc % COLS)) = v;
+          for (int c = 0; c < PER; ++c)
+            v[c] = from_f32<TO>(acc[i >> 1][(j + c / 4) >> 1].q[2 * (i & 1) + ((j + c / 4) & 1)][c & 3] + s_bias[tc + c]);
+          i32x4 p;
+          __builtin_memcpy(&p, v, 16);
+          *(i32x4*)(lds + place(i * 16 + (l & 15), tc % COLS)) = p;
         }
       }
     }
@@ -552,6 +558,8 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
   const int src0 = a.x_grouped ? row0 : 0;
   const int64_t ld = (a.K + QB - 1) / QB * QB;                         // the rows are whole slices long
   A.init((const char*)a.X + src0 * ld + k0 * QB, [&](int row) { return (int64_t)(s_src[row] - src0) * ld; });
+  // (which column a weight row in LDS belongs to is ours to choose: a lane's four fragments' columns lie side by side, 16 of them, in the unit 8 of
+  // either half, so that it writes and reads whole pieces of rows)
   Cols8 B;
   const int turn = (share.row % BAND8 * Cols8::R / BAND8) % Cols8::R;
   const int64_t swn = a.swn;
@@ -560,13 +568,18 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
   if constexpr (EPI == EPI_UNIT) {
     // tile column -> weight row: first 32 of a wave's 64 from the linear half of the rows, the others from the gate's
     const int lin_at = (a.act & 1) * F, gate_at = F - lin_at;
-    B.init((const char*)a.W + e * a.swe + k0 * QB, (int64_t)a.N * swn - k0 * QB, turn,
-           [&](int tc) { return (int64_t)(min(n0 + (tc >> 6) * 32 + (tc & 31), F - 1) + (tc & 32 ? gate_at : lin_at)) * swn; });
+    B.init((const char*)a.W + e * a.swe + k0 * QB, (int64_t)a.N * swn - k0 * QB, turn, [&](int tc) {
+      const int of_wave = ((tc & 12) << 1) + ((tc & 16) >> 2) + (tc & 3);
+      return (int64_t)(min(n0 + (tc >> 6) * 32 + of_wave, F - 1) + (tc & 32 ? gate_at : lin_at)) * swn;
+    });
     const int hc = min(n0 + wave_u * 32, F - 1);
     nb[0] = (lin_at + hc) / QB, nb[1] = (gate_at + hc) / QB;
   } else {
     const int last = a.N - 1 - n0;
-    B.init((const char*)a.W + e * a.swe + n0 * swn + k0 * QB, (a.N - n0) * swn - k0 * QB, turn, [&](int row) { return (int64_t)min(row, last) * swn; });
+    B.init((const char*)a.W + e * a.swe + n0 * swn + k0 * QB, (a.N - n0) * swn - k0 * QB, turn, [&](int tc) {
+      const int of_wave = ((tc & 12) << 2) + ((tc & 48) >> 2) + (tc & 3);
+      return (int64_t)min((tc & ~63) + of_wave, last) * swn;
+    });
     nb[0] = nb[1] = min(n0 + wave_u * TL::WTN, a.N - 1) / QB;
   }
   WeightScales<SC> W;

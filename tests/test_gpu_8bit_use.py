@@ -348,3 +348,38 @@ def test_glumlp_keeps_a_third():
         kept.append(torch.cuda.memory_allocated() - before)
         del out
     assert kept[0] - kept[1] >= 2000 * 1024 * (6 - 2 - 0.1)
+
+
+def _some_rows(name, got, x, w, which, experts, dtype):
+    """Rows `which` of got against x8[which] w[expert]^T; x (rows, K) float64 of those rows."""
+    for r, e in zip(range(len(which)), experts):
+        v, err = ref.product(ref.q8(x[r:r + 1])[0], torch.zeros_like(x[r:r + 1]), w[e], True, False)
+        ref.check("%s, row %d" % (name, int(which[r])), got[which[r]].unsqueeze(0), v, ref.rounded(v, err, dtype))
+
+
+def test_rows_that_pass_32_bit_offsets():
+    """More than 4 GiB of rows in 8 bits: tokens, and rows scaled one by one, in and out of the experts' order."""
+    E, d, n, k = 8, 4096, 16, 8
+    T = (1 << 20) + 64
+    g = torch.Generator(device=DEV).manual_seed(3)
+    w = torch.randn(E, n, d, device=DEV, generator=g) * d ** -0.5
+    q, s, qt = eight_bit.quantize_blocks(w, 128, transposed=True)
+    w64 = ref.stands_for(q, s, d)
+    some = torch.tensor([0, 1, 77777, 524288, T - 65, T - 2, T - 1])
+    x = torch.empty(T, d, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    ids = torch.randint(0, E, (T, 1), device=DEV, generator=g)
+    eid, idx, off = flatten_sort_count(ids, E)
+    y = eight_bit.parallel_linear_8bit(x, q, s, 1, eid, idx, off)
+    _some_rows("by token", y, x[some.to(DEV)].cpu().double(), w64, some, ids[some.to(DEV), 0].tolist(), torch.bfloat16)
+    del x, y
+    # the second product of a layer, 2^20 rows of 16 -> 4096, and its gradient from the tokens' times their gates
+    tokens = T // k
+    h = torch.randn(T, n, device=DEV, generator=g).bfloat16().requires_grad_()
+    gates = (torch.randint(1, 3, (tokens, k), device=DEV, generator=g) / 2).bfloat16()
+    dout = torch.empty(tokens, d, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    eid, idx, off = flatten_sort_count(ids.view(tokens, k), E)
+    out = eight_bit.parallel_linear_8bit(h, qt, s.transpose(1, 2), 1, eid, idx, off, gates=gates, grouped_in=True, weight_t=q)
+    (dh,) = torch.autograd.grad(out, h, dout)
+    slots = idx[some.to(DEV)].cpu()
+    scaled = dout[(slots // k).to(DEV)].cpu().double() * gates.view(-1)[slots.to(DEV)].cpu().double().unsqueeze(1)
+    _some_rows("scaled", dh, scaled, w64, some, eid[some.to(DEV)].tolist(), torch.bfloat16)
