@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantRowsArgs a, int
   for (int i = 0; i < 8; ++i) v[i] *= f;
   store_block(a.Q + u.row * a.ld, a.S + u.row * scale_row(a.K) + u.block, u.c, a.ld, v);
 }
-// a source row once, times each of its fan coefficients (8192 rows of 2048, 8 each: 84 us by idx, @@ so)
+// a source row once, times each of its fan coefficients (8192 rows of 2048, 8 each: 84 us by idx, 29 so)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quantize_times_kernel(QuantRowsArgs a, int blocks) {
   const Unit u(a.rows, blocks);

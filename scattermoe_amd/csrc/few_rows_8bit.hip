@@ -68,27 +68,33 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
   constexpr int HALF = EPI == EPI_UNIT ? GROUPS / 2 : GROUPS;      // groups of neighbouring columns
   const int n0 = blockIdx.x * (HALF * 8);
   const int Kp = (int)padded_row(a.K);
-  constexpr int WSB = SF ? 4 : 1;                                  // bytes of a scale (a type of its own: a branch at each of their loads
-                                                                   // would order the loads around it)
   // 32-bit offsets from the first row of either half (the launcher checks)
   e = __builtin_amdgcn_readfirstlane(e);
   const char* We = (const char*)a.W + e * a.swe;
   const int64_t n1 = n0 + (EPI == EPI_UNIT ? F : 0);
   const __amdgpu_buffer_rsrc_t W[2] = {from_here(We + (int64_t)n0 * Kp, (a.N - n0) * (int64_t)Kp), from_here(We + n1 * Kp, (a.N - n1) * Kp)};
-  const __amdgpu_buffer_rsrc_t WS = from_here((const char*)a.WS + e * a.sse * WSB, 0xffffffffLL);
   const int sub = (l & 15) >> 1, at = (l & 1) * 64 + (l >> 4) * 16;  // row of a group, and this lane's 16 values of a slice
-  unsigned woff[HALF], soff[GROUPS];
+  unsigned woff[HALF];
 #pragma unroll
-  for (int j = 0; j < GROUPS; ++j) {
-    const int n = min(n0 + (j % HALF) * 8 + sub, (EPI == EPI_UNIT ? F : a.N) - 1);
-    if (j < HALF) woff[j] = (unsigned)(n - n0) * (unsigned)Kp + at;
-    soff[j] = (unsigned)((n + (j >= HALF ? F : 0)) / QB * a.ssn) * WSB;
+  for (int j = 0; j < HALF; ++j) woff[j] = (unsigned)(min(n0 + j * 8 + sub, (EPI == EPI_UNIT ? F : a.N) - 1) - n0) * (unsigned)Kp + at;
+  // A slice's scales: one for these columns, which lie in one block of 128; in the unit one for the first half's and two for the second's, whose
+  // columns start anywhere.  A byte comes as the dword it lies in and is taken out where it is used: loaded as a byte, it is converted
+  // where it was loaded, and every slice waits for its own scales (8 experts, 4096 -> 14336, 32 rows: 90 us, 72 so).
+  constexpr int SCALES = EPI == EPI_UNIT ? 3 : 1, WSB = SF ? 4 : 1;
+  const char* ws_at = (const char*)a.WS + e * a.sse * WSB;
+  const int ws_rem = (int)((uintptr_t)ws_at & 3);
+  const __amdgpu_buffer_rsrc_t WS = from_here(ws_at - ws_rem, 0xffffffffLL);
+  int sfirst[SCALES];
+  sfirst[0] = ws_rem + (int)(n0 / QB * a.ssn) * WSB;
+  if constexpr (EPI == EPI_UNIT) {
+    const int b = (F + n0) / QB;
+    sfirst[1] = ws_rem + (int)(b * a.ssn) * WSB;
+    sfirst[2] = ws_rem + (int)(min(b + 1, (a.N - 1) / QB) * a.ssn) * WSB;
   }
   const int nk = (int)scale_blocks(a.K), first = wave * per, last = min(first + per, nk);
-  auto scale_at = [&](int kt, int j) {
-    const int o = (int)(kt * a.ssk) * WSB;
-    if constexpr (SF) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(WS, (int)soff[j], o, 0));
-    else return weight_scale((int)__builtin_amdgcn_raw_buffer_load_b8(WS, (int)soff[j], o, 0));
+  auto load_scale = [&](int kt, int h) { return (int)__builtin_amdgcn_raw_buffer_load_b32(WS, 0, (sfirst[h] + (int)(kt * a.ssk) * WSB) & ~3, 0); };
+  auto scale_in = [&](int v, int kt, int h) {
+    return SF ? __builtin_bit_cast(float, v) : weight_scale((v >> (((sfirst[h] + (int)(kt * a.ssk)) & 3) * 8)) & 255);
   };
   for (int base = 0; base < rows; base += ROWS) {                  // (by ids, an expert may have more rows than ROWS)
     const int here = min(ROWS, rows - base);
@@ -110,7 +116,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
     constexpr int XV = FROM_8BIT ? 4 : 4 * (int)sizeof(TX);
     typedef int XRegs __attribute__((ext_vector_type(XV)));
     w_i32x4 w[2][GROUPS];
-    float ws[2][GROUPS];
+    int ws[2][SCALES];
     XRegs xv[2][MF];
     int xb[2][MF];
     // slices that go two at a time: all of rows in 8 bits, which are whole slices long, whole ones of aligned float rows
@@ -122,9 +128,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
         w[p][j] = __builtin_bit_cast(w_i32x4, __builtin_amdgcn_raw_buffer_load_b128(W[j / HALF], (int)woff[j % HALF], kt * QB, 0));
       }
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j) {
-        ws[p][j] = scale_at(kt, j);
-      }
+      for (int h = 0; h < SCALES; ++h) ws[p][h] = load_scale(kt, h);
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
 #pragma unroll
@@ -140,8 +144,9 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         w[0][j] = __builtin_bit_cast(w_i32x4, __builtin_amdgcn_raw_buffer_load_b128(W[j / HALF], (int)woff[j % HALF], kt * QB, 0));
-        ws[0][j] = scale_at(kt, j);
       }
+#pragma unroll
+      for (int h = 0; h < SCALES; ++h) ws[0][h] = load_scale(kt, h);
       if constexpr (!FROM_8BIT) {
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
@@ -158,6 +163,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
       for (int i = 0; i < MF; ++i) {
         w_i32x4 q;
         int byte;
+        if constexpr (FROM_8BIT) asm volatile("" : "+v"(xb[p][i]));
         if constexpr (FROM_8BIT) {
           q = xv[p][i];
           byte = (xb[p][i] >> (8 * (min(slice, last - 1) & 3))) & 255;
@@ -179,13 +185,23 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
       }
       // (behind a row's end is the next one's, which may be no number; behind the last slice, that one again)
       const bool there = slice < end && slice * QB + at < Kp;
+      float scales[SCALES];
+#pragma unroll
+      for (int h = 0; h < SCALES; ++h) {
+        asm volatile("" : "+v"(ws[p][h]));
+        scales[h] = scale_in(ws[p][h], min(slice, end - 1), h);
+      }
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         bf16x8_8b wv[2];
         w_i32x4 q = w[p][j];
+        float scale = scales[0];
+        if constexpr (EPI == EPI_UNIT) {
+          if (j >= HALF) scale = (F + n0 + (j - HALF) * 8 + sub) / QB == (F + n0) / QB ? scales[1] : scales[2];
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) q[c] = there ? q[c] : 0;
-        to_bf16x16(q, SF ? 1.0f : ws[p][j], wv);
+        to_bf16x16(q, SF ? 1.0f : scale, wv);
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
           w_f32x4 s = SF ? w_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][j];
@@ -193,15 +209,18 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
           for (int u = 0; u < 2; ++u) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][u], wv[u], s, 0, 0, 0);
           // (columns across the lanes: a column's scale is the lane's own)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j][c] = SF ? fmaf(s[c], ws[p][j], acc[i][j][c]) : s[c];
+          for (int c = 0; c < 4; ++c) acc[i][j][c] = SF ? fmaf(s[c], scale, acc[i][j][c]) : s[c];
         }
         if (j & 1) __builtin_amdgcn_sched_barrier(0);              // (all groups' conversions at once take too many registers)
       }
     };
     // (pairs of slices; one behind the last is the last again, its weights zeros: no branches, whose joins cost registers)
     if (first < whole) {
+      // (in this order: the waits inside the loop are for what is on its way in either of its entries)
       fetch(first, 0);
+      __builtin_amdgcn_sched_barrier(0);
       fetch(first + 1, 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma nounroll
       for (int kt = first; kt < whole; kt += 2) {
         multiply(kt, 0, whole);
@@ -297,6 +316,8 @@ int launch_few_rows_8bit(const Few8Args& a, int x_dtype, int dtype, int epilogue
   if (x_dtype == SMOE_BF16) return launch_few<bf16_t, 1>(a, dtype, epilogue, st);
   if (x_dtype == SMOE_F16) return launch_few<f16_t, 1>(a, dtype, epilogue, st);
   if (x_dtype == SMOE_F32) return launch_few<float, 1>(a, dtype, epilogue, st);
+  // (8 or 16 rows of an expert at a time, us at 2, 4, 8 rows per expert, loads as 1 / rank^0.5: 8 experts, 4096 -> 14336 71, 77, 89 or 73, 74, 80;
+  // 128 experts, 2048 -> 1536 63, 66, 80 or 69, 71, 77)
   return a.L <= 4 * (int64_t)a.E ? launch_few<uint8_t, 1>(a, dtype, epilogue, st) : launch_few<uint8_t, 2>(a, dtype, epilogue, st);
 }
 
