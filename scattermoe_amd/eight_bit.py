@@ -102,12 +102,17 @@ class _Linear8bit(torch.autograd.Function):
     """y = Q(x) W^T, combined with the gates; backward dx = Q(gate dy) W from the transposed weights, nothing to the weights."""
 
     @staticmethod
-    def forward(ctx, x, gates, w, s, wt, b, idx, off, k, grouped_in, grouped_out):
+    def rows(x, gates, w, s, b, idx, off, k, grouped_in, grouped_out):
+        """(y, the experts' rows where gates weigh them)"""
         y = ops.linear_8bit(x, w, s, idx, off, k, b=b, x_grouped=grouped_in, y_grouped=grouped_out)
-        kept = None
-        if gates is not None:
-            kept = y.view(gates.size(0), gates.size(1), y.size(1))
-            y = ops.combine(kept, gates)
+        if gates is None:
+            return y, None
+        kept = y.view(gates.size(0), gates.size(1), y.size(1))
+        return ops.combine(kept, gates), kept
+
+    @staticmethod
+    def forward(ctx, x, gates, w, s, wt, b, idx, off, k, grouped_in, grouped_out):
+        y, kept = _Linear8bit.rows(x, gates, w, s, b, idx, off, k, grouped_in, grouped_out)
         ctx.save_for_backward(gates, kept if gates is not None and ctx.needs_input_grad[1] else None, wt, s, idx, off)
         ctx.k, ctx.rows, ctx.grouped = k, x.size(0), (grouped_in, grouped_out)
         return y
@@ -163,6 +168,9 @@ def parallel_linear_8bit(inputs, weight, weight_scales, k, sorted_expert_idxs, s
     if inputs.requires_grad and torch.is_grad_enabled() and weight_t is None:
         raise ValueError("%s: the gradient of the inputs needs weight_t, the transposed weight" % what)
     idx, off = ops._as_i64(sorted_scattered_idxs).contiguous(), ops._as_i64(expert_offsets).contiguous()
+    trained = torch.is_grad_enabled() and (inputs.requires_grad or (gates is not None and gates.requires_grad))
+    if not trained and not ops.has_tangents(inputs, gates, expert_biases):
+        return _Linear8bit.rows(inputs, gates, weight, scales, expert_biases, idx, off, k, grouped_in, grouped_out)[0]
     return _Linear8bit.apply(inputs, gates, weight, scales, weight_t, expert_biases, idx, off, k, grouped_in, grouped_out)
 
 

@@ -383,3 +383,15 @@ def test_rows_that_pass_32_bit_offsets():
     slots = idx[some.to(DEV)].cpu()
     scaled = dout[(slots // k).to(DEV)].cpu().double() * gates.view(-1)[slots.to(DEV)].cpu().double().unsqueeze(1)
     _some_rows("scaled", dh, scaled, w64, some, eid[some.to(DEV)].tolist(), torch.bfloat16)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+    i = _Layer(40, 2, 4, 160, 96, torch.bfloat16)
+    eid, idx, off = flatten_sort_count(i.ids, 4)
+    with fwad.dual_level():
+        x = fwad.make_dual(i.x, torch.ones_like(i.x))
+        for call in (lambda: i.forward(x), lambda: eight_bit.checkpointed_glu(x),
+                     lambda: eight_bit.parallel_linear_8bit(x, i.w1, i.s1, 2, eid, idx, off, weight_t=i.w1_t)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
