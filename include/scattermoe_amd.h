@@ -429,7 +429,7 @@ int smoe_dequantize_8bit(const void* Q, int64_t sqe, int64_t sqn, const void* S,
 
 /*
  * Gated unit that keeps its input in 8 bits.  pre (rows, 2F) row stride spm -> h (rows, F) contiguous, rounded from pre itself, and
- * P8 (rows, 2, F rounded up to 16), PS (rows, 2, ceil(F / 128)): the first and the second half of pre, each with blocks of its own.
+ * P8 (rows, 2, F rounded up to 16), PS (rows, 2, ceil(F / 128)): pre's linear half, then its gate's, each with blocks of its own.
  * Backward: dpre (rows, 2F) contiguous from P8, PS and dh (rows, F) row stride sdh; h, unless NULL, is the unit's value of what P8 stands for.
  */
 int smoe_glu_8bit_fwd(const void* pre, int64_t spm, void* h, void* P8, void* PS, int64_t rows, int64_t F, int act, int dtype, void* stream);
@@ -437,7 +437,7 @@ int smoe_glu_8bit_bwd(const void* P8, const void* PS, const void* dh, int64_t sd
                       int dtype, void* stream);
 
 /*
- * A weight in 8 bits: q (E, N, K rounded up to 16), filled with zeros, an expert's values contiguous from a multiple of 16
+ * A weight in 8 bits, K and N up to 2^21: q (E, N, K rounded up to 16), filled with zeros, an expert's values contiguous from a multiple of 16
  * bytes on; s: a scale for every 128 x 128 values, 8 bits (a power of two) or float32 (any).  Strides in elements.  A transposed
  * weight has the scales, and the scales' strides, of the weight that it is the transpose of.
  */
@@ -464,7 +464,7 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
  * A gated layer on such weights (GLUMLP.forward, scattermoe/mlp.py:74-95):
  *   pre = Q(X) W1[e]^T + b1[e];  y = Q(glu(pre)) W2[e]^T + b2[e];  OUT[t] = sum_j gates[t,j] y
  * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) by slot (y, rounded), OUT (T,d)
- * contiguous; P8, PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
+ * contiguous; P8 (16-byte aligned), PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
  * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
  * alone, and ids outside [0,E) drop their row.
  * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with

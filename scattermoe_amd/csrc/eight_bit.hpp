@@ -131,7 +131,7 @@ struct DequantArgs {
 };
 int launch_dequantize(const DequantArgs& a, int dtype, hipStream_t st);
 
-// gated unit, forward: pre (rows, 2F) in `pre_dtype` -> h in `dtype` or (H8, HS) in 8 bits; P8 (rows, 2, Fp), PS (rows, 2, FB): the halves
+// gated unit, forward: pre (rows, 2F) in `pre_dtype` -> h in `dtype` or (H8, HS) in 8 bits; P8 (rows, 2, Fp), PS (rows, 2, FB): the linear half and the gate's
 // of pre in 8 bits, each with blocks of its own (NULL: not wanted)
 struct UnitArgs {
   const void* pre; int64_t spm;

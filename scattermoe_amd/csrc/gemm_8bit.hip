@@ -218,7 +218,6 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
   const int t = late_thread<TL>(), wave = t >> 6, l = t & 63, F = a.N / 2, fb = (int)scale_blocks(F);
   const bool mine = n_tile * QB + wave * 32 < F;          // (F is a multiple of 32)
   const int64_t ld = scale_blocks(F) * QB;                         // (hidden rows are whole slices long, zeros behind the last value)
-  const int swapped = a.act & 1;                                   // the gate's half is the first one
   float* top = (float*)(lds + 3 * SIDE);                           // [the unit, its halves][wave][row]
 #pragma unroll
   for (int part = 0; part < PARTS; ++part) {
@@ -267,7 +266,7 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
         }
         Bytes::put(lds + s * SIDE, r, wave * 32 + 8 * (l >> 4), both);
         if (wave == 0 && l < 16 && part * ROWS + r < rows) {
-          uint8_t* out = s == 0 ? a.HS + row * scale_row(F) : a.PS + (2 * row + ((s - 1) ^ swapped)) * fb;
+          uint8_t* out = s == 0 ? a.HS + row * scale_row(F) : a.PS + (2 * row + s - 1) * fb;
           out[n_tile] = (uint8_t)byte;
         }
       }
@@ -278,7 +277,7 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
     if (a.P8) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        Bytes::template store<ROWS>(lds + (1 + h) * SIDE, a.P8 + (first * 2 + (h ^ swapped)) * F + n_tile * QB, 2 * F, rows - part * ROWS, min(QB, F - n_tile * QB));
+        Bytes::template store<ROWS>(lds + (1 + h) * SIDE, a.P8 + (first * 2 + h) * F + n_tile * QB, 2 * F, rows - part * ROWS, min(QB, F - n_tile * QB));
     }
   }
 }
@@ -305,9 +304,9 @@ __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8
       const int r = part * ROWS + i * 16 + (l & 15), row = row0 + min(r, rows - 1);
       const uint8_t* p8 = a.P8 + (int64_t)row * 2 * F + n;
       const uint8_t* ps = a.PS + (int64_t)row * 2 * fb + n / QB;
-      const float s1 = scale_of(ps[swapped * fb]), s2 = scale_of(ps[(1 - swapped) * fb]);
+      const float s1 = scale_of(ps[0]), s2 = scale_of(ps[fb]);
       float m1 = 0.0f, m2 = 0.0f;
-      const i32x4 lin8 = *(const i32x4*)(p8 + lin_at + 16 * (l >> 4)), gate8 = *(const i32x4*)(p8 + gate_at + 16 * (l >> 4));
+      const i32x4 lin8 = *(const i32x4*)(p8 + 16 * (l >> 4)), gate8 = *(const i32x4*)(p8 + F + 16 * (l >> 4));
 #pragma unroll
       for (int j = 0; j < 2 * TL::FN; ++j) {
         float lin[4], gate[4];

@@ -199,7 +199,7 @@ class _GluMLP8bit(torch.autograd.Function):
 
 
 def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gate_first=False, w1_t=None, w2_t=None):
-    """GLUMLP.forward on weights in 8 bits: x (..., d), expert_p and expert_idxs (tokens, k), w1 (E, 2F, d rounded up to 16) and w2 (E, d, F
+    """GLUMLP.forward on weights in 8 bits: x (..., d), expert_p and expert_idxs (tokens, k) in [0, E), w1 (E, 2F, d rounded up to 16) and w2 (E, d, F
     rounded up to 16) of float8_e4m3fn, the rest zeros, with scales s1, s2 for every 128 x 128, float8_e8m0fnu or float32; biases (E, 2F), (E, d) or
     None of x's type; SiLU on the second half of the first product's columns, on the first when `gate_first`.
 

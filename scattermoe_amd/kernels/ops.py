@@ -1314,7 +1314,7 @@ def dequantize(q, s, block_rows, K, dtype):
 
 
 def glu_8bit_fwd(pre, act=ACT_SILU):
-    """(h, p8, ps): the gated unit of pre (rows, 2F), and the halves of pre in 8 bits (rows, 2, F rounded up to 16) with their scales."""
+    """(h, p8, ps): the gated unit of pre (rows, 2F), and pre's linear and gate half in 8 bits (rows, 2, F rounded up to 16) with their scales."""
     assert pre.dim() == 2 and pre.size(1) % 2 == 0
     pre = _rows_contiguous(pre)
     rows, F = pre.size(0), pre.size(1) // 2

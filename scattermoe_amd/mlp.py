@@ -84,7 +84,7 @@ class _GatedMLP(torch.autograd.Function):
             dh = ops.scatter2scatter(dy, w2.permute(0, 2, 1), eid, idx, 1, x_grouped=True, y_grouped=True, expert_offsets=off)
             dpre, h = ops.glu_8bit_bwd(p8, ps, dh, act, need_h=need_w2 or need_b2)
         elif p8 is not None and (need_w2 or need_b2):
-            h = ops.glu_fwd(ops.dequantize(p8, ps, 1, w2.size(1), dy.dtype).flatten(1), act)
+            h = ops.glu_fwd(ops.dequantize(p8, ps, 1, w2.size(1), dy.dtype).flatten(1), ops.ACT_SILU)
         d_w2 = d_b2 = None
         if need_w2 or need_b2:
             d_w2, d_b2 = ops.group_bwd_W(DY=dy, X=h, expert_offsets=off, E=E, has_bias=b2 is not None, like=w2)

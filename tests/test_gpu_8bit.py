@@ -242,7 +242,7 @@ LAYERS = [
     (1, 1, 1, 32, 16, "any", False, False), (1, 2, 4, 128, 96, "any", True, False), (3, 4, 6, 203, 117, "any", False, True),
     (8, 2, 3, 256, 128, "same", True, False), (33, 2, 5, 130, 203, "gap", True, True), (70, 2, 4, 256, 160, "one", False, False),
     (140, 3, 4, 160, 256, "any", True, False), (0, 2, 3, 64, 32, "any", False, False),
-    (30, 2, 3, 144, 80, "one", True, False), (25, 2, 8, 200, 72, "any", True, True),
+    (45, 2, 4, 144, 96, "any", True, True), (30, 2, 3, 144, 80, "one", True, False), (25, 2, 8, 200, 72, "any", True, True),
     (40, 1, 2, 8208, 128, "any", True, True), (20, 2, 1, 96, 8200, "same", False, False),
 ]
 
