@@ -151,7 +151,7 @@ def parallel_linear_8bit(inputs, weight, weight_scales, k, sorted_expert_idxs, s
     E, N, _ = weight.shape
     rows, K = inputs.shape
     L = sorted_scattered_idxs.numel()
-    if K == 0 or E == 0 or L != (rows if grouped_in and k == 1 else rows * k) or expert_offsets.numel() != E:
+    if K == 0 or N == 0 or E == 0 or L != (rows if grouped_in and k == 1 else rows * k) or expert_offsets.numel() != E:
         raise ValueError("%s: %d rows of %d for %d (token, slot) pairs, k = %d, %d offsets for %d experts"
                          % (what, rows, K, L, k, expert_offsets.numel(), E))
     if grouped_in and k != 1:

@@ -218,12 +218,26 @@ def test_compiled_steps_are_the_eager_ones():
     def step(x, p):
         out = i.forward(x, p)
         pre = eight_bit.parallel_linear_8bit(x, i.w1, i.s1, 2, eid, idx, off, grouped_out=True, weight_t=i.w1_t)
-        return out, eight_bit.checkpointed_glu(pre)
+        return out, eight_bit.checkpointed_glu(pre), eight_bit.dequantize_blocks(*eight_bit.quantize_blocks(x))
     results = []
     for fn in (step, torch.compile(step, fullgraph=True, backend="aot_eager")):
         x, p = i.x.detach().requires_grad_(), i.p.detach().requires_grad_()
-        out, h = fn(x, p)
-        results.append([out.detach(), h.detach(), *torch.autograd.grad((out, h), (x, p), (i.dout, torch.ones_like(h)))])
+        out, h, back = fn(x, p)
+        results.append([out.detach(), h.detach(), back, *torch.autograd.grad((out, h), (x, p), (i.dout, torch.ones_like(h)))])
+    assert _same(*results)
+    torch._dynamo.reset()
+
+
+def test_compiled_step_of_a_gated_layer_with_its_checkpoint():
+    torch.manual_seed(2)
+    with torch.device(DEV):
+        m = GLUMLP(64, 96, 4, 2, checkpoint_8bit=True).bfloat16()
+    x, p = torch.randn(30, 64, device=DEV).bfloat16().requires_grad_(), torch.rand(30, 2, device=DEV).bfloat16()
+    ids = torch.randint(0, 4, (30, 2), device=DEV)
+    results = []
+    for fn in (m, torch.compile(m, fullgraph=True, backend="aot_eager")):
+        out = fn(x, p, ids)
+        results.append([out.detach(), *torch.autograd.grad(out, [x] + list(m.parameters()), torch.ones_like(out))])
     assert _same(*results)
     torch._dynamo.reset()
 

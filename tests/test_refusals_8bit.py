@@ -109,6 +109,11 @@ def test_module_keeps_its_weights_whatever_type_it_is_taken_to():
     assert not list(m.parameters())
 
 
+def test_linear_of_no_columns_is_refused():
+    with pytest.raises(ValueError):
+        _linear(w=torch.zeros(3, 0, 32, dtype=torch.uint8).view(Q8), s=torch.zeros(3, 0, 1, dtype=torch.uint8).view(S8))
+
+
 def test_gated_layer_with_its_checkpoint_is_a_silu_one():
     with pytest.raises(ValueError, match="SiLU"):
         GLUMLP(8, 8, 2, 1, activation=torch.nn.GELU(), checkpoint_8bit=True)
