@@ -76,9 +76,11 @@ static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64
   a.L = (int)L, a.K = (int)K, a.N = (int)N, a.E = E, a.fan = fan, a.x_grouped = x_grouped, a.y_grouped = y_grouped, a.act = act;
   return a;
 }
-// Streams over the weights instead of tiles: us at 2, 4, 8, 12 rows per expert, loads as 1 / rank^0.5, for 8 experts, 4096 -> 14336 71, 77, 80, 82, in tiles
-// 101, 100, 102, 101; 128 experts, 2048 -> 1536 63, 66, 77, 85, tiles 70, 72, 75, 75; 32 experts, 2880 -> 2880 41, 45, 48, 54, tiles 38 to 42.
-static bool few_rows_pay(int64_t L, int E) { return L <= 8 * (int64_t)E && L <= 32768; }   // (a segment per expert or 8 rows: a grid's second side)
+// Streams over the weights instead of tiles, for products that contract K values (the shortest of a layer): us at 2, 4, 8, 12 rows per expert, loads as
+// 1 / rank^0.5: 8 experts, 4096 -> 14336 71, 77, 80, 82, in tiles 101, 100, 102, 101; 16 experts at 10, 12, 15 rows 158, 169, 181, tiles 209, 210, 213;
+// 8 experts, 14336 -> 4096 90, 88, 89, tiles 110, 106, 110; 128 experts, 2048 -> 1536 63, 66, 77, 85, tiles 70, 72, 75, 75; 32 experts, 2880 -> 2880 41, 45,
+// 48, 54, tiles 38 to 42.  (32768 rows: a segment per expert or 8 rows is a grid's second side.)
+static bool few_rows_pay(int64_t L, int64_t K, int E) { return L <= (K >= 4096 ? 12 : 8) * (int64_t)E && L <= 32768; }
 
 }  // namespace smoe
 
@@ -171,7 +173,7 @@ size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, 
   if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
   take_rows(c, !scaled && gathers(L, K, fan_out, x_grouped, false) ? L / fan_out : L, K);
-  if (!few_rows_pay(L, E)) c.take(product_8bit_floats(L, K, N, E, dtype) * 4);
+  if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, dtype) * 4);
   return c.used;
 }
 
@@ -191,7 +193,7 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   const int fan = coeff ? 1 : fan_out;                             // rows of x per row of the product's left side
   const bool copies = !x_grouped && !by_token;
   if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
-  if (few_rows_pay(L, E)) {
+  if (few_rows_pay(L, K, E)) {
     Few8Args a = few(W, b, sbe, sbn, Y, sym, dtype, nullptr, idx, off, L, K, N, E, fan, !by_token, y_grouped, 0);
     if (transposed) a.ssn = W->s_col, a.ssk = W->s_row;
     a.X = x.q, a.sxm = block_row(K), a.XS = x.s;
@@ -207,7 +209,7 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
 enum LayerWay { LAYER_BY_IDS, LAYER_FEW, LAYER_TILES, LAYER_TILES_UNIT };
 static LayerWay layer_way(int64_t L, int64_t d, int64_t F, int E, bool ordered, bool keep) {
   if (!ordered) return LAYER_BY_IDS;
-  if (!keep && few_rows_pay(L, E)) return LAYER_FEW;
+  if (!keep && few_rows_pay(L, d < F ? d : F, E)) return LAYER_FEW;
   return unit_rides(d, F) ? LAYER_TILES_UNIT : LAYER_TILES;
 }
 // the pieces of a gated layer's workspace

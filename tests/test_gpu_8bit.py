@@ -114,6 +114,7 @@ PRODUCTS = [
     (1, 1, 1, 16, 1, "any"), (1, 2, 3, 64, 40, "any"), (5, 3, 13, 203, 117, "any"), (37, 2, 5, 300, 203, "gap"), (64, 4, 8, 128, 256, "any"),
     (130, 1, 2, 129, 257, "any"), (150, 2, 4, 520, 300, "one"), (90, 2, 6, 1000, 72, "same"), (0, 2, 3, 64, 32, "any"), (300, 2, 3, 272, 513, "any"),
     (50, 2, 16, 144, 200, "any"), (24, 4, 12, 208, 72, "same"),                                  # 4 to 8 rows per expert
+    (22, 2, 4, 4104, 136, "any"),                                                                # 11, of a long contraction
     (50, 1, 2, 8400, 260, "any"), (30, 2, 3, 72, 8320, "gap"), (70, 1, 4, 9000, 17, "one"),      # long contractions of few tiles
 ]
 
