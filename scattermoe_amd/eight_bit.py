@@ -223,17 +223,17 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
     if x.requires_grad and torch.is_grad_enabled() and (w1_t is None or w2_t is None):
         raise ValueError("%s: the gradient of x needs w1_t and w2_t, the transposed weights" % what)
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    tokens = x.reshape(T, d)
+    tokens = x if x.dim() == 2 else x.reshape(T, d)                  # (a view would be a node of the backward pass)
     trained = ((x.requires_grad or expert_p.requires_grad) and torch.is_grad_enabled()) or ops.has_tangents(x, expert_p, b1, b2)
     if not trained and T * k <= ops.FEW_ROWS_8BIT:
         out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=ops._as_i64(expert_idxs).contiguous(), act=act)[0]
-        return out.view(x.shape)
+        return out if x.dim() == 2 else out.view(x.shape)
     _, idx, off = flatten_sort_count(expert_idxs, num_experts=E)
     if trained:
         out = _GluMLP8bit.apply(tokens, expert_p, w1, s1, w1_t, b1, w2, s2, w2_t, b2, idx, off, act)
     else:
         out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, order=(idx, off), act=act)[0]
-    return out.view(x.shape)
+    return out if x.dim() == 2 else out.view(x.shape)
 
 
 class _CheckpointedGLU(torch.autograd.Function):
@@ -263,12 +263,14 @@ def checkpointed_glu(pre, gate_first=False):
         raise TypeError("checkpointed_glu: float32, bfloat16 or float16, got %s" % pre.dtype)
     F = pre.size(-1) // 2
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
-    rows = pre.reshape(-1, 2 * F) if F else pre.reshape(pre.shape[:-1].numel(), 0)
+    rows = pre                                                       # (a view would be a node of the backward pass)
+    if pre.dim() != 2:
+        rows = pre.reshape(-1, 2 * F) if F else pre.reshape(pre.shape[:-1].numel(), 0)
     if (pre.requires_grad and torch.is_grad_enabled()) or ops.has_tangents(pre):
         h = _CheckpointedGLU.apply(rows, act)
     else:
         h = ops.glu_fwd(rows, act)
-    return h.view(*pre.shape[:-1], F)
+    return h if pre.dim() == 2 else h.view(*pre.shape[:-1], F)
 
 
 class GLUMLP8bit(nn.Module):
