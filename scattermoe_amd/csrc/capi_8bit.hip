@@ -76,11 +76,11 @@ static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64
   a.L = (int)L, a.K = (int)K, a.N = (int)N, a.E = E, a.fan = fan, a.x_grouped = x_grouped, a.y_grouped = y_grouped, a.act = act;
   return a;
 }
-// Streams over the weights instead of tiles, for products that contract K values (the shortest of a layer): us at 2, 4, 8, 12 rows per expert, loads as
-// 1 / rank^0.5: 8 experts, 4096 -> 14336 71, 77, 80, 82, in tiles 101, 100, 102, 101; 16 experts at 10, 12, 15 rows 158, 169, 181, tiles 209, 210, 213;
-// 8 experts, 14336 -> 4096 90, 88, 89, tiles 110, 106, 110; 128 experts, 2048 -> 1536 63, 66, 77, 85, tiles 70, 72, 75, 75; 32 experts, 2880 -> 2880 41, 45,
-// 48, 54, tiles 38 to 42.  (32768 rows: a segment per expert or 8 rows is a grid's second side.)
-static bool few_rows_pay(int64_t L, int64_t K, int E) { return L <= (K >= 4096 ? 12 : 8) * (int64_t)E && L <= 32768; }
+// Streams over the weights instead of tiles, for products that contract K values (the shortest of a layer).  Layers, us at 2, 4, 6, 8, 11 rows per
+// expert, even loads: 8 experts, 4096 / 14336 249, 255, 260, 265, 268, in tiles of 64 rows 331 from 11 on; 32 experts, 2880 / 2880 -, 180, 196, 199, -,
+// tiles 186, 190, 190; 128 experts, 2048 / 768 127, 141, 158, 166, -, tiles 132, 141, 145, 145.  Products: 16 experts, 4096 -> 14336 at 10, 12, 15 rows
+// 158, 169, 181, tiles 184 and more.  (32768 rows: a segment per expert or 8 rows is a grid's second side.)
+static bool few_rows_pay(int64_t L, int64_t K, int E) { return L <= (K >= 4096 ? 12 : 4) * (int64_t)E && L <= 32768; }
 
 }  // namespace smoe
 

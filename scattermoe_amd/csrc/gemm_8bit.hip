@@ -1,5 +1,5 @@
 // scatter2scatter on 8-bit operands (eight_bit.hpp): Y[dst(n)] = X[src(n)] W[e(n)]^T over rows sorted by expert, in tiles of
-// 128 rows x 256 columns that never straddle two experts.
+// 128 (64) rows x 256 columns that never straddle two experts.
 //
 // A slice of the contraction is 128 values, 128 bytes a row, one block of both operands' scales and one v_mfma_scale_f32_16x16x128:
 // byte for byte the slice of 64 16-bit values of gemm_mfma.hpp, whose operand tiles (DirectOp), tile lookup and order are used as they
@@ -15,11 +15,13 @@
 
 namespace smoe {
 
-typedef Tile<128, 256, 1, 4, 2, false, 3, true> Tile8;               // (3: epilogues derive nothing from the thread's index ahead of the loop)
-typedef DirectOp<Tile8::BM, Tile8::NT> Rows8;
-typedef DirectOp<Tile8::BN, Tile8::NT> Stage8;
-static constexpr int LDS8_B = 2 * Rows8::LDS_BYTES, LDS8 = LDS8_B + Stage8::LDS_BYTES;
-static_assert(LDS8 >= Tile8::BM * Tile8::BN * 2, "the epilogues' 16-bit tile");
+static constexpr int NT8 = 256, BN8 = 256;
+// tiles of 128 rows, two workgroups per CU, or of 64, three (3 below: epilogues derive nothing from the thread's index ahead of the loop)
+template <int BM> using Tile8 = Tile<BM, BN8, 1, 4, 2, false, 3, true>;
+template <class TL> using Rows8 = DirectOp<TL::BM, NT8>;
+typedef DirectOp<BN8, NT8> Stage8;
+template <class TL> static constexpr int LDS8_B = 2 * Rows8<TL>::LDS_BYTES;
+template <class TL> static constexpr int LDS8 = LDS8_B<TL> + Stage8::LDS_BYTES;      // (the epilogues' 16-bit tile is smaller)
 
 __device__ __forceinline__ f32x4 mfma8(i32x8 w, i32x8 x, f32x4 c, int w_scale, int x_scale) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, w_scale, 0, x_scale);
@@ -62,26 +64,25 @@ struct Cols8 {
     turn = rot;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const int p = rnd(j) * Tile8::NT + t, row = p >> 3;
+      const int p = rnd(j) * NT8 + t, row = p >> 3;
       off[j] = (unsigned)row_off(row) + (((p & 7) ^ direct_swz(row)) << 4);
     }
   }
   int turn = 0;            // (see DirectOp)
   __device__ __forceinline__ int rnd(int j) const { const int r = j + turn; return r >= R ? r - R : r; }
   __device__ __forceinline__ void issue_one(unsigned tile, int kt, int j) const {
-    buffer_to_lds16(rsrc, off[j], (unsigned)kt * 128u, tile + wave_uniform_id() * 1024 + rnd(j) * Tile8::NT * 16);
+    buffer_to_lds16(rsrc, off[j], (unsigned)kt * 128u, tile + wave_uniform_id() * 1024 + rnd(j) * NT8 * 16);
   }
 };
 
 // The rows in 8 bits are whole slices long here (zeros behind the last value); sx: this thread's (t < 128) dwords of its row's scales;
 // s_scale: [2][128] dwords of LDS, four slices each.  What is loaded ahead behind the last slice is not looked at.
-template <int SC>
-__device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, char* lds,
-                                              unsigned* s_scale, Block (&acc)[Tile8::FM][Tile8::FN]) {
-  typedef Tile8 TL;
+template <class TL, int SC>
+__device__ __forceinline__ void mainloop_8bit(const Rows8<TL>& A, const Cols8& B, const WeightScales<SC>& W, const uint8_t* sx, int K, char* lds,
+                                              unsigned* s_scale, Block (&acc)[TL::FM][TL::FN]) {
   typedef typename WeightScales<SC>::V V;
-  constexpr int COLS = 2 * TL::FN, LOADS = Rows8::R + Cols8::R, PER_STEP = LOADS / 3;
-  static_assert(LOADS % 3 == 0, "the loads of the next slice go with three quarters of a slice's products");
+  constexpr int COLS = 2 * TL::FN, LOADS = Rows8<TL>::R + Cols8::R, PER_STEP = TL::FM == 4 ? LOADS / 3 : LOADS;
+  static_assert(TL::FM != 4 || LOADS % 3 == 0, "the loads of the next slice go with three quarters of a slice's products, or the first half");
   const int l = lane_id(), t = threadIdx.x, wave = t >> 6;
   const int nk = (K + 127) / 128;
   const unsigned lds_u = lds_address(lds);
@@ -90,12 +91,12 @@ __device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, co
   W.load(0, ws);
   if (t < TL::BM) s_scale[t] = *(const unsigned*)sx;
 #pragma unroll
-  for (int j = 0; j < Rows8::R; ++j) A.issue_one(lds_u, 0, j);
+  for (int j = 0; j < Rows8<TL>::R; ++j) A.issue_one(lds_u, 0, j);
 #pragma unroll
-  for (int j = 0; j < Cols8::R; ++j) B.issue_one(lds_u + LDS8_B, 0, j);
+  for (int j = 0; j < Cols8::R; ++j) B.issue_one(lds_u + LDS8_B<TL>, 0, j);
   auto slice = [&](int kt) {
-    const char* ta = lds + (kt & 1) * Rows8::LDS_BYTES;
-    const unsigned na = lds_u + ((kt & 1) ^ 1) * Rows8::LDS_BYTES;
+    const char* ta = lds + (kt & 1) * Rows8<TL>::LDS_BYTES;
+    const unsigned na = lds_u + ((kt & 1) ^ 1) * Rows8<TL>::LDS_BYTES;
     // this thread's pieces of slice kt have landed, everyone's have, and everyone is done with slice kt - 1
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // (taken here, where nothing is on its way: a wait for them further down would be one for the next slice's pieces)
@@ -103,13 +104,13 @@ __device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, co
     __builtin_amdgcn_sched_barrier(0);
     i32x8 fb[COLS];
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) fb[j] = fragment8<Stage8>(lds + LDS8_B, wave * TL::WTN + j * 16);
+    for (int j = 0; j < COLS; ++j) fb[j] = fragment8<Stage8>(lds + LDS8_B<TL>, wave * TL::WTN + j * 16);
     // (the dword of a fragment's rows is read again for each of its four slices: eight registers less)
     const unsigned* sc = s_scale + ((kt >> 2) & 1) * TL::BM + (l & 15);
     i32x8 fa[2][2];
     unsigned xs[2][2];
     auto rows = [&](int s, int i) {
-      fa[s & 1][i] = fragment8<Rows8>(ta, (2 * s + i) * 16);
+      fa[s & 1][i] = fragment8<Rows8<TL>>(ta, (2 * s + i) * 16);
       xs[s & 1][i] = sc[(2 * s + i) * 16];
     };
 #pragma unroll
@@ -137,7 +138,7 @@ __device__ __forceinline__ void mainloop_8bit(const Rows8& A, const Cols8& B, co
     for (int s = 0; s < TL::FM; ++s) {
 #pragma unroll
       for (int q = s * PER_STEP; q < (s + 1) * PER_STEP && q < LOADS; ++q) {
-        if (q < Cols8::R) B.issue_one(lds_u + LDS8_B, kt + 1, q);
+        if (q < Cols8::R) B.issue_one(lds_u + LDS8_B<TL>, kt + 1, q);
         else A.issue_one(na, (kt + 1) * 64, q - Cols8::R);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -194,10 +195,10 @@ struct ByteTile {
   // ROWS rows to `out`, `ld` bytes apart, `rows` and `cols` (a multiple of 16) of them there
   template <int ROWS>
   static __device__ __forceinline__ void store(const char* lds, uint8_t* out, int64_t ld, int rows, int cols) {
-    const int t = late_thread<Tile8>();
+    const int t = late_thread<Tile8<128>>();
 #pragma unroll
-    for (int p = 0; p < ROWS * (WIDTH / 16) / Tile8::NT; ++p) {
-      const int piece = p * Tile8::NT + t, r = piece / (WIDTH / 16), c = piece % (WIDTH / 16) * 16;
+    for (int p = 0; p < ROWS * (WIDTH / 16) / NT8; ++p) {
+      const int piece = p * NT8 + t, r = piece / (WIDTH / 16), c = piece % (WIDTH / 16) * 16;
       const i32x4 v = *(const i32x4*)(lds + r * ROW + c);
       if (r < rows && c < cols) *(i32x4*)(out + r * ld + c) = v;
     }
@@ -210,11 +211,11 @@ struct ByteTile {
 // gate's half and of columns that are not there for each value, and the scale multiplied in before a conversion without one,
 // 4150 instructions instead of 2660, 1054 instead of 1015 us (4099 tokens, 8 experts, 4096 / 14336; 8192 tokens to 8 of 128
 // experts, 2048 / 768, with the checkpoint: 319, 303).  As a pass over the product's float32 rows: 1065 + 191 us (229 + 90).
-__device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int row0, int rows, int n_tile,
+template <class TL>
+__device__ __forceinline__ void epilogue_unit(Block (&acc)[TL::FM][TL::FN], const Product8Args& a, int row0, int rows, int n_tile,
                                               const float* s_bias, char* lds) {
-  typedef Tile8 TL;
   typedef ByteTile<QB> Bytes;
-  constexpr int PARTS = 2, ROWS = TL::BM / PARTS, FR = ROWS / 16, SIDE = ROWS * Bytes::ROW;
+  constexpr int ROWS = TL::BM == 64 ? 32 : 64, PARTS = TL::BM / ROWS, FR = ROWS / 16, SIDE = ROWS * Bytes::ROW;
   const int t = late_thread<TL>(), wave = t >> 6, l = t & 63, F = a.N / 2, fb = (int)scale_blocks(F);
   const bool mine = n_tile * QB + wave * 32 < F;          // (F is a multiple of 32)
   const int64_t ld = scale_blocks(F) * QB;                         // (hidden rows are whole slices long, zeros behind the last value)
@@ -285,10 +286,10 @@ __device__ __forceinline__ void epilogue_unit(Block (&acc)[Tile8::FM][Tile8::FN]
 // The gated unit's gradient behind a product that is dh.  F is a multiple of 128, so that the blocks of both halves of d(pre) lie in a tile: 256
 // columns of dh, two blocks of each half.  32 rows at a time: the linear half's gradients take dh's registers, the gate's 32 more.
 // 8192 tokens to 8 of 128 experts, 2048 / 768: 222 us, as a pass over the product's float32 rows 229 + 112.
-__device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int row0, int rows, int n0, char* lds) {
-  typedef Tile8 TL;
+template <class TL>
+__device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[TL::FM][TL::FN], const Product8Args& a, int row0, int rows, int n0, char* lds) {
   typedef ByteTile<TL::BN> Bytes;
-  constexpr int PARTS = 4, ROWS = TL::BM / PARTS, FR = ROWS / 16;
+  constexpr int ROWS = 32, PARTS = TL::BM / ROWS, FR = ROWS / 16;
   const int t = late_thread<TL>(), wave = t >> 6, l = t & 63, F = a.N;
   float* top = (float*)(lds + 2 * ROWS * Bytes::ROW);             // [half][wave][row]
   const int swapped = a.act & 1, lin_at = swapped * F, gate_at = F - lin_at;            // the gate's half is the first one
@@ -362,17 +363,16 @@ __device__ __forceinline__ void epilogue_unit_grad(Block (&acc)[Tile8::FM][Tile8
 // in parts 461 + 16 for the sums.  At 4096 values to contract the parts save less than the sums cost (12 tile rows x 16 columns: 78 us, in parts 78 + 15).
 // Bands of 4 and 16 tile rows: 1.00 and 1.01 times the time.
 static constexpr int BAND8 = 8, PARTS8 = 8, PART_SLICES = 16, SPLIT_SLICES = 64, SPLIT_ROUNDS = 8;
-static constexpr int64_t TILE8_FLOATS = Tile8::BM * Tile8::BN;
-template <int SC> static constexpr int round_tiles = SC == SCALES_EXACT ? 256 : 512;
+template <class TL> static constexpr int64_t TILE8_FLOATS = TL::BM * TL::BN;
+template <int SC, int BM> static constexpr int round_tiles = SC == SCALES_EXACT ? 256 : BM == 64 ? 768 : 512;
 struct Share8 {
   int e, row0, rows, row, column;
   int part, parts, slice0, slices;      // the contraction's part, of `parts`; its slices
   int slot;                             // of this part's sums
 };
 // Share number b of a product (JOIN: tile number b of those whose contraction is cut).  The same answer in every wave.
-template <int ROUND, bool JOIN>
+template <int BM, int ROUND, bool JOIN>
 __device__ __forceinline__ bool find_share(const Product8Args& a, int b, int n_tiles, Share8& s) {
-  constexpr int BM = Tile8::BM;
   const int nk = (a.K + QB - 1) / QB;
   const int total = count_tile_rows<BM>(a.off, a.E) * n_tiles;
   int rest = 0;
@@ -445,10 +445,9 @@ __device__ __forceinline__ bool find_share(const Product8Args& a, int b, int n_t
 
 // A tile's sums, rounded, through LDS to its rows: 16-byte pieces, a wave whole 128-byte lines, or value by value where rows do not
 // start at multiples of 16 bytes.  Float32 goes in two halves of 128 columns, the 64 KB of a 16-bit tile.
-template <typename TO>
-__device__ __forceinline__ void store_rows(const Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int n0, const int64_t* s_dst,
+template <class TL, typename TO>
+__device__ __forceinline__ void store_rows(const Block (&acc)[TL::FM][TL::FN], const Product8Args& a, int n0, const int64_t* s_dst,
                                            const float* s_bias, char* lds) {
-  typedef Tile8 TL;
   constexpr int PER = 16 / (int)sizeof(TO), HALVES = (int)sizeof(TO) / 2, COLS = TL::BN / HALVES, CPR = COLS / PER;      // 32 pieces a row
   const int t = late_thread<TL>(), wave = t >> 6, l = t & 63;
   TO* Y = (TO*)a.Y;
@@ -504,13 +503,12 @@ __device__ __forceinline__ void store_rows(const Block (&acc)[Tile8::FM][Tile8::
 }
 
 // What follows a tile's sums: the bias, and the rows or the unit or its gradient
-template <typename TO, int EPI>
-__device__ __forceinline__ void finish(Block (&acc)[Tile8::FM][Tile8::FN], const Product8Args& a, int bias_dtype, int e, int row0, int rows, int n_tile,
+template <class TL, typename TO, int EPI>
+__device__ __forceinline__ void finish(Block (&acc)[TL::FM][TL::FN], const Product8Args& a, int bias_dtype, int e, int row0, int rows, int n_tile,
                                        const int64_t* s_dst, float* s_bias, char* lds) {
-  typedef Tile8 TL;
   const int t = late_thread<TL>(), F = a.N / 2, n0 = n_tile * (EPI == EPI_UNIT ? QB : TL::BN);
   if constexpr (EPI == EPI_UNIT_GRAD) {
-    epilogue_unit_grad(acc, a, row0, rows, n0, lds);
+    epilogue_unit_grad<TL>(acc, a, row0, rows, n0, lds);
   } else {
     // the tile's 256 columns' biases through LDS, zeros without one
     int n = n0 + t;
@@ -522,22 +520,22 @@ __device__ __forceinline__ void finish(Block (&acc)[Tile8::FM][Tile8::FN], const
     }
     s_bias[t] = a.b && there ? bias_value(a.b, e * a.sbe + n * a.sbn, bias_dtype) : 0.0f;
     __syncthreads();
-    if constexpr (EPI == EPI_UNIT) epilogue_unit(acc, a, row0, rows, n_tile, s_bias, lds);
-    else store_rows<TO>(acc, a, n0, s_dst, s_bias, lds);
+    if constexpr (EPI == EPI_UNIT) epilogue_unit<TL>(acc, a, row0, rows, n_tile, s_bias, lds);
+    else store_rows<TL, TO>(acc, a, n0, s_dst, s_bias, lds);
   }
 }
 
 // (float32 rows: the operands as bfloat16 take the registers of a second workgroup)
-template <typename TO, int SC, int EPI>
-__global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product_8bit_kernel(Product8Args a, int bias_dtype, int n_tiles) {
-  typedef Tile8 TL;
-  __shared__ __attribute__((aligned(16))) char lds[LDS8];
+template <typename TO, int SC, int EPI, int BM>
+__global__ __launch_bounds__(NT8, SC == SCALES_EXACT ? 1 : BM == 64 ? 3 : 2) void product_8bit_kernel(Product8Args a, int bias_dtype, int n_tiles) {
+  typedef Tile8<BM> TL;
+  __shared__ __attribute__((aligned(16))) char lds[LDS8<TL>];
   __shared__ unsigned s_scale[2 * TL::BM];
   __shared__ int64_t s_dst[EPI == EPI_ROWS ? TL::BM : 1];
   __shared__ __attribute__((aligned(16))) float s_bias[TL::BN];
   __shared__ int s_src[TL::BM];
   Share8 share;
-  if (!find_share<round_tiles<SC>, false>(a, blockIdx.x, n_tiles, share)) return;
+  if (!find_share<BM, round_tiles<SC, BM>, false>(a, blockIdx.x, n_tiles, share)) return;
   const int e = share.e, row0 = share.row0, rows = share.rows, n_tile = share.column, k0 = share.slice0;
   const int t = threadIdx.x, F = a.N / 2;
   const int n0 = n_tile * (EPI == EPI_UNIT ? QB : TL::BN);         // first output column of the tile (of either half)
@@ -552,8 +550,8 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
     sx = a.XS + src * scale_row(a.K) + k0;
   }
   __syncthreads();
-  Rows8 A;
-  A.rot = (n_tile % BAND8 * Rows8::R / BAND8) % Rows8::R;
+  Rows8<TL> A;
+  A.rot = (n_tile % BAND8 * Rows8<TL>::R / BAND8) % Rows8<TL>::R;
   const int src0 = a.x_grouped ? row0 : 0;
   const int64_t ld = (a.K + QB - 1) / QB * QB;                         // the rows are whole slices long
   A.init((const char*)a.X + src0 * ld + k0 * QB, [&](int row) { return (int64_t)(s_src[row] - src0) * ld; });
@@ -592,11 +590,11 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
   for (int i = 0; i < TL::FM; ++i)
 #pragma unroll
     for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
-  mainloop_8bit<SC>(A, B, W, sx, min(a.K - k0 * QB, share.slices * QB), lds, s_scale, acc);
+  mainloop_8bit<TL, SC>(A, B, W, sx, min(a.K - k0 * QB, share.slices * QB), lds, s_scale, acc);
   if (share.parts > 1) {
     // this part's sums as they lie in the registers (scalar offsets: addresses in registers would have to be held beside them)
     const __amdgpu_buffer_rsrc_t P =
-        __builtin_amdgcn_make_buffer_rsrc((void*)make_uniform((const char*)(a.partial + share.slot * TILE8_FLOATS)), 0, TILE8_FLOATS * 4, 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc((void*)make_uniform((const char*)(a.partial + share.slot * TILE8_FLOATS<TL>)), 0, TILE8_FLOATS<TL> * 4, 0x00020000);
     typedef unsigned u32x4_8b __attribute__((ext_vector_type(4)));
     const int at = late_thread<TL>() * 16;
 #pragma unroll
@@ -609,18 +607,18 @@ __global__ __launch_bounds__(Tile8::NT, SC == SCALES_EXACT ? 1 : 2) void product
     return;
   }
   __syncthreads();
-  finish<TO, EPI>(acc, a, bias_dtype, e, row0, rows, n_tile, s_dst, s_bias, lds);
+  finish<TL, TO, EPI>(acc, a, bias_dtype, e, row0, rows, n_tile, s_dst, s_bias, lds);
 }
 
 // The tiles whose contraction was cut: the parts' sums in their order, and what follows a product
-template <typename TO, int SC, int EPI>
-__global__ __launch_bounds__(Tile8::NT, 2) void product_8bit_join_kernel(Product8Args a, int bias_dtype, int n_tiles) {
-  typedef Tile8 TL;
-  __shared__ __attribute__((aligned(16))) char lds[LDS8];
+template <typename TO, int SC, int EPI, int BM>
+__global__ __launch_bounds__(NT8, 2) void product_8bit_join_kernel(Product8Args a, int bias_dtype, int n_tiles) {
+  typedef Tile8<BM> TL;
+  __shared__ __attribute__((aligned(16))) char lds[LDS8<TL>];
   __shared__ int64_t s_dst[EPI == EPI_ROWS ? TL::BM : 1];
   __shared__ __attribute__((aligned(16))) float s_bias[TL::BN];
   Share8 share;
-  if (!find_share<round_tiles<SC>, true>(a, blockIdx.x, n_tiles, share)) return;
+  if (!find_share<BM, round_tiles<SC, BM>, true>(a, blockIdx.x, n_tiles, share)) return;
   const int t = threadIdx.x;
   if (EPI == EPI_ROWS && t < TL::BM)
     s_dst[t] = t < share.rows ? (a.y_grouped ? (int64_t)(share.row0 + t) : a.idx[share.row0 + t]) * a.sym : -1;
@@ -630,7 +628,7 @@ __global__ __launch_bounds__(Tile8::NT, 2) void product_8bit_join_kernel(Product
 #pragma unroll
     for (int j = 0; j < TL::FN; ++j) acc[i][j].clear();
   for (int p = 0; p < share.parts; ++p) {
-    const f32x4* P = (const f32x4*)(a.partial + (share.slot + p) * TILE8_FLOATS) + t;
+    const f32x4* P = (const f32x4*)(a.partial + (share.slot + p) * TILE8_FLOATS<TL>) + t;
 #pragma unroll
     for (int i = 0; i < TL::FM; ++i)
 #pragma unroll
@@ -639,33 +637,40 @@ __global__ __launch_bounds__(Tile8::NT, 2) void product_8bit_join_kernel(Product
         for (int g = 0; g < 4; ++g) acc[i][j].q[g] += P[((i * TL::FN + j) * 4 + g) * TL::NT];
   }
   __syncthreads();
-  finish<TO, EPI>(acc, a, bias_dtype, share.e, share.row0, share.rows, share.column, s_dst, s_bias, lds);
+  finish<TL, TO, EPI>(acc, a, bias_dtype, share.e, share.row0, share.rows, share.column, s_dst, s_bias, lds);
 }
 
-template <typename TO, int SC, int EPI>
+template <typename TO, int SC, int EPI, int BM>
 static int launch_product(const Product8Args& a, int bias_dtype, int n_tiles, hipStream_t st) {
-  constexpr int ROUND = round_tiles<SC>;
+  constexpr int ROUND = round_tiles<SC, BM>;
   // every share of the most tiles that the rows can make, and a round of parts
-  const int64_t tiles = max_tiles(a.L, a.E, Tile8::BM) * n_tiles;
+  const int64_t tiles = max_tiles(a.L, a.E, BM) * n_tiles;
   const int64_t grid = (tiles + ROUND - 1) / ROUND * ROUND + (a.partial ? ROUND : 0);
   if (grid > 0x7fffff00LL) { set_error("product_8bit: grid too large"); return SMOE_ERR_RANGE; }
-  product_8bit_kernel<TO, SC, EPI><<<(unsigned)grid, Tile8::NT, 0, st>>>(a, bias_dtype, n_tiles);
-  if (a.partial) product_8bit_join_kernel<TO, SC, EPI><<<ROUND / 2, Tile8::NT, 0, st>>>(a, bias_dtype, n_tiles);
+  product_8bit_kernel<TO, SC, EPI, BM><<<(unsigned)grid, NT8, 0, st>>>(a, bias_dtype, n_tiles);
+  if (a.partial) product_8bit_join_kernel<TO, SC, EPI, BM><<<ROUND / 2, NT8, 0, st>>>(a, bias_dtype, n_tiles);
   return launch_status("product_8bit");
 }
+// Tiles of 64 rows instead of 128: a third workgroup per CU waits for its weights beside two others.  us in tiles of 128 -> 64 at 16, 32, 64, 128
+// rows per expert, even and as 1 / rank^0.5: 8 experts, 4096 -> 28672 214 -> 185, 215 -> 187, 220 -> 190, 230 -> 237 and 213 -> 184, 214 -> 184, 219 ->
+// 223, 217 -> 248; 128 experts, 2048 -> 1536 80 -> 67, 87 -> 76, 95 -> 86, 106 -> 111 and 79 -> 85, 85 -> 89, 93 -> 104, 119 -> 123; 32 experts,
+// 2880 -> 5760 115 -> 104, 120 -> 107, 133 -> 118, 148 -> 162 and 117 -> 106, 117 -> 132, 131 -> 161, 170 -> 180.
+static bool low_tiles(int64_t L, int E) { return L <= 24 * (int64_t)E; }
 template <typename TO, bool EXACT, int EPI>
 static int launch_product(const Product8Args& a, int bias_dtype, hipStream_t st) {
-  const int n_tiles = EPI == EPI_UNIT ? (a.N / 2 + QB - 1) / QB : (a.N + Tile8::BN - 1) / Tile8::BN;
-  if constexpr (EXACT) return launch_product<TO, SCALES_EXACT, EPI>(a, bias_dtype, n_tiles, st);
-  else return a.ws_f32 ? launch_product<TO, SCALES_FLOAT, EPI>(a, bias_dtype, n_tiles, st) : launch_product<TO, SCALES_BYTES, EPI>(a, bias_dtype, n_tiles, st);
+  const int n_tiles = EPI == EPI_UNIT ? (a.N / 2 + QB - 1) / QB : (a.N + BN8 - 1) / BN8;
+  if constexpr (EXACT) return launch_product<TO, SCALES_EXACT, EPI, 128>(a, bias_dtype, n_tiles, st);
+  else if (low_tiles(a.L, a.E)) return a.ws_f32 ? launch_product<TO, SCALES_FLOAT, EPI, 64>(a, bias_dtype, n_tiles, st) : launch_product<TO, SCALES_BYTES, EPI, 64>(a, bias_dtype, n_tiles, st);
+  else return a.ws_f32 ? launch_product<TO, SCALES_FLOAT, EPI, 128>(a, bias_dtype, n_tiles, st) : launch_product<TO, SCALES_BYTES, EPI, 128>(a, bias_dtype, n_tiles, st);
 }
 
 int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, int row_dtype) {
-  const int64_t round = row_dtype == SMOE_F32 ? round_tiles<SCALES_EXACT> : round_tiles<SCALES_BYTES>;
-  const int64_t tiles = max_tiles(L, E, Tile8::BM) * ((columns + Tile8::BN - 1) / Tile8::BN);
+  const bool exact = row_dtype == SMOE_F32, low = !exact && low_tiles(L, E);
+  const int64_t round = exact ? round_tiles<SCALES_EXACT, 128> : low ? round_tiles<SCALES_BYTES, 64> : round_tiles<SCALES_BYTES, 128>;
+  const int64_t tiles = max_tiles(L, E, low ? 64 : 128) * ((columns + BN8 - 1) / BN8);
   if ((K + QB - 1) / QB < SPLIT_SLICES || tiles > SPLIT_ROUNDS * round) return 0;
   const int64_t slots = tiles * PARTS8 < round ? tiles * PARTS8 : round;
-  return slots * TILE8_FLOATS;
+  return slots * (low ? TILE8_FLOATS<Tile8<64>> : TILE8_FLOATS<Tile8<128>>);
 }
 
 // The unit's blocks are 128 hidden columns, and a wave's 32 of either half have one scale of the weights; its weight rows are

@@ -115,6 +115,7 @@ PRODUCTS = [
     (130, 1, 2, 129, 257, "any"), (150, 2, 4, 520, 300, "one"), (90, 2, 6, 1000, 72, "same"), (0, 2, 3, 64, 32, "any"), (300, 2, 3, 272, 513, "any"),
     (50, 2, 16, 144, 200, "any"), (24, 4, 12, 208, 72, "same"),                                  # 4 to 8 rows per expert
     (22, 2, 4, 4104, 136, "any"),                                                                # 11, of a long contraction
+    (300, 1, 2, 8208, 100, "any"), (400, 2, 3, 144, 264, "gap"),                                   # 150 and 270 rows per expert
     (50, 1, 2, 8400, 260, "any"), (30, 2, 3, 72, 8320, "gap"), (70, 1, 4, 9000, 17, "one"),      # long contractions of few tiles
 ]
 
@@ -244,6 +245,7 @@ LAYERS = [
     (8, 2, 3, 256, 128, "same", True, False), (33, 2, 5, 130, 203, "gap", True, True), (70, 2, 4, 256, 160, "one", False, False),
     (140, 3, 4, 160, 256, "any", True, False), (0, 2, 3, 64, 32, "any", False, False),
     (45, 2, 4, 144, 96, "any", True, True), (30, 2, 3, 144, 80, "one", True, False), (25, 2, 8, 200, 72, "any", True, True),
+    (200, 2, 2, 144, 384, "any", True, True), (60, 1, 2, 8208, 128, "any", False, True), (150, 2, 3, 200, 96, "any", False, False),
     (40, 1, 2, 8208, 128, "any", True, True), (20, 2, 1, 96, 8200, "same", False, False),
 ]
 
