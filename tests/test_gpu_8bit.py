@@ -244,6 +244,7 @@ LAYERS = [
     (1, 1, 1, 32, 16, "any", False, False), (1, 2, 4, 128, 96, "any", True, False), (3, 4, 6, 203, 117, "any", False, True),
     (8, 2, 3, 256, 128, "same", True, False), (33, 2, 5, 130, 203, "gap", True, True), (70, 2, 4, 256, 160, "one", False, False),
     (140, 3, 4, 160, 256, "any", True, False), (0, 2, 3, 64, 32, "any", False, False),
+    (16, 2, 8, 144, 80, "one", True, False), (10, 4, 12, 203, 117, "same", False, True), (32, 2, 3, 136, 200, "any", True, True),
     (45, 2, 4, 144, 96, "any", True, True), (30, 2, 3, 144, 80, "one", True, False), (25, 2, 8, 200, 72, "any", True, True),
     (200, 2, 2, 144, 384, "any", True, True), (60, 1, 2, 8208, 128, "any", False, True), (150, 2, 3, 200, 96, "any", False, False),
     (40, 1, 2, 8208, 128, "any", True, True), (20, 2, 1, 96, 8200, "same", False, False),
@@ -275,6 +276,10 @@ def test_layer_and_its_gradients(dtype, float_scales, T, k, E, d, F, kind, bias,
     for name, got, (v, bound) in zip(("out", "dx", "dgates"), (out, dx, dp), want):
         ref.check(name, got, v, bound)
     ref.check("out, forward only", plain, *want[0])
+    if T * k <= ops.FEW_ROWS_8BIT:
+        act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
+        by_ids = ops.glu_mlp_8bit(up(x), up(p), q1, s1, up(b1), q2, s2, up(b2), experts=up(ids), act=act)[0]
+        ref.check("out, by the ids", by_ids, *want[0])
     (dp2,) = torch.autograd.grad(call(xg.detach(), pg), pg, up(dout))      # gates alone: no transposed weights
     ref.check("dgates alone", dp2, *want[2])
 
