@@ -22,9 +22,13 @@ struct Carver {
 };
 
 // Rows of 8-bit activations of a product of L rows that come by token: the tokens once, or once per slot where those are scaled, and the product looks
-// them up; a copy for each row, in the rows' order, where they pass the 32-bit offsets of a look-up
-static bool gathers(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
-  return !x_grouped && (scaled ? L : L / fan) * block_row(K) < (1LL << 32);
+// them up; a copy for each row, in the rows' order, where they pass the 32-bit offsets of a look-up.  All entry points ask here: the
+// number of rows does not tell the ways apart (at one expert per token both have L).
+struct SourceRows { bool looked_up; int64_t rows; };
+static SourceRows source_rows(int64_t L, int64_t K, int fan, int x_grouped, bool scaled) {
+  const int64_t held = scaled || x_grouped ? L : L / fan;
+  const bool looked_up = !x_grouped && held * block_row(K) < (1LL << 32);
+  return {looked_up, looked_up ? held : L};
 }
 static float* take_partial(Carver& c, int64_t floats) { return floats ? c.take<float>(floats * 4) : nullptr; }
 struct Rows8Bit { uint8_t* q; uint8_t* s; int64_t rows; };
@@ -172,7 +176,7 @@ static int workspace_check(const char* who, size_t need, const void* workspace, 
 size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, int fan_out, int x_grouped, int scaled, int dtype) {
   if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
-  take_rows(c, !scaled && gathers(L, K, fan_out, x_grouped, false) ? L / fan_out : L, K);
+  take_rows(c, source_rows(L, K, fan_out, x_grouped, scaled != 0).rows, K);
   if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, dtype) * 4);
   return c.used;
 }
@@ -188,8 +192,9 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   if (int rc = weight_checks("smoe_linear_8bit", W, transposed ? K : N, transposed ? N : K)) return rc;
   if (int rc = workspace_check("smoe_linear_8bit", smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out, x_grouped, coeff != nullptr, dtype), workspace, workspace_bytes)) return rc;
   Carver c{(char*)workspace};
-  const bool by_token = gathers(L, K, fan_out, x_grouped, coeff != nullptr);
-  const Rows8Bit x = take_rows(c, by_token && !coeff ? L / fan_out : L, K);
+  const SourceRows from = source_rows(L, K, fan_out, x_grouped, coeff != nullptr);
+  const bool by_token = from.looked_up;
+  const Rows8Bit x = take_rows(c, from.rows, K);
   const int fan = coeff ? 1 : fan_out;                             // rows of x per row of the product's left side
   const bool copies = !x_grouped && !by_token;
   if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
@@ -213,7 +218,7 @@ static LayerWay layer_way(int64_t L, int64_t d, int64_t F, int E, bool ordered, 
   return unit_rides(d, F) ? LAYER_TILES_UNIT : LAYER_TILES;
 }
 // the pieces of a gated layer's workspace
-struct LayerPieces { Rows8Bit x, h; float* pre; float* hidden; float* rows; float* partial1; float* partial2; };
+struct LayerPieces { Rows8Bit x, h; bool by_token; float* pre; float* hidden; float* rows; float* partial1; float* partial2; };
 static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64_t d, int64_t F, int E, int dtype) {
   LayerPieces p{};
   if (way == LAYER_BY_IDS) {
@@ -221,7 +226,9 @@ static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64
     p.rows = c.take<float>(L * d * 4);
     return p;
   }
-  p.x = take_rows(c, gathers(L, d, k, 0, false) ? L / k : L, d);
+  const SourceRows from = source_rows(L, d, k, 0, false);
+  p.by_token = from.looked_up;
+  p.x = take_rows(c, from.rows, d);
   p.h = take_rows(c, L, F);
   if (way == LAYER_FEW) p.hidden = c.take<float>(L * F * 4);
   if (way == LAYER_TILES) p.pre = c.take<float>(L * 2 * F * 4);
@@ -269,7 +276,7 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
     if (int rc = launch_few_rows_8bit(a, SMOE_F32, dtype, EPI_ROWS, st)) return rc;
     return launch_few_combine(p.rows, gates, experts, OUT, (int)T, k, (int)d, E, dtype, st);
   }
-  const bool by_token = p.x.rows != L || k == 1;
+  const bool by_token = p.by_token;
   if (int rc = quantize(p.x, X, sxm, by_token ? nullptr : idx, k, nullptr, d, dtype, st)) return rc;
   if (way == LAYER_FEW) {
     Few8Args a = few(W1, b1, sb1e, sb1n, p.hidden, F, SMOE_F32, nullptr, idx, off, L, d, 2 * F, E, k, !by_token, 1, act);
@@ -297,10 +304,12 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
 }
 
-struct BackPieces { Rows8Bit dy, dp; float* dh; float* partial1; float* partial2; };
-static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F, int E, int dtype) {
+struct BackPieces { Rows8Bit dy, dp; bool by_slot; float* dh; float* partial1; float* partial2; };
+static BackPieces back_pieces(Carver& c, int64_t L, int k, int64_t d, int64_t F, int E, int dtype) {
   BackPieces p{};
-  p.dy = take_rows(c, L, d);
+  const SourceRows from = source_rows(L, d, k, 0, true);
+  p.by_slot = from.looked_up;
+  p.dy = take_rows(c, from.rows, d);
   p.dp = take_rows(c, L, 2 * F);
   p.dh = unit_grad_rides(F) ? nullptr : c.take<float>(L * F * 4);
   const int64_t one = product_8bit_floats(L, d, F, E, dtype), two = product_8bit_floats(L, 2 * F, d, E, dtype);
@@ -311,7 +320,7 @@ static BackPieces back_pieces(Carver& c, int64_t L, int64_t d, int64_t F, int E,
 size_t smoe_glu_mlp_8bit_bwd_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int dtype) {
   if (T <= 0 || k <= 0 || d <= 0 || F <= 0 || E <= 0) return 0;
   Carver c{nullptr};
-  back_pieces(c, T * k, d, F, E, dtype);
+  back_pieces(c, T * k, k, d, F, E, dtype);
   return c.used;
 }
 
@@ -331,8 +340,8 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   if (int rc = workspace_check("smoe_glu_mlp_8bit_bwd", smoe_glu_mlp_8bit_bwd_workspace_bytes(T, k, d, F, E, dtype), workspace, workspace_bytes)) return rc;
   const int64_t L = T * k;
   Carver c{(char*)workspace};
-  const BackPieces p = back_pieces(c, L, d, F, E, dtype);
-  const bool by_slot = gathers(L, d, k, 0, true);
+  const BackPieces p = back_pieces(c, L, k, d, F, E, dtype);
+  const bool by_slot = p.by_slot;
   if (int rc = quantize(p.dy, DOUT, sdm, by_slot ? nullptr : idx, k, gates, d, dtype, st)) return rc;
   Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, !by_slot, 1);
   a.partial = p.partial1;
