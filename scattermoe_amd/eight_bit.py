@@ -299,6 +299,10 @@ class GLUMLP8bit(nn.Module):
         if type(getattr(module, "activation", None)) is not nn.SiLU:
             raise ValueError("GLUMLP8bit: the activation has to be SiLU")
         w1, w2 = module.experts.weight, module.output_experts.weight
+        E, d, f = module.num_experts, module.input_size, module.hidden_size
+        if w1.shape != (E, 2 * f, d) or w2.shape != (E, d, f):
+            raise ValueError("GLUMLP8bit: a gated layer of %d experts has weights (E, 2F, d) = %s and (E, d, F) = %s, got %s, %s"
+                             % (E, (E, 2 * f, d), (E, d, f), tuple(w1.shape), tuple(w2.shape)))
         m = cls(module.input_size, module.hidden_size, module.num_experts, module.top_k, bias=module.experts.bias is not None,
                 dtype=w1.dtype, input_gradients=input_gradients)
         m.w1, m.s1, m.w1_t = ops.quantize_weights(w1.detach(), input_gradients)
