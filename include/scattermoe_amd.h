@@ -450,25 +450,36 @@ typedef struct {
 } smoe_weight_8bit;
 
 /*
- * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, summed in float32 and rounded once to `dtype`; rows as for
+ * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, rounded once to `dtype`, or float32 where dtype is or-ed with
+ * SMOE_8BIT_Y_FLOAT32 (rows that are added up afterwards: smoe_combine_f32); rows as for
  * smoe_scatter2scatter.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
  * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out,
  * x_grouped, coeff != NULL, dtype) bytes, 256-byte aligned; nothing in it is read before it is written; calls that overlap in time need one each.
  */
+#define SMOE_8BIT_Y_FLOAT32 0x100
 size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, int fan_out, int x_grouped, int scaled, int dtype);
 int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_weight_8bit* W, int transposed, const void* b, int64_t sbe,
                      int64_t sbn, void* Y, int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E,
                      int fan_out, int x_grouped, int y_grouped, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * out[t] = sum_j gates[t,j] Y[t k + j] and dgates[t,j] = <Y[t k + j], dOut[t]> as smoe_combine and smoe_gate_grad have them, of float32 rows Y; gates
+ * (NULL: the sum), out, dOut and dgates of `dtype`.  experts (T,k) contiguous, or NULL: a slot whose id lies outside [0,E) is left out.
+ */
+int smoe_combine_f32(const void* Y, int64_t sym, const void* gates, int64_t sgt, int64_t sgk, const int64_t* experts, int E, void* out, int64_t som,
+                     int64_t T, int k, int64_t N, int dtype, void* stream);
+int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm, void* dgates, int64_t sgt, int64_t sgk, int64_t T, int k, int64_t N,
+                       int dtype, void* stream);
+
+/*
  * A gated layer on such weights (GLUMLP.forward, scattermoe/mlp.py:74-95):
  *   pre = Q(X) W1[e]^T + b1[e];  y = Q(glu(pre)) W2[e]^T + b2[e];  OUT[t] = sum_j gates[t,j] y
- * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) by slot (y, rounded), OUT (T,d)
+ * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) float32 by slot (y), OUT (T,d)
  * contiguous; P8 (16-byte aligned), PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
  * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
  * alone, and ids outside [0,E) drop their row.
  * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with
- * the scales of the weights; DROWS (T k, d): what every slot adds to DX (T,d).  Workspaces as above.
+ * the scales of the weights; DROWS (T k, d) float32: what every slot adds to DX (T,d).  Workspaces as above.
  */
 #define SMOE_8BIT_FEW_ROWS 64
 size_t smoe_glu_mlp_8bit_workspace_bytes(int64_t T, int k, int64_t d, int64_t F, int E, int ordered, int keep, int dtype);

@@ -23,6 +23,8 @@ _INDEX_CODES = {torch.int64: I64, torch.int32: I32, torch.int16: I16, torch.uint
 _p, _i64, _int, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 
+Y_FLOAT32_8BIT = 0x100         # SMOE_8BIT_Y_FLOAT32
+
 
 class Weight8bit(ctypes.Structure):
     """smoe_weight_8bit"""
@@ -89,6 +91,8 @@ _SIGNATURES = {
     "smoe_linear_8bit_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int, _int, _int, _int]),
     "smoe_linear_8bit": (_int, [_p, _i64, _p, _w8, _int, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _int, _int, _int, _int, _int,
                                 _p, _sz, _p]),
+    "smoe_combine_f32": (_int, [_p, _i64, _p, _i64, _i64, _p, _int, _p, _i64, _i64, _int, _i64, _int, _p]),
+    "smoe_gate_grad_f32": (_int, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _int, _i64, _int, _p]),
     "smoe_glu_mlp_8bit_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _int, _int, _int, _int]),
     "smoe_glu_mlp_8bit": (_int, [_p, _i64, _p, _p, _w8, _p, _i64, _i64, _w8, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _int, _i64, _i64,
                                  _int, _int, _int, _p, _sz, _p]),

@@ -185,6 +185,8 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
                      int64_t sbn, void* Y, int64_t sym, const int64_t* idx, const int64_t* off, int64_t L, int64_t K, int64_t N, int E,
                      int fan_out, int x_grouped, int y_grouped, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   set_error("%s", "");
+  const int out_dtype = dtype & SMOE_8BIT_Y_FLOAT32 ? SMOE_F32 : dtype;
+  dtype &= ~SMOE_8BIT_Y_FLOAT32;
   if (int rc = product_checks("smoe_linear_8bit", L, K, N, E, fan_out, dtype)) return rc;
   if (L == 0 || N == 0) return 0;
   if (!X || !Y || !idx || !off) { set_error("smoe_linear_8bit: NULL pointer"); return SMOE_ERR_NULL; }
@@ -199,14 +201,36 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   const bool copies = !x_grouped && !by_token;
   if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
   if (few_rows_pay(L, K, E)) {
-    Few8Args a = few(W, b, sbe, sbn, Y, sym, dtype, nullptr, idx, off, L, K, N, E, fan, !by_token, y_grouped, 0);
+    Few8Args a = few(W, b, sbe, sbn, Y, sym, out_dtype, nullptr, idx, off, L, K, N, E, fan, !by_token, y_grouped, 0);
     if (transposed) a.ssn = W->s_col, a.ssk = W->s_row;
     a.X = x.q, a.sxm = block_row(K), a.XS = x.s;
     return launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, (hipStream_t)stream);
   }
   Product8Args a = product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan, !by_token, y_grouped);
   a.partial = take_partial(c, product_8bit_floats(L, K, N, E, dtype));
-  return launch_product_8bit(a, dtype, dtype, (hipStream_t)stream);
+  return launch_product_8bit(a, dtype, out_dtype, (hipStream_t)stream);
+}
+
+int smoe_combine_f32(const void* Y, int64_t sym, const void* gates, int64_t sgt, int64_t sgk, const int64_t* experts, int E, void* out, int64_t som,
+                     int64_t T, int k, int64_t N, int dtype, void* stream) {
+  set_error("%s", "");
+  if (!float_type(dtype)) { set_error("smoe_combine_f32: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (T < 0 || k <= 0 || N < 0 || (experts && E <= 0)) { set_error("smoe_combine_f32: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (T > 0x7fffffffLL || N > MOST) { set_error("smoe_combine_f32: size beyond int32"); return SMOE_ERR_RANGE; }
+  if (T == 0 || N == 0) return 0;
+  if (!Y || !out) { set_error("smoe_combine_f32: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_slots_combine((const float*)Y, sym, gates, sgt, sgk, experts, E, out, som, T, k, (int)N, dtype, (hipStream_t)stream);
+}
+
+int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm, void* dgates, int64_t sgt, int64_t sgk, int64_t T, int k, int64_t N,
+                       int dtype, void* stream) {
+  set_error("%s", "");
+  if (!float_type(dtype)) { set_error("smoe_gate_grad_f32: unknown dtype %d", dtype); return SMOE_ERR_DTYPE; }
+  if (T < 0 || k <= 0 || N < 0) { set_error("smoe_gate_grad_f32: bad sizes"); return SMOE_ERR_SHAPE; }
+  if (T > 0x7fffffffLL || T * k > 0x7fffffffLL || N > MOST) { set_error("smoe_gate_grad_f32: size beyond int32"); return SMOE_ERR_RANGE; }
+  if (T == 0) return 0;
+  if (!dgates || (N > 0 && (!Y || !dOut))) { set_error("smoe_gate_grad_f32: NULL pointer"); return SMOE_ERR_NULL; }
+  return launch_slots_gate_grad((const float*)Y, sym, dOut, sdm, dgates, sgt, sgk, T, k, (int)N, dtype, (hipStream_t)stream);
 }
 
 // How a layer goes.  Without an order of its rows: by their ids, two streams over the weights of the experts that they name.  Few rows per
@@ -283,10 +307,10 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
     a.X = p.x.q, a.sxm = block_row(d), a.XS = p.x.s;
     if (int rc = launch_few_rows_8bit(a, -1, dtype, EPI_UNIT, st)) return rc;
     if (int rc = quantize(p.h, p.hidden, F, nullptr, 1, nullptr, F, SMOE_F32, st)) return rc;
-    a = few(W2, b2, sb2e, sb2n, Y, d, dtype, nullptr, idx, off, L, F, d, E, 1, 1, 0, act);
+    a = few(W2, b2, sb2e, sb2n, Y, d, SMOE_F32, nullptr, idx, off, L, F, d, E, 1, 1, 0, act);
     a.X = p.h.q, a.sxm = block_row(F), a.XS = p.h.s;
     if (int rc = launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, st)) return rc;
-    return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
+    return launch_slots_combine((const float*)Y, d, gates, k, 1, experts, E, OUT, d, T, k, (int)d, dtype, st);
   }
   Product8Args a = product(p.x, W1, false, b1, sb1e, sb1n, p.pre, 2 * F, idx, off, L, d, 2 * F, E, k, !by_token, 1);
   a.partial = p.partial1;
@@ -300,8 +324,8 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   }
   a = product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0);
   a.partial = p.partial2;
-  if (int rc = launch_product_8bit(a, dtype, dtype, st)) return rc;
-  return launch_combine(Y, d, gates, k, 1, OUT, d, T, k, (int)d, dtype, st);
+  if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st)) return rc;
+  return launch_slots_combine((const float*)Y, d, gates, k, 1, experts, E, OUT, d, T, k, (int)d, dtype, st);
 }
 
 struct BackPieces { Rows8Bit dy, dp; bool by_slot; float* dh; float* partial1; float* partial2; };
@@ -355,8 +379,8 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   }
   a = product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0);
   a.partial = p.partial2;
-  if (int rc = launch_product_8bit(a, dtype, dtype, st)) return rc;
-  return launch_combine(DROWS, d, nullptr, 0, 0, DX, d, T, k, (int)d, dtype, st);
+  if (int rc = launch_product_8bit(a, dtype, SMOE_F32, st)) return rc;
+  return launch_slots_combine((const float*)DROWS, d, nullptr, 0, 0, nullptr, E, DX, d, T, k, (int)d, dtype, st);
 }
 
 }  // extern "C"

@@ -190,6 +190,12 @@ struct Few8Args {
   int L, K, N, E, fan, x_grouped, y_grouped, act;
 };
 int launch_few_rows_8bit(const Few8Args& a, int x_dtype, int dtype, int epilogue, hipStream_t st);      // x_dtype -1: 8 bits
+// What follows the experts' float32 rows (csrc/slots_f32.hip): out[t] = sum_j G[t, j] Y[t k + j] (G NULL: the sum; ids, or NULL: slots outside [0, E) are left
+// out), and the gates' gradient <Y[t k + j], D[t]>
+int launch_slots_combine(const float* Y, int64_t sy, const void* G, int64_t sgt, int64_t sgk, const int64_t* ids, int E, void* O, int64_t so, int64_t Tn,
+                         int k, int N, int dtype, hipStream_t st);
+int launch_slots_gate_grad(const float* Y, int64_t sy, const void* D, int64_t sd, void* DG, int64_t sgt, int64_t sgk, int64_t Tn, int k, int N, int dtype,
+                           hipStream_t st);
 int launch_few_combine(const float* rows, const void* gates, const int64_t* ids, void* out, int T, int k, int d, int E, int dtype, hipStream_t st);
 __device__ __forceinline__ float bias_value(const void* b, int64_t at, int dtype) {
   if (dtype == SMOE_BF16) return to_f32(((const bf16_t*)b)[at]);

@@ -104,11 +104,11 @@ class _Linear8bit(torch.autograd.Function):
     @staticmethod
     def rows(x, gates, w, s, b, idx, off, k, grouped_in, grouped_out):
         """(y, the experts' rows where gates weigh them)"""
-        y = ops.linear_8bit(x, w, s, idx, off, k, b=b, x_grouped=grouped_in, y_grouped=grouped_out)
+        y = ops.linear_8bit(x, w, s, idx, off, k, b=b, x_grouped=grouped_in, y_grouped=grouped_out, dtype=None if gates is None else torch.float32)
         if gates is None:
             return y, None
         kept = y.view(gates.size(0), gates.size(1), y.size(1))
-        return ops.combine(kept, gates), kept
+        return ops.combine(kept, gates, dtype=x.dtype), kept
 
     @staticmethod
     def forward(ctx, x, gates, w, s, wt, b, idx, off, k, grouped_in, grouped_out):
@@ -131,8 +131,9 @@ class _Linear8bit(torch.autograd.Function):
             fan, coeff = 1, None
             if gates is not None:
                 fan, coeff = gates.size(1), gates.to(dy.dtype).contiguous()
-            d_rows = ops.linear_8bit(dy, wt, s, idx, off, fan, coeff=coeff, transposed=True, x_grouped=grouped_out, y_grouped=grouped_in)
-            dx = ops.slot_sum(d_rows, ctx.rows, ctx.k)
+            d_rows = ops.linear_8bit(dy, wt, s, idx, off, fan, coeff=coeff, transposed=True, x_grouped=grouped_out, y_grouped=grouped_in,
+                                     dtype=dy.dtype if ctx.k == 1 else torch.float32)
+            dx = ops.slot_sum(d_rows, ctx.rows, ctx.k, dtype=dy.dtype)
         return dx, d_gates, None, None, None, None, None, None, None, None, None
 
 
@@ -140,8 +141,8 @@ def parallel_linear_8bit(inputs, weight, weight_scales, k, sorted_expert_idxs, s
                          expert_biases=None, gates=None, grouped_in=False, grouped_out=False, weight_t=None):
     """`parallel_linear` on weights in 8 bits: inputs (tokens, K), or (rows, K) with `grouped_in`, float32, bfloat16 or float16, are taken to
     8 bits with a scale for every 128 of a row, multiplied by weight (E, N, K rounded up to 16, the rest zeros) of float8_e4m3fn with weight_scales
-    (E, ceil(N / 128), ceil(K / 128)) of float8_e8m0fnu or float32, summed in float32 and rounded once.  Biases (E, N) and gates (tokens, k) of
-    the inputs' type.  Routing as for `parallel_linear`; gates go with `grouped_out=False`.
+    (E, ceil(N / 128), ceil(K / 128)) of float8_e8m0fnu or float32, and rounded once: rows that gates weigh, and the gradients of a token's
+    slots, are added up in float32.  Biases (E, N) and gates (tokens, k) of the inputs' type.  Routing as for `parallel_linear`; gates go with `grouped_out=False`.
 
     Weights, scales and biases are constants.  The inputs' gradient, Q(gate dy) W, needs weight_t (E, K, N rounded up to 16), the transposed
     weight (`quantize_blocks(w, 128, transposed=True)`); gates have theirs without it."""
@@ -203,8 +204,8 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
     rounded up to 16) of float8_e4m3fn, the rest zeros, with scales s1, s2 for every 128 x 128, float8_e8m0fnu or float32; biases (E, 2F), (E, d) or
     None of x's type; SiLU on the second half of the first product's columns, on the first when `gate_first`.
 
-    The tokens and the hidden rows are taken to 8 bits; pre-activations and sums stay in float32, the experts' rows are rounded to x's type before
-    they are weighted.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
+    The tokens and the hidden rows are taken to 8 bits; pre-activations, the experts' rows and sums stay in float32, and the result is rounded
+    once.  expert_p is taken to x's type.  A step that asks for the gradient of expert_p keeps the experts' rows in float32.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
     rounded up to 16) and w2_t (E, F, d rounded up to 16); the step then keeps the pre-activation in 8 bits, and nothing else of its
     width, and the gradients that its products read are taken to 8 bits too."""
     what = "glu_mlp_8bit"

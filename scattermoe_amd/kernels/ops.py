@@ -176,6 +176,11 @@ class HipBackend:
         lib = _C.load()
         with _C.on_device(Y.device):
             sg = (gates.stride(0), gates.stride(1)) if gates is not None else (0, 0)
+            if Y.dtype != out.dtype:                                   # (float32 rows of products in 8 bits)
+                rc = lib.smoe_combine_f32(_C.ptr(Y), Y.stride(0), _C.ptr(gates), sg[0], sg[1], None, 0, _C.ptr(out), out.stride(0),
+                                          out.size(0), k, Y.size(1), _C.float_code(out.dtype), _C.stream_ptr(Y.device))
+                _C.check(rc, "smoe_combine_f32")
+                return
             rc = lib.smoe_combine(_C.ptr(Y), Y.stride(0), _C.ptr(gates), sg[0], sg[1],
                                   _C.ptr(out), out.stride(0), out.size(0), k, Y.size(1),
                                   _C.float_code(Y.dtype), _C.stream_ptr(Y.device))
@@ -186,6 +191,11 @@ class HipBackend:
         _C.require_gpu(Y, "gate_grad")
         lib = _C.load()
         with _C.on_device(Y.device):
+            if Y.dtype != d_out.dtype:
+                rc = lib.smoe_gate_grad_f32(_C.ptr(Y), Y.stride(0), _C.ptr(d_out), d_out.stride(0), _C.ptr(d_gates), d_gates.stride(0),
+                                            d_gates.stride(1), d_out.size(0), k, Y.size(1), _C.float_code(d_out.dtype), _C.stream_ptr(Y.device))
+                _C.check(rc, "smoe_gate_grad_f32")
+                return
             rc = lib.smoe_gate_grad(_C.ptr(Y), Y.stride(0), _C.ptr(d_out), d_out.stride(0),
                                     _C.ptr(d_gates), d_gates.stride(0), d_gates.stride(1),
                                     d_out.size(0), k, Y.size(1), _C.float_code(Y.dtype),
@@ -448,10 +458,11 @@ class HipBackend:
         sb = (b.stride(0), b.stride(1)) if b is not None else (0, 0)
         need = lib.smoe_linear_8bit_workspace_bytes(L, K, Y.size(1), W.size(0), k, int(x_grouped), int(coeff is not None), _C.float_code(X.dtype))
         ws = torch.empty(need, dtype=torch.uint8, device=X.device)
+        code = _C.float_code(X.dtype) | (_C.Y_FLOAT32_8BIT if Y.dtype != X.dtype else 0)
         with _C.on_device(X.device):
             rc = lib.smoe_linear_8bit(_C.ptr(X), X.stride(0), _C.ptr(coeff), _weight_8bit(W, S), int(transposed), _C.ptr(b), *sb, _C.ptr(Y),
                                       Y.stride(0), _C.ptr(idx), _C.ptr(off), L, K, Y.size(1), W.size(0), k, int(x_grouped), int(y_grouped),
-                                      _C.float_code(X.dtype), _C.ptr(ws), need, _C.stream_ptr(X.device))
+                                      code, _C.ptr(ws), need, _C.stream_ptr(X.device))
         _C.check(rc, "smoe_linear_8bit")
 
     @staticmethod
@@ -940,23 +951,27 @@ def _rows_contiguous(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def combine(expanded, gates=None):
+def combine(expanded, gates=None, dtype=None):
     """out[t] = sum_j gates[t, j] * expanded[t, j]  for expanded (T, k, N) -> (T, N)
     (the bmm of reference parallel_experts.py:44-46 as one HBM pass).  Without gates: the plain sum over the k
-    slots, accumulated in float32 in slot order and rounded once (the `.sum(-2)` of parallel_experts.py:120-123)."""
+    slots, accumulated in float32 in slot order and rounded once (the `.sum(-2)` of parallel_experts.py:120-123).
+    `dtype`: of the result, where the rows are float32."""
     T, k, N = expanded.shape
     assert gates is None or gates.shape == (T, k)
     Y = _rows_contiguous(expanded.reshape(T * k, N))
-    out = torch.empty((T, N), dtype=expanded.dtype, device=expanded.device)
-    _launch("combine", Y, None if gates is None else gates.to(expanded.dtype), out, k)
+    dtype = expanded.dtype if dtype is None else dtype
+    if expanded.dtype != torch.float32 and dtype != expanded.dtype:
+        raise TypeError("combine: dtype mismatch (%s vs %s)" % (expanded.dtype, dtype))
+    out = torch.empty((T, N), dtype=dtype, device=expanded.device)
+    _launch("combine", Y, None if gates is None else gates.to(dtype), out, k)
     return out
 
 
-def slot_sum(expanded_rows, T, k):
+def slot_sum(expanded_rows, T, k, dtype=None):
     """(T*k, N) rows in slot order -> (T, N): sum over each token's k slots (one pass, no gates)."""
     if k == 1:
         return expanded_rows
-    return combine(expanded_rows.view(T, k, expanded_rows.size(-1)))
+    return combine(expanded_rows.view(T, k, expanded_rows.size(-1)), dtype=dtype)
 
 
 def _wrote_into(t):
@@ -968,11 +983,14 @@ def _wrote_into(t):
 
 
 def gate_grad(expanded, grad_out):
-    """d_gates[t, j] = <expanded[t, j], grad_out[t]>  (the bmm of reference parallel_experts.py:79)."""
+    """d_gates[t, j] = <expanded[t, j], grad_out[t]>  (the bmm of reference parallel_experts.py:79), of grad_out's type; expanded of
+    the same or float32."""
     T, k, N = expanded.shape
     assert grad_out.shape == (T, N)
+    if expanded.dtype != torch.float32:
+        _same_dtype("gate_grad", expanded, grad_out)
     Y = _rows_contiguous(expanded.reshape(T * k, N))
-    d_gates = torch.empty((T, k), dtype=expanded.dtype, device=expanded.device)
+    d_gates = torch.empty((T, k), dtype=grad_out.dtype, device=expanded.device)
     _launch("gate_grad", Y, _rows_contiguous(grad_out), d_gates, k)
     return d_gates
 
@@ -1337,10 +1355,11 @@ def glu_8bit_bwd(p8, ps, dh, act=ACT_SILU, need_h=False):
     return dpre, h
 
 
-def linear_8bit(x, w, s, idx, off, k, b=None, coeff=None, transposed=False, x_grouped=False, y_grouped=False):
-    """scatter2scatter with x (rows of it taken to 8 bits, times coeff[slot] before that) and w (E, N, K) e4m3: (L, N) rows."""
+def linear_8bit(x, w, s, idx, off, k, b=None, coeff=None, transposed=False, x_grouped=False, y_grouped=False, dtype=None):
+    """scatter2scatter with x (rows of it taken to 8 bits, times coeff[slot] before that) and w (E, N, K) e4m3: (L, N) rows of x's type
+    or, `dtype`, of float32."""
     x = _rows_contiguous(x)
-    y = torch.empty((idx.numel(), w.size(1)), dtype=x.dtype, device=x.device)
+    y = torch.empty((idx.numel(), w.size(1)), dtype=x.dtype if dtype is None else dtype, device=x.device)
     if y.numel():
         _launch("linear_8bit", x, coeff, w, s, transposed, b, y, idx, off, k, x_grouped, y_grouped)
     return y
@@ -1350,7 +1369,7 @@ FEW_ROWS_8BIT = 64          # SMOE_8BIT_FEW_ROWS: a layer's forward goes by the 
 
 
 def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, experts=None, order=None, act=ACT_SILU, keep=False):
-    """(out (T, d), rows (T k, d) by slot or None, p8, ps): a gated layer on weights in 8 bits, from the experts (T, k) int64 for at most
+    """(out (T, d), rows (T k, d) float32 by slot or None, p8, ps): a gated layer on weights in 8 bits, from the experts (T, k) int64 for at most
     FEW_ROWS_8BIT rows, or from their order (idx, off); `keep`: the halves of its pre-activation."""
     x = _rows_contiguous(x)
     T, d, L, F = x.size(0), x.size(1), gates.numel(), w1.size(1) // 2
@@ -1358,7 +1377,7 @@ def glu_mlp_8bit(x, gates, w1, s1, b1, w2, s2, b2, experts=None, order=None, act
     rows = p8 = ps = idx = off = None
     if order is not None:
         idx, off = order
-        rows = torch.empty((L, d), dtype=x.dtype, device=x.device)
+        rows = torch.empty((L, d), dtype=torch.float32, device=x.device)
     if keep:
         p8 = torch.empty((L, 2, row_8bit(F)), dtype=TYPE_8BIT, device=x.device)
         ps = torch.empty((L, 2, blocks_8bit(F)), dtype=SCALE_8BIT, device=x.device)
@@ -1371,7 +1390,7 @@ def glu_mlp_8bit_bwd(d_out, gates, w1t, s1, w2t, s2, p8, ps, idx, off, act=ACT_S
     """The gradient of the layer's tokens, from the transposed weights."""
     d_out = _rows_contiguous(d_out)
     dx = torch.empty(d_out.shape, dtype=d_out.dtype, device=d_out.device)
-    drows = torch.empty((idx.numel(), d_out.size(1)), dtype=d_out.dtype, device=d_out.device)
+    drows = torch.empty((idx.numel(), d_out.size(1)), dtype=torch.float32, device=d_out.device)
     if dx.numel():
         _launch("glu_mlp_8bit_bwd", d_out, gates.contiguous(), w1t, s1, w2t, s2, p8, ps, drows, dx, idx, off, act)
     return dx

@@ -36,7 +36,10 @@ bool unit_grad_rides(int64_t F) { return F %% 128 == 0; }
 int launch_product_8bit(const Product8Args& a, int, int, hipStream_t, int) { note("product", a.x_grouped, a.fan); return 0; }
 int launch_few_rows_8bit(const Few8Args& a, int, int, int, hipStream_t) { note("stream", a.x_grouped, a.fan); return 0; }
 int launch_few_combine(const float*, const void*, const int64_t*, void*, int, int, int, int, int, hipStream_t) { return 0; }
-int launch_combine(const void*, int64_t, const void*, int64_t, int64_t, void*, int64_t, int64_t, int, int, int, hipStream_t) { return 0; }
+int launch_slots_combine(const float*, int64_t, const void*, int64_t, int64_t, const int64_t*, int, void*, int64_t, int64_t, int, int, int, hipStream_t) {
+  return 0;
+}
+int launch_slots_gate_grad(const float*, int64_t, const void*, int64_t, void*, int64_t, int64_t, int64_t, int, int, int, hipStream_t) { return 0; }
 }
 extern "C" const char* noted_launches() { return noted.c_str(); }
 extern "C" void forget_launches() { noted.clear(); }
