@@ -96,11 +96,11 @@ __device__ __forceinline__ void to_bf16x16(i32x4_8b q, float scale, bf16x8_8b (&
 // each loses what lies below 2^-13 of the largest one's binade before they are added (measured; the sums of eights are
 // added, and kept, in 32 bits).  128 to 4096 products of normal values end up 1.3e-5 of the result's norm off, whatever the
 // instruction: 1/130 of what rounding the result to bfloat16 costs, 1/16 of float16, and too much beside float32.  Rows that came in float32
-// are multiplied as bfloat16, which holds e4m3 exactly, at half the rate.
+// are multiplied as bfloat16, which holds e4m3 exactly, at half the rate; so are a float16 layer's, whose hidden values go to 8 bits again.
 enum Scaling8 {
   SCALES_BYTES,                                                    // all by the matrix instruction
   SCALES_FLOAT,                                                    // the rows' by the instruction, the weights' on every slice's sums
-  SCALES_EXACT                                                     // float32 rows: both on every slice's sums, of bfloat16 products
+  SCALES_EXACT                                                     // both on every slice's sums, of bfloat16 products
 };
 
 // ---- arguments ---------------------------------------------------------------------------------------
@@ -169,13 +169,13 @@ struct Product8Args {
   float* partial = nullptr;                                        // product_8bit_floats() of them, or NULL
 };
 // floats with which a product can cut the contraction of the tiles of its last round (0: it would not)
-int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, int row_dtype);
+int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, bool exact);
 // whether a product can be followed by the unit, or by its gradient, within its tiles
 bool unit_rides(int64_t d, int64_t F);
 bool unit_grad_rides(int64_t F);
 enum Epilogue8 { EPI_ROWS, EPI_UNIT, EPI_UNIT_GRAD };
-// row_dtype: of the rows that were taken to 8 bits and of the bias
-int launch_product_8bit(const Product8Args& a, int row_dtype, int out_dtype, hipStream_t st, int epilogue = EPI_ROWS);
+// exact: sums of bfloat16 products (SCALES_EXACT; whose rows come out in float32); row_dtype: of the rows that were taken to 8 bits and of the bias
+int launch_product_8bit(const Product8Args& a, bool exact, int row_dtype, int out_dtype, hipStream_t st, int epilogue = EPI_ROWS);
 
 // The same for a few rows per expert (csrc/few_rows_8bit.hip)
 struct Few8Args {

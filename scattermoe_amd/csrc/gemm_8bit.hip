@@ -664,8 +664,8 @@ static int launch_product(const Product8Args& a, int bias_dtype, hipStream_t st)
   else return a.ws_f32 ? launch_product<TO, SCALES_FLOAT, EPI, 128>(a, bias_dtype, n_tiles, st) : launch_product<TO, SCALES_BYTES, EPI, 128>(a, bias_dtype, n_tiles, st);
 }
 
-int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, int row_dtype) {
-  const bool exact = row_dtype == SMOE_F32, low = !exact && low_tiles(L, E);
+int64_t product_8bit_floats(int64_t L, int64_t K, int64_t columns, int E, bool exact) {
+  const bool low = !exact && low_tiles(L, E);
   const int64_t round = exact ? round_tiles<SCALES_EXACT, 128> : low ? round_tiles<SCALES_BYTES, 64> : round_tiles<SCALES_BYTES, 128>;
   const int64_t tiles = max_tiles(L, E, low ? 64 : 128) * ((columns + BN8 - 1) / BN8);
   if ((K + QB - 1) / QB < SPLIT_SLICES || tiles > SPLIT_ROUNDS * round) return 0;
@@ -679,8 +679,7 @@ bool unit_rides(int64_t d, int64_t F) { return F % 32 == 0 && 2 * F * padded_row
 // The gradient's blocks run along both halves: they lie within one half where F is whole blocks.
 bool unit_grad_rides(int64_t F) { return F % QB == 0; }
 
-int launch_product_8bit(const Product8Args& a, int row_dtype, int out_dtype, hipStream_t st, int epilogue) {
-  const bool exact = row_dtype == SMOE_F32;
+int launch_product_8bit(const Product8Args& a, bool exact, int row_dtype, int out_dtype, hipStream_t st, int epilogue) {
   if (epilogue == EPI_UNIT) return exact ? launch_product<float, true, EPI_UNIT>(a, row_dtype, st) : launch_product<float, false, EPI_UNIT>(a, row_dtype, st);
   if (epilogue == EPI_UNIT_GRAD)
     return exact ? launch_product<float, true, EPI_UNIT_GRAD>(a, row_dtype, st) : launch_product<float, false, EPI_UNIT_GRAD>(a, row_dtype, st);

@@ -30,10 +30,13 @@ int launch_quantize_weights(const QuantWeightsArgs&, int, hipStream_t) { return 
 int launch_dequantize(const DequantArgs&, int, hipStream_t) { return 0; }
 int launch_unit_fwd(const UnitArgs&, int, hipStream_t) { note("unit", 0, 0); return 0; }
 int launch_unit_bwd(const UnitBackArgs&, int, hipStream_t) { note("unit", 0, 0); return 0; }
-int64_t product_8bit_floats(int64_t, int64_t, int64_t, int, int) { return 0; }
+int64_t product_8bit_floats(int64_t, int64_t, int64_t, int, bool) { return 0; }
 bool unit_rides(int64_t, int64_t F) { return F %% 32 == 0; }
 bool unit_grad_rides(int64_t F) { return F %% 128 == 0; }
-int launch_product_8bit(const Product8Args& a, int, int, hipStream_t, int) { note("product", a.x_grouped, a.fan); return 0; }
+int launch_product_8bit(const Product8Args& a, bool exact, int, int, hipStream_t, int) {
+  note(exact ? "exact" : "product", a.x_grouped, a.fan);
+  return 0;
+}
 int launch_few_rows_8bit(const Few8Args& a, int, int, int, hipStream_t) { note("stream", a.x_grouped, a.fan); return 0; }
 int launch_few_combine(const float*, const void*, const int64_t*, void*, int, int, int, int, int, hipStream_t) { return 0; }
 int launch_slots_combine(const float*, int64_t, const void*, int64_t, int64_t, const int64_t*, int, void*, int64_t, int64_t, int, int, int, hipStream_t) {
@@ -116,3 +119,20 @@ def test_scaled_rows_are_copied_where_a_look_up_would_not_reach_them(lib, T, k, 
 def test_streams_over_the_weights_look_tokens_up_too(lib):
     found = _forward(lib, 40, 1, 128, 128, 64)
     assert found[1][0] == "stream" and not _rows_and_product(found, (40, 1), 40)
+
+
+def _kinds(found):
+    return [f[0] for f in found if f[0] in ("stream", "exact", "product")]
+
+
+def test_layers_of_more_bits_than_bfloat16_multiply_exactly(lib):
+    """Their hidden values go to 8 bits again; streams, which are exact, take up to 16 rows per expert then."""
+    for dtype, kind in ((_C.BF16, "product"), (_C.F16, "exact"), (_C.F32, "exact")):
+        assert _kinds(_forward(lib, 4096, 2, 128, 128, 8, dtype)) == [kind] * 2
+        assert _kinds(_backward(lib, 4096, 2, 128, 128, 8, dtype)) == [kind] * 2
+        for E, k in ((8, 2), (32, 4)):
+            for per, few in ((4, True), (5, kind == "exact"), (16, kind == "exact"), (17, False)):
+                assert _kinds(_forward(lib, per * E // k, k, 128, 128, E, dtype)) == ["stream" if few else kind] * 2
+    # a product's own result is rounded to the rows' type: float16 costs 16 times the instruction's sums
+    for dtype, kind in ((_C.BF16, "product"), (_C.F16, "product"), (_C.F32, "exact")):
+        assert _kinds(_linear(lib, 4096, 2, 128, 128, 8, dtype=dtype)) == [kind]
