@@ -452,7 +452,7 @@ typedef struct {
 /*
  * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, rounded once to `dtype`, or float32 where dtype is or-ed with
  * SMOE_8BIT_Y_FLOAT32 (rows that are added up afterwards: smoe_combine_f32); rows as for
- * smoe_scatter2scatter.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
+ * smoe_scatter2scatter, those of Y that belong to a dropped slot zeros.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
  * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out,
  * x_grouped, coeff != NULL, dtype) bytes, 256-byte aligned; nothing in it is read before it is written; calls that overlap in time need one each.
  */
@@ -477,7 +477,8 @@ int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm
  * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) float32 by slot (y), OUT (T,d)
  * contiguous; P8 (16-byte aligned), PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
  * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
- * alone, and ids outside [0,E) drop their row.
+ * alone.  Ids outside [0,E) drop their row: it adds nothing to OUT (whatever its gate, where `experts` is given beside the order too), is zeros in Y
+ * and DROWS, and adds nothing to DX.
  * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with
  * the scales of the weights; DROWS (T k, d) float32: what every slot adds to DX (T,d).  Workspaces as above.
  */

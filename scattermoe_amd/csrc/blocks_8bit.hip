@@ -88,10 +88,23 @@ static int64_t rows_per_launch(int64_t rows, int64_t blocks) {
   return rows < most ? rows : most;
 }
 
+// zeros for rows that a product may leave alone (at a kernel's end: its own work does not wait for kept[0])
+template <typename V>
+__device__ __forceinline__ void clear_all(const QuantRowsArgs::Clear& c) {
+  const int64_t wide = c.bytes / (int64_t)sizeof(V), total = c.rows * wide;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += gridDim.x * (int64_t)256) {
+    const int64_t row = i / wide;
+    ((V*)(c.at + row * c.ld))[i - row * wide] = V{};
+  }
+}
+__device__ __forceinline__ void clear_rows(const QuantRowsArgs::Clear& c) {
+  if (!c.at || c.kept[0] >= c.rows) return;
+  if ((((uintptr_t)c.at | c.bytes | c.ld) & 15) == 0) clear_all<q_i32x4>(c);
+  else clear_all<short>(c);
+}
+
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantRowsArgs a, int blocks) {
-  const Unit u(a.rows, blocks);
-  if (!u.there) return;
+__device__ __forceinline__ void quantize_unit(const QuantRowsArgs& a, const Unit& u) {
   int64_t src = u.row;
   float f = 1.0f;
   bool have = true;                                                // (a row that the routing dropped has no source)
@@ -107,20 +120,28 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantRowsArgs a, int
   for (int i = 0; i < 8; ++i) v[i] *= f;
   store_block(a.Q + u.row * a.ld, a.S + u.row * scale_row(a.K) + u.block, u.c, a.ld, v);
 }
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantRowsArgs a, int blocks) {
+  const Unit u(a.rows, blocks);
+  if (u.there) quantize_unit<T, VEC>(a, u);
+  clear_rows(a.clear);
+}
 // a source row once, times each of its fan coefficients (8192 rows of 2048, 8 each: 84 us by idx, 29 so)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quantize_times_kernel(QuantRowsArgs a, int blocks) {
   const Unit u(a.rows, blocks);
-  if (!u.there) return;
-  float v[8], x[8];
-  load8<T, VEC>((const T*)a.X + u.row * a.sxm, u.c, a.K, v);
-  for (int j = 0; j < a.fan; ++j) {
-    const int64_t n = u.row * a.fan + j;
-    const float f = to_f32(((const T*)a.coeff)[n]);
+  if (u.there) {
+    float v[8], x[8];
+    load8<T, VEC>((const T*)a.X + u.row * a.sxm, u.c, a.K, v);
+    for (int j = 0; j < a.fan; ++j) {
+      const int64_t n = u.row * a.fan + j;
+      const float f = to_f32(((const T*)a.coeff)[n]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = v[i] * f;
-    store_block(a.Q + n * a.ld, a.S + n * scale_row(a.K) + u.block, u.c, a.ld, x);
+      for (int i = 0; i < 8; ++i) x[i] = v[i] * f;
+      store_block(a.Q + n * a.ld, a.S + n * scale_row(a.K) + u.block, u.c, a.ld, x);
+    }
   }
+  clear_rows(a.clear);
 }
 
 template <typename T>
@@ -143,6 +164,7 @@ static int quantize_rows(QuantRowsArgs a, hipStream_t st) {
     if (times) a.coeff = (const T*)a.coeff + made;
     a.Q += made * a.ld;
     a.S += made * Sr;
+    a.clear.at = nullptr;
   }
   return launch_status("quantize_rows");
 }

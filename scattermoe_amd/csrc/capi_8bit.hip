@@ -39,9 +39,15 @@ static Rows8Bit take_rows(Carver& c, int64_t rows, int64_t K) {
   return r;
 }
 static int quantize(const Rows8Bit& r, const void* X, int64_t sxm, const int64_t* idx, int fan, const void* coeff, int64_t K, int dtype,
-                    hipStream_t st) {
-  QuantRowsArgs a{X, sxm, idx, fan, coeff, coeff && !idx ? r.rows / fan : r.rows, K, r.q, r.s, r.rows, block_row(K)};
+                    hipStream_t st, QuantRowsArgs::Clear clear = {}) {
+  QuantRowsArgs a{X, sxm, idx, fan, coeff, coeff && !idx ? r.rows / fan : r.rows, K, r.q, r.s, r.rows, block_row(K), clear};
   return launch_quantize_rows(a, dtype, st);
+}
+
+// the rows (L, N) of `dtype` that a product writes, for zeros where the routing dropped some
+static QuantRowsArgs::Clear dropped_rows(void* Y, int64_t sym, int64_t L, int64_t N, int dtype, const int64_t* off, int E) {
+  const int64_t size = dtype == SMOE_F32 ? 4 : 2;
+  return {(char*)Y, L, N * size, sym * size, off + E - 1};
 }
 
 static int weight_checks(const char* who, const smoe_weight_8bit* w, int64_t rows, int64_t cols) {
@@ -103,7 +109,7 @@ int smoe_quantize_rows(const void* X, int64_t sxm, int64_t rows, int64_t K, void
   if (rows == 0 || K == 0) return 0;
   if (!X || !Q || !S) { set_error("smoe_quantize_rows: NULL pointer"); return SMOE_ERR_NULL; }
   if ((uintptr_t)Q & 15) { set_error("smoe_quantize_rows: rows in 8 bits start at multiples of 16 bytes"); return SMOE_ERR_SHAPE; }
-  QuantRowsArgs a{X, sxm, nullptr, 1, nullptr, rows, K, (uint8_t*)Q, (uint8_t*)S, rows, padded_row(K)};
+  QuantRowsArgs a{X, sxm, nullptr, 1, nullptr, rows, K, (uint8_t*)Q, (uint8_t*)S, rows, padded_row(K), {}};
   return launch_quantize_rows(a, dtype, (hipStream_t)stream);
 }
 
@@ -199,7 +205,8 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
   const Rows8Bit x = take_rows(c, from.rows, K);
   const int fan = coeff ? 1 : fan_out;                             // rows of x per row of the product's left side
   const bool copies = !x_grouped && !by_token;
-  if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream)) return rc;
+  if (int rc = quantize(x, X, sxm, copies ? idx : nullptr, fan_out, coeff, K, dtype, (hipStream_t)stream,
+                        dropped_rows(Y, sym, L, N, out_dtype, off, E))) return rc;
   if (few_rows_pay(L, K, E)) {
     Few8Args a = few(W, b, sbe, sbn, Y, sym, out_dtype, nullptr, idx, off, L, K, N, E, fan, !by_token, y_grouped, 0);
     if (transposed) a.ssn = W->s_col, a.ssk = W->s_row;
@@ -309,7 +316,7 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
     return launch_few_combine(p.rows, gates, experts, OUT, (int)T, k, (int)d, E, dtype, st);
   }
   const bool by_token = p.by_token;
-  if (int rc = quantize(p.x, X, sxm, by_token ? nullptr : idx, k, nullptr, d, dtype, st)) return rc;
+  if (int rc = quantize(p.x, X, sxm, by_token ? nullptr : idx, k, nullptr, d, dtype, st, dropped_rows(Y, d, L, d, SMOE_F32, off, E))) return rc;
   if (way == LAYER_FEW) {
     Few8Args a = few(W1, b1, sb1e, sb1n, p.hidden, F, SMOE_F32, nullptr, idx, off, L, d, 2 * F, E, k, !by_token, 1, act);
     a.X = p.x.q, a.sxm = block_row(d), a.XS = p.x.s;
@@ -374,7 +381,7 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   Carver c{(char*)workspace};
   const BackPieces p = back_pieces(c, L, k, d, F, E, dtype);
   const bool by_slot = p.by_slot;
-  if (int rc = quantize(p.dy, DOUT, sdm, by_slot ? nullptr : idx, k, gates, d, dtype, st)) return rc;
+  if (int rc = quantize(p.dy, DOUT, sdm, by_slot ? nullptr : idx, k, gates, d, dtype, st, dropped_rows(DROWS, d, L, d, SMOE_F32, off, E))) return rc;
   Product8Args a = product(p.dy, W2T, true, nullptr, 0, 0, p.dh, F, idx, off, L, d, F, E, 1, !by_slot, 1);
   a.partial = p.partial1;
   if (!p.dh) {

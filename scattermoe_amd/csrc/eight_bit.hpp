@@ -112,6 +112,12 @@ struct QuantRowsArgs {
   uint8_t* Q; uint8_t* S;
   int64_t slots;                                                   // with idx: entries outside [0, slots) make a row of zeros
   int64_t ld;                                                      // bytes of a row of Q, a multiple of 16, zeros behind the last value
+  // Rows that a later product writes by slot: those of slots that the routing dropped it leaves alone, and a sum over a token's slots reads
+  // them.  All are set to zero where kept[0] < clear.rows, here, ahead of the product, since this launch is there anyway.
+  struct Clear {
+    char* at; int64_t rows, bytes, ld;
+    const int64_t* kept;
+  } clear;
 };
 int launch_quantize_rows(const QuantRowsArgs& a, int dtype, hipStream_t st);
 

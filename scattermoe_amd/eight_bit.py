@@ -144,6 +144,8 @@ def parallel_linear_8bit(inputs, weight, weight_scales, k, sorted_expert_idxs, s
     (E, ceil(N / 128), ceil(K / 128)) of float8_e8m0fnu or float32, and rounded once: rows that gates weigh, and the gradients of a token's
     slots, are added up in float32.  Biases (E, N) and gates (tokens, k) of the inputs' type.  Routing as for `parallel_linear`; gates go with `grouped_out=False`.
 
+    Slots that the routing dropped (ids outside [0, E)) have rows of zeros; gates that weigh those are finite numbers.
+
     Weights, scales and biases are constants.  The inputs' gradient, Q(gate dy) W, needs weight_t (E, K, N rounded up to 16), the transposed
     weight (`quantize_blocks(w, 128, transposed=True)`); gates have theirs without it."""
     what = "parallel_linear_8bit"
@@ -179,9 +181,9 @@ class _GluMLP8bit(torch.autograd.Function):
     """The whole layer; keeps its pre-activation in 8 bits where the tokens' gradient is asked for."""
 
     @staticmethod
-    def forward(ctx, x, gates, w1, s1, w1t, b1, w2, s2, w2t, b2, idx, off, act):
+    def forward(ctx, x, gates, experts, w1, s1, w1t, b1, w2, s2, w2t, b2, idx, off, act):
         need_x, need_g = ctx.needs_input_grad[:2]
-        out, rows, p8, ps = ops.glu_mlp_8bit(x, gates.to(x.dtype), w1, s1, b1, w2, s2, b2, order=(idx, off), act=act, keep=need_x)
+        out, rows, p8, ps = ops.glu_mlp_8bit(x, gates.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=experts, order=(idx, off), act=act, keep=need_x)
         ctx.save_for_backward(gates, rows if need_g else None, w1t, s1, w2t, s2, p8, ps, idx, off)
         ctx.act = act
         return out
@@ -196,16 +198,16 @@ class _GluMLP8bit(torch.autograd.Function):
             d_gates = ops.gate_grad(rows.view(gates.size(0), gates.size(1), rows.size(1)), d_out)
         if p8 is not None:
             dx = ops.glu_mlp_8bit_bwd(d_out, gates.to(d_out.dtype), w1t, s1, w2t, s2, p8, ps, idx, off, ctx.act)
-        return (dx, d_gates) + (None,) * 11
+        return (dx, d_gates) + (None,) * 12
 
 
 def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gate_first=False, w1_t=None, w2_t=None):
-    """GLUMLP.forward on weights in 8 bits: x (..., d), expert_p and expert_idxs (tokens, k) in [0, E), w1 (E, 2F, d rounded up to 16) and w2 (E, d, F
+    """GLUMLP.forward on weights in 8 bits: x (..., d), expert_p and expert_idxs (tokens, k), w1 (E, 2F, d rounded up to 16) and w2 (E, d, F
     rounded up to 16) of float8_e4m3fn, the rest zeros, with scales s1, s2 for every 128 x 128, float8_e8m0fnu or float32; biases (E, 2F), (E, d) or
     None of x's type; SiLU on the second half of the first product's columns, on the first when `gate_first`.
 
     The tokens and the hidden rows are taken to 8 bits; pre-activations, the experts' rows and sums stay in float32, and the result is rounded
-    once.  expert_p is taken to x's type.  A step that asks for the gradient of expert_p keeps the experts' rows in float32.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
+    once.  expert_p is taken to x's type.  A slot whose id lies outside [0, E) (padding) adds nothing, whatever its gate, and has no gradient.  A step that asks for the gradient of expert_p keeps the experts' rows in float32.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
     rounded up to 16) and w2_t (E, F, d rounded up to 16); the step then keeps the pre-activation in 8 bits, and nothing else of its
     width, and the gradients that its products read are taken to 8 bits too."""
     what = "glu_mlp_8bit"
@@ -227,14 +229,15 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
     tokens = x if x.dim() == 2 else x.reshape(T, d)                  # (a view would be a node of the backward pass)
     trained = ((x.requires_grad or expert_p.requires_grad) and torch.is_grad_enabled()) or ops.has_tangents(x, expert_p, b1, b2)
     # (by the ids an expert's weights are read once for every 8 of its rows: 64 rows of 8 experts, 4096 / 14336, 368 us, in the experts' order 265)
+    experts = ops._as_i64(expert_idxs).contiguous()
     if not trained and T * k <= min(ops.FEW_ROWS_8BIT, 4 * E):
-        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=ops._as_i64(expert_idxs).contiguous(), act=act)[0]
+        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=experts, act=act)[0]
         return out if x.dim() == 2 else out.view(x.shape)
     _, idx, off = flatten_sort_count(expert_idxs, num_experts=E)
     if trained:
-        out = _GluMLP8bit.apply(tokens, expert_p, w1, s1, w1_t, b1, w2, s2, w2_t, b2, idx, off, act)
+        out = _GluMLP8bit.apply(tokens, expert_p, experts, w1, s1, w1_t, b1, w2, s2, w2_t, b2, idx, off, act)
     else:
-        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, order=(idx, off), act=act)[0]
+        out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=experts, order=(idx, off), act=act)[0]
     return out if x.dim() == 2 else out.view(x.shape)
 
 
