@@ -173,6 +173,8 @@ class GLUMLP(_SparseMLP):
 
     def forward(self, x: torch.Tensor, expert_p: torch.Tensor, expert_idxs: torch.Tensor):
         if type(self.activation) is not nn.SiLU:
+            if self.checkpoint_8bit and torch.is_grad_enabled():       # (an activation that was put in later)
+                raise ValueError("GLUMLP: checkpoint_8bit goes with SiLU")
             return super().forward(x, expert_p, expert_idxs)
         lead = x.shape[:-1]
         tokens = x.view(-1, x.size(-1))
@@ -249,5 +251,7 @@ class RoutedGLUMLP(GLUMLP):
         self.renormalize = renormalize
 
     def forward(self, x: torch.Tensor):
+        if self.checkpoint_8bit and torch.is_grad_enabled():
+            raise ValueError("RoutedGLUMLP: checkpoint_8bit goes with GLUMLP")
         return routed_glu_mlp(x, self.router.weight, self.experts.weight, self.output_experts.weight, self.top_k,
                               b1=self.experts.bias, b2=self.output_experts.bias, renormalize=self.renormalize)
