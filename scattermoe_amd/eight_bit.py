@@ -60,6 +60,13 @@ def dequantize_blocks(q, scales, block_rows=1, size=None, dtype=torch.bfloat16):
     return ops.dequantize(q, scales, ops.BLOCK_8BIT, K, dtype)
 
 
+def _experts_in_place(q):
+    """q (E, N, K) where each expert's values are contiguous and experts lie multiples of 16 bytes apart (every second one, one for all); else a copy."""
+    if q.stride(2) == 1 and q.stride(1) == q.size(2) and (q.size(0) == 1 or q.stride(0) % 16 == 0):
+        return q
+    return q.contiguous()
+
+
 def _weight(what, name, q, s, device, E, N, K, t=None):
     """The weight (E, N, K), its scales and its transpose as the kernels take them, or an error."""
     if q.dtype != ops.TYPE_8BIT or (t is not None and t.dtype != ops.TYPE_8BIT):
@@ -80,7 +87,7 @@ def _weight(what, name, q, s, device, E, N, K, t=None):
             raise RuntimeError("%s: all tensors on the device of the rows (%s)" % (what, device))
     if s.size(1) * s.stride(1) + s.size(2) * s.stride(2) > 1 << 28:
         s = s.contiguous()
-    return q.contiguous(), s, None if t is None else t.contiguous()
+    return _experts_in_place(q), s, None if t is None else _experts_in_place(t)
 
 
 def _rows_and_bias(what, x, b, name, shape):

@@ -52,10 +52,10 @@ def _whole_rows(x):
 
 
 def _weight_8bit(q, s):
-    """smoe_weight_8bit of a contiguous weight (E, N, K) and its scales."""
+    """smoe_weight_8bit of a weight (E, N, K), each expert's values contiguous, and its scales."""
     if q.data_ptr() % 16 != 0:                   # (a view of other bytes; under a compiler the address is known here only)
         q = q.clone()
-    w = _C.Weight8bit(q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), s.stride(1), s.stride(2),
+    w = _C.Weight8bit(q.data_ptr(), q.stride(0) if q.size(0) > 1 else 0, s.data_ptr(), s.stride(0), s.stride(1), s.stride(2),
                       int(s.dtype == torch.float32))
     w.held = q
     return w

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from scattermoe_amd import eight_bit
+from scattermoe_amd.kernels import ops
 from scattermoe_amd.mlp import GLUMLP, MLP, RoutedGLUMLP
 
 
@@ -29,3 +30,19 @@ def test_a_checkpoint_that_a_layer_cannot_keep_is_refused_where_it_would_be():
         for call in (lambda: m(x, p, ids), lambda: r(x)):
             with pytest.raises(RuntimeError, match="ROCm GPU"):
                 call()
+
+
+def test_weights_whose_experts_lie_apart_are_taken_where_they_are():
+    """Every second expert of a checkpoint's, one expert for all, the last ones, one alone; a weight whose rows lie apart is copied."""
+    E, N, K = 6, 40, 32
+    full = torch.zeros(2 * E, N, K, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    s = torch.ones(E, 1, 1)
+    for q in (full[::2], full[:1].expand(E, N, K), full[E:], full.view(torch.uint8).as_strided((E, N, K), (N * K + 48, K, 1)).view(full.dtype)):
+        got, _, t = eight_bit._weight("call", "w", q, s, q.device, E, N, K)
+        assert got.data_ptr() == q.data_ptr() and got.stride() == q.stride() and t is None
+    one = full.view(torch.uint8).as_strided((1, N, K), (7, K, 1)).view(full.dtype)
+    held = ops._weight_8bit(eight_bit._weight("call", "w", one, s[:1], one.device, 1, N, K)[0], s[:1])
+    assert held.q == one.data_ptr() and held.q_expert % 16 == 0
+    for q in (full[:E].transpose(1, 2).contiguous().transpose(1, 2), full.view(torch.uint8).as_strided((E, N, K), (N * K + 8, K, 1)).view(full.dtype),
+              full.view(torch.uint8).as_strided((E, N, K), (N * 2 * K, 2 * K, 1)).view(full.dtype)):
+        assert eight_bit._weight("call", "w", q, s, q.device, E, N, K)[0].stride() == (N * K, K, 1)
