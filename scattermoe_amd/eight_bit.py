@@ -323,12 +323,16 @@ class GLUMLP8bit(nn.Module):
         return m
 
     def _apply(self, fn, recurse=True):
-        held = {name: getattr(self, name) for name in self._held}
-        super()._apply(fn, recurse)
-        for name, t in held.items():                                 # (a cast to another type is for the biases only)
-            now = getattr(self, name)
-            if t is not None and now.dtype != t.dtype:
-                setattr(self, name, t.to(device=now.device))
+        held = {name: self._buffers[name] for name in self._held}
+        self._buffers.update(dict.fromkeys(self._held))              # (a cast to another type is for the biases only)
+        try:
+            super()._apply(fn, recurse)
+            for name, t in held.items():
+                if t is not None:
+                    like = fn(t.new_empty(0))                        # where it goes, and whether as what it is
+                    held[name] = fn(t) if like.dtype == t.dtype else t.to(device=like.device)
+        finally:
+            self._buffers.update(held)
         return self
 
     def extra_repr(self):

@@ -46,3 +46,24 @@ def test_weights_whose_experts_lie_apart_are_taken_where_they_are():
     for q in (full[:E].transpose(1, 2).contiguous().transpose(1, 2), full.view(torch.uint8).as_strided((E, N, K), (N * K + 8, K, 1)).view(full.dtype),
               full.view(torch.uint8).as_strided((E, N, K), (N * 2 * K, 2 * K, 1)).view(full.dtype)):
         assert eight_bit._weight("call", "w", q, s, q.device, E, N, K)[0].stride() == (N * K, K, 1)
+
+
+def test_casting_a_module_does_not_cast_its_weights_on_the_way():
+    m = eight_bit.GLUMLP8bit(64, 48, 3, 2, bias=True, input_gradients=True)
+    keys, seen = list(m.state_dict()), []
+
+    def cast(t):
+        seen.append((t.dtype, t.numel()))
+        return t.to(torch.float16)
+
+    held = {n: getattr(m, n) for n in m._held}
+    m._apply(cast)
+    assert all(n == 0 for dtype, n in seen if dtype not in (torch.bfloat16,))
+    assert m.b1.dtype == torch.float16 and all(getattr(m, n) is t for n, t in held.items()) and list(m.state_dict()) == keys
+    # what is no cast reaches them: another device, memory of their own
+    m = m.to("meta")
+    assert all(getattr(m, n).device.type == "meta" and getattr(m, n).dtype == t.dtype for n, t in held.items())
+    m = m.to_empty(device="cpu")
+    assert all(getattr(m, n).shape == t.shape and getattr(m, n).device.type == "cpu" for n, t in held.items())
+    n = eight_bit.GLUMLP8bit(64, 48, 3, 2, scale_type=torch.float32).to("meta", torch.float16)
+    assert n.w1.device.type == n.s1.device.type == "meta" and n.s1.dtype == torch.float32 and n.w1.dtype == m.w1.dtype and n.w1_t is None
