@@ -183,7 +183,7 @@ size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, 
   if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
   take_rows(c, source_rows(L, K, fan_out, x_grouped, scaled != 0).rows, K);
-  if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, dtype == SMOE_F32) * 4);
+  if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, (dtype & ~SMOE_8BIT_Y_FLOAT32) == SMOE_F32) * 4);
   return c.used;
 }
 

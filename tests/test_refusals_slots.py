@@ -33,3 +33,12 @@ def test_rows_of_another_type_are_float32():
     for call in (lambda: ops.combine(rows.float(), dtype=torch.float16), lambda: ops.gate_grad(rows.float(), torch.zeros(3, 8, dtype=torch.float16))):
         with pytest.raises(RuntimeError, match="ROCm GPU"):
             call()
+
+
+def test_workspace_of_float32_rows():
+    """The same bytes whether or not the product's rows come out in float32, however the caller asks for them."""
+    lib = _C.load()
+    for dtype in (_C.F32, _C.BF16, _C.F16):
+        for L, K, N, E in ((8, 64, 64, 2), (300, 16384, 256, 2), (300, 9000, 9000, 4)):
+            plain, floats = (lib.smoe_linear_8bit_workspace_bytes(L, K, N, E, 1, 0, 0, d) for d in (dtype, dtype | _C.Y_FLOAT32_8BIT))
+            assert plain == floats > 0
