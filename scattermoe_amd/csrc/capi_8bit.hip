@@ -92,6 +92,13 @@ static Few8Args few(const smoe_weight_8bit* w, const void* b, int64_t sbe, int64
 // 158, 169, 181, tiles 184 and more.  (32768 rows: a segment per expert or 8 rows is a grid's second side.)
 static bool few_rows_pay(int64_t L, int64_t K, int E) { return L <= (K >= 4096 ? 12 : 4) * (int64_t)E && L <= 32768; }
 
+// Products of a layer that multiply exactly (SCALES_EXACT), beside those of float32 rows: of float16 rows the ones whose results go to 8 bits again.  A
+// hidden value, or a gradient, whose sum is 1e-5 off may fall to the other side of a border between two 8-bit values, a step of 2^-4,
+// and such steps cost 1e-3 of the result, five times float16's own rounding (65 tokens to 4 of 32 experts, 2880 / 2880, against 64 bits:
+// 1.4e-3, so 2.1e-4, as the plain form).  Bfloat16 rounds to 1.7e-3 by itself, which the steps make 2.0e-3 to 2.2e-3.
+static bool product_exact(int dtype) { return dtype == SMOE_F32; }
+static bool inner_exact(int dtype) { return dtype != SMOE_BF16; }
+
 }  // namespace smoe
 
 using namespace smoe;
@@ -183,7 +190,7 @@ size_t smoe_linear_8bit_workspace_bytes(int64_t L, int64_t K, int64_t N, int E, 
   if (L <= 0 || K <= 0 || N <= 0 || E <= 0 || fan_out <= 0) return 0;
   Carver c{nullptr};
   take_rows(c, source_rows(L, K, fan_out, x_grouped, scaled != 0).rows, K);
-  if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, (dtype & ~SMOE_8BIT_Y_FLOAT32) == SMOE_F32) * 4);
+  if (!few_rows_pay(L, K, E)) c.take(product_8bit_floats(L, K, N, E, product_exact(dtype & ~SMOE_8BIT_Y_FLOAT32)) * 4);
   return c.used;
 }
 
@@ -214,8 +221,8 @@ int smoe_linear_8bit(const void* X, int64_t sxm, const void* coeff, const smoe_w
     return launch_few_rows_8bit(a, -1, dtype, EPI_ROWS, (hipStream_t)stream);
   }
   Product8Args a = product(x, W, transposed != 0, b, sbe, sbn, Y, sym, idx, off, L, K, N, E, fan, !by_token, y_grouped);
-  a.partial = take_partial(c, product_8bit_floats(L, K, N, E, dtype == SMOE_F32));
-  return launch_product_8bit(a, dtype == SMOE_F32, dtype, out_dtype, (hipStream_t)stream);
+  a.partial = take_partial(c, product_8bit_floats(L, K, N, E, product_exact(dtype)));
+  return launch_product_8bit(a, product_exact(dtype), dtype, out_dtype, (hipStream_t)stream);
 }
 
 int smoe_combine_f32(const void* Y, int64_t sym, const void* gates, int64_t sgt, int64_t sgk, const int64_t* experts, int E, void* out, int64_t som,
@@ -240,20 +247,19 @@ int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm
   return launch_slots_gate_grad((const float*)Y, sym, dOut, sdm, dgates, sgt, sgk, T, k, (int)N, dtype, (hipStream_t)stream);
 }
 
-// Layers whose rows hold more bits than bfloat16 multiply exactly (SCALES_EXACT): a hidden value whose sum is 1e-5 off may fall to the other side of
-// a border between two 8-bit values, a step of 2^-4, and such steps cost 1e-3 of the result, five times float16's own rounding (65 tokens to 4 of
-// 32 experts, 2880 / 2880, against 64 bits: 1.4e-3, exactly 3.2e-4, as the plain form).  Tiles take about twice as long for it; streams multiply
-// exactly anyhow, and pay against such tiles up to 16 rows per expert, the most that one reading of the weights takes: layers in float16, us at 8, 12, 16, 24
-// rows per expert, streams and tiles: 8 experts, 4096 / 14336 261, 268, 278, 414 and 515 from 8 on; 32 experts, 2880 / 2880 195, 204, 211, 316 and 325;
-// 128 experts, 2048 / 768 162, 173, 179, 264 and 250.
-static bool layer_exact(int dtype) { return dtype != SMOE_BF16; }
+// Streams multiply exactly anyhow, and pay against such tiles up to 16 rows per expert, the most that one reading of the weights takes.  Layers in float32,
+// us at 8, 12, 16, 24 rows per expert, streams and tiles: 8 experts, 4096 / 14336 261, 268, 278, 414 and 515 from 8 on; 32 experts, 2880 / 2880
+// 195, 204, 211, 316 and 325; 128 experts, 2048 / 768 162, 173, 179, 264 and 250.  In float16 the same streams, tiles 463, 276 and 219.
+static bool streams_pay(int64_t L, int64_t d, int64_t F, int E, int dtype) {
+  return few_rows_pay(L, d < F ? d : F, E) || (inner_exact(dtype) && L <= 16 * (int64_t)E && L <= 32768);
+}
 
 // How a layer goes.  Without an order of its rows: by their ids, two streams over the weights of the experts that they name.  Few rows per
 // expert: streams over the weights, rows by expert.  Else tiles, with the unit behind the first product where it rides.
 enum LayerWay { LAYER_BY_IDS, LAYER_FEW, LAYER_TILES, LAYER_TILES_UNIT };
 static LayerWay layer_way(int64_t L, int64_t d, int64_t F, int E, bool ordered, bool keep, int dtype) {
   if (!ordered) return LAYER_BY_IDS;
-  if (!keep && (few_rows_pay(L, d < F ? d : F, E) || (layer_exact(dtype) && L <= 16 * (int64_t)E && L <= 32768))) return LAYER_FEW;
+  if (!keep && streams_pay(L, d, F, E, dtype)) return LAYER_FEW;
   return unit_rides(d, F) ? LAYER_TILES_UNIT : LAYER_TILES;
 }
 // the pieces of a gated layer's workspace
@@ -272,7 +278,7 @@ static LayerPieces layer_pieces(Carver& c, LayerWay way, int64_t L, int k, int64
   if (way == LAYER_FEW) p.hidden = c.take<float>(L * F * 4);
   if (way == LAYER_TILES) p.pre = c.take<float>(L * 2 * F * 4);
   if (way != LAYER_FEW) {                                          // (one after the other: the same piece for both products)
-    const int64_t one = product_8bit_floats(L, d, 2 * F, E, layer_exact(dtype)), two = product_8bit_floats(L, F, d, E, layer_exact(dtype));
+    const int64_t one = product_8bit_floats(L, d, 2 * F, E, inner_exact(dtype)), two = product_8bit_floats(L, F, d, E, product_exact(dtype));
     float* both = take_partial(c, one > two ? one : two);
     p.partial1 = one ? both : nullptr, p.partial2 = two ? both : nullptr;
   }
@@ -331,15 +337,15 @@ int smoe_glu_mlp_8bit(const void* X, int64_t sxm, const void* gates, const int64
   a.partial = p.partial1;
   if (way == LAYER_TILES_UNIT) {
     a.H8 = p.h.q, a.HS = p.h.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
-    if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st, EPI_UNIT)) return rc;
+    if (int rc = launch_product_8bit(a, inner_exact(dtype), dtype, SMOE_F32, st, EPI_UNIT)) return rc;
   } else {
-    if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st)) return rc;
+    if (int rc = launch_product_8bit(a, inner_exact(dtype), dtype, SMOE_F32, st)) return rc;
     UnitArgs u{p.pre, 2 * F, nullptr, p.h.q, p.h.s, (uint8_t*)P8, (uint8_t*)PS, L, F, act};
     if (int rc = launch_unit_fwd(u, SMOE_F32, st)) return rc;
   }
   a = product(p.h, W2, false, b2, sb2e, sb2n, Y, d, idx, off, L, F, d, E, 1, 1, 0);
   a.partial = p.partial2;
-  if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st)) return rc;
+  if (int rc = launch_product_8bit(a, product_exact(dtype), dtype, SMOE_F32, st)) return rc;
   return launch_slots_combine((const float*)Y, d, gates, k, 1, experts, E, OUT, d, T, k, (int)d, dtype, st);
 }
 
@@ -351,7 +357,7 @@ static BackPieces back_pieces(Carver& c, int64_t L, int k, int64_t d, int64_t F,
   p.dy = take_rows(c, from.rows, d);
   p.dp = take_rows(c, L, 2 * F);
   p.dh = unit_grad_rides(F) ? nullptr : c.take<float>(L * F * 4);
-  const int64_t one = product_8bit_floats(L, d, F, E, layer_exact(dtype)), two = product_8bit_floats(L, 2 * F, d, E, layer_exact(dtype));
+  const int64_t one = product_8bit_floats(L, d, F, E, inner_exact(dtype)), two = product_8bit_floats(L, 2 * F, d, E, product_exact(dtype));
   float* both = take_partial(c, one > two ? one : two);
   p.partial1 = one ? both : nullptr, p.partial2 = two ? both : nullptr;
   return p;
@@ -386,15 +392,15 @@ int smoe_glu_mlp_8bit_bwd(const void* DOUT, int64_t sdm, const void* gates, cons
   a.partial = p.partial1;
   if (!p.dh) {
     a.H8 = p.dp.q, a.HS = p.dp.s, a.P8 = (uint8_t*)P8, a.PS = (uint8_t*)PS, a.act = act;
-    if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st, EPI_UNIT_GRAD)) return rc;
+    if (int rc = launch_product_8bit(a, inner_exact(dtype), dtype, SMOE_F32, st, EPI_UNIT_GRAD)) return rc;
   } else {
-    if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st)) return rc;
+    if (int rc = launch_product_8bit(a, inner_exact(dtype), dtype, SMOE_F32, st)) return rc;
     UnitBackArgs u{(const uint8_t*)P8, (const uint8_t*)PS, p.dh, F, nullptr, p.dp.q, p.dp.s, nullptr, L, F, act};
     if (int rc = launch_unit_bwd(u, SMOE_F32, st)) return rc;
   }
   a = product(p.dp, W1T, true, nullptr, 0, 0, DROWS, d, idx, off, L, 2 * F, d, E, 1, 1, 0);
   a.partial = p.partial2;
-  if (int rc = launch_product_8bit(a, layer_exact(dtype), dtype, SMOE_F32, st)) return rc;
+  if (int rc = launch_product_8bit(a, product_exact(dtype), dtype, SMOE_F32, st)) return rc;
   return launch_slots_combine((const float*)DROWS, d, nullptr, 0, 0, nullptr, E, DX, d, T, k, (int)d, dtype, st);
 }
 

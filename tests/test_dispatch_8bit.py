@@ -125,14 +125,14 @@ def _kinds(found):
     return [f[0] for f in found if f[0] in ("stream", "exact", "product")]
 
 
-def test_layers_of_more_bits_than_bfloat16_multiply_exactly(lib):
-    """Their hidden values go to 8 bits again; streams, which are exact, take up to 16 rows per expert then."""
-    for dtype, kind in ((_C.BF16, "product"), (_C.F16, "exact"), (_C.F32, "exact")):
-        assert _kinds(_forward(lib, 4096, 2, 128, 128, 8, dtype)) == [kind] * 2
-        assert _kinds(_backward(lib, 4096, 2, 128, 128, 8, dtype)) == [kind] * 2
+def test_products_whose_results_go_to_8_bits_again_are_exact_of_more_bits_than_bfloat16(lib):
+    """The first of a layer and the first of its backward pass; streams, which are exact, take up to 16 rows per expert then."""
+    for dtype, first, other in ((_C.BF16, "product", "product"), (_C.F16, "exact", "product"), (_C.F32, "exact", "exact")):
+        for F in (128, 96, 72):                                         # with the unit behind the product, and its gradient, or without
+            assert _kinds(_forward(lib, 4096, 2, 128, F, 8, dtype)) == [first, other]
+            assert _kinds(_backward(lib, 4096, 2, 128, F, 8, dtype)) == [first, other]
         for E, k in ((8, 2), (32, 4)):
-            for per, few in ((4, True), (5, kind == "exact"), (16, kind == "exact"), (17, False)):
-                assert _kinds(_forward(lib, per * E // k, k, 128, 128, E, dtype)) == ["stream" if few else kind] * 2
-    # a product's own result is rounded to the rows' type: float16 costs 16 times the instruction's sums
-    for dtype, kind in ((_C.BF16, "product"), (_C.F16, "product"), (_C.F32, "exact")):
-        assert _kinds(_linear(lib, 4096, 2, 128, 128, 8, dtype=dtype)) == [kind]
+            for per, few in ((4, True), (5, first == "exact"), (16, first == "exact"), (17, False)):
+                assert _kinds(_forward(lib, per * E // k, k, 128, 128, E, dtype)) == (["stream"] * 2 if few else [first, other])
+        # a product's own result is rounded to the rows' type: float16 costs 16 times the instruction's sums
+        assert _kinds(_linear(lib, 4096, 2, 128, 128, 8, dtype=dtype)) == [other]
