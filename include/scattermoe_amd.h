@@ -450,7 +450,8 @@ typedef struct {
 } smoe_weight_8bit;
 
 /*
- * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, rounded once to `dtype`, or float32 where dtype is or-ed with
+ * Y[dst(n)] = Q(c X[src(n)]) W[e(n)]^T (+ b[e(n)]), Q: as smoe_quantize_rows, summed by the 8-bit matrix instruction (1.3e-5 of the result off) or, for
+ * float32 X and for few rows, in float32, and rounded once to `dtype`, or float32 where dtype is or-ed with
  * SMOE_8BIT_Y_FLOAT32 (rows that are added up afterwards: smoe_combine_f32); rows as for
  * smoe_scatter2scatter, those of Y that belong to a dropped slot zeros.  coeff (L) contiguous by slot, or NULL: the factor c of row n is coeff[idx[n]] (x_grouped 0 only).  `transposed`: W is the transpose of
  * the weight that its scales' strides belong to.  workspace: smoe_linear_8bit_workspace_bytes(L, K, N, E, fan_out,
@@ -474,7 +475,8 @@ int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm
 /*
  * A gated layer on such weights (GLUMLP.forward, scattermoe/mlp.py:74-95):
  *   pre = Q(X) W1[e]^T + b1[e];  y = Q(glu(pre)) W2[e]^T + b2[e];  OUT[t] = sum_j gates[t,j] y
- * pre and the hidden values are float32 until they are taken to 8 bits.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) float32 by slot (y), OUT (T,d)
+ * pre and the hidden values are float32 until they are taken to 8 bits; sums whose results are taken to 8 bits are the 8-bit matrix instruction's for
+ * bfloat16 alone.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) float32 by slot (y), OUT (T,d)
  * contiguous; P8 (16-byte aligned), PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
  * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
  * alone.  Ids outside [0,E) drop their row: it adds nothing to OUT (whatever its gate, where `experts` is given beside the order too), is zeros in Y

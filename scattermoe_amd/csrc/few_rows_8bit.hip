@@ -68,7 +68,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void few_rows_8bit_kernel(Few8Args a, in
   constexpr int HALF = EPI == EPI_UNIT ? GROUPS / 2 : GROUPS;      // groups of neighbouring columns
   const int n0 = blockIdx.x * (HALF * 8);
   const int Kp = (int)padded_row(a.K);
-  // 32-bit offsets from the first row of either half (the launcher checks)
+  // 32-bit offsets from the first row of either half: at most 64 rows of 2^21 bytes (product_checks in capi_8bit.hip refuses longer ones)
   e = __builtin_amdgcn_readfirstlane(e);
   const char* We = (const char*)a.W + e * a.swe;
   const int64_t n1 = n0 + (EPI == EPI_UNIT ? F : 0);

@@ -654,7 +654,9 @@ static int launch_product(const Product8Args& a, int bias_dtype, int n_tiles, hi
 // Tiles of 64 rows instead of 128: a third workgroup per CU waits for its weights beside two others.  us in tiles of 128 -> 64 at 16, 32, 64, 128
 // rows per expert, even and as 1 / rank^0.5: 8 experts, 4096 -> 28672 214 -> 185, 215 -> 187, 220 -> 190, 230 -> 237 and 213 -> 184, 214 -> 184, 219 ->
 // 223, 217 -> 248; 128 experts, 2048 -> 1536 80 -> 67, 87 -> 76, 95 -> 86, 106 -> 111 and 79 -> 85, 85 -> 89, 93 -> 104, 119 -> 123; 32 experts,
-// 2880 -> 5760 115 -> 104, 120 -> 107, 133 -> 118, 148 -> 162 and 117 -> 106, 117 -> 132, 131 -> 161, 170 -> 180.
+// 2880 -> 5760 115 -> 104, 120 -> 107, 133 -> 118, 148 -> 162 and 117 -> 106, 117 -> 132, 131 -> 161, 170 -> 180.  What decides is the tile rows that the
+// loads make, which the host does not know; by the average, 24 rows lie between the even loads, which gain up to 32 (wide experts up to 64), and
+// the uneven ones, of which many small experts lose 6 % at 16.
 static bool low_tiles(int64_t L, int E) { return L <= 24 * (int64_t)E; }
 template <typename TO, bool EXACT, int EPI>
 static int launch_product(const Product8Args& a, int bias_dtype, hipStream_t st) {

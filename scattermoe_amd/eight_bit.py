@@ -149,7 +149,9 @@ def parallel_linear_8bit(inputs, weight, weight_scales, k, sorted_expert_idxs, s
     """`parallel_linear` on weights in 8 bits: inputs (tokens, K), or (rows, K) with `grouped_in`, float32, bfloat16 or float16, are taken to
     8 bits with a scale for every 128 of a row, multiplied by weight (E, N, K rounded up to 16, the rest zeros) of float8_e4m3fn with weight_scales
     (E, ceil(N / 128), ceil(K / 128)) of float8_e8m0fnu or float32, and rounded once: rows that gates weigh, and the gradients of a token's
-    slots, are added up in float32.  Biases (E, N) and gates (tokens, k) of the inputs' type.  Routing as for `parallel_linear`; gates go with `grouped_out=False`.
+    slots, are added up in float32.  A product's own sums are those of the 8-bit matrix instruction, 1.3e-5 of the result off, where rows of 16 bits
+    are many, and float32 ones where they are float32 (`inputs.float()` chooses those, at half the rate).  Biases (E, N) and gates (tokens, k) of
+    the inputs' type.  Routing as for `parallel_linear`; gates go with `grouped_out=False`.
 
     Slots that the routing dropped (ids outside [0, E)) have rows of zeros; gates that weigh those are finite numbers.
 
@@ -214,7 +216,9 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
     None of x's type; SiLU on the second half of the first product's columns, on the first when `gate_first`.
 
     The tokens and the hidden rows are taken to 8 bits; pre-activations, the experts' rows and sums stay in float32, and the result is rounded
-    once.  expert_p is taken to x's type.  A slot whose id lies outside [0, E) (padding) adds nothing, whatever its gate, and has no gradient.  A step that asks for the gradient of expert_p keeps the experts' rows in float32.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
+    once.  Sums whose results go to 8 bits again (hidden values, their gradients) are those of the 8-bit matrix instruction for bfloat16, where a value
+    next to a border of 8 bits may fall to its other side (2.0e-3 to 2.2e-3 of the result against 64 bits, bfloat16's rounding alone 1.7e-3), and
+    float32 ones for float16 and float32: tokens of those types choose them, at half the rate.  expert_p is taken to x's type.  A slot whose id lies outside [0, E) (padding) adds nothing, whatever its gate, and has no gradient.  A step that asks for the gradient of expert_p keeps the experts' rows in float32.  Weights, scales and biases are constants.  The gradient of x needs the transposed weights w1_t (E, d, 2F
     rounded up to 16) and w2_t (E, F, d rounded up to 16); the step then keeps the pre-activation in 8 bits, and nothing else of its
     width, and the gradients that its products read are taken to 8 bits too."""
     what = "glu_mlp_8bit"
@@ -235,7 +239,8 @@ def glu_mlp_8bit(x, expert_p, expert_idxs, w1, s1, w2, s2, b1=None, b2=None, gat
     act = ops.ACT_SILU_GATE_FIRST if gate_first else ops.ACT_SILU
     tokens = x if x.dim() == 2 else x.reshape(T, d)                  # (a view would be a node of the backward pass)
     trained = ((x.requires_grad or expert_p.requires_grad) and torch.is_grad_enabled()) or ops.has_tangents(x, expert_p, b1, b2)
-    # (by the ids an expert's weights are read once for every 8 of its rows: 64 rows of 8 experts, 4096 / 14336, 368 us, in the experts' order 265)
+    # (by the ids an expert's weights are read once for every 8 of its rows: 64 rows of 8 experts, 4096 / 14336, 368 us, in the experts' order 265.
+    # The ids are on the device: of few experts, 64 rows of one of 16, 4096 / 4096, it is 151 us for 56 and the routing, of all 16 161 for 155)
     experts = ops._as_i64(expert_idxs).contiguous()
     if not trained and T * k <= min(ops.FEW_ROWS_8BIT, 4 * E):
         out = ops.glu_mlp_8bit(tokens, expert_p.to(x.dtype), w1, s1, b1, w2, s2, b2, experts=experts, act=act)[0]
