@@ -479,8 +479,8 @@ int smoe_gate_grad_f32(const void* Y, int64_t sym, const void* dOut, int64_t sdm
  * bfloat16 alone.  W1 (E, 2F, d), W2 (E, d, F); gates (T,k), Y (T k, d) float32 by slot (y), OUT (T,d)
  * contiguous; P8 (16-byte aligned), PS: the halves of pre as smoe_glu_8bit_fwd keeps them, rows sorted by expert, or NULL (`keep` 0).  At most
  * SMOE_8BIT_FEW_ROWS rows T k without P8 may go without their order (idx NULL, `ordered` 0): experts (T,k) contiguous is read instead, Y is left
- * alone.  Ids outside [0,E) drop their row: it adds nothing to OUT (whatever its gate, where `experts` is given beside the order too), is zeros in Y
- * and DROWS, and adds nothing to DX.
+ * alone.  With their order, experts are the ids that it was made of, or NULL.  Ids outside [0,E) drop their row: it adds nothing to OUT (with experts NULL:
+ * if its gate is a finite number), is zeros in Y and DROWS, and adds nothing to DX.
  * Backward: DX[t] = sum_j Q(glu'(P8) (Q(gates[t,j] DOUT[t]) W2[e])) W1[e]; blocks along all 2F columns.  W1T (E, d, 2F), W2T (E, F, d): transposes, with
  * the scales of the weights; DROWS (T k, d) float32: what every slot adds to DX (T,d).  Workspaces as above.
  */

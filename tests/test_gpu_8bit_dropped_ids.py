@@ -90,3 +90,42 @@ def test_products(dtype, T, k, E, K, N, share):
     got = eight_bit.parallel_linear_8bit(h.float(), q, s, 1, eid, idx, off, gates=p.float(), grouped_in=True)
     want = (rows.view(T, k, N) * p.float().unsqueeze(-1)).double().sum(1)
     assert bool(((got - want).abs() <= (k + 2) * 2.0 ** -24 * (rows.view(T, k, N).abs() * p.float().unsqueeze(-1)).sum(1) + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,k,E,d,F", [(5, 2, 4, 128, 96), (40, 3, 48, 136, 64), (150, 2, 5, 256, 128)])
+def test_replayed_with_other_padding(dtype, T, k, E, d, F):
+    """A captured forward pass and a captured step, replayed with no, some and only dropped slots, and none again: each the eager call's bits."""
+    (q1, s1, t1), (q2, s2, t2) = _weights(E, 2 * F, d, 1), _weights(E, d, F, 2)
+    g = torch.Generator().manual_seed(d)
+    x, dout = (torch.randn(T, d, generator=g).to(DEV, dtype) for _ in range(2))
+    p = (torch.rand(T, k, generator=g) + 0.2).to(DEV, dtype)
+    ids = _ids(T, k, E, 0.0, 1)[0]
+
+    def step():
+        a, b = x.detach().requires_grad_(), p.detach().requires_grad_()
+        out = eight_bit.glu_mlp_8bit(a, b, ids, q1, s1, q2, s2, w1_t=t1, w2_t=t2)
+        return [out.detach(), *torch.autograd.grad(out, (a, b), dout)]
+
+    def forward():
+        with torch.no_grad():
+            return eight_bit.glu_mlp_8bit(x, p, ids, q1, s1, q2, s2)
+
+    forward(), step()
+    torch.cuda.synchronize()
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        out = forward()
+    with torch.cuda.graph(two, pool=one.pool()):
+        got = step()
+    for r, share in enumerate((0.0, 0.3, 1.0, 0.2, 0.0)):
+        ids.copy_(_ids(T, k, E, share, r)[0])
+        x.copy_(torch.randn(T, d, generator=g))
+        one.replay()
+        want = forward()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), r
+        two.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), r
